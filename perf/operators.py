@@ -434,7 +434,7 @@ def exact(case, seed):
         q[:live] = turned(s["q"])
         flat = s["slots"][:live].long()
         for cache, rows in ((k_cache, turned(s["k"])), (v_cache, s["v"][:live].double())):
-            lines = cache.transpose(1, 2).reshape(-1, case["kv_heads"], case["dim"])
+            lines = cache.transpose(1, 2).reshape(-1, case["kv_heads"], case["dim"]).clone()
             lines[flat] = rows
             cache.copy_(lines.view(cache.shape[0], PAGE, case["kv_heads"], case["dim"]).transpose(1, 2))
         return {"q": q, "k_cache": k_cache, "v_cache": v_cache}
