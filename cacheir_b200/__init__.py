@@ -4,6 +4,7 @@ Public surface (mirrors the reference names for this path):
   B200DecodeRuntime / create_runtime   -- drop-in for CudaRuntime on decode
   B200KVPageAllocator, B200PagedKVCache -- paged KV pool + page tables
   quantization, ops, hybrid_ops, expert_ops -- pack format and C-ABI wrappers
+  serving_ops                           -- operators of batches that share prompts
   load_model, models                    -- model registry: a folder's config.json picks the family
 Importing the package does not need a GPU; calling a kernel without the built
 library or without CUDA raises (there is no fallback path).

@@ -1,6 +1,6 @@
 """ctypes binding of libcacheir_b200.so (the C ABI declared in include/cacheir_b200.h) and of the libraries of the
 ragged families: libcacheir_b200_ragged.so, _hybrid.so, _recurrence.so, _experts.so, _talking.so and _delta.so (headers of the
-same names).
+same names), and of libcacheir_b200_serving.so, the operators of batches that share prompts.
 
 There is no fallback: if the shared library is missing the import of any
 compute entry point raises, telling the user to build it.
@@ -8,11 +8,11 @@ compute entry point raises, telling the user to build it.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_longlong, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_longlong, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libcacheir_b200.so"
-GROUP_PATHS = {name: LIB_PATH.with_name(f"libcacheir_b200_{name}.so") for name in ("ragged", "hybrid", "recurrence", "experts", "talking", "delta")}
+GROUP_PATHS = {name: LIB_PATH.with_name(f"libcacheir_b200_{name}.so") for name in ("ragged", "hybrid", "recurrence", "experts", "talking", "delta", "serving")}
 
 # name -> (restype, argtypes); mirrors include/cacheir_b200.h one to one
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -197,6 +197,24 @@ class RouteRule(ctypes.Structure):
     _fields_ = [("softmax", c_int), ("identity", c_int), ("groups", c_int), ("keep", c_int), ("correction", c_void_p), ("scale", c_float)]
 
 
+class RotaryArgs(ctypes.Structure):
+    """cacheir_b200_rotary_args"""
+
+    _fields_ = [(name, c_void_p) for name in ("q", "k", "v", "q_out", "k_out", "k_cache", "v_cache", "positions", "slots", "turns")] + \
+               [(name, c_longlong) for name in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride")] + \
+               [(name, c_int) for name in ("rows", "heads", "kv_heads", "dim", "rot", "layout", "num_slots", "page_size", "dtype")] + [("factor", c_float)]
+
+
+class PrefixArgs(ctypes.Structure):
+    """cacheir_b200_prefix_args"""
+
+    _fields_ = [(name, c_void_p) for name in ("q", "k_cache", "v_cache", "out", "page_table", "seq_lens", "group_rows", "prefix_table", "prefix_lens",
+                                              "workspace")] + \
+               [("workspace_bytes", c_size_t), ("q_stride", c_longlong), ("out_stride", c_longlong)] + \
+               [(name, c_int) for name in ("batch", "heads", "kv_heads", "dim", "page_size", "num_slots", "max_pages", "groups", "prefix_pages",
+                                           "dtype")] + [("softmax_scale", c_float)]
+
+
 _NEXT = [c_int, c_void_p, c_void_p, c_float, c_void_p]      # next_mode next_w next_b next_alpha next_out
 # group -> signatures; each mirrors include/cacheir_b200_<group>.h one to one
 GROUP_SIGNATURES: dict[str, dict[str, tuple[object, list[object]]]] = {
@@ -288,6 +306,15 @@ GROUP_SIGNATURES: dict[str, dict[str, tuple[object, list[object]]]] = {
         "cacheir_b200_combine_residual": (
             c_int, [c_void_p] * 4 + [c_int, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int] + _NEXT + [c_int, c_void_p]),
         "cacheir_b200_experts_device_status": (c_int, [c_int]),
+    },
+    "serving": {
+        "cacheir_b200_extend_page_tables": (c_int, [c_void_p] * 5 + [c_int] * 5 + [c_void_p] * 6),
+        "cacheir_b200_shrink_page_tables": (c_int, [c_void_p] * 6 + [c_int] * 4 + [c_void_p] * 2),
+        "cacheir_b200_rotary_append": (c_int, [c_void_p, c_void_p]),
+        "cacheir_b200_shared_prefix_workspace_bytes": (c_size_t, [c_int] * 3),
+        "cacheir_b200_shared_prefix_attention": (c_int, [c_void_p, c_void_p]),
+        "cacheir_b200_token_logprobs": (c_int, [c_void_p, c_longlong] + [c_void_p] * 5 + [c_int] * 3 + [c_double, c_int, c_void_p]),
+        "cacheir_b200_serving_device_status": (c_int, [c_int]),
     },
 }
 # entry points of glue.cu and misc.cu, which the core and the ragged library carry

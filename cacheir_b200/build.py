@@ -8,7 +8,8 @@ with the static CUDA runtime: `core` (libcacheir_b200.so, Llama-shaped models),
 `ragged` (dense products and row operators of the families with ragged steps),
 `hybrid` (latent attention), `recurrence` (linear recurrences, matrix memory, state
 spaces), `experts` (tied attention, mixtures of experts), `talking` (talking-heads
-attention) and `delta` (short convolutions, delta rule). A model family names the groups it needs, so a fresh
+attention), `delta` (short convolutions, delta rule) and `serving` (operators of batches that share prompts: page
+tables, rotary append, prefix attention, token log probabilities). A model family names the groups it needs, so a fresh
 checkout compiles only those. Objects are rebuilt only when their source or a
 header is newer.
 """
@@ -34,6 +35,7 @@ GROUP_FILES = {
     "recurrence": ("linear_recurrence",),
     "talking": ("talking_attention", "talking_prompt"),
     "delta": ("short_conv", "delta_rule"),
+    "serving": ("page_tables", "rotary_append", "shared_prefix", "token_logprobs"),
     "experts": ("tied_attention", "tied_prompt", "grouped_gemm", "expert_routing"),
 }
 LIB_PATHS = {"core": LIB_DIR / "libcacheir_b200.so", **{name: LIB_DIR / f"libcacheir_b200_{name}.so" for name in GROUP_FILES}}

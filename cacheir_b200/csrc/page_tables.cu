@@ -1,0 +1,229 @@
+// Page tables of a batch, kept on the device: pages for new tokens off a stack of free ones, the map from the rows of a step to page
+// slots, and the way back.
+//
+// With P tokens to a page, sequence b of len tokens that gets n more needs ceil((len + n) / P) - ceil(len / P) new pages. Two running
+// sums over the sequences, of rows and of pages, say where its rows stand and which pages of the stack are its own; everything else is
+// then independent: a page goes to its place in a table, a row finds its sequence by bisection in the row sums.
+//
+// Little data (12 bytes a row, 8 a page, 12 a sequence) and much latency: read lengths, sum, look up, write. So it is one launch. A call
+// changes what it reads (lengths, stack height), so all reads of those come before all writes: the blocks are one thread-block cluster,
+// each of which sums all sequences by itself, and meet once in between.
+#include "cacheir_b200_serving.h"
+#include "common.cuh"
+#include "tc_ptx.cuh"
+
+namespace cb200 {
+namespace {
+
+constexpr int kThreads = 1024;
+constexpr int kClusterBlocks = 8;
+
+struct TableArgs {
+  int32_t* page_table;
+  int32_t* seq_lens;
+  const int32_t* change;      // extend: new tokens; shrink: tokens kept
+  const int32_t* held_pages;  // shrink
+  int32_t* free_pages;
+  int32_t* free_count;
+  int32_t* positions;
+  int32_t* row_seq;
+  int32_t* slots;
+  int32_t* cu_rows;
+  int32_t* status;
+  int sequences, max_pages, page_size, capacity, rows;
+};
+
+__device__ __forceinline__ int pages_of(long long tokens, int page_size) { return static_cast<int>((tokens + page_size - 1) / page_size); }
+
+// Exclusive sums over the block of two numbers per thread, and their totals.
+__device__ __forceinline__ void block_scan(long long (&v)[2], long long (&total)[2]) {
+  __shared__ long long s_warp[2][kThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long own[2] = {v[0], v[1]};
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const long long up = __shfl_up_sync(0xffffffffu, v[i], off);
+      if (lane >= off) v[i] += up;
+    }
+  if (lane == 31) { s_warp[0][warp] = v[0]; s_warp[1][warp] = v[1]; }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    long long w = lane < static_cast<int>(blockDim.x >> 5) ? s_warp[i][lane] : 0;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, w, off);
+      if (lane >= off) w += up;
+    }
+    total[i] = __shfl_sync(0xffffffffu, w, 31);
+    const long long before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+    v[i] = v[i] - own[i] + (warp > 0 ? before : 0);
+  }
+}
+
+// Last index i with starts[i] <= at (starts[0] = 0, n entries).
+__device__ __forceinline__ int owner(const int32_t* starts, int n, int at) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= at) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+template <bool EXTEND>
+__global__ void __launch_bounds__(kThreads)
+page_tables_kernel(const TableArgs p) {
+  chain_enter();
+  extern __shared__ int32_t smem[];
+  int32_t* s_len = smem;                                    // [sequences] tokens before
+  int32_t* s_page = s_len + p.sequences;                    // [sequences] first page of the call that is this sequence's
+  int32_t* s_row = s_page + p.sequences;                    // extend: [sequences] first row
+  const int rank = blockIdx.x, ranks = gridDim.x, n = p.sequences;
+  const int per = (n + blockDim.x - 1) / blockDim.x;        // neighbouring sequences of a thread
+  const int lo = min(n, static_cast<int>(threadIdx.x) * per), hi = min(n, lo + per);
+  const int count = *p.free_count;
+
+  // ---- what every sequence needs ----
+  long long sum[2] = {0, 0}, total[2];
+  bool bad = false;
+  const long long room = static_cast<long long>(p.max_pages) * p.page_size;
+  auto need = [&](int b, int len, int* tokens) {            // pages that come or go
+    if constexpr (EXTEND) {
+      *tokens = max(p.change[b], 0);
+      return pages_of(static_cast<long long>(len) + *tokens, p.page_size) - pages_of(len, p.page_size);
+    } else {
+      *tokens = min(max(p.change[b], 0), len);
+      const int first = max(pages_of(*tokens, p.page_size), p.held_pages ? p.held_pages[b] : 0);
+      return max(0, pages_of(len, p.page_size) - first);
+    }
+  };
+  for (int b = lo; b < hi; ++b) {
+    const int len = max(p.seq_lens[b], 0);
+    int tokens;
+    const int pages = need(b, len, &tokens);
+    bad = bad || static_cast<long long>(len) + (EXTEND ? tokens : 0) > room;
+    s_len[b] = len;
+    sum[0] += tokens;
+    sum[1] += pages;
+  }
+  block_scan(sum, total);
+  const bool too_long = __syncthreads_or(bad ? 1 : 0) != 0;
+  int why = 0;
+  if (too_long) why = -2;
+  else if (count < 0 || count > p.capacity || (!EXTEND && count + total[1] > p.capacity)) why = -3;
+  else if (EXTEND && total[0] > p.rows) why = -1;
+  else if (EXTEND && total[1] > count) why = static_cast<int>(min(total[1] - count, 0x7fffffffLL));
+  // (sums that are used below fit in 32 bits: rows <= p.rows, pages <= capacity)
+  if (why == 0) {
+    long long row = sum[0], page = sum[1];
+    for (int b = lo; b < hi; ++b) {
+      int tokens;
+      const int pages = need(b, s_len[b], &tokens);
+      s_page[b] = static_cast<int32_t>(page);
+      if constexpr (EXTEND) s_row[b] = static_cast<int32_t>(row);
+      row += tokens;
+      page += pages;
+    }
+  }
+  __syncthreads();
+  if (ranks > 1) ptx::cluster_sync_release();               // everybody has read what the call changes
+  const int pages = why == 0 ? static_cast<int>(total[1]) : 0;
+
+  // ---- lengths, heights, row starts ----
+  if (rank == 0) {
+    if (why != 0) {
+      if (threadIdx.x == 0 && *p.status == 0) *p.status = why;
+      if constexpr (EXTEND)
+        for (int b = threadIdx.x; b <= n; b += blockDim.x) p.cu_rows[b] = 0;
+    } else {
+      for (int b = threadIdx.x; b < n; b += blockDim.x) {
+        const int len = s_len[b];
+        if constexpr (EXTEND) {
+          const int first = s_row[b], end = b + 1 < n ? s_row[b + 1] : static_cast<int>(total[0]);
+          p.cu_rows[b] = first;
+          p.seq_lens[b] = len + end - first;
+        } else {
+          p.seq_lens[b] = min(max(p.change[b], 0), len);
+        }
+      }
+      if (threadIdx.x == 0) {
+        if constexpr (EXTEND) p.cu_rows[n] = static_cast<int32_t>(total[0]);
+        *p.free_count = EXTEND ? count - pages : count + pages;
+      }
+    }
+  }
+  // ---- pages ----
+  const int thread = rank * blockDim.x + threadIdx.x, threads = ranks * blockDim.x;
+  for (int i = thread; i < pages; i += threads) {
+    const int b = owner(s_page, n, i);
+    int32_t* row = p.page_table + static_cast<size_t>(b) * p.max_pages;
+    if constexpr (EXTEND) {
+      row[pages_of(s_len[b], p.page_size) + i - s_page[b]] = p.free_pages[count - 1 - i];
+    } else {
+      const int after = b + 1 < n ? s_page[b + 1] : pages;  // the sequence's pages are its last ones
+      p.free_pages[count + pages - 1 - i] = row[pages_of(s_len[b], p.page_size) - (after - i)];
+    }
+  }
+  // ---- rows ----
+  if constexpr (EXTEND) {
+    const int used = why == 0 ? static_cast<int>(total[0]) : 0;
+    for (int r = thread; r < p.rows; r += threads) {
+      int pos = 0, b = -1, slot = -1;
+      if (r < used) {
+        b = owner(s_row, n, r);
+        pos = s_len[b] + r - s_row[b];
+        const int page = pos / p.page_size, opened = page - pages_of(s_len[b], p.page_size);
+        const int id = opened < 0 ? p.page_table[static_cast<size_t>(b) * p.max_pages + page] : p.free_pages[count - 1 - (s_page[b] + opened)];
+        slot = id * p.page_size + pos % p.page_size;
+      }
+      p.positions[r] = pos;
+      p.row_seq[r] = b;
+      p.slots[r] = slot;
+    }
+  }
+}
+
+template <bool EXTEND>
+int launch_tables(const TableArgs& a, int blocks, cudaStream_t stream) {
+  const size_t smem = static_cast<size_t>(a.sequences) * (EXTEND ? 3 : 2) * 4;
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(page_tables_kernel<EXTEND>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  const cudaError_t e = launch_clusters(page_tables_kernel<EXTEND>, dim3(blocks), dim3(kThreads), smem, stream, dim3(blocks), a);
+  return e != cudaSuccess ? static_cast<int>(e) : launch_status();
+}
+
+}  // namespace
+}  // namespace cb200
+
+using namespace cb200;
+
+extern "C" int cacheir_b200_extend_page_tables(int32_t* page_table, int32_t* seq_lens, const int32_t* new_lens, const int32_t* free_pages,
+                                               int32_t* free_count, int sequences, int max_pages, int page_size, int capacity, int rows,
+                                               int32_t* positions, int32_t* row_seq, int32_t* slots, int32_t* cu_rows, int32_t* status,
+                                               void* stream) {
+  if (sequences <= 0 || rows <= 0) return 0;
+  if (!page_table || !seq_lens || !new_lens || !free_pages || !free_count || !positions || !row_seq || !slots || !cu_rows || !status ||
+      max_pages <= 0 || page_size <= 0 || capacity <= 0)
+    return CACHEIR_B200_EINVAL;
+  if (sequences > CACHEIR_B200_MAX_SEQUENCES || static_cast<long long>(max_pages) * page_size > 0x7fffffffLL) return CACHEIR_B200_ELIMIT;
+  TableArgs a{page_table, seq_lens, new_lens, nullptr, const_cast<int32_t*>(free_pages), free_count, positions, row_seq, slots, cu_rows, status,
+              sequences, max_pages, page_size, capacity, rows};
+  return launch_tables<true>(a, rows > 2 * kThreads ? kClusterBlocks : 1, as_stream(stream));
+}
+
+extern "C" int cacheir_b200_shrink_page_tables(const int32_t* page_table, int32_t* seq_lens, const int32_t* keep_lens, const int32_t* held_pages,
+                                               int32_t* free_pages, int32_t* free_count, int sequences, int max_pages, int page_size,
+                                               int capacity, int32_t* status, void* stream) {
+  if (sequences <= 0) return 0;
+  if (!page_table || !seq_lens || !keep_lens || !free_pages || !free_count || !status || max_pages <= 0 || page_size <= 0 || capacity <= 0)
+    return CACHEIR_B200_EINVAL;
+  if (sequences > CACHEIR_B200_MAX_SEQUENCES || static_cast<long long>(max_pages) * page_size > 0x7fffffffLL) return CACHEIR_B200_ELIMIT;
+  TableArgs a{const_cast<int32_t*>(page_table), seq_lens, keep_lens, held_pages, free_pages, free_count, nullptr, nullptr, nullptr, nullptr, status,
+              sequences, max_pages, page_size, capacity, 0};
+  return launch_tables<false>(a, 1, as_stream(stream));
+}

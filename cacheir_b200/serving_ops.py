@@ -1,0 +1,365 @@
+"""Torch-tensor wrappers over the operators of batches whose requests share prompts (include/cacheir_b200_serving.h).
+
+The operators of a step, in its order: pages and slots for new tokens (`extend_page_tables`, and back: `shrink_page_tables`), rotary
+positions with the append to the page pool (`rotary_append`), decode attention that reads a common prefix once for all of its requests
+(`shared_prefix_attention`), log probabilities of tokens (`token_logprobs`).
+
+Same rules as `ops`: validate, pass device pointers on the current stream, raise on a non-zero status. All tensors of a call are on one
+CUDA device, which need not be the current one; the call runs on that device's current stream.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from contextlib import contextmanager
+from dataclasses import dataclass
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import PrefixArgs, RotaryArgs, check
+from .ops import _ptr, _require_cuda, dtype_code
+
+MAX_TOP = 32
+MAX_SEQUENCES = 16384
+LAYOUTS = {"interleaved": 0, "half": 1}
+
+
+@contextmanager
+def _launch(*tensors: torch.Tensor | None):
+    """The stream to launch on: the current one of the device that all the tensors are on."""
+    _require_cuda(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"all tensors of a call must be on one device, got {sorted(map(str, devices))}")
+    device = devices.pop()
+    with torch.cuda.device(device):
+        yield torch.cuda.current_stream(device).cuda_stream
+
+
+def _check_ints(what: str, *tensors: torch.Tensor | None) -> None:
+    for t in tensors:
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            raise TypeError(f"{what} must be contiguous int32 tensors")
+
+
+def _check_heads(name: str, t: torch.Tensor, rows: int | None = None) -> None:
+    if t.dim() != 3 or min(t.shape[1:]) < 1 or (t.stride(2) != 1 and t.shape[2] > 1) or (t.stride(1) != t.shape[2] and t.shape[1] > 1) or \
+            (rows is not None and t.shape[0] != rows):
+        raise ValueError(f"{name} must be [rows, heads, dim] with dense heads: only the row stride may differ from heads * dim")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1] * t.shape[2]:
+        raise ValueError(f"{name}: rows must not overlap")
+
+
+# ---- page tables -----------------------------------------------------------------------------------------------------
+@dataclass
+class TokenMap:
+    """The rows of a step (all int32, on the device): row r is the token at `positions[r]` of sequence `row_seq[r]`, its key and value
+    go to `slots[r]` (page * page_size + offset); sequence b has the rows cu_rows[b] .. cu_rows[b + 1] - 1. Rows behind the last token:
+    position 0, sequence -1, slot -1. `status` keeps the first refusal until it is set to 0 (see `extend_page_tables`)."""
+
+    positions: torch.Tensor
+    row_seq: torch.Tensor
+    slots: torch.Tensor
+    cu_rows: torch.Tensor
+    status: torch.Tensor
+
+
+def token_map(rows: int, sequences: int, device: torch.device | str) -> TokenMap:
+    """Room for `rows` tokens of `sequences` sequences."""
+    if rows < 1 or sequences < 1:
+        raise ValueError("a token map has at least one row and one sequence")
+    sizes = (rows, rows, rows, sequences + 1, 1)
+    return TokenMap(*(torch.zeros(n, dtype=torch.int32, device=device) for n in sizes))
+
+
+def _check_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, change: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+                  status: torch.Tensor, page_size: int) -> int:
+    _check_ints("page tables, lengths, free pages and status", page_table, seq_lens, change, free_pages, free_count, status)
+    if page_table.dim() != 2 or page_table.shape[1] < 1:
+        raise ValueError("page_table must be [sequences, max_pages]")
+    sequences = int(page_table.shape[0])
+    if tuple(seq_lens.shape) != (sequences,) or tuple(change.shape) != (sequences,):
+        raise ValueError("lengths must be [sequences]")
+    if not 1 <= sequences <= MAX_SEQUENCES:
+        raise ValueError(f"a call takes 1 to {MAX_SEQUENCES} sequences")
+    if free_pages.dim() != 1 or free_pages.numel() < 1 or free_count.numel() != 1 or status.numel() != 1:
+        raise ValueError("free_pages must be a stack [capacity], free_count and status one number each")
+    if int(page_size) < 1:
+        raise ValueError("page_size must be positive")
+    if change.data_ptr() == seq_lens.data_ptr():
+        raise ValueError("the lengths that a call changes cannot also be its other lengths")
+    return sequences
+
+
+def extend_page_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor,
+                       free_count: torch.Tensor, tokens: TokenMap, *, page_size: int) -> TokenMap:
+    """Room for new_lens[b] more tokens of every sequence b, and where they go.
+
+    New pages come off the stack free_pages[: free_count] into page_table [sequences, max_pages] int32, sequence by sequence; seq_lens
+    and free_count are brought up to date and `tokens` is filled. Everything stays on the device, so that a captured graph can do it.
+    Nothing changes (and `tokens` has no rows, every slot -1) where the call cannot be done; tokens.status then holds, until the caller sets
+    it to 0, the number of missing pages, -1 (more tokens than rows), -2 (a sequence longer than its table) or -3 (free_count outside the
+    stack). Beside `kv_cache.B200PagedKVCache.extend`, which walks the same pages on the host."""
+    sequences = _check_tables(page_table, seq_lens, new_lens, free_pages, free_count, tokens.status, page_size)
+    _check_ints("token map", tokens.positions, tokens.row_seq, tokens.slots, tokens.cu_rows)
+    rows = tokens.positions.numel()
+    if tokens.row_seq.numel() != rows or tokens.slots.numel() != rows or tokens.cu_rows.numel() != sequences + 1:
+        raise ValueError("the token map was made for other sizes")
+    with _launch(page_table, seq_lens, new_lens, free_pages, free_count, tokens.positions, tokens.row_seq, tokens.slots, tokens.cu_rows,
+                 tokens.status) as stream:
+        check(_lib.load_group("serving").cacheir_b200_extend_page_tables(
+            page_table.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), sequences,
+            int(page_table.shape[1]), int(page_size), free_pages.numel(), rows, tokens.positions.data_ptr(), tokens.row_seq.data_ptr(),
+            tokens.slots.data_ptr(), tokens.cu_rows.data_ptr(), tokens.status.data_ptr(), stream), "extend_page_tables")
+    return tokens
+
+
+def shrink_page_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, keep_lens: torch.Tensor, free_pages: torch.Tensor,
+                       free_count: torch.Tensor, status: torch.Tensor, *, page_size: int, held_pages: torch.Tensor | None = None) -> None:
+    """Sequence b keeps its first min(keep_lens[b], seq_lens[b]) tokens (0: it ends); the pages behind them return to the stack, the first
+    one on top, so that extending again gives them back in their order. page_table keeps its entries. The first held_pages[b] pages of a
+    row belong to somebody else (a common prefix) and never return. `status` as in `extend_page_tables` (-2, -3)."""
+    sequences = _check_tables(page_table, seq_lens, keep_lens, free_pages, free_count, status, page_size)
+    _check_ints("held_pages", held_pages)
+    if held_pages is not None and tuple(held_pages.shape) != (sequences,):
+        raise ValueError("held_pages must be [sequences]")
+    with _launch(page_table, seq_lens, keep_lens, free_pages, free_count, status, held_pages) as stream:
+        check(_lib.load_group("serving").cacheir_b200_shrink_page_tables(
+            page_table.data_ptr(), seq_lens.data_ptr(), keep_lens.data_ptr(), _ptr(held_pages), free_pages.data_ptr(), free_count.data_ptr(),
+            sequences, int(page_table.shape[1]), int(page_size), free_pages.numel(), status.data_ptr(), stream), "shrink_page_tables")
+
+
+# ---- rotary positions ------------------------------------------------------------------------------------------------
+@dataclass
+class RotaryRule:
+    """How heads turn: `turns` int64 [rot/2] (turns per position of every pair as a binary fraction, bits of an unsigned number), the pair
+    layout, and a factor of cosine and sine."""
+
+    turns: torch.Tensor
+    layout: str
+    factor: float = 1.0
+
+    @property
+    def rot(self) -> int:
+        return 2 * int(self.turns.numel())
+
+
+def turn_fractions(frequencies: np.ndarray) -> np.ndarray:
+    """Angles per position (radians, float64) as turns: freq / 2 pi modulo 1, in units of 2^-64, as int64 bits."""
+    freq = np.asarray(frequencies, dtype=np.float64)
+    if freq.ndim != 1 or freq.size < 1 or not np.all(np.isfinite(freq)):
+        raise ValueError("frequencies must be a row of finite numbers")
+    turns = freq / (2.0 * np.pi)
+    bits = [int((t - math.floor(t)) * 2.0 ** 64) & (2 ** 64 - 1) for t in turns.tolist()]
+    return np.array(bits, dtype=np.uint64).view(np.int64)
+
+
+def rotary_rule(rot: int, base: float, *, layout: str = "interleaved", scaling: tuple[float, float, float, float] | None = None,
+                yarn: tuple[float, float, float, float] | None = None, device: torch.device | str = "cuda") -> RotaryRule:
+    """The rule of frequencies base^(-2i/rot), as they are or scaled for long contexts as `ragged.rotary_frequencies` (scaling: factor,
+    low, high, original) or `ragged.yarn_frequencies` (yarn: factor, original, fast, slow) do it."""
+    from .ragged import rotary_frequencies, yarn_frequencies
+    if layout not in LAYOUTS:
+        raise ValueError(f"unknown pair layout {layout!r}: {sorted(LAYOUTS)}")
+    if rot < 2 or rot % 2 or not base > 0:
+        raise ValueError("rot must be an even number of at least 2 and base positive")
+    if scaling is not None and yarn is not None:
+        raise ValueError("one kind of scaling at a time")
+    freq, factor = yarn_frequencies(rot, base, *yarn) if yarn is not None else (rotary_frequencies(rot, base, scaling), 1.0)
+    return RotaryRule(torch.from_numpy(turn_fractions(freq)).to(device), layout, factor)
+
+
+def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, rule: RotaryRule, positions: torch.Tensor, *,
+                  slots: torch.Tensor | None = None, k_cache: torch.Tensor | None = None, v_cache: torch.Tensor | None = None,
+                  q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> None:
+    """Turns the first rule.rot values of every head of q [R, H, D] and k [R, KVH, D] to positions int32 [R] (rows may be strided views of
+    a fused buffer), into q_out (default: in place) and k_out. With slots int32 [R] and the pools [slots, KVH, page, D] the turned k and v
+    [R, KVH, D] are also appended: row r to page slots[r] // page, offset slots[r] % page; rows whose slot is outside the pool (padding: -1)
+    are left out altogether. Without slots, k_out defaults to in place; with them, to nowhere but the pool.
+
+    Beside `ops.rope_append`: both pair layouts, part of a head, scaled frequencies, float32 to bfloat16, far positions exactly."""
+    rows = int(q.shape[0])
+    for name, t in (("q", q), ("k", k), ("v", v), ("q_out", q_out), ("k_out", k_out)):
+        if t is not None:
+            _check_heads(name, t, rows)
+    heads, kv_heads, dim = int(q.shape[1]), int(k.shape[1]), int(q.shape[2])
+    if k.shape[2] != dim or rule.rot > dim or (v is not None and v.shape != k.shape):
+        raise ValueError("q, k and v must share their head size, of which the rule turns no more than all")
+    if rule.turns.dtype != torch.int64 or not rule.turns.is_contiguous() or rule.layout not in LAYOUTS:
+        raise ValueError("the rule must come from rotary_rule")
+    _check_ints("positions and slots", positions, slots)
+    if positions.numel() != rows or (slots is not None and slots.numel() != rows):
+        raise ValueError("positions and slots must have one number per row")
+    pools = (k_cache, v_cache)
+    if slots is None:
+        if any(t is not None for t in pools):
+            raise ValueError("an append to the pools needs slots")
+    elif v is None or any(t is None for t in pools):
+        raise ValueError("slots need v and both pools")
+    else:
+        if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[1] != kv_heads or k_cache.shape[3] != dim or k_cache.shape[0] < 1 or k_cache.shape[2] < 1:
+            raise ValueError("the pools must be [slots, KVH, page, D]")
+        if not all(t.is_contiguous() for t in pools):
+            raise ValueError("the pools must be contiguous")
+        if k_cache.shape[0] * k_cache.shape[2] > 2 ** 31:
+            raise ValueError("slots reach pools of up to 2^31 rows")
+    q_out = q if q_out is None else q_out
+    if k_out is None and slots is None:
+        k_out = k
+    if q_out.shape != q.shape or (k_out is not None and k_out.shape != k.shape):
+        raise ValueError("outputs must have their inputs' shapes")
+    given = [t for t in (q, k, v, q_out, k_out, *pools) if t is not None]
+    if any(t.dtype != q.dtype for t in given):
+        raise TypeError("q, k, v, the outputs and the pools must have one dtype")
+    if rows == 0:
+        return
+    code = dtype_code(q.dtype)
+    with _launch(*given, positions, slots, rule.turns) as stream:
+        a = RotaryArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), _ptr(positions), _ptr(slots),
+                       _ptr(rule.turns), q.stride(0), k.stride(0), 0 if v is None else v.stride(0), q_out.stride(0),
+                       0 if k_out is None else k_out.stride(0), rows, heads, kv_heads, dim, rule.rot, LAYOUTS[rule.layout],
+                       0 if k_cache is None else int(k_cache.shape[0]), 0 if k_cache is None else int(k_cache.shape[2]), code, float(rule.factor))
+        check(_lib.load_group("serving").cacheir_b200_rotary_append(ctypes.byref(a), stream), "rotary_append")
+
+
+# ---- attention over common prefixes ----------------------------------------------------------------------------------
+@dataclass
+class PrefixGroups:
+    """Neighbouring rows of a batch that open with the same tokens: rows rows[g] .. rows[g + 1] - 1 share the first lens[g] tokens, which lie
+    in the pages table[g] (int32 [G + 1], [G, prefix pages], [G], on the device). Any row's own page list starts with those pages
+    where the rows alias them (`kv_cache.B200PagedKVCache.share_prefix`)."""
+
+    rows: torch.Tensor
+    table: torch.Tensor
+    lens: torch.Tensor
+
+
+def prefix_groups(caches, device: torch.device | str, *, min_tokens: int = 1) -> PrefixGroups | None:
+    """The groups of a batch of `kv_cache.B200PagedKVCache`: neighbours that alias the same leading pages, with as many common tokens as all
+    of a group's rows share. A row joins the group before it where that has at least `min_tokens` common tokens with it. None: no two
+    neighbours share anything."""
+    starts, shared, page_size = [0], [], None
+    for cache in caches:
+        ids, page_size = cache.page_ids()[: cache.tokens // cache.page_size], cache.page_size       # whole pages
+        if shared:
+            common = 0
+            for a, b in zip(shared[-1], ids):
+                if a != b:
+                    break
+                common += 1
+            if common * page_size >= max(1, min_tokens):
+                shared[-1] = shared[-1][:common]
+                starts[-1] += 1
+                continue
+        shared.append(ids)
+        starts.append(starts[-1] + 1)
+    if not shared or starts[-1] == len(shared):
+        return None
+    sizes = [b - a for a, b in zip(starts, starts[1:])]
+    lens = [len(ids) * page_size if n > 1 else 0 for ids, n in zip(shared, sizes)]
+    width = max(max((n // page_size for n in lens)), 1)
+    table = [ids[:width] + [0] * (width - len(ids)) if n else [0] * width for ids, n in zip(shared, lens)]
+    return PrefixGroups(*(torch.tensor(v, dtype=torch.int32, device=device) for v in (starts, table, lens)))
+
+
+def shared_prefix_workspace_bytes(batch: int, heads: int, head_dim: int) -> int:
+    """Scratch of `shared_prefix_attention`."""
+    return int(_lib.load_group("serving").cacheir_b200_shared_prefix_workspace_bytes(int(batch), int(heads), int(head_dim)))
+
+
+def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                            groups: PrefixGroups | None, *, out: torch.Tensor | None = None, softmax_scale: float | None = None,
+                            workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """`ops.paged_attention_decode_batch` for rows that share prefixes: the keys and values of a group's common tokens are read once and
+    multiplied with the queries of all of its rows.
+
+    q: [B, H, D] (rows may be strided views); k_cache/v_cache: [slots, KVH, page, D] contiguous, of q's dtype; page_table: int32
+    [B, max_pages], every row's own page list from its first token on; seq_lens: int32 [B]. Row b attends to tokens t < seq_lens[b]:
+    those below its group's prefix through groups.table, the others through page_table (whose entries below the prefix are not read). A row
+    of length 0, or below, gives zeros. `workspace`: `shared_prefix_workspace_bytes(B, H, D)` bytes of any type; calls that may overlap
+    need one each (default: a fresh one)."""
+    _check_heads("q", q)
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("expected k_cache/v_cache [slots,KVH,page,D]")
+    batch, heads, dim = (int(n) for n in q.shape)
+    slots, kv_heads, page_size, pool_dim = (int(n) for n in k_cache.shape)
+    if pool_dim != dim or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError("q and the KV pool must share head_dim and dtype")
+    if kv_heads < 1 or heads % kv_heads or slots < 1:
+        raise ValueError("the query heads must be a multiple of the pool's heads")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("the KV pool must be contiguous")
+    _check_ints("page_table, seq_lens and the groups", page_table, seq_lens, *((groups.rows, groups.table, groups.lens) if groups else ()))
+    if page_table.dim() != 2 or page_table.shape[0] != batch or page_table.shape[1] < 1 or seq_lens.numel() != batch:
+        raise ValueError("page_table must be [B, max_pages] and seq_lens [B]")
+    count = 0
+    if groups is not None:
+        count = int(groups.lens.numel())
+        if groups.rows.numel() != count + 1 or groups.table.dim() != 2 or groups.table.shape[0] != count or count < 1 or groups.table.shape[1] < 1:
+            raise ValueError("prefix groups must have rows [G + 1], table [G, prefix pages] and lens [G]")
+    if out is None:
+        out = torch.empty((batch, heads, dim), device=q.device, dtype=q.dtype)
+    else:
+        _check_heads("out", out)
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out must match q's shape and dtype")
+    if batch == 0:
+        return out
+    scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError("softmax_scale must be positive")
+    code = dtype_code(q.dtype)
+    if workspace is None:
+        workspace = torch.empty(shared_prefix_workspace_bytes(batch, heads, dim), device=q.device, dtype=torch.uint8)
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    extra = (groups.rows, groups.table, groups.lens) if groups is not None else (None, None, None)
+    with _launch(q, k_cache, v_cache, page_table, seq_lens, out, workspace, *extra) as stream:
+        a = PrefixArgs(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(page_table), _ptr(seq_lens), _ptr(extra[0]), _ptr(extra[1]),
+                       _ptr(extra[2]), _ptr(workspace), workspace.numel() * workspace.element_size(), q.stride(0), out.stride(0), batch, heads,
+                       kv_heads, dim, page_size, slots, int(page_table.shape[1]), count, 0 if groups is None else int(groups.table.shape[1]), code,
+                       scale)
+        check(_lib.load_group("serving").cacheir_b200_shared_prefix_attention(ctypes.byref(a), stream), "shared_prefix_attention")
+    return out
+
+
+# ---- log probabilities -----------------------------------------------------------------------------------------------
+@dataclass
+class TokenLogprobs:
+    """float32 [R] log probabilities of the tokens and entropies (nats); int64 / float32 [R, top] likeliest tokens."""
+
+    logprobs: torch.Tensor | None
+    entropy: torch.Tensor
+    top_ids: torch.Tensor | None
+    top_logprobs: torch.Tensor | None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, *, top: int = 0, temperature: float = 1.0) -> TokenLogprobs:
+    """Log probabilities of tokens int64 [R] under softmax(logits / temperature), the rows' entropies, and the `top` likeliest tokens with
+    theirs (equal logits by rising index, like `ops.argmax_rows`). logits: [R, V] with dense rows (the row stride may be wider).
+
+    -inf masks a token out; a row of nothing else has log probabilities -inf and entropy 0. NaN or +inf in a row give NaN. A token below 0
+    means none (log probability 0), one of V or more gives NaN."""
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("logits must be [R, V] with dense rows")
+    rows, vocab = (int(n) for n in logits.shape)
+    if rows > 1 and logits.stride(0) < vocab:
+        raise ValueError("rows of logits must not overlap")
+    if vocab < 1 or not 0 <= int(top) <= min(MAX_TOP, vocab):
+        raise ValueError(f"top must be 0 to {MAX_TOP} and no more than the vocabulary")
+    if not (temperature > 0.0 and 1e-30 <= temperature <= 1e30):
+        raise ValueError("temperature must be positive")
+    if tokens is not None and (tokens.dtype != torch.int64 or tokens.numel() != rows or not tokens.is_contiguous()):
+        raise ValueError("tokens must be contiguous int64 [R]")
+    code = dtype_code(logits.dtype)
+    with _launch(logits, tokens) as stream:
+        new = {"device": logits.device}
+        result = TokenLogprobs(None if tokens is None else torch.empty(rows, dtype=torch.float32, **new), torch.empty(rows, dtype=torch.float32, **new),
+                               torch.empty((rows, top), dtype=torch.int64, **new) if top else None,
+                               torch.empty((rows, top), dtype=torch.float32, **new) if top else None)
+        check(_lib.load_group("serving").cacheir_b200_token_logprobs(
+            logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _ptr(tokens), _ptr(result.logprobs), result.entropy.data_ptr(),
+            _ptr(result.top_ids), _ptr(result.top_logprobs), rows, vocab, int(top), float(temperature), code, stream), "token_logprobs")
+    return result
