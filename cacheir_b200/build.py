@@ -35,7 +35,7 @@ GROUP_FILES = {
     "recurrence": ("linear_recurrence",),
     "talking": ("talking_attention", "talking_prompt"),
     "delta": ("short_conv", "delta_rule"),
-    "serving": ("page_tables", "rotary_append", "shared_prefix", "token_logprobs"),
+    "serving": ("page_tables", "rotary_append", "shared_prefix", "shared_prefix_mma", "token_logprobs"),
     "experts": ("tied_attention", "tied_prompt", "grouped_gemm", "expert_routing"),
 }
 LIB_PATHS = {"core": LIB_DIR / "libcacheir_b200.so", **{name: LIB_DIR / f"libcacheir_b200_{name}.so" for name in GROUP_FILES}}

@@ -196,7 +196,7 @@ using namespace cb200;
 extern "C" size_t cacheir_b200_shared_prefix_workspace_bytes(int batch, int heads, int dim) {
   if (batch <= 0 || heads <= 0 || dim <= 0) return 0;
   const int pieces = prefix_pieces(batch, heads, dim);
-  return prefix_ml_bytes(batch, heads, pieces) + static_cast<size_t>(pieces) * batch * heads * dim * 4;
+  return prefix_plan_bytes(batch) + prefix_ml_bytes(batch, heads, pieces) + static_cast<size_t>(pieces) * batch * heads * dim * 4;
 }
 
 extern "C" int cacheir_b200_shared_prefix_attention(const cacheir_b200_prefix_args* args, void* stream) {
@@ -206,6 +206,7 @@ extern "C" int cacheir_b200_shared_prefix_attention(const cacheir_b200_prefix_ar
   if (!a.q || !a.k_cache || !a.v_cache || !a.out || !a.page_table || !a.seq_lens || a.kv_heads <= 0 || a.heads % a.kv_heads != 0 || a.dim <= 0 ||
       a.page_size <= 0 || a.num_slots <= 0 || a.max_pages <= 0 || a.groups < 0 || dtype_size(a.dtype) == 0)
     return CACHEIR_B200_EINVAL;
+  if (a.groups > a.batch) return CACHEIR_B200_EINVAL;
   if (a.groups > 0 && (!a.group_rows || !a.prefix_table || !a.prefix_lens || a.prefix_pages <= 0)) return CACHEIR_B200_EINVAL;
   if (a.dim > kGeneralDim) return CACHEIR_B200_EUNSUPPORTED;
   if (a.batch > 65535 || a.kv_heads > 65535 || static_cast<long long>(a.max_pages) * a.page_size > 0x7fffffffLL ||
@@ -216,14 +217,14 @@ extern "C" int cacheir_b200_shared_prefix_attention(const cacheir_b200_prefix_ar
   if (!(a.softmax_scale > 0.f)) a.softmax_scale = 1.0f / sqrtf(static_cast<float>(a.dim));
   PrefixParts parts;
   parts.pieces = prefix_pieces(a.batch, a.heads, a.dim);
-  parts.ml = static_cast<float*>(a.workspace);
-  parts.acc = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + prefix_ml_bytes(a.batch, a.heads, parts.pieces));
+  char* scratch = static_cast<char*>(a.workspace);
+  parts.plan = reinterpret_cast<PrefixPlan*>(scratch);
+  parts.ml = reinterpret_cast<float*>(scratch += prefix_plan_bytes(a.batch));
+  parts.acc = reinterpret_cast<float*>(scratch + prefix_ml_bytes(a.batch, a.heads, parts.pieces));
+  if (prefix_fast_supported(a)) return launch_prefix_fast(a, parts, as_stream(stream));
   if (a.dtype == CACHEIR_B200_F32) return launch_general<float>(a, parts, as_stream(stream));
   if (a.dtype == CACHEIR_B200_F16) return launch_general<__half>(a, parts, as_stream(stream));
   return launch_general<__nv_bfloat16>(a, parts, as_stream(stream));
 }
 
-extern "C" int cacheir_b200_serving_device_status(int reset) {
-  (void)reset;
-  return 0;
-}
+extern "C" int cacheir_b200_serving_device_status(int reset) { return prefix_device_status(reset != 0); }

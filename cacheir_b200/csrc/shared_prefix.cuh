@@ -6,8 +6,16 @@
 
 namespace cb200 {
 
-// Where partial results go: for every (piece, row, head) a maximum (log2 domain) and a denominator, and the unnormalised output.
+// What the kernel of the common parts leaves for the one that joins: how its work was cut (see shared_prefix_mma.cu).
+struct PrefixPlan {
+  long long units;            // key tiles of all items
+  long long ctas;             // blocks that share them
+  long long start[1];         // [groups + 1] first unit of every group
+};
+
+// The scratch: plan, then for every (piece, row, head) a maximum (log2 domain) and a denominator, and the unnormalised output.
 struct PrefixParts {
+  PrefixPlan* plan;
   float* ml;       // [pieces][batch][heads][2]
   float* acc;      // [pieces][batch][heads][dim]
   int pieces;
@@ -16,15 +24,20 @@ struct PrefixParts {
 // First row of group g, inside the batch whatever the caller's array holds.
 __device__ __forceinline__ int group_start(const cacheir_b200_prefix_args& a, int g) { return min(max(a.group_rows[g], 0), a.batch); }
 
-// The group of a row (group_rows is ascending); -1 outside every group.
+// The group of a row (group_rows is ascending), -1 outside every group; a whole warp, which looks at 32 starts at a time.
 __device__ __forceinline__ int group_of_row(const cacheir_b200_prefix_args& a, int row) {
-  if (a.groups <= 0 || row < a.group_rows[0] || row >= a.group_rows[a.groups]) return -1;
-  int lo = 0, hi = a.groups;               // last g with group_rows[g] <= row
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.group_rows[mid] <= row) lo = mid; else hi = mid;
+  if (a.groups <= 0) return -1;
+  int lo = 0, hi = a.groups + 1;           // the number of starts up to `row` is in lo .. hi
+  const int lane = threadIdx.x & 31;
+  while (hi > lo) {
+    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const int below = __popc(__ballot_sync(0xffffffffu, at < hi && a.group_rows[at] <= row));
+    if (below == 0) break;
+    const int first = lo + (below - 1) * step;        // its start is at or below the row
+    hi = min(hi, first + step);
+    lo = first + 1;
   }
-  return lo;
+  return lo == a.groups + 1 ? -1 : lo - 1;
 }
 
 __device__ __forceinline__ int prefix_of_group(const cacheir_b200_prefix_args& a, int g) {
@@ -33,14 +46,20 @@ __device__ __forceinline__ int prefix_of_group(const cacheir_b200_prefix_args& a
 }
 
 constexpr int kMaxPieces = 64;
+constexpr int kMinPieces = 4;
 // Pieces per row that the scratch holds: 64 MB of them, but 4 at least.
 inline int prefix_pieces(int batch, int heads, int dim) {
   const size_t one = static_cast<size_t>(batch) * heads * dim * 4;
-  const size_t n = one > 0 ? (static_cast<size_t>(64) << 20) / one : 4;
-  return n < 4 ? 4 : n > kMaxPieces ? kMaxPieces : static_cast<int>(n);
+  const size_t n = one > 0 ? (static_cast<size_t>(64) << 20) / one : kMinPieces;
+  return n < kMinPieces ? kMinPieces : n > kMaxPieces ? kMaxPieces : static_cast<int>(n);
 }
-inline size_t prefix_ml_bytes(int batch, int heads, int pieces) {
-  return (static_cast<size_t>(pieces) * batch * heads * 2 * 4 + 255) / 256 * 256;
-}
+inline size_t round_up_256(size_t n) { return (n + 255) / 256 * 256; }
+inline size_t prefix_plan_bytes(int batch) { return round_up_256(sizeof(PrefixPlan) + static_cast<size_t>(batch) * sizeof(long long)); }
+inline size_t prefix_ml_bytes(int batch, int heads, int pieces) { return round_up_256(static_cast<size_t>(pieces) * batch * heads * 2 * 4); }
+
+// Tensor-core kernels (shared_prefix_mma.cu): 16-bit types, head sizes 64 and 128, pages of a multiple of 16 tokens.
+bool prefix_fast_supported(const cacheir_b200_prefix_args& a);
+int launch_prefix_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cudaStream_t stream);
+int prefix_device_status(bool reset);
 
 }  // namespace cb200

@@ -1,0 +1,929 @@
+// Decode attention of groups of sequences with a common prefix on the tensor cores: 16-bit types, head sizes 64 and 128, pages of a multiple
+// of 16 tokens, up to 64 query heads per key/value head.
+//
+// Two kernels. The first one multiplies the common keys of a group, once, with the queries of all of its rows that share a key/value
+// head: S = Q K^T and O = P V as tcgen05 MMAs of 128 query rows, scores, probabilities and outputs in tensor memory. The second one takes
+// every row's own keys with warp MMAs, like the ordinary decode attention, and joins the pieces.
+//
+// Common part. An item is (group, key/value head, tile of up to 256 query rows); its keys come in tiles of 128. The key tiles of all items,
+// in a row, are cut evenly over the blocks, so that lengths and sizes of groups do not matter; an item that is cut leaves one piece per
+// block. One warp brings keys and values (TMA, page by page, into a ring of 32 KB slots), one issues the MMAs, and two groups of four
+// warps do the softmax, a thread per query row. Above 128 rows each group of warps has its own 128 of them and the two take turns on the
+// tensor cores with the same keys; else the first one has them all and scores run one tile ahead. A row's maximum is a reference that
+// moves only when it is exceeded by 2^14, so that the outputs, which stay in tensor memory, are hardly ever rescaled; probabilities are
+// rounded to the element type as the second MMA's operand, their sums are not.
+#include "shared_prefix.cuh"
+
+#include <cuda.h>
+
+#include "hybrid_common.cuh"
+#include "tc_ptx.cuh"
+
+namespace cb200 {
+namespace {
+
+using namespace ptx;
+
+constexpr int kKeys = 128;                     // keys of a tile
+constexpr int kRows = 128;                     // query rows of a group of warps
+constexpr int kChunk = 16;                     // keys that one copy brings: no page ends inside
+constexpr int kCommonThreads = 320;
+constexpr int kPlanGroups = 128;               // groups that every block lays out by itself
+constexpr int kMaxHeadsPerKv = 64;
+constexpr float kAhead = 6.f;                  // a new reference is the maximum less this: probabilities start at 2^6 ..
+constexpr float kStale = 14.f;                 // .. and may grow to 2^14 (in fp16: 2^-24 of that is still a number)
+
+__device__ int g_prefix_status = 0;
+
+struct CommonParams {
+  cacheir_b200_prefix_args a;
+  PrefixParts parts;
+  int plan_ready;                              // the plan is in the scratch already
+  int tile_rows;                               // batch rows of an item
+  float scale_log2;
+};
+
+// ---- PTX that only these kernels use ----
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_st_x32(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Operand whose rows are the MMA's k: boxes of 64 columns by 128 rows (16 KB apart), 8-row groups 1024 B apart.
+__device__ __forceinline__ uint64_t smem_desc_columns(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | static_cast<uint64_t>((kKeys * 128) >> 4) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
+         static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// ---- how the common parts are cut ----
+__device__ __forceinline__ long long group_units(const cacheir_b200_prefix_args& a, int tile_rows, int g, long long* tiles) {
+  const int rows = group_start(a, g + 1) - group_start(a, g), keys = rows > 0 ? prefix_of_group(a, g) : 0;
+  *tiles = (keys + kKeys - 1) / kKeys;
+  return rows > 0 ? static_cast<long long>(a.kv_heads) * ((rows + tile_rows - 1) / tile_rows) * *tiles : 0;
+}
+// Blocks that take part: one unit each at least, and no item in more pieces than there is scratch for (`longest` key tiles in
+// units / ctas at a time, cut anywhere: two more than the quotient at most).
+__device__ __forceinline__ long long plan_ctas(long long units, long long longest, int grid, int pieces) {
+  if (units <= 0) return 0;
+  const long long most = units * (pieces - 2) / longest;
+  return max(1LL, min(min(static_cast<long long>(grid), units), most));
+}
+
+// The plan of more groups than a block lays out by itself.
+__global__ void __launch_bounds__(1024)
+prefix_plan_kernel(const CommonParams p, const int grid) {
+  chain_enter();
+  __shared__ long long s_sum[32], s_max[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long base = 0, longest = 0;
+  for (int g0 = 0; g0 < p.a.groups; g0 += 1024) {
+    const int g = g0 + threadIdx.x;
+    long long tiles = 0, own = g < p.a.groups ? group_units(p.a, p.tile_rows, g, &tiles) : 0, sum = own;
+    if (own > 0) longest = max(longest, tiles);
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= off) sum += up;
+    }
+    if (lane == 31) s_sum[warp] = sum;
+    __syncthreads();
+    long long before = 0, all = 0;
+    for (int w = 0; w < 32; ++w) {
+      if (w < warp) before += s_sum[w];
+      all += s_sum[w];
+    }
+    if (g < p.a.groups) p.parts.plan->start[g] = base + before + sum - own;
+    base += all;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, off));
+  if (lane == 0) s_max[warp] = longest;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < 32; ++w) longest = max(longest, s_max[w]);
+    p.parts.plan->start[p.a.groups] = base;
+    p.parts.plan->units = base;
+    p.parts.plan->ctas = plan_ctas(base, longest, grid, p.parts.pieces);
+  }
+}
+
+// A block's share of the units, item by item.
+struct Walk {
+  const long long* start;      // of every group
+  long long units, ctas, at, end;
+  // the item
+  int group, kvh, row0, rows, tile, tiles, prefix, piece;      // key tiles tile .. tile + tiles - 1 of it are this block's
+  const int32_t* pages;
+
+  __device__ __forceinline__ void init(const long long* s, long long u, long long c, int block) {
+    start = s;
+    units = u;
+    ctas = c;
+    at = block * u / c;
+    end = (block + 1) * u / c;
+  }
+  __device__ __forceinline__ bool next(const CommonParams& p) {
+    if (at >= end) return false;
+    int lo = 0, hi = p.a.groups;                               // last group that starts at or before `at` (empty ones start where the next does)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (start[mid] <= at) lo = mid; else hi = mid;
+    }
+    group = lo;
+    const int first = group_start(p.a, lo), count = group_start(p.a, lo + 1) - first;
+    prefix = prefix_of_group(p.a, lo);
+    pages = p.a.prefix_table + static_cast<size_t>(lo) * p.a.prefix_pages;
+    const int all = (prefix + kKeys - 1) / kKeys, row_tiles = (count + p.tile_rows - 1) / p.tile_rows;
+    const long long rel = at - start[lo], item = rel / all;
+    kvh = static_cast<int>(item / row_tiles);
+    row0 = first + static_cast<int>(item % row_tiles) * p.tile_rows;
+    rows = min(p.tile_rows, first + count - row0);
+    tile = static_cast<int>(rel - item * all);
+    tiles = static_cast<int>(min(static_cast<long long>(all - tile), end - at));
+    piece = static_cast<int>(blockIdx.x - ((start[lo] + item * all + 1) * ctas - 1) / units);
+    at += tiles;
+    return true;
+  }
+};
+
+template <int D>
+struct CommonSmem {
+  static constexpr int kSlotBytes = kKeys * D * 2;
+  static constexpr int kSlots = D == 128 ? 5 : 10;
+  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kTiles = 2 * kQBytes + kSlots * kSlotBytes;
+  // then: barriers full, empty [slots], q[2], s[2], p[2], o[2]; tensor memory address; group starts
+  static constexpr int kBarriers = 2 * kSlots + 8;
+  static constexpr int kBytes = 1024 + kTiles + kBarriers * 8 + 16 + (kPlanGroups + 1) * 8;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kCommonThreads, 1)
+prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CommonParams p) {
+  using L = CommonSmem<D>;
+  constexpr int kSlots = L::kSlots;
+  chain_enter();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* s_q = smem;                                         // [2][D / 64][128 rows][128 B]
+  uint8_t* s_kv = smem + 2 * L::kQBytes;                       // [slots][D / 64][128 keys][128 B]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kTiles);
+  uint64_t* empty = full + kSlots;
+  uint64_t* bar_q = empty + kSlots;                            // a group of warps has left its queries
+  uint64_t* bar_s = bar_q + 2;                                 // scores are in tensor memory
+  uint64_t* bar_p = bar_s + 2;                                 // probabilities are
+  uint64_t* bar_o = bar_p + 2;                                 // .. and have been added to the output
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_o + 2);
+  long long* s_start = reinterpret_cast<long long*>(tmem_slot + 4);
+  __shared__ long long s_plan[2];
+  __shared__ long long s_scan[4], s_longest[4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const cacheir_b200_prefix_args& a = p.a;
+
+  // ---- the plan ----
+  if (!p.plan_ready) {
+    long long own = 0, sum = 0;
+    if (warp < kPlanGroups / 32) {
+      long long tiles = 0;
+      const int g = threadIdx.x;
+      own = g < a.groups ? group_units(a, p.tile_rows, g, &tiles) : 0;
+      long long longest = own > 0 ? tiles : 0;
+      sum = own;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, sum, off);
+        if (lane >= off) sum += up;
+        longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, off));
+      }
+      if (lane == 31) { s_scan[warp] = sum; s_longest[warp] = longest; }
+    }
+    __syncthreads();
+    if (warp < kPlanGroups / 32) {
+      long long before = 0, all = 0, longest = 0;
+#pragma unroll
+      for (int w = 0; w < kPlanGroups / 32; ++w) {
+        if (w < warp) before += s_scan[w];
+        all += s_scan[w];
+        longest = max(longest, s_longest[w]);
+      }
+      if (static_cast<int>(threadIdx.x) < a.groups) s_start[threadIdx.x] = before + sum - own;
+      if (threadIdx.x == 0) {
+        s_start[a.groups] = all;
+        s_plan[0] = all;
+        s_plan[1] = plan_ctas(all, longest, gridDim.x, p.parts.pieces);
+      }
+    }
+  }
+  if (threadIdx.x == 288) {
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&bar_q[b]), kRows);
+      mbar_init(smem_u32(&bar_s[b]), 1);
+      mbar_init(smem_u32(&bar_p[b]), kRows);
+      mbar_init(smem_u32(&bar_o[b]), 1);
+    }
+    mbar_fence_init();
+  }
+  __syncthreads();
+  const long long* start = p.plan_ready ? p.parts.plan->start : s_start;
+  const long long units = p.plan_ready ? p.parts.plan->units : s_plan[0], ctas = p.plan_ready ? p.parts.plan->ctas : s_plan[1];
+  if (!p.plan_ready && blockIdx.x == 0) {                      // for the kernel that joins
+    for (int g = threadIdx.x; g <= a.groups; g += kCommonThreads) p.parts.plan->start[g] = s_start[g];
+    if (threadIdx.x == 0) {
+      p.parts.plan->units = units;
+      p.parts.plan->ctas = ctas;
+    }
+  }
+  if (static_cast<long long>(blockIdx.x) >= ctas) return;
+  if (warp == 8) tc_alloc(smem_u32(tmem_slot), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;                            // scores [2][128 columns] (probabilities over them), outputs [2][D]
+  const uint32_t tmem_o = tmem + 2 * kKeys;
+  const int group = a.heads / a.kv_heads;
+  Walk walk;
+  walk.init(start, units, ctas, blockIdx.x);
+  bool ok = true;
+
+  if (warp == 9) {
+    // ---------------- copies: a lane per 16 keys and 64 columns ----------------
+    constexpr int kBoxes = D / 64;
+    const int chunk = lane / kBoxes, box = lane % kBoxes;
+    const bool copies = chunk < kKeys / kChunk;
+    const int outside = a.num_slots * a.kv_heads * a.page_size;         // rows behind the pool read as zeros
+    int slot = 0;
+    uint32_t phase = 1, sent = 0;
+    while (ok && walk.next(p)) {
+      auto line_of = [&](int tile) {                           // first row of this lane's keys in the pool
+        const int key = tile * kKeys + chunk * kChunk;
+        if (!copies || key >= walk.prefix) return outside;
+        const int id = walk.pages[key / a.page_size];
+        return id >= 0 && id < a.num_slots ? (id * a.kv_heads + walk.kvh) * a.page_size + key % a.page_size : outside;
+      };
+      int line = line_of(walk.tile);
+      for (int t = walk.tile; t < walk.tile + walk.tiles && ok; ++t) {
+        const int next = t + 1 < walk.tile + walk.tiles ? line_of(t + 1) : 0;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          ok = ok && mbar_wait(smem_u32(&empty[slot]), phase, &g_prefix_status, (15 << 8) | 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(smem_u32(&full[slot]), L::kSlotBytes);
+          __syncwarp();
+          if (copies)
+            tma_load_2d(smem_u32(s_kv + slot * L::kSlotBytes + box * kKeys * 128 + chunk * kChunk * 128), kv == 0 ? &tmap_k : &tmap_v,
+                        smem_u32(&full[slot]), box * 64, line);
+          ++sent;
+          if (++slot == kSlots) { slot = 0; phase ^= 1; }
+        }
+        line = next;
+      }
+    }
+    // nothing may still be on its way when the block ends, also after a wait that gave up
+    for (uint32_t i = sent > kSlots ? sent - kSlots : 0; i < sent; ++i)
+      mbar_wait(smem_u32(&full[i % kSlots]), (i / kSlots) & 1, &g_prefix_status, (15 << 8) | 2);
+  } else if (warp == 8) {
+    // ---------------- MMA issue ----------------
+    constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
+    const uint32_t id_s = (1u << 4) | (kType << 7) | (kType << 10) | (static_cast<uint32_t>(kKeys >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
+    const uint32_t id_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) |
+                          (static_cast<uint32_t>(kRows >> 4) << 24);
+    const uint64_t dq = smem_desc_sw128(smem_u32(s_q)), dk = smem_desc_sw128(smem_u32(s_kv)), dv = smem_desc_columns(smem_u32(s_kv));
+    // Scores and outputs step through the same (tile, buffer) sequence, scores up to two steps ahead.
+    struct Steps {
+      Walk walk;
+      int left = 0, two = 0, second = 0, tile = 0, first = 0;  // key tiles left in the item, two steps per tile?, the second of them?, tiles so far
+      __device__ __forceinline__ bool ready(const CommonParams& p, int group) {
+        if (left > 0) return true;
+        if (!walk.next(p)) return false;
+        left = first = walk.tiles;
+        two = walk.rows * group > kRows ? 1 : 0;
+        return true;
+      }
+      // (returns whether the tile's slot is free after this step)
+      __device__ __forceinline__ bool advance() {
+        if (two && !second) { second = 1; return false; }
+        second = 0;
+        --left;
+        ++tile;
+        return true;
+      }
+    } score, output;
+    score.walk = walk;
+    output.walk = walk;
+    int next_s = 0, next_o = 0;
+    uint32_t q_seen[2] = {0, 0};
+    while (ok) {
+      // (an item's queries come after the last output of the item before)
+      if (next_s - next_o < 2 && score.ready(p, group) && (next_s == next_o || score.left < score.first || score.second)) {
+        const int b = next_s & 1, w = score.two ? b : 0, slot = (2 * score.tile) % kSlots;
+        if (score.left == score.first) {                       // the item's first tile: its queries are new
+          ok = mbar_wait(smem_u32(&bar_q[w]), q_seen[w] & 1, &g_prefix_status, (15 << 8) | 3);
+          ++q_seen[w];
+        }
+        ok = ok && mbar_wait(smem_u32(&full[slot]), (2 * score.tile / kSlots) & 1, &g_prefix_status, (15 << 8) | 4);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc_fence_after();
+        const bool frees = score.advance();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_ss(tmem + b * kKeys, dq + ((w * L::kQBytes + (k >> 2) * kRows * 128 + (k & 3) * 32) >> 4),
+                   dk + ((slot * L::kSlotBytes + (k >> 2) * kKeys * 128 + (k & 3) * 32) >> 4), id_s, k > 0 ? 1u : 0u);
+          tc_commit(smem_u32(&bar_s[b]));
+          if (frees) tc_commit(smem_u32(&empty[slot]));
+        }
+        __syncwarp();
+        ++next_s;
+        continue;
+      }
+      if (!output.ready(p, group)) break;
+      const int b = next_o & 1, w = output.two ? b : 0, at = 2 * output.tile + 1, slot = at % kSlots;
+      ok = mbar_wait(smem_u32(&full[slot]), (at / kSlots) & 1, &g_prefix_status, (15 << 8) | 5);
+      ok = ok && mbar_wait(smem_u32(&bar_p[b]), (next_o >> 1) & 1, &g_prefix_status, (15 << 8) | 6);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      tc_fence_after();
+      const bool opens = output.left == output.first, frees = output.advance();
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k)
+          mma_ts(tmem_o + w * D, tmem + b * kKeys + k * 8, dv + ((slot * L::kSlotBytes + k * 16 * 128) >> 4), id_o, opens && k == 0 ? 0u : 1u);
+        tc_commit(smem_u32(&bar_o[b]));
+        if (frees) tc_commit(smem_u32(&empty[slot]));
+      }
+      __syncwarp();
+      ++next_o;
+    }
+  } else {
+    // ---------------- softmax: a thread per query row ----------------
+    const int w = warp >> 2, r = threadIdx.x & (kRows - 1);
+    const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    int step = 0, tile = 0;                                    // of the block so far
+    while (ok && walk.next(p)) {
+      const int used = walk.rows * group, two = used > kRows ? 1 : 0, steps = walk.tiles * (two ? 2 : 1);
+      if (!two && w == 1) {                                    // (its barrier's phases pass all the same)
+        for (int s = step | 1; s < step + steps && ok; s += 2) ok = mbar_wait(smem_u32(&bar_s[1]), (s >> 1) & 1, &g_prefix_status, (15 << 8) | 7);
+        step += steps;
+        tile += walk.tiles;
+        continue;
+      }
+      // queries: rows of this group of warps, zeros behind the last one
+      const int q_row0 = w * kRows;
+      for (int i = r; i < kRows * (D / 8); i += kRows) {
+        const int row = i / (D / 8), c = i % (D / 8), at = q_row0 + row;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (at < used)
+          v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + static_cast<size_t>(walk.row0 + at / group) * a.q_stride +
+                                              static_cast<size_t>(walk.kvh * group + at % group) * D + c * 8);
+        *reinterpret_cast<uint4*>(s_q + w * L::kQBytes + (c >> 3) * kRows * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+      }
+      fence_async_smem();
+      mbar_arrive(smem_u32(&bar_q[w]));
+      const int mine = q_row0 + r;
+      const bool real = mine < used;
+      const int b_row = walk.row0 + (real ? mine / group : 0), head = walk.kvh * group + (real ? mine % group : 0);
+      const int limit = real ? min(walk.prefix, a.seq_lens[b_row]) : walk.prefix;      // keys that the row sees
+      float m_ref = -INFINITY, l_run = 0.f;
+      int last = 0;
+      for (int t = 0, s = two ? step + ((step ^ w) & 1) : step; t < walk.tiles && ok; ++t, s += two ? 2 : 1) {
+        const int b = s & 1, base = (walk.tile + t) * kKeys;
+        ok = mbar_wait(smem_u32(&bar_s[b]), (s >> 1) & 1, &g_prefix_status, (15 << 8) | 8);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t v[kKeys];
+        const uint32_t scores = tmem + b * kKeys + lane_addr;
+#pragma unroll
+        for (int c = 0; c < kKeys; c += 32) tmem_ld_x32(scores + c, v + c);
+        tc_wait_ld();
+        if (!__all_sync(0xffffffffu, base + kKeys <= limit)) {
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i)
+            if (base + i >= limit) v[i] = 0xff800000u;         // -inf
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        const bool grown = top > m_ref + kStale;
+        if (__any_sync(0xffffffffu, grown)) {
+          const float fresh = grown ? top - kAhead : m_ref, alpha = grown ? ex2(m_ref - fresh) : 1.f;
+          m_ref = fresh;
+          l_run *= alpha;
+          if (t > 0) {                                         // bring the output to the new reference
+            // (with two groups of warps this buffer's last output came before these scores)
+            if (!two) ok = mbar_wait(smem_u32(&bar_o[(s - 1) & 1]), ((s - 1) >> 1) & 1, &g_prefix_status, (15 << 8) | 9);
+            __syncwarp();
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld_x32(tmem_o + w * D + lane_addr + c, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_x32(tmem_o + w * D + lane_addr + c, o);
+            }
+          }
+        }
+        const float ref = m_ref > -INFINITY ? m_ref : 0.f;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 2) {
+          const float x = ex2(fmaf(__uint_as_float(v[i]), p.scale_log2, -ref)), y = ex2(fmaf(__uint_as_float(v[i + 1]), p.scale_log2, -ref));
+          sum[i & 2] += x;
+          sum[(i & 2) + 1] += y;
+          v[i >> 1] = pack_pair<T>(x, y);
+        }
+        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st_x32(scores, v);
+        tmem_st_x32(scores + 32, v + 32);
+        tmem_wait_st();
+        // keys behind the prefix in its last page may hold anything: zero their values, so that 0 * value stays 0
+        const int rest = walk.prefix - base;
+        if (rest < kKeys && rest % kChunk != 0) {
+          const int at = 2 * (tile + t) + 1, slot = at % kSlots;
+          ok = mbar_wait(smem_u32(&full[slot]), (at / kSlots) & 1, &g_prefix_status, (15 << 8) | 10);
+          const int rows = kChunk - rest % kChunk;
+          for (int i = r; i < rows * (D / 8); i += kRows) {
+            const int key = rest + i / (D / 8), c = i % (D / 8);
+            *reinterpret_cast<uint4*>(s_kv + slot * L::kSlotBytes + (c >> 3) * kKeys * 128 + key * 128 + ((c & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_smem();
+        }
+        tc_fence_before();
+        mbar_arrive(smem_u32(&bar_p[b]));
+        last = s;
+      }
+      step += steps;
+      tile += walk.tiles;
+      if (!ok) break;
+      ok = mbar_wait(smem_u32(&bar_o[last & 1]), (last >> 1) & 1, &g_prefix_status, (15 << 8) | 11);
+      __syncwarp();
+      tc_fence_after();
+      const size_t at = (static_cast<size_t>(walk.piece) * a.batch + b_row) * a.heads + head;
+      if (real) *reinterpret_cast<float2*>(p.parts.ml + 2 * at) = make_float2(m_ref, l_run);
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        tmem_ld_x32(tmem_o + w * D + lane_addr + c, o);
+        tc_wait_ld();
+        if (real) {
+          uint4* dst = reinterpret_cast<uint4*>(p.parts.acc + at * D + c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+      }
+      tc_fence_before();
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tc_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Every row's own keys, and the pieces joined. One block per (part of the row's own keys, key/value head and up to 16 of its query heads, row);
+// the parts are a thread-block cluster. Keys and values come 16 tokens at a time (TMA) through a ring, four warps take one chunk of a
+// stage each with warp MMAs, the query heads as their 16 rows: bound by the memory's rate. None of that needs the common part's kernel:
+// this one starts as soon as that one's blocks leave room, and waits for it before it joins.
+constexpr int kOwnWarps = 4;
+constexpr int kOwnThreads = (kOwnWarps + 1) * 32;
+constexpr int kOwnStages = 3;
+constexpr int kMaxOwnSplits = 8;
+
+struct OwnParams {
+  cacheir_b200_prefix_args a;
+  PrefixParts parts;
+  int common;                                  // a kernel of common parts runs before
+  int tile_rows, head_chunks, splits;
+  float scale_log2;
+};
+
+template <int D>
+struct OwnSmem {
+  static constexpr int kTileBytes = kChunk * D * 2;
+  static constexpr int kStageBytes = kOwnWarps * 2 * kTileBytes;
+  // over the ring afterwards: the warps' states, the block's, and the weights of all sources of a head
+  static constexpr int kSources = kMaxPieces + kMaxOwnSplits;
+  static constexpr int kJoin = (kOwnWarps * 16 * (D + 2) + 16 * (D + 2) + 16 * kSources) * 4;
+  static constexpr int kRing = kOwnStages * kStageBytes;
+  static constexpr int kBytes = 1024 + (kRing > kJoin ? kRing : kJoin) + 2 * kOwnStages * 8;
+};
+
+__device__ __forceinline__ void ldsm_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+template <typename T>
+__device__ __forceinline__ void mma_pair(float (&c)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));
+  else
+    mma_bf16(c, x, b0, b1);
+}
+__device__ __forceinline__ float ld_rank_f32(const float* local, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(smem_u32(local), rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_rank_f32x4(const float* local, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(map_to_rank(smem_u32(local), rank)) : "memory");
+  return v;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kOwnThreads)
+prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ OwnParams p) {
+  using L = OwnSmem<D>;
+  constexpr int kBoxes = D / 64;
+  // What stands before this wait reads what was there before the common part's kernel began: its blocks let this one in only after they
+  // had waited for all earlier ones.
+  if (!p.common) chain_enter();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw + L::kBytes - 2 * kOwnStages * 8);
+  uint64_t* empty = full + kOwnStages;
+  const cacheir_b200_prefix_args& a = p.a;
+  const int split = blockIdx.x, kvh = blockIdx.y / p.head_chunks, row = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = a.heads / a.kv_heads, head0 = kvh * group + blockIdx.y % p.head_chunks * 16, heads = min(16, (kvh + 1) * group - head0);
+  const int g = lane >> 2, t4 = lane & 3;
+  uint32_t qa[D / 16][4];                                       // queries as the A operand: rows = heads
+  if (warp < kOwnWarps) {
+    const T* q = static_cast<const T*>(a.q) + static_cast<size_t>(row) * a.q_stride + static_cast<size_t>(head0) * D;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int h = g + (i & 1) * 8, col = k * 16 + 2 * t4 + (i >> 1) * 8;
+        qa[k][i] = h < heads ? *reinterpret_cast<const uint32_t*>(q + static_cast<size_t>(h) * D + col) : 0u;
+      }
+  }
+  const int len = min(max(a.seq_lens[row], 0), a.max_pages * a.page_size);
+  const int of = group_of_row(a, row);
+  const int prefix = of < 0 ? 0 : prefix_of_group(a, of);
+  const int from = min(prefix, len);
+  const int chunk0 = from / kChunk, chunks = len > from ? (len + kChunk - 1) / kChunk - chunk0 : 0, per = (chunks + p.splits - 1) / p.splits;
+  const int begin = chunk0 + min(chunks, split * per), count = min(chunks, (split + 1) * per) - min(chunks, split * per);
+  const int iters = (count + kOwnWarps - 1) / kOwnWarps;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kOwnStages; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), kOwnWarps);
+    }
+    mbar_fence_init();
+  }
+  __syncthreads();
+
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f}, o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  bool ok = true;
+  if (warp == kOwnWarps) {
+    // ---------------- copies: a lane per chunk and 64 columns of the keys, the same of the values ----------------
+    const int32_t* pages = a.page_table + static_cast<size_t>(row) * a.max_pages;
+    const int outside = a.num_slots * a.kv_heads * a.page_size;
+    const int c = lane / kBoxes, box = lane % kBoxes;
+    auto line_of = [&](int it) {
+      const int at = it * kOwnWarps + c;
+      if (c >= kOwnWarps || at >= count) return outside;
+      const int key = (begin + at) * kChunk, id = pages[key / a.page_size];
+      return id >= 0 && id < a.num_slots ? (id * a.kv_heads + kvh) * a.page_size + key % a.page_size : outside;
+    };
+    int line = line_of(0);
+    for (int it = 0; it < iters && ok; ++it) {
+      const int s = it % kOwnStages, now = min(kOwnWarps, count - it * kOwnWarps);
+      const int next = line_of(it + 1);
+      ok = mbar_wait(smem_u32(&empty[s]), ((it / kOwnStages) & 1) ^ 1, &g_prefix_status, (15 << 8) | 12);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane == 0) mbar_expect_tx(smem_u32(&full[s]), now * 2 * L::kTileBytes);
+      __syncwarp();
+      if (c < now) {
+        const uint32_t dst = smem_u32(smem + s * L::kStageBytes + c * 2 * L::kTileBytes + box * kChunk * 128);
+        tma_load_2d(dst, &tmap_k, smem_u32(&full[s]), box * 64, line);
+        tma_load_2d(dst + L::kTileBytes, &tmap_v, smem_u32(&full[s]), box * 64, line);
+      }
+      line = next;
+    }
+    if (!ok)                                                    // nothing may still be on its way when the ring is used for something else
+      for (int s = 0; s < kOwnStages; ++s) {
+        mbar_wait(smem_u32(&full[s]), 0, &g_prefix_status, (15 << 8) | 13);
+        mbar_wait(smem_u32(&full[s]), 1, &g_prefix_status, (15 << 8) | 13);
+      }
+  } else {
+    const uint32_t lrow = lane & 7, lmat = lane >> 3;
+    for (int it = 0; it < iters && ok; ++it) {
+      const int s = it % kOwnStages, mine = it * kOwnWarps + warp;
+      ok = mbar_wait(smem_u32(&full[s]), (it / kOwnStages) & 1, &g_prefix_status, (15 << 8) | 14);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (mine < count) {
+        const uint32_t kbase = smem_u32(smem + s * L::kStageBytes + warp * 2 * L::kTileBytes), vbase = kbase + L::kTileBytes;
+        float sc[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+          const uint32_t token = n * 8 + lrow;
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k) {
+            const uint32_t c = 4 * k + lmat;
+            uint32_t kb[4];
+            ldsm_x4(kbase + (c >> 3) * (kChunk * 128) + token * 128 + (((c & 7) ^ (token & 7)) << 4), kb);
+            mma_pair<T>(sc[n], qa[2 * k], kb[0], kb[1]);
+            mma_pair<T>(sc[n], qa[2 * k + 1], kb[2], kb[3]);
+          }
+        }
+        const int key0 = (begin + mine) * kChunk;
+        const bool whole = key0 >= from && key0 + kChunk <= len;
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + n * 8 + 2 * t4 + (e & 1);
+            const float v = whole || (key >= from && key < len) ? sc[n][e] * p.scale_log2 : -INFINITY;
+            sc[n][e] = v;
+            top[e >> 1] = fmaxf(top[e >> 1], v);
+          }
+        float corr[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+          const float m_new = fmaxf(m_run[r], top[r]);           // finite: every chunk has a key that counts
+          corr[r] = ex2(m_run[r] - m_new);
+          m_run[r] = m_new;
+        }
+        float pr[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pr[n][e] = ex2(sc[n][e] - m_run[e >> 1]);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) l_run[r] = l_run[r] * corr[r] + (pr[0][2 * r] + pr[0][2 * r + 1] + pr[1][2 * r] + pr[1][2 * r + 1]);
+        const uint32_t pa[4] = {pack_pair<T>(pr[0][0], pr[0][1]), pack_pair<T>(pr[0][2], pr[0][3]), pack_pair<T>(pr[1][0], pr[1][1]),
+                                pack_pair<T>(pr[1][2], pr[1][3])};
+        if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) { o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1]; }
+        }
+        // values of keys that do not count may hold anything: cleared, so that 0 * value stays 0
+        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int key = key0 + i * 8 + 2 * t4;
+            keep[i] = (key >= from && key < len ? 0x0000ffffu : 0u) | (key + 1 >= from && key + 1 < len ? 0xffff0000u : 0u);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          const uint32_t token = (lmat & 1) * 8 + lrow, c = 2 * j + (lmat >> 1);
+          uint32_t vb[4];
+          ldsm_trans(vbase + (c >> 3) * (kChunk * 128) + token * 128 + (((c & 7) ^ (token & 7)) << 4), vb);
+          if (!whole) { vb[0] &= keep[0]; vb[1] &= keep[1]; vb[2] &= keep[0]; vb[3] &= keep[1]; }
+          mma_pair<T>(o[2 * j], pa, vb[0], vb[1]);
+          mma_pair<T>(o[2 * j + 1], pa, vb[2], vb[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
+      l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
+    }
+  }
+
+  // ---------------- the warps' states in warp order ----------------
+  __syncthreads();                                               // the ring is drained
+  float* s_wm = reinterpret_cast<float*>(smem);                  // [warps][16] maxima, denominators
+  float* s_wl = s_wm + kOwnWarps * 16;
+  float* s_m = s_wl + kOwnWarps * 16;                            // [16] the block's
+  float* s_l = s_m + 16;
+  float* s_o = s_l + 16;                                         // [16][D]
+  float* s_w = s_o + 16 * D;                                     // [16][sources] weights
+  float* s_wo = s_w + 16 * L::kSources;                          // [warps][16][D]
+  if (warp < kOwnWarps) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int h = g + r * 8;
+      if (t4 == 0) { s_wm[warp * 16 + h] = m_run[r]; s_wl[warp * 16 + h] = l_run[r]; }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(s_wo + (warp * 16 + h) * D + i * 8 + 2 * t4) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < heads * (D / 4); i += kOwnThreads) {
+    const int h = i / (D / 4), d = i % (D / 4) * 4;
+    float m = -INFINITY, l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kOwnWarps; ++k) m = fmaxf(m, s_wm[k * 16 + h]);
+#pragma unroll
+    for (int k = 0; k < kOwnWarps; ++k) {
+      const float mk = s_wm[k * 16 + h], wgt = mk > -INFINITY ? ex2(mk - m) : 0.f;
+      l = fmaf(s_wl[k * 16 + h], wgt, l);
+      const float4 x = *reinterpret_cast<const float4*>(s_wo + (k * 16 + h) * D + d);
+      v[0] = fmaf(x.x, wgt, v[0]); v[1] = fmaf(x.y, wgt, v[1]); v[2] = fmaf(x.z, wgt, v[2]); v[3] = fmaf(x.w, wgt, v[3]);
+    }
+    *reinterpret_cast<float4*>(s_o + h * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+    if (d == 0) { s_m[h] = m; s_l[h] = l; }
+  }
+  // ---------------- all pieces: the cluster's own parts, then the common ones ----------------
+  if (p.common) {
+    chain_wait();
+    chain_next();
+  }
+  __syncwarp();
+  if (p.splits > 1) cluster_sync_release(); else __syncthreads();
+  int pieces = 0;
+  if (p.common && prefix > 0 && p.parts.plan->ctas > 0) {        // (a row in a group with a prefix: the plan has its item)
+    const long long units = p.parts.plan->units, ctas = p.parts.plan->ctas, first_unit = p.parts.plan->start[of];
+    const int first = group_start(a, of), rows = group_start(a, of + 1) - first, row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+    const int tiles = (prefix + kKeys - 1) / kKeys;
+    const long long unit = first_unit + (static_cast<long long>(kvh) * row_tiles + (row - first) / p.tile_rows) * tiles;
+    pieces = static_cast<int>(((unit + tiles) * ctas - 1) / units - ((unit + 1) * ctas - 1) / units) + 1;
+  }
+  const size_t at0 = static_cast<size_t>(row) * a.heads + head0, step = static_cast<size_t>(a.batch) * a.heads;
+  const int sources = p.splits + pieces;
+  for (int h = warp; h < heads; h += kOwnThreads / 32) {         // a warp per head: the weight of every source
+    float m = -INFINITY, l = 0.f, ms[3], ls[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {                                // (at most 72)
+      const int k = i * 32 + lane;
+      ms[i] = -INFINITY;
+      ls[i] = 0.f;
+      if (k < p.splits) {
+        ms[i] = p.splits > 1 ? ld_rank_f32(s_m + h, k) : s_m[h];
+        ls[i] = p.splits > 1 ? ld_rank_f32(s_l + h, k) : s_l[h];
+      } else if (k < sources) {
+        const float2 x = *reinterpret_cast<const float2*>(p.parts.ml + 2 * ((k - p.splits) * step + at0 + h));
+        ms[i] = x.x;
+        ls[i] = x.y;
+      }
+      m = fmaxf(m, ms[i]);
+    }
+    m = warp_max(m);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      ms[i] = ms[i] > -INFINITY ? ex2(ms[i] - m) : 0.f;
+      l += ls[i] * ms[i];
+    }
+    l = warp_sum(l);
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i * 32 + lane < sources) s_w[h * L::kSources + i * 32 + lane] = ms[i] * inv;
+  }
+  __syncthreads();
+  for (int i = split * kOwnThreads + threadIdx.x; i < heads * (D / 4); i += p.splits * kOwnThreads) {
+    const int h = i / (D / 4), d = i % (D / 4) * 4;
+    const float* wgt = s_w + h * L::kSources;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](const float4& x, float f) {
+      v[0] = fmaf(x.x, f, v[0]); v[1] = fmaf(x.y, f, v[1]); v[2] = fmaf(x.z, f, v[2]); v[3] = fmaf(x.w, f, v[3]);
+    };
+    const float4* acc = reinterpret_cast<const float4*>(p.parts.acc + (at0 + h) * D + d);
+    for (int k = 0; k < p.splits; ++k) add(p.splits > 1 ? ld_rank_f32x4(s_o + h * D + d, k) : *reinterpret_cast<const float4*>(s_o + h * D + d), wgt[k]);
+    int k = 0;
+    for (; k + 4 <= pieces; k += 4) {
+      float4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = acc[(k + j) * step * (D / 4)];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) add(x[j], wgt[p.splits + k + j]);
+    }
+    for (; k < pieces; ++k) add(acc[k * step * (D / 4)], wgt[p.splits + k]);
+    T* out = static_cast<T*>(a.out) + static_cast<size_t>(row) * a.out_stride + static_cast<size_t>(head0 + h) * D + d;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) Elem<T>::st(out + j, v[j]);
+  }
+  if (p.splits > 1) {
+    __syncwarp();
+    cluster_sync_release();                                      // nobody leaves while its part is being read
+  }
+}
+
+template <typename T>
+bool encode_pool(CUtensorMap* map, const void* base, uint64_t rows, int dim) {
+  EncodeTiledFn fn = tensor_map_encoder();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(dim), rows};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(dim) * 2};
+  const cuuint32_t box[2] = {64, kChunk};
+  const cuuint32_t elem_strides[2] = {1, 1};
+  return fn(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
+            strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+int launch_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cudaStream_t stream) {
+  CUtensorMap tk, tv;
+  const uint64_t rows = static_cast<uint64_t>(a.num_slots) * a.kv_heads * a.page_size;
+  if (!encode_pool<T>(&tk, a.k_cache, rows, D) || !encode_pool<T>(&tv, a.v_cache, rows, D)) return CACHEIR_B200_EUNSUPPORTED;
+  const int group = a.heads / a.kv_heads;
+  const float scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  const int tile_rows = 2 * kRows / group;
+  cudaError_t e = cudaSuccess;
+  if (a.groups > 0) {
+    CommonParams c{a, parts, a.groups > kPlanGroups ? 1 : 0, tile_rows, scale_log2};
+    // no more blocks than there can be units
+    const long long tiles = (static_cast<long long>(a.prefix_pages) * a.page_size + kKeys - 1) / kKeys;
+    const long long most = tiles * a.kv_heads * ((a.batch + tile_rows - 1) / tile_rows + a.groups);
+    const int grid = static_cast<int>(most < kNumSMs ? most : kNumSMs);
+    if (c.plan_ready) e = launch_chained(prefix_plan_kernel, dim3(1), dim3(1024), 0, stream, c, grid);
+    auto kern = prefix_common_kernel<T, D>;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CommonSmem<D>::kBytes);
+    if (e == cudaSuccess) e = launch_chained(kern, dim3(grid), dim3(kCommonThreads), CommonSmem<D>::kBytes, stream, tk, tv, c);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  OwnParams o{a, parts, a.groups > 0 ? 1 : 0, tile_rows, (group + 15) / 16, 1, scale_log2};
+  // Parts of a row's own keys: while they find room on the GPU (two blocks on an SM), but no more than there are chunks to share.
+  const long long blocks = static_cast<long long>(a.batch) * a.kv_heads * o.head_chunks;
+  const long long chunks = static_cast<long long>(a.max_pages) * a.page_size / kChunk;
+  while (o.splits < kMaxOwnSplits && 2 * o.splits * blocks <= 2 * kNumSMs && 2 * o.splits * kOwnWarps <= chunks) o.splits *= 2;
+  auto kern = prefix_own_kernel<T, D>;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, OwnSmem<D>::kBytes);
+  if (e == cudaSuccess)
+    e = launch_clusters(kern, dim3(o.splits, a.kv_heads * o.head_chunks, a.batch), dim3(kOwnThreads), OwnSmem<D>::kBytes, stream, dim3(o.splits), tk, tv, o);
+  return e != cudaSuccess ? static_cast<int>(e) : launch_status();
+}
+
+}  // namespace
+
+bool prefix_fast_supported(const cacheir_b200_prefix_args& a) {
+  const int group = a.heads / a.kv_heads;
+  return (a.dtype == CACHEIR_B200_F16 || a.dtype == CACHEIR_B200_BF16) && (a.dim == 64 || a.dim == 128) && a.page_size % kChunk == 0 &&
+         group <= kMaxHeadsPerKv && aligned_to(a.q, 16) && a.q_stride % 8 == 0 && aligned_to(a.k_cache, 16) && aligned_to(a.v_cache, 16) &&
+         static_cast<long long>(a.num_slots) * a.kv_heads * a.page_size <= 0x7fffffffLL - kChunk &&
+         static_cast<long long>(a.kv_heads) * ((group + 15) / 16) <= 65535;
+}
+
+int launch_prefix_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cudaStream_t stream) {
+  if (a.dtype == CACHEIR_B200_F16) return a.dim == 128 ? launch_fast<__half, 128>(a, parts, stream) : launch_fast<__half, 64>(a, parts, stream);
+  return a.dim == 128 ? launch_fast<__nv_bfloat16, 128>(a, parts, stream) : launch_fast<__nv_bfloat16, 64>(a, parts, stream);
+}
+
+int prefix_device_status(bool reset) { return device_status_word(g_prefix_status, reset); }
+
+}  // namespace cb200

@@ -11,7 +11,6 @@ from __future__ import annotations
 
 import ctypes
 import math
-from contextlib import contextmanager
 from dataclasses import dataclass
 
 import numpy as np
@@ -26,30 +25,43 @@ MAX_SEQUENCES = 16384
 LAYOUTS = {"interleaved": 0, "half": 1}
 
 
-@contextmanager
-def _launch(*tensors: torch.Tensor | None):
-    """The stream to launch on: the current one of the device that all the tensors are on."""
-    _require_cuda(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1:
-        raise ValueError(f"all tensors of a call must be on one device, got {sorted(map(str, devices))}")
-    device = devices.pop()
-    with torch.cuda.device(device):
-        yield torch.cuda.current_stream(device).cuda_stream
+# (As these launch kernels of a few microseconds, what they do on the host is kept to about as many: shapes and strides are taken once, the
+# current device is looked up and only switched where the tensors are on another one.)
+def _launch(what: str, tensors: tuple, *args) -> None:
+    """Calls the entry point `what` with `args` and the current stream of the device that all the tensors are on."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            _require_cuda(*tensors)
+            raise ValueError(f"all tensors of a call must be on one device, got {sorted({str(t.device) for t in tensors if t is not None})}")
+    if index < 0:
+        _require_cuda(*tensors)
+    call = getattr(_lib.load_group("serving"), "cacheir_b200_" + what)
+    if index == torch.cuda.current_device():
+        code = call(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            code = call(*args, torch.cuda.current_stream(index).cuda_stream)
+    if code:
+        check(code, what)
 
 
 def _check_ints(what: str, *tensors: torch.Tensor | None) -> None:
     for t in tensors:
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous()):
             raise TypeError(f"{what} must be contiguous int32 tensors")
 
 
-def _check_heads(name: str, t: torch.Tensor, rows: int | None = None) -> None:
-    if t.dim() != 3 or min(t.shape[1:]) < 1 or (t.stride(2) != 1 and t.shape[2] > 1) or (t.stride(1) != t.shape[2] and t.shape[1] > 1) or \
-            (rows is not None and t.shape[0] != rows):
-        raise ValueError(f"{name} must be [rows, heads, dim] with dense heads: only the row stride may differ from heads * dim")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1] * t.shape[2]:
-        raise ValueError(f"{name}: rows must not overlap")
+def _check_heads(name: str, t: torch.Tensor) -> tuple[int, int, int, int]:
+    """(rows, heads, head size, row stride)"""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 3:
+        rows, heads, dim = shape
+        if heads > 0 and dim > 0 and (stride[2] == 1 or dim == 1) and (stride[1] == dim or heads == 1):
+            if rows > 1 and stride[0] < heads * dim:
+                raise ValueError(f"{name}: rows must not overlap")
+            return rows, heads, dim, stride[0]
+    raise ValueError(f"{name} must be [rows, heads, dim] with dense heads: only the row stride may differ from heads * dim")
 
 
 # ---- page tables -----------------------------------------------------------------------------------------------------
@@ -75,22 +87,23 @@ def token_map(rows: int, sequences: int, device: torch.device | str) -> TokenMap
 
 
 def _check_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, change: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
-                  status: torch.Tensor, page_size: int) -> int:
+                  status: torch.Tensor, page_size: int) -> tuple[int, int]:
     _check_ints("page tables, lengths, free pages and status", page_table, seq_lens, change, free_pages, free_count, status)
-    if page_table.dim() != 2 or page_table.shape[1] < 1:
+    shape = page_table.shape
+    if len(shape) != 2 or shape[1] < 1:
         raise ValueError("page_table must be [sequences, max_pages]")
-    sequences = int(page_table.shape[0])
-    if tuple(seq_lens.shape) != (sequences,) or tuple(change.shape) != (sequences,):
+    sequences, max_pages = shape
+    if seq_lens.numel() != sequences or change.numel() != sequences:
         raise ValueError("lengths must be [sequences]")
     if not 1 <= sequences <= MAX_SEQUENCES:
         raise ValueError(f"a call takes 1 to {MAX_SEQUENCES} sequences")
-    if free_pages.dim() != 1 or free_pages.numel() < 1 or free_count.numel() != 1 or status.numel() != 1:
+    if free_pages.numel() < 1 or free_count.numel() != 1 or status.numel() != 1:
         raise ValueError("free_pages must be a stack [capacity], free_count and status one number each")
-    if int(page_size) < 1:
+    if page_size < 1:
         raise ValueError("page_size must be positive")
     if change.data_ptr() == seq_lens.data_ptr():
         raise ValueError("the lengths that a call changes cannot also be its other lengths")
-    return sequences
+    return sequences, max_pages
 
 
 def extend_page_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor,
@@ -102,17 +115,15 @@ def extend_page_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, new_len
     Nothing changes (and `tokens` has no rows, every slot -1) where the call cannot be done; tokens.status then holds, until the caller sets
     it to 0, the number of missing pages, -1 (more tokens than rows), -2 (a sequence longer than its table) or -3 (free_count outside the
     stack). Beside `kv_cache.B200PagedKVCache.extend`, which walks the same pages on the host."""
-    sequences = _check_tables(page_table, seq_lens, new_lens, free_pages, free_count, tokens.status, page_size)
-    _check_ints("token map", tokens.positions, tokens.row_seq, tokens.slots, tokens.cu_rows)
-    rows = tokens.positions.numel()
-    if tokens.row_seq.numel() != rows or tokens.slots.numel() != rows or tokens.cu_rows.numel() != sequences + 1:
+    positions, row_seq, slots, cu_rows, status = tokens.positions, tokens.row_seq, tokens.slots, tokens.cu_rows, tokens.status
+    sequences, max_pages = _check_tables(page_table, seq_lens, new_lens, free_pages, free_count, status, page_size)
+    _check_ints("token map", positions, row_seq, slots, cu_rows)
+    rows = positions.numel()
+    if row_seq.numel() != rows or slots.numel() != rows or cu_rows.numel() != sequences + 1:
         raise ValueError("the token map was made for other sizes")
-    with _launch(page_table, seq_lens, new_lens, free_pages, free_count, tokens.positions, tokens.row_seq, tokens.slots, tokens.cu_rows,
-                 tokens.status) as stream:
-        check(_lib.load_group("serving").cacheir_b200_extend_page_tables(
-            page_table.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), sequences,
-            int(page_table.shape[1]), int(page_size), free_pages.numel(), rows, tokens.positions.data_ptr(), tokens.row_seq.data_ptr(),
-            tokens.slots.data_ptr(), tokens.cu_rows.data_ptr(), tokens.status.data_ptr(), stream), "extend_page_tables")
+    _launch("extend_page_tables", (page_table, seq_lens, new_lens, free_pages, free_count, positions, row_seq, slots, cu_rows, status),
+            page_table.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), sequences, max_pages,
+            page_size, free_pages.numel(), rows, positions.data_ptr(), row_seq.data_ptr(), slots.data_ptr(), cu_rows.data_ptr(), status.data_ptr())
     return tokens
 
 
@@ -121,14 +132,14 @@ def shrink_page_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, keep_le
     """Sequence b keeps its first min(keep_lens[b], seq_lens[b]) tokens (0: it ends); the pages behind them return to the stack, the first
     one on top, so that extending again gives them back in their order. page_table keeps its entries. The first held_pages[b] pages of a
     row belong to somebody else (a common prefix) and never return. `status` as in `extend_page_tables` (-2, -3)."""
-    sequences = _check_tables(page_table, seq_lens, keep_lens, free_pages, free_count, status, page_size)
-    _check_ints("held_pages", held_pages)
-    if held_pages is not None and tuple(held_pages.shape) != (sequences,):
-        raise ValueError("held_pages must be [sequences]")
-    with _launch(page_table, seq_lens, keep_lens, free_pages, free_count, status, held_pages) as stream:
-        check(_lib.load_group("serving").cacheir_b200_shrink_page_tables(
+    sequences, max_pages = _check_tables(page_table, seq_lens, keep_lens, free_pages, free_count, status, page_size)
+    if held_pages is not None:
+        _check_ints("held_pages", held_pages)
+        if held_pages.numel() != sequences:
+            raise ValueError("held_pages must be [sequences]")
+    _launch("shrink_page_tables", (page_table, seq_lens, keep_lens, free_pages, free_count, status, held_pages),
             page_table.data_ptr(), seq_lens.data_ptr(), keep_lens.data_ptr(), _ptr(held_pages), free_pages.data_ptr(), free_count.data_ptr(),
-            sequences, int(page_table.shape[1]), int(page_size), free_pages.numel(), status.data_ptr(), stream), "shrink_page_tables")
+            sequences, max_pages, page_size, free_pages.numel(), status.data_ptr())
 
 
 # ---- rotary positions ------------------------------------------------------------------------------------------------
@@ -180,48 +191,59 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, rule
     are left out altogether. Without slots, k_out defaults to in place; with them, to nowhere but the pool.
 
     Beside `ops.rope_append`: both pair layouts, part of a head, scaled frequencies, float32 to bfloat16, far positions exactly."""
-    rows = int(q.shape[0])
-    for name, t in (("q", q), ("k", k), ("v", v), ("q_out", q_out), ("k_out", k_out)):
-        if t is not None:
-            _check_heads(name, t, rows)
-    heads, kv_heads, dim = int(q.shape[1]), int(k.shape[1]), int(q.shape[2])
-    if k.shape[2] != dim or rule.rot > dim or (v is not None and v.shape != k.shape):
-        raise ValueError("q, k and v must share their head size, of which the rule turns no more than all")
-    if rule.turns.dtype != torch.int64 or not rule.turns.is_contiguous() or rule.layout not in LAYOUTS:
+    rows, heads, dim, q_stride = _check_heads("q", q)
+    k_rows, kv_heads, k_dim, k_stride = _check_heads("k", k)
+    turns, layout = rule.turns, LAYOUTS.get(rule.layout)
+    rot = 2 * turns.numel()
+    if k_dim != dim or k_rows != rows or rot > dim:
+        raise ValueError("q and k must share their rows and their head size, of which the rule turns no more than all")
+    if turns.dtype is not torch.int64 or not turns.is_contiguous() or layout is None or rot < 2:
         raise ValueError("the rule must come from rotary_rule")
     _check_ints("positions and slots", positions, slots)
     if positions.numel() != rows or (slots is not None and slots.numel() != rows):
         raise ValueError("positions and slots must have one number per row")
-    pools = (k_cache, v_cache)
+    dtype = q.dtype
+    v_stride = q_out_stride = k_out_stride = num_slots = page_size = 0
     if slots is None:
-        if any(t is not None for t in pools):
+        if k_cache is not None or v_cache is not None:
             raise ValueError("an append to the pools needs slots")
-    elif v is None or any(t is None for t in pools):
-        raise ValueError("slots need v and both pools")
+        if k_out is None:
+            k_out = k
     else:
-        if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[1] != kv_heads or k_cache.shape[3] != dim or k_cache.shape[0] < 1 or k_cache.shape[2] < 1:
+        if v is None or k_cache is None or v_cache is None:
+            raise ValueError("slots need v and both pools")
+        v_rows, v_heads, v_dim, v_stride = _check_heads("v", v)
+        if v_rows != rows or v_heads != kv_heads or v_dim != dim:
+            raise ValueError("k and v must have one shape")
+        shape = k_cache.shape
+        if len(shape) != 4 or v_cache.shape != shape or shape[1] != kv_heads or shape[3] != dim or shape[0] < 1 or shape[2] < 1:
             raise ValueError("the pools must be [slots, KVH, page, D]")
-        if not all(t.is_contiguous() for t in pools):
+        num_slots, _, page_size, _ = shape
+        if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
             raise ValueError("the pools must be contiguous")
-        if k_cache.shape[0] * k_cache.shape[2] > 2 ** 31:
+        if num_slots * page_size > 2 ** 31:
             raise ValueError("slots reach pools of up to 2^31 rows")
-    q_out = q if q_out is None else q_out
-    if k_out is None and slots is None:
-        k_out = k
-    if q_out.shape != q.shape or (k_out is not None and k_out.shape != k.shape):
-        raise ValueError("outputs must have their inputs' shapes")
-    given = [t for t in (q, k, v, q_out, k_out, *pools) if t is not None]
-    if any(t.dtype != q.dtype for t in given):
+        if v.dtype is not dtype or k_cache.dtype is not dtype or v_cache.dtype is not dtype:
+            raise TypeError("q, k, v, the outputs and the pools must have one dtype")
+    if q_out is None:
+        q_out, q_out_stride = q, q_stride
+    else:
+        out_rows, out_heads, out_dim, q_out_stride = _check_heads("q_out", q_out)
+        if out_rows != rows or out_heads != heads or out_dim != dim:
+            raise ValueError("outputs must have their inputs' shapes")
+    if k_out is not None:
+        out_rows, out_heads, out_dim, k_out_stride = _check_heads("k_out", k_out)
+        if out_rows != rows or out_heads != kv_heads or out_dim != dim:
+            raise ValueError("outputs must have their inputs' shapes")
+    if k.dtype is not dtype or q_out.dtype is not dtype or (k_out is not None and k_out.dtype is not dtype):
         raise TypeError("q, k, v, the outputs and the pools must have one dtype")
+    code = dtype_code(dtype)
     if rows == 0:
         return
-    code = dtype_code(q.dtype)
-    with _launch(*given, positions, slots, rule.turns) as stream:
-        a = RotaryArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), _ptr(positions), _ptr(slots),
-                       _ptr(rule.turns), q.stride(0), k.stride(0), 0 if v is None else v.stride(0), q_out.stride(0),
-                       0 if k_out is None else k_out.stride(0), rows, heads, kv_heads, dim, rule.rot, LAYOUTS[rule.layout],
-                       0 if k_cache is None else int(k_cache.shape[0]), 0 if k_cache is None else int(k_cache.shape[2]), code, float(rule.factor))
-        check(_lib.load_group("serving").cacheir_b200_rotary_append(ctypes.byref(a), stream), "rotary_append")
+    args = RotaryArgs(q.data_ptr(), k.data_ptr(), _ptr(v), q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), positions.data_ptr(), _ptr(slots),
+                      turns.data_ptr(), q_stride, k_stride, v_stride, q_out_stride, k_out_stride, rows, heads, kv_heads, dim, rot, layout, num_slots,
+                      page_size, code, rule.factor)
+    _launch("rotary_append", (q, k, q_out, positions, turns, slots, v, k_out, k_cache, v_cache), ctypes.byref(args))
 
 
 # ---- attention over common prefixes ----------------------------------------------------------------------------------
@@ -280,48 +302,51 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     those below its group's prefix through groups.table, the others through page_table (whose entries below the prefix are not read). A row
     of length 0, or below, gives zeros. `workspace`: `shared_prefix_workspace_bytes(B, H, D)` bytes of any type; calls that may overlap
     need one each (default: a fresh one)."""
-    _check_heads("q", q)
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+    batch, heads, dim, q_stride = _check_heads("q", q)
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("expected k_cache/v_cache [slots,KVH,page,D]")
-    batch, heads, dim = (int(n) for n in q.shape)
-    slots, kv_heads, page_size, pool_dim = (int(n) for n in k_cache.shape)
-    if pool_dim != dim or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    slots, kv_heads, page_size, pool_dim = shape
+    dtype = q.dtype
+    if pool_dim != dim or k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         raise ValueError("q and the KV pool must share head_dim and dtype")
-    if kv_heads < 1 or heads % kv_heads or slots < 1:
+    if kv_heads < 1 or heads % kv_heads or slots < 1 or page_size < 1:
         raise ValueError("the query heads must be a multiple of the pool's heads")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("the KV pool must be contiguous")
-    _check_ints("page_table, seq_lens and the groups", page_table, seq_lens, *((groups.rows, groups.table, groups.lens) if groups else ()))
-    if page_table.dim() != 2 or page_table.shape[0] != batch or page_table.shape[1] < 1 or seq_lens.numel() != batch:
+    _check_ints("page_table and seq_lens", page_table, seq_lens)
+    shape = page_table.shape
+    if len(shape) != 2 or shape[0] != batch or shape[1] < 1 or seq_lens.numel() != batch:
         raise ValueError("page_table must be [B, max_pages] and seq_lens [B]")
-    count = 0
+    max_pages, count, prefix_pages = shape[1], 0, 0
+    group_rows = prefix_table = prefix_lens = None
     if groups is not None:
-        count = int(groups.lens.numel())
-        if groups.rows.numel() != count + 1 or groups.table.dim() != 2 or groups.table.shape[0] != count or count < 1 or groups.table.shape[1] < 1:
-            raise ValueError("prefix groups must have rows [G + 1], table [G, prefix pages] and lens [G]")
+        group_rows, prefix_table, prefix_lens = groups.rows, groups.table, groups.lens
+        _check_ints("the prefix groups", group_rows, prefix_table, prefix_lens)
+        count, shape = prefix_lens.numel(), prefix_table.shape
+        if group_rows.numel() != count + 1 or len(shape) != 2 or shape[0] != count or not 1 <= count <= max(1, batch) or shape[1] < 1:
+            raise ValueError("prefix groups must have rows [G + 1], table [G, prefix pages] and lens [G], G no more than the batch's rows")
+        prefix_pages = shape[1]
     if out is None:
-        out = torch.empty((batch, heads, dim), device=q.device, dtype=q.dtype)
-    else:
-        _check_heads("out", out)
-        if out.shape != q.shape or out.dtype != q.dtype:
-            raise ValueError("out must match q's shape and dtype")
-    if batch == 0:
-        return out
+        out = torch.empty((batch, heads, dim), device=q.device, dtype=dtype)
+    out_rows, out_heads, out_dim, out_stride = _check_heads("out", out)
+    if out_rows != batch or out_heads != heads or out_dim != dim or out.dtype is not dtype:
+        raise ValueError("out must match q's shape and dtype")
     scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError("softmax_scale must be positive")
-    code = dtype_code(q.dtype)
+    code = dtype_code(dtype)
+    if batch == 0:
+        return out
     if workspace is None:
         workspace = torch.empty(shared_prefix_workspace_bytes(batch, heads, dim), device=q.device, dtype=torch.uint8)
     elif not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    extra = (groups.rows, groups.table, groups.lens) if groups is not None else (None, None, None)
-    with _launch(q, k_cache, v_cache, page_table, seq_lens, out, workspace, *extra) as stream:
-        a = PrefixArgs(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(page_table), _ptr(seq_lens), _ptr(extra[0]), _ptr(extra[1]),
-                       _ptr(extra[2]), _ptr(workspace), workspace.numel() * workspace.element_size(), q.stride(0), out.stride(0), batch, heads,
-                       kv_heads, dim, page_size, slots, int(page_table.shape[1]), count, 0 if groups is None else int(groups.table.shape[1]), code,
-                       scale)
-        check(_lib.load_group("serving").cacheir_b200_shared_prefix_attention(ctypes.byref(a), stream), "shared_prefix_attention")
+    args = PrefixArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), _ptr(group_rows),
+                      _ptr(prefix_table), _ptr(prefix_lens), workspace.data_ptr(), workspace.nbytes, q_stride, out_stride, batch, heads, kv_heads, dim,
+                      page_size, slots, max_pages, count, prefix_pages, code, scale)
+    _launch("shared_prefix_attention", (q, k_cache, v_cache, page_table, seq_lens, out, workspace, group_rows, prefix_table, prefix_lens),
+            ctypes.byref(args))
     return out
 
 
@@ -342,24 +367,22 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, *, top: in
 
     -inf masks a token out; a row of nothing else has log probabilities -inf and entropy 0. NaN or +inf in a row give NaN. A token below 0
     means none (log probability 0), one of V or more gives NaN."""
-    if logits.dim() != 2 or logits.stride(1) != 1:
-        raise ValueError("logits must be [R, V] with dense rows")
-    rows, vocab = (int(n) for n in logits.shape)
-    if rows > 1 and logits.stride(0) < vocab:
-        raise ValueError("rows of logits must not overlap")
-    if vocab < 1 or not 0 <= int(top) <= min(MAX_TOP, vocab):
+    shape = logits.shape
+    if len(shape) != 2:
+        raise ValueError("logits must be [R, V]")
+    (rows, vocab), (row_stride, stride) = shape, logits.stride()
+    if vocab < 1 or (stride != 1 and vocab > 1) or (rows > 1 and row_stride < vocab):
+        raise ValueError("logits must be [R, V] with dense rows that do not overlap")
+    if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must be 0 to {MAX_TOP} and no more than the vocabulary")
-    if not (temperature > 0.0 and 1e-30 <= temperature <= 1e30):
+    if not 1e-30 <= temperature <= 1e30:
         raise ValueError("temperature must be positive")
-    if tokens is not None and (tokens.dtype != torch.int64 or tokens.numel() != rows or not tokens.is_contiguous()):
+    if tokens is not None and (tokens.dtype is not torch.int64 or tokens.numel() != rows or not tokens.is_contiguous()):
         raise ValueError("tokens must be contiguous int64 [R]")
-    code = dtype_code(logits.dtype)
-    with _launch(logits, tokens) as stream:
-        new = {"device": logits.device}
-        result = TokenLogprobs(None if tokens is None else torch.empty(rows, dtype=torch.float32, **new), torch.empty(rows, dtype=torch.float32, **new),
-                               torch.empty((rows, top), dtype=torch.int64, **new) if top else None,
-                               torch.empty((rows, top), dtype=torch.float32, **new) if top else None)
-        check(_lib.load_group("serving").cacheir_b200_token_logprobs(
-            logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _ptr(tokens), _ptr(result.logprobs), result.entropy.data_ptr(),
-            _ptr(result.top_ids), _ptr(result.top_logprobs), rows, vocab, int(top), float(temperature), code, stream), "token_logprobs")
+    code, device = dtype_code(logits.dtype), logits.device
+    result = TokenLogprobs(None if tokens is None else torch.empty(rows, dtype=torch.float32, device=device), torch.empty(rows, dtype=torch.float32, device=device),
+                           torch.empty((rows, top), dtype=torch.int64, device=device) if top else None,
+                           torch.empty((rows, top), dtype=torch.float32, device=device) if top else None)
+    _launch("token_logprobs", (logits, tokens), logits.data_ptr(), row_stride if rows > 1 else vocab, _ptr(tokens), _ptr(result.logprobs),
+            result.entropy.data_ptr(), _ptr(result.top_ids), _ptr(result.top_logprobs), rows, vocab, top, temperature, code)
     return result

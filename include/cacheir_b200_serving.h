@@ -81,7 +81,8 @@ int cacheir_b200_rotary_append(const cacheir_b200_rotary_args* args, void* strea
  * The results of cacheir_b200_paged_attention_decode_batch (the reference's `paged_attention_decode_batch_kernel`,
  * cacheir/backends/triton_kernels.py:174-217) for batches in which neighbouring sequences open with the same tokens: the keys and values
  * of the common part are read once for a group and multiplied with the queries of all of its rows together.
- *   group_rows int32 [groups + 1], ascending: the rows of group g are group_rows[g] .. group_rows[g + 1] - 1
+ *   group_rows int32 [groups + 1], ascending: the rows of group g are group_rows[g] .. group_rows[g + 1] - 1 (a group may be empty, but there
+ *   are no more groups than rows)
  *   prefix_lens int32 [groups]: common tokens of the group; prefix_table int32 [groups][prefix_pages]: the pages that hold them
  * Row b attends to tokens t < seq_lens[b]; those below its group's prefix are read through prefix_table, the others through
  * page_table[b] (entries of pages that lie wholly in the prefix are not read). A prefix may end inside a page. A prefix longer than
