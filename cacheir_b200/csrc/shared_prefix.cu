@@ -48,8 +48,7 @@ prefix_general_kernel(const cacheir_b200_prefix_args a, const PrefixParts parts,
     base = tile / per_row;
     first = tile % per_row * kTileRows;
     rows = min(kTileRows, group - first);
-    const int g = group_of_row(a, base);
-    key_lo = g < 0 ? 0 : prefix_of_group(a, g);
+    group_of_row(a, base, &key_lo);
     key_hi = min(max(a.seq_lens[base], 0), a.max_pages * a.page_size);
     pages = a.page_table + static_cast<size_t>(base) * a.max_pages;
   }
@@ -152,7 +151,8 @@ __global__ void __launch_bounds__(128)
 prefix_join_kernel(const cacheir_b200_prefix_args a, const PrefixParts parts) {
   chain_enter();
   const int head = blockIdx.x, row = blockIdx.y, half = parts.pieces / 2;
-  const int from = group_of_row(a, row) < 0 ? half : 0;      // no group: no common pieces were written
+  int prefix;
+  const int from = group_of_row(a, row, &prefix) < 0 ? half : 0;      // no group: no common pieces were written
   const size_t at = static_cast<size_t>(row) * a.heads + head, step = static_cast<size_t>(a.batch) * a.heads;
   float m = -INFINITY, l = 0.f;
   for (int s = from; s < parts.pieces; ++s) m = fmaxf(m, parts.ml[(s * step + at) * 2]);

@@ -8,9 +8,9 @@ namespace cb200 {
 
 // What the kernel of the common parts leaves for the one that joins: how its work was cut (see shared_prefix_mma.cu).
 struct PrefixPlan {
-  long long units;            // key tiles of all items
-  long long ctas;             // blocks that share them
-  long long start[1];         // [groups + 1] first unit of every group
+  int units;                  // of all items
+  int ctas;                   // blocks that share them
+  int start[2];               // [groups + 1] first unit of every group
 };
 
 // The scratch: plan, then for every (piece, row, head) a maximum (log2 domain) and a denominator, and the unnormalised output.
@@ -24,11 +24,30 @@ struct PrefixParts {
 // First row of group g, inside the batch whatever the caller's array holds.
 __device__ __forceinline__ int group_start(const cacheir_b200_prefix_args& a, int g) { return min(max(a.group_rows[g], 0), a.batch); }
 
-// The group of a row (group_rows is ascending), -1 outside every group; a whole warp, which looks at 32 starts at a time.
-__device__ __forceinline__ int group_of_row(const cacheir_b200_prefix_args& a, int row) {
+// The group of a row (group_rows is ascending), -1 outside every group, and its common tokens; a whole warp. Up to 32 groups are looked at
+// in one round of loads.
+__device__ __forceinline__ int prefix_of_group(const cacheir_b200_prefix_args& a, int g) {
+  const long long room = static_cast<long long>(a.prefix_pages) * a.page_size;
+  return static_cast<int>(min(static_cast<long long>(max(a.prefix_lens[g], 0)), room));
+}
+__device__ __forceinline__ int group_of_row(const cacheir_b200_prefix_args& a, int row, int* prefix) {
+  *prefix = 0;
   if (a.groups <= 0) return -1;
-  int lo = 0, hi = a.groups + 1;           // the number of starts up to `row` is in lo .. hi
   const int lane = threadIdx.x & 31;
+  if (a.groups <= 32) {
+    bool mine = false;
+    int len = 0;
+    if (lane < a.groups) {
+      mine = a.group_rows[lane] <= row && row < a.group_rows[lane + 1];
+      len = prefix_of_group(a, lane);
+    }
+    const uint32_t found = __ballot_sync(0xffffffffu, mine);
+    if (found == 0) return -1;
+    const int g = 31 - __clz(found);
+    *prefix = __shfl_sync(0xffffffffu, len, g);
+    return g;
+  }
+  int lo = 0, hi = a.groups + 1;           // the number of starts up to `row` is in lo .. hi; 32 of them are looked at at a time
   while (hi > lo) {
     const int step = (hi - lo + 31) / 32, at = lo + lane * step;
     const int below = __popc(__ballot_sync(0xffffffffu, at < hi && a.group_rows[at] <= row));
@@ -37,12 +56,9 @@ __device__ __forceinline__ int group_of_row(const cacheir_b200_prefix_args& a, i
     hi = min(hi, first + step);
     lo = first + 1;
   }
-  return lo == a.groups + 1 ? -1 : lo - 1;
-}
-
-__device__ __forceinline__ int prefix_of_group(const cacheir_b200_prefix_args& a, int g) {
-  const long long room = static_cast<long long>(a.prefix_pages) * a.page_size;
-  return static_cast<int>(min(static_cast<long long>(max(a.prefix_lens[g], 0)), room));
+  if (lo == 0 || lo == a.groups + 1) return -1;
+  *prefix = prefix_of_group(a, lo - 1);
+  return lo - 1;
 }
 
 constexpr int kMaxPieces = 64;
@@ -54,7 +70,7 @@ inline int prefix_pieces(int batch, int heads, int dim) {
   return n < kMinPieces ? kMinPieces : n > kMaxPieces ? kMaxPieces : static_cast<int>(n);
 }
 inline size_t round_up_256(size_t n) { return (n + 255) / 256 * 256; }
-inline size_t prefix_plan_bytes(int batch) { return round_up_256(sizeof(PrefixPlan) + static_cast<size_t>(batch) * sizeof(long long)); }
+inline size_t prefix_plan_bytes(int batch) { return round_up_256(sizeof(PrefixPlan) + static_cast<size_t>(batch) * sizeof(int)); }
 inline size_t prefix_ml_bytes(int batch, int heads, int pieces) { return round_up_256(static_cast<size_t>(pieces) * batch * heads * 2 * 4); }
 
 // Tensor-core kernels (shared_prefix_mma.cu): 16-bit types, head sizes 64 and 128, pages of a multiple of 16 tokens.

@@ -102,38 +102,53 @@ __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float lo, float hi)
 }
 
 // ---- how the common parts are cut ----
-__device__ __forceinline__ long long group_units(const cacheir_b200_prefix_args& a, int tile_rows, int g, long long* tiles) {
-  const int rows = group_start(a, g + 1) - group_start(a, g), keys = rows > 0 ? prefix_of_group(a, g) : 0;
-  *tiles = (keys + kKeys - 1) / kKeys;
-  return rows > 0 ? static_cast<long long>(a.kv_heads) * ((rows + tile_rows - 1) / tile_rows) * *tiles : 0;
+// An item of n key tiles is kItemUnits + n units: what it costs to begin with (queries, the first tile's latency, the output) is about
+// that of so many tiles. The units are dealt out as evenly as whole numbers can be.
+constexpr int kItemUnits = 2;
+
+struct Deal {
+  int share, more;             // every block has `share` units, the first `more` one more
+  __device__ __forceinline__ Deal(int units, int ctas) : share(units / ctas), more(units % ctas) {}
+  __device__ __forceinline__ int begin(int block) const { return block * share + min(block, more); }
+  __device__ __forceinline__ int owner(int unit) const {
+    const int big = more * (share + 1);
+    return unit < big ? unit / (share + 1) : more + (unit - big) / share;
+  }
+};
+
+__device__ __forceinline__ int key_tiles(int keys) { return (keys + kKeys - 1) / kKeys; }
+// Units of group g (the launcher has seen that all of them fit an int), and its key tiles.
+__device__ __forceinline__ int group_units(const cacheir_b200_prefix_args& a, int tile_rows, int g, int* tiles) {
+  const int rows = group_start(a, g + 1) - group_start(a, g);
+  *tiles = key_tiles(prefix_of_group(a, g));
+  return rows > 0 && *tiles > 0 ? a.kv_heads * ((rows + tile_rows - 1) / tile_rows) * (kItemUnits + *tiles) : 0;
 }
-// Blocks that take part: one unit each at least, and no item in more pieces than there is scratch for (`longest` key tiles in
-// units / ctas at a time, cut anywhere: two more than the quotient at most).
-__device__ __forceinline__ long long plan_ctas(long long units, long long longest, int grid, int pieces) {
+// Blocks that take part: no item may be in more pieces than there is scratch for. n tiles touch ceil((n - 1) / share) + 1 blocks at most.
+__device__ __forceinline__ int plan_ctas(int units, int longest, int grid, int pieces) {
   if (units <= 0) return 0;
-  const long long most = units * (pieces - 2) / longest;
-  return max(1LL, min(min(static_cast<long long>(grid), units), most));
+  const int least = max(1, (longest - 1 + pieces - 2) / (pieces - 1));
+  return max(1, min(grid, units / least));
 }
 
 // The plan of more groups than a block lays out by itself.
 __global__ void __launch_bounds__(1024)
 prefix_plan_kernel(const CommonParams p, const int grid) {
   chain_enter();
-  __shared__ long long s_sum[32], s_max[32];
+  __shared__ int s_sum[32], s_max[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long base = 0, longest = 0;
+  int base = 0, longest = 0;
   for (int g0 = 0; g0 < p.a.groups; g0 += 1024) {
     const int g = g0 + threadIdx.x;
-    long long tiles = 0, own = g < p.a.groups ? group_units(p.a, p.tile_rows, g, &tiles) : 0, sum = own;
+    int tiles = 0, own = g < p.a.groups ? group_units(p.a, p.tile_rows, g, &tiles) : 0, sum = own;
     if (own > 0) longest = max(longest, tiles);
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, sum, off);
+      const int up = __shfl_up_sync(0xffffffffu, sum, off);
       if (lane >= off) sum += up;
     }
     if (lane == 31) s_sum[warp] = sum;
     __syncthreads();
-    long long before = 0, all = 0;
+    int before = 0, all = 0;
     for (int w = 0; w < 32; ++w) {
       if (w < warp) before += s_sum[w];
       all += s_sum[w];
@@ -142,8 +157,7 @@ prefix_plan_kernel(const CommonParams p, const int grid) {
     base += all;
     __syncthreads();
   }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, off));
+  longest = __reduce_max_sync(0xffffffffu, longest);
   if (lane == 0) s_max[warp] = longest;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -156,40 +170,42 @@ prefix_plan_kernel(const CommonParams p, const int grid) {
 
 // A block's share of the units, item by item.
 struct Walk {
-  const long long* start;      // of every group
-  long long units, ctas, at, end;
+  const int* start;            // of every group
+  Deal deal;
+  int at, end;
   // the item
   int group, kvh, row0, rows, tile, tiles, prefix, piece;      // key tiles tile .. tile + tiles - 1 of it are this block's
   const int32_t* pages;
 
-  __device__ __forceinline__ void init(const long long* s, long long u, long long c, int block) {
-    start = s;
-    units = u;
-    ctas = c;
-    at = block * u / c;
-    end = (block + 1) * u / c;
+  __device__ __forceinline__ Walk(const int* s, int units, int ctas) : start(s), deal(units, ctas) {
+    at = deal.begin(blockIdx.x);
+    end = deal.begin(blockIdx.x + 1);
   }
   __device__ __forceinline__ bool next(const CommonParams& p) {
-    if (at >= end) return false;
-    int lo = 0, hi = p.a.groups;                               // last group that starts at or before `at` (empty ones start where the next does)
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (start[mid] <= at) lo = mid; else hi = mid;
+    while (at < end) {
+      int lo = 0, hi = p.a.groups;                             // last group that starts at or before `at` (empty ones start where the next does)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= at) lo = mid; else hi = mid;
+      }
+      group = lo;
+      const int first = group_start(p.a, lo), count = group_start(p.a, lo + 1) - first;
+      prefix = prefix_of_group(p.a, lo);
+      const int all = kItemUnits + key_tiles(prefix), row_tiles = (count + p.tile_rows - 1) / p.tile_rows;
+      const int rel = at - start[lo], item = rel / all, item0 = start[lo] + item * all, tile0 = item0 + kItemUnits;
+      const int stop = min(end, item0 + all);
+      tile = max(at - tile0, 0);
+      tiles = stop - tile0 - tile;
+      at = stop;
+      if (tiles <= 0) continue;                                // (no more than an item's beginning: the next block has its tiles)
+      kvh = item / row_tiles;
+      row0 = first + (item - kvh * row_tiles) * p.tile_rows;
+      rows = min(p.tile_rows, first + count - row0);
+      piece = blockIdx.x - deal.owner(tile0);
+      pages = p.a.prefix_table + static_cast<size_t>(lo) * p.a.prefix_pages;
+      return true;
     }
-    group = lo;
-    const int first = group_start(p.a, lo), count = group_start(p.a, lo + 1) - first;
-    prefix = prefix_of_group(p.a, lo);
-    pages = p.a.prefix_table + static_cast<size_t>(lo) * p.a.prefix_pages;
-    const int all = (prefix + kKeys - 1) / kKeys, row_tiles = (count + p.tile_rows - 1) / p.tile_rows;
-    const long long rel = at - start[lo], item = rel / all;
-    kvh = static_cast<int>(item / row_tiles);
-    row0 = first + static_cast<int>(item % row_tiles) * p.tile_rows;
-    rows = min(p.tile_rows, first + count - row0);
-    tile = static_cast<int>(rel - item * all);
-    tiles = static_cast<int>(min(static_cast<long long>(all - tile), end - at));
-    piece = static_cast<int>(blockIdx.x - ((start[lo] + item * all + 1) * ctas - 1) / units);
-    at += tiles;
-    return true;
+    return false;
   }
 };
 
@@ -201,7 +217,7 @@ struct CommonSmem {
   static constexpr int kTiles = 2 * kQBytes + kSlots * kSlotBytes;
   // then: barriers full, empty [slots], q[2], s[2], p[2], o[2]; tensor memory address; group starts
   static constexpr int kBarriers = 2 * kSlots + 8;
-  static constexpr int kBytes = 1024 + kTiles + kBarriers * 8 + 16 + (kPlanGroups + 1) * 8;
+  static constexpr int kBytes = 1024 + kTiles + kBarriers * 8 + 16 + (kPlanGroups + 1) * 4;
 };
 
 template <typename T, int D>
@@ -221,32 +237,30 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   uint64_t* bar_p = bar_s + 2;                                 // probabilities are
   uint64_t* bar_o = bar_p + 2;                                 // .. and have been added to the output
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_o + 2);
-  long long* s_start = reinterpret_cast<long long*>(tmem_slot + 4);
-  __shared__ long long s_plan[2];
-  __shared__ long long s_scan[4], s_longest[4];
+  int* s_start = reinterpret_cast<int*>(tmem_slot + 4);
+  __shared__ int s_plan[2], s_scan[4], s_longest[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const cacheir_b200_prefix_args& a = p.a;
 
   // ---- the plan ----
   if (!p.plan_ready) {
-    long long own = 0, sum = 0;
+    int own = 0, sum = 0;
     if (warp < kPlanGroups / 32) {
-      long long tiles = 0;
+      int tiles = 0;
       const int g = threadIdx.x;
       own = g < a.groups ? group_units(a, p.tile_rows, g, &tiles) : 0;
-      long long longest = own > 0 ? tiles : 0;
+      const int longest = __reduce_max_sync(0xffffffffu, own > 0 ? tiles : 0);
       sum = own;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, sum, off);
+        const int up = __shfl_up_sync(0xffffffffu, sum, off);
         if (lane >= off) sum += up;
-        longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, off));
       }
       if (lane == 31) { s_scan[warp] = sum; s_longest[warp] = longest; }
     }
     __syncthreads();
     if (warp < kPlanGroups / 32) {
-      long long before = 0, all = 0, longest = 0;
+      int before = 0, all = 0, longest = 0;
 #pragma unroll
       for (int w = 0; w < kPlanGroups / 32; ++w) {
         if (w < warp) before += s_scan[w];
@@ -275,8 +289,8 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     mbar_fence_init();
   }
   __syncthreads();
-  const long long* start = p.plan_ready ? p.parts.plan->start : s_start;
-  const long long units = p.plan_ready ? p.parts.plan->units : s_plan[0], ctas = p.plan_ready ? p.parts.plan->ctas : s_plan[1];
+  const int* start = p.plan_ready ? p.parts.plan->start : s_start;
+  const int units = p.plan_ready ? p.parts.plan->units : s_plan[0], ctas = p.plan_ready ? p.parts.plan->ctas : s_plan[1];
   if (!p.plan_ready && blockIdx.x == 0) {                      // for the kernel that joins
     for (int g = threadIdx.x; g <= a.groups; g += kCommonThreads) p.parts.plan->start[g] = s_start[g];
     if (threadIdx.x == 0) {
@@ -284,7 +298,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       p.parts.plan->ctas = ctas;
     }
   }
-  if (static_cast<long long>(blockIdx.x) >= ctas) return;
+  if (static_cast<int>(blockIdx.x) >= ctas) return;
   if (warp == 8) tc_alloc(smem_u32(tmem_slot), 512);
   tc_fence_before();
   __syncthreads();
@@ -292,8 +306,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   const uint32_t tmem = *tmem_slot;                            // scores [2][128 columns] (probabilities over them), outputs [2][D]
   const uint32_t tmem_o = tmem + 2 * kKeys;
   const int group = a.heads / a.kv_heads;
-  Walk walk;
-  walk.init(start, units, ctas, blockIdx.x);
+  Walk walk(start, units, ctas);
   bool ok = true;
 
   if (warp == 9) {
@@ -343,6 +356,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     // Scores and outputs step through the same (tile, buffer) sequence, scores up to two steps ahead.
     struct Steps {
       Walk walk;
+      __device__ __forceinline__ explicit Steps(const Walk& w) : walk(w) {}
       int left = 0, two = 0, second = 0, tile = 0, first = 0;  // key tiles left in the item, two steps per tile?, the second of them?, tiles so far
       __device__ __forceinline__ bool ready(const CommonParams& p, int group) {
         if (left > 0) return true;
@@ -359,9 +373,8 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         ++tile;
         return true;
       }
-    } score, output;
-    score.walk = walk;
-    output.walk = walk;
+    };
+    Steps score(walk), output(walk);
     int next_s = 0, next_o = 0;
     uint32_t q_seen[2] = {0, 0};
     while (ok) {
@@ -409,6 +422,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     // ---------------- softmax: a thread per query row ----------------
     const int w = warp >> 2, r = threadIdx.x & (kRows - 1);
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int by_group = (65536 + group - 1) / group;          // n / group = n * by_group >> 16 for n < 256, group <= 64
     int step = 0, tile = 0;                                    // of the block so far
     while (ok && walk.next(p)) {
       const int used = walk.rows * group, two = used > kRows ? 1 : 0, steps = walk.tiles * (two ? 2 : 1);
@@ -420,20 +434,23 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       }
       // queries: rows of this group of warps, zeros behind the last one
       const int q_row0 = w * kRows;
-      for (int i = r; i < kRows * (D / 8); i += kRows) {
-        const int row = i / (D / 8), c = i % (D / 8), at = q_row0 + row;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (at < used)
-          v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + static_cast<size_t>(walk.row0 + at / group) * a.q_stride +
-                                              static_cast<size_t>(walk.kvh * group + at % group) * D + c * 8);
-        *reinterpret_cast<uint4*>(s_q + w * L::kQBytes + (c >> 3) * kRows * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+#pragma unroll 4
+      for (int i = r; i < kRows * (D / 8); i += kRows) {       // (all of them on their way at once)
+        const int row = i / (D / 8), c = i % (D / 8), at = q_row0 + row, b_row = at * by_group >> 16;
+        const T* src = static_cast<const T*>(a.q);
+        if (at < used) src += static_cast<size_t>(walk.row0 + b_row) * a.q_stride + static_cast<size_t>(walk.kvh * group + at - b_row * group) * D + c * 8;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                     ::"r"(smem_u32(s_q + w * L::kQBytes + (c >> 3) * kRows * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4))), "l"(src),
+                       "r"(at < used ? 16 : 0) : "memory");
       }
-      fence_async_smem();
-      mbar_arrive(smem_u32(&bar_q[w]));
       const int mine = q_row0 + r;
       const bool real = mine < used;
-      const int b_row = walk.row0 + (real ? mine / group : 0), head = walk.kvh * group + (real ? mine % group : 0);
+      const int in_tile = real ? mine * by_group >> 16 : 0;
+      const int b_row = walk.row0 + in_tile, head = walk.kvh * group + (real ? mine - in_tile * group : 0);
       const int limit = real ? min(walk.prefix, a.seq_lens[b_row]) : walk.prefix;      // keys that the row sees
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_async_smem();
+      mbar_arrive(smem_u32(&bar_q[w]));
       float m_ref = -INFINITY, l_run = 0.f;
       int last = 0;
       for (int t = 0, s = two ? step + ((step ^ w) & 1) : step; t < walk.tiles && ok; ++t, s += two ? 2 : 1) {
@@ -538,11 +555,11 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Every row's own keys, and the pieces joined. One block per (part of the row's own keys, key/value head and up to 16 of its query heads, row);
-// the parts are a thread-block cluster. Keys and values come 16 tokens at a time (TMA) through a ring, four warps take one chunk of a
-// stage each with warp MMAs, the query heads as their 16 rows: bound by the memory's rate. None of that needs the common part's kernel:
-// this one starts as soon as that one's blocks leave room, and waits for it before it joins.
-constexpr int kOwnWarps = 4;
-constexpr int kOwnThreads = (kOwnWarps + 1) * 32;
+// the parts are a thread-block cluster. Keys and values come 16 tokens at a time (TMA): every warp takes every WARPS-th chunk of the part
+// through a ring of its own, with warp MMAs that have the query heads as their 16 rows. Bound by the memory's rate where there are many
+// rows: then blocks of two warps, four of them on an SM, so that while some begin or join others keep the memory busy; where there are
+// few, blocks of eight. None of that needs the common part's kernel: this one starts as soon as that one's blocks leave room, and waits for
+// it before it joins.
 constexpr int kOwnStages = 3;
 constexpr int kMaxOwnSplits = 8;
 
@@ -554,15 +571,14 @@ struct OwnParams {
   float scale_log2;
 };
 
-template <int D>
+template <int D, int WARPS>
 struct OwnSmem {
   static constexpr int kTileBytes = kChunk * D * 2;
-  static constexpr int kStageBytes = kOwnWarps * 2 * kTileBytes;
+  static constexpr int kRing = WARPS * kOwnStages * 2 * kTileBytes;
   // over the ring afterwards: the warps' states, the block's, and the weights of all sources of a head
   static constexpr int kSources = kMaxPieces + kMaxOwnSplits;
-  static constexpr int kJoin = (kOwnWarps * 16 * (D + 2) + 16 * (D + 2) + 16 * kSources) * 4;
-  static constexpr int kRing = kOwnStages * kStageBytes;
-  static constexpr int kBytes = 1024 + (kRing > kJoin ? kRing : kJoin) + 2 * kOwnStages * 8;
+  static constexpr int kJoin = (WARPS * 16 * (D + 2) + 16 * (D + 2) + 16 * kSources) * 4;
+  static constexpr int kBytes = 1024 + (kRing > kJoin ? kRing : kJoin) + WARPS * kOwnStages * 8;
 };
 
 __device__ __forceinline__ void ldsm_trans(uint32_t addr, uint32_t (&r)[4]) {
@@ -589,24 +605,44 @@ __device__ __forceinline__ float4 ld_rank_f32x4(const float* local, uint32_t ran
   return v;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kOwnThreads)
+template <typename T, int D, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32)
 prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ OwnParams p) {
-  using L = OwnSmem<D>;
-  constexpr int kBoxes = D / 64;
+  using L = OwnSmem<D, WARPS>;
+  constexpr int kBoxes = D / 64, kThreads = WARPS * 32;
   // What stands before this wait reads what was there before the common part's kernel began: its blocks let this one in only after they
   // had waited for all earlier ones.
   if (!p.common) chain_enter();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw + L::kBytes - 2 * kOwnStages * 8);
-  uint64_t* empty = full + kOwnStages;
   const cacheir_b200_prefix_args& a = p.a;
   const int split = blockIdx.x, kvh = blockIdx.y / p.head_chunks, row = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.heads / a.kv_heads, head0 = kvh * group + blockIdx.y % p.head_chunks * 16, heads = min(16, (kvh + 1) * group - head0);
+  const uint32_t bars = smem_u32(smem_raw + L::kBytes - WARPS * kOwnStages * 8) + warp * kOwnStages * 8;
+  const uint32_t ring = smem_u32(smem) + warp * kOwnStages * 2 * L::kTileBytes;
   const int g = lane >> 2, t4 = lane & 3;
-  uint32_t qa[D / 16][4];                                       // queries as the A operand: rows = heads
-  if (warp < kOwnWarps) {
+  if (lane == 0) {
+    for (int s = 0; s < kOwnStages; ++s) mbar_init(bars + s * 8, 1);
+    mbar_fence_init();
+  }
+  // Lengths, group, first page ids and queries are asked for together as far as they can be.
+  const int len = min(max(a.seq_lens[row], 0), a.max_pages * a.page_size);
+  int prefix;
+  const int of = group_of_row(a, row, &prefix);
+  const int from = min(prefix, len);
+  const int chunk0 = from / kChunk, chunks = len > from ? (len + kChunk - 1) / kChunk - chunk0 : 0, per = (chunks + p.splits - 1) / p.splits;
+  const int begin = chunk0 + min(chunks, split * per), end = chunk0 + min(chunks, (split + 1) * per);
+  const int32_t* pages = a.page_table + static_cast<size_t>(row) * a.max_pages;
+  const int outside = a.num_slots * a.kv_heads * a.page_size;   // rows behind the pool read as zeros
+  const int mine = begin + warp < end ? (end - begin - warp + WARPS - 1) / WARPS : 0;          // chunks begin + warp + i * WARPS
+  auto line_of = [&](int i) {                                    // first row of this warp's i-th chunk in the pool
+    if (i >= mine) return outside;
+    const int key = (begin + warp + i * WARPS) * kChunk, id = pages[key / a.page_size];
+    return id >= 0 && id < a.num_slots ? (id * a.kv_heads + kvh) * a.page_size + key % a.page_size : outside;
+  };
+  int lines = line_of(lane), lines_next = mine > 32 ? line_of(32 + lane) : outside;            // of chunks 32 k + lane, k rising
+  uint32_t qa[D / 16][4];                                        // queries as the A operand: rows = heads
+  {
     const T* q = static_cast<const T*>(a.q) + static_cast<size_t>(row) * a.q_stride + static_cast<size_t>(head0) * D;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k)
@@ -616,170 +652,145 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         qa[k][i] = h < heads ? *reinterpret_cast<const uint32_t*>(q + static_cast<size_t>(h) * D + col) : 0u;
       }
   }
-  const int len = min(max(a.seq_lens[row], 0), a.max_pages * a.page_size);
-  const int of = group_of_row(a, row);
-  const int prefix = of < 0 ? 0 : prefix_of_group(a, of);
-  const int from = min(prefix, len);
-  const int chunk0 = from / kChunk, chunks = len > from ? (len + kChunk - 1) / kChunk - chunk0 : 0, per = (chunks + p.splits - 1) / p.splits;
-  const int begin = chunk0 + min(chunks, split * per), count = min(chunks, (split + 1) * per) - min(chunks, split * per);
-  const int iters = (count + kOwnWarps - 1) / kOwnWarps;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kOwnStages; ++s) {
-      mbar_init(smem_u32(&full[s]), 1);
-      mbar_init(smem_u32(&empty[s]), kOwnWarps);
-    }
-    mbar_fence_init();
-  }
-  __syncthreads();
+  __syncwarp();
+  auto copy = [&](int i, int s) {                                // chunk i into stage s: a lane per 64 columns of keys and of values
+    const int line = __shfl_sync(0xffffffffu, lines, i & 31);
+    if (lane == 0) mbar_expect_tx(bars + s * 8, 2 * L::kTileBytes);
+    __syncwarp();
+    if (lane < 2 * kBoxes)
+      tma_load_2d(ring + s * 2 * L::kTileBytes + (lane / kBoxes) * L::kTileBytes + (lane % kBoxes) * kChunk * 128, lane < kBoxes ? &tmap_k : &tmap_v,
+                  bars + s * 8, (lane % kBoxes) * 64, line);
+  };
+  for (int s = 0; s < kOwnStages; ++s)
+    if (s < mine) copy(s, s);
 
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f}, o[D / 8][4];
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  const uint32_t lrow = lane & 7, lmat = lane >> 3;
+  int stage = 0;
+  uint32_t phase = 0;
   bool ok = true;
-  if (warp == kOwnWarps) {
-    // ---------------- copies: a lane per chunk and 64 columns of the keys, the same of the values ----------------
-    const int32_t* pages = a.page_table + static_cast<size_t>(row) * a.max_pages;
-    const int outside = a.num_slots * a.kv_heads * a.page_size;
-    const int c = lane / kBoxes, box = lane % kBoxes;
-    auto line_of = [&](int it) {
-      const int at = it * kOwnWarps + c;
-      if (c >= kOwnWarps || at >= count) return outside;
-      const int key = (begin + at) * kChunk, id = pages[key / a.page_size];
-      return id >= 0 && id < a.num_slots ? (id * a.kv_heads + kvh) * a.page_size + key % a.page_size : outside;
-    };
-    int line = line_of(0);
-    for (int it = 0; it < iters && ok; ++it) {
-      const int s = it % kOwnStages, now = min(kOwnWarps, count - it * kOwnWarps);
-      const int next = line_of(it + 1);
-      ok = mbar_wait(smem_u32(&empty[s]), ((it / kOwnStages) & 1) ^ 1, &g_prefix_status, (15 << 8) | 12);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (lane == 0) mbar_expect_tx(smem_u32(&full[s]), now * 2 * L::kTileBytes);
-      __syncwarp();
-      if (c < now) {
-        const uint32_t dst = smem_u32(smem + s * L::kStageBytes + c * 2 * L::kTileBytes + box * kChunk * 128);
-        tma_load_2d(dst, &tmap_k, smem_u32(&full[s]), box * 64, line);
-        tma_load_2d(dst + L::kTileBytes, &tmap_v, smem_u32(&full[s]), box * 64, line);
+#pragma unroll 1
+  for (int it = 0; it < mine; ++it) {
+    ok = __all_sync(0xffffffffu, mbar_wait(bars + stage * 8, phase, &g_prefix_status, (15 << 8) | 12));
+    if (!ok) {                                                   // the copies that are still under way are waited for
+      for (int i = it + 1; i < min(mine, it + kOwnStages); ++i) {
+        if (++stage == kOwnStages) { stage = 0; phase ^= 1; }
+        mbar_wait(bars + stage * 8, phase, &g_prefix_status, (15 << 8) | 13);
       }
-      line = next;
+      break;
     }
-    if (!ok)                                                    // nothing may still be on its way when the ring is used for something else
-      for (int s = 0; s < kOwnStages; ++s) {
-        mbar_wait(smem_u32(&full[s]), 0, &g_prefix_status, (15 << 8) | 13);
-        mbar_wait(smem_u32(&full[s]), 1, &g_prefix_status, (15 << 8) | 13);
+    const uint32_t kbase = ring + stage * 2 * L::kTileBytes, vbase = kbase + L::kTileBytes;
+    float sc[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+      const uint32_t token = n * 8 + lrow;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {
+        const uint32_t c = 4 * k + lmat;
+        uint32_t kb[4];
+        ldsm_x4(kbase + (c >> 3) * (kChunk * 128) + token * 128 + (((c & 7) ^ (token & 7)) << 4), kb);
+        mma_pair<T>(sc[n], qa[2 * k], kb[0], kb[1]);
+        mma_pair<T>(sc[n], qa[2 * k + 1], kb[2], kb[3]);
       }
-  } else {
-    const uint32_t lrow = lane & 7, lmat = lane >> 3;
-    for (int it = 0; it < iters && ok; ++it) {
-      const int s = it % kOwnStages, mine = it * kOwnWarps + warp;
-      ok = mbar_wait(smem_u32(&full[s]), (it / kOwnStages) & 1, &g_prefix_status, (15 << 8) | 14);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (mine < count) {
-        const uint32_t kbase = smem_u32(smem + s * L::kStageBytes + warp * 2 * L::kTileBytes), vbase = kbase + L::kTileBytes;
-        float sc[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-          const uint32_t token = n * 8 + lrow;
-#pragma unroll
-          for (int k = 0; k < D / 32; ++k) {
-            const uint32_t c = 4 * k + lmat;
-            uint32_t kb[4];
-            ldsm_x4(kbase + (c >> 3) * (kChunk * 128) + token * 128 + (((c & 7) ^ (token & 7)) << 4), kb);
-            mma_pair<T>(sc[n], qa[2 * k], kb[0], kb[1]);
-            mma_pair<T>(sc[n], qa[2 * k + 1], kb[2], kb[3]);
-          }
-        }
-        const int key0 = (begin + mine) * kChunk;
-        const bool whole = key0 >= from && key0 + kChunk <= len;
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = key0 + n * 8 + 2 * t4 + (e & 1);
-            const float v = whole || (key >= from && key < len) ? sc[n][e] * p.scale_log2 : -INFINITY;
-            sc[n][e] = v;
-            top[e >> 1] = fmaxf(top[e >> 1], v);
-          }
-        float corr[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-          const float m_new = fmaxf(m_run[r], top[r]);           // finite: every chunk has a key that counts
-          corr[r] = ex2(m_run[r] - m_new);
-          m_run[r] = m_new;
-        }
-        float pr[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) pr[n][e] = ex2(sc[n][e] - m_run[e >> 1]);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) l_run[r] = l_run[r] * corr[r] + (pr[0][2 * r] + pr[0][2 * r + 1] + pr[1][2 * r] + pr[1][2 * r + 1]);
-        const uint32_t pa[4] = {pack_pair<T>(pr[0][0], pr[0][1]), pack_pair<T>(pr[0][2], pr[0][3]), pack_pair<T>(pr[1][0], pr[1][1]),
-                                pack_pair<T>(pr[1][2], pr[1][3])};
-        if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) { o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1]; }
-        }
-        // values of keys that do not count may hold anything: cleared, so that 0 * value stays 0
-        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-        if (!whole) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int key = key0 + i * 8 + 2 * t4;
-            keep[i] = (key >= from && key < len ? 0x0000ffffu : 0u) | (key + 1 >= from && key + 1 < len ? 0xffff0000u : 0u);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-          const uint32_t token = (lmat & 1) * 8 + lrow, c = 2 * j + (lmat >> 1);
-          uint32_t vb[4];
-          ldsm_trans(vbase + (c >> 3) * (kChunk * 128) + token * 128 + (((c & 7) ^ (token & 7)) << 4), vb);
-          if (!whole) { vb[0] &= keep[0]; vb[1] &= keep[1]; vb[2] &= keep[0]; vb[3] &= keep[1]; }
-          mma_pair<T>(o[2 * j], pa, vb[0], vb[1]);
-          mma_pair<T>(o[2 * j + 1], pa, vb[2], vb[3]);
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
     }
+    const int key0 = (begin + warp + it * WARPS) * kChunk;
+    const bool whole = key0 >= from && key0 + kChunk <= len;
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = key0 + n * 8 + 2 * t4 + (e & 1);
+        const float v = whole || (key >= from && key < len) ? sc[n][e] * p.scale_log2 : -INFINITY;
+        sc[n][e] = v;
+        top[e >> 1] = fmaxf(top[e >> 1], v);
+      }
+    float corr[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
-      l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+      const float m_new = fmaxf(m_run[r], top[r]);               // finite: every chunk has a key that counts
+      corr[r] = ex2(m_run[r] - m_new);
+      m_run[r] = m_new;
     }
+    float pr[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pr[n][e] = ex2(sc[n][e] - m_run[e >> 1]);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) l_run[r] = l_run[r] * corr[r] + (pr[0][2 * r] + pr[0][2 * r + 1] + pr[1][2 * r] + pr[1][2 * r + 1]);
+    const uint32_t pa[4] = {pack_pair<T>(pr[0][0], pr[0][1]), pack_pair<T>(pr[0][2], pr[0][3]), pack_pair<T>(pr[1][0], pr[1][1]),
+                            pack_pair<T>(pr[1][2], pr[1][3])};
+    if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) { o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1]; }
+    }
+    // values of keys that do not count may hold anything: cleared, so that 0 * value stays 0
+    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = key0 + i * 8 + 2 * t4;
+        keep[i] = (key >= from && key < len ? 0x0000ffffu : 0u) | (key + 1 >= from && key + 1 < len ? 0xffff0000u : 0u);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      const uint32_t token = (lmat & 1) * 8 + lrow, c = 2 * j + (lmat >> 1);
+      uint32_t vb[4];
+      ldsm_trans(vbase + (c >> 3) * (kChunk * 128) + token * 128 + (((c & 7) ^ (token & 7)) << 4), vb);
+      vb[0] &= keep[0]; vb[1] &= keep[1]; vb[2] &= keep[0]; vb[3] &= keep[1];
+      mma_pair<T>(o[2 * j], pa, vb[0], vb[1]);
+      mma_pair<T>(o[2 * j + 1], pa, vb[2], vb[3]);
+    }
+    __syncwarp();                                                // the stage has been read
+    const int ahead = it + kOwnStages;
+    if (ahead < mine) {
+      if ((ahead & 31) == 0) {                                   // (its line and those behind it are the next round's)
+        lines = lines_next;
+        lines_next = line_of(ahead + 32 + lane);
+      }
+      copy(ahead, stage);
+    }
+    if (++stage == kOwnStages) { stage = 0; phase ^= 1; }
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
+    l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
   }
 
   // ---------------- the warps' states in warp order ----------------
-  __syncthreads();                                               // the ring is drained
+  __syncthreads();                                               // the rings are drained
   float* s_wm = reinterpret_cast<float*>(smem);                  // [warps][16] maxima, denominators
-  float* s_wl = s_wm + kOwnWarps * 16;
-  float* s_m = s_wl + kOwnWarps * 16;                            // [16] the block's
+  float* s_wl = s_wm + WARPS * 16;
+  float* s_m = s_wl + WARPS * 16;                                // [16] the block's
   float* s_l = s_m + 16;
   float* s_o = s_l + 16;                                         // [16][D]
   float* s_w = s_o + 16 * D;                                     // [16][sources] weights
   float* s_wo = s_w + 16 * L::kSources;                          // [warps][16][D]
-  if (warp < kOwnWarps) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int h = g + r * 8;
-      if (t4 == 0) { s_wm[warp * 16 + h] = m_run[r]; s_wl[warp * 16 + h] = l_run[r]; }
+  for (int r = 0; r < 2; ++r) {
+    const int h = g + r * 8;
+    if (t4 == 0) { s_wm[warp * 16 + h] = m_run[r]; s_wl[warp * 16 + h] = l_run[r]; }
+    if (h < heads) {
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(s_wo + (warp * 16 + h) * D + i * 8 + 2 * t4) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < heads * (D / 4); i += kOwnThreads) {
+  for (int i = threadIdx.x; i < heads * (D / 4); i += kThreads) {
     const int h = i / (D / 4), d = i % (D / 4) * 4;
     float m = -INFINITY, l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < kOwnWarps; ++k) m = fmaxf(m, s_wm[k * 16 + h]);
+    for (int k = 0; k < WARPS; ++k) m = fmaxf(m, s_wm[k * 16 + h]);
 #pragma unroll
-    for (int k = 0; k < kOwnWarps; ++k) {
+    for (int k = 0; k < WARPS; ++k) {
       const float mk = s_wm[k * 16 + h], wgt = mk > -INFINITY ? ex2(mk - m) : 0.f;
       l = fmaf(s_wl[k * 16 + h], wgt, l);
       const float4 x = *reinterpret_cast<const float4*>(s_wo + (k * 16 + h) * D + d);
@@ -796,16 +807,16 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   __syncwarp();
   if (p.splits > 1) cluster_sync_release(); else __syncthreads();
   int pieces = 0;
-  if (p.common && prefix > 0 && p.parts.plan->ctas > 0) {        // (a row in a group with a prefix: the plan has its item)
-    const long long units = p.parts.plan->units, ctas = p.parts.plan->ctas, first_unit = p.parts.plan->start[of];
-    const int first = group_start(a, of), rows = group_start(a, of + 1) - first, row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
-    const int tiles = (prefix + kKeys - 1) / kKeys;
-    const long long unit = first_unit + (static_cast<long long>(kvh) * row_tiles + (row - first) / p.tile_rows) * tiles;
-    pieces = static_cast<int>(((unit + tiles) * ctas - 1) / units - ((unit + 1) * ctas - 1) / units) + 1;
+  if (p.common && prefix > 0) {                                  // (then the row is in a group that has items)
+    const int start = p.parts.plan->start[of];
+    const Deal deal(p.parts.plan->units, p.parts.plan->ctas);
+    const int first = group_start(a, of), row_tiles = (group_start(a, of + 1) - first + p.tile_rows - 1) / p.tile_rows;
+    const int all = kItemUnits + key_tiles(prefix), item0 = start + (kvh * row_tiles + (row - first) / p.tile_rows) * all;
+    pieces = deal.owner(item0 + all - 1) - deal.owner(item0 + kItemUnits) + 1;
   }
   const size_t at0 = static_cast<size_t>(row) * a.heads + head0, step = static_cast<size_t>(a.batch) * a.heads;
   const int sources = p.splits + pieces;
-  for (int h = warp; h < heads; h += kOwnThreads / 32) {         // a warp per head: the weight of every source
+  for (int h = warp; h < heads; h += WARPS) {                    // a warp per head: the weight of every source
     float m = -INFINITY, l = 0.f, ms[3], ls[3];
 #pragma unroll
     for (int i = 0; i < 3; ++i) {                                // (at most 72)
@@ -835,7 +846,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       if (i * 32 + lane < sources) s_w[h * L::kSources + i * 32 + lane] = ms[i] * inv;
   }
   __syncthreads();
-  for (int i = split * kOwnThreads + threadIdx.x; i < heads * (D / 4); i += p.splits * kOwnThreads) {
+  for (int i = split * kThreads + threadIdx.x; i < heads * (D / 4); i += p.splits * kThreads) {
     const int h = i / (D / 4), d = i % (D / 4) * 4;
     const float* wgt = s_w + h * L::kSources;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -845,12 +856,12 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
     const float4* acc = reinterpret_cast<const float4*>(p.parts.acc + (at0 + h) * D + d);
     for (int k = 0; k < p.splits; ++k) add(p.splits > 1 ? ld_rank_f32x4(s_o + h * D + d, k) : *reinterpret_cast<const float4*>(s_o + h * D + d), wgt[k]);
     int k = 0;
-    for (; k + 4 <= pieces; k += 4) {
-      float4 x[4];
+    for (; k + 8 <= pieces; k += 8) {
+      float4 x[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = acc[(k + j) * step * (D / 4)];
+      for (int j = 0; j < 8; ++j) x[j] = acc[(k + j) * step * (D / 4)];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) add(x[j], wgt[p.splits + k + j]);
+      for (int j = 0; j < 8; ++j) add(x[j], wgt[p.splits + k + j]);
     }
     for (; k < pieces; ++k) add(acc[k * step * (D / 4)], wgt[p.splits + k]);
     T* out = static_cast<T*>(a.out) + static_cast<size_t>(row) * a.out_stride + static_cast<size_t>(head0 + h) * D + d;
@@ -876,21 +887,35 @@ bool encode_pool(CUtensorMap* map, const void* base, uint64_t rows, int dim) {
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <typename T, int D, int WARPS>
+int launch_own(const OwnParams& o, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t stream) {
+  auto kern = prefix_own_kernel<T, D, WARPS>;
+  constexpr int bytes = OwnSmem<D, WARPS>::kBytes;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess)
+    e = launch_clusters(kern, dim3(o.splits, o.a.kv_heads * o.head_chunks, o.a.batch), dim3(WARPS * 32), bytes, stream, dim3(o.splits), tk, tv, o);
+  return e != cudaSuccess ? static_cast<int>(e) : launch_status();
+}
+
+// Units of all items, at most.
+long long most_units(const cacheir_b200_prefix_args& a, int tile_rows) {
+  const long long tiles = (static_cast<long long>(a.prefix_pages) * a.page_size + kKeys - 1) / kKeys;
+  return (kItemUnits + tiles) * a.kv_heads * (a.batch / tile_rows + a.groups);
+}
+int rows_of_tile(const cacheir_b200_prefix_args& a) { return 2 * kRows / (a.heads / a.kv_heads); }
+
 template <typename T, int D>
 int launch_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cudaStream_t stream) {
   CUtensorMap tk, tv;
   const uint64_t rows = static_cast<uint64_t>(a.num_slots) * a.kv_heads * a.page_size;
   if (!encode_pool<T>(&tk, a.k_cache, rows, D) || !encode_pool<T>(&tv, a.v_cache, rows, D)) return CACHEIR_B200_EUNSUPPORTED;
-  const int group = a.heads / a.kv_heads;
+  const int group = a.heads / a.kv_heads, tile_rows = rows_of_tile(a);
   const float scale_log2 = a.softmax_scale * 1.4426950408889634f;
-  const int tile_rows = 2 * kRows / group;
-  cudaError_t e = cudaSuccess;
   if (a.groups > 0) {
-    CommonParams c{a, parts, a.groups > kPlanGroups ? 1 : 0, tile_rows, scale_log2};
-    // no more blocks than there can be units
-    const long long tiles = (static_cast<long long>(a.prefix_pages) * a.page_size + kKeys - 1) / kKeys;
-    const long long most = tiles * a.kv_heads * ((a.batch + tile_rows - 1) / tile_rows + a.groups);
+    const CommonParams c{a, parts, a.groups > kPlanGroups ? 1 : 0, tile_rows, scale_log2};
+    const long long most = most_units(a, tile_rows);
     const int grid = static_cast<int>(most < kNumSMs ? most : kNumSMs);
+    cudaError_t e = cudaSuccess;
     if (c.plan_ready) e = launch_chained(prefix_plan_kernel, dim3(1), dim3(1024), 0, stream, c, grid);
     auto kern = prefix_common_kernel<T, D>;
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CommonSmem<D>::kBytes);
@@ -898,15 +923,12 @@ int launch_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cud
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   OwnParams o{a, parts, a.groups > 0 ? 1 : 0, tile_rows, (group + 15) / 16, 1, scale_log2};
-  // Parts of a row's own keys: while they find room on the GPU (two blocks on an SM), but no more than there are chunks to share.
   const long long blocks = static_cast<long long>(a.batch) * a.kv_heads * o.head_chunks;
+  if (blocks > 2 * kNumSMs) return launch_own<T, D, 2>(o, tk, tv, stream);
+  // Parts of a row's own keys while there are SMs for them, but no more than there are chunks to share.
   const long long chunks = static_cast<long long>(a.max_pages) * a.page_size / kChunk;
-  while (o.splits < kMaxOwnSplits && 2 * o.splits * blocks <= 2 * kNumSMs && 2 * o.splits * kOwnWarps <= chunks) o.splits *= 2;
-  auto kern = prefix_own_kernel<T, D>;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, OwnSmem<D>::kBytes);
-  if (e == cudaSuccess)
-    e = launch_clusters(kern, dim3(o.splits, a.kv_heads * o.head_chunks, a.batch), dim3(kOwnThreads), OwnSmem<D>::kBytes, stream, dim3(o.splits), tk, tv, o);
-  return e != cudaSuccess ? static_cast<int>(e) : launch_status();
+  while (o.splits < kMaxOwnSplits && 2 * o.splits * blocks <= kNumSMs && 2 * o.splits * 8 <= chunks) o.splits *= 2;
+  return launch_own<T, D, 8>(o, tk, tv, stream);
 }
 
 }  // namespace
@@ -916,7 +938,7 @@ bool prefix_fast_supported(const cacheir_b200_prefix_args& a) {
   return (a.dtype == CACHEIR_B200_F16 || a.dtype == CACHEIR_B200_BF16) && (a.dim == 64 || a.dim == 128) && a.page_size % kChunk == 0 &&
          group <= kMaxHeadsPerKv && aligned_to(a.q, 16) && a.q_stride % 8 == 0 && aligned_to(a.k_cache, 16) && aligned_to(a.v_cache, 16) &&
          static_cast<long long>(a.num_slots) * a.kv_heads * a.page_size <= 0x7fffffffLL - kChunk &&
-         static_cast<long long>(a.kv_heads) * ((group + 15) / 16) <= 65535;
+         static_cast<long long>(a.kv_heads) * ((group + 15) / 16) <= 65535 && most_units(a, rows_of_tile(a)) <= 0x7fffffffLL;
 }
 
 int launch_prefix_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cudaStream_t stream) {
