@@ -7,10 +7,16 @@
 namespace cb200 {
 
 // What the kernel of the common parts leaves for the one that joins: how its work was cut (see shared_prefix_mma.cu).
+struct PlanGroup {
+  int start;                  // its first unit
+  int row, rows;              // its rows
+  int prefix;                 // its common tokens
+};
 struct PrefixPlan {
   int units;                  // of all items
   int ctas;                   // blocks that share them
-  int start[2];               // [groups + 1] first unit of every group
+  int unused[2];
+  PlanGroup group[1];         // [groups], and the end of the last one's units
 };
 
 // The scratch: plan, then for every (piece, row, head) a maximum (log2 domain) and a denominator, and the unnormalised output.
@@ -70,7 +76,7 @@ inline int prefix_pieces(int batch, int heads, int dim) {
   return n < kMinPieces ? kMinPieces : n > kMaxPieces ? kMaxPieces : static_cast<int>(n);
 }
 inline size_t round_up_256(size_t n) { return (n + 255) / 256 * 256; }
-inline size_t prefix_plan_bytes(int batch) { return round_up_256(sizeof(PrefixPlan) + static_cast<size_t>(batch) * sizeof(int)); }
+inline size_t prefix_plan_bytes(int batch) { return round_up_256(sizeof(PrefixPlan) + static_cast<size_t>(batch) * sizeof(PlanGroup)); }
 inline size_t prefix_ml_bytes(int batch, int heads, int pieces) { return round_up_256(static_cast<size_t>(pieces) * batch * heads * 2 * 4); }
 
 // Tensor-core kernels (shared_prefix_mma.cu): 16-bit types, head sizes 64 and 128, pages of a multiple of 16 tokens.

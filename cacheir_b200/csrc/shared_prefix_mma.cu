@@ -28,7 +28,7 @@ constexpr int kKeys = 128;                     // keys of a tile
 constexpr int kRows = 128;                     // query rows of a group of warps
 constexpr int kChunk = 16;                     // keys that one copy brings: no page ends inside
 constexpr int kCommonThreads = 320;
-constexpr int kPlanGroups = 128;               // groups that every block lays out by itself
+constexpr int kPlanGroups = 64;                // groups that every block lays out by itself
 constexpr int kMaxHeadsPerKv = 64;
 constexpr float kAhead = 6.f;                  // a new reference is the maximum less this: probabilities start at 2^6 ..
 constexpr float kStale = 14.f;                 // .. and may grow to 2^14 (in fp16: 2^-24 of that is still a number)
@@ -68,6 +68,15 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t addr, uint32_t* r) {
         "=r"(r[31])
       : "r"(addr) : "memory");
 }
+// Waits for this thread's loads; v is one that must not be looked at before.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                 "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]),
+                 "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]),
+                 "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+               :: "memory");
+}
 __device__ __forceinline__ void tmem_st_x32(uint32_t addr, const uint32_t* v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
@@ -75,6 +84,29 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t addr, const uint32_t* v) {
       ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
       "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
       "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+               ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+               "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+// two floats of a register pair at a time
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void unpair(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 x, f32x2 y, f32x2 z) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
+  return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 x, f32x2 y) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  return d;
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -117,11 +149,12 @@ struct Deal {
 };
 
 __device__ __forceinline__ int key_tiles(int keys) { return (keys + kKeys - 1) / kKeys; }
-// Units of group g (the launcher has seen that all of them fit an int), and its key tiles.
-__device__ __forceinline__ int group_units(const cacheir_b200_prefix_args& a, int tile_rows, int g, int* tiles) {
-  const int rows = group_start(a, g + 1) - group_start(a, g);
-  *tiles = key_tiles(prefix_of_group(a, g));
-  return rows > 0 && *tiles > 0 ? a.kv_heads * ((rows + tile_rows - 1) / tile_rows) * (kItemUnits + *tiles) : 0;
+// Group g, and its units (the launcher has seen that all of them fit an int).
+__device__ __forceinline__ int group_units(const cacheir_b200_prefix_args& a, int tile_rows, int g, PlanGroup* out) {
+  out->row = group_start(a, g);
+  out->rows = max(group_start(a, g + 1) - out->row, 0);
+  out->prefix = prefix_of_group(a, g);
+  return out->rows > 0 && out->prefix > 0 ? a.kv_heads * ((out->rows + tile_rows - 1) / tile_rows) * (kItemUnits + key_tiles(out->prefix)) : 0;
 }
 // Blocks that take part: no item may be in more pieces than there is scratch for. n tiles touch ceil((n - 1) / share) + 1 blocks at most.
 __device__ __forceinline__ int plan_ctas(int units, int longest, int grid, int pieces) {
@@ -139,8 +172,10 @@ prefix_plan_kernel(const CommonParams p, const int grid) {
   int base = 0, longest = 0;
   for (int g0 = 0; g0 < p.a.groups; g0 += 1024) {
     const int g = g0 + threadIdx.x;
-    int tiles = 0, own = g < p.a.groups ? group_units(p.a, p.tile_rows, g, &tiles) : 0, sum = own;
-    if (own > 0) longest = max(longest, tiles);
+    PlanGroup group{};
+    const int own = g < p.a.groups ? group_units(p.a, p.tile_rows, g, &group) : 0;
+    int sum = own;
+    if (own > 0) longest = max(longest, key_tiles(group.prefix));
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, sum, off);
@@ -153,7 +188,8 @@ prefix_plan_kernel(const CommonParams p, const int grid) {
       if (w < warp) before += s_sum[w];
       all += s_sum[w];
     }
-    if (g < p.a.groups) p.parts.plan->start[g] = base + before + sum - own;
+    group.start = base + before + sum - own;
+    if (g < p.a.groups) p.parts.plan->group[g] = group;
     base += all;
     __syncthreads();
   }
@@ -162,7 +198,7 @@ prefix_plan_kernel(const CommonParams p, const int grid) {
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 0; w < 32; ++w) longest = max(longest, s_max[w]);
-    p.parts.plan->start[p.a.groups] = base;
+    p.parts.plan->group[p.a.groups].start = base;
     p.parts.plan->units = base;
     p.parts.plan->ctas = plan_ctas(base, longest, grid, p.parts.pieces);
   }
@@ -170,14 +206,13 @@ prefix_plan_kernel(const CommonParams p, const int grid) {
 
 // A block's share of the units, item by item.
 struct Walk {
-  const int* start;            // of every group
+  const PlanGroup* groups;
   Deal deal;
   int at, end;
   // the item
   int group, kvh, row0, rows, tile, tiles, prefix, piece;      // key tiles tile .. tile + tiles - 1 of it are this block's
-  const int32_t* pages;
 
-  __device__ __forceinline__ Walk(const int* s, int units, int ctas) : start(s), deal(units, ctas) {
+  __device__ __forceinline__ Walk(const PlanGroup* g, int units, int ctas) : groups(g), deal(units, ctas) {
     at = deal.begin(blockIdx.x);
     end = deal.begin(blockIdx.x + 1);
   }
@@ -186,23 +221,22 @@ struct Walk {
       int lo = 0, hi = p.a.groups;                             // last group that starts at or before `at` (empty ones start where the next does)
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (start[mid] <= at) lo = mid; else hi = mid;
+        if (groups[mid].start <= at) lo = mid; else hi = mid;
       }
-      group = lo;
-      const int first = group_start(p.a, lo), count = group_start(p.a, lo + 1) - first;
-      prefix = prefix_of_group(p.a, lo);
-      const int all = kItemUnits + key_tiles(prefix), row_tiles = (count + p.tile_rows - 1) / p.tile_rows;
-      const int rel = at - start[lo], item = rel / all, item0 = start[lo] + item * all, tile0 = item0 + kItemUnits;
+      const PlanGroup of = groups[lo];
+      const int all = kItemUnits + key_tiles(of.prefix), row_tiles = (of.rows + p.tile_rows - 1) / p.tile_rows;
+      const int rel = at - of.start, item = rel / all, item0 = of.start + item * all, tile0 = item0 + kItemUnits;
       const int stop = min(end, item0 + all);
       tile = max(at - tile0, 0);
       tiles = stop - tile0 - tile;
       at = stop;
       if (tiles <= 0) continue;                                // (no more than an item's beginning: the next block has its tiles)
+      group = lo;
+      prefix = of.prefix;
       kvh = item / row_tiles;
-      row0 = first + (item - kvh * row_tiles) * p.tile_rows;
-      rows = min(p.tile_rows, first + count - row0);
+      row0 = of.row + (item - kvh * row_tiles) * p.tile_rows;
+      rows = min(p.tile_rows, of.row + of.rows - row0);
       piece = blockIdx.x - deal.owner(tile0);
-      pages = p.a.prefix_table + static_cast<size_t>(lo) * p.a.prefix_pages;
       return true;
     }
     return false;
@@ -215,9 +249,9 @@ struct CommonSmem {
   static constexpr int kSlots = D == 128 ? 5 : 10;
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kTiles = 2 * kQBytes + kSlots * kSlotBytes;
-  // then: barriers full, empty [slots], q[2], s[2], p[2], o[2]; tensor memory address; group starts
+  // then: barriers full, empty [slots], q[2], s[2], p[2], o[2]; tensor memory address; groups
   static constexpr int kBarriers = 2 * kSlots + 8;
-  static constexpr int kBytes = 1024 + kTiles + kBarriers * 8 + 16 + (kPlanGroups + 1) * 4;
+  static constexpr int kBytes = 1024 + kTiles + kBarriers * 8 + 16 + (kPlanGroups + 1) * static_cast<int>(sizeof(PlanGroup));
 };
 
 template <typename T, int D>
@@ -237,19 +271,18 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   uint64_t* bar_p = bar_s + 2;                                 // probabilities are
   uint64_t* bar_o = bar_p + 2;                                 // .. and have been added to the output
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_o + 2);
-  int* s_start = reinterpret_cast<int*>(tmem_slot + 4);
-  __shared__ int s_plan[2], s_scan[4], s_longest[4];
+  PlanGroup* s_group = reinterpret_cast<PlanGroup*>(tmem_slot + 4);
+  __shared__ int s_plan[2], s_scan[kPlanGroups / 32], s_longest[kPlanGroups / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const cacheir_b200_prefix_args& a = p.a;
 
   // ---- the plan ----
   if (!p.plan_ready) {
+    PlanGroup mine{};
     int own = 0, sum = 0;
     if (warp < kPlanGroups / 32) {
-      int tiles = 0;
-      const int g = threadIdx.x;
-      own = g < a.groups ? group_units(a, p.tile_rows, g, &tiles) : 0;
-      const int longest = __reduce_max_sync(0xffffffffu, own > 0 ? tiles : 0);
+      own = static_cast<int>(threadIdx.x) < a.groups ? group_units(a, p.tile_rows, threadIdx.x, &mine) : 0;
+      const int longest = __reduce_max_sync(0xffffffffu, own > 0 ? key_tiles(mine.prefix) : 0);
       sum = own;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -267,9 +300,10 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         all += s_scan[w];
         longest = max(longest, s_longest[w]);
       }
-      if (static_cast<int>(threadIdx.x) < a.groups) s_start[threadIdx.x] = before + sum - own;
+      mine.start = before + sum - own;
+      if (static_cast<int>(threadIdx.x) < a.groups) s_group[threadIdx.x] = mine;
       if (threadIdx.x == 0) {
-        s_start[a.groups] = all;
+        s_group[a.groups].start = all;
         s_plan[0] = all;
         s_plan[1] = plan_ctas(all, longest, gridDim.x, p.parts.pieces);
       }
@@ -289,10 +323,10 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     mbar_fence_init();
   }
   __syncthreads();
-  const int* start = p.plan_ready ? p.parts.plan->start : s_start;
+  const PlanGroup* groups = p.plan_ready ? p.parts.plan->group : s_group;
   const int units = p.plan_ready ? p.parts.plan->units : s_plan[0], ctas = p.plan_ready ? p.parts.plan->ctas : s_plan[1];
   if (!p.plan_ready && blockIdx.x == 0) {                      // for the kernel that joins
-    for (int g = threadIdx.x; g <= a.groups; g += kCommonThreads) p.parts.plan->start[g] = s_start[g];
+    for (int g = threadIdx.x; g < a.groups; g += kCommonThreads) p.parts.plan->group[g] = s_group[g];
     if (threadIdx.x == 0) {
       p.parts.plan->units = units;
       p.parts.plan->ctas = ctas;
@@ -306,7 +340,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   const uint32_t tmem = *tmem_slot;                            // scores [2][128 columns] (probabilities over them), outputs [2][D]
   const uint32_t tmem_o = tmem + 2 * kKeys;
   const int group = a.heads / a.kv_heads;
-  Walk walk(start, units, ctas);
+  Walk walk(groups, units, ctas);
   bool ok = true;
 
   if (warp == 9) {
@@ -318,10 +352,11 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     int slot = 0;
     uint32_t phase = 1, sent = 0;
     while (ok && walk.next(p)) {
+      const int32_t* pages = a.prefix_table + static_cast<size_t>(walk.group) * a.prefix_pages;
       auto line_of = [&](int tile) {                           // first row of this lane's keys in the pool
         const int key = tile * kKeys + chunk * kChunk;
         if (!copies || key >= walk.prefix) return outside;
-        const int id = walk.pages[key / a.page_size];
+        const int id = pages[key / a.page_size];
         return id >= 0 && id < a.num_slots ? (id * a.kv_heads + walk.kvh) * a.page_size + key % a.page_size : outside;
       };
       int line = line_of(walk.tile);
@@ -375,6 +410,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       }
     };
     Steps score(walk), output(walk);
+    const bool leader = elect_one();
     int next_s = 0, next_o = 0;
     uint32_t q_seen[2] = {0, 0};
     while (ok) {
@@ -389,11 +425,14 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
         const bool frees = score.advance();
-        if (elect_one()) {
+        const uint64_t q_at = dq + (w * L::kQBytes >> 4), k_at = dk + (slot * L::kSlotBytes >> 4);
+        const uint32_t to = tmem + b * kKeys;
+        if (leader) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            mma_ss(tmem + b * kKeys, dq + ((w * L::kQBytes + (k >> 2) * kRows * 128 + (k & 3) * 32) >> 4),
-                   dk + ((slot * L::kSlotBytes + (k >> 2) * kKeys * 128 + (k & 3) * 32) >> 4), id_s, k > 0 ? 1u : 0u);
+          for (int k = 0; k < D / 16; ++k) {
+            constexpr int kHalf = kRows * 128 >> 4;            // 64 columns further
+            mma_ss(to, q_at + (k >> 2) * kHalf + (k & 3) * 2, k_at + (k >> 2) * kHalf + (k & 3) * 2, id_s, k > 0 ? 1u : 0u);
+          }
           tc_commit(smem_u32(&bar_s[b]));
           if (frees) tc_commit(smem_u32(&empty[slot]));
         }
@@ -407,11 +446,13 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       ok = ok && mbar_wait(smem_u32(&bar_p[b]), (next_o >> 1) & 1, &g_prefix_status, (15 << 8) | 6);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       tc_fence_after();
-      const bool opens = output.left == output.first, frees = output.advance();
-      if (elect_one()) {
+      const uint32_t add = output.left == output.first ? 0u : 1u;
+      const bool frees = output.advance();
+      const uint64_t v_at = dv + (slot * L::kSlotBytes >> 4);
+      const uint32_t to = tmem_o + w * D, from = tmem + b * kKeys;
+      if (leader) {
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-          mma_ts(tmem_o + w * D, tmem + b * kKeys + k * 8, dv + ((slot * L::kSlotBytes + k * 16 * 128) >> 4), id_o, opens && k == 0 ? 0u : 1u);
+        for (int k = 0; k < kKeys / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (16 * 128 >> 4), id_o, k == 0 ? add : 1u);
         tc_commit(smem_u32(&bar_o[b]));
         if (frees) tc_commit(smem_u32(&empty[slot]));
       }
@@ -458,19 +499,36 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         ok = mbar_wait(smem_u32(&bar_s[b]), (s >> 1) & 1, &g_prefix_status, (15 << 8) | 8);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
-        uint32_t v[kKeys];
         const uint32_t scores = tmem + b * kKeys + lane_addr;
+        const bool whole = __all_sync(0xffffffffu, base + kKeys <= limit);
+        // The row's 128 scores are looked at twice. For the maximum the second half comes first: the first half then stays in registers,
+        // and its probabilities may be written over scores 0 .. 31 while the second half is still where it was.
+        uint32_t x[32], y[32];
+        auto masked = [&](uint32_t (&v)[32], int first) {
 #pragma unroll
-        for (int c = 0; c < kKeys; c += 32) tmem_ld_x32(scores + c, v + c);
-        tc_wait_ld();
-        if (!__all_sync(0xffffffffu, base + kKeys <= limit)) {
-#pragma unroll
-          for (int i = 0; i < kKeys; ++i)
-            if (base + i >= limit) v[i] = 0xff800000u;         // -inf
-        }
+          for (int i = 0; i < 32; ++i)
+            if (base + first + i >= limit) v[i] = 0xff800000u;           // -inf
+        };
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto largest = [&](const uint32_t (&v)[32]) {
 #pragma unroll
-        for (int i = 0; i < kKeys; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
+          for (int i = 0; i < 32; i += 2)
+            asm("max.f32 %0, %1, %2, %0;" : "+f"(mx[(i >> 1) & 3]) : "f"(__uint_as_float(v[i])), "f"(__uint_as_float(v[i + 1])));
+        };
+        tmem_ld_x32(scores + 64, x);
+        tmem_ld_x32(scores + 96, y);
+        tmem_wait_ld(x);
+        tmem_wait_ld(y);
+        if (!whole) { masked(x, 64); masked(y, 96); }
+        largest(x);
+        largest(y);
+        tmem_ld_x32(scores, x);
+        tmem_ld_x32(scores + 32, y);
+        tmem_wait_ld(x);
+        tmem_wait_ld(y);
+        if (!whole) { masked(x, 0); masked(y, 32); }
+        largest(x);
+        largest(y);
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
         const bool grown = top > m_ref + kStale;
         if (__any_sync(0xffffffffu, grown)) {
@@ -482,29 +540,50 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
             if (!two) ok = mbar_wait(smem_u32(&bar_o[(s - 1) & 1]), ((s - 1) >> 1) & 1, &g_prefix_status, (15 << 8) | 9);
             __syncwarp();
             tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld_x32(tmem_o + w * D + lane_addr + c, o);
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tc_ld_x16(tmem_o + w * D + lane_addr + c, o);
               tc_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st_x32(tmem_o + w * D + lane_addr + c, o);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_x16(tmem_o + w * D + lane_addr + c, o);
             }
           }
         }
-        const float ref = m_ref > -INFINITY ? m_ref : 0.f;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float less = m_ref > -INFINITY ? -m_ref : 0.f;
+        f32x2 sum[2] = {0ull, 0ull};
+        const f32x2 scale2 = pair(p.scale_log2, p.scale_log2), less2 = pair(less, less);
+        auto weigh = [&](const uint32_t (&v)[32], uint32_t* out) {
 #pragma unroll
-        for (int i = 0; i < kKeys; i += 2) {
-          const float x = ex2(fmaf(__uint_as_float(v[i]), p.scale_log2, -ref)), y = ex2(fmaf(__uint_as_float(v[i + 1]), p.scale_log2, -ref));
-          sum[i & 2] += x;
-          sum[(i & 2) + 1] += y;
-          v[i >> 1] = pack_pair<T>(x, y);
+          for (int i = 0; i < 32; i += 2) {
+            float a0, a1;
+            unpair(fma2(pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), scale2, less2), a0, a1);
+            a0 = ex2(a0);
+            a1 = ex2(a1);
+            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pair(a0, a1));
+            out[i >> 1] = pack_pair<T>(a0, a1);
+          }
+        };
+        {
+          uint32_t out[32];
+          weigh(x, out);
+          tmem_ld_x32(scores + 64, x);                         // (on its way meanwhile)
+          weigh(y, out + 16);
+          tmem_wait_ld(x);
+          tmem_ld_x32(scores + 96, y);
+          tmem_st_x32(scores, out);
+          if (!whole) masked(x, 64);
+          weigh(x, out);
+          tmem_wait_ld(y);
+          if (!whole) masked(y, 96);
+          weigh(y, out + 16);
+          tmem_st_x32(scores + 32, out);
         }
-        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st_x32(scores, v);
-        tmem_st_x32(scores + 32, v + 32);
+        float s0, s1, s2, s3;
+        unpair(sum[0], s0, s1);
+        unpair(sum[1], s2, s3);
+        l_run += (s0 + s1) + (s2 + s3);
         tmem_wait_st();
         // keys behind the prefix in its last page may hold anything: zero their values, so that 0 * value stays 0
         const int rest = walk.prefix - base;
@@ -528,18 +607,27 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       ok = mbar_wait(smem_u32(&bar_o[last & 1]), (last >> 1) & 1, &g_prefix_status, (15 << 8) | 11);
       __syncwarp();
       tc_fence_after();
-      const size_t at = (static_cast<size_t>(walk.piece) * a.batch + b_row) * a.heads + head;
-      if (real) *reinterpret_cast<float2*>(p.parts.ml + 2 * at) = make_float2(m_ref, l_run);
-#pragma unroll
+      const int at = static_cast<int>(static_cast<size_t>(b_row) * a.heads + head);
+      const size_t piece0 = static_cast<size_t>(walk.piece) * a.batch * a.heads;
+      if (real) *reinterpret_cast<float2*>(p.parts.ml + 2 * (piece0 + at)) = make_float2(m_ref, l_run);
+      // By way of shared memory (the queries' place), so that a store writes whole lines: a lane has a row, a store 128 bytes of four rows.
+      float* s_row = reinterpret_cast<float*>(s_q + w * L::kQBytes + (warp & 3) * (L::kQBytes / 4));
+      const int lanes = min(32, used - q_row0 - (warp & 3) * 32);        // rows of this warp
+#pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
         tmem_ld_x32(tmem_o + w * D + lane_addr + c, o);
         tc_wait_ld();
-        if (real) {
-          uint4* dst = reinterpret_cast<uint4*>(p.parts.acc + at * D + c);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(s_row + lane * 32 + ((i ^ (lane & 7)) << 2)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = 4 * i + (lane >> 3), to = __shfl_sync(0xffffffffu, at, row);
+          const uint4 v = *reinterpret_cast<const uint4*>(s_row + row * 32 + (((lane & 7) ^ (row & 7)) << 2));
+          if (row < lanes) *reinterpret_cast<uint4*>(p.parts.acc + (piece0 + to) * D + c + (lane & 7) * 4) = v;
         }
+        __syncwarp();
       }
       tc_fence_before();
     }
@@ -558,7 +646,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
 // the parts are a thread-block cluster. Keys and values come 16 tokens at a time (TMA): every warp takes every WARPS-th chunk of the part
 // through a ring of its own, with warp MMAs that have the query heads as their 16 rows. Bound by the memory's rate where there are many
 // rows: then blocks of two warps, four of them on an SM, so that while some begin or join others keep the memory busy; where there are
-// few, blocks of eight. None of that needs the common part's kernel: this one starts as soon as that one's blocks leave room, and waits for
+// few, blocks of four or eight. None of that needs the common part's kernel: this one starts as soon as that one's blocks leave room, and waits for
 // it before it joins.
 constexpr int kOwnStages = 3;
 constexpr int kMaxOwnSplits = 8;
@@ -808,10 +896,10 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   if (p.splits > 1) cluster_sync_release(); else __syncthreads();
   int pieces = 0;
   if (p.common && prefix > 0) {                                  // (then the row is in a group that has items)
-    const int start = p.parts.plan->start[of];
+    const PlanGroup in = p.parts.plan->group[of];
     const Deal deal(p.parts.plan->units, p.parts.plan->ctas);
-    const int first = group_start(a, of), row_tiles = (group_start(a, of + 1) - first + p.tile_rows - 1) / p.tile_rows;
-    const int all = kItemUnits + key_tiles(prefix), item0 = start + (kvh * row_tiles + (row - first) / p.tile_rows) * all;
+    const int row_tiles = (in.rows + p.tile_rows - 1) / p.tile_rows;
+    const int all = kItemUnits + key_tiles(prefix), item0 = in.start + (kvh * row_tiles + (row - in.row) / p.tile_rows) * all;
     pieces = deal.owner(item0 + all - 1) - deal.owner(item0 + kItemUnits) + 1;
   }
   const size_t at0 = static_cast<size_t>(row) * a.heads + head0, step = static_cast<size_t>(a.batch) * a.heads;
@@ -925,6 +1013,7 @@ int launch_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cud
   OwnParams o{a, parts, a.groups > 0 ? 1 : 0, tile_rows, (group + 15) / 16, 1, scale_log2};
   const long long blocks = static_cast<long long>(a.batch) * a.kv_heads * o.head_chunks;
   if (blocks > 2 * kNumSMs) return launch_own<T, D, 2>(o, tk, tv, stream);
+  if (blocks > kNumSMs) return launch_own<T, D, 4>(o, tk, tv, stream);
   // Parts of a row's own keys while there are SMs for them, but no more than there are chunks to share.
   const long long chunks = static_cast<long long>(a.max_pages) * a.page_size / kChunk;
   while (o.splits < kMaxOwnSplits && 2 * o.splits * blocks <= kNumSMs && 2 * o.splits * 8 <= chunks) o.splits *= 2;
