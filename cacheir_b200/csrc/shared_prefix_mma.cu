@@ -7,8 +7,8 @@
 //
 // Common part. An item is (group, key/value head, tile of up to 256 query rows); its keys come in tiles of 128. The key tiles of all items,
 // in a row, are cut evenly over the blocks, so that lengths and sizes of groups do not matter; an item that is cut leaves one piece per
-// block. One warp brings keys and values (TMA, page by page, into a ring of 32 KB slots), one issues the MMAs, and two groups of four
-// warps do the softmax, a thread per query row. Above 128 rows each group of warps has its own 128 of them and the two take turns on the
+// block. One warp brings keys and one values (TMA, 16 tokens at a time, into a ring of 32 KB slots; by one warp the copies' issue, 66 cycles
+// each, was what the tensor cores waited for), one issues the MMAs, and two groups of four warps do the softmax, a thread per query row. Above 128 rows each group of warps has its own 128 of them and the two take turns on the
 // tensor cores with the same keys; else the first one has them all and scores run one tile ahead. A row's maximum is a reference that
 // moves only when it is exceeded by 2^14, so that the outputs, which stay in tensor memory, are hardly ever rescaled; probabilities are
 // rounded to the element type as the second MMA's operand, their sums are not.
@@ -27,7 +27,7 @@ using namespace ptx;
 constexpr int kKeys = 128;                     // keys of a tile
 constexpr int kRows = 128;                     // query rows of a group of warps
 constexpr int kChunk = 16;                     // keys that one copy brings: no page ends inside
-constexpr int kCommonThreads = 320;
+constexpr int kCommonThreads = 352;
 constexpr int kPlanGroups = 64;                // groups that every block lays out by itself
 constexpr int kMaxHeadsPerKv = 64;
 constexpr float kAhead = 6.f;                  // a new reference is the maximum less this: probabilities start at 2^6 ..
@@ -109,10 +109,18 @@ __device__ __forceinline__ f32x2 add2(f32x2 x, f32x2 y) {
   return d;
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// Operand whose rows are the MMA's k: boxes of 64 columns by 128 rows (16 KB apart), 8-row groups 1024 B apart.
+// Operand whose rows are the MMA's k: boxes of 64 columns by 16 rows (2 KB apart), 8-row groups 1024 B apart.
 __device__ __forceinline__ uint64_t smem_desc_columns(uint32_t addr) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | static_cast<uint64_t>((kKeys * 128) >> 4) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | static_cast<uint64_t>((kChunk * 128) >> 4) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
          static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -310,6 +318,8 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     }
   }
   if (threadIdx.x == 288) {
+    prefetch_map(&tmap_k);
+    prefetch_map(&tmap_v);
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(smem_u32(&full[s]), 1);
       mbar_init(smem_u32(&empty[s]), 1);
@@ -343,44 +353,46 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   Walk walk(groups, units, ctas);
   bool ok = true;
 
-  if (warp == 9) {
-    // ---------------- copies: a lane per 16 keys and 64 columns ----------------
-    constexpr int kBoxes = D / 64;
-    const int chunk = lane / kBoxes, box = lane % kBoxes;
+  if (warp >= 9) {
+    // ------- copies: warp 9 keys, a lane per 16 of them and 64 columns; warp 10 values, a lane per 16 of them -------
+    const bool keys = warp == 9;
+    const int boxes = keys ? D / 64 : 1, chunk = lane / boxes, box = lane % boxes;
     const bool copies = chunk < kKeys / kChunk;
     const int outside = a.num_slots * a.kv_heads * a.page_size;         // rows behind the pool read as zeros
-    int slot = 0;
-    uint32_t phase = 1, sent = 0;
+    const uint32_t dst = smem_u32(s_kv) + (keys ? box * kKeys * 128 + chunk * kChunk * 128 : chunk * kChunk * D * 2);
+    int slot = keys ? 0 : 1;
+    uint32_t phase = 1, sent = 0;                              // slots of a tile: its keys', its values'
     while (ok && walk.next(p)) {
       const int32_t* pages = a.prefix_table + static_cast<size_t>(walk.group) * a.prefix_pages;
-      auto line_of = [&](int tile) {                           // first row of this lane's keys in the pool
+      auto line_of = [&](int tile) {                           // first row of this lane's 16 in the pool
         const int key = tile * kKeys + chunk * kChunk;
         if (!copies || key >= walk.prefix) return outside;
         const int id = pages[key / a.page_size];
         return id >= 0 && id < a.num_slots ? (id * a.kv_heads + walk.kvh) * a.page_size + key % a.page_size : outside;
       };
       int line = line_of(walk.tile);
-      for (int t = walk.tile; t < walk.tile + walk.tiles && ok; ++t) {
+      for (int t = walk.tile; t < walk.tile + walk.tiles; ++t) {
         const int next = t + 1 < walk.tile + walk.tiles ? line_of(t + 1) : 0;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          ok = ok && mbar_wait(smem_u32(&empty[slot]), phase, &g_prefix_status, (15 << 8) | 1);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (lane == 0) mbar_expect_tx(smem_u32(&full[slot]), L::kSlotBytes);
-          __syncwarp();
-          if (copies)
-            tma_load_2d(smem_u32(s_kv + slot * L::kSlotBytes + box * kKeys * 128 + chunk * kChunk * 128), kv == 0 ? &tmap_k : &tmap_v,
-                        smem_u32(&full[slot]), box * 64, line);
-          ++sent;
-          if (++slot == kSlots) { slot = 0; phase ^= 1; }
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[slot]), phase, &g_prefix_status, (15 << 8) | 1));
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(smem_u32(&full[slot]), L::kSlotBytes);
+        __syncwarp();
+        if (copies) {
+          if (keys) tma_load_3d(dst + slot * L::kSlotBytes, &tmap_k, smem_u32(&full[slot]), 0, line, box);
+          else tma_load_3d(dst + slot * L::kSlotBytes, &tmap_v, smem_u32(&full[slot]), 0, line, 0);
         }
+        ++sent;
+        slot += 2;
+        if (slot >= kSlots) { slot -= kSlots; phase ^= 1; }
         line = next;
       }
     }
     // nothing may still be on its way when the block ends, also after a wait that gave up
-    for (uint32_t i = sent > kSlots ? sent - kSlots : 0; i < sent; ++i)
-      mbar_wait(smem_u32(&full[i % kSlots]), (i / kSlots) & 1, &g_prefix_status, (15 << 8) | 2);
+    for (uint32_t i = sent > kSlots ? sent - kSlots : 0; i < sent; ++i) {
+      const uint32_t n = 2 * i + (keys ? 0 : 1);
+      if (ok && n + kSlots < 2 * sent) continue;               // its slot has been filled again since: it came, and that phase is long over
+      mbar_wait(smem_u32(&full[n % kSlots]), (n / kSlots) & 1, &g_prefix_status, (15 << 8) | 2);
+    }
   } else if (warp == 8) {
     // ---------------- MMA issue ----------------
     constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
@@ -452,7 +464,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       const uint32_t to = tmem_o + w * D, from = tmem + b * kKeys;
       if (leader) {
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (16 * 128 >> 4), id_o, k == 0 ? add : 1u);
+        for (int k = 0; k < kKeys / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, k == 0 ? add : 1u);
         tc_commit(smem_u32(&bar_o[b]));
         if (frees) tc_commit(smem_u32(&empty[slot]));
       }
@@ -593,7 +605,8 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           const int rows = kChunk - rest % kChunk;
           for (int i = r; i < rows * (D / 8); i += kRows) {
             const int key = rest + i / (D / 8), c = i % (D / 8);
-            *reinterpret_cast<uint4*>(s_kv + slot * L::kSlotBytes + (c >> 3) * kKeys * 128 + key * 128 + ((c & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(s_kv + slot * L::kSlotBytes + (key / kChunk) * kChunk * D * 2 + (c >> 3) * kChunk * 128 + key % kChunk * 128 + ((c & 7) << 4)) =
+                make_uint4(0u, 0u, 0u, 0u);
           }
           fence_async_smem();
         }
@@ -645,28 +658,29 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
 // Every row's own keys, and the pieces joined. One block per (part of the row's own keys, key/value head and up to 16 of its query heads, row);
 // the parts are a thread-block cluster. Keys and values come 16 tokens at a time (TMA): every warp takes every WARPS-th chunk of the part
 // through a ring of its own, with warp MMAs that have the query heads as their 16 rows. Bound by the memory's rate where there are many
-// rows: then blocks of two warps, four of them on an SM, so that while some begin or join others keep the memory busy; where there are
+// rows: then blocks of two warps, six of them on an SM, so that while some begin or join others keep the memory busy; where there are
 // few, blocks of four or eight. None of that needs the common part's kernel: this one starts as soon as that one's blocks leave room, and waits for
 // it before it joins.
-constexpr int kOwnStages = 3;
 constexpr int kMaxOwnSplits = 8;
 
 struct OwnParams {
   cacheir_b200_prefix_args a;
   PrefixParts parts;
   int common;                                  // a kernel of common parts runs before
+  int grid;                                    // .. of so many blocks
   int tile_rows, head_chunks, splits;
   float scale_log2;
 };
 
 template <int D, int WARPS>
 struct OwnSmem {
+  static constexpr int kStages = WARPS == 2 ? 2 : 3;
   static constexpr int kTileBytes = kChunk * D * 2;
-  static constexpr int kRing = WARPS * kOwnStages * 2 * kTileBytes;
+  static constexpr int kRing = WARPS * kStages * 2 * kTileBytes;
   // over the ring afterwards: the warps' states, the block's, and the weights of all sources of a head
   static constexpr int kSources = kMaxPieces + kMaxOwnSplits;
   static constexpr int kJoin = (WARPS * 16 * (D + 2) + 16 * (D + 2) + 16 * kSources) * 4;
-  static constexpr int kBytes = 1024 + (kRing > kJoin ? kRing : kJoin) + WARPS * kOwnStages * 8;
+  static constexpr int kBytes = 1024 + (kRing > kJoin ? kRing : kJoin) + WARPS * kStages * 8;
 };
 
 __device__ __forceinline__ void ldsm_trans(uint32_t addr, uint32_t (&r)[4]) {
@@ -693,11 +707,51 @@ __device__ __forceinline__ float4 ld_rank_f32x4(const float* local, uint32_t ran
   return v;
 }
 
+// A row's group (rows and prefix 0 outside every group). Up to 32 groups, a lane each, the warp lays the plan out beside that: one round of
+// loads, and nothing of it has to wait for the common part's kernel.
+struct RowGroup {
+  PlanGroup in;
+  int group, planned, units, ctas;             // planned: ctas is the longest item's key tiles (what plan_ctas takes)
+};
+__device__ __forceinline__ RowGroup row_group(const cacheir_b200_prefix_args& a, int tile_rows, int row) {
+  RowGroup r{};
+  r.group = -1;
+  if (a.groups <= 0) return r;
+  if (a.groups > 32) {
+    r.group = group_of_row(a, row, &r.in.prefix);
+    if (r.group >= 0) {
+      r.in.row = group_start(a, r.group);
+      r.in.rows = group_start(a, r.group + 1) - r.in.row;
+    }
+    return r;
+  }
+  const int lane = threadIdx.x & 31;
+  PlanGroup mine{};
+  const int own = lane < a.groups ? group_units(a, tile_rows, lane, &mine) : 0;
+  int sum = own;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, sum, off);
+    if (lane >= off) sum += up;
+  }
+  r.planned = 1;
+  r.units = __shfl_sync(0xffffffffu, sum, 31);
+  r.ctas = __reduce_max_sync(0xffffffffu, own > 0 ? key_tiles(mine.prefix) : 0);
+  const uint32_t found = __ballot_sync(0xffffffffu, mine.rows > 0 && mine.row <= row && row < mine.row + mine.rows);
+  if (found == 0) return r;
+  r.group = 31 - __clz(found);
+  r.in.start = __shfl_sync(0xffffffffu, sum - own, r.group);
+  r.in.row = __shfl_sync(0xffffffffu, mine.row, r.group);
+  r.in.rows = __shfl_sync(0xffffffffu, mine.rows, r.group);
+  r.in.prefix = __shfl_sync(0xffffffffu, mine.prefix, r.group);
+  return r;
+}
+
 template <typename T, int D, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32)
 prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ OwnParams p) {
   using L = OwnSmem<D, WARPS>;
-  constexpr int kBoxes = D / 64, kThreads = WARPS * 32;
+  constexpr int kThreads = WARPS * 32, kStages = L::kStages;
   // What stands before this wait reads what was there before the common part's kernel began: its blocks let this one in only after they
   // had waited for all earlier ones.
   if (!p.common) chain_enter();
@@ -706,29 +760,23 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   const cacheir_b200_prefix_args& a = p.a;
   const int split = blockIdx.x, kvh = blockIdx.y / p.head_chunks, row = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.heads / a.kv_heads, head0 = kvh * group + blockIdx.y % p.head_chunks * 16, heads = min(16, (kvh + 1) * group - head0);
-  const uint32_t bars = smem_u32(smem_raw + L::kBytes - WARPS * kOwnStages * 8) + warp * kOwnStages * 8;
-  const uint32_t ring = smem_u32(smem) + warp * kOwnStages * 2 * L::kTileBytes;
+  const uint32_t bars = smem_u32(smem_raw + L::kBytes - WARPS * kStages * 8) + warp * kStages * 8;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * L::kTileBytes;
   const int g = lane >> 2, t4 = lane & 3;
   if (lane == 0) {
-    for (int s = 0; s < kOwnStages; ++s) mbar_init(bars + s * 8, 1);
+    for (int s = 0; s < kStages; ++s) mbar_init(bars + s * 8, 1);
     mbar_fence_init();
+    if (warp == 0) {
+      prefetch_map(&tmap_k);
+      prefetch_map(&tmap_v);
+    }
   }
   // Lengths, group, first page ids and queries are asked for together as far as they can be.
   const int len = min(max(a.seq_lens[row], 0), a.max_pages * a.page_size);
-  int prefix;
-  const int of = group_of_row(a, row, &prefix);
-  const int from = min(prefix, len);
+  RowGroup of = row_group(p.a, p.tile_rows, row);
+  const int prefix = of.in.prefix, from = min(prefix, len);
   const int chunk0 = from / kChunk, chunks = len > from ? (len + kChunk - 1) / kChunk - chunk0 : 0, per = (chunks + p.splits - 1) / p.splits;
   const int begin = chunk0 + min(chunks, split * per), end = chunk0 + min(chunks, (split + 1) * per);
-  const int32_t* pages = a.page_table + static_cast<size_t>(row) * a.max_pages;
-  const int outside = a.num_slots * a.kv_heads * a.page_size;   // rows behind the pool read as zeros
-  const int mine = begin + warp < end ? (end - begin - warp + WARPS - 1) / WARPS : 0;          // chunks begin + warp + i * WARPS
-  auto line_of = [&](int i) {                                    // first row of this warp's i-th chunk in the pool
-    if (i >= mine) return outside;
-    const int key = (begin + warp + i * WARPS) * kChunk, id = pages[key / a.page_size];
-    return id >= 0 && id < a.num_slots ? (id * a.kv_heads + kvh) * a.page_size + key % a.page_size : outside;
-  };
-  int lines = line_of(lane), lines_next = mine > 32 ? line_of(32 + lane) : outside;            // of chunks 32 k + lane, k rising
   uint32_t qa[D / 16][4];                                        // queries as the A operand: rows = heads
   {
     const T* q = static_cast<const T*>(a.q) + static_cast<size_t>(row) * a.q_stride + static_cast<size_t>(head0) * D;
@@ -740,16 +788,23 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         qa[k][i] = h < heads ? *reinterpret_cast<const uint32_t*>(q + static_cast<size_t>(h) * D + col) : 0u;
       }
   }
+  const int32_t* pages = a.page_table + static_cast<size_t>(row) * a.max_pages;
+  const int outside = a.num_slots * a.kv_heads * a.page_size;   // rows behind the pool read as zeros
+  const int mine = begin + warp < end ? (end - begin - warp + WARPS - 1) / WARPS : 0;          // chunks begin + warp + i * WARPS
+  auto line_of = [&](int i) {                                    // first row of this warp's i-th chunk in the pool
+    if (i >= mine) return outside;
+    const int key = (begin + warp + i * WARPS) * kChunk, id = pages[key / a.page_size];
+    return id >= 0 && id < a.num_slots ? (id * a.kv_heads + kvh) * a.page_size + key % a.page_size : outside;
+  };
+  int lines = line_of(lane), lines_next = mine > 32 ? line_of(32 + lane) : outside;            // of chunks 32 k + lane, k rising
   __syncwarp();
-  auto copy = [&](int i, int s) {                                // chunk i into stage s: a lane per 64 columns of keys and of values
+  auto copy = [&](int i, int s) {                                // chunk i into stage s: a lane for the keys, one for the values
     const int line = __shfl_sync(0xffffffffu, lines, i & 31);
     if (lane == 0) mbar_expect_tx(bars + s * 8, 2 * L::kTileBytes);
     __syncwarp();
-    if (lane < 2 * kBoxes)
-      tma_load_2d(ring + s * 2 * L::kTileBytes + (lane / kBoxes) * L::kTileBytes + (lane % kBoxes) * kChunk * 128, lane < kBoxes ? &tmap_k : &tmap_v,
-                  bars + s * 8, (lane % kBoxes) * 64, line);
+    if (lane < 2) tma_load_3d(ring + (2 * s + lane) * L::kTileBytes, lane == 0 ? &tmap_k : &tmap_v, bars + s * 8, 0, line, 0);
   };
-  for (int s = 0; s < kOwnStages; ++s)
+  for (int s = 0; s < kStages; ++s)
     if (s < mine) copy(s, s);
 
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f}, o[D / 8][4];
@@ -763,8 +818,8 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   for (int it = 0; it < mine; ++it) {
     ok = __all_sync(0xffffffffu, mbar_wait(bars + stage * 8, phase, &g_prefix_status, (15 << 8) | 12));
     if (!ok) {                                                   // the copies that are still under way are waited for
-      for (int i = it + 1; i < min(mine, it + kOwnStages); ++i) {
-        if (++stage == kOwnStages) { stage = 0; phase ^= 1; }
+      for (int i = it + 1; i < min(mine, it + kStages); ++i) {
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
         mbar_wait(bars + stage * 8, phase, &g_prefix_status, (15 << 8) | 13);
       }
       break;
@@ -837,7 +892,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       mma_pair<T>(o[2 * j + 1], pa, vb[2], vb[3]);
     }
     __syncwarp();                                                // the stage has been read
-    const int ahead = it + kOwnStages;
+    const int ahead = it + kStages;
     if (ahead < mine) {
       if ((ahead & 31) == 0) {                                   // (its line and those behind it are the next round's)
         lines = lines_next;
@@ -845,7 +900,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       }
       copy(ahead, stage);
     }
-    if (++stage == kOwnStages) { stage = 0; phase ^= 1; }
+    if (++stage == kStages) { stage = 0; phase ^= 1; }
   }
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
@@ -896,10 +951,16 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   if (p.splits > 1) cluster_sync_release(); else __syncthreads();
   int pieces = 0;
   if (p.common && prefix > 0) {                                  // (then the row is in a group that has items)
-    const PlanGroup in = p.parts.plan->group[of];
-    const Deal deal(p.parts.plan->units, p.parts.plan->ctas);
-    const int row_tiles = (in.rows + p.tile_rows - 1) / p.tile_rows;
-    const int all = kItemUnits + key_tiles(prefix), item0 = in.start + (kvh * row_tiles + (row - in.row) / p.tile_rows) * all;
+    if (!of.planned) {
+      of.in.start = p.parts.plan->group[of.group].start;
+      of.units = p.parts.plan->units;
+      of.ctas = p.parts.plan->ctas;
+    } else {
+      of.ctas = plan_ctas(of.units, of.ctas, p.grid, p.parts.pieces);
+    }
+    const Deal deal(of.units, of.ctas);
+    const int row_tiles = (of.in.rows + p.tile_rows - 1) / p.tile_rows;
+    const int all = kItemUnits + key_tiles(prefix), item0 = of.in.start + (kvh * row_tiles + (row - of.in.row) / p.tile_rows) * all;
     pieces = deal.owner(item0 + all - 1) - deal.owner(item0 + kItemUnits) + 1;
   }
   const size_t at0 = static_cast<size_t>(row) * a.heads + head0, step = static_cast<size_t>(a.batch) * a.heads;
@@ -934,43 +995,72 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       if (i * 32 + lane < sources) s_w[h * L::kSources + i * 32 + lane] = ms[i] * inv;
   }
   __syncthreads();
-  for (int i = split * kThreads + threadIdx.x; i < heads * (D / 4); i += p.splits * kThreads) {
-    const int h = i / (D / 4), d = i % (D / 4) * 4;
-    const float* wgt = s_w + h * L::kSources;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    auto add = [&](const float4& x, float f) {
-      v[0] = fmaf(x.x, f, v[0]); v[1] = fmaf(x.y, f, v[1]); v[2] = fmaf(x.z, f, v[2]); v[3] = fmaf(x.w, f, v[3]);
-    };
-    const float4* acc = reinterpret_cast<const float4*>(p.parts.acc + (at0 + h) * D + d);
-    for (int k = 0; k < p.splits; ++k) add(p.splits > 1 ? ld_rank_f32x4(s_o + h * D + d, k) : *reinterpret_cast<const float4*>(s_o + h * D + d), wgt[k]);
-    int k = 0;
-    for (; k + 8 <= pieces; k += 8) {
-      float4 x[8];
+  // Four neighbouring outputs are a place; ITEMS places of a thread and DEEP pieces of each are on their way at once.
+  const int stride = p.splits * kThreads, places = heads * (D / 4);
+  auto finish = [&](auto items, auto deep) {
+    constexpr int ITEMS = decltype(items)::value, DEEP = decltype(deep)::value;
+    for (int i0 = split * kThreads + threadIdx.x; i0 < places; i0 += ITEMS * stride) {
+      float v[ITEMS][4];
+      const float* acc[ITEMS];
+      const float* wgt[ITEMS];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = acc[(k + j) * step * (D / 4)];
+      for (int j = 0; j < ITEMS; ++j) {
+        const int i = min(i0 + j * stride, places - 1), h = i / (D / 4), d = i % (D / 4) * 4;
+        acc[j] = p.parts.acc + (at0 + h) * D + d;
+        wgt[j] = s_w + h * L::kSources;
+        v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0.f;
+        for (int k = 0; k < p.splits; ++k) {
+          const float4 x = p.splits > 1 ? ld_rank_f32x4(s_o + h * D + d, k) : *reinterpret_cast<const float4*>(s_o + h * D + d);
+          const float f = wgt[j][k];
+          v[j][0] = fmaf(x.x, f, v[j][0]); v[j][1] = fmaf(x.y, f, v[j][1]); v[j][2] = fmaf(x.z, f, v[j][2]); v[j][3] = fmaf(x.w, f, v[j][3]);
+        }
+      }
+      const int live = min(ITEMS, (places - i0 + stride - 1) / stride);
+#pragma unroll 1
+      for (int k = 0; k < pieces; k += DEEP) {
+        float4 x[DEEP][ITEMS];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) add(x[j], wgt[p.splits + k + j]);
+        for (int e = 0; e < DEEP; ++e)
+#pragma unroll
+          for (int j = 0; j < ITEMS; ++j)
+            x[e][j] = j < live && k + e < pieces ? *reinterpret_cast<const float4*>(acc[j] + (k + e) * step * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int e = 0; e < DEEP; ++e)
+#pragma unroll
+          for (int j = 0; j < ITEMS; ++j) {
+            const float f = k + e < pieces ? wgt[j][p.splits + k + e] : 0.f;
+            v[j][0] = fmaf(x[e][j].x, f, v[j][0]); v[j][1] = fmaf(x[e][j].y, f, v[j][1]);
+            v[j][2] = fmaf(x[e][j].z, f, v[j][2]); v[j][3] = fmaf(x[e][j].w, f, v[j][3]);
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < ITEMS; ++j)
+        if (j < live) {
+          const int i = i0 + j * stride, h = i / (D / 4), d = i % (D / 4) * 4;
+          T* out = static_cast<T*>(a.out) + static_cast<size_t>(row) * a.out_stride + static_cast<size_t>(head0 + h) * D + d;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) Elem<T>::st(out + e, v[j][e]);
+        }
     }
-    for (; k < pieces; ++k) add(acc[k * step * (D / 4)], wgt[p.splits + k]);
-    T* out = static_cast<T*>(a.out) + static_cast<size_t>(row) * a.out_stride + static_cast<size_t>(head0 + h) * D + d;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) Elem<T>::st(out + j, v[j]);
-  }
+  };
+  if (places <= stride) finish(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+  else finish(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
   if (p.splits > 1) {
     __syncwarp();
     cluster_sync_release();                                      // nobody leaves while its part is being read
   }
 }
 
+// A pool as [dim / 64][rows][64]: boxes of 16 rows and 64 columns, or of 16 rows and all columns, 64 by 64.
 template <typename T>
-bool encode_pool(CUtensorMap* map, const void* base, uint64_t rows, int dim) {
+bool encode_pool(CUtensorMap* map, const void* base, uint64_t rows, int dim, bool whole) {
   EncodeTiledFn fn = tensor_map_encoder();
   if (!fn) return false;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(dim), rows};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(dim) * 2};
-  const cuuint32_t box[2] = {64, kChunk};
-  const cuuint32_t elem_strides[2] = {1, 1};
-  return fn(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
+  const cuuint64_t dims[3] = {64, rows, static_cast<cuuint64_t>(dim / 64)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(dim) * 2, 128};
+  const cuuint32_t box[3] = {64, kChunk, whole ? static_cast<cuuint32_t>(dim / 64) : 1u};
+  const cuuint32_t elem_strides[3] = {1, 1, 1};
+  return fn(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
             strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -994,23 +1084,26 @@ int rows_of_tile(const cacheir_b200_prefix_args& a) { return 2 * kRows / (a.head
 
 template <typename T, int D>
 int launch_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cudaStream_t stream) {
-  CUtensorMap tk, tv;
+  CUtensorMap tk, tv, tk_half;
   const uint64_t rows = static_cast<uint64_t>(a.num_slots) * a.kv_heads * a.page_size;
-  if (!encode_pool<T>(&tk, a.k_cache, rows, D) || !encode_pool<T>(&tv, a.v_cache, rows, D)) return CACHEIR_B200_EUNSUPPORTED;
+  if (!encode_pool<T>(&tk, a.k_cache, rows, D, true) || !encode_pool<T>(&tv, a.v_cache, rows, D, true) ||
+      (a.groups > 0 && !encode_pool<T>(&tk_half, a.k_cache, rows, D, false)))
+    return CACHEIR_B200_EUNSUPPORTED;
   const int group = a.heads / a.kv_heads, tile_rows = rows_of_tile(a);
   const float scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  int grid = 0;
   if (a.groups > 0) {
     const CommonParams c{a, parts, a.groups > kPlanGroups ? 1 : 0, tile_rows, scale_log2};
     const long long most = most_units(a, tile_rows);
-    const int grid = static_cast<int>(most < kNumSMs ? most : kNumSMs);
+    grid = static_cast<int>(most < kNumSMs ? most : kNumSMs);
     cudaError_t e = cudaSuccess;
     if (c.plan_ready) e = launch_chained(prefix_plan_kernel, dim3(1), dim3(1024), 0, stream, c, grid);
     auto kern = prefix_common_kernel<T, D>;
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CommonSmem<D>::kBytes);
-    if (e == cudaSuccess) e = launch_chained(kern, dim3(grid), dim3(kCommonThreads), CommonSmem<D>::kBytes, stream, tk, tv, c);
+    if (e == cudaSuccess) e = launch_chained(kern, dim3(grid), dim3(kCommonThreads), CommonSmem<D>::kBytes, stream, tk_half, tv, c);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  OwnParams o{a, parts, a.groups > 0 ? 1 : 0, tile_rows, (group + 15) / 16, 1, scale_log2};
+  OwnParams o{a, parts, a.groups > 0 ? 1 : 0, grid, tile_rows, (group + 15) / 16, 1, scale_log2};
   const long long blocks = static_cast<long long>(a.batch) * a.kv_heads * o.head_chunks;
   if (blocks > 2 * kNumSMs) return launch_own<T, D, 2>(o, tk, tv, stream);
   if (blocks > kNumSMs) return launch_own<T, D, 4>(o, tk, tv, stream);

@@ -12,6 +12,14 @@ DEV = "cuda"
 HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}      # a rounding, relative to the value
 
 
+@pytest.fixture(autouse=True)
+def no_wait_gave_up():
+    from cacheir_b200 import _lib
+
+    yield
+    assert _lib.load_group("serving").cacheir_b200_serving_device_status(1) == 0
+
+
 def _gen(seed):
     return torch.Generator(device=DEV).manual_seed(seed)
 
