@@ -227,4 +227,7 @@ extern "C" int cacheir_b200_shared_prefix_attention(const cacheir_b200_prefix_ar
   return launch_general<__nv_bfloat16>(a, parts, as_stream(stream));
 }
 
-extern "C" int cacheir_b200_serving_device_status(int reset) { return prefix_device_status(reset != 0); }
+extern "C" int cacheir_b200_serving_device_status(int reset) {
+  const int prefix = prefix_device_status(reset != 0), logprobs = logprobs_device_status(reset != 0);
+  return prefix != 0 ? prefix : logprobs;
+}

@@ -1,33 +1,74 @@
-// Log probabilities of given tokens, entropies and the likeliest alternatives of rows of logits.
+// Log probabilities of given tokens, entropies and the likeliest alternatives of rows of logits, in one pass over the row.
 //
-// In units of log 2, y = x log2(e) / T:  Z = sum 2^(y - m),  log p(t) = ln 2 (y_t - m) - ln Z,  H = ln Z - ln 2 sum 2^(y - m) (y - m) / Z
-// with m the row's largest y: both terms of H are non-negative, nothing cancels. Sums are 32-bit floats, one per thread with a running
-// maximum, joined by a tree.
+// With m the row's largest value and y = (x - m) log2(e) / T:  Z = sum 2^y,  S = sum 2^y y,
+//   log p(t) = (x_t - m) / T - ln Z,   H = ln Z - ln 2 S / Z   (both terms are non-negative: nothing cancels).
+// Every lane keeps 32-bit sums of its own relative to the largest value that it has met; they are joined by trees.
+//
+// The likeliest `top` come out of the same pass. A lane looks at 64 bytes at a time (a group: neighbouring values) and leaves the group's
+// largest value in shared memory. Of the groups only the `top` first by (largest value, lower index) can hold one of the `top` first values
+// by (value, lower index): each group before a given one has a value before all of that one's. So a few hundred values are read again, and
+// that holds for any data, ties and masks included.
+//
+// Bound by memory for many rows (2048 x 128256 in bf16), by latency for few. A row is read by one block, or by a thread-block cluster where
+// there are few; every warp copies 2 KB pieces (bulk copies, a ring of its own: no barrier between warps) and has four to six of them on
+// their way. Per value that is half an instruction each for maximum and minimum, one to widen it, one for the exponent's argument, one
+// exponential (16 a cycle and SM: 73 % of the memory's rate), half each for the two sums.
 #include "cacheir_b200_serving.h"
-#include "common.cuh"
+#include "hybrid_common.cuh"
+#include "serving_status.h"
+#include "tc_ptx.cuh"
 
 namespace cb200 {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr float kLowest = -1e30f;          // stands for masked values: 2^(kLowest - m) is 0 and its product with (y - m) too
+using namespace ptx;
 
-struct Sums { float m, z, s; };             // largest value (unscaled), sum of e = 2^(c (x - m)), sum of e c (x - m)
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTileBytes = 2048;           // of a warp's copy: 64 bytes a lane
+constexpr int kTopStages = 4, kSumStages = 6;
+constexpr int kMaxTiles = 256;             // of a block, where its groups' largest values are kept
+constexpr int kMaxCluster = 8;
+constexpr int kList = 256;                 // candidates that are ranked against one another
+constexpr float kMasked = -1e30f;          // what is at or below it weighs nothing beside anything above it
+constexpr float kHuge = 1e30f;
+constexpr float kFar = -1e6f;              // 2^kFar is 0, and kFar times a sum is a number
 
-// log2-domain change of reference
+__device__ int g_logprobs_status = 0;
+
+struct Args {
+  const void* logits;
+  long long stride;
+  const int64_t* tokens;
+  float* logprobs;
+  float* entropy;
+  int64_t* top_ids;
+  float* top_logprobs;
+  int vocab, top, cluster, stages;
+  double inv_t;
+};
+
+struct Sums {
+  float m, z, s;                           // the largest x (-inf: nothing yet), Z, S
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ Sums joined(const Sums& a, const Sums& b, float c) {
-  if (!(b.m > -INFINITY) && b.m == b.m) return a;           // nothing in b
-  if (!(a.m > -INFINITY) && a.m == a.m) return b;
+  if (b.m == -INFINITY) return a;
+  if (a.m == -INFINITY) return b;
   Sums r;
   r.m = fmaxf(a.m, b.m);
-  const float da = fmaxf((a.m - r.m) * c, kLowest), db = fmaxf((b.m - r.m) * c, kLowest);
-  const float wa = exp2f(da), wb = exp2f(db);
+  const float da = fmaxf((a.m - r.m) * c, kFar), db = fmaxf((b.m - r.m) * c, kFar), wa = ex2(da), wb = ex2(db);
   r.z = a.z * wa + b.z * wb;
   r.s = (a.s + da * a.z) * wa + (b.s + db * b.z) * wb;
   return r;
 }
 
-// Values as integers of the same order, NaN above all; -0 is 0.
+// Values as integers of the same order, NaN above all; -0 is 0. 0 is no value.
 __device__ __forceinline__ uint32_t ordered_bits(float v) {
   if (v != v) return 0xffffffffu;
   const uint32_t b = __float_as_uint(v + 0.f);
@@ -36,76 +77,503 @@ __device__ __forceinline__ uint32_t ordered_bits(float v) {
 __device__ __forceinline__ float from_ordered(uint32_t b) {
   return b == 0xffffffffu ? NAN : __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
+__device__ __forceinline__ unsigned long long key_of(uint32_t value, uint32_t index) { return static_cast<unsigned long long>(value) << 32 | (~index & 0xffffffffu); }
+
+// two floats of a register pair at a time
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void unpair(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 x, f32x2 y, f32x2 z) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
+  return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 x, f32x2 y) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 x, f32x2 y) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  return d;
+}
+
+// 64 bytes of a row: largest (NaN if there is one) and smallest value, and its values two by two
+template <typename T>
+struct Group;
+template <>
+struct Group<float> {
+  static constexpr int kPairs = 8;
+  static __device__ __forceinline__ void range(const uint32_t (&w)[16], float& mx, float& mn) {
+    mx = __uint_as_float(w[0]);
+    mn = mx;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) {
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(mx) : "f"(__uint_as_float(w[i])));
+      mn = fminf(mn, __uint_as_float(w[i]));
+    }
+  }
+  static __device__ __forceinline__ void two(const uint32_t (&w)[16], int i, float& lo, float& hi) { lo = __uint_as_float(w[2 * i]); hi = __uint_as_float(w[2 * i + 1]); }
+  static constexpr uint32_t kNothing = 0xff800000u;       // -inf
+};
+template <>
+struct Group<__half> {
+  static constexpr int kPairs = 16;
+  static __device__ __forceinline__ void range(const uint32_t (&w)[16], float& mx, float& mn) {
+    __half2 hi = *reinterpret_cast<const __half2*>(&w[0]), lo = hi;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) {
+      hi = __hmax2_nan(hi, *reinterpret_cast<const __half2*>(&w[i]));
+      lo = __hmin2(lo, *reinterpret_cast<const __half2*>(&w[i]));
+    }
+    mx = __half2float(__hmax_nan(__low2half(hi), __high2half(hi)));
+    mn = __half2float(__hmin(__low2half(lo), __high2half(lo)));
+  }
+  static __device__ __forceinline__ void two(const uint32_t (&w)[16], int i, float& lo, float& hi) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    lo = f.x;
+    hi = f.y;
+  }
+  static constexpr uint32_t kNothing = 0xfc00fc00u;
+};
+template <>
+struct Group<__nv_bfloat16> {
+  static constexpr int kPairs = 16;
+  static __device__ __forceinline__ void range(const uint32_t (&w)[16], float& mx, float& mn) {
+    __nv_bfloat162 hi = *reinterpret_cast<const __nv_bfloat162*>(&w[0]), lo = hi;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) {
+      hi = __hmax2_nan(hi, *reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+      lo = __hmin2(lo, *reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+    }
+    mx = __bfloat162float(__hmax_nan(__low2bfloat16(hi), __high2bfloat16(hi)));
+    mn = __bfloat162float(__hmin(__low2bfloat16(lo), __high2bfloat16(lo)));
+  }
+  static __device__ __forceinline__ void two(const uint32_t (&w)[16], int i, float& lo, float& hi) {
+    lo = __uint_as_float(w[i] << 16);
+    hi = __uint_as_float(w[i] & 0xffff0000u);
+  }
+  static constexpr uint32_t kNothing = 0xff80ff80u;
+};
+
+__device__ __forceinline__ uint32_t ld_rank_u32(const void* local, uint32_t rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(map_to_rank(smem_u32(local), rank)) : "memory");
+  return v;
+}
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-token_logprobs_kernel(const T* __restrict__ logits, long long stride, const int64_t* __restrict__ tokens, float* __restrict__ logprobs,
-                      float* __restrict__ entropy, int64_t* __restrict__ top_ids, float* __restrict__ top_logprobs, int vocab, int top, double inv_t) {
+__global__ void __launch_bounds__(kThreads, 2)
+token_logprobs_kernel(const __grid_constant__ Args p) {
   chain_enter();
-  __shared__ Sums s_sums[kThreads / 32];
-  __shared__ unsigned long long s_key[kThreads / 32];
-  __shared__ int s_nan[1];
+  using G = Group<T>;
+  constexpr int kGroup = 64 / sizeof(T), kTile = kTileBytes / sizeof(T), kVec = 16 / sizeof(T);
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t s_bar[kWarps * kSumStages];
+  __shared__ Sums s_sums[kWarps];
+  __shared__ int s_flags[kWarps];
+  __shared__ Sums s_block;
+  __shared__ int s_block_flags;
+  __shared__ unsigned long long s_top[CACHEIR_B200_MAX_TOP];
+  __shared__ __align__(16) uint32_t s_best[kThreads];     // (read four at a time)
+  __shared__ uint32_t s_bound;
+  __shared__ int s_count;
+  __shared__ int s_selected[CACHEIR_B200_MAX_TOP];
+  __shared__ unsigned long long s_round[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const T* row = logits + static_cast<size_t>(blockIdx.x) * stride;
-  const float c = static_cast<float>(inv_t * 1.4426950408889634);
-  Sums a{-INFINITY, 0.f, 0.f};
-  bool bad = false;
-  for (int i = threadIdx.x; i < vocab; i += kThreads) {
-    const float x = Elem<T>::ld(row + i);
-    if (!(x < INFINITY)) bad = true;
-    else if (x > -INFINITY) a = joined(a, Sums{x, 1.f, 0.f}, c);
+  const int rank = p.cluster > 1 ? blockIdx.x % p.cluster : 0, row = blockIdx.x / p.cluster;
+  const T* x = static_cast<const T*>(p.logits) + static_cast<size_t>(row) * p.stride;
+  // The row as single values up to the first 16-byte boundary, tiles, and single values behind the last whole 16 bytes.
+  const int head = min(p.vocab, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T)));
+  const int body = (p.vocab - head) / kVec * kVec, tail = p.vocab - head - body, all_tiles = (body + kTile - 1) / kTile;
+  const int per_block = (all_tiles + p.cluster - 1) / p.cluster, tile0 = min(all_tiles, rank * per_block), tiles = min(all_tiles, tile0 + per_block) - tile0;
+  uint8_t* ring = smem + warp * p.stages * kTileBytes;
+  float* s_max = reinterpret_cast<float*>(smem + kWarps * p.stages * kTileBytes);      // [tiles * 32 groups], with `top` only
+  const uint32_t bar = smem_u32(&s_bar[warp * kSumStages]);
+  const float c = static_cast<float>(p.inv_t * 1.4426950408889634);
+
+  const int mine = warp < tiles ? (tiles - warp + kWarps - 1) / kWarps : 0;            // this warp's tiles: warp + i * kWarps
+  auto bytes_of = [&](int i) { return min(kTile, body - (tile0 + warp + i * kWarps) * kTile) * static_cast<int>(sizeof(T)); };
+  auto copy = [&](int i, int s) {                          // (one lane)
+    const uint32_t n = bytes_of(i);
+    mbar_expect_tx(bar + s * 8, n);
+    bulk_load(smem_u32(ring + s * kTileBytes), x + head + static_cast<size_t>(tile0 + warp + i * kWarps) * kTile, n, bar + s * 8);
+  };
+  if (lane == 0) {
+    for (int s = 0; s < p.stages; ++s) mbar_init(bar + s * 8, 1);
+    mbar_fence_init();
+    for (int s = 0; s < p.stages && s < mine; ++s) copy(s, s);
   }
-  if (threadIdx.x == 0) s_nan[0] = 0;
-  const bool nan = __syncthreads_or(bad ? 1 : 0) != 0;
+  __syncwarp();
+
+  float m = -INFINITY;
+  f32x2 z2 = 0ull, s2 = 0ull;                              // (both halves)
+  int flags = 0;                                           // 1: NaN or +inf, 2: values beyond kHuge, 4: some at or below kMasked that are not -inf
+  auto rescale = [&](float mx) {                           // the lane's sums become relative to mx
+    if (m > -INFINITY) {
+      const float d = fmaxf((m - mx) * c, kFar), w = ex2(d);
+      const f32x2 w2 = pair(w, w), d2 = pair(d, d);
+      s2 = mul2(fma2(d2, z2, s2), w2);
+      z2 = mul2(z2, w2);
+    }
+    m = mx;
+  };
+  // A few values at a time are added as they are; what is masked weighs nothing.
+  auto add_one = [&](float v) {
+    if (!(v < kHuge)) { flags |= v < INFINITY ? 2 : 1; return; }
+    if (v <= kMasked) { if (v > -INFINITY) flags |= 4; return; }
+    if (v > m) rescale(v);
+    const float y = (v - m) * c, e = ex2(y);
+    z2 = add2(z2, pair(e, 0.f));
+    s2 = fma2(pair(e, 0.f), pair(y, 0.f), s2);
+  };
+  int stage = 0;
+  uint32_t phase = 0;
+#pragma unroll 1
+  for (int i = 0; i < mine; ++i) {
+    if (!__all_sync(0xffffffffu, mbar_wait(bar + stage * 8, phase, &g_logprobs_status, (16 << 8) | 1))) {
+      for (int k = i + 1; k < min(mine, i + p.stages); ++k) {        // the copies that are still under way
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+        mbar_wait(bar + stage * 8, phase, &g_logprobs_status, (16 << 8) | 2);
+      }
+      flags |= 1;                                          // (the row's results are no numbers)
+      break;
+    }
+    uint32_t w[16];
+    const int n16 = bytes_of(i) / 16;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = lane * 4 + ((j + (lane >> 1)) & 3);   // (in an order in which eight lanes reach all banks)
+      const uint4 v = *reinterpret_cast<const uint4*>(ring + stage * kTileBytes + at * 16);
+      w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+      if (at >= n16) w[4 * j] = w[4 * j + 1] = w[4 * j + 2] = w[4 * j + 3] = G::kNothing;
+    }
+    __syncwarp();
+    if (lane == 0 && i + p.stages < mine) copy(i + p.stages, stage);
+    if (++stage == p.stages) { stage = 0; phase ^= 1; }
+    float mx, mn;
+    G::range(w, mx, mn);
+    if (p.top > 0) s_max[(warp + i * kWarps) * 32 + lane] = mx;
+    const bool plain = mx < kHuge && mn > kMasked;
+    if (__all_sync(0xffffffffu, plain)) {
+      if (mx > m) rescale(mx);
+      const f32x2 c2 = pair(c, c), less = pair(-m, -m);
+#pragma unroll
+      for (int k = 0; k < G::kPairs; ++k) {
+        float lo, hi, y0, y1;
+        G::two(w, k, lo, hi);
+        const f32x2 y = mul2(add2(pair(lo, hi), less), c2);
+        unpair(y, y0, y1);
+        const f32x2 e = pair(ex2(y0), ex2(y1));
+        z2 = add2(z2, e);
+        s2 = fma2(e, y, s2);
+      }
+    } else if (!(mx < kHuge)) {
+      flags |= mx < INFINITY ? 2 : 1;
+    } else if (mx <= kMasked) {
+      if (mx > -INFINITY) flags |= 4;
+    } else {
+      if (mx > m) rescale(mx);
+      const f32x2 c2 = pair(c, c), less = pair(-m, -m);
+#pragma unroll
+      for (int k = 0; k < G::kPairs; ++k) {
+        float lo, hi, y0, y1;
+        G::two(w, k, lo, hi);
+        const f32x2 y = mul2(add2(pair(fmaxf(lo, kMasked), fmaxf(hi, kMasked)), less), c2);
+        unpair(y, y0, y1);
+        const f32x2 e = pair(ex2(y0), ex2(y1));
+        z2 = add2(z2, e);
+        s2 = fma2(e, y, s2);
+      }
+    }
+  }
+  // the single values of both ends: lanes of the first block's first warp, of the last block's
+  if (warp == 0 && rank == 0 && lane < head) add_one(Elem<T>::ld(x + lane));
+  if (warp == 0 && rank == p.cluster - 1 && lane < tail) add_one(Elem<T>::ld(x + head + body + lane));
+
+  // ---- sums ----
+  Sums a;
+  {
+    float z0, z1, s0, s1;
+    unpair(z2, z0, z1);
+    unpair(s2, s0, s1);
+    a = Sums{m, z0 + z1, s0 + s1};
+  }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
-    Sums o{__shfl_xor_sync(0xffffffffu, a.m, off), __shfl_xor_sync(0xffffffffu, a.z, off), __shfl_xor_sync(0xffffffffu, a.s, off)};
+    const Sums o{__shfl_xor_sync(0xffffffffu, a.m, off), __shfl_xor_sync(0xffffffffu, a.z, off), __shfl_xor_sync(0xffffffffu, a.s, off)};
     a = lane & off ? joined(o, a, c) : joined(a, o, c);
   }
-  if (lane == 0) s_sums[warp] = a;
-  __syncthreads();
-  a = s_sums[0];
-  for (int w = 1; w < kThreads / 32; ++w) a = joined(a, s_sums[w], c);
-  const bool empty = !(a.m > -INFINITY);
-  const float log_z = logf(a.z);
-  auto log_p = [&](float x) {
-    if (nan) return static_cast<float>(NAN);
-    if (empty) return -INFINITY;
-    return static_cast<float>(static_cast<double>(x - a.m) * inv_t - static_cast<double>(log_z));
-  };
+  flags = __reduce_or_sync(0xffffffffu, flags);
+  if (lane == 0) { s_sums[warp] = a; s_flags[warp] = flags; }
+  if (threadIdx.x == 0) s_count = 0;
+  __syncthreads();                                         // (the rings are drained)
   if (threadIdx.x == 0) {
-    if (logprobs) {
-      const int64_t t = tokens[blockIdx.x];
-      logprobs[blockIdx.x] = t < 0 ? 0.f : t >= vocab ? static_cast<float>(NAN) : log_p(Elem<T>::ld(row + t));
-    }
-    if (entropy) entropy[blockIdx.x] = nan ? static_cast<float>(NAN) : empty ? 0.f : log_z - 0.6931471805599453f * a.s / a.z;
+    a = s_sums[0];
+    flags = s_flags[0];
+    for (int w = 1; w < kWarps; ++w) { a = joined(a, s_sums[w], c); flags |= s_flags[w]; }
+    s_block = a;
+    s_block_flags = flags;
   }
-  unsigned long long last = ~0ull;
-  for (int k = 0; k < top; ++k) {
-    unsigned long long best = 0;
-    for (int i = threadIdx.x; i < vocab; i += kThreads) {
-      const unsigned long long key = (static_cast<unsigned long long>(ordered_bits(Elem<T>::ld(row + i))) << 32) | static_cast<uint32_t>(~i);
-      if (key > best && key < last) best = key;
-    }
+
+  // ---- the block's likeliest `top` ----
+  if (p.top > 0) {
+    const int top = p.top, ends = (rank == 0 && head > 0 ? 1 : 0) + (rank == p.cluster - 1 && tail > 0 ? 1 : 0);
+    const int first = rank == 0 && head > 0 ? 1 : 0, groups = tiles * 32 + ends;       // in order: the head, those of the tiles, the tail
+    unsigned long long* s_list = reinterpret_cast<unsigned long long*>(smem);          // [kList], over the rings
+    auto value_of = [&](int g) -> uint32_t {
+      if (g >= first && g - first < tiles * 32) {
+        // (group g - first of the tiles; those behind the last value hold none)
+        return tile0 * kTile + (g - first) * kGroup < body ? ordered_bits(s_max[g - first]) : 0u;
+      }
+      const bool front = g < first;
+      uint32_t best = 0;
+      for (int i = 0; i < (front ? head : tail); ++i) best = max(best, ordered_bits(Elem<T>::ld(x + (front ? 0 : head + body) + i)));
+      return best;
+    };
+    auto range_of = [&](int g, int* from) {                // its values
+      if (g >= first && g - first < tiles * 32) {
+        const int at = tile0 * kTile + (g - first) * kGroup;
+        *from = head + at;
+        return min(kGroup, body - at);
+      }
+      *from = g < first ? 0 : head + body;
+      return g < first ? head : tail;
+    };
+    // the largest key below `last` that anybody offers (the slow way, for lists that do not fit)
+    auto next_best = [&](unsigned long long best) {
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, off);
-      if (o > best) best = o;
+      for (int off = 16; off > 0; off >>= 1) {
+        const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, off);
+        if (o > best) best = o;
+      }
+      __syncthreads();
+      if (lane == 0) s_round[warp] = best;
+      __syncthreads();
+      for (int w = 0; w < kWarps; ++w)
+        if (s_round[w] > best) best = s_round[w];
+      return best;
+    };
+    // A bound from below: of the threads' best groups the `top`-th.
+    uint32_t best = 0;
+    for (int g = threadIdx.x; g < groups; g += kThreads) best = max(best, value_of(g));
+    s_best[threadIdx.x] = best;
+    if (threadIdx.x < CACHEIR_B200_MAX_TOP) { s_selected[threadIdx.x] = -1; s_top[threadIdx.x] = 0; }
+    __syncthreads();
+    int ahead = 0;
+    for (int i = 0; i < kThreads; i += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(&s_best[i]);
+      ahead += (o.x > best || (o.x == best && i < static_cast<int>(threadIdx.x))) + (o.y > best || (o.y == best && i + 1 < static_cast<int>(threadIdx.x))) +
+               (o.z > best || (o.z == best && i + 2 < static_cast<int>(threadIdx.x))) + (o.w > best || (o.w == best && i + 3 < static_cast<int>(threadIdx.x)));
+    }
+    if (ahead == top - 1) s_bound = best;
+    __syncthreads();
+    const uint32_t bound = s_bound;
+    for (int g = threadIdx.x; g < groups; g += kThreads) {
+      const uint32_t v = value_of(g);
+      if (v >= bound && v > 0) {
+        const int at = atomicAdd(&s_count, 1);             // (any order: they are ranked)
+        if (at < kList) s_list[at] = key_of(v, g);
+      }
     }
     __syncthreads();
-    if (lane == 0) s_key[warp] = best;
+    const int found = s_count;
+    if (found <= kList) {
+      if (static_cast<int>(threadIdx.x) < found) {
+        const unsigned long long key = s_list[threadIdx.x];
+        int before = 0;
+        for (int i = 0; i < found; ++i) before += s_list[i] > key ? 1 : 0;
+        if (before < top) {
+          s_selected[before] = static_cast<int>(~static_cast<uint32_t>(key));
+          if (before == top - 1) s_bound = static_cast<uint32_t>(key >> 32);
+        }
+      }
+      if (found < top && threadIdx.x == 0) s_bound = 0;
+    } else {
+      unsigned long long last = ~0ull;
+      for (int k = 0; k < top; ++k) {
+        unsigned long long mine_best = 0;
+        for (int g = threadIdx.x; g < groups; g += kThreads) {
+          const unsigned long long key = key_of(value_of(g), g);
+          if (key < last && key > mine_best && (key >> 32) > 0) mine_best = key;
+        }
+        last = next_best(mine_best);
+        if (threadIdx.x == 0) {
+          s_selected[k] = static_cast<int>(~static_cast<uint32_t>(last));
+          s_bound = static_cast<uint32_t>(last >> 32);
+        }
+      }
+    }
     __syncthreads();
-    for (int w = 0; w < kThreads / 32; ++w) if (s_key[w] > best) best = s_key[w];
-    last = best;
+    // Their values: every one that can be among the first has at least the last selected group's largest value.
+    constexpr int kPer = CACHEIR_B200_MAX_TOP * kGroup / kThreads;
+    unsigned long long keys[kPer];
+    const uint32_t least = s_bound;
+    if (threadIdx.x == 0) s_count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int at = threadIdx.x + j * kThreads, k = at / kGroup, e = at % kGroup;
+      keys[j] = 0;
+      if (k >= top || s_selected[k] < 0) continue;
+      int from;
+      if (e >= range_of(s_selected[k], &from)) continue;
+      const uint32_t v = ordered_bits(Elem<T>::ld(x + from + e));
+      if (v < least) continue;
+      keys[j] = key_of(v, from + e);
+      const int place = atomicAdd(&s_count, 1);
+      if (place < kList) s_list[place] = keys[j];
+    }
+    __syncthreads();
+    const int values = s_count;
+    if (values <= kList) {
+      if (static_cast<int>(threadIdx.x) < values) {
+        const unsigned long long key = s_list[threadIdx.x];
+        int before = 0;
+        for (int i = 0; i < values; ++i) before += s_list[i] > key ? 1 : 0;
+        if (before < top) s_top[before] = key;
+      }
+    } else {
+      unsigned long long last = ~0ull;
+      for (int k = 0; k < top; ++k) {
+        unsigned long long mine_best = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (keys[j] < last && keys[j] > mine_best) mine_best = keys[j];
+        last = next_best(mine_best);
+        if (threadIdx.x == 0) s_top[k] = last;
+      }
+    }
+  }
+
+  // ---- the row ----
+  __syncthreads();
+  if (p.cluster > 1) cluster_sync_release();
+  if (rank == 0) {
+    a = s_block;
+    flags = s_block_flags;
+    for (int r = 1; r < p.cluster; ++r) {
+      const Sums o{__uint_as_float(ld_rank_u32(&s_block.m, r)), __uint_as_float(ld_rank_u32(&s_block.z, r)), __uint_as_float(ld_rank_u32(&s_block.s, r))};
+      a = joined(a, o, c);
+      flags |= static_cast<int>(ld_rank_u32(&s_block_flags, r));
+    }
+    double log_z = 0.0, entropy = 0.0;
+    const bool nan = (flags & 1) != 0;
+    bool empty = false;
+    if (!nan && ((flags & 2) || (a.m == -INFINITY && (flags & 4)))) {
+      // Values of 1e30 and more, or none above -1e30: the same in 64 bits, relative to the largest one.
+      double mx = -INFINITY, z = 0.0, s = 0.0;
+      for (int i = threadIdx.x; i < p.vocab; i += kThreads) mx = fmax(mx, static_cast<double>(Elem<T>::ld(x + i)));
+      __shared__ double s_wide[3][kThreads];
+      s_wide[0][threadIdx.x] = mx;
+      __syncthreads();
+      for (int i = 0; i < kThreads; ++i) mx = fmax(mx, s_wide[0][i]);
+      for (int i = threadIdx.x; i < p.vocab; i += kThreads) {
+        const double y = (static_cast<double>(Elem<T>::ld(x + i)) - mx) * p.inv_t;
+        if (y > -1e4) {
+          const double e = exp(y);
+          z += e;
+          s += e * y;
+        }
+      }
+      s_wide[1][threadIdx.x] = z;
+      s_wide[2][threadIdx.x] = s;
+      __syncthreads();
+      z = s = 0.0;
+      for (int i = 0; i < kThreads; ++i) { z += s_wide[1][i]; s += s_wide[2][i]; }
+      a.m = static_cast<float>(mx);
+      log_z = log(z);
+      entropy = log_z - s / z;
+    } else if (!nan && a.m == -INFINITY) {
+      empty = true;
+    } else if (!nan) {
+      log_z = log(static_cast<double>(a.z));
+      entropy = log_z - 0.6931471805599453 * static_cast<double>(a.s) / static_cast<double>(a.z);
+    }
+    auto log_p = [&](float v) {
+      if (nan) return static_cast<float>(NAN);
+      if (empty || v == -INFINITY) return -INFINITY;
+      return static_cast<float>((static_cast<double>(v) - static_cast<double>(a.m)) * p.inv_t - log_z);
+    };
     if (threadIdx.x == 0) {
-      const size_t at = static_cast<size_t>(blockIdx.x) * top + k;
-      top_ids[at] = static_cast<int64_t>(~static_cast<uint32_t>(best));
-      top_logprobs[at] = log_p(from_ordered(static_cast<uint32_t>(best >> 32)));
+      if (p.logprobs) {
+        const int64_t t = p.tokens[row];
+        p.logprobs[row] = t < 0 ? 0.f : t >= p.vocab ? static_cast<float>(NAN) : log_p(Elem<T>::ld(x + t));
+      }
+      if (p.entropy) p.entropy[row] = nan ? static_cast<float>(NAN) : empty ? 0.f : static_cast<float>(entropy);
     }
+    if (p.top > 0) {
+      unsigned long long key = 0;
+      int before = -1;
+      if (p.cluster == 1) {
+        if (static_cast<int>(threadIdx.x) < p.top) { key = s_top[threadIdx.x]; before = threadIdx.x; }
+      } else {                                             // the blocks' lists ranked against one another
+        unsigned long long* s_list = reinterpret_cast<unsigned long long*>(smem);
+        const int n = p.cluster * p.top;
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+          const int r = i / p.top, k = i % p.top;
+          const uint32_t* from = reinterpret_cast<const uint32_t*>(&s_top[k]);
+          s_list[i] = static_cast<unsigned long long>(ld_rank_u32(from + 1, r)) << 32 | ld_rank_u32(from, r);
+        }
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < n) {
+          key = s_list[threadIdx.x];
+          before = 0;
+          for (int i = 0; i < n; ++i) before += s_list[i] > key ? 1 : 0;
+        }
+      }
+      if (before >= 0 && before < p.top && key > 0) {
+        const size_t at = static_cast<size_t>(row) * p.top + before;
+        p.top_ids[at] = static_cast<int64_t>(~static_cast<uint32_t>(key));
+        p.top_logprobs[at] = log_p(from_ordered(static_cast<uint32_t>(key >> 32)));
+      }
+    }
+  }
+  if (p.cluster > 1) {
+    __syncwarp();
+    cluster_sync_release();                                // nobody leaves while its results are being read
   }
 }
 
+// Blocks for a row: as many waves of them as there are places (two on an SM), each as long as its tiles and what begins and ends it, about
+// 24 tiles' time.
+int cluster_of(int rows, int tiles, int least) {
+  int best = least;
+  long long shortest = -1;
+  for (int n = least; n <= kMaxCluster; n *= 2) {
+    const long long waves = (static_cast<long long>(rows) * n + 2 * kNumSMs - 1) / (2 * kNumSMs);
+    const long long time = waves * ((tiles + n - 1) / n + 24);
+    if (shortest < 0 || time < shortest) { shortest = time; best = n; }
+  }
+  return best;
+}
+
+template <typename T>
+int launch_logprobs(Args a, int rows, cudaStream_t stream) {
+  const long long tiles = (static_cast<long long>(a.vocab) * sizeof(T) + kTileBytes - 1) / kTileBytes;
+  int least = 1;
+  if (a.top > 0)
+    while (least < kMaxCluster && tiles > static_cast<long long>(least) * kMaxTiles) least *= 2;
+  if (a.top > 0 && tiles > static_cast<long long>(least) * kMaxTiles) return CACHEIR_B200_ELIMIT;
+  a.cluster = cluster_of(rows, static_cast<int>(tiles), least);
+  a.stages = a.top > 0 ? kTopStages : kSumStages;
+  const int per_block = static_cast<int>((tiles + a.cluster - 1) / a.cluster);
+  const size_t smem = static_cast<size_t>(kWarps) * a.stages * kTileBytes + (a.top > 0 ? static_cast<size_t>(per_block) * 32 * 4 : 0);
+  auto kern = token_logprobs_kernel<T>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e == cudaSuccess) e = launch_clusters(kern, dim3(static_cast<unsigned>(rows) * a.cluster), dim3(kThreads), smem, stream, dim3(a.cluster), a);
+  return e != cudaSuccess ? static_cast<int>(e) : launch_status();
+}
+
 }  // namespace
+
+int logprobs_device_status(bool reset) { return device_status_word(g_logprobs_status, reset); }
+
 }  // namespace cb200
 
 using namespace cb200;
@@ -114,18 +582,14 @@ extern "C" int cacheir_b200_token_logprobs(const void* logits, long long row_str
                                            int64_t* top_ids, float* top_logprobs, int rows, int vocab, int top, double temperature, int dtype,
                                            void* stream) {
   if (rows <= 0 || vocab <= 0) return 0;
-  if (!logits || (logprobs && !tokens) || top < 0 || (top > 0 && (!top_ids || !top_logprobs)) || !(temperature > 0.0) || temperature > 1e30 ||
-      temperature < 1e-30 || dtype_size(dtype) == 0 || (row_stride != 0 && row_stride < vocab && rows > 1))
+  if (!logits || (logprobs && !tokens) || top < 0 || (top > 0 && (!top_ids || !top_logprobs)) || !(temperature >= 1e-6) || temperature > 1e6 ||
+      dtype_size(dtype) == 0 || (row_stride != 0 && row_stride < vocab && rows > 1))
     return CACHEIR_B200_EINVAL;
-  if (top > CACHEIR_B200_MAX_TOP || top > vocab) return CACHEIR_B200_ELIMIT;
+  if (top > CACHEIR_B200_MAX_TOP || top > vocab || rows > 0x7fffffff / kMaxCluster) return CACHEIR_B200_ELIMIT;
+  if (!aligned_to(logits, dtype_size(dtype))) return CACHEIR_B200_EALIGN;
   if (row_stride == 0) row_stride = vocab;
-#define CB200_LOGPROBS(T)                                                                                                                    \
-  launch_chained(token_logprobs_kernel<T>, dim3(rows), dim3(kThreads), 0, as_stream(stream), static_cast<const T*>(logits), row_stride, tokens, \
-                 logprobs, entropy, top_ids, top_logprobs, vocab, top, 1.0 / temperature)
-  cudaError_t e;
-  if (dtype == CACHEIR_B200_F32) e = CB200_LOGPROBS(float);
-  else if (dtype == CACHEIR_B200_F16) e = CB200_LOGPROBS(__half);
-  else e = CB200_LOGPROBS(__nv_bfloat16);
-#undef CB200_LOGPROBS
-  return e != cudaSuccess ? static_cast<int>(e) : launch_status();
+  const Args a{logits, row_stride, tokens, logprobs, entropy, top_ids, top_logprobs, vocab, top, 1, 0, 1.0 / temperature};
+  if (dtype == CACHEIR_B200_F32) return launch_logprobs<float>(a, rows, as_stream(stream));
+  if (dtype == CACHEIR_B200_F16) return launch_logprobs<__half>(a, rows, as_stream(stream));
+  return launch_logprobs<__nv_bfloat16>(a, rows, as_stream(stream));
 }

@@ -375,8 +375,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, *, top: in
         raise ValueError("logits must be [R, V] with dense rows that do not overlap")
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must be 0 to {MAX_TOP} and no more than the vocabulary")
-    if not 1e-30 <= temperature <= 1e30:
-        raise ValueError("temperature must be positive")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError("temperature must be 1e-6 to 1e6")
     if tokens is not None and (tokens.dtype is not torch.int64 or tokens.numel() != rows or not tokens.is_contiguous()):
         raise ValueError("tokens must be contiguous int64 [R]")
     code, device = dtype_code(logits.dtype), logits.device

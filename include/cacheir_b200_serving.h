@@ -117,12 +117,14 @@ int cacheir_b200_shared_prefix_attention(const cacheir_b200_prefix_args* args, v
  * Stands beside cacheir_b200_argmax_rows (`argmax` of the reference's scheduler, cacheir/runtime/scheduler.py:456-478).
  * -inf is a masked value (probability 0). A row of nothing else has logprobs -inf and entropy 0. A row with NaN or +inf has NaN for both
  * and for top_logprobs; NaN is the largest value for top_ids. tokens[r] < 0: no token, logprobs 0; tokens[r] >= vocab: NaN.
- * logprobs (with tokens), entropy and the top pair may be NULL. top <= CACHEIR_B200_MAX_TOP (CACHEIR_B200_ELIMIT) and <= vocab. */
+ * logprobs (with tokens), entropy and the top pair may be NULL. 1e-6 <= temperature <= 1e6. top <= CACHEIR_B200_MAX_TOP and <= vocab, and
+ * with it rows of up to 4 MB (CACHEIR_B200_ELIMIT). */
 #define CACHEIR_B200_MAX_TOP 32
 int cacheir_b200_token_logprobs(const void* logits, long long row_stride, const int64_t* tokens, float* logprobs, float* entropy,
                                 int64_t* top_ids, float* top_logprobs, int rows, int vocab, int top, double temperature, int dtype,
                                 void* stream);
 
+/* First bounded wait of a kernel of this library that gave up on the current device (0: none); synchronises. */
 int cacheir_b200_serving_device_status(int reset);
 
 #ifdef __cplusplus
