@@ -10,8 +10,8 @@
 // that holds for any data, ties and masks included.
 //
 // Bound by memory for many rows (2048 x 128256 in bf16), by latency for few. A row is read by one block, or by a thread-block cluster where
-// there are few; every warp copies 2 KB pieces (bulk copies, a ring of its own: no barrier between warps) and has four to six of them on
-// their way. Per value that is half an instruction each for maximum and minimum, one to widen it, one for the exponent's argument, one
+// there are few; every warp copies 4 KB pieces (bulk copies, a ring of its own: no barrier between warps) and has two of them on
+// their way. Per value that is half an instruction for the maximum, one to widen it, one for the exponent's argument, one
 // exponential (16 a cycle and SM: 73 % of the memory's rate), half each for the two sums.
 #include "cacheir_b200_serving.h"
 #include "hybrid_common.cuh"
@@ -25,9 +25,9 @@ using namespace ptx;
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kTileBytes = 2048;           // of a warp's copy: 64 bytes a lane
-constexpr int kTopStages = 4, kSumStages = 6;
-constexpr int kMaxTiles = 256;             // of a block, where its groups' largest values are kept
+constexpr int kTileBytes = 4096;           // of a warp's copy: two groups a lane
+constexpr int kStages = 2;
+constexpr int kMaxTiles = 128;             // of a block, where its groups' largest values are kept
 constexpr int kMaxCluster = 8;
 constexpr int kList = 256;                 // candidates that are ranked against one another
 constexpr float kMasked = -1e30f;          // what is at or below it weighs nothing beside anything above it
@@ -44,7 +44,7 @@ struct Args {
   float* entropy;
   int64_t* top_ids;
   float* top_logprobs;
-  int vocab, top, cluster, stages;
+  int vocab, top, cluster;
   double inv_t;
 };
 
@@ -103,20 +103,18 @@ __device__ __forceinline__ f32x2 add2(f32x2 x, f32x2 y) {
   return d;
 }
 
-// 64 bytes of a row: largest (NaN if there is one) and smallest value, and its values two by two
+// 64 bytes of a row: largest value (NaN if there is one), and its values two by two
 template <typename T>
 struct Group;
 template <>
 struct Group<float> {
   static constexpr int kPairs = 8;
-  static __device__ __forceinline__ void range(const uint32_t (&w)[16], float& mx, float& mn) {
-    mx = __uint_as_float(w[0]);
-    mn = mx;
+  static __device__ __forceinline__ float largest(const uint32_t (&w)[16]) {
+    float mx = __uint_as_float(w[0]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) {
-      asm("max.NaN.f32 %0, %0, %1;" : "+f"(mx) : "f"(__uint_as_float(w[i])));
-      mn = fminf(mn, __uint_as_float(w[i]));
-    }
+    for (int i = 1; i < 15; i += 2) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(mx) : "f"(__uint_as_float(w[i])), "f"(__uint_as_float(w[i + 1])));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(mx) : "f"(__uint_as_float(w[15])));
+    return mx;
   }
   static __device__ __forceinline__ void two(const uint32_t (&w)[16], int i, float& lo, float& hi) { lo = __uint_as_float(w[2 * i]); hi = __uint_as_float(w[2 * i + 1]); }
   static constexpr uint32_t kNothing = 0xff800000u;       // -inf
@@ -124,15 +122,11 @@ struct Group<float> {
 template <>
 struct Group<__half> {
   static constexpr int kPairs = 16;
-  static __device__ __forceinline__ void range(const uint32_t (&w)[16], float& mx, float& mn) {
-    __half2 hi = *reinterpret_cast<const __half2*>(&w[0]), lo = hi;
+  static __device__ __forceinline__ float largest(const uint32_t (&w)[16]) {
+    __half2 mx = *reinterpret_cast<const __half2*>(&w[0]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) {
-      hi = __hmax2_nan(hi, *reinterpret_cast<const __half2*>(&w[i]));
-      lo = __hmin2(lo, *reinterpret_cast<const __half2*>(&w[i]));
-    }
-    mx = __half2float(__hmax_nan(__low2half(hi), __high2half(hi)));
-    mn = __half2float(__hmin(__low2half(lo), __high2half(lo)));
+    for (int i = 1; i < 16; ++i) mx = __hmax2_nan(mx, *reinterpret_cast<const __half2*>(&w[i]));
+    return __half2float(__hmax_nan(__low2half(mx), __high2half(mx)));
   }
   static __device__ __forceinline__ void two(const uint32_t (&w)[16], int i, float& lo, float& hi) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
@@ -144,15 +138,11 @@ struct Group<__half> {
 template <>
 struct Group<__nv_bfloat16> {
   static constexpr int kPairs = 16;
-  static __device__ __forceinline__ void range(const uint32_t (&w)[16], float& mx, float& mn) {
-    __nv_bfloat162 hi = *reinterpret_cast<const __nv_bfloat162*>(&w[0]), lo = hi;
+  static __device__ __forceinline__ float largest(const uint32_t (&w)[16]) {
+    __nv_bfloat162 mx = *reinterpret_cast<const __nv_bfloat162*>(&w[0]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) {
-      hi = __hmax2_nan(hi, *reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-      lo = __hmin2(lo, *reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-    }
-    mx = __bfloat162float(__hmax_nan(__low2bfloat16(hi), __high2bfloat16(hi)));
-    mn = __bfloat162float(__hmin(__low2bfloat16(lo), __high2bfloat16(lo)));
+    for (int i = 1; i < 16; ++i) mx = __hmax2_nan(mx, *reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+    return __bfloat162float(__hmax_nan(__low2bfloat16(mx), __high2bfloat16(mx)));
   }
   static __device__ __forceinline__ void two(const uint32_t (&w)[16], int i, float& lo, float& hi) {
     lo = __uint_as_float(w[i] << 16);
@@ -168,13 +158,13 @@ __device__ __forceinline__ uint32_t ld_rank_u32(const void* local, uint32_t rank
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 3)
 token_logprobs_kernel(const __grid_constant__ Args p) {
   chain_enter();
   using G = Group<T>;
   constexpr int kGroup = 64 / sizeof(T), kTile = kTileBytes / sizeof(T), kVec = 16 / sizeof(T);
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t s_bar[kWarps * kSumStages];
+  __shared__ uint64_t s_bar[kWarps * kStages];
   __shared__ Sums s_sums[kWarps];
   __shared__ int s_flags[kWarps];
   __shared__ Sums s_block;
@@ -192,9 +182,9 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
   const int head = min(p.vocab, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T)));
   const int body = (p.vocab - head) / kVec * kVec, tail = p.vocab - head - body, all_tiles = (body + kTile - 1) / kTile;
   const int per_block = (all_tiles + p.cluster - 1) / p.cluster, tile0 = min(all_tiles, rank * per_block), tiles = min(all_tiles, tile0 + per_block) - tile0;
-  uint8_t* ring = smem + warp * p.stages * kTileBytes;
-  float* s_max = reinterpret_cast<float*>(smem + kWarps * p.stages * kTileBytes);      // [tiles * 32 groups], with `top` only
-  const uint32_t bar = smem_u32(&s_bar[warp * kSumStages]);
+  uint8_t* ring = smem + warp * kStages * kTileBytes;
+  float* s_max = reinterpret_cast<float*>(smem + kWarps * kStages * kTileBytes);      // [tiles * 64 groups], with `top` only
+  const uint32_t bar = smem_u32(&s_bar[warp * kStages]);
   const float c = static_cast<float>(p.inv_t * 1.4426950408889634);
 
   const int mine = warp < tiles ? (tiles - warp + kWarps - 1) / kWarps : 0;            // this warp's tiles: warp + i * kWarps
@@ -205,9 +195,9 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
     bulk_load(smem_u32(ring + s * kTileBytes), x + head + static_cast<size_t>(tile0 + warp + i * kWarps) * kTile, n, bar + s * 8);
   };
   if (lane == 0) {
-    for (int s = 0; s < p.stages; ++s) mbar_init(bar + s * 8, 1);
+    for (int s = 0; s < kStages; ++s) mbar_init(bar + s * 8, 1);
     mbar_fence_init();
-    for (int s = 0; s < p.stages && s < mine; ++s) copy(s, s);
+    for (int s = 0; s < kStages && s < mine; ++s) copy(s, s);
   }
   __syncwarp();
 
@@ -237,60 +227,69 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
 #pragma unroll 1
   for (int i = 0; i < mine; ++i) {
     if (!__all_sync(0xffffffffu, mbar_wait(bar + stage * 8, phase, &g_logprobs_status, (16 << 8) | 1))) {
-      for (int k = i + 1; k < min(mine, i + p.stages); ++k) {        // the copies that are still under way
-        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      for (int k = i + 1; k < min(mine, i + kStages); ++k) {        // the copies that are still under way
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
         mbar_wait(bar + stage * 8, phase, &g_logprobs_status, (16 << 8) | 2);
       }
       flags |= 1;                                          // (the row's results are no numbers)
       break;
     }
-    uint32_t w[16];
     const int n16 = bytes_of(i) / 16;
+    const uint8_t* tile = ring + stage * kTileBytes;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = lane * 4 + ((j + (lane >> 1)) & 3);   // (in an order in which eight lanes reach all banks)
-      const uint4 v = *reinterpret_cast<const uint4*>(ring + stage * kTileBytes + at * 16);
-      w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
-      if (at >= n16) w[4 * j] = w[4 * j + 1] = w[4 * j + 2] = w[4 * j + 3] = G::kNothing;
-    }
-    __syncwarp();
-    if (lane == 0 && i + p.stages < mine) copy(i + p.stages, stage);
-    if (++stage == p.stages) { stage = 0; phase ^= 1; }
-    float mx, mn;
-    G::range(w, mx, mn);
-    if (p.top > 0) s_max[(warp + i * kWarps) * 32 + lane] = mx;
-    const bool plain = mx < kHuge && mn > kMasked;
-    if (__all_sync(0xffffffffu, plain)) {
-      if (mx > m) rescale(mx);
-      const f32x2 c2 = pair(c, c), less = pair(-m, -m);
+    for (int half = 0; half < 2; ++half) {                 // a lane has 128 bytes: two groups
+      const int which = half ^ (lane >> 2 & 1);
+      uint32_t w[16];
 #pragma unroll
-      for (int k = 0; k < G::kPairs; ++k) {
-        float lo, hi, y0, y1;
-        G::two(w, k, lo, hi);
-        const f32x2 y = mul2(add2(pair(lo, hi), less), c2);
-        unpair(y, y0, y1);
-        const f32x2 e = pair(ex2(y0), ex2(y1));
-        z2 = add2(z2, e);
-        s2 = fma2(e, y, s2);
+      for (int j = 0; j < 4; ++j) {
+        const int at = lane * 8 + which * 4 + ((j + lane) & 3);        // (in an order in which eight lanes reach all banks)
+        const uint4 v = *reinterpret_cast<const uint4*>(tile + at * 16);
+        w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+        if (at >= n16) w[4 * j] = w[4 * j + 1] = w[4 * j + 2] = w[4 * j + 3] = G::kNothing;
       }
-    } else if (!(mx < kHuge)) {
-      flags |= mx < INFINITY ? 2 : 1;
-    } else if (mx <= kMasked) {
-      if (mx > -INFINITY) flags |= 4;
-    } else {
-      if (mx > m) rescale(mx);
-      const f32x2 c2 = pair(c, c), less = pair(-m, -m);
+      if (half == 1) {
+        __syncwarp();
+        if (lane == 0 && i + kStages < mine) copy(i + kStages, stage);
+      }
+      const float mx = G::largest(w);
+      if (p.top > 0) s_max[((warp + i * kWarps) * 32 + lane) * 2 + which] = mx;
+      if (!(mx < kHuge)) {
+        flags |= mx < INFINITY ? 2 : 1;
+      } else if (mx <= kMasked) {
+        if (mx > -INFINITY) flags |= 4;
+      } else {
+        if (mx > m) rescale(mx);
+        const f32x2 c2 = pair(c, c), less = pair(-m, -m);
+        f32x2 gz[2] = {0ull, 0ull}, gs[2] = {0ull, 0ull};
 #pragma unroll
-      for (int k = 0; k < G::kPairs; ++k) {
-        float lo, hi, y0, y1;
-        G::two(w, k, lo, hi);
-        const f32x2 y = mul2(add2(pair(fmaxf(lo, kMasked), fmaxf(hi, kMasked)), less), c2);
-        unpair(y, y0, y1);
-        const f32x2 e = pair(ex2(y0), ex2(y1));
-        z2 = add2(z2, e);
-        s2 = fma2(e, y, s2);
+        for (int k = 0; k < G::kPairs; ++k) {
+          float lo, hi, y0, y1;
+          G::two(w, k, lo, hi);
+          const f32x2 y = mul2(add2(pair(lo, hi), less), c2);
+          unpair(y, y0, y1);
+          const f32x2 e = pair(ex2(y0), ex2(y1));
+          gz[k & 1] = add2(gz[k & 1], e);
+          gs[k & 1] = fma2(e, y, gs[k & 1]);
+        }
+        gs[0] = add2(gs[0], gs[1]);
+        float s0, s1;
+        unpair(gs[0], s0, s1);
+        if (!(s0 + s1 == s0 + s1)) {                       // a masked value: its weight of 0 times -inf is no number
+          gs[0] = 0ull;
+#pragma unroll
+          for (int k = 0; k < G::kPairs; ++k) {
+            float lo, hi, y0, y1;
+            G::two(w, k, lo, hi);
+            const f32x2 y = mul2(add2(pair(fmaxf(lo, kMasked), fmaxf(hi, kMasked)), less), c2);
+            unpair(y, y0, y1);
+            gs[0] = fma2(pair(ex2(y0), ex2(y1)), y, gs[0]);
+          }
+        }
+        z2 = add2(z2, add2(gz[0], gz[1]));
+        s2 = add2(s2, gs[0]);
       }
     }
+    if (++stage == kStages) { stage = 0; phase ^= 1; }
   }
   // the single values of both ends: lanes of the first block's first warp, of the last block's
   if (warp == 0 && rank == 0 && lane < head) add_one(Elem<T>::ld(x + lane));
@@ -324,10 +323,10 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
   // ---- the block's likeliest `top` ----
   if (p.top > 0) {
     const int top = p.top, ends = (rank == 0 && head > 0 ? 1 : 0) + (rank == p.cluster - 1 && tail > 0 ? 1 : 0);
-    const int first = rank == 0 && head > 0 ? 1 : 0, groups = tiles * 32 + ends;       // in order: the head, those of the tiles, the tail
+    const int first = rank == 0 && head > 0 ? 1 : 0, groups = tiles * 64 + ends;       // in order: the head, those of the tiles, the tail
     unsigned long long* s_list = reinterpret_cast<unsigned long long*>(smem);          // [kList], over the rings
     auto value_of = [&](int g) -> uint32_t {
-      if (g >= first && g - first < tiles * 32) {
+      if (g >= first && g - first < tiles * 64) {
         // (group g - first of the tiles; those behind the last value hold none)
         return tile0 * kTile + (g - first) * kGroup < body ? ordered_bits(s_max[g - first]) : 0u;
       }
@@ -337,7 +336,7 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
       return best;
     };
     auto range_of = [&](int g, int* from) {                // its values
-      if (g >= first && g - first < tiles * 32) {
+      if (g >= first && g - first < tiles * 64) {
         const int at = tile0 * kTile + (g - first) * kGroup;
         *from = head + at;
         return min(kGroup, body - at);
@@ -540,14 +539,14 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
   }
 }
 
-// Blocks for a row: as many waves of them as there are places (two on an SM), each as long as its tiles and what begins and ends it, about
-// 24 tiles' time.
+// Blocks for a row: as many waves of them as there are places (three on an SM), each as long as its tiles and what begins and ends it, about
+// 12 tiles' time.
 int cluster_of(int rows, int tiles, int least) {
   int best = least;
   long long shortest = -1;
   for (int n = least; n <= kMaxCluster; n *= 2) {
-    const long long waves = (static_cast<long long>(rows) * n + 2 * kNumSMs - 1) / (2 * kNumSMs);
-    const long long time = waves * ((tiles + n - 1) / n + 24);
+    const long long waves = (static_cast<long long>(rows) * n + 3 * kNumSMs - 1) / (3 * kNumSMs);
+    const long long time = waves * ((tiles + n - 1) / n + 12);
     if (shortest < 0 || time < shortest) { shortest = time; best = n; }
   }
   return best;
@@ -561,9 +560,9 @@ int launch_logprobs(Args a, int rows, cudaStream_t stream) {
     while (least < kMaxCluster && tiles > static_cast<long long>(least) * kMaxTiles) least *= 2;
   if (a.top > 0 && tiles > static_cast<long long>(least) * kMaxTiles) return CACHEIR_B200_ELIMIT;
   a.cluster = cluster_of(rows, static_cast<int>(tiles), least);
-  a.stages = a.top > 0 ? kTopStages : kSumStages;
+
   const int per_block = static_cast<int>((tiles + a.cluster - 1) / a.cluster);
-  const size_t smem = static_cast<size_t>(kWarps) * a.stages * kTileBytes + (a.top > 0 ? static_cast<size_t>(per_block) * 32 * 4 : 0);
+  const size_t smem = static_cast<size_t>(kWarps) * kStages * kTileBytes + (a.top > 0 ? static_cast<size_t>(per_block) * 64 * 4 : 0);
   auto kern = token_logprobs_kernel<T>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e == cudaSuccess) e = launch_clusters(kern, dim3(static_cast<unsigned>(rows) * a.cluster), dim3(kThreads), smem, stream, dim3(a.cluster), a);
@@ -588,7 +587,7 @@ extern "C" int cacheir_b200_token_logprobs(const void* logits, long long row_str
   if (top > CACHEIR_B200_MAX_TOP || top > vocab || rows > 0x7fffffff / kMaxCluster) return CACHEIR_B200_ELIMIT;
   if (!aligned_to(logits, dtype_size(dtype))) return CACHEIR_B200_EALIGN;
   if (row_stride == 0) row_stride = vocab;
-  const Args a{logits, row_stride, tokens, logprobs, entropy, top_ids, top_logprobs, vocab, top, 1, 0, 1.0 / temperature};
+  const Args a{logits, row_stride, tokens, logprobs, entropy, top_ids, top_logprobs, vocab, top, 1, 1.0 / temperature};
   if (dtype == CACHEIR_B200_F32) return launch_logprobs<float>(a, rows, as_stream(stream));
   if (dtype == CACHEIR_B200_F16) return launch_logprobs<__half>(a, rows, as_stream(stream));
   return launch_logprobs<__nv_bfloat16>(a, rows, as_stream(stream));
