@@ -57,14 +57,13 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b, float c) {
-  if (b.m == -INFINITY) return a;
-  if (a.m == -INFINITY) return b;
+// The lanes' sums as one, in every lane.
+__device__ __forceinline__ Sums joined(const Sums& a, float c) {
   Sums r;
-  r.m = fmaxf(a.m, b.m);
-  const float da = fmaxf((a.m - r.m) * c, kFar), db = fmaxf((b.m - r.m) * c, kFar), wa = ex2(da), wb = ex2(db);
-  r.z = a.z * wa + b.z * wb;
-  r.s = (a.s + da * a.z) * wa + (b.s + db * b.z) * wb;
+  r.m = warp_max(a.m);
+  const float d = a.m > -INFINITY ? fmaxf((a.m - r.m) * c, kFar) : kFar, w = ex2(d);
+  r.z = warp_sum(a.z * w);
+  r.s = warp_sum((a.s + d * a.z) * w);
   return r;
 }
 
@@ -156,6 +155,11 @@ __device__ __forceinline__ uint32_t ld_rank_u32(const void* local, uint32_t rank
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(map_to_rank(smem_u32(local), rank)) : "memory");
   return v;
 }
+__device__ __forceinline__ unsigned long long ld_rank_u64(const void* local, uint32_t rank) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(map_to_rank(smem_u32(local), rank)) : "memory");
+  return v;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 3)
@@ -170,7 +174,7 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
   __shared__ Sums s_block;
   __shared__ int s_block_flags;
   __shared__ unsigned long long s_top[CACHEIR_B200_MAX_TOP];
-  __shared__ __align__(16) uint32_t s_best[kThreads];     // (read four at a time)
+  __shared__ uint32_t s_warp_bound[kWarps];
   __shared__ uint32_t s_bound;
   __shared__ int s_count;
   __shared__ int s_selected[CACHEIR_B200_MAX_TOP];
@@ -183,7 +187,7 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
   const int body = (p.vocab - head) / kVec * kVec, tail = p.vocab - head - body, all_tiles = (body + kTile - 1) / kTile;
   const int per_block = (all_tiles + p.cluster - 1) / p.cluster, tile0 = min(all_tiles, rank * per_block), tiles = min(all_tiles, tile0 + per_block) - tile0;
   uint8_t* ring = smem + warp * kStages * kTileBytes;
-  float* s_max = reinterpret_cast<float*>(smem + kWarps * kStages * kTileBytes);      // [tiles * 64 groups], with `top` only
+  uint32_t* s_max = reinterpret_cast<uint32_t*>(smem + kWarps * kStages * kTileBytes);      // [tiles * 64 groups] ordered, with `top` only
   const uint32_t bar = smem_u32(&s_bar[warp * kStages]);
   const float c = static_cast<float>(p.inv_t * 1.4426950408889634);
 
@@ -201,6 +205,8 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
   }
   __syncwarp();
 
+  const bool asks = warp == 0 && rank == 0 && p.logprobs;
+  const int64_t token = asks ? p.tokens[row] : -1;         // (on its way beside the row's first pieces, its value beside the sums)
   float m = -INFINITY;
   f32x2 z2 = 0ull, s2 = 0ull;                              // (both halves)
   int flags = 0;                                           // 1: NaN or +inf, 2: values beyond kHuge, 4: some at or below kMasked that are not -inf
@@ -252,7 +258,7 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
         if (lane == 0 && i + kStages < mine) copy(i + kStages, stage);
       }
       const float mx = G::largest(w);
-      if (p.top > 0) s_max[((warp + i * kWarps) * 32 + lane) * 2 + which] = mx;
+      if (p.top > 0) s_max[((warp + i * kWarps) * 32 + lane) * 2 + which] = lane * 8 + which * 4 < n16 ? ordered_bits(mx) : 0u;
       if (!(mx < kHuge)) {
         flags |= mx < INFINITY ? 2 : 1;
       } else if (mx <= kMasked) {
@@ -291,6 +297,7 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
     }
     if (++stage == kStages) { stage = 0; phase ^= 1; }
   }
+  const float asked = token >= 0 && token < p.vocab ? Elem<T>::ld(x + token) : 0.f;
   // the single values of both ends: lanes of the first block's first warp, of the last block's
   if (warp == 0 && rank == 0 && lane < head) add_one(Elem<T>::ld(x + lane));
   if (warp == 0 && rank == p.cluster - 1 && lane < tail) add_one(Elem<T>::ld(x + head + body + lane));
@@ -303,21 +310,15 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
     unpair(s2, s0, s1);
     a = Sums{m, z0 + z1, s0 + s1};
   }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const Sums o{__shfl_xor_sync(0xffffffffu, a.m, off), __shfl_xor_sync(0xffffffffu, a.z, off), __shfl_xor_sync(0xffffffffu, a.s, off)};
-    a = lane & off ? joined(o, a, c) : joined(a, o, c);
-  }
+  a = joined(a, c);
   flags = __reduce_or_sync(0xffffffffu, flags);
   if (lane == 0) { s_sums[warp] = a; s_flags[warp] = flags; }
   if (threadIdx.x == 0) s_count = 0;
   __syncthreads();                                         // (the rings are drained)
-  if (threadIdx.x == 0) {
-    a = s_sums[0];
-    flags = s_flags[0];
-    for (int w = 1; w < kWarps; ++w) { a = joined(a, s_sums[w], c); flags |= s_flags[w]; }
-    s_block = a;
-    s_block_flags = flags;
+  if (warp == 0) {
+    a = joined(lane < kWarps ? s_sums[lane] : Sums{-INFINITY, 0.f, 0.f}, c);
+    flags = __reduce_or_sync(0xffffffffu, lane < kWarps ? s_flags[lane] : 0);
+    if (lane == 0) { s_block = a; s_block_flags = flags; }
   }
 
   // ---- the block's likeliest `top` ----
@@ -326,10 +327,7 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
     const int first = rank == 0 && head > 0 ? 1 : 0, groups = tiles * 64 + ends;       // in order: the head, those of the tiles, the tail
     unsigned long long* s_list = reinterpret_cast<unsigned long long*>(smem);          // [kList], over the rings
     auto value_of = [&](int g) -> uint32_t {
-      if (g >= first && g - first < tiles * 64) {
-        // (group g - first of the tiles; those behind the last value hold none)
-        return tile0 * kTile + (g - first) * kGroup < body ? ordered_bits(s_max[g - first]) : 0u;
-      }
+      if (g >= first && g - first < tiles * 64) return s_max[g - first];
       const bool front = g < first;
       uint32_t best = 0;
       for (int i = 0; i < (front ? head : tail); ++i) best = max(best, ordered_bits(Elem<T>::ld(x + (front ? 0 : head + body) + i)));
@@ -343,6 +341,14 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
       }
       *from = g < first ? 0 : head + body;
       return g < first ? head : tail;
+    };
+    auto list = [&](bool wanted, unsigned long long key) { // (a whole warp; any order: they are ranked)
+      const uint32_t who = __ballot_sync(0xffffffffu, wanted);
+      if (who == 0) return;
+      int at = 0;
+      if (lane == __ffs(who) - 1) at = atomicAdd(&s_count, __popc(who));
+      at = __shfl_sync(0xffffffffu, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1));
+      if (wanted && at < kList) s_list[at] = key;
     };
     // the largest key below `last` that anybody offers (the slow way, for lists that do not fit)
     auto next_best = [&](unsigned long long best) {
@@ -358,27 +364,23 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
         if (s_round[w] > best) best = s_round[w];
       return best;
     };
-    // A bound from below: of the threads' best groups the `top`-th.
+    // A bound from below that `top` groups reach: every warp's share of them among its lanes' best ones, and the least of that.
     uint32_t best = 0;
     for (int g = threadIdx.x; g < groups; g += kThreads) best = max(best, value_of(g));
-    s_best[threadIdx.x] = best;
+    uint32_t nth = 0;
+    for (int k = 0; k < (top + kWarps - 1) / kWarps; ++k) {
+      nth = __reduce_max_sync(0xffffffffu, best);
+      if (lane == __ffs(__ballot_sync(0xffffffffu, best == nth)) - 1) best = 0;
+    }
+    if (lane == 0) s_warp_bound[warp] = nth;
     if (threadIdx.x < CACHEIR_B200_MAX_TOP) { s_selected[threadIdx.x] = -1; s_top[threadIdx.x] = 0; }
     __syncthreads();
-    int ahead = 0;
-    for (int i = 0; i < kThreads; i += 4) {
-      const uint4 o = *reinterpret_cast<const uint4*>(&s_best[i]);
-      ahead += (o.x > best || (o.x == best && i < static_cast<int>(threadIdx.x))) + (o.y > best || (o.y == best && i + 1 < static_cast<int>(threadIdx.x))) +
-               (o.z > best || (o.z == best && i + 2 < static_cast<int>(threadIdx.x))) + (o.w > best || (o.w == best && i + 3 < static_cast<int>(threadIdx.x)));
-    }
-    if (ahead == top - 1) s_bound = best;
-    __syncthreads();
-    const uint32_t bound = s_bound;
-    for (int g = threadIdx.x; g < groups; g += kThreads) {
-      const uint32_t v = value_of(g);
-      if (v >= bound && v > 0) {
-        const int at = atomicAdd(&s_count, 1);             // (any order: they are ranked)
-        if (at < kList) s_list[at] = key_of(v, g);
-      }
+    uint32_t bound = s_warp_bound[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) bound = min(bound, s_warp_bound[w]);
+    for (int g = threadIdx.x; g - lane < groups; g += kThreads) {
+      const uint32_t v = g < groups ? value_of(g) : 0u;
+      list(v >= bound && v > 0, key_of(v, g));
     }
     __syncthreads();
     const int found = s_count;
@@ -418,16 +420,15 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int at = threadIdx.x + j * kThreads, k = at / kGroup, e = at % kGroup;
-      keys[j] = 0;
-      if (k >= top || s_selected[k] < 0) continue;
       int from;
-      if (e >= range_of(s_selected[k], &from)) continue;
-      const uint32_t v = ordered_bits(Elem<T>::ld(x + from + e));
-      if (v < least) continue;
-      keys[j] = key_of(v, from + e);
-      const int place = atomicAdd(&s_count, 1);
-      if (place < kList) s_list[place] = keys[j];
+      keys[j] = 0;
+      if (k < top && s_selected[k] >= 0 && e < range_of(s_selected[k], &from)) {
+        const uint32_t v = ordered_bits(Elem<T>::ld(x + from + e));
+        if (v >= least) keys[j] = key_of(v, from + e);
+      }
     }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) list(keys[j] > 0, keys[j]);
     __syncthreads();
     const int values = s_count;
     if (values <= kList) {
@@ -454,12 +455,14 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
   __syncthreads();
   if (p.cluster > 1) cluster_sync_release();
   if (rank == 0) {
-    a = s_block;
-    flags = s_block_flags;
-    for (int r = 1; r < p.cluster; ++r) {
-      const Sums o{__uint_as_float(ld_rank_u32(&s_block.m, r)), __uint_as_float(ld_rank_u32(&s_block.z, r)), __uint_as_float(ld_rank_u32(&s_block.s, r))};
-      a = joined(a, o, c);
-      flags |= static_cast<int>(ld_rank_u32(&s_block_flags, r));
+    if (p.cluster > 1) {
+      const Sums o{__uint_as_float(ld_rank_u32(&s_block.m, lane % p.cluster)), __uint_as_float(ld_rank_u32(&s_block.z, lane % p.cluster)),
+                   __uint_as_float(ld_rank_u32(&s_block.s, lane % p.cluster))};
+      a = joined(lane < p.cluster ? o : Sums{-INFINITY, 0.f, 0.f}, c);
+      flags = __reduce_or_sync(0xffffffffu, static_cast<int>(ld_rank_u32(&s_block_flags, lane % p.cluster)));
+    } else {
+      a = s_block;
+      flags = s_block_flags;
     }
     double log_z = 0.0, entropy = 0.0;
     const bool nan = (flags & 1) != 0;
@@ -491,8 +494,9 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
     } else if (!nan && a.m == -INFINITY) {
       empty = true;
     } else if (!nan) {
-      log_z = log(static_cast<double>(a.z));
-      entropy = log_z - 0.6931471805599453 * static_cast<double>(a.s) / static_cast<double>(a.z);
+      const float lz = logf(a.z);
+      log_z = lz;
+      entropy = lz - 0.6931471805599453f * (a.s / a.z);
     }
     auto log_p = [&](float v) {
       if (nan) return static_cast<float>(NAN);
@@ -501,8 +505,7 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
     };
     if (threadIdx.x == 0) {
       if (p.logprobs) {
-        const int64_t t = p.tokens[row];
-        p.logprobs[row] = t < 0 ? 0.f : t >= p.vocab ? static_cast<float>(NAN) : log_p(Elem<T>::ld(x + t));
+        p.logprobs[row] = token < 0 ? 0.f : token >= p.vocab ? static_cast<float>(NAN) : log_p(asked);
       }
       if (p.entropy) p.entropy[row] = nan ? static_cast<float>(NAN) : empty ? 0.f : static_cast<float>(entropy);
     }
@@ -516,8 +519,7 @@ token_logprobs_kernel(const __grid_constant__ Args p) {
         const int n = p.cluster * p.top;
         for (int i = threadIdx.x; i < n; i += kThreads) {
           const int r = i / p.top, k = i % p.top;
-          const uint32_t* from = reinterpret_cast<const uint32_t*>(&s_top[k]);
-          s_list[i] = static_cast<unsigned long long>(ld_rank_u32(from + 1, r)) << 32 | ld_rank_u32(from, r);
+          s_list[i] = ld_rank_u64(&s_top[k], r);
         }
         __syncthreads();
         if (static_cast<int>(threadIdx.x) < n) {
