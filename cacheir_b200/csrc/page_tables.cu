@@ -5,9 +5,11 @@
 // sums over the sequences, of rows and of pages, say where its rows stand and which pages of the stack are its own; everything else is
 // then independent: a page goes to its place in a table, a row finds its sequence by bisection in the row sums.
 //
-// Little data (12 bytes a row, 8 a page, 12 a sequence) and much latency: read lengths, sum, look up, write. So it is one launch. A call
-// changes what it reads (lengths, stack height), so all reads of those come before all writes: the blocks are one thread-block cluster,
-// each of which sums all sequences by itself, and meet once in between.
+// Little data (12 bytes a row, 8 a page, 12 a sequence) and much latency: read lengths, sum, look up, write. So it is one launch, of one block
+// where there is little to do. A call changes what it reads (lengths, stack height), so all reads of those come before all writes: the
+// blocks are one thread-block cluster, each of which sums all sequences by itself, and meet once in between. Many rows (above 2048) are left
+// to a second kernel on all SMs, which needs only what the first one leaves: 1024 sequences with 0 to 255 new tokens each in 140001
+// rows and the way back took 40.6 us with the rows in one cluster of eight blocks and the way back in one block, 15.5 us like this.
 #include "cacheir_b200_serving.h"
 #include "common.cuh"
 #include "tc_ptx.cuh"
@@ -17,6 +19,8 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kClusterBlocks = 8;
+constexpr int kOwnRows = 2048;              // rows that the first kernel takes itself
+constexpr int kRowsPerWarp = 128;
 
 struct TableArgs {
   int32_t* page_table;
@@ -31,6 +35,7 @@ struct TableArgs {
   int32_t* cu_rows;
   int32_t* status;
   int sequences, max_pages, page_size, capacity, rows;
+  int fills;                  // extend: the rows are filled in here
 };
 
 __device__ __forceinline__ int pages_of(long long tokens, int page_size) { return static_cast<int>((tokens + page_size - 1) / page_size); }
@@ -170,7 +175,7 @@ page_tables_kernel(const TableArgs p) {
   // ---- rows ----
   if constexpr (EXTEND) {
     const int used = why == 0 ? static_cast<int>(total[0]) : 0;
-    for (int r = thread; r < p.rows; r += threads) {
+    for (int r = thread; r < (p.fills ? p.rows : 0); r += threads) {
       int pos = 0, b = -1, slot = -1;
       if (r < used) {
         b = owner(s_row, n, r);
@@ -186,14 +191,79 @@ page_tables_kernel(const TableArgs p) {
   }
 }
 
+// The rows of a call whose sequences have been dealt with: 128 neighbours a warp, four a lane.
+__global__ void __launch_bounds__(256)
+token_rows_kernel(const TableArgs p) {
+  chain_enter();
+  const int lane = threadIdx.x & 31, first = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kRowsPerWarp, r0 = first + lane * 4;
+  if (first >= p.rows) return;
+  const int n = p.sequences, used = p.cu_rows[n];
+  int pos[4] = {0, 0, 0, 0}, seq[4] = {-1, -1, -1, -1}, slot[4] = {-1, -1, -1, -1};
+  if (first < used) {
+    // The sequence of the warp's first row: the starts up to it are counted, 32 of them looked at at a time.
+    int lo = 0, hi = n;
+    while (hi > lo) {
+      const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+      const int below = __popc(__ballot_sync(0xffffffffu, at < hi && p.cu_rows[at] <= first));
+      if (below == 0) break;
+      const int found = lo + (below - 1) * step;
+      hi = min(hi, found + step);
+      lo = found + 1;
+    }
+    const int base = lo - 1, last = min(first + kRowsPerWarp, used) - 1;
+    int count[4] = {base, base, base, base};
+    for (int b = base + 1; b < n; b += 32) {               // .. and of the others: the starts behind that
+      const int start = b + lane < n ? p.cu_rows[b + lane] : 0x7fffffff;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int s = __shfl_sync(0xffffffffu, start, i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) count[j] += s <= r0 + j ? 1 : 0;
+      }
+      if (__shfl_sync(0xffffffffu, start, 31) > last) break;
+    }
+    int end[4], len[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      end[j] = r0 + j < used ? p.cu_rows[count[j] + 1] : 0;
+      len[j] = r0 + j < used ? p.seq_lens[count[j]] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (r0 + j < used) {
+        seq[j] = count[j];
+        pos[j] = len[j] - (end[j] - (r0 + j));
+        slot[j] = p.page_table[static_cast<size_t>(seq[j]) * p.max_pages + pos[j] / p.page_size] * p.page_size + pos[j] % p.page_size;
+      }
+  }
+  const bool wide = ((reinterpret_cast<uintptr_t>(p.positions) | reinterpret_cast<uintptr_t>(p.row_seq) | reinterpret_cast<uintptr_t>(p.slots)) & 15) == 0;
+  if (wide && r0 + 4 <= p.rows) {
+    *reinterpret_cast<int4*>(p.positions + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+    *reinterpret_cast<int4*>(p.row_seq + r0) = make_int4(seq[0], seq[1], seq[2], seq[3]);
+    *reinterpret_cast<int4*>(p.slots + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (r0 + j < p.rows) {
+        p.positions[r0 + j] = pos[j];
+        p.row_seq[r0 + j] = seq[j];
+        p.slots[r0 + j] = slot[j];
+      }
+  }
+}
+
 template <bool EXTEND>
-int launch_tables(const TableArgs& a, int blocks, cudaStream_t stream) {
+int launch_tables(const TableArgs& a, cudaStream_t stream) {
   const size_t smem = static_cast<size_t>(a.sequences) * (EXTEND ? 3 : 2) * 4;
   if (smem > 40 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(page_tables_kernel<EXTEND>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  const cudaError_t e = launch_clusters(page_tables_kernel<EXTEND>, dim3(blocks), dim3(kThreads), smem, stream, dim3(blocks), a);
+  const bool few = a.sequences <= 128 && (!EXTEND || a.rows <= 512);
+  const int blocks = a.sequences > 256 || (EXTEND && a.rows > 1024) ? kClusterBlocks : 1;
+  cudaError_t e = launch_clusters(page_tables_kernel<EXTEND>, dim3(blocks), dim3(few ? 128 : kThreads), smem, stream, dim3(blocks), a);
+  if (EXTEND && !a.fills && e == cudaSuccess)
+    e = launch_chained(token_rows_kernel, dim3((a.rows + 8 * kRowsPerWarp - 1) / (8 * kRowsPerWarp)), dim3(256), 0, stream, a);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }
 
@@ -212,8 +282,8 @@ extern "C" int cacheir_b200_extend_page_tables(int32_t* page_table, int32_t* seq
     return CACHEIR_B200_EINVAL;
   if (sequences > CACHEIR_B200_MAX_SEQUENCES || static_cast<long long>(max_pages) * page_size > 0x7fffffffLL) return CACHEIR_B200_ELIMIT;
   TableArgs a{page_table, seq_lens, new_lens, nullptr, const_cast<int32_t*>(free_pages), free_count, positions, row_seq, slots, cu_rows, status,
-              sequences, max_pages, page_size, capacity, rows};
-  return launch_tables<true>(a, rows > 2 * kThreads ? kClusterBlocks : 1, as_stream(stream));
+              sequences, max_pages, page_size, capacity, rows, rows <= kOwnRows ? 1 : 0};
+  return launch_tables<true>(a, as_stream(stream));
 }
 
 extern "C" int cacheir_b200_shrink_page_tables(const int32_t* page_table, int32_t* seq_lens, const int32_t* keep_lens, const int32_t* held_pages,
@@ -224,6 +294,6 @@ extern "C" int cacheir_b200_shrink_page_tables(const int32_t* page_table, int32_
     return CACHEIR_B200_EINVAL;
   if (sequences > CACHEIR_B200_MAX_SEQUENCES || static_cast<long long>(max_pages) * page_size > 0x7fffffffLL) return CACHEIR_B200_ELIMIT;
   TableArgs a{const_cast<int32_t*>(page_table), seq_lens, keep_lens, held_pages, free_pages, free_count, nullptr, nullptr, nullptr, nullptr, status,
-              sequences, max_pages, page_size, capacity, 0};
-  return launch_tables<false>(a, 1, as_stream(stream));
+              sequences, max_pages, page_size, capacity, 0, 0};
+  return launch_tables<false>(a, as_stream(stream));
 }

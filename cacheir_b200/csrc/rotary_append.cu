@@ -7,15 +7,17 @@
 // position of a million has an angle as good as position 1 (in 32-bit floats it would be off by 0.06 rad). The fraction's nearest quarter
 // turn is split off as an integer too; what is left lies in [-1/4, 1/4) half turns and keeps 2^-26 of a turn in a float.
 //
-// Bound by memory: every value is read and written once. One block per row; its cosines are worked out once for all heads while the
-// row's values are on their way.
+// Bound by memory: every value is read and written once. One block per row; its cosines are worked out once for all heads. Where there are
+// many rows, small blocks: 16384 rows of 64 + 8 heads of 128 in fp16 take 116 us (5.8 TB/s) with 64 threads a block, 119 with 128 and 134
+// with 192; few rows want more of a row under way (32 rows: 4.8, 3.5 and 3.1 us). Asking for the values before the cosines, cosines in
+// registers, and rows streamed through shared memory by bulk copies (201 us) were all slower.
 #include "cacheir_b200_serving.h"
 #include "common.cuh"
 
 namespace cb200 {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kMaxThreads = 256;
 constexpr int kMaxDim = 1024;
 
 __device__ __forceinline__ float2 turn_cos_sin(uint64_t turns, int position, float factor) {
@@ -30,11 +32,11 @@ __device__ __forceinline__ float2 turn_cos_sin(uint64_t turns, int position, flo
 
 // A unit is VEC pairs (or 2 VEC values that are only copied): two vectors of VEC values.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kMaxThreads)
 rotary_append_kernel(const cacheir_b200_rotary_args p) {
   chain_enter();
   __shared__ float2 s_turn[kMaxDim / 2];
-  const int row = blockIdx.x;
+  const int row = blockIdx.x, threads = blockDim.x;
   long long line = 0;                                       // of the pool, in rows of a kv head
   if (p.slots) {
     const int slot = p.slots[row];
@@ -42,11 +44,11 @@ rotary_append_kernel(const cacheir_b200_rotary_args p) {
     line = static_cast<long long>(slot / p.page_size) * p.kv_heads * p.page_size + slot % p.page_size;
   }
   const int half = p.rot / 2, position = p.positions[row];
-  for (int i = threadIdx.x; i < half; i += kThreads) s_turn[i] = turn_cos_sin(p.turns[i], position, p.factor);
+  for (int i = threadIdx.x; i < half; i += threads) s_turn[i] = turn_cos_sin(p.turns[i], position, p.factor);
   __syncthreads();
   const int turning = half / VEC, units = turning + (p.dim - p.rot + 2 * VEC - 1) / (2 * VEC);       // per head
   const int heads = p.heads + (p.slots ? 2 : 1) * p.kv_heads;
-  for (int u = threadIdx.x; u < heads * units; u += kThreads) {
+  for (int u = threadIdx.x; u < heads * units; u += threads) {
     const int head = u / units, j = u - head * units;
     const bool is_q = head < p.heads, is_v = head >= p.heads + p.kv_heads;
     const int h = is_q ? head : (head - p.heads) % p.kv_heads;
@@ -98,8 +100,9 @@ int launch_rotary(const cacheir_b200_rotary_args& a, cudaStream_t stream) {
                           static_cast<const void*>(a.v_cache)})
     wide = wide && aligned_to(ptr, 16);
   for (long long stride : {a.q_stride, a.k_stride, a.v_stride, a.q_out_stride, a.k_out_stride}) wide = wide && stride % VEC == 0;
-  const cudaError_t e = wide ? launch_chained(rotary_append_kernel<T, VEC>, dim3(a.rows), dim3(kThreads), 0, stream, a)
-                             : launch_chained(rotary_append_kernel<T, 1>, dim3(a.rows), dim3(kThreads), 0, stream, a);
+  const int threads = a.rows > 4096 ? 64 : a.rows > 4 * kNumSMs ? 128 : kMaxThreads;
+  const cudaError_t e = wide ? launch_chained(rotary_append_kernel<T, VEC>, dim3(a.rows), dim3(threads), 0, stream, a)
+                             : launch_chained(rotary_append_kernel<T, 1>, dim3(a.rows), dim3(threads), 0, stream, a);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }
 

@@ -228,6 +228,8 @@ extern "C" int cacheir_b200_shared_prefix_attention(const cacheir_b200_prefix_ar
 }
 
 extern "C" int cacheir_b200_serving_device_status(int reset) {
-  const int prefix = prefix_device_status(reset != 0), logprobs = logprobs_device_status(reset != 0);
-  return prefix != 0 ? prefix : logprobs;
+  const int found[] = {prefix_device_status(reset != 0), logprobs_device_status(reset != 0)};
+  for (int status : found)
+    if (status != 0) return status;
+  return 0;
 }

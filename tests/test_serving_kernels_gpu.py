@@ -219,7 +219,8 @@ def _rotated(x, angle, rot, layout, factor):
 @pytest.mark.parametrize("layout", ["interleaved", "half"])
 @pytest.mark.parametrize("rows,heads,kv_heads,dim,rot,page,yarn", [
     (1, 4, 2, 128, 128, 16, False), (33, 8, 1, 128, 64, 16, True), (7, 3, 3, 96, 32, 5, False), (5, 2, 1, 64, 22, 16, False), (4, 1, 1, 7, 4, 3, False),
-    (300, 4, 4, 64, 64, 16, True), (2, 5, 1, 1024, 1024, 2, False), (3, 2, 2, 2, 2, 1, False)])
+    (300, 4, 4, 64, 64, 16, True), (2, 5, 1, 1024, 1024, 2, False), (3, 2, 2, 2, 2, 1, False), (593, 32, 8, 128, 128, 16, True), (1200, 4, 2, 64, 32, 16, False),
+    (3001, 3, 1, 96, 96, 16, False)])
 def test_rotary_append_against_complex_numbers(dtype, layout, rows, heads, kv_heads, dim, rot, page, yarn):
     from cacheir_b200 import serving_ops as S
     from cacheir_b200.ragged import rotary_frequencies, yarn_frequencies
