@@ -12,6 +12,7 @@
 // rows and the way back took 40.6 us with the rows in one cluster of eight blocks and the way back in one block, 15.5 us like this.
 #include "cacheir_b200_serving.h"
 #include "common.cuh"
+#include "serving_status.h"
 #include "tc_ptx.cuh"
 
 namespace cb200 {
@@ -256,7 +257,8 @@ template <bool EXTEND>
 int launch_tables(const TableArgs& a, cudaStream_t stream) {
   const size_t smem = static_cast<size_t>(a.sequences) * (EXTEND ? 3 : 2) * 4;
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(page_tables_kernel<EXTEND>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    static std::atomic<unsigned long long> done{0};
+    const cudaError_t e = allow_shared_memory(done, reinterpret_cast<const void*>(page_tables_kernel<EXTEND>), CACHEIR_B200_MAX_SEQUENCES * 12);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   const bool few = a.sequences <= 128 && (!EXTEND || a.rows <= 512);

@@ -141,6 +141,21 @@ __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float lo, float hi)
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// A warp's wait; false in all lanes where it gave up in one.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, &g_prefix_status, code));
+}
+// n / d for a d that mostly is a power of two (pages).
+struct Division {
+  int d, shift;
+  __device__ __forceinline__ explicit Division(int n) {
+    d = n;
+    shift = (n & (n - 1)) == 0 ? 31 - __clz(n) : -1;
+  }
+  __device__ __forceinline__ int of(int n) const { return shift >= 0 ? n >> shift : n / d; }
+};
+
 // ---- how the common parts are cut ----
 // An item of n key tiles is kItemUnits + n units: what it costs to begin with (queries, the first tile's latency, the output) is about
 // that of so many tiles. The units are dealt out as evenly as whole numbers can be.
@@ -360,6 +375,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     const bool copies = chunk < kKeys / kChunk;
     const int outside = a.num_slots * a.kv_heads * a.page_size;         // rows behind the pool read as zeros
     const uint32_t dst = smem_u32(s_kv) + (keys ? box * kKeys * 128 + chunk * kChunk * 128 : chunk * kChunk * D * 2);
+    const Division by_page(a.page_size);
     int slot = keys ? 0 : 1;
     uint32_t phase = 1, sent = 0;                              // slots of a tile: its keys', its values'
     while (ok && walk.next(p)) {
@@ -367,13 +383,13 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       auto line_of = [&](int tile) {                           // first row of this lane's 16 in the pool
         const int key = tile * kKeys + chunk * kChunk;
         if (!copies || key >= walk.prefix) return outside;
-        const int id = pages[key / a.page_size];
-        return id >= 0 && id < a.num_slots ? (id * a.kv_heads + walk.kvh) * a.page_size + key % a.page_size : outside;
+        const int page = by_page.of(key), id = pages[page];
+        return id >= 0 && id < a.num_slots ? (id * a.kv_heads + walk.kvh) * a.page_size + key - page * a.page_size : outside;
       };
       int line = line_of(walk.tile);
       for (int t = walk.tile; t < walk.tile + walk.tiles; ++t) {
         const int next = t + 1 < walk.tile + walk.tiles ? line_of(t + 1) : 0;
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[slot]), phase, &g_prefix_status, (15 << 8) | 1));
+        ok = warp_wait(smem_u32(&empty[slot]), phase, (15 << 8) | 1);
         if (!ok) break;
         if (lane == 0) mbar_expect_tx(smem_u32(&full[slot]), L::kSlotBytes);
         __syncwarp();
@@ -400,76 +416,67 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     const uint32_t id_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) |
                           (static_cast<uint32_t>(kRows >> 4) << 24);
     const uint64_t dq = smem_desc_sw128(smem_u32(s_q)), dk = smem_desc_sw128(smem_u32(s_kv)), dv = smem_desc_columns(smem_u32(s_kv));
-    // Scores and outputs step through the same (tile, buffer) sequence, scores up to two steps ahead.
-    struct Steps {
-      Walk walk;
-      __device__ __forceinline__ explicit Steps(const Walk& w) : walk(w) {}
-      int left = 0, two = 0, second = 0, tile = 0, first = 0;  // key tiles left in the item, two steps per tile?, the second of them?, tiles so far
-      __device__ __forceinline__ bool ready(const CommonParams& p, int group) {
-        if (left > 0) return true;
-        if (!walk.next(p)) return false;
-        left = first = walk.tiles;
-        two = walk.rows * group > kRows ? 1 : 0;
-        return true;
-      }
-      // (returns whether the tile's slot is free after this step)
-      __device__ __forceinline__ bool advance() {
-        if (two && !second) { second = 1; return false; }
-        second = 0;
-        --left;
-        ++tile;
-        return true;
-      }
-    };
-    Steps score(walk), output(walk);
+    // An item's steps: a tile each, or a tile for either group of warps. Scores are one step ahead of outputs. Whatever can be carried along
+    // is (this is one warp's chain of dependent instructions between the tensor cores' products).
     const bool leader = elect_one();
-    int next_s = 0, next_o = 0;
-    uint32_t q_seen[2] = {0, 0};
-    while (ok) {
-      // (an item's queries come after the last output of the item before)
-      if (next_s - next_o < 2 && score.ready(p, group) && (next_s == next_o || score.left < score.first || score.second)) {
-        const int b = next_s & 1, w = score.two ? b : 0, slot = (2 * score.tile) % kSlots;
-        if (score.left == score.first) {                       // the item's first tile: its queries are new
-          ok = mbar_wait(smem_u32(&bar_q[w]), q_seen[w] & 1, &g_prefix_status, (15 << 8) | 3);
-          ++q_seen[w];
+    int b_s = 0, b_o = 0, k_slot = 0, v_slot = 1;              // buffers of scores and probabilities; slots
+    uint32_t k_phase = 0, v_phase = 0, q_phase = 0, p_phase = 0;        // (of the two buffers of queries and probabilities: a bit each)
+    while (ok && walk.next(p)) {
+      const bool two = walk.rows * group > kRows;
+      const int steps = two ? 2 * walk.tiles : walk.tiles;
+      auto score = [&](int j) {
+        const int w = two ? b_s : 0;
+        if (j < (two ? 2 : 1)) {                               // the item's first tile: its queries are new
+          if (!warp_wait(smem_u32(&bar_q[w]), q_phase >> w & 1, (15 << 8) | 3)) return false;
+          q_phase ^= 1u << w;
         }
-        ok = ok && mbar_wait(smem_u32(&full[slot]), (2 * score.tile / kSlots) & 1, &g_prefix_status, (15 << 8) | 4);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        if (!(two && (j & 1)) && !warp_wait(smem_u32(&full[k_slot]), k_phase, (15 << 8) | 4)) return false;
         tc_fence_after();
-        const bool frees = score.advance();
-        const uint64_t q_at = dq + (w * L::kQBytes >> 4), k_at = dk + (slot * L::kSlotBytes >> 4);
-        const uint32_t to = tmem + b * kKeys;
+        const uint64_t q_at = dq + (w * L::kQBytes >> 4), k_at = dk + (k_slot * L::kSlotBytes >> 4);
+        const uint32_t to = tmem + b_s * kKeys;
+        const bool frees = !two || (j & 1);
         if (leader) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             constexpr int kHalf = kRows * 128 >> 4;            // 64 columns further
             mma_ss(to, q_at + (k >> 2) * kHalf + (k & 3) * 2, k_at + (k >> 2) * kHalf + (k & 3) * 2, id_s, k > 0 ? 1u : 0u);
           }
-          tc_commit(smem_u32(&bar_s[b]));
-          if (frees) tc_commit(smem_u32(&empty[slot]));
+          tc_commit(smem_u32(&bar_s[b_s]));
+          if (frees) tc_commit(smem_u32(&empty[k_slot]));
         }
         __syncwarp();
-        ++next_s;
-        continue;
-      }
-      if (!output.ready(p, group)) break;
-      const int b = next_o & 1, w = output.two ? b : 0, at = 2 * output.tile + 1, slot = at % kSlots;
-      ok = mbar_wait(smem_u32(&full[slot]), (at / kSlots) & 1, &g_prefix_status, (15 << 8) | 5);
-      ok = ok && mbar_wait(smem_u32(&bar_p[b]), (next_o >> 1) & 1, &g_prefix_status, (15 << 8) | 6);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      tc_fence_after();
-      const uint32_t add = output.left == output.first ? 0u : 1u;
-      const bool frees = output.advance();
-      const uint64_t v_at = dv + (slot * L::kSlotBytes >> 4);
-      const uint32_t to = tmem_o + w * D, from = tmem + b * kKeys;
-      if (leader) {
+        b_s ^= 1;
+        if (frees) {
+          k_slot += 2;
+          if (k_slot >= kSlots) { k_slot -= kSlots; k_phase ^= 1; }
+        }
+        return true;
+      };
+      // (an item's queries come after the last output of the item before: nothing of it is scored earlier)
+      ok = score(0);
+      for (int j = 0; j < steps && ok; ++j) {
+        if (j + 1 < steps) ok = score(j + 1);
+        if (!(two && (j & 1))) ok = ok && warp_wait(smem_u32(&full[v_slot]), v_phase, (15 << 8) | 5);
+        ok = ok && warp_wait(smem_u32(&bar_p[b_o]), p_phase >> b_o & 1, (15 << 8) | 6);
+        if (!ok) break;
+        p_phase ^= 1u << b_o;
+        tc_fence_after();
+        const uint64_t v_at = dv + (v_slot * L::kSlotBytes >> 4);
+        const uint32_t to = tmem_o + (two ? b_o * D : 0), from = tmem + b_o * kKeys, add = j < (two ? 2 : 1) ? 0u : 1u;
+        const bool frees = !two || (j & 1);
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, k == 0 ? add : 1u);
-        tc_commit(smem_u32(&bar_o[b]));
-        if (frees) tc_commit(smem_u32(&empty[slot]));
+          for (int k = 0; k < kKeys / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, k == 0 ? add : 1u);
+          tc_commit(smem_u32(&bar_o[b_o]));
+          if (frees) tc_commit(smem_u32(&empty[v_slot]));
+        }
+        __syncwarp();
+        b_o ^= 1;
+        if (frees) {
+          v_slot += 2;
+          if (v_slot >= kSlots) { v_slot -= kSlots; v_phase ^= 1; }
+        }
       }
-      __syncwarp();
-      ++next_o;
     }
   } else {
     // ---------------- softmax: a thread per query row ----------------
@@ -508,8 +515,8 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       int last = 0;
       for (int t = 0, s = two ? step + ((step ^ w) & 1) : step; t < walk.tiles && ok; ++t, s += two ? 2 : 1) {
         const int b = s & 1, base = (walk.tile + t) * kKeys;
-        ok = mbar_wait(smem_u32(&bar_s[b]), (s >> 1) & 1, &g_prefix_status, (15 << 8) | 8);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        ok = warp_wait(smem_u32(&bar_s[b]), (s >> 1) & 1, (15 << 8) | 8);
+        if (!ok) break;
         tc_fence_after();
         const uint32_t scores = tmem + b * kKeys + lane_addr;
         const bool whole = __all_sync(0xffffffffu, base + kKeys <= limit);
@@ -791,10 +798,11 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   const int32_t* pages = a.page_table + static_cast<size_t>(row) * a.max_pages;
   const int outside = a.num_slots * a.kv_heads * a.page_size;   // rows behind the pool read as zeros
   const int mine = begin + warp < end ? (end - begin - warp + WARPS - 1) / WARPS : 0;          // chunks begin + warp + i * WARPS
+  const Division by_page(a.page_size);
   auto line_of = [&](int i) {                                    // first row of this warp's i-th chunk in the pool
     if (i >= mine) return outside;
-    const int key = (begin + warp + i * WARPS) * kChunk, id = pages[key / a.page_size];
-    return id >= 0 && id < a.num_slots ? (id * a.kv_heads + kvh) * a.page_size + key % a.page_size : outside;
+    const int key = (begin + warp + i * WARPS) * kChunk, page = by_page.of(key), id = pages[page];
+    return id >= 0 && id < a.num_slots ? (id * a.kv_heads + kvh) * a.page_size + key - page * a.page_size : outside;
   };
   int lines = line_of(lane), lines_next = mine > 32 ? line_of(32 + lane) : outside;            // of chunks 32 k + lane, k rising
   __syncwarp();
@@ -816,7 +824,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   bool ok = true;
 #pragma unroll 1
   for (int it = 0; it < mine; ++it) {
-    ok = __all_sync(0xffffffffu, mbar_wait(bars + stage * 8, phase, &g_prefix_status, (15 << 8) | 12));
+    ok = warp_wait(bars + stage * 8, phase, (15 << 8) | 12);
     if (!ok) {                                                   // the copies that are still under way are waited for
       for (int i = it + 1; i < min(mine, it + kStages); ++i) {
         if (++stage == kStages) { stage = 0; phase ^= 1; }
@@ -1069,7 +1077,8 @@ template <typename T, int D, int WARPS>
 int launch_own(const OwnParams& o, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t stream) {
   auto kern = prefix_own_kernel<T, D, WARPS>;
   constexpr int bytes = OwnSmem<D, WARPS>::kBytes;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = allow_shared_memory(done, reinterpret_cast<const void*>(kern), bytes);
   if (e == cudaSuccess)
     e = launch_clusters(kern, dim3(o.splits, o.a.kv_heads * o.head_chunks, o.a.batch), dim3(WARPS * 32), bytes, stream, dim3(o.splits), tk, tv, o);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
@@ -1099,7 +1108,8 @@ int launch_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cud
     cudaError_t e = cudaSuccess;
     if (c.plan_ready) e = launch_chained(prefix_plan_kernel, dim3(1), dim3(1024), 0, stream, c, grid);
     auto kern = prefix_common_kernel<T, D>;
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CommonSmem<D>::kBytes);
+    static std::atomic<unsigned long long> done{0};
+    if (e == cudaSuccess) e = allow_shared_memory(done, reinterpret_cast<const void*>(kern), CommonSmem<D>::kBytes);
     if (e == cudaSuccess) e = launch_chained(kern, dim3(grid), dim3(kCommonThreads), CommonSmem<D>::kBytes, stream, tk_half, tv, c);
     if (e != cudaSuccess) return static_cast<int>(e);
   }

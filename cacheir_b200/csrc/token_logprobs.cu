@@ -566,7 +566,8 @@ int launch_logprobs(Args a, int rows, cudaStream_t stream) {
   const int per_block = static_cast<int>((tiles + a.cluster - 1) / a.cluster);
   const size_t smem = static_cast<size_t>(kWarps) * kStages * kTileBytes + (a.top > 0 ? static_cast<size_t>(per_block) * 64 * 4 : 0);
   auto kern = token_logprobs_kernel<T>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = allow_shared_memory(done, reinterpret_cast<const void*>(kern), kWarps * kStages * kTileBytes + kMaxTiles * 64 * 4);
   if (e == cudaSuccess) e = launch_clusters(kern, dim3(static_cast<unsigned>(rows) * a.cluster), dim3(kThreads), smem, stream, dim3(a.cluster), a);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }

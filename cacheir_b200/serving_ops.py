@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from dataclasses import dataclass
 
 import numpy as np
@@ -18,11 +19,22 @@ import torch
 
 from . import _lib
 from ._lib import PrefixArgs, RotaryArgs, check
-from .ops import _ptr, _require_cuda, dtype_code
+from .ops import _require_cuda, dtype_code
 
 MAX_TOP = 32
 MAX_SEQUENCES = 16384
 LAYOUTS = {"interleaved": 0, "half": 1}
+# the argument structs as bytes (a third of the time that their ctypes classes take to fill)
+ROTARY_BYTES = struct.Struct("@10Q5q9if")
+PREFIX_BYTES = struct.Struct("@11Q2q10if")
+assert ROTARY_BYTES.size == ctypes.sizeof(RotaryArgs) and PREFIX_BYTES.size <= ctypes.sizeof(PrefixArgs)
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_calls: dict[str, object] = {}         # entry points that have been called
+
+
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 # (As these launch kernels of a few microseconds, what they do on the host is kept to about as many: shapes and strides are taken once, the
@@ -36,12 +48,14 @@ def _launch(what: str, tensors: tuple, *args) -> None:
             raise ValueError(f"all tensors of a call must be on one device, got {sorted({str(t.device) for t in tensors if t is not None})}")
     if index < 0:
         _require_cuda(*tensors)
-    call = getattr(_lib.load_group("serving"), "cacheir_b200_" + what)
+    call = _calls.get(what)
+    if call is None:
+        call = _calls[what] = getattr(_lib.load_group("serving"), "cacheir_b200_" + what)
     if index == torch.cuda.current_device():
-        code = call(*args, torch.cuda.current_stream(index).cuda_stream)
+        code = call(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            code = call(*args, torch.cuda.current_stream(index).cuda_stream)
+            code = call(*args, _raw_stream(index))
     if code:
         check(code, what)
 
@@ -240,10 +254,10 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, rule
     code = dtype_code(dtype)
     if rows == 0:
         return
-    args = RotaryArgs(q.data_ptr(), k.data_ptr(), _ptr(v), q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), positions.data_ptr(), _ptr(slots),
-                      turns.data_ptr(), q_stride, k_stride, v_stride, q_out_stride, k_out_stride, rows, heads, kv_heads, dim, rot, layout, num_slots,
+    args = ROTARY_BYTES.pack(
+        q.data_ptr(), k.data_ptr(), _ptr(v), q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), positions.data_ptr(), _ptr(slots), turns.data_ptr(), q_stride, k_stride, v_stride, q_out_stride, k_out_stride, rows, heads, kv_heads, dim, rot, layout, num_slots,
                       page_size, code, rule.factor)
-    _launch("rotary_append", (q, k, q_out, positions, turns, slots, v, k_out, k_cache, v_cache), ctypes.byref(args))
+    _launch("rotary_append", (q, k, q_out, positions, turns, slots, v, k_out, k_cache, v_cache), args)
 
 
 # ---- attention over common prefixes ----------------------------------------------------------------------------------
@@ -342,11 +356,10 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         workspace = torch.empty(shared_prefix_workspace_bytes(batch, heads, dim), device=q.device, dtype=torch.uint8)
     elif not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    args = PrefixArgs(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), _ptr(group_rows),
+    args = PREFIX_BYTES.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), _ptr(group_rows),
                       _ptr(prefix_table), _ptr(prefix_lens), workspace.data_ptr(), workspace.nbytes, q_stride, out_stride, batch, heads, kv_heads, dim,
                       page_size, slots, max_pages, count, prefix_pages, code, scale)
-    _launch("shared_prefix_attention", (q, k_cache, v_cache, page_table, seq_lens, out, workspace, group_rows, prefix_table, prefix_lens),
-            ctypes.byref(args))
+    _launch("shared_prefix_attention", (q, k_cache, v_cache, page_table, seq_lens, out, workspace, group_rows, prefix_table, prefix_lens), args)
     return out
 
 
