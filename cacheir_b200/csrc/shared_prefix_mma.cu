@@ -114,6 +114,11 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -272,14 +277,15 @@ struct CommonSmem {
   static constexpr int kSlots = D == 128 ? 5 : 10;
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kTiles = 2 * kQBytes + kSlots * kSlotBytes;
-  // then: barriers full, empty [slots], q[2], s[2], p[2], o[2]; tensor memory address; groups
-  static constexpr int kBarriers = 2 * kSlots + 8;
+  // then: barriers full, empty [slots], q[2], place of q[2], s[2], p[2][2], o[2]; tensor memory address; groups
+  static constexpr int kBarriers = 2 * kSlots + 12;
   static constexpr int kBytes = 1024 + kTiles + kBarriers * 8 + 16 + (kPlanGroups + 1) * static_cast<int>(sizeof(PlanGroup));
 };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kCommonThreads, 1)
-prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CommonParams p) {
+prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_q,
+                     const __grid_constant__ CommonParams p) {
   using L = CommonSmem<D>;
   constexpr int kSlots = L::kSlots;
   chain_enter();
@@ -289,10 +295,11 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   uint8_t* s_kv = smem + 2 * L::kQBytes;                       // [slots][D / 64][128 keys][128 B]
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kTiles);
   uint64_t* empty = full + kSlots;
-  uint64_t* bar_q = empty + kSlots;                            // a group of warps has left its queries
-  uint64_t* bar_s = bar_q + 2;                                 // scores are in tensor memory
-  uint64_t* bar_p = bar_s + 2;                                 // probabilities are
-  uint64_t* bar_o = bar_p + 2;                                 // .. and have been added to the output
+  uint64_t* bar_q = empty + kSlots;                            // queries of a group of warps are there
+  uint64_t* bar_free = bar_q + 2;                              // .. and their place is free again
+  uint64_t* bar_s = bar_free + 2;                              // scores are in tensor memory
+  uint64_t* bar_p = bar_s + 2;                                 // probabilities are, [buffer][half of the keys]
+  uint64_t* bar_o = bar_p + 4;                                 // .. and have been added to the output
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_o + 2);
   PlanGroup* s_group = reinterpret_cast<PlanGroup*>(tmem_slot + 4);
   __shared__ int s_plan[2], s_scan[kPlanGroups / 32], s_longest[kPlanGroups / 32];
@@ -333,6 +340,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     }
   }
   if (threadIdx.x == 288) {
+    prefetch_map(&tmap_q);
     prefetch_map(&tmap_k);
     prefetch_map(&tmap_v);
     for (int s = 0; s < kSlots; ++s) {
@@ -340,9 +348,11 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       mbar_init(smem_u32(&empty[s]), 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(smem_u32(&bar_q[b]), kRows);
+      mbar_init(smem_u32(&bar_q[b]), 1);
+      mbar_init(smem_u32(&bar_free[b]), 4);
       mbar_init(smem_u32(&bar_s[b]), 1);
-      mbar_init(smem_u32(&bar_p[b]), kRows);
+      mbar_init(smem_u32(&bar_p[2 * b]), kRows);
+      mbar_init(smem_u32(&bar_p[2 * b + 1]), kRows);
       mbar_init(smem_u32(&bar_o[b]), 1);
     }
     mbar_fence_init();
@@ -364,7 +374,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;                            // scores [2][128 columns] (probabilities over them), outputs [2][D]
   const uint32_t tmem_o = tmem + 2 * kKeys;
-  const int group = a.heads / a.kv_heads;
+  const int group = a.heads / a.kv_heads, half_rows = p.tile_rows / 2;        // batch rows of a group of warps
   Walk walk(groups, units, ctas);
   bool ok = true;
 
@@ -377,7 +387,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     const uint32_t dst = smem_u32(s_kv) + (keys ? box * kKeys * 128 + chunk * kChunk * 128 : chunk * kChunk * D * 2);
     const Division by_page(a.page_size);
     int slot = keys ? 0 : 1;
-    uint32_t phase = 1, sent = 0;                              // slots of a tile: its keys', its values'
+    uint32_t phase = 1, sent = 0, q_phase = 3;                 // (slots of a tile: its keys', its values'; q_phase: a bit for either place)
     while (ok && walk.next(p)) {
       const int32_t* pages = a.prefix_table + static_cast<size_t>(walk.group) * a.prefix_pages;
       auto line_of = [&](int tile) {                           // first row of this lane's 16 in the pool
@@ -387,7 +397,19 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         return id >= 0 && id < a.num_slots ? (id * a.kv_heads + walk.kvh) * a.page_size + key - page * a.page_size : outside;
       };
       int line = line_of(walk.tile);
-      for (int t = walk.tile; t < walk.tile + walk.tiles; ++t) {
+      if (!keys)                                               // the item's queries: rows, heads, 64 columns at a time
+        for (int w = 0; w < (walk.rows > half_rows ? 2 : 1) && ok; ++w) {
+          ok = warp_wait(smem_u32(&bar_free[w]), q_phase >> w & 1, (15 << 8) | 7);
+          if (!ok) break;
+          q_phase ^= 1u << w;
+          if (lane == 0) {
+            mbar_expect_tx(smem_u32(&bar_q[w]), (D / 64) * half_rows * group * 128);
+            for (int z = 0; z < D / 64; ++z)
+              tma_load_4d(smem_u32(s_q + w * L::kQBytes + z * kRows * 128), &tmap_q, smem_u32(&bar_q[w]), 0, walk.kvh * group, walk.row0 + w * half_rows, z);
+          }
+          __syncwarp();
+        }
+      for (int t = walk.tile; t < walk.tile + walk.tiles && ok; ++t) {
         const int next = t + 1 < walk.tile + walk.tiles ? line_of(t + 1) : 0;
         ok = warp_wait(smem_u32(&empty[slot]), phase, (15 << 8) | 1);
         if (!ok) break;
@@ -409,6 +431,9 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       if (ok && n + kSlots < 2 * sent) continue;               // its slot has been filled again since: it came, and that phase is long over
       mbar_wait(smem_u32(&full[n % kSlots]), (n / kSlots) & 1, &g_prefix_status, (15 << 8) | 2);
     }
+    // (queries are waited for by the products; after a wait that gave up: both phases of both places)
+    if (!keys && !ok)
+      for (int w = 0; w < 4; ++w) mbar_wait(smem_u32(&bar_q[w >> 1]), w & 1, &g_prefix_status, (15 << 8) | 2);
   } else if (warp == 8) {
     // ---------------- MMA issue ----------------
     constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
@@ -422,7 +447,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     int b_s = 0, b_o = 0, k_slot = 0, v_slot = 1;              // buffers of scores and probabilities; slots
     uint32_t k_phase = 0, v_phase = 0, q_phase = 0, p_phase = 0;        // (of the two buffers of queries and probabilities: a bit each)
     while (ok && walk.next(p)) {
-      const bool two = walk.rows * group > kRows;
+      const bool two = walk.rows > half_rows;
       const int steps = two ? 2 * walk.tiles : walk.tiles;
       auto score = [&](int j) {
         const int w = two ? b_s : 0;
@@ -457,16 +482,24 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       for (int j = 0; j < steps && ok; ++j) {
         if (j + 1 < steps) ok = score(j + 1);
         if (!(two && (j & 1))) ok = ok && warp_wait(smem_u32(&full[v_slot]), v_phase, (15 << 8) | 5);
-        ok = ok && warp_wait(smem_u32(&bar_p[b_o]), p_phase >> b_o & 1, (15 << 8) | 6);
+        ok = ok && warp_wait(smem_u32(&bar_p[2 * b_o]), p_phase >> b_o & 1, (15 << 8) | 6);
         if (!ok) break;
-        p_phase ^= 1u << b_o;
         tc_fence_after();
         const uint64_t v_at = dv + (v_slot * L::kSlotBytes >> 4);
         const uint32_t to = tmem_o + (two ? b_o * D : 0), from = tmem + b_o * kKeys, add = j < (two ? 2 : 1) ? 0u : 1u;
         const bool frees = !two || (j & 1);
+        if (leader) {                                          // (the first half of the keys while the other half's probabilities are worked out)
+#pragma unroll
+          for (int k = 0; k < kKeys / 32; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, k == 0 ? add : 1u);
+        }
+        __syncwarp();
+        ok = warp_wait(smem_u32(&bar_p[2 * b_o + 1]), p_phase >> b_o & 1, (15 << 8) | 6);
+        if (!ok) break;
+        p_phase ^= 1u << b_o;
+        tc_fence_after();
         if (leader) {
 #pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, k == 0 ? add : 1u);
+          for (int k = kKeys / 32; k < kKeys / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, 1u);
           tc_commit(smem_u32(&bar_o[b_o]));
           if (frees) tc_commit(smem_u32(&empty[v_slot]));
         }
@@ -485,32 +518,17 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     const int by_group = (65536 + group - 1) / group;          // n / group = n * by_group >> 16 for n < 256, group <= 64
     int step = 0, tile = 0;                                    // of the block so far
     while (ok && walk.next(p)) {
-      const int used = walk.rows * group, two = used > kRows ? 1 : 0, steps = walk.tiles * (two ? 2 : 1);
+      const int two = walk.rows > half_rows ? 1 : 0, steps = walk.tiles * (two ? 2 : 1);
       if (!two && w == 1) {                                    // (its barrier's phases pass all the same)
-        for (int s = step | 1; s < step + steps && ok; s += 2) ok = mbar_wait(smem_u32(&bar_s[1]), (s >> 1) & 1, &g_prefix_status, (15 << 8) | 7);
+        for (int s = step | 1; s < step + steps && ok; s += 2) ok = warp_wait(smem_u32(&bar_s[1]), (s >> 1) & 1, (15 << 8) | 14);
         step += steps;
         tile += walk.tiles;
         continue;
       }
-      // queries: rows of this group of warps, zeros behind the last one
-      const int q_row0 = w * kRows;
-#pragma unroll 4
-      for (int i = r; i < kRows * (D / 8); i += kRows) {       // (all of them on their way at once)
-        const int row = i / (D / 8), c = i % (D / 8), at = q_row0 + row, b_row = at * by_group >> 16;
-        const T* src = static_cast<const T*>(a.q);
-        if (at < used) src += static_cast<size_t>(walk.row0 + b_row) * a.q_stride + static_cast<size_t>(walk.kvh * group + at - b_row * group) * D + c * 8;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                     ::"r"(smem_u32(s_q + w * L::kQBytes + (c >> 3) * kRows * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4))), "l"(src),
-                       "r"(at < used ? 16 : 0) : "memory");
-      }
-      const int mine = q_row0 + r;
-      const bool real = mine < used;
-      const int in_tile = real ? mine * by_group >> 16 : 0;
-      const int b_row = walk.row0 + in_tile, head = walk.kvh * group + (real ? mine - in_tile * group : 0);
+      const int in_tile = w * half_rows + (r * by_group >> 16);          // this thread's row of the item
+      const bool real = r < half_rows * group && in_tile < walk.rows;
+      const int b_row = walk.row0 + (real ? in_tile : 0), head = walk.kvh * group + (real ? r - (r * by_group >> 16) * group : 0);
       const int limit = real ? min(walk.prefix, a.seq_lens[b_row]) : walk.prefix;      // keys that the row sees
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      fence_async_smem();
-      mbar_arrive(smem_u32(&bar_q[w]));
       float m_ref = -INFINITY, l_run = 0.f;
       int last = 0;
       for (int t = 0, s = two ? step + ((step ^ w) & 1) : step; t < walk.tiles && ok; ++t, s += two ? 2 : 1) {
@@ -570,6 +588,20 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
             }
           }
         }
+        // keys behind the prefix in its last page may hold anything: zero their values, so that 0 * value stays 0
+        auto clear_values = [&] {
+          const int rest = walk.prefix - base;
+          if (rest >= kKeys || rest % kChunk == 0) return;
+          const int at = 2 * (tile + t) + 1, slot = at % kSlots;
+          ok = warp_wait(smem_u32(&full[slot]), (at / kSlots) & 1, (15 << 8) | 10) && ok;
+          const int rows = kChunk - rest % kChunk;
+          for (int i = r; i < rows * (D / 8); i += kRows) {
+            const int key = rest + i / (D / 8), c = i % (D / 8);
+            *reinterpret_cast<uint4*>(s_kv + slot * L::kSlotBytes + (key / kChunk) * kChunk * D * 2 + (c >> 3) * kChunk * 128 + key % kChunk * 128 + ((c & 7) << 4)) =
+                make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_smem();
+        };
         const float less = m_ref > -INFINITY ? -m_ref : 0.f;
         f32x2 sum[2] = {0ull, 0ull};
         const f32x2 scale2 = pair(p.scale_log2, p.scale_log2), less2 = pair(less, less);
@@ -592,6 +624,10 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           tmem_wait_ld(x);
           tmem_ld_x32(scores + 96, y);
           tmem_st_x32(scores, out);
+          tmem_wait_st();
+          clear_values();
+          tc_fence_before();
+          mbar_arrive(smem_u32(&bar_p[2 * b]));
           if (!whole) masked(x, 64);
           weigh(x, out);
           tmem_wait_ld(y);
@@ -604,21 +640,8 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         unpair(sum[1], s2, s3);
         l_run += (s0 + s1) + (s2 + s3);
         tmem_wait_st();
-        // keys behind the prefix in its last page may hold anything: zero their values, so that 0 * value stays 0
-        const int rest = walk.prefix - base;
-        if (rest < kKeys && rest % kChunk != 0) {
-          const int at = 2 * (tile + t) + 1, slot = at % kSlots;
-          ok = mbar_wait(smem_u32(&full[slot]), (at / kSlots) & 1, &g_prefix_status, (15 << 8) | 10);
-          const int rows = kChunk - rest % kChunk;
-          for (int i = r; i < rows * (D / 8); i += kRows) {
-            const int key = rest + i / (D / 8), c = i % (D / 8);
-            *reinterpret_cast<uint4*>(s_kv + slot * L::kSlotBytes + (key / kChunk) * kChunk * D * 2 + (c >> 3) * kChunk * 128 + key % kChunk * 128 + ((c & 7) << 4)) =
-                make_uint4(0u, 0u, 0u, 0u);
-          }
-          fence_async_smem();
-        }
         tc_fence_before();
-        mbar_arrive(smem_u32(&bar_p[b]));
+        mbar_arrive(smem_u32(&bar_p[2 * b + 1]));
         last = s;
       }
       step += steps;
@@ -627,12 +650,11 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       ok = mbar_wait(smem_u32(&bar_o[last & 1]), (last >> 1) & 1, &g_prefix_status, (15 << 8) | 11);
       __syncwarp();
       tc_fence_after();
-      const int at = static_cast<int>(static_cast<size_t>(b_row) * a.heads + head);
+      const int at = real ? b_row * a.heads + head : -1;
       const size_t piece0 = static_cast<size_t>(walk.piece) * a.batch * a.heads;
       if (real) *reinterpret_cast<float2*>(p.parts.ml + 2 * (piece0 + at)) = make_float2(m_ref, l_run);
       // By way of shared memory (the queries' place), so that a store writes whole lines: a lane has a row, a store 128 bytes of four rows.
       float* s_row = reinterpret_cast<float*>(s_q + w * L::kQBytes + (warp & 3) * (L::kQBytes / 4));
-      const int lanes = min(32, used - q_row0 - (warp & 3) * 32);        // rows of this warp
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
@@ -645,11 +667,14 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         for (int i = 0; i < 8; ++i) {
           const int row = 4 * i + (lane >> 3), to = __shfl_sync(0xffffffffu, at, row);
           const uint4 v = *reinterpret_cast<const uint4*>(s_row + row * 32 + (((lane & 7) ^ (row & 7)) << 2));
-          if (row < lanes) *reinterpret_cast<uint4*>(p.parts.acc + (piece0 + to) * D + c + (lane & 7) * 4) = v;
+          if (to >= 0) *reinterpret_cast<uint4*>(p.parts.acc + (piece0 + to) * D + c + (lane & 7) * 4) = v;
         }
         __syncwarp();
       }
       tc_fence_before();
+      fence_async_smem();                                      // (the next queries come by copies)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_free[w]));
     }
   }
   __syncwarp();
@@ -1052,6 +1077,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
     }
   };
   if (places <= stride) finish(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+  else if (places <= 2 * stride) finish(std::integral_constant<int, 2>{}, std::integral_constant<int, 6>{});
   else finish(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
   if (p.splits > 1) {
     __syncwarp();
@@ -1073,6 +1099,21 @@ bool encode_pool(CUtensorMap* map, const void* base, uint64_t rows, int dim, boo
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Queries as [dim / 64][batch][heads][64]: boxes of 64 columns of the heads of a key/value head of `rows` rows.
+template <typename T>
+bool encode_queries(CUtensorMap* map, const cacheir_b200_prefix_args& a, int rows) {
+  EncodeTiledFn fn = tensor_map_encoder();
+  if (!fn) return false;
+  const long long stride = a.batch > 1 ? a.q_stride : static_cast<long long>(a.heads) * a.dim;
+  const cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(a.heads), static_cast<cuuint64_t>(a.batch), static_cast<cuuint64_t>(a.dim / 64)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(a.dim) * 2, static_cast<cuuint64_t>(stride) * 2, 128};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(a.heads / a.kv_heads), static_cast<cuuint32_t>(rows), 1};
+  const cuuint32_t elem_strides[4] = {1, 1, 1, 1};
+  return fn(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(a.q), dims,
+            strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D, int WARPS>
 int launch_own(const OwnParams& o, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t stream) {
   auto kern = prefix_own_kernel<T, D, WARPS>;
@@ -1089,14 +1130,15 @@ long long most_units(const cacheir_b200_prefix_args& a, int tile_rows) {
   const long long tiles = (static_cast<long long>(a.prefix_pages) * a.page_size + kKeys - 1) / kKeys;
   return (kItemUnits + tiles) * a.kv_heads * (a.batch / tile_rows + a.groups);
 }
-int rows_of_tile(const cacheir_b200_prefix_args& a) { return 2 * kRows / (a.heads / a.kv_heads); }
+// Batch rows of an item: as many as two groups of warps have rows for.
+int rows_of_tile(const cacheir_b200_prefix_args& a) { return 2 * (kRows / (a.heads / a.kv_heads)); }
 
 template <typename T, int D>
 int launch_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cudaStream_t stream) {
-  CUtensorMap tk, tv, tk_half;
+  CUtensorMap tk, tv, tk_half, tq;
   const uint64_t rows = static_cast<uint64_t>(a.num_slots) * a.kv_heads * a.page_size;
   if (!encode_pool<T>(&tk, a.k_cache, rows, D, true) || !encode_pool<T>(&tv, a.v_cache, rows, D, true) ||
-      (a.groups > 0 && !encode_pool<T>(&tk_half, a.k_cache, rows, D, false)))
+      (a.groups > 0 && (!encode_pool<T>(&tk_half, a.k_cache, rows, D, false) || !encode_queries<T>(&tq, a, rows_of_tile(a) / 2))))
     return CACHEIR_B200_EUNSUPPORTED;
   const int group = a.heads / a.kv_heads, tile_rows = rows_of_tile(a);
   const float scale_log2 = a.softmax_scale * 1.4426950408889634f;
@@ -1110,7 +1152,7 @@ int launch_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cud
     auto kern = prefix_common_kernel<T, D>;
     static std::atomic<unsigned long long> done{0};
     if (e == cudaSuccess) e = allow_shared_memory(done, reinterpret_cast<const void*>(kern), CommonSmem<D>::kBytes);
-    if (e == cudaSuccess) e = launch_chained(kern, dim3(grid), dim3(kCommonThreads), CommonSmem<D>::kBytes, stream, tk_half, tv, c);
+    if (e == cudaSuccess) e = launch_chained(kern, dim3(grid), dim3(kCommonThreads), CommonSmem<D>::kBytes, stream, tk_half, tv, tq, c);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   OwnParams o{a, parts, a.groups > 0 ? 1 : 0, grid, tile_rows, (group + 15) / 16, 1, scale_log2};
