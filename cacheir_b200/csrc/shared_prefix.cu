@@ -195,7 +195,7 @@ using namespace cb200;
 
 extern "C" size_t cacheir_b200_shared_prefix_workspace_bytes(int batch, int heads, int dim) {
   if (batch <= 0 || heads <= 0 || dim <= 0) return 0;
-  const int pieces = prefix_pieces(batch, heads, dim);
+  const int pieces = prefix_pieces(batch, heads, dim) + own_parts(batch);
   return prefix_plan_bytes(batch) + prefix_ml_bytes(batch, heads, pieces) + static_cast<size_t>(pieces) * batch * heads * dim * 4;
 }
 
@@ -217,10 +217,11 @@ extern "C" int cacheir_b200_shared_prefix_attention(const cacheir_b200_prefix_ar
   if (!(a.softmax_scale > 0.f)) a.softmax_scale = 1.0f / sqrtf(static_cast<float>(a.dim));
   PrefixParts parts;
   parts.pieces = prefix_pieces(a.batch, a.heads, a.dim);
+  parts.own = own_parts(a.batch);
   char* scratch = static_cast<char*>(a.workspace);
   parts.plan = reinterpret_cast<PrefixPlan*>(scratch);
   parts.ml = reinterpret_cast<float*>(scratch += prefix_plan_bytes(a.batch));
-  parts.acc = reinterpret_cast<float*>(scratch + prefix_ml_bytes(a.batch, a.heads, parts.pieces));
+  parts.acc = reinterpret_cast<float*>(scratch + prefix_ml_bytes(a.batch, a.heads, parts.pieces + parts.own));
   if (prefix_fast_supported(a)) return launch_prefix_fast(a, parts, as_stream(stream));
   if (a.dtype == CACHEIR_B200_F32) return launch_general<float>(a, parts, as_stream(stream));
   if (a.dtype == CACHEIR_B200_F16) return launch_general<__half>(a, parts, as_stream(stream));

@@ -20,12 +20,13 @@ struct PrefixPlan {
   PlanGroup group[1];         // [groups], and the end of the last one's units
 };
 
-// The scratch: plan, then for every (piece, row, head) a maximum (log2 domain) and a denominator, and the unnormalised output.
+// The scratch: plan, then for every (piece, row, head) a maximum (log2 domain) and a denominator, and the unnormalised output. Up to `pieces`
+// of them come from the common parts (general kernels: from either), up to `own` from a row's own keys.
 struct PrefixParts {
   PrefixPlan* plan;
-  float* ml;       // [pieces][batch][heads][2]
-  float* acc;      // [pieces][batch][heads][dim]
-  int pieces;
+  float* ml;       // [pieces + own][batch][heads][2]
+  float* acc;      // [pieces + own][batch][heads][dim]
+  int pieces, own;
 };
 
 // First row of group g, inside the batch whatever the caller's array holds.
@@ -75,6 +76,13 @@ inline int prefix_pieces(int batch, int heads, int dim) {
   const size_t one = static_cast<size_t>(batch) * heads * dim * 4;
   const size_t n = one > 0 ? (static_cast<size_t>(64) << 20) / one : kMinPieces;
   return n < kMinPieces ? kMinPieces : n > kMaxPieces ? kMaxPieces : static_cast<int>(n);
+}
+// Parts of a row's own keys: more than one where there are few rows.
+constexpr int kMaxOwnParts = 8;
+inline int own_parts(int batch) {
+  int n = 1;
+  while (n < kMaxOwnParts && 2 * n * batch <= kNumSMs) n *= 2;
+  return n;
 }
 inline size_t round_up_256(size_t n) { return (n + 255) / 256 * 256; }
 inline size_t prefix_plan_bytes(int batch) { return round_up_256(sizeof(PrefixPlan) + static_cast<size_t>(batch) * sizeof(PlanGroup)); }

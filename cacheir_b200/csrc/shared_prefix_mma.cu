@@ -1,9 +1,10 @@
 // Decode attention of groups of sequences with a common prefix on the tensor cores: 16-bit types, head sizes 64 and 128, pages of a multiple
 // of 16 tokens, up to 64 query heads per key/value head.
 //
-// Two kernels. The first one multiplies the common keys of a group, once, with the queries of all of its rows that share a key/value
+// Three kernels. The first one multiplies the common keys of a group, once, with the queries of all of its rows that share a key/value
 // head: S = Q K^T and O = P V as tcgen05 MMAs of 128 query rows, scores, probabilities and outputs in tensor memory. The second one takes
-// every row's own keys with warp MMAs, like the ordinary decode attention, and joins the pieces.
+// every row's own keys with warp MMAs, like the ordinary decode attention, beside the first one on the SMs that are left to it. The third
+// one joins the pieces.
 //
 // Common part. An item is (group, key/value head, tile of up to 256 query rows); its keys come in tiles of 128. The key tiles of all items,
 // in a row, are cut evenly over the blocks, so that lengths and sizes of groups do not matter; an item that is cut leaves one piece per
@@ -40,6 +41,7 @@ struct CommonParams {
   PrefixParts parts;
   int plan_ready;                              // the plan is in the scratch already
   int tile_rows;                               // batch rows of an item
+  int own_heads;                               // blocks that a row has for its own keys
   float scale_log2;
 };
 
@@ -184,26 +186,54 @@ __device__ __forceinline__ int group_units(const cacheir_b200_prefix_args& a, in
   out->prefix = prefix_of_group(a, g);
   return out->rows > 0 && out->prefix > 0 ? a.kv_heads * ((out->rows + tile_rows - 1) / tile_rows) * (kItemUnits + key_tiles(out->prefix)) : 0;
 }
-// Blocks that take part: no item may be in more pieces than there is scratch for. n tiles touch ceil((n - 1) / share) + 1 blocks at most.
-__device__ __forceinline__ int plan_ctas(int units, int longest, int grid, int pieces) {
+// What decides how many blocks take part, besides the units.
+struct Weights {
+  int longest;                 // key tiles of the longest item
+  long long common;            // tokens times rows of the common parts
+  long long cost;              // units, those of items for two groups of warps half as much again
+};
+__device__ __forceinline__ Weights group_weights(const PlanGroup& g, int units, int half_rows) {
+  return Weights{units > 0 ? key_tiles(g.prefix) : 0, static_cast<long long>(g.rows) * g.prefix, g.rows > half_rows ? units + units / 2 : units};
+}
+// Blocks that take part. No item may be in more pieces than there is scratch for: n tiles touch ceil((n - 1) / share) + 1 blocks at most. And
+// the common parts get as many SMs as is their share of the work, so that the other kernel can have the rest of them meanwhile: 16 own
+// tokens of a key/value head (8 KB) take an SM about a twelfth of a unit's time (64 KB). `lens`: tokens of all rows.
+__device__ __forceinline__ int plan_ctas(const CommonParams& p, int units, const Weights& w, long long lens, int grid) {
   if (units <= 0) return 0;
-  const int least = max(1, (longest - 1 + pieces - 2) / (pieces - 1));
-  return max(1, min(grid, units / least));
+  const int least = max(1, (w.longest - 1 + p.parts.pieces - 2) / (p.parts.pieces - 1));
+  const long long own = (max(lens - w.common, 0LL) / kChunk + p.a.batch) * p.own_heads / 12;
+  const long long mine = (kNumSMs * w.cost + w.cost + own - 1) / (w.cost + own);
+  return max(1, min(min(grid, units / least), static_cast<int>(mine)));
+}
+// Tokens of all rows, a thread's part of them.
+__device__ __forceinline__ long long lens_part(const cacheir_b200_prefix_args& a, int thread, int threads) {
+  const int room = a.max_pages * a.page_size;
+  long long sum = 0;
+  for (int b = thread; b < a.batch; b += threads) sum += min(max(a.seq_lens[b], 0), room);
+  return sum;
+}
+__device__ __forceinline__ long long warp_sum64(long long v) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
 }
 
 // The plan of more groups than a block lays out by itself.
 __global__ void __launch_bounds__(1024)
 prefix_plan_kernel(const CommonParams p, const int grid) {
   chain_enter();
-  __shared__ int s_sum[32], s_max[32];
+  __shared__ int s_sum[32], s_longest[32];
+  __shared__ long long s_wide[3][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int base = 0, longest = 0;
+  int base = 0;
+  Weights all{0, 0, 0};
   for (int g0 = 0; g0 < p.a.groups; g0 += 1024) {
     const int g = g0 + threadIdx.x;
     PlanGroup group{};
     const int own = g < p.a.groups ? group_units(p.a, p.tile_rows, g, &group) : 0;
     int sum = own;
-    if (own > 0) longest = max(longest, key_tiles(group.prefix));
+    const Weights w = group_weights(group, own, p.tile_rows / 2);
+    all = Weights{max(all.longest, w.longest), all.common + w.common, all.cost + w.cost};
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, sum, off);
@@ -211,24 +241,30 @@ prefix_plan_kernel(const CommonParams p, const int grid) {
     }
     if (lane == 31) s_sum[warp] = sum;
     __syncthreads();
-    int before = 0, all = 0;
+    int before = 0, total = 0;
     for (int w = 0; w < 32; ++w) {
       if (w < warp) before += s_sum[w];
-      all += s_sum[w];
+      total += s_sum[w];
     }
     group.start = base + before + sum - own;
     if (g < p.a.groups) p.parts.plan->group[g] = group;
-    base += all;
+    base += total;
     __syncthreads();
   }
-  longest = __reduce_max_sync(0xffffffffu, longest);
-  if (lane == 0) s_max[warp] = longest;
+  const int longest = __reduce_max_sync(0xffffffffu, all.longest);
+  const long long lens = warp_sum64(lens_part(p.a, threadIdx.x, 1024)), common = warp_sum64(all.common), cost = warp_sum64(all.cost);
+  if (lane == 0) { s_longest[warp] = longest; s_wide[0][warp] = lens; s_wide[1][warp] = common; s_wide[2][warp] = cost; }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 0; w < 32; ++w) longest = max(longest, s_max[w]);
+    Weights w{0, 0, 0};
+    long long tokens = 0;
+    for (int i = 0; i < 32; ++i) {
+      w = Weights{max(w.longest, s_longest[i]), w.common + s_wide[1][i], w.cost + s_wide[2][i]};
+      tokens += s_wide[0][i];
+    }
     p.parts.plan->group[p.a.groups].start = base;
     p.parts.plan->units = base;
-    p.parts.plan->ctas = plan_ctas(base, longest, grid, p.parts.pieces);
+    p.parts.plan->ctas = plan_ctas(p, base, w, tokens, grid);
   }
 }
 
@@ -303,6 +339,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_o + 2);
   PlanGroup* s_group = reinterpret_cast<PlanGroup*>(tmem_slot + 4);
   __shared__ int s_plan[2], s_scan[kPlanGroups / 32], s_longest[kPlanGroups / 32];
+  __shared__ long long s_lens[kCommonThreads / 32], s_common[kPlanGroups / 32], s_cost[kPlanGroups / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const cacheir_b200_prefix_args& a = p.a;
 
@@ -310,32 +347,41 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   if (!p.plan_ready) {
     PlanGroup mine{};
     int own = 0, sum = 0;
+    const long long lens = lens_part(a, threadIdx.x, kCommonThreads);
     if (warp < kPlanGroups / 32) {
       own = static_cast<int>(threadIdx.x) < a.groups ? group_units(a, p.tile_rows, threadIdx.x, &mine) : 0;
-      const int longest = __reduce_max_sync(0xffffffffu, own > 0 ? key_tiles(mine.prefix) : 0);
+      const Weights w = group_weights(mine, own, p.tile_rows / 2);
+      const int longest = __reduce_max_sync(0xffffffffu, w.longest);
+      const long long common = warp_sum64(w.common), cost = warp_sum64(w.cost);
       sum = own;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, sum, off);
         if (lane >= off) sum += up;
       }
-      if (lane == 31) { s_scan[warp] = sum; s_longest[warp] = longest; }
+      if (lane == 31) { s_scan[warp] = sum; s_longest[warp] = longest; s_common[warp] = common; s_cost[warp] = cost; }
     }
+    const long long warp_lens = warp_sum64(lens);
+    if (lane == 0) s_lens[warp] = warp_lens;
     __syncthreads();
     if (warp < kPlanGroups / 32) {
-      int before = 0, all = 0, longest = 0;
+      int before = 0, all = 0;
+      Weights w{0, 0, 0};
 #pragma unroll
-      for (int w = 0; w < kPlanGroups / 32; ++w) {
-        if (w < warp) before += s_scan[w];
-        all += s_scan[w];
-        longest = max(longest, s_longest[w]);
+      for (int i = 0; i < kPlanGroups / 32; ++i) {
+        if (i < warp) before += s_scan[i];
+        all += s_scan[i];
+        w = Weights{max(w.longest, s_longest[i]), w.common + s_common[i], w.cost + s_cost[i]};
       }
       mine.start = before + sum - own;
       if (static_cast<int>(threadIdx.x) < a.groups) s_group[threadIdx.x] = mine;
       if (threadIdx.x == 0) {
+        long long tokens = 0;
+#pragma unroll
+        for (int i = 0; i < kCommonThreads / 32; ++i) tokens += s_lens[i];
         s_group[a.groups].start = all;
         s_plan[0] = all;
-        s_plan[1] = plan_ctas(all, longest, gridDim.x, p.parts.pieces);
+        s_plan[1] = plan_ctas(p, all, w, tokens, gridDim.x);
       }
     }
   }
@@ -386,7 +432,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     const int outside = a.num_slots * a.kv_heads * a.page_size;         // rows behind the pool read as zeros
     const uint32_t dst = smem_u32(s_kv) + (keys ? box * kKeys * 128 + chunk * kChunk * 128 : chunk * kChunk * D * 2);
     const Division by_page(a.page_size);
-    int slot = keys ? 0 : 1;
+    int slot = keys ? 0 : 1, q_place = 0;
     uint32_t phase = 1, sent = 0, q_phase = 3;                 // (slots of a tile: its keys', its values'; q_phase: a bit for either place)
     while (ok && walk.next(p)) {
       const int32_t* pages = a.prefix_table + static_cast<size_t>(walk.group) * a.prefix_pages;
@@ -397,18 +443,23 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         return id >= 0 && id < a.num_slots ? (id * a.kv_heads + walk.kvh) * a.page_size + key - page * a.page_size : outside;
       };
       int line = line_of(walk.tile);
-      if (!keys)                                               // the item's queries: rows, heads, 64 columns at a time
-        for (int w = 0; w < (walk.rows > half_rows ? 2 : 1) && ok; ++w) {
-          ok = warp_wait(smem_u32(&bar_free[w]), q_phase >> w & 1, (15 << 8) | 7);
+      if (!keys) {                                             // the item's queries: rows, heads, 64 columns at a time
+        const bool two = walk.rows > half_rows;
+        for (int w = 0; w < (two ? 2 : 1) && ok; ++w) {
+          const int place = two ? w : q_place;
+          ok = warp_wait(smem_u32(&bar_free[place]), q_phase >> place & 1, (15 << 8) | 7);
           if (!ok) break;
-          q_phase ^= 1u << w;
+          q_phase ^= 1u << place;
           if (lane == 0) {
-            mbar_expect_tx(smem_u32(&bar_q[w]), (D / 64) * half_rows * group * 128);
+            mbar_expect_tx(smem_u32(&bar_q[place]), (D / 64) * half_rows * group * 128);
             for (int z = 0; z < D / 64; ++z)
-              tma_load_4d(smem_u32(s_q + w * L::kQBytes + z * kRows * 128), &tmap_q, smem_u32(&bar_q[w]), 0, walk.kvh * group, walk.row0 + w * half_rows, z);
+              tma_load_4d(smem_u32(s_q + place * L::kQBytes + z * kRows * 128), &tmap_q, smem_u32(&bar_q[place]), 0, walk.kvh * group,
+                          walk.row0 + w * half_rows, z);
           }
           __syncwarp();
         }
+        if (!two) q_place ^= 1;
+      }
       for (int t = walk.tile; t < walk.tile + walk.tiles && ok; ++t) {
         const int next = t + 1 < walk.tile + walk.tiles ? line_of(t + 1) : 0;
         ok = warp_wait(smem_u32(&empty[slot]), phase, (15 << 8) | 1);
@@ -444,13 +495,13 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     // An item's steps: a tile each, or a tile for either group of warps. Scores are one step ahead of outputs. Whatever can be carried along
     // is (this is one warp's chain of dependent instructions between the tensor cores' products).
     const bool leader = elect_one();
-    int b_s = 0, b_o = 0, k_slot = 0, v_slot = 1;              // buffers of scores and probabilities; slots
+    int b_s = 0, b_o = 0, k_slot = 0, v_slot = 1, q_place = 0; // buffers of scores and probabilities; slots
     uint32_t k_phase = 0, v_phase = 0, q_phase = 0, p_phase = 0;        // (of the two buffers of queries and probabilities: a bit each)
     while (ok && walk.next(p)) {
       const bool two = walk.rows > half_rows;
       const int steps = two ? 2 * walk.tiles : walk.tiles;
       auto score = [&](int j) {
-        const int w = two ? b_s : 0;
+        const int w = two ? b_s : q_place;
         if (j < (two ? 2 : 1)) {                               // the item's first tile: its queries are new
           if (!warp_wait(smem_u32(&bar_q[w]), q_phase >> w & 1, (15 << 8) | 3)) return false;
           q_phase ^= 1u << w;
@@ -477,7 +528,6 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         }
         return true;
       };
-      // (an item's queries come after the last output of the item before: nothing of it is scored earlier)
       ok = score(0);
       for (int j = 0; j < steps && ok; ++j) {
         if (j + 1 < steps) ok = score(j + 1);
@@ -510,21 +560,25 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           if (v_slot >= kSlots) { v_slot -= kSlots; v_phase ^= 1; }
         }
       }
+      if (!two) q_place ^= 1;
     }
   } else {
     // ---------------- softmax: a thread per query row ----------------
     const int w = warp >> 2, r = threadIdx.x & (kRows - 1);
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int by_group = (65536 + group - 1) / group;          // n / group = n * by_group >> 16 for n < 256, group <= 64
-    int step = 0, tile = 0;                                    // of the block so far
+    int step = 0, tile = 0, q_place = 0;                       // of the block so far; where the queries of an item of one group of warps are
     while (ok && walk.next(p)) {
       const int two = walk.rows > half_rows ? 1 : 0, steps = walk.tiles * (two ? 2 : 1);
       if (!two && w == 1) {                                    // (its barrier's phases pass all the same)
         for (int s = step | 1; s < step + steps && ok; s += 2) ok = warp_wait(smem_u32(&bar_s[1]), (s >> 1) & 1, (15 << 8) | 14);
         step += steps;
         tile += walk.tiles;
+        q_place ^= 1;
         continue;
       }
+      const int place = two ? w : q_place;
+      if (!two) q_place ^= 1;
       const int in_tile = w * half_rows + (r * by_group >> 16);          // this thread's row of the item
       const bool real = r < half_rows * group && in_tile < walk.rows;
       const int b_row = walk.row0 + (real ? in_tile : 0), head = walk.kvh * group + (real ? r - (r * by_group >> 16) * group : 0);
@@ -654,7 +708,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       const size_t piece0 = static_cast<size_t>(walk.piece) * a.batch * a.heads;
       if (real) *reinterpret_cast<float2*>(p.parts.ml + 2 * (piece0 + at)) = make_float2(m_ref, l_run);
       // By way of shared memory (the queries' place), so that a store writes whole lines: a lane has a row, a store 128 bytes of four rows.
-      float* s_row = reinterpret_cast<float*>(s_q + w * L::kQBytes + (warp & 3) * (L::kQBytes / 4));
+      float* s_row = reinterpret_cast<float*>(s_q + place * L::kQBytes + (warp & 3) * (L::kQBytes / 4));
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
@@ -674,7 +728,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       tc_fence_before();
       fence_async_smem();                                      // (the next queries come by copies)
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_free[w]));
+      if (lane == 0) mbar_arrive(smem_u32(&bar_free[place]));
     }
   }
   __syncwarp();
@@ -687,31 +741,25 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// Every row's own keys, and the pieces joined. One block per (part of the row's own keys, key/value head and up to 16 of its query heads, row);
-// the parts are a thread-block cluster. Keys and values come 16 tokens at a time (TMA): every warp takes every WARPS-th chunk of the part
-// through a ring of its own, with warp MMAs that have the query heads as their 16 rows. Bound by the memory's rate where there are many
-// rows: then blocks of two warps, six of them on an SM, so that while some begin or join others keep the memory busy; where there are
-// few, blocks of four or eight. None of that needs the common part's kernel: this one starts as soon as that one's blocks leave room, and waits for
-// it before it joins.
-constexpr int kMaxOwnSplits = 8;
-
+// Every row's own keys. One block per (part of the row's own keys, key/value head and up to 16 of its query heads, row). Keys and values come
+// 16 tokens at a time (TMA): every warp takes every WARPS-th chunk of the part through a ring of its own, with warp MMAs that have the query
+// heads as their 16 rows. Bound by the memory's rate where there are many rows: then blocks of two warps, six of them on an SM, so that
+// while some begin or end others keep the memory busy; where there are few, blocks of four or eight. None of that needs the common part's
+// kernel: this one starts as soon as that one's blocks have their places, on the SMs that they leave.
 struct OwnParams {
   cacheir_b200_prefix_args a;
   PrefixParts parts;
   int common;                                  // a kernel of common parts runs before
-  int grid;                                    // .. of so many blocks
   int tile_rows, head_chunks, splits;
   float scale_log2;
 };
 
 template <int D, int WARPS>
 struct OwnSmem {
-  static constexpr int kStages = WARPS == 2 ? 2 : 3;
+  static constexpr int kStages = WARPS <= 4 ? 2 : 3;
   static constexpr int kTileBytes = kChunk * D * 2;
   static constexpr int kRing = WARPS * kStages * 2 * kTileBytes;
-  // over the ring afterwards: the warps' states, the block's, and the weights of all sources of a head
-  static constexpr int kSources = kMaxPieces + kMaxOwnSplits;
-  static constexpr int kJoin = (WARPS * 16 * (D + 2) + 16 * (D + 2) + 16 * kSources) * 4;
+  static constexpr int kJoin = WARPS * 16 * (D + 2) * 4;       // over the ring afterwards: the warps' states
   static constexpr int kBytes = 1024 + (kRing > kJoin ? kRing : kJoin) + WARPS * kStages * 8;
 };
 
@@ -727,23 +775,11 @@ __device__ __forceinline__ void mma_pair(float (&c)[4], const uint32_t (&x)[4], 
   else
     mma_bf16(c, x, b0, b1);
 }
-__device__ __forceinline__ float ld_rank_f32(const float* local, uint32_t rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(smem_u32(local), rank)) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 ld_rank_f32x4(const float* local, uint32_t rank) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(map_to_rank(smem_u32(local), rank)) : "memory");
-  return v;
-}
-
 // A row's group (rows and prefix 0 outside every group). Up to 32 groups, a lane each, the warp lays the plan out beside that: one round of
 // loads, and nothing of it has to wait for the common part's kernel.
 struct RowGroup {
   PlanGroup in;
-  int group, planned, units, ctas;             // planned: ctas is the longest item's key tiles (what plan_ctas takes)
+  int group, planned, units;                   // planned: its first unit and the number of units are known already
 };
 __device__ __forceinline__ RowGroup row_group(const cacheir_b200_prefix_args& a, int tile_rows, int row) {
   RowGroup r{};
@@ -768,7 +804,6 @@ __device__ __forceinline__ RowGroup row_group(const cacheir_b200_prefix_args& a,
   }
   r.planned = 1;
   r.units = __shfl_sync(0xffffffffu, sum, 31);
-  r.ctas = __reduce_max_sync(0xffffffffu, own > 0 ? key_tiles(mine.prefix) : 0);
   const uint32_t found = __ballot_sync(0xffffffffu, mine.rows > 0 && mine.row <= row && row < mine.row + mine.rows);
   if (found == 0) return r;
   r.group = 31 - __clz(found);
@@ -784,9 +819,10 @@ __global__ void __launch_bounds__(WARPS * 32)
 prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ OwnParams p) {
   using L = OwnSmem<D, WARPS>;
   constexpr int kThreads = WARPS * 32, kStages = L::kStages;
-  // What stands before this wait reads what was there before the common part's kernel began: its blocks let this one in only after they
-  // had waited for all earlier ones.
-  if (!p.common) chain_enter();
+  // This kernel reads what was there before the common part's kernel began, whose blocks let this one in only after they had waited for all
+  // earlier ones. (One block waits for that kernel in the end, so that the end of this one implies the end of both.)
+  if (!p.common) chain_wait();
+  chain_next();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const cacheir_b200_prefix_args& a = p.a;
@@ -805,8 +841,9 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   }
   // Lengths, group, first page ids and queries are asked for together as far as they can be.
   const int len = min(max(a.seq_lens[row], 0), a.max_pages * a.page_size);
-  RowGroup of = row_group(p.a, p.tile_rows, row);
-  const int prefix = of.in.prefix, from = min(prefix, len);
+  int prefix;
+  group_of_row(a, row, &prefix);
+  const int from = min(prefix, len);
   const int chunk0 = from / kChunk, chunks = len > from ? (len + kChunk - 1) / kChunk - chunk0 : 0, per = (chunks + p.splits - 1) / p.splits;
   const int begin = chunk0 + min(chunks, split * per), end = chunk0 + min(chunks, (split + 1) * per);
   uint32_t qa[D / 16][4];                                        // queries as the A operand: rows = heads
@@ -945,11 +982,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   __syncthreads();                                               // the rings are drained
   float* s_wm = reinterpret_cast<float*>(smem);                  // [warps][16] maxima, denominators
   float* s_wl = s_wm + WARPS * 16;
-  float* s_m = s_wl + WARPS * 16;                                // [16] the block's
-  float* s_l = s_m + 16;
-  float* s_o = s_l + 16;                                         // [16][D]
-  float* s_w = s_o + 16 * D;                                     // [16][sources] weights
-  float* s_wo = s_w + 16 * L::kSources;                          // [warps][16][D]
+  float* s_wo = s_wl + WARPS * 16;                               // [warps][16][D]
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int h = g + r * 8;
@@ -960,6 +993,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
     }
   }
   __syncthreads();
+  const size_t to = (static_cast<size_t>(p.parts.pieces + split) * a.batch + row) * a.heads + head0;
   for (int i = threadIdx.x; i < heads * (D / 4); i += kThreads) {
     const int h = i / (D / 4), d = i % (D / 4) * 4;
     float m = -INFINITY, l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -972,47 +1006,53 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       const float4 x = *reinterpret_cast<const float4*>(s_wo + (k * 16 + h) * D + d);
       v[0] = fmaf(x.x, wgt, v[0]); v[1] = fmaf(x.y, wgt, v[1]); v[2] = fmaf(x.z, wgt, v[2]); v[3] = fmaf(x.w, wgt, v[3]);
     }
-    *reinterpret_cast<float4*>(s_o + h * D + d) = make_float4(v[0], v[1], v[2], v[3]);
-    if (d == 0) { s_m[h] = m; s_l[h] = l; }
+    *reinterpret_cast<float4*>(p.parts.acc + (to + h) * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+    if (d == 0) *reinterpret_cast<float2*>(p.parts.ml + 2 * (to + h)) = make_float2(m, l);
   }
-  // ---------------- all pieces: the cluster's own parts, then the common ones ----------------
-  if (p.common) {
-    chain_wait();
-    chain_next();
-  }
-  __syncwarp();
-  if (p.splits > 1) cluster_sync_release(); else __syncthreads();
+  if (p.common && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) chain_wait();
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// The pieces of a row, in order: its own keys' parts, then the common ones. A block per key/value head (and up to 16 of its query heads) and
+// row; bound by latency and by the rate at which L2 gives the pieces back.
+constexpr int kJoinThreads = 128;
+constexpr int kSources = kMaxPieces + kMaxOwnParts;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads)
+prefix_join_pieces_kernel(const __grid_constant__ OwnParams p) {
+  __shared__ float s_w[16][kSources];
+  const cacheir_b200_prefix_args& a = p.a;
+  const int kvh = blockIdx.x / p.head_chunks, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = a.heads / a.kv_heads, head0 = kvh * group + blockIdx.x % p.head_chunks * 16, heads = min(16, (kvh + 1) * group - head0);
+  // (the kernel before this one was let in after all earlier ones had ended, and so was this one: the groups may be read ahead)
+  RowGroup of = row_group(a, p.tile_rows, row);
+  chain_wait();
+  chain_next();
   int pieces = 0;
-  if (p.common && prefix > 0) {                                  // (then the row is in a group that has items)
+  if (p.common && of.in.prefix > 0) {                            // (then the row is in a group that has items)
+    const int ctas = p.parts.plan->ctas;
     if (!of.planned) {
       of.in.start = p.parts.plan->group[of.group].start;
       of.units = p.parts.plan->units;
-      of.ctas = p.parts.plan->ctas;
-    } else {
-      of.ctas = plan_ctas(of.units, of.ctas, p.grid, p.parts.pieces);
     }
-    const Deal deal(of.units, of.ctas);
+    const Deal deal(of.units, ctas);
     const int row_tiles = (of.in.rows + p.tile_rows - 1) / p.tile_rows;
-    const int all = kItemUnits + key_tiles(prefix), item0 = of.in.start + (kvh * row_tiles + (row - of.in.row) / p.tile_rows) * all;
+    const int all = kItemUnits + key_tiles(of.in.prefix), item0 = of.in.start + (kvh * row_tiles + (row - of.in.row) / p.tile_rows) * all;
     pieces = deal.owner(item0 + all - 1) - deal.owner(item0 + kItemUnits) + 1;
   }
   const size_t at0 = static_cast<size_t>(row) * a.heads + head0, step = static_cast<size_t>(a.batch) * a.heads;
   const int sources = p.splits + pieces;
-  for (int h = warp; h < heads; h += WARPS) {                    // a warp per head: the weight of every source
+  auto slot_of = [&](int k) { return k < p.splits ? p.parts.pieces + k : k - p.splits; };
+  for (int h = warp; h < heads; h += kJoinThreads / 32) {        // a warp per head: the weight of every source
     float m = -INFINITY, l = 0.f, ms[3], ls[3];
 #pragma unroll
     for (int i = 0; i < 3; ++i) {                                // (at most 72)
       const int k = i * 32 + lane;
-      ms[i] = -INFINITY;
-      ls[i] = 0.f;
-      if (k < p.splits) {
-        ms[i] = p.splits > 1 ? ld_rank_f32(s_m + h, k) : s_m[h];
-        ls[i] = p.splits > 1 ? ld_rank_f32(s_l + h, k) : s_l[h];
-      } else if (k < sources) {
-        const float2 x = *reinterpret_cast<const float2*>(p.parts.ml + 2 * ((k - p.splits) * step + at0 + h));
-        ms[i] = x.x;
-        ls[i] = x.y;
-      }
+      float2 x = make_float2(-INFINITY, 0.f);
+      if (k < sources) x = *reinterpret_cast<const float2*>(p.parts.ml + 2 * (slot_of(k) * step + at0 + h));
+      ms[i] = x.x;
+      ls[i] = x.y;
       m = fmaxf(m, ms[i]);
     }
     m = warp_max(m);
@@ -1025,64 +1065,55 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
     for (int i = 0; i < 3; ++i)
-      if (i * 32 + lane < sources) s_w[h * L::kSources + i * 32 + lane] = ms[i] * inv;
+      if (i * 32 + lane < sources) s_w[h][i * 32 + lane] = ms[i] * inv;
   }
   __syncthreads();
   // Four neighbouring outputs are a place; ITEMS places of a thread and DEEP pieces of each are on their way at once.
-  const int stride = p.splits * kThreads, places = heads * (D / 4);
+  const int places = heads * (D / 4);
   auto finish = [&](auto items, auto deep) {
     constexpr int ITEMS = decltype(items)::value, DEEP = decltype(deep)::value;
-    for (int i0 = split * kThreads + threadIdx.x; i0 < places; i0 += ITEMS * stride) {
+    for (int i0 = threadIdx.x; i0 < places; i0 += ITEMS * kJoinThreads) {
       float v[ITEMS][4];
       const float* acc[ITEMS];
       const float* wgt[ITEMS];
+      bool live[ITEMS];
 #pragma unroll
       for (int j = 0; j < ITEMS; ++j) {
-        const int i = min(i0 + j * stride, places - 1), h = i / (D / 4), d = i % (D / 4) * 4;
+        live[j] = i0 + j * kJoinThreads < places;
+        const int i = live[j] ? i0 + j * kJoinThreads : i0, h = i / (D / 4), d = i % (D / 4) * 4;
         acc[j] = p.parts.acc + (at0 + h) * D + d;
-        wgt[j] = s_w + h * L::kSources;
+        wgt[j] = s_w[h];
         v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0.f;
-        for (int k = 0; k < p.splits; ++k) {
-          const float4 x = p.splits > 1 ? ld_rank_f32x4(s_o + h * D + d, k) : *reinterpret_cast<const float4*>(s_o + h * D + d);
-          const float f = wgt[j][k];
-          v[j][0] = fmaf(x.x, f, v[j][0]); v[j][1] = fmaf(x.y, f, v[j][1]); v[j][2] = fmaf(x.z, f, v[j][2]); v[j][3] = fmaf(x.w, f, v[j][3]);
-        }
       }
-      const int live = min(ITEMS, (places - i0 + stride - 1) / stride);
 #pragma unroll 1
-      for (int k = 0; k < pieces; k += DEEP) {
+      for (int k = 0; k < sources; k += DEEP) {
         float4 x[DEEP][ITEMS];
 #pragma unroll
         for (int e = 0; e < DEEP; ++e)
 #pragma unroll
           for (int j = 0; j < ITEMS; ++j)
-            x[e][j] = j < live && k + e < pieces ? *reinterpret_cast<const float4*>(acc[j] + (k + e) * step * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[e][j] = live[j] && k + e < sources ? *reinterpret_cast<const float4*>(acc[j] + slot_of(k + e) * step * D) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int e = 0; e < DEEP; ++e)
 #pragma unroll
           for (int j = 0; j < ITEMS; ++j) {
-            const float f = k + e < pieces ? wgt[j][p.splits + k + e] : 0.f;
+            const float f = k + e < sources ? wgt[j][k + e] : 0.f;
             v[j][0] = fmaf(x[e][j].x, f, v[j][0]); v[j][1] = fmaf(x[e][j].y, f, v[j][1]);
             v[j][2] = fmaf(x[e][j].z, f, v[j][2]); v[j][3] = fmaf(x[e][j].w, f, v[j][3]);
           }
       }
 #pragma unroll
       for (int j = 0; j < ITEMS; ++j)
-        if (j < live) {
-          const int i = i0 + j * stride, h = i / (D / 4), d = i % (D / 4) * 4;
+        if (live[j]) {
+          const int i = i0 + j * kJoinThreads, h = i / (D / 4), d = i % (D / 4) * 4;
           T* out = static_cast<T*>(a.out) + static_cast<size_t>(row) * a.out_stride + static_cast<size_t>(head0 + h) * D + d;
 #pragma unroll
           for (int e = 0; e < 4; ++e) Elem<T>::st(out + e, v[j][e]);
         }
     }
   };
-  if (places <= stride) finish(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
-  else if (places <= 2 * stride) finish(std::integral_constant<int, 2>{}, std::integral_constant<int, 6>{});
-  else finish(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
-  if (p.splits > 1) {
-    __syncwarp();
-    cluster_sync_release();                                      // nobody leaves while its part is being read
-  }
+  if (places <= kJoinThreads) finish(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+  else finish(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
 }
 
 // A pool as [dim / 64][rows][64]: boxes of 16 rows and 64 columns, or of 16 rows and all columns, 64 by 64.
@@ -1121,7 +1152,9 @@ int launch_own(const OwnParams& o, const CUtensorMap& tk, const CUtensorMap& tv,
   static std::atomic<unsigned long long> done{0};
   cudaError_t e = allow_shared_memory(done, reinterpret_cast<const void*>(kern), bytes);
   if (e == cudaSuccess)
-    e = launch_clusters(kern, dim3(o.splits, o.a.kv_heads * o.head_chunks, o.a.batch), dim3(WARPS * 32), bytes, stream, dim3(o.splits), tk, tv, o);
+    e = launch_chained(kern, dim3(o.splits, o.a.kv_heads * o.head_chunks, o.a.batch), dim3(WARPS * 32), bytes, stream, tk, tv, o);
+  if (e == cudaSuccess)
+    e = launch_chained(prefix_join_pieces_kernel<T, D>, dim3(o.a.kv_heads * o.head_chunks, o.a.batch), dim3(kJoinThreads), 0, stream, o);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }
 
@@ -1142,11 +1175,10 @@ int launch_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cud
     return CACHEIR_B200_EUNSUPPORTED;
   const int group = a.heads / a.kv_heads, tile_rows = rows_of_tile(a);
   const float scale_log2 = a.softmax_scale * 1.4426950408889634f;
-  int grid = 0;
   if (a.groups > 0) {
-    const CommonParams c{a, parts, a.groups > kPlanGroups ? 1 : 0, tile_rows, scale_log2};
+    const CommonParams c{a, parts, a.groups > kPlanGroups ? 1 : 0, tile_rows, a.kv_heads * ((group + 15) / 16), scale_log2};
     const long long most = most_units(a, tile_rows);
-    grid = static_cast<int>(most < kNumSMs ? most : kNumSMs);
+    const int grid = static_cast<int>(most < kNumSMs ? most : kNumSMs);
     cudaError_t e = cudaSuccess;
     if (c.plan_ready) e = launch_chained(prefix_plan_kernel, dim3(1), dim3(1024), 0, stream, c, grid);
     auto kern = prefix_common_kernel<T, D>;
@@ -1155,13 +1187,13 @@ int launch_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cud
     if (e == cudaSuccess) e = launch_chained(kern, dim3(grid), dim3(kCommonThreads), CommonSmem<D>::kBytes, stream, tk_half, tv, tq, c);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  OwnParams o{a, parts, a.groups > 0 ? 1 : 0, grid, tile_rows, (group + 15) / 16, 1, scale_log2};
+  OwnParams o{a, parts, a.groups > 0 ? 1 : 0, tile_rows, (group + 15) / 16, 1, scale_log2};
   const long long blocks = static_cast<long long>(a.batch) * a.kv_heads * o.head_chunks;
-  if (blocks > 2 * kNumSMs) return launch_own<T, D, 2>(o, tk, tv, stream);
+  if (blocks > 3 * kNumSMs) return launch_own<T, D, 2>(o, tk, tv, stream);
   if (blocks > kNumSMs) return launch_own<T, D, 4>(o, tk, tv, stream);
   // Parts of a row's own keys while there are SMs for them, but no more than there are chunks to share.
   const long long chunks = static_cast<long long>(a.max_pages) * a.page_size / kChunk;
-  while (o.splits < kMaxOwnSplits && 2 * o.splits * blocks <= kNumSMs && 2 * o.splits * 8 <= chunks) o.splits *= 2;
+  while (2 * o.splits <= parts.own && 2 * o.splits * blocks <= kNumSMs && 2 * o.splits * 8 <= chunks) o.splits *= 2;
   return launch_own<T, D, 8>(o, tk, tv, stream);
 }
 
