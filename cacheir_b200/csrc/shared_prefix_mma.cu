@@ -201,9 +201,8 @@ __device__ __forceinline__ Weights group_weights(const PlanGroup& g, int units, 
 __device__ __forceinline__ int plan_ctas(const CommonParams& p, int units, const Weights& w, long long lens, int grid) {
   if (units <= 0) return 0;
   const int least = max(1, (w.longest - 1 + p.parts.pieces - 2) / (p.parts.pieces - 1));
-  const long long own = (max(lens - w.common, 0LL) / kChunk + p.a.batch) * p.own_heads / 12;
-  const long long mine = (kNumSMs * w.cost + w.cost + own - 1) / (w.cost + own);
-  return max(1, min(min(grid, units / least), static_cast<int>(mine)));
+  const float cost = static_cast<float>(w.cost), own = (static_cast<float>(max(lens - w.common, 0LL)) / kChunk + p.a.batch) * p.own_heads / 12.f;
+  return max(1, min(min(grid, units / least), static_cast<int>(kNumSMs * cost / (cost + own)) + 1));
 }
 // Tokens of all rows, a thread's part of them.
 __device__ __forceinline__ long long lens_part(const cacheir_b200_prefix_args& a, int thread, int threads) {
@@ -343,6 +342,25 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const cacheir_b200_prefix_args& a = p.a;
 
+  if (warp == 8) tc_alloc(smem_u32(tmem_slot), 512);           // (beside the loads of the plan)
+  if (threadIdx.x == 288) {
+    prefetch_map(&tmap_q);
+    prefetch_map(&tmap_k);
+    prefetch_map(&tmap_v);
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&bar_q[b]), 1);
+      mbar_init(smem_u32(&bar_free[b]), 4);
+      mbar_init(smem_u32(&bar_s[b]), 1);
+      mbar_init(smem_u32(&bar_p[2 * b]), kRows);
+      mbar_init(smem_u32(&bar_p[2 * b + 1]), kRows);
+      mbar_init(smem_u32(&bar_o[b]), 1);
+    }
+    mbar_fence_init();
+  }
   // ---- the plan ----
   if (!p.plan_ready) {
     PlanGroup mine{};
@@ -385,25 +403,9 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       }
     }
   }
-  if (threadIdx.x == 288) {
-    prefetch_map(&tmap_q);
-    prefetch_map(&tmap_k);
-    prefetch_map(&tmap_v);
-    for (int s = 0; s < kSlots; ++s) {
-      mbar_init(smem_u32(&full[s]), 1);
-      mbar_init(smem_u32(&empty[s]), 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(smem_u32(&bar_q[b]), 1);
-      mbar_init(smem_u32(&bar_free[b]), 4);
-      mbar_init(smem_u32(&bar_s[b]), 1);
-      mbar_init(smem_u32(&bar_p[2 * b]), kRows);
-      mbar_init(smem_u32(&bar_p[2 * b + 1]), kRows);
-      mbar_init(smem_u32(&bar_o[b]), 1);
-    }
-    mbar_fence_init();
-  }
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
   const PlanGroup* groups = p.plan_ready ? p.parts.plan->group : s_group;
   const int units = p.plan_ready ? p.parts.plan->units : s_plan[0], ctas = p.plan_ready ? p.parts.plan->ctas : s_plan[1];
   if (!p.plan_ready && blockIdx.x == 0) {                      // for the kernel that joins
@@ -413,15 +415,12 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       p.parts.plan->ctas = ctas;
     }
   }
-  if (static_cast<int>(blockIdx.x) >= ctas) return;
-  if (warp == 8) tc_alloc(smem_u32(tmem_slot), 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
   const uint32_t tmem = *tmem_slot;                            // scores [2][128 columns] (probabilities over them), outputs [2][D]
   const uint32_t tmem_o = tmem + 2 * kKeys;
   const int group = a.heads / a.kv_heads, half_rows = p.tile_rows / 2;        // batch rows of a group of warps
-  Walk walk(groups, units, ctas);
+  const bool takes_part = static_cast<int>(blockIdx.x) < ctas;
+  Walk walk(groups, max(units, 1), max(ctas, 1));
+  if (!takes_part) walk.end = walk.at;
   bool ok = true;
 
   if (warp >= 9) {
@@ -492,73 +491,81 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
     const uint32_t id_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) |
                           (static_cast<uint32_t>(kRows >> 4) << 24);
     const uint64_t dq = smem_desc_sw128(smem_u32(s_q)), dk = smem_desc_sw128(smem_u32(s_kv)), dv = smem_desc_columns(smem_u32(s_kv));
-    // An item's steps: a tile each, or a tile for either group of warps. Scores are one step ahead of outputs. Whatever can be carried along
-    // is (this is one warp's chain of dependent instructions between the tensor cores' products).
+    // An item's steps: a tile each, or a tile for either group of warps. Scores are two steps ahead of outputs, and are issued right behind the
+    // output that frees their buffer. This is one warp's chain of dependent instructions, which the tensor cores wait for where it is not
+    // done in time: whatever can be carried along is, and keys are waited for between the two halves of an output.
     const bool leader = elect_one();
     int b_s = 0, b_o = 0, k_slot = 0, v_slot = 1, q_place = 0; // buffers of scores and probabilities; slots
     uint32_t k_phase = 0, v_phase = 0, q_phase = 0, p_phase = 0;        // (of the two buffers of queries and probabilities: a bit each)
     while (ok && walk.next(p)) {
       const bool two = walk.rows > half_rows;
       const int steps = two ? 2 * walk.tiles : walk.tiles;
-      auto score = [&](int j) {
-        const int w = two ? b_s : q_place;
+      auto wait_scores = [&](int j) {                          // the operands of step j's scores
         if (j < (two ? 2 : 1)) {                               // the item's first tile: its queries are new
+          const int w = two ? b_s : q_place;
           if (!warp_wait(smem_u32(&bar_q[w]), q_phase >> w & 1, (15 << 8) | 3)) return false;
           q_phase ^= 1u << w;
         }
-        if (!(two && (j & 1)) && !warp_wait(smem_u32(&full[k_slot]), k_phase, (15 << 8) | 4)) return false;
-        tc_fence_after();
-        const uint64_t q_at = dq + (w * L::kQBytes >> 4), k_at = dk + (k_slot * L::kSlotBytes >> 4);
+        return (two && (j & 1)) || warp_wait(smem_u32(&full[k_slot]), k_phase, (15 << 8) | 4);
+      };
+      auto score = [&](int j) {                                // (one lane)
+        const uint64_t q_at = dq + ((two ? b_s : q_place) * L::kQBytes >> 4), k_at = dk + (k_slot * L::kSlotBytes >> 4);
         const uint32_t to = tmem + b_s * kKeys;
-        const bool frees = !two || (j & 1);
-        if (leader) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            constexpr int kHalf = kRows * 128 >> 4;            // 64 columns further
-            mma_ss(to, q_at + (k >> 2) * kHalf + (k & 3) * 2, k_at + (k >> 2) * kHalf + (k & 3) * 2, id_s, k > 0 ? 1u : 0u);
-          }
-          tc_commit(smem_u32(&bar_s[b_s]));
-          if (frees) tc_commit(smem_u32(&empty[k_slot]));
+        for (int k = 0; k < D / 16; ++k) {
+          constexpr int kHalf = kRows * 128 >> 4;              // 64 columns further
+          mma_ss(to, q_at + (k >> 2) * kHalf + (k & 3) * 2, k_at + (k >> 2) * kHalf + (k & 3) * 2, id_s, k > 0 ? 1u : 0u);
         }
-        __syncwarp();
+        tc_commit(smem_u32(&bar_s[b_s]));
+        if (!two || (j & 1)) tc_commit(smem_u32(&empty[k_slot]));
+      };
+      auto scored = [&](int j) {                               // (the whole warp)
         b_s ^= 1;
-        if (frees) {
+        if (!two || (j & 1)) {
           k_slot += 2;
           if (k_slot >= kSlots) { k_slot -= kSlots; k_phase ^= 1; }
         }
-        return true;
       };
-      ok = score(0);
+      for (int j = 0; j < 2 && j < steps && ok; ++j) {
+        ok = wait_scores(j);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) score(j);
+        __syncwarp();
+        scored(j);
+      }
       for (int j = 0; j < steps && ok; ++j) {
-        if (j + 1 < steps) ok = score(j + 1);
-        if (!(two && (j & 1))) ok = ok && warp_wait(smem_u32(&full[v_slot]), v_phase, (15 << 8) | 5);
+        if (!(two && (j & 1))) ok = warp_wait(smem_u32(&full[v_slot]), v_phase, (15 << 8) | 5);
         ok = ok && warp_wait(smem_u32(&bar_p[2 * b_o]), p_phase >> b_o & 1, (15 << 8) | 6);
         if (!ok) break;
         tc_fence_after();
         const uint64_t v_at = dv + (v_slot * L::kSlotBytes >> 4);
         const uint32_t to = tmem_o + (two ? b_o * D : 0), from = tmem + b_o * kKeys, add = j < (two ? 2 : 1) ? 0u : 1u;
-        const bool frees = !two || (j & 1);
+        const bool frees = !two || (j & 1), more = j + 2 < steps;
         if (leader) {                                          // (the first half of the keys while the other half's probabilities are worked out)
 #pragma unroll
           for (int k = 0; k < kKeys / 32; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, k == 0 ? add : 1u);
         }
         __syncwarp();
-        ok = warp_wait(smem_u32(&bar_p[2 * b_o + 1]), p_phase >> b_o & 1, (15 << 8) | 6);
+        if (more) ok = wait_scores(j + 2);
+        ok = ok && warp_wait(smem_u32(&bar_p[2 * b_o + 1]), p_phase >> b_o & 1, (15 << 8) | 6);
         if (!ok) break;
-        p_phase ^= 1u << b_o;
         tc_fence_after();
         if (leader) {
 #pragma unroll
           for (int k = kKeys / 32; k < kKeys / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, 1u);
           tc_commit(smem_u32(&bar_o[b_o]));
           if (frees) tc_commit(smem_u32(&empty[v_slot]));
+          if (more) score(j + 2);
         }
         __syncwarp();
+        p_phase ^= 1u << b_o;
         b_o ^= 1;
         if (frees) {
           v_slot += 2;
           if (v_slot >= kSlots) { v_slot -= kSlots; v_phase ^= 1; }
         }
+        if (more) scored(j + 2);
       }
       if (!two) q_place ^= 1;
     }
