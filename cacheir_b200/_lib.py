@@ -312,6 +312,7 @@ GROUP_SIGNATURES: dict[str, dict[str, tuple[object, list[object]]]] = {
         "cacheir_b200_shrink_page_tables": (c_int, [c_void_p] * 6 + [c_int] * 4 + [c_void_p] * 2),
         "cacheir_b200_rotary_append": (c_int, [c_void_p, c_void_p]),
         "cacheir_b200_shared_prefix_workspace_bytes": (c_size_t, [c_int] * 3),
+        "cacheir_b200_shared_prefix_launches": (c_int, [c_int] * 7),
         "cacheir_b200_shared_prefix_attention": (c_int, [c_void_p, c_void_p]),
         "cacheir_b200_token_logprobs": (c_int, [c_void_p, c_longlong] + [c_void_p] * 5 + [c_int] * 3 + [c_double, c_int, c_void_p]),
         "cacheir_b200_serving_device_status": (c_int, [c_int]),

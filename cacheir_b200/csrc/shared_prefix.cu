@@ -199,6 +199,21 @@ extern "C" size_t cacheir_b200_shared_prefix_workspace_bytes(int batch, int head
   return prefix_plan_bytes(batch) + prefix_ml_bytes(batch, heads, pieces) + static_cast<size_t>(pieces) * batch * heads * dim * 4;
 }
 
+extern "C" int cacheir_b200_shared_prefix_launches(int batch, int heads, int kv_heads, int dim, int page_size, int groups, int dtype) {
+  if (batch <= 0 || heads <= 0) return 0;
+  if (kv_heads <= 0 || heads % kv_heads != 0 || dim <= 0 || page_size <= 0) return CACHEIR_B200_EINVAL;
+  cacheir_b200_prefix_args a{};
+  a.batch = batch;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.dim = dim;
+  a.page_size = page_size;
+  a.num_slots = a.max_pages = a.prefix_pages = 1;
+  a.groups = groups;
+  a.dtype = dtype;
+  return prefix_fast_supported(a) ? prefix_fast_launches(groups) : 2;
+}
+
 extern "C" int cacheir_b200_shared_prefix_attention(const cacheir_b200_prefix_args* args, void* stream) {
   if (!args) return CACHEIR_B200_EINVAL;
   cacheir_b200_prefix_args a = *args;

@@ -90,6 +90,7 @@ inline size_t prefix_ml_bytes(int batch, int heads, int pieces) { return round_u
 
 // Tensor-core kernels (shared_prefix_mma.cu): 16-bit types, head sizes 64 and 128, pages of a multiple of 16 tokens.
 bool prefix_fast_supported(const cacheir_b200_prefix_args& a);
+int prefix_fast_launches(int groups);
 int launch_prefix_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cudaStream_t stream);
 
 }  // namespace cb200

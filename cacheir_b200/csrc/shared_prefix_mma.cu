@@ -1214,6 +1214,8 @@ bool prefix_fast_supported(const cacheir_b200_prefix_args& a) {
          static_cast<long long>(a.kv_heads) * ((group + 15) / 16) <= 65535 && most_units(a, rows_of_tile(a)) <= 0x7fffffffLL;
 }
 
+int prefix_fast_launches(int groups) { return groups > kPlanGroups ? 4 : groups > 0 ? 3 : 2; }
+
 int launch_prefix_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cudaStream_t stream) {
   if (a.dtype == CACHEIR_B200_F16) return a.dim == 128 ? launch_fast<__half, 128>(a, parts, stream) : launch_fast<__half, 64>(a, parts, stream);
   return a.dim == 128 ? launch_fast<__nv_bfloat16, 128>(a, parts, stream) : launch_fast<__nv_bfloat16, 64>(a, parts, stream);

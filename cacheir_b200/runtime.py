@@ -31,7 +31,7 @@ from typing import Any, Callable, Iterable
 import numpy as np
 import torch
 
-from . import hybrid_ops, ops
+from . import hybrid_ops, ops, serving_ops
 from .artifact import CompileArtifact
 from .kv_cache import B200KVPageAllocator, B200PagedKVCache, KVPoolExhausted
 from .quantization import B200PackedWeight, concat_rows, quant_bits, to_tiled
@@ -132,8 +132,9 @@ class _Engine:
     def __init__(self, artifact: Any, *, device: torch.device, dtype: torch.dtype, weights: B200WeightStore | None,
                  tensor_source: Any, kv_allocator: B200KVPageAllocator | None, max_seq_len: int | None,
                  use_cuda_graph: bool, attention_splits: int, max_plans: int, tensor_parallel: TensorParallel | None = None,
-                 kv_dtype: str = "same", fuse_attention_prepass: bool = True):
+                 kv_dtype: str = "same", fuse_attention_prepass: bool = True, shared_prefixes: bool = False):
         self.artifact = artifact
+        self.shared_prefixes = bool(shared_prefixes)                 # decode steps read the pages that neighbours alias once
         self.fuse_attention_prepass = bool(fuse_attention_prepass)   # attention writes the next projection's activation planes
         self.tp = tensor_parallel or TensorParallel(0, 1)
         self.device = device
@@ -152,6 +153,8 @@ class _Engine:
         if self.allocator.page_size != self.page_size:
             raise ValueError("kv_allocator page_size differs from the artifact's decode page size")
         self.ragged = bool(getattr(self.config, "ragged", False))
+        if self.shared_prefixes and (self.ragged or kv_dtype != "same"):
+            raise ValueError("shared_prefixes needs a Llama-shaped model with pages of the activation type")
         self.plan_class: type = RaggedPlan if self.ragged else _DecodePlan
         if self.ragged:
             if self.tp.enabled or kv_dtype != "same" or dtype == torch.float16:
@@ -470,7 +473,8 @@ class _Engine:
         length or page list changed. Admitting or retiring a request therefore costs a few small copies, not
         a new lowering and a new CUDA-graph capture."""
         needed_pages = max((s.kv_cache.tokens + 1 + self.page_size - 1) // self.page_size for s in sessions)
-        return self._plan(("decode", len(sessions)), needed_pages, lambda width: self.plan_class(self, len(sessions), width))
+        more = {"shared_prefixes": True} if self.shared_prefixes else {}
+        return self._plan(("decode", len(sessions)), needed_pages, lambda width: self.plan_class(self, len(sessions), width, **more))
 
 
 class _DecodePlan:
@@ -478,13 +482,17 @@ class _DecodePlan:
     fixed batch size; optionally a CUDA graph of that list."""
 
     decodes = True       # one row per sequence, lengths advance on the device
+    groups: serving_ops.PrefixGroups | None = None       # of rows that alias pages (a plan with `shared_prefixes`)
+    synced_groups: list[tuple[str, int]] | None = None
 
-    def __init__(self, engine: _Engine, batch: int, width: int):
+    def __init__(self, engine: _Engine, batch: int, width: int, shared_prefixes: bool = False):
         self.engine = engine
         self.batch = batch
         self.width = width
         self.pool_generation = engine.allocator.generation
         self._make_buffers()
+        if shared_prefixes:
+            self._make_groups()
         self.synced_owner_state: list[tuple[str, int, int, int]] | None = None
         self.repeat_key: tuple | None = None     # the session list whose next steps need only new token ids (see _repeat_step)
         self.repeat_tokens: list[int] = []
@@ -508,6 +516,36 @@ class _DecodePlan:
         self.host_ids = torch.zeros((batch,), dtype=torch.int64).pin_memory()
         self.host_lens = torch.zeros((batch,), dtype=torch.int32).pin_memory()
         self.host_table = torch.zeros((batch, width), dtype=torch.int32).pin_memory()
+
+    def _make_groups(self) -> None:
+        # as many groups as there are rows, most of them empty; one buffer, so that they change with one copy
+        batch, width = self.batch, self.width
+        cuts = (batch + 1, batch, batch * width)
+        device = torch.zeros((sum(cuts),), device=self.engine.device, dtype=torch.int32)
+        host = torch.zeros((sum(cuts),), dtype=torch.int32).pin_memory()
+        self.group_words = (device, host)
+        rows, lens, table = device.split(cuts)
+        self.groups = serving_ops.PrefixGroups(rows, table.view(batch, width), lens)
+        self.host_groups = tuple(part.numpy() for part in host.split(cuts))
+
+    def _sync_groups(self, caches: list[B200PagedKVCache]) -> None:
+        """The groups of neighbours that alias pages. They change only with who is in the batch: what a session shares, it shares from its
+        first token on."""
+        state = [(c.owner_id, c.epoch) for c in caches]
+        if state == self.synced_groups:
+            return
+        rows, lens, table = self.host_groups
+        rows[:] = len(caches)
+        lens[:] = 0
+        found = serving_ops.prefix_groups(caches, "cpu")
+        if found is None:
+            rows[:] = 0                                          # every row outside every group
+        else:
+            rows[: found.rows.numel()] = found.rows.numpy()
+            lens[: found.lens.numel()] = found.lens.numpy()
+            table.reshape(self.batch, self.width)[: found.table.shape[0], : found.table.shape[1]] = found.table.numpy()
+        self.group_words[0].copy_(self.group_words[1], non_blocking=True)
+        self.synced_groups = state
 
     # -- graph lowering --------------------------------------------------------------
     def _emit(self, fn: Callable[[], None], count_key: str, launches: int = 1) -> None:
@@ -832,6 +870,13 @@ class _DecodePlan:
                 self._emit(lambda: ops.kv_append_q8(k, v, k_pool, v_pool, kv_scales, self.page_table, self.positions), "b200.kv_append_q8")
             else:
                 self._emit(lambda: ops.kv_append(k, v, k_pool, v_pool, self.page_table, self.positions), "b200.kv_append")
+        if self.groups is not None:
+            scratch = eng.scratch("shared_prefix", serving_ops.shared_prefix_workspace_bytes(self.batch, heads, head_dim))
+            self._emit(lambda: serving_ops.shared_prefix_attention(q3, k_pool, v_pool, self.page_table, self.seq_lens, self.groups, out=out3,
+                                                                   workspace=scratch),
+                       "b200.shared_prefix_attention",
+                       launches=serving_ops.shared_prefix_launches(self.batch, heads, kv_heads, head_dim, eng.page_size, self.batch, q.dtype))
+            return out, False
         if (quant_ws is not None and splits == 1 and kv_scales is None
                 and ops.attention_quantize_supported(self.batch, heads, kv_heads, self.width, eng.page_size, head_dim, out.dtype)):
             self._emit(lambda: ops.paged_attention_decode_batch_quantize(q3, k_pool, v_pool, self.page_table, self.seq_lens,
@@ -865,6 +910,8 @@ class _DecodePlan:
             for row, s in enumerate(sessions):
                 lens[row] = s.kv_cache.tokens - 1   # the step itself advances the device copy by one
             self.seq_lens.copy_(self.host_lens, non_blocking=True)
+        if self.groups is not None:
+            self._sync_groups([s.kv_cache for s in sessions])
         self.synced_owner_state = state
 
     def sync_prefill_rows(self, rows: list[tuple[B200PagedKVCache, int, int]]) -> None:
@@ -1095,6 +1142,7 @@ class B200DecodeRuntime:
         memory_limit_mb: float | None = None,
         kv_dtype: str = "same",
         fuse_attention_prepass: bool = True,
+        shared_prefixes: bool = False,
         _engine: _Engine | None = None,
     ):
         if isinstance(artifact, (str, Path)):
@@ -1117,7 +1165,7 @@ class B200DecodeRuntime:
                 _engine = _Engine(artifact, device=dev, dtype=selected, weights=weights, tensor_source=tensor_source,
                                   kv_allocator=kv_allocator, max_seq_len=max_seq_len, use_cuda_graph=use_cuda_graph,
                                   attention_splits=attention_splits, max_plans=max_plans, tensor_parallel=tensor_parallel,
-                                  kv_dtype=kv_dtype, fuse_attention_prepass=fuse_attention_prepass)
+                                  kv_dtype=kv_dtype, fuse_attention_prepass=fuse_attention_prepass, shared_prefixes=shared_prefixes)
         self._engine = _engine
         self.artifact = _engine.artifact
         self.device = _engine.device
@@ -1573,6 +1621,16 @@ class B200DecodeRuntime:
             yield self.tokenizer.decode([next_id])
             logits = self.run([[next_id]], mode="decode")
 
+    def score_tokens(self, token_ids, *, top: int = 0, temperature: float = 1.0) -> serving_ops.TokenLogprobs:
+        """Runs `token_ids` as a new prompt and gives the log probability of every token but the first under what comes before it, the
+        entropies of those distributions, and the `top` likeliest tokens there (`serving_ops.token_logprobs`)."""
+        ids = [int(t) for t in token_ids]
+        if len(ids) < 2:
+            raise ValueError("score_tokens needs at least two tokens")
+        logits = self.run([ids], mode="prefill", reset_kv=True)
+        tokens = torch.tensor(ids[1:], dtype=torch.int64).to(self.device)
+        return serving_ops.token_logprobs(logits[0, :-1], tokens, top=top, temperature=temperature)
+
     def remember_prefix(self, token_ids) -> None:
         self.prefix_cache.put(token_ids, self.kv_cache)
 
@@ -1610,6 +1668,8 @@ class B200DecodeRuntime:
         from . import _lib
         with torch.cuda.device(self.device):
             status = hybrid_ops.device_status() if self._engine.ragged else int(_lib.load().cacheir_b200_device_status(1))
+            if status == 0 and self._engine.shared_prefixes:
+                status = _lib.group_device_status()
         if status != 0:
             raise RuntimeError(f"cacheir_b200 device status {status:#x}: a bounded wait on the GPU gave up "
                                f"(kernel class {status >> 8}, wait {status & 0xFF}); the last results are undefined")

@@ -274,8 +274,8 @@ class PrefixGroups:
 
 def prefix_groups(caches, device: torch.device | str, *, min_tokens: int = 1) -> PrefixGroups | None:
     """The groups of a batch of `kv_cache.B200PagedKVCache`: neighbours that alias the same leading pages, with as many common tokens as all
-    of a group's rows share. A row joins the group before it where that has at least `min_tokens` common tokens with it. None: no two
-    neighbours share anything."""
+    of a group's rows share. A row joins the group before it where they have at least `min_tokens` in common and no fewer tokens are then
+    shared in all than without it. None: no two neighbours share anything."""
     starts, shared, page_size = [0], [], None
     for cache in caches:
         ids, page_size = cache.page_ids()[: cache.tokens // cache.page_size], cache.page_size       # whole pages
@@ -285,7 +285,8 @@ def prefix_groups(caches, device: torch.device | str, *, min_tokens: int = 1) ->
                 if a != b:
                     break
                 common += 1
-            if common * page_size >= max(1, min_tokens):
+            rows = starts[-1] - starts[-2]
+            if common * page_size >= max(1, min_tokens) and (rows == 1 or rows * common >= (rows - 1) * len(shared[-1])):
                 shared[-1] = shared[-1][:common]
                 starts[-1] += 1
                 continue
@@ -303,6 +304,12 @@ def prefix_groups(caches, device: torch.device | str, *, min_tokens: int = 1) ->
 def shared_prefix_workspace_bytes(batch: int, heads: int, head_dim: int) -> int:
     """Scratch of `shared_prefix_attention`."""
     return int(_lib.load_group("serving").cacheir_b200_shared_prefix_workspace_bytes(int(batch), int(heads), int(head_dim)))
+
+
+def shared_prefix_launches(batch: int, heads: int, kv_heads: int, head_dim: int, page_size: int, groups: int, dtype: torch.dtype) -> int:
+    """Kernels that one `shared_prefix_attention` launches for these extents (aligned, dense q)."""
+    return int(_lib.load_group("serving").cacheir_b200_shared_prefix_launches(int(batch), int(heads), int(kv_heads), int(head_dim), int(page_size),
+                                                                             int(groups), dtype_code(dtype)))
 
 
 def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,

@@ -108,6 +108,9 @@ typedef struct {
   float softmax_scale;
 } cacheir_b200_prefix_args;
 size_t cacheir_b200_shared_prefix_workspace_bytes(int batch, int heads, int dim);
+/* Kernels that one call launches for these extents (aligned, dense q): 2 on CUDA cores; on tensor cores (fp16 and bf16, dim 64 and 128,
+ * pages of a multiple of 16 tokens, up to 64 query heads per key/value head) 2 without groups, 3 with up to 64 of them, 4 with more. */
+int cacheir_b200_shared_prefix_launches(int batch, int heads, int kv_heads, int dim, int page_size, int groups, int dtype);
 int cacheir_b200_shared_prefix_attention(const cacheir_b200_prefix_args* args, void* stream);
 
 /* ------------------------------------------------------------------------

@@ -219,3 +219,32 @@ def test_groups_of_a_batch_are_the_pages_that_neighbours_alias():
     groups = S.prefix_groups([a, b, e, f], "cpu", min_tokens=12)
     assert groups.rows.tolist() == [0, 1, 2, 4] and groups.lens.tolist() == [0, 0, 16]
     assert groups.table[2].tolist() == e.page_ids()[:4]
+
+
+def test_a_row_joins_a_group_only_where_no_fewer_tokens_are_shared():
+    from cacheir_b200 import serving_ops as S
+    from cacheir_b200.kv_cache import B200KVPageAllocator, B200PagedKVCache
+
+    alloc = B200KVPageAllocator(page_size=4)
+    first = B200PagedKVCache(alloc, 1)
+    first.extend(40)
+
+    def cache(common):
+        c = B200PagedKVCache(alloc, 1)
+        c.share_prefix(first, common)
+        c.extend(3)
+        return c
+    long, short = [cache(36) for _ in range(3)], [cache(8) for _ in range(4)]
+    groups = S.prefix_groups([*long, *short], "cpu")
+    assert groups.rows.tolist() == [0, 3, 7] and groups.lens.tolist() == [36, 8]
+    groups = S.prefix_groups([long[0], *short, long[1]], "cpu")       # (a lone row loses nothing by joining)
+    assert groups.rows.tolist() == [0, 6] and groups.lens.tolist() == [8]
+
+
+def test_launches_by_extents(lib):
+    from cacheir_b200 import serving_ops as S
+
+    launches = lambda groups, dtype=torch.float16, dim=128, page=16, heads=32, kv=8: S.shared_prefix_launches(4, heads, kv, dim, page, groups, dtype)
+    assert [launches(0), launches(1), launches(64), launches(65)] == [2, 3, 3, 4]
+    assert [launches(1, torch.float32), launches(1, dim=80), launches(1, page=24), launches(1, heads=130, kv=2)] == [2] * 4
+    assert launches(1, torch.bfloat16, dim=64, page=48) == 3
