@@ -98,7 +98,8 @@ prefix_general_kernel(const cacheir_b200_prefix_args a, const PrefixParts parts,
       for (int d = 0; d < D; ++d) s = fmaf(s_q[r * D + d], s_k[lane * (D + 1) + d], s);
       s = lane < n && k0 + lane < row_len[e] ? s * qscale : -INFINITY;
       const float m_new = fmaxf(m_run[e], warp_max(s));
-      const float corr = m_new > -INFINITY ? exp2f(m_run[e] - m_new) : 1.f, p = m_new > -INFINITY ? exp2f(s - m_new) : 0.f;
+      const float less = m_new > -INFINITY ? m_new : 0.f;             // (nothing seen yet: weights 0, but what is no number stays none)
+      const float corr = exp2f(m_run[e] - less), p = exp2f(s - less);
       l_run[e] = l_run[e] * corr + warp_sum(p);
       m_run[e] = m_new;
       s_p[r * (kTileKeys + 1) + lane] = p;
@@ -158,7 +159,7 @@ prefix_join_kernel(const cacheir_b200_prefix_args a, const PrefixParts parts) {
   for (int s = from; s < parts.pieces; ++s) m = fmaxf(m, parts.ml[(s * step + at) * 2]);
   for (int s = from; s < parts.pieces; ++s) {
     const float ms = parts.ml[(s * step + at) * 2];
-    if (ms > -INFINITY) l += parts.ml[(s * step + at) * 2 + 1] * exp2f(ms - m);
+    l = fmaf(parts.ml[(s * step + at) * 2 + 1], ms > -INFINITY ? exp2f(ms - m) : 0.f, l);
   }
   for (int d = threadIdx.x; d < a.dim; d += 128) {
     float o = 0.f;
@@ -166,7 +167,7 @@ prefix_join_kernel(const cacheir_b200_prefix_args a, const PrefixParts parts) {
       const float ms = parts.ml[(s * step + at) * 2];
       if (ms > -INFINITY) o = fmaf(parts.acc[(s * step + at) * a.dim + d], exp2f(ms - m), o);
     }
-    Elem<T>::st(static_cast<T*>(a.out) + static_cast<size_t>(row) * a.out_stride + static_cast<size_t>(head) * a.dim + d, l > 0.f ? o / l : 0.f);
+    Elem<T>::st(static_cast<T*>(a.out) + static_cast<size_t>(row) * a.out_stride + static_cast<size_t>(head) * a.dim + d, l > 0.f || l != l ? o / l : 0.f);
   }
 }
 
@@ -224,8 +225,8 @@ extern "C" int cacheir_b200_shared_prefix_attention(const cacheir_b200_prefix_ar
   if (a.groups > a.batch) return CACHEIR_B200_EINVAL;
   if (a.groups > 0 && (!a.group_rows || !a.prefix_table || !a.prefix_lens || a.prefix_pages <= 0)) return CACHEIR_B200_EINVAL;
   if (a.dim > kGeneralDim) return CACHEIR_B200_EUNSUPPORTED;
-  if (a.batch > 65535 || a.kv_heads > 65535 || static_cast<long long>(a.max_pages) * a.page_size > 0x7fffffffLL ||
-      static_cast<long long>(a.prefix_pages) * a.page_size > 0x7fffffffLL)
+  if (a.batch > 65535 || a.kv_heads > 65535 || static_cast<long long>(a.max_pages) * a.page_size > 1LL << 30 ||
+      static_cast<long long>(a.prefix_pages) * a.page_size > 1LL << 30)
     return CACHEIR_B200_ELIMIT;
   if (!a.workspace || a.workspace_bytes < cacheir_b200_shared_prefix_workspace_bytes(a.batch, a.heads, a.dim)) return CACHEIR_B200_EWORKSPACE;
   if (!aligned_to(a.workspace, 16)) return CACHEIR_B200_EALIGN;

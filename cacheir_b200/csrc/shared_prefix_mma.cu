@@ -928,20 +928,21 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         sc[n][e] = v;
         top[e >> 1] = fmaxf(top[e >> 1], v);
       }
-    float corr[2];
+    float corr[2], less[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      const float m_new = fmaxf(m_run[r], top[r]);               // finite: every chunk has a key that counts
-      corr[r] = ex2(m_run[r] - m_new);
+      const float m_new = fmaxf(m_run[r], top[r]);               // (-inf where all scores so far are)
+      less[r] = m_new > -INFINITY ? m_new : 0.f;
+      corr[r] = ex2(m_run[r] - less[r]);
       m_run[r] = m_new;
     }
     float pr[2][4];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pr[n][e] = ex2(sc[n][e] - m_run[e >> 1]);
+      for (int e = 0; e < 4; ++e) pr[n][e] = ex2(sc[n][e] - less[e >> 1]);
 #pragma unroll
     for (int r = 0; r < 2; ++r) l_run[r] = l_run[r] * corr[r] + (pr[0][2 * r] + pr[0][2 * r + 1] + pr[1][2 * r] + pr[1][2 * r + 1]);
     const uint32_t pa[4] = {pack_pair<T>(pr[0][0], pr[0][1]), pack_pair<T>(pr[0][2], pr[0][3]), pack_pair<T>(pr[1][0], pr[1][1]),
@@ -1046,7 +1047,7 @@ prefix_join_pieces_kernel(const __grid_constant__ OwnParams p) {
     const Deal deal(of.units, ctas);
     const int row_tiles = (of.in.rows + p.tile_rows - 1) / p.tile_rows;
     const int all = kItemUnits + key_tiles(of.in.prefix), item0 = of.in.start + (kvh * row_tiles + (row - of.in.row) / p.tile_rows) * all;
-    pieces = deal.owner(item0 + all - 1) - deal.owner(item0 + kItemUnits) + 1;
+    pieces = min(max(deal.owner(item0 + all - 1) - deal.owner(item0 + kItemUnits) + 1, 0), p.parts.pieces);      // (as it is where groups ascend)
   }
   const size_t at0 = static_cast<size_t>(row) * a.heads + head0, step = static_cast<size_t>(a.batch) * a.heads;
   const int sources = p.splits + pieces;
@@ -1075,8 +1076,10 @@ prefix_join_pieces_kernel(const __grid_constant__ OwnParams p) {
       if (i * 32 + lane < sources) s_w[h][i * 32 + lane] = ms[i] * inv;
   }
   __syncthreads();
+  // A piece without weight is not looked at: a row that ends before it has zeros there, times values that may be no numbers.
   // Four neighbouring outputs are a place; ITEMS places of a thread and DEEP pieces of each are on their way at once.
   const int places = heads * (D / 4);
+  const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && a.out_stride % 4 == 0;
   auto finish = [&](auto items, auto deep) {
     constexpr int ITEMS = decltype(items)::value, DEEP = decltype(deep)::value;
     for (int i0 = threadIdx.x; i0 < places; i0 += ITEMS * kJoinThreads) {
@@ -1099,7 +1102,7 @@ prefix_join_pieces_kernel(const __grid_constant__ OwnParams p) {
         for (int e = 0; e < DEEP; ++e)
 #pragma unroll
           for (int j = 0; j < ITEMS; ++j)
-            x[e][j] = live[j] && k + e < sources ? *reinterpret_cast<const float4*>(acc[j] + slot_of(k + e) * step * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[e][j] = live[j] && k + e < sources && wgt[j][k + e] != 0.f ? *reinterpret_cast<const float4*>(acc[j] + slot_of(k + e) * step * D) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int e = 0; e < DEEP; ++e)
 #pragma unroll
@@ -1114,8 +1117,10 @@ prefix_join_pieces_kernel(const __grid_constant__ OwnParams p) {
         if (live[j]) {
           const int i = i0 + j * kJoinThreads, h = i / (D / 4), d = i % (D / 4) * 4;
           T* out = static_cast<T*>(a.out) + static_cast<size_t>(row) * a.out_stride + static_cast<size_t>(head0 + h) * D + d;
+          if (wide) *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<T>(v[j][0], v[j][1]), pack_pair<T>(v[j][2], v[j][3]));
+          else
 #pragma unroll
-          for (int e = 0; e < 4; ++e) Elem<T>::st(out + e, v[j][e]);
+            for (int e = 0; e < 4; ++e) Elem<T>::st(out + e, v[j][e]);
         }
     }
   };

@@ -388,6 +388,70 @@ def test_shared_prefix_attention_against_64_bits(dtype, shape):
     _check_attention(S.shared_prefix_attention(q, keys, values, table, lens, None), want, size, dtype)
 
 
+MANY = [
+    # as SHAPES; more groups than a warp (32) and than a block (64) lays out by itself, several items for every block, tiles of one and of two
+    # groups of 128 query rows in turn, heads per key/value head that do not divide 128, long common parts in many pieces, long own parts
+    ([(1 + i % 3, 20 + 37 * i) for i in range(36)], [[j for j in range(1 + i % 3)] for i in range(36)], 8, 2, 128, 16),
+    ([(2, 40 + i % 5 * 130) for i in range(70)], [[i % 7, 0] for i in range(70)], 8, 2, 64, 32),
+    ([(i % 4, 300 if i % 5 else 0) for i in range(130)], [[i % 19 + 1] * (i % 4) for i in range(130)], 4, 4, 128, 16),
+    ([(8, 1000)] * 8, [[3] * 8] * 8, 64, 8, 128, 16),
+    ([(20 if i % 2 else 3, 500 - 9 * i) for i in range(40)], [[i % 30 for j in range(20 if i % 2 else 3)] for i in range(40)], 64, 4, 128, 16),
+    ([(90, 700), (30, 260), (7, 1400)] * 6, [[i % 40 for i in range(90)], [i for i in range(30)], [0] * 7] * 6, 36, 12, 64, 16),
+    ([(64, 9000)], [[i % 9 for i in range(64)]], 8, 2, 128, 16),
+    ([(2, 6000), (1, 900)], [[5, 3000], [2100]], 16, 4, 128, 16),
+    ([(3, 31)] * 11, [[1, 700, 33]] * 11, 48, 12, 128, 48),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", range(len(MANY)))
+def test_shared_prefix_attention_of_many_groups_and_pieces(dtype, shape):
+    from cacheir_b200 import serving_ops as S
+
+    groups, tails, heads, kv_heads, dim, page = MANY[shape]
+    q, keys, values, table, lens, starts, prefix_table, prefix_lens = _paged(shape + 50, groups, tails, heads, kv_heads, dim, page, dtype)
+    given = S.PrefixGroups(_i32(starts), prefix_table, _i32(prefix_lens))
+    got = S.shared_prefix_attention(q, keys, values, table, lens, given)
+    want, size = _attend(q, keys, values, table, lens, dim ** -0.5, _owners(starts, len(lens)), prefix_table, prefix_lens)
+    _check_attention(got, want, size, dtype)
+    assert torch.equal(got, S.shared_prefix_attention(q, keys, values, table, lens, given))
+
+
+@pytest.mark.parametrize("dtype,dim,page", [(torch.float16, 128, 16), (torch.bfloat16, 64, 16), (torch.float32, 64, 16), (torch.bfloat16, 80, 16)])
+def test_shared_prefix_attention_with_infinite_scores_and_values_that_are_no_numbers(dtype, dim, page):
+    from cacheir_b200 import serving_ops as S
+
+    # a whole tile of keys and single ones, common and own, with a score of -inf: they have no weight
+    groups, tails = [(3, 200), (2, 300)], [[40, 0, 9], [17, 90]]
+    q, keys, values, table, lens, starts, prefix_table, prefix_lens = _paged(5, groups, tails, 8, 2, dim, page, dtype)
+    q[..., 0] = 1.0
+    for ids, tokens in ((prefix_table[0], range(128)), (prefix_table[1], (0, 5, 299)), (table[0], (*range(200, 216), 230)), (table[4], (389,))):
+        for t in tokens:
+            keys[ids[t // page], :, t % page, 0] = float("-inf")
+    for b in range(3):           # (own copies of the page that the prefix ends in hold what it holds)
+        keys[table[b, 192 // page], :, : 200 % page] = keys[prefix_table[0, 192 // page], :, : 200 % page]
+    for b in (3, 4):
+        keys[table[b, 288 // page], :, : 300 % page] = keys[prefix_table[1, 288 // page], :, : 300 % page]
+    given = S.PrefixGroups(_i32(starts), prefix_table, _i32(prefix_lens))
+    want, size = _attend(q, keys, values, table, lens, dim ** -0.5, _owners(starts, 5), prefix_table, prefix_lens)
+    for g in (given, None):
+        _check_attention(S.shared_prefix_attention(q, keys, values, table, lens, g), want, size, dtype)
+    # a row with a NaN among its keys is NaN in every head that sees it, the others are as before; a row of no tokens is 0 whatever its group holds
+    keys[table[3, 305 // page], 1, 305 % page, 3] = float("nan")
+    lens[1] = 0
+    values[prefix_table[0, 0], 0, 3] = float("nan")
+    values[prefix_table[0, 1], 1, 3] = float("inf")
+    for g in (given, None):
+        got = S.shared_prefix_attention(q, keys, values, table, lens, g)
+        assert bool(got[3, 4:].isnan().all()) and bool((got[1] == 0).all())
+        _check_attention(got[3:, :4], want[3:, :4], size[3:, :4], dtype)
+        _check_attention(got[4], want[4], size[4], dtype)
+    keys[prefix_table[1, 0], 0, 0, 1] = float("nan")
+    keys[prefix_table[1, 0], 0, 0, 0] = 0.0
+    got = S.shared_prefix_attention(q, keys, values, table, lens, given)
+    assert bool(got[3:, :4].isnan().all()) and bool(got[4, 4:].isfinite().all())
+
+
 @pytest.mark.parametrize("dtype,dim,page", [(torch.float16, 128, 16), (torch.bfloat16, 64, 16), (torch.float32, 64, 16), (torch.float16, 128, 8)])
 def test_shared_prefix_attention_edges(dtype, dim, page):
     """Rows outside every group, empty groups, rows that end inside their prefix or are empty, prefixes cut by their table, foreign page ids
