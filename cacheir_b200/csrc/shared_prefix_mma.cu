@@ -9,10 +9,18 @@
 // Common part. An item is (group, key/value head, tile of up to 256 query rows); its keys come in tiles of 128. The key tiles of all items,
 // in a row, are cut evenly over the blocks, so that lengths and sizes of groups do not matter; an item that is cut leaves one piece per
 // block. One warp brings keys and one values (TMA, 16 tokens at a time, into a ring of 32 KB slots; by one warp the copies' issue, 66 cycles
-// each, was what the tensor cores waited for), one issues the MMAs, and two groups of four warps do the softmax, a thread per query row. Above 128 rows each group of warps has its own 128 of them and the two take turns on the
-// tensor cores with the same keys; else the first one has them all and scores run one tile ahead. A row's maximum is a reference that
-// moves only when it is exceeded by 2^14, so that the outputs, which stay in tensor memory, are hardly ever rescaled; probabilities are
-// rounded to the element type as the second MMA's operand, their sums are not.
+// each, was what the tensor cores waited for), one issues the MMAs, and two groups of four warps do the softmax, a thread per query row.
+// Above 128 rows each group of warps has its own 128 of them and the two take turns on the tensor cores with the same keys; else the first
+// one has them all and scores run one tile ahead. A row's maximum is a reference that moves only when it is exceeded by 2^14, so that the
+// outputs, which stay in tensor memory, are hardly ever rescaled; probabilities are rounded to the element type as the second MMA's operand,
+// their sums are not.
+//
+// Measured (32 query and 8 key/value heads of 128, fp16, whole call): 64 rows behind 32768 common tokens 54 us, of which 25.6 us are the
+// bytes and 20.8 us the products; 32 rows behind 2048 tokens 21.5 us (bytes 7.1 us). 128 rows in 16 groups of ragged prefixes with 64 and 8
+// heads, bf16: 68.9 us (bytes 46.5 us). A call spends about 5.5 us before the first scores (launch, plan, page ids, copies), and about 3 us on
+// joining. In between a tile of 256 query rows takes 3300 cycles, of which the tensor cores work 2048: the rest is the way from scores by
+// the softmax to the second product (2300 cycles a step, 1500 of them exponentials), which the other group of warps hides in part. Neither
+// a share of the exponentials by polynomials nor reading scores once into 128 registers changed that (56.0 us became 55.7 and 56.3).
 #include "shared_prefix.cuh"
 
 #include <cuda.h>
@@ -26,6 +34,7 @@ namespace {
 using namespace ptx;
 
 constexpr int kKeys = 128;                     // keys of a tile
+constexpr int kFirst = 96;                     // .. whose probabilities go to the second MMA first: less of it is left when the others come
 constexpr int kRows = 128;                     // query rows of a group of warps
 constexpr int kChunk = 16;                     // keys that one copy brings: no page ends inside
 constexpr int kCommonThreads = 352;
@@ -197,12 +206,15 @@ __device__ __forceinline__ Weights group_weights(const PlanGroup& g, int units, 
 }
 // Blocks that take part. No item may be in more pieces than there is scratch for: n tiles touch ceil((n - 1) / share) + 1 blocks at most. And
 // the common parts get as many SMs as is their share of the work, so that the other kernel can have the rest of them meanwhile: 16 own
-// tokens of a key/value head (8 KB) take an SM about a twelfth of a unit's time (64 KB). `lens`: tokens of all rows.
-__device__ __forceinline__ int plan_ctas(const CommonParams& p, int units, const Weights& w, long long lens, int grid) {
+// tokens of a key/value head (8 KB) take an SM about a sixteenth of a unit's time (64 KB), and a row's own part costs as much as eight of
+// those before it has any. `lens`: tokens of all rows. (64 rows with 144 own tokens on average behind 32768, 128 rows with 350 behind up to 4095:
+// 53.5 and 69.6 us; with a twelfth and one 56.0 and 69.4, with an eighth and one 52.0 and 78.5.)
+__device__ __forceinline__ int plan_ctas(const cacheir_b200_prefix_args& a, int pieces, int own_heads, int units, const Weights& w, long long lens, int grid) {
   if (units <= 0) return 0;
-  const int least = max(1, (w.longest - 1 + p.parts.pieces - 2) / (p.parts.pieces - 1));
-  const float cost = static_cast<float>(w.cost), own = (static_cast<float>(max(lens - w.common, 0LL)) / kChunk + p.a.batch) * p.own_heads / 12.f;
-  return max(1, min(min(grid, units / least), static_cast<int>(kNumSMs * cost / (cost + own)) + 1));
+  const int least = max(1, (w.longest - 1 + pieces - 2) / (pieces - 1));
+  const float cost = static_cast<float>(w.cost), own = __fmul_rn(static_cast<float>(max(lens - w.common, 0LL) / kChunk + 8LL * a.batch), own_heads / 16.f);
+  const float sms = __fdiv_rn(__fmul_rn(kNumSMs, cost), __fadd_rn(cost, own));       // (two kernels work this out and have to agree)
+  return max(1, min(min(grid, units / least), static_cast<int>(sms) + 1));
 }
 // Tokens of all rows, a thread's part of them.
 __device__ __forceinline__ long long lens_part(const cacheir_b200_prefix_args& a, int thread, int threads) {
@@ -263,7 +275,7 @@ prefix_plan_kernel(const CommonParams p, const int grid) {
     }
     p.parts.plan->group[p.a.groups].start = base;
     p.parts.plan->units = base;
-    p.parts.plan->ctas = plan_ctas(p, base, w, tokens, grid);
+    p.parts.plan->ctas = plan_ctas(p.a, p.parts.pieces, p.own_heads, base, w, tokens, grid);
   }
 }
 
@@ -333,7 +345,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
   uint64_t* bar_q = empty + kSlots;                            // queries of a group of warps are there
   uint64_t* bar_free = bar_q + 2;                              // .. and their place is free again
   uint64_t* bar_s = bar_free + 2;                              // scores are in tensor memory
-  uint64_t* bar_p = bar_s + 2;                                 // probabilities are, [buffer][half of the keys]
+  uint64_t* bar_p = bar_s + 2;                                 // probabilities are, [buffer][first keys, the others]
   uint64_t* bar_o = bar_p + 4;                                 // .. and have been added to the output
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_o + 2);
   PlanGroup* s_group = reinterpret_cast<PlanGroup*>(tmem_slot + 4);
@@ -399,7 +411,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         for (int i = 0; i < kCommonThreads / 32; ++i) tokens += s_lens[i];
         s_group[a.groups].start = all;
         s_plan[0] = all;
-        s_plan[1] = plan_ctas(p, all, w, tokens, gridDim.x);
+        s_plan[1] = plan_ctas(a, p.parts.pieces, p.own_heads, all, w, tokens, gridDim.x);
       }
     }
   }
@@ -542,9 +554,9 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         const uint64_t v_at = dv + (v_slot * L::kSlotBytes >> 4);
         const uint32_t to = tmem_o + (two ? b_o * D : 0), from = tmem + b_o * kKeys, add = j < (two ? 2 : 1) ? 0u : 1u;
         const bool frees = !two || (j & 1), more = j + 2 < steps;
-        if (leader) {                                          // (the first half of the keys while the other half's probabilities are worked out)
+        if (leader) {                                          // (the first keys while the others' probabilities are worked out)
 #pragma unroll
-          for (int k = 0; k < kKeys / 32; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, k == 0 ? add : 1u);
+          for (int k = 0; k < kFirst / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, k == 0 ? add : 1u);
         }
         __syncwarp();
         if (more) ok = wait_scores(j + 2);
@@ -553,7 +565,7 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
         tc_fence_after();
         if (leader) {
 #pragma unroll
-          for (int k = kKeys / 32; k < kKeys / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, 1u);
+          for (int k = kFirst / 16; k < kKeys / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, 1u);
           tc_commit(smem_u32(&bar_o[b_o]));
           if (frees) tc_commit(smem_u32(&empty[v_slot]));
           if (more) score(j + 2);
@@ -685,16 +697,18 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           tmem_wait_ld(x);
           tmem_ld_x32(scores + 96, y);
           tmem_st_x32(scores, out);
+          if (!whole) masked(x, 64);
+          uint32_t rest[16];
+          weigh(x, rest);
+          tmem_wait_ld(y);
+          tmem_st_x16(scores + 32, rest);
           tmem_wait_st();
           clear_values();
           tc_fence_before();
           mbar_arrive(smem_u32(&bar_p[2 * b]));
-          if (!whole) masked(x, 64);
-          weigh(x, out);
-          tmem_wait_ld(y);
           if (!whole) masked(y, 96);
-          weigh(y, out + 16);
-          tmem_st_x32(scores + 32, out);
+          weigh(y, rest);
+          tmem_st_x16(scores + 48, rest);
         }
         float s0, s1, s2, s3;
         unpair(sum[0], s0, s1);
@@ -758,6 +772,7 @@ struct OwnParams {
   PrefixParts parts;
   int common;                                  // a kernel of common parts runs before
   int tile_rows, head_chunks, splits;
+  int grid;                                    // .. its blocks
   float scale_log2;
 };
 
@@ -782,11 +797,12 @@ __device__ __forceinline__ void mma_pair(float (&c)[4], const uint32_t (&x)[4], 
   else
     mma_bf16(c, x, b0, b1);
 }
-// A row's group (rows and prefix 0 outside every group). Up to 32 groups, a lane each, the warp lays the plan out beside that: one round of
-// loads, and nothing of it has to wait for the common part's kernel.
+// A row's group (rows and prefix 0 outside every group). Up to 32 groups, a lane each, the warp lays the plan out beside that, as nothing of it
+// has to wait for the common part's kernel.
 struct RowGroup {
   PlanGroup in;
-  int group, planned, units;                   // planned: its first unit and the number of units are known already
+  int group, planned, units;                   // planned: its first unit, the number of units and what decides about blocks are known already
+  Weights weights;
 };
 __device__ __forceinline__ RowGroup row_group(const cacheir_b200_prefix_args& a, int tile_rows, int row) {
   RowGroup r{};
@@ -811,6 +827,8 @@ __device__ __forceinline__ RowGroup row_group(const cacheir_b200_prefix_args& a,
   }
   r.planned = 1;
   r.units = __shfl_sync(0xffffffffu, sum, 31);
+  const Weights w = group_weights(mine, own, tile_rows / 2);
+  r.weights = Weights{__reduce_max_sync(0xffffffffu, w.longest), warp_sum64(w.common), warp_sum64(w.cost)};
   const uint32_t found = __ballot_sync(0xffffffffu, mine.rows > 0 && mine.row <= row && row < mine.row + mine.rows);
   if (found == 0) return r;
   r.group = 31 - __clz(found);
@@ -1022,7 +1040,9 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // The pieces of a row, in order: its own keys' parts, then the common ones. A block per key/value head (and up to 16 of its query heads) and
-// row; bound by latency and by the rate at which L2 gives the pieces back.
+// row; bound by latency: which pieces there are is known before the kernels that write them have ended (up to 32 groups), and the first
+// outputs are asked for together with the maxima. (32 rows behind 2048 tokens: 2.1 us from the end of the kernel before to that of this one, 3.8
+// with the plan read back, then the maxima, then the outputs.)
 constexpr int kJoinThreads = 128;
 constexpr int kSources = kMaxPieces + kMaxOwnParts;
 
@@ -1030,92 +1050,120 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
 prefix_join_pieces_kernel(const __grid_constant__ OwnParams p) {
   __shared__ float s_w[16][kSources];
+  __shared__ long long s_lens[kJoinThreads / 32];
   const cacheir_b200_prefix_args& a = p.a;
   const int kvh = blockIdx.x / p.head_chunks, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.heads / a.kv_heads, head0 = kvh * group + blockIdx.x % p.head_chunks * 16, heads = min(16, (kvh + 1) * group - head0);
-  // (the kernel before this one was let in after all earlier ones had ended, and so was this one: the groups may be read ahead)
-  RowGroup of = row_group(a, p.tile_rows, row);
+  int pieces = 0;
+  if (p.common) {
+    // (the kernel before this one was let in after all earlier ones had ended, and so was this one: groups and lengths may be read ahead)
+    RowGroup of = row_group(a, p.tile_rows, row);
+    int ctas = 0;
+    if (of.planned) {
+      const long long mine = warp_sum64(lens_part(a, threadIdx.x, kJoinThreads));
+      if (lane == 0) s_lens[warp] = mine;
+      __syncthreads();
+      long long lens = 0;
+#pragma unroll
+      for (int i = 0; i < kJoinThreads / 32; ++i) lens += s_lens[i];
+      ctas = plan_ctas(a, p.parts.pieces, a.kv_heads * p.head_chunks, of.units, of.weights, lens, p.grid);
+    }
+    const int row_tiles = (of.in.rows + p.tile_rows - 1) / p.tile_rows, all = kItemUnits + key_tiles(of.in.prefix);
+    const int rel = (kvh * row_tiles + (row - of.in.row) / p.tile_rows) * all;
+    if (!of.planned) {
+      chain_wait();
+      if (of.group >= 0) {
+        of.in.start = p.parts.plan->group[of.group].start;
+        of.units = p.parts.plan->units;
+        ctas = p.parts.plan->ctas;
+      }
+    }
+    if (of.in.prefix > 0 && ctas > 0) {                          // (then the row is in a group that has items)
+      const Deal deal(of.units, ctas);
+      const int item0 = of.in.start + rel;
+      pieces = min(max(deal.owner(item0 + all - 1) - deal.owner(item0 + kItemUnits) + 1, 0), p.parts.pieces);      // (as it is where groups ascend)
+    }
+  }
   chain_wait();
   chain_next();
-  int pieces = 0;
-  if (p.common && of.in.prefix > 0) {                            // (then the row is in a group that has items)
-    const int ctas = p.parts.plan->ctas;
-    if (!of.planned) {
-      of.in.start = p.parts.plan->group[of.group].start;
-      of.units = p.parts.plan->units;
-    }
-    const Deal deal(of.units, ctas);
-    const int row_tiles = (of.in.rows + p.tile_rows - 1) / p.tile_rows;
-    const int all = kItemUnits + key_tiles(of.in.prefix), item0 = of.in.start + (kvh * row_tiles + (row - of.in.row) / p.tile_rows) * all;
-    pieces = min(max(deal.owner(item0 + all - 1) - deal.owner(item0 + kItemUnits) + 1, 0), p.parts.pieces);      // (as it is where groups ascend)
-  }
   const size_t at0 = static_cast<size_t>(row) * a.heads + head0, step = static_cast<size_t>(a.batch) * a.heads;
   const int sources = p.splits + pieces;
   auto slot_of = [&](int k) { return k < p.splits ? p.parts.pieces + k : k - p.splits; };
-  for (int h = warp; h < heads; h += kJoinThreads / 32) {        // a warp per head: the weight of every source
-    float m = -INFINITY, l = 0.f, ms[3], ls[3];
+  // A warp per head: the weight of every source.
+  auto weigh = [&] {
+    for (int h = warp; h < heads; h += kJoinThreads / 32) {
+      float m = -INFINITY, l = 0.f, ms[3], ls[3];
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {                                // (at most 72)
-      const int k = i * 32 + lane;
-      float2 x = make_float2(-INFINITY, 0.f);
-      if (k < sources) x = *reinterpret_cast<const float2*>(p.parts.ml + 2 * (slot_of(k) * step + at0 + h));
-      ms[i] = x.x;
-      ls[i] = x.y;
-      m = fmaxf(m, ms[i]);
+      for (int i = 0; i < 3; ++i) {                              // (at most 72)
+        const int k = i * 32 + lane;
+        float2 x = make_float2(-INFINITY, 0.f);
+        if (k < sources) x = *reinterpret_cast<const float2*>(p.parts.ml + 2 * (slot_of(k) * step + at0 + h));
+        ms[i] = x.x;
+        ls[i] = x.y;
+        m = fmaxf(m, ms[i]);
+      }
+      m = warp_max(m);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        ms[i] = ms[i] > -INFINITY ? ex2(ms[i] - m) : 0.f;
+        l += ls[i] * ms[i];
+      }
+      l = warp_sum(l);
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (i * 32 + lane < sources) s_w[h][i * 32 + lane] = ms[i] * inv;
     }
-    m = warp_max(m);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      ms[i] = ms[i] > -INFINITY ? ex2(ms[i] - m) : 0.f;
-      l += ls[i] * ms[i];
-    }
-    l = warp_sum(l);
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (i * 32 + lane < sources) s_w[h][i * 32 + lane] = ms[i] * inv;
-  }
-  __syncthreads();
-  // A piece without weight is not looked at: a row that ends before it has zeros there, times values that may be no numbers.
-  // Four neighbouring outputs are a place; ITEMS places of a thread and DEEP pieces of each are on their way at once.
+    __syncthreads();
+  };
+  // Four neighbouring outputs are a place; ITEMS places of a thread and DEEP pieces of each are on their way at once. A piece without weight
+  // does not count: a row that ends before it has zeros there, times values that may be no numbers.
   const int places = heads * (D / 4);
   const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && a.out_stride % 4 == 0;
   auto finish = [&](auto items, auto deep) {
     constexpr int ITEMS = decltype(items)::value, DEEP = decltype(deep)::value;
-    for (int i0 = threadIdx.x; i0 < places; i0 += ITEMS * kJoinThreads) {
+    for (int first = 0; first < places; first += ITEMS * kJoinThreads) {
       float v[ITEMS][4];
       const float* acc[ITEMS];
       const float* wgt[ITEMS];
       bool live[ITEMS];
 #pragma unroll
       for (int j = 0; j < ITEMS; ++j) {
-        live[j] = i0 + j * kJoinThreads < places;
-        const int i = live[j] ? i0 + j * kJoinThreads : i0, h = i / (D / 4), d = i % (D / 4) * 4;
+        const int at = first + threadIdx.x + j * kJoinThreads;
+        live[j] = at < places;
+        const int i = live[j] ? at : 0, h = i / (D / 4), d = i % (D / 4) * 4;
         acc[j] = p.parts.acc + (at0 + h) * D + d;
         wgt[j] = s_w[h];
         v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0.f;
       }
-#pragma unroll 1
-      for (int k = 0; k < sources; k += DEEP) {
-        float4 x[DEEP][ITEMS];
+      float4 x[DEEP][ITEMS];
+      auto load = [&](int k) {
 #pragma unroll
         for (int e = 0; e < DEEP; ++e)
 #pragma unroll
           for (int j = 0; j < ITEMS; ++j)
-            x[e][j] = live[j] && k + e < sources && wgt[j][k + e] != 0.f ? *reinterpret_cast<const float4*>(acc[j] + slot_of(k + e) * step * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[e][j] = live[j] && k + e < sources ? *reinterpret_cast<const float4*>(acc[j] + slot_of(k + e) * step * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+      };
+      load(0);
+      if (first == 0) weigh();
+#pragma unroll 1
+      for (int k = 0; k < sources; k += DEEP) {
+        if (k > 0) load(k);
 #pragma unroll
         for (int e = 0; e < DEEP; ++e)
 #pragma unroll
           for (int j = 0; j < ITEMS; ++j) {
             const float f = k + e < sources ? wgt[j][k + e] : 0.f;
-            v[j][0] = fmaf(x[e][j].x, f, v[j][0]); v[j][1] = fmaf(x[e][j].y, f, v[j][1]);
-            v[j][2] = fmaf(x[e][j].z, f, v[j][2]); v[j][3] = fmaf(x[e][j].w, f, v[j][3]);
+            if (f != 0.f) {
+              v[j][0] = fmaf(x[e][j].x, f, v[j][0]); v[j][1] = fmaf(x[e][j].y, f, v[j][1]);
+              v[j][2] = fmaf(x[e][j].z, f, v[j][2]); v[j][3] = fmaf(x[e][j].w, f, v[j][3]);
+            }
           }
       }
 #pragma unroll
       for (int j = 0; j < ITEMS; ++j)
         if (live[j]) {
-          const int i = i0 + j * kJoinThreads, h = i / (D / 4), d = i % (D / 4) * 4;
+          const int i = first + threadIdx.x + j * kJoinThreads, h = i / (D / 4), d = i % (D / 4) * 4;
           T* out = static_cast<T*>(a.out) + static_cast<size_t>(row) * a.out_stride + static_cast<size_t>(head0 + h) * D + d;
           if (wide) *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<T>(v[j][0], v[j][1]), pack_pair<T>(v[j][2], v[j][3]));
           else
@@ -1187,10 +1235,10 @@ int launch_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cud
     return CACHEIR_B200_EUNSUPPORTED;
   const int group = a.heads / a.kv_heads, tile_rows = rows_of_tile(a);
   const float scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  const long long most = most_units(a, tile_rows);
+  const int grid = static_cast<int>(most < kNumSMs ? most : kNumSMs);
   if (a.groups > 0) {
     const CommonParams c{a, parts, a.groups > kPlanGroups ? 1 : 0, tile_rows, a.kv_heads * ((group + 15) / 16), scale_log2};
-    const long long most = most_units(a, tile_rows);
-    const int grid = static_cast<int>(most < kNumSMs ? most : kNumSMs);
     cudaError_t e = cudaSuccess;
     if (c.plan_ready) e = launch_chained(prefix_plan_kernel, dim3(1), dim3(1024), 0, stream, c, grid);
     auto kern = prefix_common_kernel<T, D>;
@@ -1199,7 +1247,7 @@ int launch_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cud
     if (e == cudaSuccess) e = launch_chained(kern, dim3(grid), dim3(kCommonThreads), CommonSmem<D>::kBytes, stream, tk_half, tv, tq, c);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  OwnParams o{a, parts, a.groups > 0 ? 1 : 0, tile_rows, (group + 15) / 16, 1, scale_log2};
+  OwnParams o{a, parts, a.groups > 0 ? 1 : 0, tile_rows, (group + 15) / 16, 1, grid, scale_log2};
   const long long blocks = static_cast<long long>(a.batch) * a.kv_heads * o.head_chunks;
   if (blocks > 3 * kNumSMs) return launch_own<T, D, 2>(o, tk, tv, stream);
   if (blocks > kNumSMs) return launch_own<T, D, 4>(o, tk, tv, stream);
