@@ -913,9 +913,9 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   for (int it = 0; it < mine; ++it) {
     ok = warp_wait(bars + stage * 8, phase, (15 << 8) | 12);
     if (!ok) {                                                   // the copies that are still under way are waited for
-      for (int i = it + 1; i < min(mine, it + kStages); ++i) {
-        if (++stage == kStages) { stage = 0; phase ^= 1; }
+      for (int i = it; i < min(mine, it + kStages); ++i) {
         mbar_wait(bars + stage * 8, phase, &g_prefix_status, (15 << 8) | 13);
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
       break;
     }

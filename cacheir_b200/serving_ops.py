@@ -255,8 +255,9 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, rule
     if rows == 0:
         return
     args = ROTARY_BYTES.pack(
-        q.data_ptr(), k.data_ptr(), _ptr(v), q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), positions.data_ptr(), _ptr(slots), turns.data_ptr(), q_stride, k_stride, v_stride, q_out_stride, k_out_stride, rows, heads, kv_heads, dim, rot, layout, num_slots,
-                      page_size, code, rule.factor)
+        q.data_ptr(), k.data_ptr(), _ptr(v), q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), positions.data_ptr(), _ptr(slots),
+        turns.data_ptr(), q_stride, k_stride, v_stride, q_out_stride, k_out_stride, rows, heads, kv_heads, dim, rot, layout, num_slots, page_size,
+        code, rule.factor)
     _launch("rotary_append", (q, k, q_out, positions, turns, slots, v, k_out, k_cache, v_cache), args)
 
 
@@ -400,9 +401,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, *, top: in
     if tokens is not None and (tokens.dtype is not torch.int64 or tokens.numel() != rows or not tokens.is_contiguous()):
         raise ValueError("tokens must be contiguous int64 [R]")
     code, device = dtype_code(logits.dtype), logits.device
-    result = TokenLogprobs(None if tokens is None else torch.empty(rows, dtype=torch.float32, device=device), torch.empty(rows, dtype=torch.float32, device=device),
-                           torch.empty((rows, top), dtype=torch.int64, device=device) if top else None,
-                           torch.empty((rows, top), dtype=torch.float32, device=device) if top else None)
+    entropy = torch.empty(rows, dtype=torch.float32, device=device)
+    result = TokenLogprobs(None if tokens is None else torch.empty_like(entropy), entropy,
+                           entropy.new_empty((rows, top), dtype=torch.int64) if top else None, entropy.new_empty((rows, top)) if top else None)
     _launch("token_logprobs", (logits, tokens), logits.data_ptr(), row_stride if rows > 1 else vocab, _ptr(tokens), _ptr(result.logprobs),
             result.entropy.data_ptr(), _ptr(result.top_ids), _ptr(result.top_logprobs), rows, vocab, top, temperature, code)
     return result
