@@ -764,3 +764,64 @@ def test_calls_on_another_stream_and_of_no_rows():
     empty = S.shared_prefix_attention(torch.zeros(0, 4, 64, device=DEV), pool, pool, torch.zeros(0, 3, device=DEV, dtype=torch.int32), _i32([]), None)
     assert empty.shape == (0, 4, 64)
     S.rotary_append(torch.zeros(0, 4, 64, device=DEV), torch.zeros(0, 2, 64, device=DEV), None, S.rotary_rule(64, 1e4, device=DEV), _i32([]))
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float32, 48)])
+def test_a_whole_step_captured_and_replayed_beside_the_same_steps_called(dtype, dim):
+    """Pages, slots, append, attention, scores and the way back as one graph on a stream of its own; the same bits as calls of the same state."""
+    from cacheir_b200 import serving_ops as S
+
+    batch, heads, kv_heads, page, vocab, shared = 6, 8, 2, 16, 1003, 3
+    rule = S.rotary_rule(dim, 10000.0, layout="interleaved", scaling=(8.0, 1.0, 4.0, 8192.0), device=DEV)
+    qkv = torch.zeros(24, (heads + 2 * kv_heads) * dim, device=DEV, dtype=dtype)
+    q, k, v = (t.unflatten(1, (-1, dim)) for t in qkv.split((heads * dim, kv_heads * dim, kv_heads * dim), dim=1))
+    logits, sampled = torch.zeros(batch, vocab, device=DEV, dtype=dtype), torch.zeros(batch, device=DEV, dtype=torch.int64)
+    new, keep = (torch.zeros(batch, device=DEV, dtype=torch.int32) for _ in range(2))
+    held = _i32([shared] * 4 + [0, 0])
+    groups = S.PrefixGroups(_i32([0, 4]), _i32([[60, 61, 62]]), _i32([shared * page]))
+
+    def state():
+        pools = [_randn(i, 64, kv_heads, page, dim, dtype=dtype) for i in (1, 2)]
+        table = torch.zeros(batch, 12, device=DEV, dtype=torch.int32)
+        table[:4, :shared] = groups.table
+        return dict(pools=pools, table=table, lens=_i32([shared * page] * 4 + [0, 0]), free=_i32(list(range(60))), count=_i32([60]),
+                    tokens=S.token_map(24, batch, DEV), turned=torch.zeros(24, heads, dim, device=DEV, dtype=dtype),
+                    workspace=torch.zeros(S.shared_prefix_workspace_bytes(batch, heads, dim), device=DEV, dtype=torch.uint8))
+
+    def step(s):
+        S.extend_page_tables(s["table"], s["lens"], new, s["free"], s["count"], s["tokens"], page_size=page)
+        S.rotary_append(q, k, v, rule, s["tokens"].positions, slots=s["tokens"].slots, k_cache=s["pools"][0], v_cache=s["pools"][1], q_out=s["turned"])
+        out = S.shared_prefix_attention(s["turned"][:batch], *s["pools"], s["table"], s["lens"], groups, workspace=s["workspace"])
+        scores = S.token_logprobs(logits, sampled, top=4)
+        S.shrink_page_tables(s["table"], s["lens"], keep, s["free"], s["count"], s["tokens"].status, page_size=page, held_pages=held)
+        return out, scores
+
+    called, captured = state(), state()
+    step(state())                                    # (everything has been launched once before it is captured)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+        out, scores = step(captured)
+    torch.cuda.synchronize()
+    rng = random.Random(4)
+    for i in range(12):
+        lens = called["lens"].tolist()
+        add = [rng.randrange(0, 5) for _ in range(batch)]
+        qkv.copy_(_randn(100 + i, *qkv.shape, dtype=dtype))
+        logits.copy_(_randn(200 + i, batch, vocab, dtype=dtype))
+        sampled.copy_(torch.tensor([rng.randrange(-1, vocab + 1) for _ in range(batch)]))
+        new.copy_(_i32(add))
+        keep.copy_(_i32([n + a - rng.randrange(0, 3) if n + a > 50 else n + a for n, a in zip(lens, add)]))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        want, want_scores = step(called)             # (beside it)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        for a, b in ((scores.logprobs, want_scores.logprobs), (scores.entropy, want_scores.entropy), (scores.top_logprobs, want_scores.top_logprobs)):
+            assert bool(((a == b) | (a.isnan() & b.isnan())).all())
+        assert torch.equal(scores.top_ids, want_scores.top_ids)
+        for name in ("table", "lens", "free", "count"):
+            assert torch.equal(captured[name], called[name]), name
+        assert all(torch.equal(a, b) for a, b in zip(captured["pools"], called["pools"]))
+        assert int(called["tokens"].status) == 0 and int(captured["tokens"].status) == 0
