@@ -197,6 +197,21 @@ class RouteRule(ctypes.Structure):
     _fields_ = [("softmax", c_int), ("identity", c_int), ("groups", c_int), ("keep", c_int), ("correction", c_void_p), ("scale", c_float)]
 
 
+class TablesArgs(ctypes.Structure):
+    """cacheir_b200_tables_args"""
+
+    _fields_ = [(name, c_void_p) for name in ("page_table", "seq_lens", "change", "held_pages", "free_pages", "free_count", "positions", "row_seq", "slots",
+                                              "cu_rows", "status")] + \
+               [(name, c_int) for name in ("sequences", "max_pages", "page_size", "capacity", "rows")]
+
+
+class LogprobsArgs(ctypes.Structure):
+    """cacheir_b200_logprobs_args"""
+
+    _fields_ = [(name, c_void_p) for name in ("logits", "tokens", "logprobs", "entropy", "top_ids", "top_logprobs")] + \
+               [("row_stride", c_longlong), ("temperature", c_double)] + [(name, c_int) for name in ("rows", "vocab", "top", "dtype")]
+
+
 class RotaryArgs(ctypes.Structure):
     """cacheir_b200_rotary_args"""
 
@@ -308,13 +323,13 @@ GROUP_SIGNATURES: dict[str, dict[str, tuple[object, list[object]]]] = {
         "cacheir_b200_experts_device_status": (c_int, [c_int]),
     },
     "serving": {
-        "cacheir_b200_extend_page_tables": (c_int, [c_void_p] * 5 + [c_int] * 5 + [c_void_p] * 6),
-        "cacheir_b200_shrink_page_tables": (c_int, [c_void_p] * 6 + [c_int] * 4 + [c_void_p] * 2),
+        "cacheir_b200_extend_page_tables": (c_int, [c_void_p, c_void_p]),
+        "cacheir_b200_shrink_page_tables": (c_int, [c_void_p, c_void_p]),
         "cacheir_b200_rotary_append": (c_int, [c_void_p, c_void_p]),
         "cacheir_b200_shared_prefix_workspace_bytes": (c_size_t, [c_int] * 3),
         "cacheir_b200_shared_prefix_launches": (c_int, [c_int] * 7),
         "cacheir_b200_shared_prefix_attention": (c_int, [c_void_p, c_void_p]),
-        "cacheir_b200_token_logprobs": (c_int, [c_void_p, c_longlong] + [c_void_p] * 5 + [c_int] * 3 + [c_double, c_int, c_void_p]),
+        "cacheir_b200_token_logprobs": (c_int, [c_void_p, c_void_p]),
         "cacheir_b200_serving_device_status": (c_int, [c_int]),
     },
 }

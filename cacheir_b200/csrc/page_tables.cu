@@ -23,19 +23,7 @@ constexpr int kClusterBlocks = 8;
 constexpr int kOwnRows = 2048;              // rows that the first kernel takes itself
 constexpr int kRowsPerWarp = 128;
 
-struct TableArgs {
-  int32_t* page_table;
-  int32_t* seq_lens;
-  const int32_t* change;      // extend: new tokens; shrink: tokens kept
-  const int32_t* held_pages;  // shrink
-  int32_t* free_pages;
-  int32_t* free_count;
-  int32_t* positions;
-  int32_t* row_seq;
-  int32_t* slots;
-  int32_t* cu_rows;
-  int32_t* status;
-  int sequences, max_pages, page_size, capacity, rows;
+struct TableArgs : cacheir_b200_tables_args {
   int fills;                  // extend: the rows are filled in here
 };
 
@@ -274,28 +262,23 @@ int launch_tables(const TableArgs& a, cudaStream_t stream) {
 
 using namespace cb200;
 
-extern "C" int cacheir_b200_extend_page_tables(int32_t* page_table, int32_t* seq_lens, const int32_t* new_lens, const int32_t* free_pages,
-                                               int32_t* free_count, int sequences, int max_pages, int page_size, int capacity, int rows,
-                                               int32_t* positions, int32_t* row_seq, int32_t* slots, int32_t* cu_rows, int32_t* status,
-                                               void* stream) {
-  if (sequences <= 0 || rows <= 0) return 0;
-  if (!page_table || !seq_lens || !new_lens || !free_pages || !free_count || !positions || !row_seq || !slots || !cu_rows || !status ||
-      max_pages <= 0 || page_size <= 0 || capacity <= 0)
+extern "C" int cacheir_b200_extend_page_tables(const cacheir_b200_tables_args* args, void* stream) {
+  if (!args) return CACHEIR_B200_EINVAL;
+  const cacheir_b200_tables_args& a = *args;
+  if (a.sequences <= 0 || a.rows <= 0) return 0;
+  if (!a.page_table || !a.seq_lens || !a.change || !a.free_pages || !a.free_count || !a.positions || !a.row_seq || !a.slots || !a.cu_rows || !a.status ||
+      a.max_pages <= 0 || a.page_size <= 0 || a.capacity <= 0)
     return CACHEIR_B200_EINVAL;
-  if (sequences > CACHEIR_B200_MAX_SEQUENCES || static_cast<long long>(max_pages) * page_size > 0x7fffffffLL) return CACHEIR_B200_ELIMIT;
-  TableArgs a{page_table, seq_lens, new_lens, nullptr, const_cast<int32_t*>(free_pages), free_count, positions, row_seq, slots, cu_rows, status,
-              sequences, max_pages, page_size, capacity, rows, rows <= kOwnRows ? 1 : 0};
-  return launch_tables<true>(a, as_stream(stream));
+  if (a.sequences > CACHEIR_B200_MAX_SEQUENCES || static_cast<long long>(a.max_pages) * a.page_size > 0x7fffffffLL) return CACHEIR_B200_ELIMIT;
+  return launch_tables<true>(TableArgs{a, a.rows <= kOwnRows ? 1 : 0}, as_stream(stream));
 }
 
-extern "C" int cacheir_b200_shrink_page_tables(const int32_t* page_table, int32_t* seq_lens, const int32_t* keep_lens, const int32_t* held_pages,
-                                               int32_t* free_pages, int32_t* free_count, int sequences, int max_pages, int page_size,
-                                               int capacity, int32_t* status, void* stream) {
-  if (sequences <= 0) return 0;
-  if (!page_table || !seq_lens || !keep_lens || !free_pages || !free_count || !status || max_pages <= 0 || page_size <= 0 || capacity <= 0)
+extern "C" int cacheir_b200_shrink_page_tables(const cacheir_b200_tables_args* args, void* stream) {
+  if (!args) return CACHEIR_B200_EINVAL;
+  const cacheir_b200_tables_args& a = *args;
+  if (a.sequences <= 0) return 0;
+  if (!a.page_table || !a.seq_lens || !a.change || !a.free_pages || !a.free_count || !a.status || a.max_pages <= 0 || a.page_size <= 0 || a.capacity <= 0)
     return CACHEIR_B200_EINVAL;
-  if (sequences > CACHEIR_B200_MAX_SEQUENCES || static_cast<long long>(max_pages) * page_size > 0x7fffffffLL) return CACHEIR_B200_ELIMIT;
-  TableArgs a{const_cast<int32_t*>(page_table), seq_lens, keep_lens, held_pages, free_pages, free_count, nullptr, nullptr, nullptr, nullptr, status,
-              sequences, max_pages, page_size, capacity, 0, 0};
-  return launch_tables<false>(a, as_stream(stream));
+  if (a.sequences > CACHEIR_B200_MAX_SEQUENCES || static_cast<long long>(a.max_pages) * a.page_size > 0x7fffffffLL) return CACHEIR_B200_ELIMIT;
+  return launch_tables<false>(TableArgs{a, 0}, as_stream(stream));
 }

@@ -581,18 +581,18 @@ int logprobs_device_status(bool reset) { return device_status_word(g_logprobs_st
 
 using namespace cb200;
 
-extern "C" int cacheir_b200_token_logprobs(const void* logits, long long row_stride, const int64_t* tokens, float* logprobs, float* entropy,
-                                           int64_t* top_ids, float* top_logprobs, int rows, int vocab, int top, double temperature, int dtype,
-                                           void* stream) {
-  if (rows <= 0 || vocab <= 0) return 0;
-  if (!logits || (logprobs && !tokens) || top < 0 || (top > 0 && (!top_ids || !top_logprobs)) || !(temperature >= 1e-6) || temperature > 1e6 ||
-      dtype_size(dtype) == 0 || (row_stride != 0 && row_stride < vocab && rows > 1))
+extern "C" int cacheir_b200_token_logprobs(const cacheir_b200_logprobs_args* args, void* stream) {
+  if (!args) return CACHEIR_B200_EINVAL;
+  const cacheir_b200_logprobs_args& g = *args;
+  if (g.rows <= 0 || g.vocab <= 0) return 0;
+  if (!g.logits || (g.logprobs && !g.tokens) || g.top < 0 || (g.top > 0 && (!g.top_ids || !g.top_logprobs)) || !(g.temperature >= 1e-6) ||
+      g.temperature > 1e6 || dtype_size(g.dtype) == 0 || (g.row_stride != 0 && g.row_stride < g.vocab && g.rows > 1))
     return CACHEIR_B200_EINVAL;
-  if (top > CACHEIR_B200_MAX_TOP || top > vocab || rows > 0x7fffffff / kMaxCluster) return CACHEIR_B200_ELIMIT;
-  if (!aligned_to(logits, dtype_size(dtype))) return CACHEIR_B200_EALIGN;
-  if (row_stride == 0) row_stride = vocab;
-  const Args a{logits, row_stride, tokens, logprobs, entropy, top_ids, top_logprobs, vocab, top, 1, 1.0 / temperature};
-  if (dtype == CACHEIR_B200_F32) return launch_logprobs<float>(a, rows, as_stream(stream));
-  if (dtype == CACHEIR_B200_F16) return launch_logprobs<__half>(a, rows, as_stream(stream));
-  return launch_logprobs<__nv_bfloat16>(a, rows, as_stream(stream));
+  if (g.top > CACHEIR_B200_MAX_TOP || g.top > g.vocab || g.rows > 0x7fffffff / kMaxCluster) return CACHEIR_B200_ELIMIT;
+  if (!aligned_to(g.logits, dtype_size(g.dtype))) return CACHEIR_B200_EALIGN;
+  const Args a{g.logits, g.row_stride == 0 ? g.vocab : g.row_stride, g.tokens, g.logprobs, g.entropy, g.top_ids, g.top_logprobs, g.vocab, g.top, 1,
+               1.0 / g.temperature};
+  if (g.dtype == CACHEIR_B200_F32) return launch_logprobs<float>(a, g.rows, as_stream(stream));
+  if (g.dtype == CACHEIR_B200_F16) return launch_logprobs<__half>(a, g.rows, as_stream(stream));
+  return launch_logprobs<__nv_bfloat16>(a, g.rows, as_stream(stream));
 }

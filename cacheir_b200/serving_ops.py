@@ -18,18 +18,23 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import PrefixArgs, RotaryArgs, check
+from ._lib import LogprobsArgs, PrefixArgs, RotaryArgs, TablesArgs, check
 from .ops import _require_cuda, dtype_code
 
 MAX_TOP = 32
 MAX_SEQUENCES = 16384
 LAYOUTS = {"interleaved": 0, "half": 1}
-# the argument structs as bytes (a third of the time that their ctypes classes take to fill)
+# the argument structs as bytes (a third of the time that their ctypes classes take to fill, half of that of as many arguments)
+TABLES_BYTES = struct.Struct("@11Q5i4x")
 ROTARY_BYTES = struct.Struct("@10Q5q9if")
-PREFIX_BYTES = struct.Struct("@11Q2q10if")
-assert ROTARY_BYTES.size == ctypes.sizeof(RotaryArgs) and PREFIX_BYTES.size <= ctypes.sizeof(PrefixArgs)
+PREFIX_BYTES = struct.Struct("@11Q2q10if4x")
+LOGPROBS_BYTES = struct.Struct("@6Qqd4i")
+assert [s.size for s in (TABLES_BYTES, ROTARY_BYTES, PREFIX_BYTES, LOGPROBS_BYTES)] == [
+    ctypes.sizeof(c) for c in (TablesArgs, RotaryArgs, PrefixArgs, LogprobsArgs)]
 
+_I32 = torch.int32
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _calls: dict[str, object] = {}         # entry points that have been called
 
 
@@ -39,8 +44,8 @@ def _ptr(t: torch.Tensor | None) -> int:
 
 # (As these launch kernels of a few microseconds, what they do on the host is kept to about as many: shapes and strides are taken once, the
 # current device is looked up and only switched where the tensors are on another one.)
-def _launch(what: str, tensors: tuple, *args) -> None:
-    """Calls the entry point `what` with `args` and the current stream of the device that all the tensors are on."""
+def _launch(what: str, tensors: tuple, args: bytes) -> None:
+    """Calls the entry point `what` with its struct and the current stream of the device that all the tensors are on."""
     index = tensors[0].get_device()
     for t in tensors:
         if t is not None and t.get_device() != index:
@@ -51,18 +56,18 @@ def _launch(what: str, tensors: tuple, *args) -> None:
     call = _calls.get(what)
     if call is None:
         call = _calls[what] = getattr(_lib.load_group("serving"), "cacheir_b200_" + what)
-    if index == torch.cuda.current_device():
-        code = call(*args, _raw_stream(index))
+    if index == _current_device():
+        code = call(args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            code = call(*args, _raw_stream(index))
+            code = call(args, _raw_stream(index))
     if code:
         check(code, what)
 
 
 def _check_ints(what: str, *tensors: torch.Tensor | None) -> None:
     for t in tensors:
-        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous()):
+        if t is not None and (t.dtype is not _I32 or not t.is_contiguous()):
             raise TypeError(f"{what} must be contiguous int32 tensors")
 
 
@@ -135,9 +140,10 @@ def extend_page_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, new_len
     rows = positions.numel()
     if row_seq.numel() != rows or slots.numel() != rows or cu_rows.numel() != sequences + 1:
         raise ValueError("the token map was made for other sizes")
-    _launch("extend_page_tables", (page_table, seq_lens, new_lens, free_pages, free_count, positions, row_seq, slots, cu_rows, status),
-            page_table.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), sequences, max_pages,
-            page_size, free_pages.numel(), rows, positions.data_ptr(), row_seq.data_ptr(), slots.data_ptr(), cu_rows.data_ptr(), status.data_ptr())
+    args = TABLES_BYTES.pack(page_table.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(), 0, free_pages.data_ptr(), free_count.data_ptr(),
+                             positions.data_ptr(), row_seq.data_ptr(), slots.data_ptr(), cu_rows.data_ptr(), status.data_ptr(), sequences, max_pages,
+                             page_size, free_pages.numel(), rows)
+    _launch("extend_page_tables", (page_table, seq_lens, new_lens, free_pages, free_count, positions, row_seq, slots, cu_rows, status), args)
     return tokens
 
 
@@ -151,9 +157,9 @@ def shrink_page_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, keep_le
         _check_ints("held_pages", held_pages)
         if held_pages.numel() != sequences:
             raise ValueError("held_pages must be [sequences]")
-    _launch("shrink_page_tables", (page_table, seq_lens, keep_lens, free_pages, free_count, status, held_pages),
-            page_table.data_ptr(), seq_lens.data_ptr(), keep_lens.data_ptr(), _ptr(held_pages), free_pages.data_ptr(), free_count.data_ptr(),
-            sequences, max_pages, page_size, free_pages.numel(), status.data_ptr())
+    args = TABLES_BYTES.pack(page_table.data_ptr(), seq_lens.data_ptr(), keep_lens.data_ptr(), _ptr(held_pages), free_pages.data_ptr(),
+                             free_count.data_ptr(), 0, 0, 0, 0, status.data_ptr(), sequences, max_pages, page_size, free_pages.numel(), 0)
+    _launch("shrink_page_tables", (page_table, seq_lens, keep_lens, free_pages, free_count, status, held_pages), args)
 
 
 # ---- rotary positions ------------------------------------------------------------------------------------------------
@@ -404,6 +410,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, *, top: in
     entropy = torch.empty(rows, dtype=torch.float32, device=device)
     result = TokenLogprobs(None if tokens is None else torch.empty_like(entropy), entropy,
                            entropy.new_empty((rows, top), dtype=torch.int64) if top else None, entropy.new_empty((rows, top)) if top else None)
-    _launch("token_logprobs", (logits, tokens), logits.data_ptr(), row_stride if rows > 1 else vocab, _ptr(tokens), _ptr(result.logprobs),
-            result.entropy.data_ptr(), _ptr(result.top_ids), _ptr(result.top_logprobs), rows, vocab, top, temperature, code)
+    args = LOGPROBS_BYTES.pack(logits.data_ptr(), _ptr(tokens), _ptr(result.logprobs), entropy.data_ptr(), _ptr(result.top_ids),
+                               _ptr(result.top_logprobs), row_stride if rows > 1 else vocab, temperature, rows, vocab, top, code)
+    _launch("token_logprobs", (logits, tokens), args)
     return result

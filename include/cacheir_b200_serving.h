@@ -36,13 +36,23 @@ extern "C" {
  *   -2   a sequence is longer than its table  -3  the stack's height is below 0 or (would be) above its capacity
  * At most CACHEIR_B200_MAX_SEQUENCES sequences, tables of fewer than 2^31 tokens (CACHEIR_B200_ELIMIT). */
 #define CACHEIR_B200_MAX_SEQUENCES 16384
-int cacheir_b200_extend_page_tables(int32_t* page_table, int32_t* seq_lens, const int32_t* new_lens, const int32_t* free_pages,
-                                    int32_t* free_count, int sequences, int max_pages, int page_size, int capacity, int rows,
-                                    int32_t* positions, int32_t* row_seq, int32_t* slots, int32_t* cu_rows, int32_t* status,
-                                    void* stream);
-int cacheir_b200_shrink_page_tables(const int32_t* page_table, int32_t* seq_lens, const int32_t* keep_lens, const int32_t* held_pages,
-                                    int32_t* free_pages, int32_t* free_count, int sequences, int max_pages, int page_size,
-                                    int capacity, int32_t* status, void* stream);
+typedef struct {
+  int32_t* page_table;
+  int32_t* seq_lens;
+  const int32_t* change;      /* extend: new_lens; shrink: keep_lens */
+  const int32_t* held_pages;  /* shrink */
+  int32_t* free_pages;        /* extend reads them only */
+  int32_t* free_count;
+  int32_t* positions;         /* this one and the next three: extend */
+  int32_t* row_seq;
+  int32_t* slots;
+  int32_t* cu_rows;
+  int32_t* status;
+  int sequences, max_pages, page_size, capacity;
+  int rows;                   /* extend */
+} cacheir_b200_tables_args;
+int cacheir_b200_extend_page_tables(const cacheir_b200_tables_args* args, void* stream);
+int cacheir_b200_shrink_page_tables(const cacheir_b200_tables_args* args, void* stream);
 
 /* ------------------------------------------------------------------------
  * Rotary positions of q and k rows and, with slots, the append of k and v to the page pool.
@@ -126,9 +136,18 @@ int cacheir_b200_shared_prefix_attention(const cacheir_b200_prefix_args* args, v
  * logprobs (with tokens), entropy and the top pair may be NULL. 1e-6 <= temperature <= 1e6. top <= CACHEIR_B200_MAX_TOP and <= vocab, and
  * with it rows of up to 4 MB (CACHEIR_B200_ELIMIT). */
 #define CACHEIR_B200_MAX_TOP 32
-int cacheir_b200_token_logprobs(const void* logits, long long row_stride, const int64_t* tokens, float* logprobs, float* entropy,
-                                int64_t* top_ids, float* top_logprobs, int rows, int vocab, int top, double temperature, int dtype,
-                                void* stream);
+typedef struct {
+  const void* logits;
+  const int64_t* tokens;
+  float* logprobs;
+  float* entropy;
+  int64_t* top_ids;
+  float* top_logprobs;
+  long long row_stride;       /* 0: vocab */
+  double temperature;
+  int rows, vocab, top, dtype;
+} cacheir_b200_logprobs_args;
+int cacheir_b200_token_logprobs(const cacheir_b200_logprobs_args* args, void* stream);
 
 /* First bounded wait of a kernel of this library that gave up on the current device (0: none); synchronises. */
 int cacheir_b200_serving_device_status(int reset);

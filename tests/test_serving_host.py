@@ -33,7 +33,8 @@ def test_argument_structs_have_the_compiler_s_layout(tmp_path):
     from cacheir_b200 import _lib
 
     lines, want = [], []
-    for name, struct in (("cacheir_b200_rotary_args", _lib.RotaryArgs), ("cacheir_b200_prefix_args", _lib.PrefixArgs)):
+    for name, struct in (("cacheir_b200_tables_args", _lib.TablesArgs), ("cacheir_b200_rotary_args", _lib.RotaryArgs),
+                         ("cacheir_b200_prefix_args", _lib.PrefixArgs), ("cacheir_b200_logprobs_args", _lib.LogprobsArgs)):
         want.append(ctypes.sizeof(struct))
         lines.append(f'std::printf("%zu ", sizeof({name}));')
         for field, _ in struct._fields_:
@@ -47,16 +48,19 @@ def test_argument_structs_have_the_compiler_s_layout(tmp_path):
 
 def test_c_entry_points_refuse_before_they_launch(lib):
     """Codes of calls that never reach the device: missing pointers, extents, limits, scratch."""
-    from cacheir_b200._lib import PrefixArgs, RotaryArgs
+    from cacheir_b200._lib import LogprobsArgs, PrefixArgs, RotaryArgs, TablesArgs
 
     some = 4096                                               # an address that no refused call looks at
-    tables = lambda n=4, pages=8, size=16, capacity=9, rows=3, null=None: lib.cacheir_b200_extend_page_tables(
-        *(None if i == null else some for i in range(5)), n, pages, size, capacity, rows, *(None if i + 5 == null else some for i in range(5)), None)
+    names = ("page_table", "seq_lens", "change", "free_pages", "free_count", "positions", "row_seq", "slots", "cu_rows", "status")
+    tables = lambda n=4, pages=8, size=16, capacity=9, rows=3, null=None: lib.cacheir_b200_extend_page_tables(ctypes.byref(TablesArgs(
+        **{name: None if i == null else some for i, name in enumerate(names)}, sequences=n, max_pages=pages, page_size=size, capacity=capacity, rows=rows)), None)
     assert [tables(n=0), tables(rows=0)] == [0, 0]
     assert [tables(null=i) for i in range(10)] == [-1] * 10
     assert [tables(pages=0), tables(size=0), tables(capacity=0)] == [-1] * 3
     assert [tables(n=16385), tables(pages=1 << 28)] == [-5, -5]
-    shrink = lambda n=4, pages=8, size=16, capacity=9: lib.cacheir_b200_shrink_page_tables(some, some, some, None, some, some, n, pages, size, capacity, some, None)
+    shrink = lambda n=4, pages=8, size=16, capacity=9: lib.cacheir_b200_shrink_page_tables(ctypes.byref(TablesArgs(
+        page_table=some, seq_lens=some, change=some, free_pages=some, free_count=some, status=some, sequences=n, max_pages=pages, page_size=size,
+        capacity=capacity)), None)
     assert [shrink(n=0), shrink(pages=0), shrink(n=16385), shrink(capacity=0)] == [0, -1, -5, -1]
 
     good = dict(q=some, k=some, v=some, q_out=some, k_cache=some, v_cache=some, positions=some, slots=some, turns=some, rows=2, heads=4, kv_heads=2, dim=64,
@@ -80,7 +84,9 @@ def test_c_entry_points_refuse_before_they_launch(lib):
     assert [prefix(workspace=None), prefix(workspace_bytes=need - 1), prefix(workspace=some + 4), prefix(dim=513), prefix(batch=65536)] == [-3, -3, -2, -4, -5]
 
     logprobs = lambda logits=some, stride=0, tokens=some, out=some, ids=some, rows=2, vocab=9, top=3, t=1.0, dtype=0: lib.cacheir_b200_token_logprobs(
-        logits, stride, tokens, out, out, ids, ids, rows, vocab, top, t, dtype, None)
+        ctypes.byref(LogprobsArgs(logits=logits, tokens=tokens, logprobs=out, entropy=out, top_ids=ids, top_logprobs=ids, row_stride=stride, temperature=t,
+                                  rows=rows, vocab=vocab, top=top, dtype=dtype)), None)
+    assert [call(None, None) for call in (lib.cacheir_b200_extend_page_tables, lib.cacheir_b200_shrink_page_tables, lib.cacheir_b200_token_logprobs)] == [-1] * 3
     assert [logprobs(rows=0), logprobs(vocab=0)] == [0, 0]
     bad = [dict(logits=None), dict(tokens=None), dict(ids=None), dict(top=-1), dict(t=0.0), dict(t=float("nan")), dict(t=-1.0), dict(dtype=9), dict(stride=8)]
     assert [logprobs(**b) for b in bad] == [-1] * len(bad)
