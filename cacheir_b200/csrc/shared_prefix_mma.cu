@@ -15,9 +15,9 @@
 // outputs, which stay in tensor memory, are hardly ever rescaled; probabilities are rounded to the element type as the second MMA's operand,
 // their sums are not.
 //
-// Measured (32 query and 8 key/value heads of 128, fp16, whole call): 64 rows behind 32768 common tokens 54 us, of which 25.6 us are the
-// bytes and 20.8 us the products; 32 rows behind 2048 tokens 21.5 us (bytes 7.1 us). 128 rows in 16 groups of ragged prefixes with 64 and 8
-// heads, bf16: 68.9 us (bytes 46.5 us). A call spends about 5.5 us before the first scores (launch, plan, page ids, copies), and about 3 us on
+// Measured (32 query and 8 key/value heads of 128, fp16, whole call): 64 rows behind 32768 common tokens 51 us, of which 25.6 us are the
+// bytes and 20.8 us the products; 32 rows behind 2048 tokens 20.0 us (bytes 7.1 us). 128 rows in 16 groups of ragged prefixes with 64 and 8
+// heads, bf16: 66.6 us (bytes 46.5 us). A call spends about 5.5 us before the first scores (launch, plan, page ids, copies), and about 3 us on
 // joining. In between a tile of 256 query rows takes 3300 cycles, of which the tensor cores work 2048: the rest is the way from scores by
 // the softmax to the second product (2300 cycles a step, 1500 of them exponentials), which the other group of warps hides in part. Neither
 // a share of the exponentials by polynomials nor reading scores once into 128 registers changed that (56.0 us became 55.7 and 56.3).
@@ -206,13 +206,13 @@ __device__ __forceinline__ Weights group_weights(const PlanGroup& g, int units, 
 }
 // Blocks that take part. No item may be in more pieces than there is scratch for: n tiles touch ceil((n - 1) / share) + 1 blocks at most. And
 // the common parts get as many SMs as is their share of the work, so that the other kernel can have the rest of them meanwhile: 16 own
-// tokens of a key/value head (8 KB) take an SM about a sixteenth of a unit's time (64 KB), and a row's own part costs as much as eight of
+// tokens of a key/value head (8 KB) take an SM about a twentieth of a unit's time (64 KB), and a row's own part costs as much as eleven of
 // those before it has any. `lens`: tokens of all rows. (64 rows with 144 own tokens on average behind 32768, 128 rows with 350 behind up to 4095:
-// 53.5 and 69.6 us; with a twelfth and one 56.0 and 69.4, with an eighth and one 52.0 and 78.5.)
+// 51.2 and 66.6 us; an eighteenth 51.3 and 68.5, a twenty-second 52.8 and 66.5, fourteen and a twentieth 51.4 and 68.2.)
 __device__ __forceinline__ int plan_ctas(const cacheir_b200_prefix_args& a, int pieces, int own_heads, int units, const Weights& w, long long lens, int grid) {
   if (units <= 0) return 0;
   const int least = max(1, (w.longest - 1 + pieces - 2) / (pieces - 1));
-  const float cost = static_cast<float>(w.cost), own = __fmul_rn(static_cast<float>(max(lens - w.common, 0LL) / kChunk + 8LL * a.batch), own_heads / 16.f);
+  const float cost = static_cast<float>(w.cost), own = __fmul_rn(static_cast<float>(max(lens - w.common, 0LL) / kChunk + 11LL * a.batch), own_heads / 20.f);
   const float sms = __fdiv_rn(__fmul_rn(kNumSMs, cost), __fadd_rn(cost, own));       // (two kernels work this out and have to agree)
   return max(1, min(min(grid, units / least), static_cast<int>(sms) + 1));
 }
@@ -765,7 +765,10 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
 // Every row's own keys. One block per (part of the row's own keys, key/value head and up to 16 of its query heads, row). Keys and values come
 // 16 tokens at a time (TMA): every warp takes every WARPS-th chunk of the part through a ring of its own, with warp MMAs that have the query
 // heads as their 16 rows. Bound by the memory's rate where there are many rows: then blocks of two warps, six of them on an SM, so that
-// while some begin or end others keep the memory busy; where there are few, blocks of four or eight. None of that needs the common part's
+// while some begin or end others keep the memory busy; where there are few, blocks of four or eight, and the longest row counts: a chunk takes
+// a warp about 1 us, half its copy's latency and half its own chain of instructions (masks and cleared values only in chunks that are not
+// whole, two chains of products a score, and the scale inside the exponent's argument made 20.0 us of 21.7 for 32 rows of up to 512 own
+// tokens; a reference that moves as seldom as that of the common keys made nothing of it). None of that needs the common part's
 // kernel: this one starts as soon as that one's blocks have their places, on the SMs that they leave.
 struct OwnParams {
   cacheir_b200_prefix_args a;
@@ -923,6 +926,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
     float sc[2][4];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
+      float odd[4] = {0.f, 0.f, 0.f, 0.f};                       // (two chains of products a score: this warp waits for its own results only)
       sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
       const uint32_t token = n * 8 + lrow;
 #pragma unroll
@@ -931,27 +935,31 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         uint32_t kb[4];
         ldsm_x4(kbase + (c >> 3) * (kChunk * 128) + token * 128 + (((c & 7) ^ (token & 7)) << 4), kb);
         mma_pair<T>(sc[n], qa[2 * k], kb[0], kb[1]);
-        mma_pair<T>(sc[n], qa[2 * k + 1], kb[2], kb[3]);
+        mma_pair<T>(odd, qa[2 * k + 1], kb[2], kb[3]);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[n][e] += odd[e];
     }
     const int key0 = (begin + warp + it * WARPS) * kChunk;
     const bool whole = key0 >= from && key0 + kChunk <= len;
-    float top[2] = {-INFINITY, -INFINITY};
+    if (!whole) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = key0 + n * 8 + 2 * t4 + (e & 1);
-        const float v = whole || (key >= from && key < len) ? sc[n][e] * p.scale_log2 : -INFINITY;
-        sc[n][e] = v;
-        top[e >> 1] = fmaxf(top[e >> 1], v);
-      }
+        for (int e = 0; e < 4; ++e) {
+          const int key = key0 + n * 8 + 2 * t4 + (e & 1);
+          if (key < from || key >= len) sc[n][e] = -INFINITY;
+        }
+    }
+    float top[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) top[r] = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
     float corr[2], less[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      const float m_new = fmaxf(m_run[r], top[r]);               // (-inf where all scores so far are)
+      const float m_new = fmaxf(m_run[r], top[r] * p.scale_log2);                  // (-inf where all scores so far are)
       less[r] = m_new > -INFINITY ? m_new : 0.f;
       corr[r] = ex2(m_run[r] - less[r]);
       m_run[r] = m_new;
@@ -960,7 +968,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pr[n][e] = ex2(sc[n][e] - less[e >> 1]);
+      for (int e = 0; e < 4; ++e) pr[n][e] = ex2(fmaf(sc[n][e], p.scale_log2, -less[e >> 1]));
 #pragma unroll
     for (int r = 0; r < 2; ++r) l_run[r] = l_run[r] * corr[r] + (pr[0][2 * r] + pr[0][2 * r + 1] + pr[1][2 * r] + pr[1][2 * r + 1]);
     const uint32_t pa[4] = {pack_pair<T>(pr[0][0], pr[0][1]), pack_pair<T>(pr[0][2], pr[0][3]), pack_pair<T>(pr[1][0], pr[1][1]),
@@ -969,23 +977,29 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) { o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[1]; o[i][3] *= corr[1]; }
     }
-    // values of keys that do not count may hold anything: cleared, so that 0 * value stays 0
-    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-    if (!whole) {
+    auto add_values = [&](auto clear, const uint32_t keep0, const uint32_t keep1) {
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        const uint32_t token = (lmat & 1) * 8 + lrow, c = 2 * j + (lmat >> 1);
+        uint32_t vb[4];
+        ldsm_trans(vbase + (c >> 3) * (kChunk * 128) + token * 128 + (((c & 7) ^ (token & 7)) << 4), vb);
+        if constexpr (decltype(clear)::value) {
+          vb[0] &= keep0; vb[1] &= keep1; vb[2] &= keep0; vb[3] &= keep1;
+        }
+        mma_pair<T>(o[2 * j], pa, vb[0], vb[1]);
+        mma_pair<T>(o[2 * j + 1], pa, vb[2], vb[3]);
+      }
+    };
+    if (whole) {
+      add_values(std::false_type{}, 0u, 0u);
+    } else {                                                     // values of keys that do not count may hold anything: cleared, so that 0 * value stays 0
+      uint32_t keep[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int key = key0 + i * 8 + 2 * t4;
         keep[i] = (key >= from && key < len ? 0x0000ffffu : 0u) | (key + 1 >= from && key + 1 < len ? 0xffff0000u : 0u);
       }
-    }
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      const uint32_t token = (lmat & 1) * 8 + lrow, c = 2 * j + (lmat >> 1);
-      uint32_t vb[4];
-      ldsm_trans(vbase + (c >> 3) * (kChunk * 128) + token * 128 + (((c & 7) ^ (token & 7)) << 4), vb);
-      vb[0] &= keep[0]; vb[1] &= keep[1]; vb[2] &= keep[0]; vb[3] &= keep[1];
-      mma_pair<T>(o[2 * j], pa, vb[0], vb[1]);
-      mma_pair<T>(o[2 * j + 1], pa, vb[2], vb[3]);
+      add_values(std::true_type{}, keep[0], keep[1]);
     }
     __syncwarp();                                                // the stage has been read
     const int ahead = it + kStages;
