@@ -647,8 +647,8 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
           l_run *= alpha;
           if (t > 0) {                                         // bring the output to the new reference
             // (with two groups of warps this buffer's last output came before these scores)
-            if (!two) ok = mbar_wait(smem_u32(&bar_o[(s - 1) & 1]), ((s - 1) >> 1) & 1, &g_prefix_status, (15 << 8) | 9);
-            __syncwarp();
+            if (!two) ok = warp_wait(smem_u32(&bar_o[(s - 1) & 1]), ((s - 1) >> 1) & 1, (15 << 8) | 9);
+            if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
@@ -722,8 +722,8 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       step += steps;
       tile += walk.tiles;
       if (!ok) break;
-      ok = mbar_wait(smem_u32(&bar_o[last & 1]), (last >> 1) & 1, &g_prefix_status, (15 << 8) | 11);
-      __syncwarp();
+      ok = warp_wait(smem_u32(&bar_o[last & 1]), (last >> 1) & 1, (15 << 8) | 11);
+      if (!ok) break;
       tc_fence_after();
       const int at = real ? b_row * a.heads + head : -1;
       const size_t piece0 = static_cast<size_t>(walk.piece) * a.batch * a.heads;

@@ -254,3 +254,13 @@ def test_launches_by_extents(lib):
     assert [launches(0), launches(1), launches(64), launches(65)] == [2, 3, 3, 4]
     assert [launches(1, torch.float32), launches(1, dim=80), launches(1, page=24), launches(1, heads=130, kv=2)] == [2] * 4
     assert launches(1, torch.bfloat16, dim=64, page=48) == 3
+
+
+def test_what_a_wait_says_is_the_same_in_all_lanes_of_a_warp():
+    """Loops around waits hold votes and instructions of whole warps: a lane whose wait gave up must not leave alone while the others go on. What a
+    bounded wait says is kept nowhere but where a vote has made it the warp's; elsewhere it is only waited."""
+    for name in ("shared_prefix_mma.cu", "token_logprobs.cu"):
+        lines = (ROOT / "cacheir_b200" / "csrc" / name).read_text().splitlines()
+        kept = [line.strip() for line in lines if re.search(r"\bmbar_(try_)?wait\(", line) and "__all_sync(" not in line
+                and not re.match(r"\s*(for \([^()]*\) )?mbar_wait\(", line)]
+        assert not kept, (name, kept)
