@@ -13,6 +13,8 @@ constexpr int kTileRows = 8;
 constexpr int kTileKeys = 32;
 constexpr int kGeneralThreads = 128;
 constexpr int kGeneralDim = 512;
+// queries, keys (a float further a row, so that lanes reach different banks), values, weights, scales
+constexpr size_t general_smem(int dim) { return (static_cast<size_t>(kTileRows) * dim + kTileKeys * (2 * dim + 1) + kTileRows * (kTileKeys + 2)) * 4; }
 
 template <typename T>
 __global__ void __launch_bounds__(kGeneralThreads)
@@ -180,8 +182,9 @@ int launch_general(const cacheir_b200_prefix_args& a, PrefixParts parts, cudaStr
   const long long want = 4LL * kNumSMs / (tiles * a.kv_heads);
   const int half = static_cast<int>(want < 1 ? 1 : want > parts.pieces / 2 ? parts.pieces / 2 : want);
   parts.pieces = 2 * half;
-  const size_t smem = (static_cast<size_t>(kTileRows) * a.dim + kTileKeys * (2 * a.dim + 1) + kTileRows * (kTileKeys + 2)) * 4;
-  cudaError_t e = cudaFuncSetAttribute(prefix_general_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  const size_t smem = general_smem(a.dim);
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = allow_shared_memory(done, reinterpret_cast<const void*>(prefix_general_kernel<T>), static_cast<int>(general_smem(kGeneralDim)));
   if (e == cudaSuccess)
     e = launch_chained(prefix_general_kernel<T>, dim3(half, a.kv_heads, static_cast<unsigned>(tiles)), dim3(kGeneralThreads), smem, stream, a, parts,
                        static_cast<int>(a.groups > 0 ? common : 0));

@@ -825,3 +825,40 @@ def test_a_whole_step_captured_and_replayed_beside_the_same_steps_called(dtype, 
             assert torch.equal(captured[name], called[name]), name
         assert all(torch.equal(a, b) for a, b in zip(captured["pools"], called["pools"]))
         assert int(called["tokens"].status) == 0 and int(captured["tokens"].status) == 0
+
+
+def test_two_threads_with_streams_and_head_sizes_of_their_own():
+    """Calls of both kinds of kernels from two threads at once: each gets the bits that it gets alone."""
+    import threading
+
+    from cacheir_b200 import serving_ops as S
+
+    shapes = [[(512, torch.float32), (128, torch.float16), (64, torch.float32)], [(80, torch.float32), (64, torch.bfloat16), (256, torch.float32)]]
+    plans = []
+    for side, kinds in enumerate(shapes):
+        calls = []
+        for i, (dim, dtype) in enumerate(kinds):
+            q, keys, values, table, lens, starts, prefix_table, prefix_lens = _paged(60 + 3 * side + i, [(3, 90), (2, 33)], [[4, 0, 20], [1, 50]], 8, 2, dim, 16, dtype)
+            given = S.PrefixGroups(_i32(starts), prefix_table, _i32(prefix_lens))
+            workspace = torch.empty(S.shared_prefix_workspace_bytes(5, 8, dim), device=DEV, dtype=torch.uint8)
+            args = (q, keys, values, table, lens, given)
+            calls.append((args, workspace, S.shared_prefix_attention(*args, workspace=workspace)))
+        plans.append((torch.cuda.Stream(), calls))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(stream, calls):
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(60):
+                    for args, workspace, want in calls:
+                        if not torch.equal(S.shared_prefix_attention(*args, workspace=workspace), want):
+                            wrong.append(want.shape)
+        except Exception as error:                           # (a thread's exception would be lost)
+            wrong.append(error)
+    threads = [threading.Thread(target=work, args=plan) for plan in plans]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

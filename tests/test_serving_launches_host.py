@@ -132,3 +132,19 @@ def test_every_lookup_of_the_encoder_is_made_once_for_all_threads():
     for source in sorted((ROOT / "cacheir_b200" / "csrc").glob("*.cu*")):
         for call in re.finditer(r"cudaGetDriverEntryPoint\(", text := source.read_text()):
             assert re.search(r"static const EncodeTiledFn fn = \[\] \{[^}]*$", text[: call.start()]), source.name
+
+
+def test_shared_memory_of_a_kernel_never_shrinks(tmp_path):
+    """Head sizes of the general attention kernels need 36 to 148 KB. What a kernel may have holds for all threads: a call with a smaller head must
+    not take from another what that has just asked for. It is asked for once per element type."""
+    two, after = _run(tmp_path, """
+  int a = 1, b = 1;
+  beside([&] { a = attention(4, 8, 2, 512, CACHEIR_B200_F32, 1); }, [&] { b = attention(4, 8, 2, 96, CACHEIR_B200_F32, 1); });
+  std::printf("%d %d\\n", a, b);
+  asked = 0;
+  for (int dtype : {CACHEIR_B200_F32, CACHEIR_B200_F16, CACHEIR_B200_BF16})
+    for (int dim : {512, 80, 512, 33})
+      if (attention(4, 8, 2, dim, dtype, 1)) return 1;
+  std::printf("%d %d\\n", lowered, asked);""")
+    assert two == [0, 0]
+    assert after == [0, 2]
