@@ -384,7 +384,7 @@ def load_shared() -> ctypes.CDLL:
 
 
 def group_device_status(reset: bool = True) -> int:
-    """First bounded wait that gave up in any loaded library of the ragged families (0: none)."""
+    """First bounded wait that gave up in any loaded library beside the core one (0: none)."""
     found = [int(getattr(lib, f"cacheir_b200_{name}_device_status")(int(reset))) for name, lib in _GROUPS.items()]
     return next((status for status in found if status != 0), 0)
 

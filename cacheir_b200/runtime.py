@@ -1667,9 +1667,9 @@ class B200DecodeRuntime:
         and clears the word."""
         from . import _lib
         with torch.cuda.device(self.device):
-            status = hybrid_ops.device_status() if self._engine.ragged else int(_lib.load().cacheir_b200_device_status(1))
-            if status == 0 and self._engine.shared_prefixes:
-                status = _lib.group_device_status()
+            # (all words are read, and so cleared: any runtime may have called the serving library)
+            found = [0 if self._engine.ragged else int(_lib.load().cacheir_b200_device_status(1)), _lib.group_device_status()]
+        status = next((word for word in found if word != 0), 0)
         if status != 0:
             raise RuntimeError(f"cacheir_b200 device status {status:#x}: a bounded wait on the GPU gave up "
                                f"(kernel class {status >> 8}, wait {status & 0xFF}); the last results are undefined")

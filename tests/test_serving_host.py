@@ -264,3 +264,36 @@ def test_what_a_wait_says_is_the_same_in_all_lanes_of_a_warp():
         kept = [line.strip() for line in lines if re.search(r"\bmbar_(try_)?wait\(", line) and "__all_sync(" not in line
                 and not re.match(r"\s*(for \([^()]*\) )?mbar_wait\(", line)]
         assert not kept, (name, kept)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("shared_prefixes", [False, True])
+def test_a_runtime_reports_waits_of_every_library_that_it_may_call(monkeypatch, ragged, shared_prefixes):
+    """`score_tokens` calls the serving library on any runtime. Each check reads and clears all words, so that the next one reports what came after it."""
+    from types import SimpleNamespace
+
+    from cacheir_b200 import _lib
+    from cacheir_b200.runtime import B200DecodeRuntime
+
+    words = {"core": 0, "ragged": 0, "serving": 0}
+
+    def word(name):
+        def read(reset):
+            found = words[name]
+            words[name] = 0 if reset else found
+            return found
+        return read
+    monkeypatch.setattr(_lib, "_LIB", SimpleNamespace(cacheir_b200_device_status=word("core")))
+    monkeypatch.setattr(_lib, "_GROUPS", {name: SimpleNamespace(**{f"cacheir_b200_{name}_device_status": word(name)}) for name in ("ragged", "serving")})
+    if ragged:
+        monkeypatch.setattr(_lib, "_LIB", None)               # (a ragged family's process may not have the core library at all)
+        monkeypatch.setattr(_lib, "load", lambda: pytest.fail("the core library is not this runtime's"))
+    runtime = SimpleNamespace(device=-1, _engine=SimpleNamespace(ragged=ragged, shared_prefixes=shared_prefixes))
+    check = lambda: B200DecodeRuntime.check_device_status(runtime)
+    check()
+    for gave_up in ({"serving": 0x1001}, {"ragged" if ragged else "core": 0x302, "serving": 0x1001}):
+        words.update(gave_up)
+        with pytest.raises(RuntimeError, match="gave up"):
+            check()
+        check()
+        assert not any(words.values())
