@@ -27,26 +27,28 @@ prefix_general_kernel(const cacheir_b200_prefix_args a, const PrefixParts parts,
   float* s_v = s_k + kTileKeys * (D + 1);              // [kTileKeys][D]
   float* s_p = s_v + kTileKeys * D;                    // [kTileRows][kTileKeys + 1]
   float* s_scale = s_p + kTileRows * (kTileKeys + 1);  // [kTileRows]
-  const bool common = static_cast<int>(blockIdx.z) < common_tiles;
+  const bool common = static_cast<int>(blockIdx.x) < common_tiles;
   // ---- which query rows (row = base + i / group, head i % group) and which keys ----
   int base, first, rows, key_lo, key_hi;
   const int32_t* pages;
   if (common) {
-    int tile = blockIdx.z, g = 0;
-    for (; g < a.groups; ++g) {
-      const int tiles = ((group_start(a, g + 1) - group_start(a, g)) * group + kTileRows - 1) / kTileRows;
-      if (tile < tiles) break;
-      tile -= max(tiles, 0);
+    // Group g has the tiles from floor(start heads / kTileRows) + g on: at least as many up to those of the next group as its rows fill.
+    const int tile = blockIdx.x;
+    auto first_tile = [&](int g) { return static_cast<int>(static_cast<long long>(group_start(a, g)) * group / kTileRows) + g; };
+    int g = 0, hi = a.groups;
+    while (hi - g > 1) {
+      const int mid = (g + hi) >> 1;
+      if (first_tile(mid) <= tile) g = mid; else hi = mid;
     }
-    if (g == a.groups) return;
     base = group_start(a, g);
-    first = tile * kTileRows;
+    first = (tile - first_tile(g)) * kTileRows;
     rows = min(kTileRows, (group_start(a, g + 1) - base) * group - first);
+    if (first < 0 || rows <= 0) return;
     key_lo = 0;
     key_hi = prefix_of_group(a, g);
     pages = a.prefix_table + static_cast<size_t>(g) * a.prefix_pages;
   } else {
-    const int per_row = (group + kTileRows - 1) / kTileRows, tile = blockIdx.z - common_tiles;
+    const int per_row = (group + kTileRows - 1) / kTileRows, tile = blockIdx.x - common_tiles;
     base = tile / per_row;
     first = tile % per_row * kTileRows;
     rows = min(kTileRows, group - first);
@@ -56,7 +58,7 @@ prefix_general_kernel(const cacheir_b200_prefix_args a, const PrefixParts parts,
   }
   // neighbouring pieces of the same size, whole key tiles
   const int keys = max(key_hi - key_lo, 0), step = ((keys + half - 1) / half + kTileKeys - 1) / kTileKeys * kTileKeys;
-  const int piece = blockIdx.x;
+  const int piece = blockIdx.z;
   const long long begin = key_lo + static_cast<long long>(piece) * step;
   const int lo = static_cast<int>(min(begin, static_cast<long long>(key_hi))), hi = static_cast<int>(min(begin + step, static_cast<long long>(key_hi)));
 
@@ -176,9 +178,9 @@ prefix_join_kernel(const cacheir_b200_prefix_args a, const PrefixParts parts) {
 template <typename T>
 int launch_general(const cacheir_b200_prefix_args& a, PrefixParts parts, cudaStream_t stream) {
   const int group = a.heads / a.kv_heads;
-  const long long common = (static_cast<long long>(a.batch) * group + kTileRows - 1) / kTileRows + a.groups;
+  const long long common = static_cast<long long>(a.batch) * group / kTileRows + a.groups;
   const long long tiles = (a.groups > 0 ? common : 0) + static_cast<long long>(a.batch) * ((group + kTileRows - 1) / kTileRows);
-  if (tiles > 65535) return CACHEIR_B200_ELIMIT;
+  if (tiles > 0x7fffffffLL) return CACHEIR_B200_ELIMIT;
   const long long want = 4LL * kNumSMs / (tiles * a.kv_heads);
   const int half = static_cast<int>(want < 1 ? 1 : want > parts.pieces / 2 ? parts.pieces / 2 : want);
   parts.pieces = 2 * half;
@@ -186,7 +188,7 @@ int launch_general(const cacheir_b200_prefix_args& a, PrefixParts parts, cudaStr
   static std::atomic<unsigned long long> done{0};
   cudaError_t e = allow_shared_memory(done, reinterpret_cast<const void*>(prefix_general_kernel<T>), static_cast<int>(general_smem(kGeneralDim)));
   if (e == cudaSuccess)
-    e = launch_chained(prefix_general_kernel<T>, dim3(half, a.kv_heads, static_cast<unsigned>(tiles)), dim3(kGeneralThreads), smem, stream, a, parts,
+    e = launch_chained(prefix_general_kernel<T>, dim3(static_cast<unsigned>(tiles), a.kv_heads, half), dim3(kGeneralThreads), smem, stream, a, parts,
                        static_cast<int>(a.groups > 0 ? common : 0));
   if (e == cudaSuccess) e = launch_chained(prefix_join_kernel<T>, dim3(a.heads, a.batch), dim3(128), 0, stream, a, parts);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();

@@ -328,8 +328,8 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     q: [B, H, D] (rows may be strided views); k_cache/v_cache: [slots, KVH, page, D] contiguous, of q's dtype; page_table: int32
     [B, max_pages], every row's own page list from its first token on; seq_lens: int32 [B]. Row b attends to tokens t < seq_lens[b]:
     those below its group's prefix through groups.table, the others through page_table (whose entries below the prefix are not read). A row
-    of length 0, or below, gives zeros. `workspace`: `shared_prefix_workspace_bytes(B, H, D)` bytes of any type; calls that may overlap
-    need one each (default: a fresh one)."""
+    of length 0, or below, gives zeros. B up to 65535, D up to 512. `workspace`: `shared_prefix_workspace_bytes(B, H, D)` bytes of any type;
+    calls that may overlap need one each (default: a fresh one)."""
     batch, heads, dim, q_stride = _check_heads("q", q)
     shape = k_cache.shape
     if len(shape) != 4 or v_cache.shape != shape:

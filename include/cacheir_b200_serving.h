@@ -99,7 +99,8 @@ int cacheir_b200_rotary_append(const cacheir_b200_rotary_args* args, void* strea
  * prefix_pages * page_size counts as that long; rows outside every group have no prefix. seq_lens[b] <= 0 gives zeros.
  * A key with a score of -inf has no weight (a row of such keys alone gives zeros); NaN among a row's scores gives NaN. A row that ends
  * inside its group's prefix expects finite keys and values in all of the prefix: those behind its end are weighed with 0, not left out.
- * Tables of up to 2^30 tokens (CACHEIR_B200_ELIMIT).
+ * Up to 65535 rows and as many key/value heads, tables of up to 2^30 tokens (CACHEIR_B200_ELIMIT), heads of up to 512
+ * (CACHEIR_B200_EUNSUPPORTED).
  *   num_slots: slots of the pools; page ids outside them read as zeros.
  *   workspace: cacheir_b200_shared_prefix_workspace_bytes(...) bytes, 16-byte aligned, used by this call's kernels only: calls that may
  *   overlap need one each.

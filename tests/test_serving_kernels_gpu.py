@@ -862,3 +862,26 @@ def test_two_threads_with_streams_and_head_sizes_of_their_own():
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("groups", [[(i % 5, i * 7 % 40) for i in range(2110)], [(4220, 19)]])
+def test_general_attention_of_more_tiles_than_a_narrow_grid_takes(groups):
+    """64 heads on one key/value head, thousands of rows of a few tokens: 67 thousand tiles and more."""
+    from cacheir_b200 import serving_ops as S
+
+    tails = [[(i + j) % 6 for j in range(n)] for i, (n, _) in enumerate(groups)]
+    q, keys, values, table, lens, starts, prefix_table, prefix_lens = _paged(70, groups, tails, 64, 1, 16, 8, torch.float32)
+    rows = len(lens)
+    assert rows * 64 // 8 * 2 > 65535
+    owner = [g for g, (n, _) in enumerate(groups) for _ in range(n)]
+    got = S.shared_prefix_attention(q, keys, values, table, lens, S.PrefixGroups(_i32(starts), prefix_table, _i32(prefix_lens)))
+    want, size = _attend(q, keys, values, table, lens, 0.25, owner, prefix_table, prefix_lens)
+    _check_attention(got, want, size, torch.float32)
+    # rows before the first group and behind the last one belong to none: the same keys out of their own pages
+    part = S.PrefixGroups(_i32([starts[1] if len(groups) > 1 else 700, starts[-2] if len(groups) > 1 else 4000]), prefix_table[1:2] if len(groups) > 1 else prefix_table,
+                          _i32([0 if len(groups) > 1 else 16]))
+    mine = table.clone()
+    for b in range(rows):
+        shared = prefix_lens[owner[b]] // 8
+        mine[b, :shared] = prefix_table[owner[b], :shared]
+    _check_attention(S.shared_prefix_attention(q, keys, values, mine, lens, part), want, size, torch.float32)

@@ -148,3 +148,12 @@ def test_shared_memory_of_a_kernel_never_shrinks(tmp_path):
   std::printf("%d %d\\n", lowered, asked);""")
     assert two == [0, 0]
     assert after == [0, 2]
+
+
+def test_general_attention_takes_any_number_of_rows_that_the_entry_takes(tmp_path):
+    """Tiles of the general kernels go where a grid is widest. Rows, heads per key/value head, groups: what counted 65536 tiles and more was refused."""
+    [codes] = _run(tmp_path, """
+  const int codes[] = {attention(65535, 8, 8, 80, CACHEIR_B200_F32, 65535), attention(4096, 64, 1, 80, CACHEIR_B200_BF16, 1), attention(65535, 64, 1, 64, CACHEIR_B200_F32, 0),
+                       attention(65535, 8, 1, 64, CACHEIR_B200_F16, 3, 8), attention(65536, 8, 8, 80, CACHEIR_B200_F32, 1)};
+  for (int code : codes) std::printf("%d ", code);""")
+    assert codes == [0, 0, 0, 0, -5]
