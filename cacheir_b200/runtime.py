@@ -473,7 +473,7 @@ class _Engine:
         length or page list changed. Admitting or retiring a request therefore costs a few small copies, not
         a new lowering and a new CUDA-graph capture."""
         needed_pages = max((s.kv_cache.tokens + 1 + self.page_size - 1) // self.page_size for s in sessions)
-        more = {"shared_prefixes": True} if self.shared_prefixes else {}
+        more = {"shared_prefixes": True} if self.shared_prefixes and len(sessions) > 1 else {}      # (one row shares nothing)
         return self._plan(("decode", len(sessions)), needed_pages, lambda width: self.plan_class(self, len(sessions), width, **more))
 
 

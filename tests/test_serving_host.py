@@ -297,3 +297,19 @@ def test_a_runtime_reports_waits_of_every_library_that_it_may_call(monkeypatch, 
             check()
         check()
         assert not any(words.values())
+
+
+def test_a_decode_step_of_one_row_shares_nothing():
+    """It is lowered like that of a runtime without `shared_prefixes`: one launch of the ordinary attention, fused with the next product's activations
+    where there are such."""
+    from types import SimpleNamespace
+
+    from cacheir_b200.runtime import _Engine
+
+    def lowered(shared_prefixes, sessions):
+        engine = SimpleNamespace(page_size=16, shared_prefixes=shared_prefixes, _plan=lambda key, pages, make: (key, make(pages)),
+                                 plan_class=lambda engine, batch, width, **more: (batch, width, more))
+        return _Engine.plan_for(engine, [SimpleNamespace(kv_cache=SimpleNamespace(tokens=20)) for _ in range(sessions)])
+    assert lowered(False, 1) == lowered(True, 1) == (("decode", 1), (1, 2, {}))
+    assert lowered(False, 3) == (("decode", 3), (3, 2, {}))
+    assert lowered(True, 3) == (("decode", 3), (3, 2, {"shared_prefixes": True}))

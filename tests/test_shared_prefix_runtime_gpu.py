@@ -129,3 +129,20 @@ def test_scores_of_tokens(dtype, length):
     assert rt.kv_cache.tokens == length
     with pytest.raises(ValueError):
         rt.score_tokens([1])
+
+
+def test_a_session_alone_takes_the_ordinary_attention():
+    """Its logits are the bits of a runtime without the option, its launches too (int8: attention writes the next product's activations)."""
+    found = []
+    for on in (False, True):
+        rt = _runtime("float16", heads=8, kv_heads=2, head_dim=128, quant="int8", shared_prefixes=on)
+        holder = rt.fork()
+        holder.prefill_tokens(PROMPT)
+        s = rt.fork()
+        s.kv_cache.share_prefix(holder.kv_cache, 128)
+        s.run([[5, 6, 7]], mode="prefill", reset_kv=False)
+        logits = [rt.run_decode_batch([s], [t]).clone() for t in (3, 1, 4, 1, 5)]
+        counts = {name: n for name, n in rt.cache_stats()["kernel_counts"].items() if "attention" in name}
+        found.append((torch.cat(logits), counts, rt._engine.plans[("decode", 1)].launches_per_step))
+    assert torch.equal(found[0][0], found[1][0]) and found[0][1:] == found[1][1:]
+    assert "b200.shared_prefix_attention" not in found[1][1]
