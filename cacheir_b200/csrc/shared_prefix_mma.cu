@@ -601,7 +601,9 @@ prefix_common_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_co
       const int in_tile = w * half_rows + (r * by_group >> 16);          // this thread's row of the item
       const bool real = r < half_rows * group && in_tile < walk.rows;
       const int b_row = walk.row0 + (real ? in_tile : 0), head = walk.kvh * group + (real ? r - (r * by_group >> 16) * group : 0);
-      const int limit = real ? min(walk.prefix, a.seq_lens[b_row]) : walk.prefix;      // keys that the row sees
+      // Keys that the row sees: all, or none where it ends inside the prefix. What stands behind its end may hold anything, also values that are
+      // no numbers, and 0 * value would not be 0: such a row's keys are its own, and the outputs that it gets here have no weight.
+      const int limit = real && a.seq_lens[b_row] < walk.prefix ? 0 : walk.prefix;
       float m_ref = -INFINITY, l_run = 0.f;
       int last = 0;
       for (int t = 0, s = two ? step + ((step ^ w) & 1) : step; t < walk.tiles && ok; ++t, s += two ? 2 : 1) {
@@ -868,10 +870,11 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
     }
   }
   // Lengths, group, first page ids and queries are asked for together as far as they can be.
-  const int len = min(max(a.seq_lens[row], 0), a.max_pages * a.page_size);
+  const int tokens = max(a.seq_lens[row], 0);
   int prefix;
-  group_of_row(a, row, &prefix);
-  const int from = min(prefix, len);
+  const int in_group = group_of_row(a, row, &prefix);
+  const bool inside = tokens < prefix;                           // (no key of it is common)
+  const int len = inside ? tokens : min(tokens, a.max_pages * a.page_size), from = inside ? 0 : min(prefix, len);
   const int chunk0 = from / kChunk, chunks = len > from ? (len + kChunk - 1) / kChunk - chunk0 : 0, per = (chunks + p.splits - 1) / p.splits;
   const int begin = chunk0 + min(chunks, split * per), end = chunk0 + min(chunks, (split + 1) * per);
   uint32_t qa[D / 16][4];                                        // queries as the A operand: rows = heads
@@ -885,7 +888,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
         qa[k][i] = h < heads ? *reinterpret_cast<const uint32_t*>(q + static_cast<size_t>(h) * D + col) : 0u;
       }
   }
-  const int32_t* pages = a.page_table + static_cast<size_t>(row) * a.max_pages;
+  const int32_t* pages = inside ? a.prefix_table + static_cast<size_t>(in_group) * a.prefix_pages : a.page_table + static_cast<size_t>(row) * a.max_pages;
   const int outside = a.num_slots * a.kv_heads * a.page_size;   // rows behind the pool read as zeros
   const int mine = begin + warp < end ? (end - begin - warp + WARPS - 1) / WARPS : 0;          // chunks begin + warp + i * WARPS
   const Division by_page(a.page_size);

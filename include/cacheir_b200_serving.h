@@ -97,8 +97,9 @@ int cacheir_b200_rotary_append(const cacheir_b200_rotary_args* args, void* strea
  * Row b attends to tokens t < seq_lens[b]; those below its group's prefix are read through prefix_table, the others through
  * page_table[b] (entries of pages that lie wholly in the prefix are not read). A prefix may end inside a page. A prefix longer than
  * prefix_pages * page_size counts as that long; rows outside every group have no prefix. seq_lens[b] <= 0 gives zeros.
- * A key with a score of -inf has no weight (a row of such keys alone gives zeros); NaN among a row's scores gives NaN. A row that ends
- * inside its group's prefix expects finite keys and values in all of the prefix: those behind its end are weighed with 0, not left out.
+ * A key with a score of -inf has no weight (a row of such keys alone gives zeros); NaN among a row's scores gives NaN. What stands behind a
+ * row's end, in its last page or in the rest of its group's prefix, may hold anything. A row that ends inside its group's prefix reads its
+ * keys for itself, through prefix_table.
  * Up to 65535 rows and as many key/value heads, tables of up to 2^30 tokens (CACHEIR_B200_ELIMIT), heads of up to 512
  * (CACHEIR_B200_EUNSUPPORTED).
  *   num_slots: slots of the pools; page ids outside them read as zeros.

@@ -885,3 +885,32 @@ def test_general_attention_of_more_tiles_than_a_narrow_grid_takes(groups):
         shared = prefix_lens[owner[b]] // 8
         mine[b, :shared] = prefix_table[owner[b], :shared]
     _check_attention(S.shared_prefix_attention(q, keys, values, mine, lens, part), want, size, torch.float32)
+
+
+@pytest.mark.parametrize("dtype,dim,page", [(torch.float16, 128, 16), (torch.bfloat16, 64, 48), (torch.bfloat16, 128, 16), (torch.float32, 64, 16)])
+@pytest.mark.parametrize("more", [0, 40, 70])
+def test_rows_that_end_inside_their_prefix_see_nothing_behind_their_end(dtype, dim, page, more):
+    """Others of the group go on to tokens whose keys and values are no numbers, or infinite. More groups than a warp and than a block lays out by itself."""
+    from cacheir_b200 import serving_ops as S
+
+    groups = [(70, 300), (3, 1000)] + [(1, 17)] * more
+    ends = [1, 15, 16, 17, 127, 128, 129, 140, 141, 142]
+    tails = [[(ends[i % 10] if i % 10 else i // 10) - 300 for i in range(68)] + [0, 9], [-999, -700, 40]] + [[i % 3] for i in range(more)]
+    q, keys, values, table, lens, starts, prefix_table, prefix_lens = _paged(80 + more, groups, tails, 8, 2, dim, page, dtype)
+    owner = _owners(starts, len(lens))
+    want, size = _attend(q, keys, values, table, lens, dim ** -0.5, owner, prefix_table, prefix_lens)
+    given = S.PrefixGroups(_i32(starts), prefix_table, _i32(prefix_lens))
+    _check_attention(S.shared_prefix_attention(q, keys, values, table, lens, given), want, size, dtype)
+    for t, k, v in ((142, math.nan, math.nan), (143, math.inf, -math.inf), (299, 1.0, math.inf), (200, math.nan, 1.0)):
+        keys[prefix_table[0, t // page], :, t % page] = k
+        values[prefix_table[0, t // page], :, t % page] = v
+    keys[prefix_table[1, 300 // page], :, 300 % page] = math.nan
+    values[prefix_table[1, 300 // page], :, 300 % page] = math.nan
+    # (a row's own table is not read below the prefix)
+    for b in range(73):
+        table[b, : prefix_lens[owner[b]] // page] = -7
+    got = S.shared_prefix_attention(q, keys, values, table, lens, given)
+    live = torch.tensor([b not in (68, 69, 72) for b in range(len(lens))], device=DEV)
+    _check_attention(got[live], want[live], size[live], dtype)
+    assert bool(got[[68, 69, 72]].isnan().all())
+    assert torch.equal(got[live], S.shared_prefix_attention(q, keys, values, table, lens, given)[live])
