@@ -1627,6 +1627,7 @@ class B200DecodeRuntime:
         ids = [int(t) for t in token_ids]
         if len(ids) < 2:
             raise ValueError("score_tokens needs at least two tokens")
+        serving_ops.check_scoring(int(self._engine.config.vocab_size), top, temperature)       # (before the session's pages are given up)
         logits = self.run([ids], mode="prefill", reset_kv=True)
         tokens = torch.tensor(ids[1:], dtype=torch.int64).to(self.device)
         return serving_ops.token_logprobs(logits[0, :-1], tokens, top=top, temperature=temperature)

@@ -388,6 +388,14 @@ class TokenLogprobs:
     top_logprobs: torch.Tensor | None
 
 
+def check_scoring(vocab: int, top: int, temperature: float) -> None:
+    """What `token_logprobs` takes."""
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"top must be 0 to {MAX_TOP} and no more than the vocabulary")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError("temperature must be 1e-6 to 1e6")
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, *, top: int = 0, temperature: float = 1.0) -> TokenLogprobs:
     """Log probabilities of tokens int64 [R] under softmax(logits / temperature), the rows' entropies, and the `top` likeliest tokens with
     theirs (equal logits by rising index, like `ops.argmax_rows`). logits: [R, V] with dense rows (the row stride may be wider).
@@ -400,10 +408,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, *, top: in
     (rows, vocab), (row_stride, stride) = shape, logits.stride()
     if vocab < 1 or (stride != 1 and vocab > 1) or (rows > 1 and row_stride < vocab):
         raise ValueError("logits must be [R, V] with dense rows that do not overlap")
-    if not 0 <= top <= min(MAX_TOP, vocab):
-        raise ValueError(f"top must be 0 to {MAX_TOP} and no more than the vocabulary")
-    if not 1e-6 <= temperature <= 1e6:
-        raise ValueError("temperature must be 1e-6 to 1e6")
+    check_scoring(vocab, top, temperature)
     if tokens is not None and (tokens.dtype is not torch.int64 or tokens.numel() != rows or not tokens.is_contiguous()):
         raise ValueError("tokens must be contiguous int64 [R]")
     code, device = dtype_code(logits.dtype), logits.device

@@ -313,3 +313,17 @@ def test_a_decode_step_of_one_row_shares_nothing():
     assert lowered(False, 1) == lowered(True, 1) == (("decode", 1), (1, 2, {}))
     assert lowered(False, 3) == (("decode", 3), (3, 2, {}))
     assert lowered(True, 3) == (("decode", 3), (3, 2, {"shared_prefixes": True}))
+
+
+def test_scores_are_refused_before_the_session_is_given_up():
+    """A refused `score_tokens` leaves the session's tokens where they are and runs nothing."""
+    from types import SimpleNamespace
+
+    from cacheir_b200.runtime import B200DecodeRuntime
+
+    runtime = SimpleNamespace(_engine=SimpleNamespace(config=SimpleNamespace(vocab_size=20)), device="cpu", run=lambda *a, **k: pytest.fail("the prompt was run"))
+    for wrong in (dict(top=33), dict(top=21), dict(top=-1), dict(temperature=0.0), dict(temperature=float("nan")), dict(temperature=1e7)):
+        with pytest.raises(ValueError):
+            B200DecodeRuntime.score_tokens(runtime, [1, 2, 3], **wrong)
+    with pytest.raises(ValueError):
+        B200DecodeRuntime.score_tokens(runtime, [1])
