@@ -208,7 +208,8 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, rule
     """Turns the first rule.rot values of every head of q [R, H, D] and k [R, KVH, D] to positions int32 [R] (rows may be strided views of
     a fused buffer), into q_out (default: in place) and k_out. With slots int32 [R] and the pools [slots, KVH, page, D] the turned k and v
     [R, KVH, D] are also appended: row r to page slots[r] // page, offset slots[r] % page; rows whose slot is outside the pool (padding: -1)
-    are left out altogether. Without slots, k_out defaults to in place; with them, to nowhere but the pool.
+    are left out altogether. Rows with one slot: each value there is of one of them, any. Without slots, k_out defaults to in place; with
+    them, to nowhere but the pool.
 
     Beside `ops.rope_append`: both pair layouts, part of a head, scaled frequencies, float32 to bfloat16, far positions exactly."""
     rows, heads, dim, q_stride = _check_heads("q", q)

@@ -65,7 +65,7 @@ int cacheir_b200_shrink_page_tables(const cacheir_b200_tables_args* args, void* 
  * q [rows][heads][dim], k, v [rows][kv_heads][dim], rows q_stride / k_stride / v_stride elements apart, heads dense. q_out, k_out (either
  * may be NULL, or its input) are dense or have their own row strides. With slots (else NULL, and no pools): row r's k and v go to row
  * slots[r] % page_size of page slots[r] / page_size of k_cache, v_cache [num_slots][kv_heads][page_size][dim]; a row whose slot is
- * outside the pool is left out altogether, q_out and k_out included. Two rows with one slot: either may be the one that stays. */
+ * outside the pool is left out altogether, q_out and k_out included. Rows with one slot: each value there is of one of them, any. */
 #define CACHEIR_B200_ROTARY_INTERLEAVED 0
 #define CACHEIR_B200_ROTARY_HALF 1
 typedef struct {

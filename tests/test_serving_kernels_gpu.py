@@ -914,3 +914,72 @@ def test_rows_that_end_inside_their_prefix_see_nothing_behind_their_end(dtype, d
     _check_attention(got[live], want[live], size[live], dtype)
     assert bool(got[[68, 69, 72]].isnan().all())
     assert torch.equal(got[live], S.shared_prefix_attention(q, keys, values, table, lens, given)[live])
+
+
+def test_rotary_append_of_two_rows_to_one_slot_leaves_values_of_either():
+    """Which of them stays is open, value by value; nothing else of the pool is touched and every row's q is its own."""
+    from cacheir_b200 import serving_ops as S
+
+    rule = S.rotary_rule(64, 10000.0, layout="half", device=DEV)
+    q, k, v = (_randn(i, 300, heads, 64, dtype=torch.float16) for i, heads in ((1, 4), (2, 2), (3, 2)))
+    positions = torch.arange(300, device=DEV, dtype=torch.int32)
+    alone_q, alone_k = torch.empty_like(q), torch.empty_like(k)
+    S.rotary_append(q, k, None, rule, positions, q_out=alone_q, k_out=alone_k)
+    pools = [torch.full((4, 2, 16, 64), 9.0, device=DEV, dtype=torch.float16) for _ in range(2)]
+    out = torch.empty_like(q)
+    slots = torch.where(positions % 3 == 0, 37, 5).to(torch.int32)
+    S.rotary_append(q, k, v, rule, positions, slots=slots, k_cache=pools[0], v_cache=pools[1], q_out=out)
+    assert torch.equal(out, alone_q)
+    for pool, rows in zip(pools, (alone_k, v)):
+        lines = pool.transpose(1, 2).reshape(64, 2, 64)
+        for slot in (5, 37):
+            assert bool((lines[slot] == rows[slots == slot]).any(0).all())
+        rest = torch.ones(64, dtype=torch.bool, device=DEV)
+        rest[[5, 37]] = False
+        assert bool((lines[rest] == 9.0).all())
+
+
+def test_pools_and_logits_of_more_than_two_to_the_31_values():
+    """What lies behind 2^31 values (and 2^32 bytes) is found: appended to, attended to by both kinds of kernels, scored."""
+    from cacheir_b200 import serving_ops as S
+
+    heads, kv_heads, dim, dtype = 16, 8, 128, torch.float16
+    slots = 2 ** 31 // (kv_heads * 16 * dim) + 4000
+    pools = [torch.empty(slots, kv_heads, 16, dim, device=DEV, dtype=dtype) for _ in range(2)]
+    assert pools[0].numel() > 2 ** 31
+    ids = [slots - 1, 3, slots - 3000, 131072, slots - 17, 131071, slots // 2, 70000, slots - 2]
+    for i, pool in enumerate(pools):
+        for page in ids:
+            pool[page] = _randn(page % 1000 + i, kv_heads, 16, dim, dtype=dtype)
+    # appends to both ends of the pool
+    rule = S.rotary_rule(dim, 10000.0, layout="half", device=DEV)
+    q, k, v = (_randn(i, 4, h, dim, dtype=dtype) for i, h in ((1, heads), (2, kv_heads), (3, kv_heads)))
+    where, offset = [slots - 1, 3, 131072, slots - 17], [15, 0, 7, 2]
+    turned, turned_k = torch.empty_like(q), torch.empty_like(k)
+    S.rotary_append(q, k, None, rule, _i32([5, 6, 7, 8]), q_out=turned, k_out=turned_k)
+    S.rotary_append(q, k, v, rule, _i32([5, 6, 7, 8]), slots=_i32([p * 16 + o for p, o in zip(where, offset)]), k_cache=pools[0], v_cache=pools[1], q_out=q)
+    assert torch.equal(q, turned)
+    for row, (p, o) in enumerate(zip(where, offset)):
+        assert torch.equal(pools[0][p, :, o], turned_k[row]) and torch.equal(pools[1][p, :, o], v[row])
+    table = _i32([ids[:3] + [ids[3], ids[4]], ids[:3] + [ids[5], 0], ids[:3] + [ids[6], ids[7]], [ids[8], ids[7], ids[5], 0, 0]])
+    lens, given = _i32([80, 50, 65, 33]), S.PrefixGroups(_i32([0, 3]), _i32([ids[:3]]), _i32([48]))
+    want, size = _attend(q, *pools, table, lens, dim ** -0.5, [0, 0, 0, -1], given.table, [48])
+    for groups in (given, None):
+        _check_attention(S.shared_prefix_attention(q, *pools, table, lens, groups), want, size, dtype)
+    # the same memory as pages of eight tokens, for the general kernels
+    small = [pool.view(2 * slots, kv_heads, 8, dim) for pool in pools]
+    halves = lambda t: torch.stack([2 * t, 2 * t + 1], dim=-1).flatten(-2).to(torch.int32).contiguous()
+    given = S.PrefixGroups(given.rows, halves(given.table), given.lens)
+    want, size = _attend(q, *small, halves(table), lens, dim ** -0.5, [0, 0, 0, -1], given.table, [48])
+    for groups in (given, None):
+        _check_attention(S.shared_prefix_attention(q, *small, halves(table), lens, groups), want, size, dtype)
+    del pools, small, pool
+    logits = torch.empty(17000, 128256, device=DEV, dtype=torch.bfloat16)
+    assert logits.numel() > 2 ** 31
+    rows = [0, 8371, 8372, 16742, 16744, 16999]              # on both sides of 2^30 and 2^31 values
+    for r in rows:
+        logits[r] = _randn(r, 128256, dtype=torch.bfloat16) * 3.0
+    tokens = torch.arange(17000, device=DEV) * 7 % 128256
+    got, at = S.token_logprobs(logits, tokens, top=3), torch.tensor(rows, device=DEV)
+    picked = S.TokenLogprobs(got.logprobs[at], got.entropy[at], got.top_ids[at], got.top_logprobs[at])
+    _check_logprobs(picked, logits[at], tokens[at], 3, 1.0)
