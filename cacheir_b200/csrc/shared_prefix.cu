@@ -21,34 +21,35 @@ __global__ void __launch_bounds__(kGeneralThreads)
 prefix_general_kernel(const cacheir_b200_prefix_args a, const PrefixParts parts, const int common_tiles) {
   chain_enter();
   extern __shared__ float smem[];
-  const int D = a.dim, group = a.heads / a.kv_heads, kvh = blockIdx.y, half = parts.pieces / 2;
+  // Blocks in the order of tiles, key/value heads, pieces: the common parts, which are long, come first.
+  const int D = a.dim, group = a.heads / a.kv_heads, half = parts.pieces / 2;
+  const int piece = blockIdx.x % half, kvh = blockIdx.x / half % a.kv_heads, place = blockIdx.x / half / a.kv_heads;
   float* s_q = smem;                                   // [kTileRows][D]
   float* s_k = s_q + kTileRows * D;                    // [kTileKeys][D + 1]
   float* s_v = s_k + kTileKeys * (D + 1);              // [kTileKeys][D]
   float* s_p = s_v + kTileKeys * D;                    // [kTileRows][kTileKeys + 1]
   float* s_scale = s_p + kTileRows * (kTileKeys + 1);  // [kTileRows]
-  const bool common = static_cast<int>(blockIdx.x) < common_tiles;
+  const bool common = place < common_tiles;
   // ---- which query rows (row = base + i / group, head i % group) and which keys ----
   int base, first, rows, key_lo, key_hi;
   const int32_t* pages;
   if (common) {
     // Group g has the tiles from floor(start heads / kTileRows) + g on: at least as many up to those of the next group as its rows fill.
-    const int tile = blockIdx.x;
     auto first_tile = [&](int g) { return static_cast<int>(static_cast<long long>(group_start(a, g)) * group / kTileRows) + g; };
     int g = 0, hi = a.groups;
     while (hi - g > 1) {
       const int mid = (g + hi) >> 1;
-      if (first_tile(mid) <= tile) g = mid; else hi = mid;
+      if (first_tile(mid) <= place) g = mid; else hi = mid;
     }
     base = group_start(a, g);
-    first = (tile - first_tile(g)) * kTileRows;
+    first = (place - first_tile(g)) * kTileRows;
     rows = min(kTileRows, (group_start(a, g + 1) - base) * group - first);
-    if (first < 0 || rows <= 0) return;
+    if (first < 0) return;                             // (rows before the first group)
     key_lo = 0;
-    key_hi = prefix_of_group(a, g);
+    key_hi = rows <= 0 ? 0 : prefix_of_group(a, g);    // (a tile of no rows looks at no keys)
     pages = a.prefix_table + static_cast<size_t>(g) * a.prefix_pages;
   } else {
-    const int per_row = (group + kTileRows - 1) / kTileRows, tile = blockIdx.x - common_tiles;
+    const int per_row = (group + kTileRows - 1) / kTileRows, tile = place - common_tiles;
     base = tile / per_row;
     first = tile % per_row * kTileRows;
     rows = min(kTileRows, group - first);
@@ -58,7 +59,6 @@ prefix_general_kernel(const cacheir_b200_prefix_args a, const PrefixParts parts,
   }
   // neighbouring pieces of the same size, whole key tiles
   const int keys = max(key_hi - key_lo, 0), step = ((keys + half - 1) / half + kTileKeys - 1) / kTileKeys * kTileKeys;
-  const int piece = blockIdx.z;
   const long long begin = key_lo + static_cast<long long>(piece) * step;
   const int lo = static_cast<int>(min(begin, static_cast<long long>(key_hi))), hi = static_cast<int>(min(begin + step, static_cast<long long>(key_hi)));
 
@@ -180,15 +180,16 @@ int launch_general(const cacheir_b200_prefix_args& a, PrefixParts parts, cudaStr
   const int group = a.heads / a.kv_heads;
   const long long common = static_cast<long long>(a.batch) * group / kTileRows + a.groups;
   const long long tiles = (a.groups > 0 ? common : 0) + static_cast<long long>(a.batch) * ((group + kTileRows - 1) / kTileRows);
-  if (tiles > 0x7fffffffLL) return CACHEIR_B200_ELIMIT;
   const long long want = 4LL * kNumSMs / (tiles * a.kv_heads);
   const int half = static_cast<int>(want < 1 ? 1 : want > parts.pieces / 2 ? parts.pieces / 2 : want);
   parts.pieces = 2 * half;
+  const long long blocks = tiles * a.kv_heads * half;
+  if (blocks > 0x7fffffffLL) return CACHEIR_B200_ELIMIT;
   const size_t smem = general_smem(a.dim);
   static std::atomic<unsigned long long> done{0};
   cudaError_t e = allow_shared_memory(done, reinterpret_cast<const void*>(prefix_general_kernel<T>), static_cast<int>(general_smem(kGeneralDim)));
   if (e == cudaSuccess)
-    e = launch_chained(prefix_general_kernel<T>, dim3(static_cast<unsigned>(tiles), a.kv_heads, half), dim3(kGeneralThreads), smem, stream, a, parts,
+    e = launch_chained(prefix_general_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(kGeneralThreads), smem, stream, a, parts,
                        static_cast<int>(a.groups > 0 ? common : 0));
   if (e == cudaSuccess) e = launch_chained(prefix_join_kernel<T>, dim3(a.heads, a.batch), dim3(128), 0, stream, a, parts);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
