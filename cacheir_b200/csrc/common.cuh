@@ -129,7 +129,8 @@ __device__ __forceinline__ float silu_fast(float g) { return __fdividef(g, 1.f +
 // until it has ended and its results can be seen. What stands in front of chain_wait touches nothing that another kernel may write:
 // barriers, and requests that bring weights into L2 (which any later store would still go through). Every thread calls chain_wait
 // before it looks at memory, so that the end of one kernel implies the end of all before it, and chain_next after it, so that no
-// more than one kernel is ahead. Tensor memory is allocated behind chain_wait: a CTA that came early could otherwise hold what
+// more than one kernel is ahead. (The kernels of a row's own keys and of the join of shared_prefix_mma.cu look at inputs earlier and say there why
+// they may.) Tensor memory is allocated behind chain_wait: a CTA that came early could otherwise hold what
 // the kernel that it waits for still has to allocate.
 // Launch and first steps of a kernel are 0.9 to 1.2 us of its 2 to 10 us in a decode step; a chain of plain streaming kernels of
 // 8 MB takes 3.0 us each without, 1.5 with weights asked for ahead (34 MB: 6.7 and 4.9).

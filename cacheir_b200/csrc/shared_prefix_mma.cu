@@ -15,12 +15,14 @@
 // outputs, which stay in tensor memory, are hardly ever rescaled; probabilities are rounded to the element type as the second MMA's operand,
 // their sums are not.
 //
-// Measured (32 query and 8 key/value heads of 128, fp16, whole call): 64 rows behind 32768 common tokens 51 us, of which 25.6 us are the
-// bytes and 20.8 us the products; 32 rows behind 2048 tokens 20.0 us (bytes 7.1 us). 128 rows in 16 groups of ragged prefixes with 64 and 8
-// heads, bf16: 66.6 us (bytes 46.5 us). A call spends about 5.5 us before the first scores (launch, plan, page ids, copies), and about 3 us on
-// joining. In between a tile of 256 query rows takes 3300 cycles, of which the tensor cores work 2048: the rest is the way from scores by
-// the softmax to the second product (2300 cycles a step, 1500 of them exponentials), which the other group of warps hides in part. Neither
-// a share of the exponentials by polynomials nor reading scores once into 128 registers changed that (56.0 us became 55.7 and 56.3).
+// Measured (32 query and 8 key/value heads of 128, fp16; all three kernels, replayed from a graph in bursts at 1965 MHz; a second of calls on end,
+// under the power cap, is slower: 59.1 us for the first): 64 rows behind 32768 common tokens 52.2 us, of which 25.6 us are the bytes and 20.8 us
+// the products; 32 rows behind 2048 tokens 20.3 us (bytes 7.1 us). 128 rows in 16 groups of ragged prefixes with 64 and 8 heads, bf16: 66.6 us
+// (bytes 46.5 us). A call spends about 5.5 us before the first scores (launch, plan, page ids, copies), and about 3 us on joining. In between a
+// tile of 256 query rows takes 3300 cycles, of which the tensor cores work 2048: probabilities lie over the scores they come from, so that a
+// group of warps' next scores are issued behind its second product, and its step is scores (512), softmax (2300, 1500 of them exponentials) and
+// second product (512) one after the other, beside which only the other group's run. Neither a share of the exponentials by polynomials nor
+// reading scores once into 128 registers changed that (56.0 us became 55.7 and 56.3).
 #include "shared_prefix.cuh"
 
 #include <cuda.h>
@@ -207,7 +209,7 @@ __device__ __forceinline__ Weights group_weights(const PlanGroup& g, int units, 
 // Blocks that take part. No item may be in more pieces than there is scratch for: n tiles touch ceil((n - 1) / share) + 1 blocks at most. And
 // the common parts get as many SMs as is their share of the work, so that the other kernel can have the rest of them meanwhile: 16 own
 // tokens of a key/value head (8 KB) take an SM about a twentieth of a unit's time (64 KB), and a row's own part costs as much as eleven of
-// those before it has any. `lens`: tokens of all rows. (64 rows with 144 own tokens on average behind 32768, 128 rows with 350 behind up to 4095:
+// those before it has any. `lens`: tokens of all rows. (Device times: 64 rows with 144 own tokens on average behind 32768, 128 rows with 350 behind up to 4095:
 // 51.2 and 66.6 us; an eighteenth 51.3 and 68.5, a twenty-second 52.8 and 66.5, fourteen and a twentieth 51.4 and 68.2.)
 __device__ __forceinline__ int plan_ctas(const cacheir_b200_prefix_args& a, int pieces, int own_heads, int units, const Weights& w, long long lens, int grid) {
   if (units <= 0) return 0;
@@ -1266,8 +1268,9 @@ int launch_fast(const cacheir_b200_prefix_args& a, const PrefixParts& parts, cud
   }
   OwnParams o{a, parts, a.groups > 0 ? 1 : 0, tile_rows, (group + 15) / 16, 1, grid, scale_log2};
   const long long blocks = static_cast<long long>(a.batch) * a.kv_heads * o.head_chunks;
-  // (64 rows behind a document, 512 blocks: 51.2 us with two warps, 52.5 with four; 32 rows behind instructions, 256 blocks: 20.1 with four, 23.5
-  // with two, 23.1 with eight; 2 rows of 16000 own tokens, 16 blocks in eight parts: 26.9 with eight, 28.2 with four)
+  // (Device times: 64 rows behind a document, 512 blocks: 51.2 us with two warps, 52.5 with four; 32 rows behind instructions, 256 blocks: 20.1
+  // with four, 23.5 with two, 23.1 with eight, which have rings of three stages and so an SM for themselves; 2 rows of 16000 own tokens, 16 blocks
+  // in eight parts: 26.9 with eight, 28.2 with four)
   if (blocks > 3 * kNumSMs) return launch_own<T, D, 2>(o, tk, tv, stream);
   if (blocks > kNumSMs) return launch_own<T, D, 4>(o, tk, tv, stream);
   // Parts of a row's own keys while there are SMs for them, but no more than there are chunks to share.

@@ -324,7 +324,9 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                             groups: PrefixGroups | None, *, out: torch.Tensor | None = None, softmax_scale: float | None = None,
                             workspace: torch.Tensor | None = None) -> torch.Tensor:
     """`ops.paged_attention_decode_batch` for rows that share prefixes: the keys and values of a group's common tokens are read once and
-    multiplied with the queries of all of its rows.
+    multiplied with the queries of all of its rows. On tensor cores: float16 and bfloat16, heads of 64 and 128, pages of a multiple of 16
+    tokens, up to 64 query heads per key/value head. Everything else takes general kernels that are slower than `ops.paged_attention_decode_batch`
+    is on the same batch.
 
     q: [B, H, D] (rows may be strided views); k_cache/v_cache: [slots, KVH, page, D] contiguous, of q's dtype; page_table: int32
     [B, max_pages], every row's own page list from its first token on; seq_lens: int32 [B]. Row b attends to tokens t < seq_lens[b]:

@@ -28,7 +28,8 @@ extern "C" {
  *   row_seq -1 and slot -1. (Pages come from the caller: slots are meant for pools of fewer than 2^31 rows.)
  * shrink: sequence b keeps its first min(keep_lens[b], seq_lens[b]) tokens (below 0: none). The pages behind them return to the stack,
  *   the first one of the call on top, so that the same tokens would get the same pages again; page_table keeps its entries. The first
- *   held_pages[b] pages of a row (held_pages may be NULL) belong to somebody else and never return.
+ *   held_pages[b] pages of a row (held_pages may be NULL) belong to somebody else and never return. (A sequence that keeps fewer tokens than
+ *   those pages hold has let go of them: extending opens pages of its own in their place, which held_pages must not count any more.)
  *
  * Each is all or nothing. A call that cannot be done changes nothing but `status` (and, for extend, the outputs: no rows, all slots
  * -1); status[0] keeps the first such reason until the caller sets it to 0:
@@ -123,7 +124,8 @@ typedef struct {
   float softmax_scale;
 } cacheir_b200_prefix_args;
 size_t cacheir_b200_shared_prefix_workspace_bytes(int batch, int heads, int dim);
-/* Kernels that one call launches for these extents (aligned, dense q): 2 on CUDA cores; on tensor cores (fp16 and bf16, dim 64 and 128,
+/* Kernels that one call launches for these extents (aligned, dense q): 2 on CUDA cores (any type and size, slower than
+ * cacheir_b200_paged_attention_decode_batch on the same batch); on tensor cores (fp16 and bf16, dim 64 and 128,
  * pages of a multiple of 16 tokens, up to 64 query heads per key/value head) 2 without groups, 3 with up to 64 of them, 4 with more. */
 int cacheir_b200_shared_prefix_launches(int batch, int heads, int kv_heads, int dim, int page_size, int groups, int dtype);
 int cacheir_b200_shared_prefix_attention(const cacheir_b200_prefix_args* args, void* stream);
