@@ -8,7 +8,7 @@
 // turn is split off as an integer too; what is left lies in [-1/4, 1/4) half turns and keeps 2^-26 of a turn in a float.
 //
 // Bound by memory: every value is read and written once. One block per row; its cosines are worked out once for all heads. Where there are
-// many rows, small blocks: 16384 rows of 64 + 8 heads of 128 in fp16 take 116 us (5.8 TB/s; from a graph, in bursts: 124 on end, under the power
+// many rows, small blocks: 16384 rows of 64 + 8 heads of 128 in fp16 take 116 us (5.8 TB/s; from a graph, in bursts: 126 on end, under the power
 // cap) with 64 threads a block, 119 with 128 and 134 with 192; few rows want more of a row under way (32 rows: 4.8, 3.5 and 3.1 us). Asking for the values before the cosines, cosines in
 // registers, and rows streamed through shared memory by bulk copies (201 us) were all slower.
 #include "cacheir_b200_serving.h"

@@ -16,7 +16,7 @@
 // their sums are not.
 //
 // Measured (32 query and 8 key/value heads of 128, fp16; all three kernels, replayed from a graph in bursts at 1965 MHz; a second of calls on end,
-// under the power cap, is slower: 59.1 us for the first): 64 rows behind 32768 common tokens 52.2 us, of which 25.6 us are the bytes and 20.8 us
+// under the power cap, is slower: 60 us for the first): 64 rows behind 32768 common tokens 52.2 us, of which 25.6 us are the bytes and 20.8 us
 // the products; 32 rows behind 2048 tokens 20.3 us (bytes 7.1 us). 128 rows in 16 groups of ragged prefixes with 64 and 8 heads, bf16: 66.6 us
 // (bytes 46.5 us). A call spends about 5.5 us before the first scores (launch, plan, page ids, copies), and about 3 us on joining. In between a
 // tile of 256 query rows takes 3300 cycles, of which the tensor cores work 2048: probabilities lie over the scores they come from, so that a

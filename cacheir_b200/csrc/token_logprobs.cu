@@ -10,7 +10,7 @@
 // that holds for any data, ties and masks included.
 //
 // Bound by memory for many rows (2048 x 128256 in bf16: 90 us, 5.8 TB/s), by latency for few (1 x 128256 in fp16 with 5 alternatives: 7.9 us,
-// 64 x 50001 in fp32 with 20: 13.8 us; from a graph, in bursts: a second of the first on end runs into the power cap, 104 us). A row is read by one block, or by a thread-block cluster where
+// 64 x 50001 in fp32 with 20: 13.8 us; from a graph, in bursts: a second of the first on end runs into the power cap, 106 us). A row is read by one block, or by a thread-block cluster where
 // there are few; every warp copies 4 KB pieces (bulk copies, a ring of its own: no barrier between warps) and has two of them on
 // their way. Per value that is half an instruction for the maximum, one to widen it, one for the exponent's argument, one
 // exponential (16 a cycle and SM: 73 % of the memory's rate), half each for the two sums.
