@@ -284,6 +284,7 @@ def prepare(case, seed):
                                                    cu_rows=state["cu_rows"], status=_i32([0]))
             state["tree"] = draft_ops.draft_tree(rows, words, DEV)
             state["accepted"] = draft_ops.accepted_drafts(case["sequences"], state["depth"], DEV)
+            state["handle"] = draft_ops.page_pools([pool for layer in state["pools"] for pool in layer])
     return state
 
 
@@ -397,7 +398,7 @@ def _run_drafts(s):
         from cacheir_b200 import draft_ops
         tree = draft_ops.map_drafts(s["parents"], s["seq_lens"], s["tokens"], s["tree"])
         accepted = draft_ops.accept_drafts(s["chosen"], s["draft_ids"], s["parents"], s["seq_lens"], s["tokens"], s["accepted"])
-        draft_ops.keep_accepted(accepted, s["tokens"], s["pools"])
+        draft_ops.keep_accepted(accepted, s["tokens"], s["handle"])
         return {"positions": tree.positions, "visible": tree.visible, "counts": accepted.counts, "rows": accepted.rows, "next_ids": accepted.next_ids,
                 "keep_lens": accepted.keep_lens, "keys": s["keys"], "values": s["values"]}
     cu, row_seq, most, depth = s["cu_rows"].long(), s["row_seq"].long(), s["most"], s["depth"]
