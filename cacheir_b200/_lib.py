@@ -1,6 +1,7 @@
 """ctypes binding of libcacheir_b200.so (the C ABI declared in include/cacheir_b200.h) and of the libraries of the
 ragged families: libcacheir_b200_ragged.so, _hybrid.so, _recurrence.so, _experts.so, _talking.so and _delta.so (headers of the
-same names), and of libcacheir_b200_serving.so, the operators of batches that share prompts.
+same names), of libcacheir_b200_serving.so, the operators of batches that share prompts, and of libcacheir_b200_drafts.so, those of
+steps that verify drafted tokens.
 
 There is no fallback: if the shared library is missing the import of any
 compute entry point raises, telling the user to build it.
@@ -12,7 +13,8 @@ from ctypes import c_char_p, c_double, c_float, c_int, c_longlong, c_size_t, c_v
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libcacheir_b200.so"
-GROUP_PATHS = {name: LIB_PATH.with_name(f"libcacheir_b200_{name}.so") for name in ("ragged", "hybrid", "recurrence", "experts", "talking", "delta", "serving")}
+GROUP_PATHS = {name: LIB_PATH.with_name(f"libcacheir_b200_{name}.so") for name in ("ragged", "hybrid", "recurrence", "experts", "talking", "delta", "serving",
+                                                                           "drafts")}
 
 # name -> (restype, argtypes); mirrors include/cacheir_b200.h one to one
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -230,6 +232,51 @@ class PrefixArgs(ctypes.Structure):
                                            "dtype")] + [("softmax_scale", c_float)]
 
 
+class NormRotaryArgs(ctypes.Structure):
+    """cacheir_b200_norm_rotary_args"""
+
+    _fields_ = [("rotary", RotaryArgs), ("q_weight", c_void_p), ("k_weight", c_void_p), ("weight_dtype", c_int), ("eps", c_float), ("offset", c_float)]
+
+
+class TreeArgs(ctypes.Structure):
+    """cacheir_b200_tree_args"""
+
+    _fields_ = [(name, c_void_p) for name in ("q", "k_cache", "v_cache", "out", "page_table", "seq_lens", "cu_rows", "visible", "workspace")] + \
+               [("workspace_bytes", c_size_t), ("q_stride", c_longlong), ("out_stride", c_longlong)] + \
+               [(name, c_int) for name in ("rows", "sequences", "heads", "kv_heads", "dim", "page_size", "num_slots", "max_pages", "words", "dtype")] + \
+               [("softmax_scale", c_float)]
+
+
+class LogitsArgs(ctypes.Structure):
+    """cacheir_b200_logits_args"""
+
+    _fields_ = [(name, c_void_p) for name in ("logits", "out", "row_seq", "history", "history_lens", "prompt_lens", "draft_ids", "cu_rows", "visible",
+                                              "repetition", "frequency", "presence", "bias_ids", "bias_values", "allowed")] + \
+               [("row_stride", c_longlong), ("out_stride", c_longlong)] + \
+               [(name, c_int) for name in ("rows", "sequences", "vocab", "history_width", "words", "biases", "dtype", "out_dtype")]
+
+
+class DraftMapArgs(ctypes.Structure):
+    """cacheir_b200_draft_map_args"""
+
+    _fields_ = [(name, c_void_p) for name in ("parents", "cu_rows", "seq_lens", "positions", "visible", "status")] + \
+               [(name, c_int) for name in ("rows", "sequences", "words")]
+
+
+class AcceptArgs(ctypes.Structure):
+    """cacheir_b200_accept_args"""
+
+    _fields_ = [(name, c_void_p) for name in ("chosen", "draft_ids", "parents", "cu_rows", "seq_lens", "counts", "path", "next_ids", "keep_lens")] + \
+               [(name, c_int) for name in ("rows", "sequences", "depth")]
+
+
+class KeepArgs(ctypes.Structure):
+    """cacheir_b200_keep_args"""
+
+    _fields_ = [(name, c_void_p) for name in ("pools", "slots", "cu_rows", "counts", "path")] + \
+               [(name, c_int) for name in ("pool_count", "rows", "sequences", "depth", "num_slots", "kv_heads", "page_size", "dim", "dtype")]
+
+
 _NEXT = [c_int, c_void_p, c_void_p, c_float, c_void_p]      # next_mode next_w next_b next_alpha next_out
 # group -> signatures; each mirrors include/cacheir_b200_<group>.h one to one
 GROUP_SIGNATURES: dict[str, dict[str, tuple[object, list[object]]]] = {
@@ -331,6 +378,16 @@ GROUP_SIGNATURES: dict[str, dict[str, tuple[object, list[object]]]] = {
         "cacheir_b200_shared_prefix_attention": (c_int, [c_void_p, c_void_p]),
         "cacheir_b200_token_logprobs": (c_int, [c_void_p, c_void_p]),
         "cacheir_b200_serving_device_status": (c_int, [c_int]),
+    },
+    "drafts": {
+        "cacheir_b200_norm_rotary_append": (c_int, [c_void_p, c_void_p]),
+        "cacheir_b200_tree_attention_workspace_bytes": (c_size_t, [c_int] * 3),
+        "cacheir_b200_tree_attention": (c_int, [c_void_p, c_void_p]),
+        "cacheir_b200_adjust_logits": (c_int, [c_void_p, c_void_p]),
+        "cacheir_b200_map_drafts": (c_int, [c_void_p, c_void_p]),
+        "cacheir_b200_accept_drafts": (c_int, [c_void_p, c_void_p]),
+        "cacheir_b200_keep_accepted": (c_int, [c_void_p, c_void_p]),
+        "cacheir_b200_drafts_device_status": (c_int, [c_int]),
     },
 }
 # entry points of glue.cu and misc.cu, which the core and the ragged library carry

@@ -3,32 +3,19 @@
 //
 //   (a, b) -> factor * (a cos - b sin, a sin + b cos), angle = position * frequency
 //
-// The angle is found modulo one turn in 64-bit binary fractions: position * turns[i] in integers drops whole turns exactly, so that a
-// position of a million has an angle as good as position 1 (in 32-bit floats it would be off by 0.06 rad). The fraction's nearest quarter
-// turn is split off as an integer too; what is left lies in [-1/4, 1/4) half turns and keeps 2^-26 of a turn in a float.
-//
 // Bound by memory: every value is read and written once. One block per row; its cosines are worked out once for all heads. Where there are
 // many rows, small blocks: 16384 rows of 64 + 8 heads of 128 in fp16 take 116 us (5.8 TB/s; from a graph, in bursts: 126 on end, under the power
 // cap) with 64 threads a block, 119 with 128 and 134 with 192; few rows want more of a row under way (32 rows: 4.8, 3.5 and 3.1 us). Asking for the values before the cosines, cosines in
 // registers, and rows streamed through shared memory by bulk copies (201 us) were all slower.
 #include "cacheir_b200_serving.h"
 #include "common.cuh"
+#include "rotary_turn.cuh"
 
 namespace cb200 {
 namespace {
 
 constexpr int kMaxThreads = 256;
 constexpr int kMaxDim = 1024;
-
-__device__ __forceinline__ float2 turn_cos_sin(uint64_t turns, int position, float factor) {
-  const uint64_t f = turns * static_cast<uint64_t>(static_cast<long long>(position));
-  const uint64_t quarter = (f + (1ull << 61)) >> 62;
-  const long long rest = static_cast<long long>(f - (quarter << 62));
-  float s, c;
-  sincospif(static_cast<float>(rest) * 1.0842021724855044e-19f, &s, &c);       // 2^-63: rest in half turns
-  const float2 r = (quarter & 1) ? make_float2(-s, c) : make_float2(c, s);
-  return (quarter & 2) ? make_float2(-r.x * factor, -r.y * factor) : make_float2(r.x * factor, r.y * factor);
-}
 
 // A unit is VEC pairs (or 2 VEC values that are only copied): two vectors of VEC values.
 template <typename T, int VEC>

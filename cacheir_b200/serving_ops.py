@@ -44,8 +44,8 @@ def _ptr(t: torch.Tensor | None) -> int:
 
 # (As these launch kernels of a few microseconds, what they do on the host is kept to about as many: shapes and strides are taken once, the
 # current device is looked up and only switched where the tensors are on another one.)
-def _launch(what: str, tensors: tuple, args: bytes) -> None:
-    """Calls the entry point `what` with its struct and the current stream of the device that all the tensors are on."""
+def _launch(what: str, tensors: tuple, args: bytes, group: str = "serving") -> None:
+    """Calls the entry point `what` of a library group with its struct and the current stream of the device that all the tensors are on."""
     index = tensors[0].get_device()
     for t in tensors:
         if t is not None and t.get_device() != index:
@@ -55,7 +55,7 @@ def _launch(what: str, tensors: tuple, args: bytes) -> None:
         _require_cuda(*tensors)
     call = _calls.get(what)
     if call is None:
-        call = _calls[what] = getattr(_lib.load_group("serving"), "cacheir_b200_" + what)
+        call = _calls[what] = getattr(_lib.load_group(group), "cacheir_b200_" + what)
     if index == _current_device():
         code = call(args, _raw_stream(index))
     else:
@@ -202,16 +202,9 @@ def rotary_rule(rot: int, base: float, *, layout: str = "interleaved", scaling: 
     return RotaryRule(torch.from_numpy(turn_fractions(freq)).to(device), layout, factor)
 
 
-def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, rule: RotaryRule, positions: torch.Tensor, *,
-                  slots: torch.Tensor | None = None, k_cache: torch.Tensor | None = None, v_cache: torch.Tensor | None = None,
-                  q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> None:
-    """Turns the first rule.rot values of every head of q [R, H, D] and k [R, KVH, D] to positions int32 [R] (rows may be strided views of
-    a fused buffer), into q_out (default: in place) and k_out. With slots int32 [R] and the pools [slots, KVH, page, D] the turned k and v
-    [R, KVH, D] are also appended: row r to page slots[r] // page, offset slots[r] % page; rows whose slot is outside the pool (padding: -1)
-    are left out altogether. Rows with one slot: each value there is of one of them, any. Without slots, k_out defaults to in place; with
-    them, to nowhere but the pool.
-
-    Beside `ops.rope_append`: both pair layouts, part of a head, scaled frequencies, float32 to bfloat16, far positions exactly."""
+def _rotary_call(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, rule: RotaryRule, positions: torch.Tensor, slots: torch.Tensor | None,
+                 k_cache: torch.Tensor | None, v_cache: torch.Tensor | None, q_out: torch.Tensor | None, k_out: torch.Tensor | None) -> tuple[bytes, tuple]:
+    """The checked arguments of a rotary append as the C struct's bytes, and its tensors. No bytes: there are no rows."""
     rows, heads, dim, q_stride = _check_heads("q", q)
     k_rows, kv_heads, k_dim, k_stride = _check_heads("k", k)
     turns, layout = rule.turns, LAYOUTS.get(rule.layout)
@@ -259,13 +252,28 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, rule
     if k.dtype is not dtype or q_out.dtype is not dtype or (k_out is not None and k_out.dtype is not dtype):
         raise TypeError("q, k, v, the outputs and the pools must have one dtype")
     code = dtype_code(dtype)
+    tensors = (q, k, q_out, positions, turns, slots, v, k_out, k_cache, v_cache)
     if rows == 0:
-        return
-    args = ROTARY_BYTES.pack(
+        return b"", tensors
+    return ROTARY_BYTES.pack(
         q.data_ptr(), k.data_ptr(), _ptr(v), q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), positions.data_ptr(), _ptr(slots),
         turns.data_ptr(), q_stride, k_stride, v_stride, q_out_stride, k_out_stride, rows, heads, kv_heads, dim, rot, layout, num_slots, page_size,
-        code, rule.factor)
-    _launch("rotary_append", (q, k, q_out, positions, turns, slots, v, k_out, k_cache, v_cache), args)
+        code, rule.factor), tensors
+
+
+def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, rule: RotaryRule, positions: torch.Tensor, *,
+                  slots: torch.Tensor | None = None, k_cache: torch.Tensor | None = None, v_cache: torch.Tensor | None = None,
+                  q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> None:
+    """Turns the first rule.rot values of every head of q [R, H, D] and k [R, KVH, D] to positions int32 [R] (rows may be strided views of
+    a fused buffer), into q_out (default: in place) and k_out. With slots int32 [R] and the pools [slots, KVH, page, D] the turned k and v
+    [R, KVH, D] are also appended: row r to page slots[r] // page, offset slots[r] % page; rows whose slot is outside the pool (padding: -1)
+    are left out altogether. Rows with one slot: each value there is of one of them, any. Without slots, k_out defaults to in place; with
+    them, to nowhere but the pool.
+
+    Beside `ops.rope_append`: both pair layouts, part of a head, scaled frequencies, float32 to bfloat16, far positions exactly."""
+    args, tensors = _rotary_call(q, k, v, rule, positions, slots, k_cache, v_cache, q_out, k_out)
+    if args:
+        _launch("rotary_append", tensors, args)
 
 
 # ---- attention over common prefixes ----------------------------------------------------------------------------------
