@@ -37,7 +37,7 @@ GROUP_FILES = {
     "talking": ("talking_attention", "talking_prompt"),
     "delta": ("short_conv", "delta_rule"),
     "serving": ("page_tables", "rotary_append", "shared_prefix", "shared_prefix_mma", "token_logprobs"),
-    "drafts": ("norm_rotary", "tree_attention", "adjust_logits", "draft_rows"),
+    "drafts": ("norm_rotary", "tree_attention", "tree_attention_mma", "adjust_logits", "draft_rows"),
     "experts": ("tied_attention", "tied_prompt", "grouped_gemm", "expert_routing"),
 }
 LIB_PATHS = {"core": LIB_DIR / "libcacheir_b200.so", **{name: LIB_DIR / f"libcacheir_b200_{name}.so" for name in GROUP_FILES}}

@@ -184,7 +184,8 @@ using namespace cb200;
 
 extern "C" size_t cacheir_b200_tree_attention_workspace_bytes(int rows, int heads, int dim) {
   if (rows <= 0 || heads <= 0 || dim <= 0) return 0;
-  return static_cast<size_t>(tree_pieces(rows, heads, dim)) * rows * heads * (dim + 2) * 4;
+  const size_t general = static_cast<size_t>(tree_pieces(rows, heads, dim)) * rows * heads * (dim + 2) * 4, fast = tree_fast_bytes(dim);
+  return general > fast ? general : fast;
 }
 
 extern "C" int cacheir_b200_tree_attention(const cacheir_b200_tree_args* args, void* stream) {
@@ -201,9 +202,11 @@ extern "C" int cacheir_b200_tree_attention(const cacheir_b200_tree_args* args, v
   if (!a.workspace || a.workspace_bytes < cacheir_b200_tree_attention_workspace_bytes(a.rows, a.heads, a.dim)) return CACHEIR_B200_EWORKSPACE;
   if (!aligned_to(a.workspace, 16)) return CACHEIR_B200_EALIGN;
   if (!(a.softmax_scale > 0.f)) a.softmax_scale = 1.0f / sqrtf(static_cast<float>(a.dim));
+  if (a.rows == 1) a.q_stride = a.out_stride = static_cast<long long>(a.heads) * a.dim;
+  if (tree_fast_supported(a)) return launch_tree_fast(a, as_stream(stream));
   if (a.dtype == CACHEIR_B200_F32) return launch_general<float>(a, as_stream(stream));
   if (a.dtype == CACHEIR_B200_F16) return launch_general<__half>(a, as_stream(stream));
   return launch_general<__nv_bfloat16>(a, as_stream(stream));
 }
 
-extern "C" int cacheir_b200_drafts_device_status(int) { return 0; }
+extern "C" int cacheir_b200_drafts_device_status(int reset) { return tree_device_status(reset != 0); }

@@ -38,4 +38,10 @@ inline int tree_pieces(int rows, int heads, int dim) {
   return n < 1 ? 1 : n > kMaxTreePieces ? kMaxTreePieces : static_cast<int>(n);
 }
 
+// Tensor-core kernels (tree_attention_mma.cu): 16-bit types, head sizes 64 and 128, pages of a multiple of 16 tokens.
+size_t tree_fast_bytes(int dim);
+bool tree_fast_supported(const cacheir_b200_tree_args& a);
+int launch_tree_fast(const cacheir_b200_tree_args& a, cudaStream_t stream);
+int tree_device_status(bool reset);
+
 }  // namespace cb200

@@ -1,0 +1,828 @@
+// Attention of drafted tokens over their sequence's pages on the tensor cores: 16-bit types, head sizes 64 and 128, pages of a multiple of 16
+// tokens, up to 64 query heads per key/value head.
+//
+// S = Q K^T and O = P V as tcgen05 MMAs of 128 query rows, which are the (token, head) pairs of a sequence that share a key/value head; scores,
+// probabilities and outputs in tensor memory. An item is (sequence, up to 256 query rows, key/value head); its keys come in tiles of 128, from
+// the sequence's first token to the last that one of its rows can see, so that a sequence's keys are read once for all rows of an item. The key tiles of all items, in a row, are cut
+// evenly over the blocks, whatever the lengths. An item that one block has alone is written as it ends; of others every block leaves a piece, and a second kernel joins them.
+//
+// One warp brings keys and one values (TMA, 16 tokens at a time, into a ring of slots), one issues the MMAs, and two groups of four warps do the
+// softmax, a thread per query row, each with scores, probabilities and an output of its own in tensor memory. Above 128 query rows each group
+// has its own 128 of them and both use the same keys. With fewer, which is what decoding with drafts has mostly, both have the same
+// rows and take turns with the key tiles: what bounds such an item is the memory's rate, and one group alone would not keep up with it. The two halves are added up
+// from tensor memory at the item's end.
+//
+// Masks are looked at only in tiles that hold drafted tokens: 128 bits a row, shifted to the tile. Whatever stands in a key that a row does not
+// see, its weight is 0; but 0 times a value that is no number is none. So one more warp looks through the drafted tokens' values before the second product has them, puts
+// zeros for infinities and NaN, and says that it did; rows that see such a value get it added at the end, by themselves.
+//
+// A row's maximum is a reference that moves only when it is exceeded by 2^14, so that outputs are hardly ever rescaled; probabilities are rounded to
+// the element type as the second MMA's operand, their sums are not.
+#include "attention_ptx.cuh"
+#include "hybrid_common.cuh"
+#include "tree_attention.cuh"
+
+namespace cb200 {
+namespace {
+
+using namespace ptx;
+
+constexpr int kKeys = 128;                     // keys of a tile
+constexpr int kFirst = 96;                     // .. whose probabilities go to the second MMA first: less of it is left when the others come
+constexpr int kRows = 128;                     // query rows of a group of warps
+constexpr int kThreads = 384;
+constexpr int kMaxHeadsPerKv = 64;
+constexpr int kPlanThreads = 128;              // that lay the plan out, some sequences each
+constexpr int kJoinRows = 16;                  // query rows of a joining block
+constexpr float kAhead = 6.f;                  // a new reference is the maximum less this: probabilities start at 2^6 ..
+constexpr float kStale = 14.f;                 // .. and may grow to 2^14 (in fp16: 2^-24 of that is still a number)
+
+__device__ int g_tree_status = 0;
+
+// What a block that ends an item which others began leaves for the kernel that joins (rows 0: nothing).
+struct TreeJoin {
+  int row, rows, kvh, first;                   // first row and number of rows; the blocks from `first` to this one have a piece each
+};
+struct FastParams {
+  cacheir_b200_tree_args a;
+  TreeJoin* joins;                             // [blocks]
+  float* ml;                                   // [blocks][2][256][2]: maxima (log2 domain) and denominators of the blocks' pieces
+  float* acc;                                  // [blocks][2][256][dim]: unnormalised outputs
+  int half_rows;                               // tokens of a group of warps
+  float scale_log2;
+};
+
+// A warp's wait; false in all lanes where it gave up in one.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, &g_tree_status, code));
+}
+// n / d for a d that mostly is a power of two (pages).
+struct Division {
+  int d, shift;
+  __device__ __forceinline__ explicit Division(int n) {
+    d = n;
+    shift = (n & (n - 1)) == 0 ? 31 - __clz(n) : -1;
+  }
+  __device__ __forceinline__ int of(int n) const { return shift >= 0 ? n >> shift : n / d; }
+};
+
+// ---- how the work is cut ----
+// An item of n key tiles is kItemUnits + n units: what it costs to begin with (queries, the first tile's latency, the output) is about
+// that of so many tiles. The units are dealt out as evenly as whole numbers can be.
+constexpr int kItemUnits = 2;
+
+struct Deal {
+  int share, more;             // every block has `share` units, the first `more` one more
+  __device__ __forceinline__ Deal(int units, int ctas) : share(units / ctas), more(units % ctas) {}
+  __device__ __forceinline__ int begin(int block) const { return block * share + min(block, more); }
+  __device__ __forceinline__ int owner(int unit) const {
+    const int big = more * (share + 1);
+    return unit < big ? unit / (share + 1) : more + (unit - big) / share;
+  }
+};
+// Keys that rows below `end` of a sequence can see (with a mask any of its tokens), and the units of such an item.
+__device__ __forceinline__ int item_keys(const cacheir_b200_tree_args& a, const TreeSequence& s, int end) {
+  return a.visible ? s.keys : max(min(s.keys, s.front + min(end, s.rows)), 0);
+}
+__device__ __forceinline__ int item_units(int keys) { return kItemUnits + max((keys + kKeys - 1) / kKeys, 1); }
+// Of a sequence, for one key/value head after the other in every tile of rows.
+__device__ __forceinline__ int sequence_units(const cacheir_b200_tree_args& a, const TreeSequence& s, int tile_rows) {
+  const int tiles = (s.rows + tile_rows - 1) / tile_rows;
+  if (a.visible) return a.kv_heads * tiles * item_units(s.keys);
+  int units = 0;
+  for (int j = 1; j <= tiles; ++j) units += item_units(item_keys(a, s, j * tile_rows));
+  return a.kv_heads * units;
+}
+
+// A block's share of the units, item by item.
+struct Walk {
+  const cacheir_b200_tree_args& a;
+  Deal deal;
+  int at, end, tile_rows;
+  int b, start;                // the sequence, and the first unit of its row tile
+  TreeSequence s;
+  int row_tile, units;         // .. the row tile, and the units of an item in it
+  // the item
+  int kvh, row0, rows, tile, tiles, keys, first;     // rows from row0 of the sequence on; key tiles tile .. tile + tiles - 1 of it are this block's;
+  bool begins, ends;                                 // block `first` has its first one
+
+  // starts: the first units of runs of `run` sequences
+  __device__ __forceinline__ Walk(const cacheir_b200_tree_args& args, int rows_of_item, const int* starts, int run, int total, int ctas)
+      : a(args), deal(total, ctas), tile_rows(rows_of_item) {
+    at = deal.begin(blockIdx.x);
+    end = deal.begin(blockIdx.x + 1);
+    int lo = 0, hi = kPlanThreads;                             // last run that starts at or before `at` (empty ones start where the next does)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (starts[mid] <= at) lo = mid; else hi = mid;
+    }
+    b = lo * run;
+    start = starts[lo];
+    s = tree_sequence(a, min(b, a.sequences - 1));
+    row_tile = 0;
+    units = item_units(item_keys(a, s, tile_rows));
+  }
+  __device__ __forceinline__ bool next() {
+    while (at < end) {
+      // the row tile that `at` is in
+      while (row_tile * tile_rows >= s.rows || start + a.kv_heads * units <= at) {
+        if (row_tile * tile_rows < s.rows) {
+          start += a.kv_heads * units;
+          ++row_tile;
+        }
+        if (row_tile * tile_rows >= s.rows) {
+          if (++b >= a.sequences) return false;
+          s = tree_sequence(a, b);
+          row_tile = 0;
+        }
+        units = item_units(item_keys(a, s, (row_tile + 1) * tile_rows));
+      }
+      kvh = (at - start) / units;
+      const int item0 = start + kvh * units, tile0 = item0 + kItemUnits, stop = min(end, item0 + units);
+      tile = max(at - tile0, 0);
+      tiles = stop - tile0 - tile;
+      begins = at <= tile0;
+      ends = stop == item0 + units;
+      at = stop;
+      if (tiles <= 0) continue;                                // (no more than an item's beginning: the next block has its tiles)
+      first = begins ? static_cast<int>(blockIdx.x) : deal.owner(tile0);
+      row0 = row_tile * tile_rows;
+      rows = min(tile_rows, s.rows - row0);
+      keys = item_keys(a, s, row0 + rows);
+      return true;
+    }
+    return false;
+  }
+};
+
+template <int D>
+struct Smem {
+  static constexpr int kSlotBytes = kKeys * D * 2;
+  static constexpr int kSlots = D == 128 ? 5 : 10;
+  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kTiles = 2 * kQBytes + kSlots * kSlotBytes;
+  // then: barriers of keys, of values, empty, clean [slots], q[2], place of q[2], s[2], p[2][2], o[2], end[3]; tensor memory address; starts of runs
+  static constexpr int kBarriers = 4 * kSlots + 15;
+  static constexpr int kBytes = 1024 + kTiles + kBarriers * 8 + 16 + (kPlanThreads + 1) * 4;
+};
+constexpr int kSpoilt = 8;                     // items that a flag of spoilt values may be set ahead
+
+// Where a column of a lane's line of 32 lies in shared memory: lanes that read the same one reach different banks.
+__device__ __forceinline__ int staged(int lane, int column) { return lane * 32 + (((column >> 2) ^ (lane & 7)) << 2) + (column & 3); }
+// What row `row` of the item gets of values that are no numbers, of the tokens that it sees in the tiles from `tile` on, added to columns c .. end - 1
+// of its place `to`, which this warp has written.
+template <typename T, int D, typename O>
+__device__ __noinline__ void add_spoilt(const cacheir_b200_tree_args& a, const TreeSequence s, const int32_t* pages, int row, int head, int tile, int tiles, int keys, int c,
+                                        int end, O* to) {
+  const int kvh = head / (a.heads / a.kv_heads);
+  const T* q = static_cast<const T*>(a.q) + static_cast<size_t>(s.row + row) * a.q_stride + static_cast<size_t>(head) * D;
+  for (int t = max(tile * kKeys, max(s.front, 0)); t < min((tile + tiles) * kKeys, keys); ++t) {
+    const int j = t - s.front;
+    if (!(tree_word(a, s, row, j >> 5) >> (j & 31) & 1)) continue;
+    const int id = pages[t / a.page_size];
+    if (id < 0 || id >= a.num_slots) continue;
+    const size_t at = ((static_cast<size_t>(id) * a.kv_heads + kvh) * a.page_size + t % a.page_size) * D;
+    const T* v = static_cast<const T*>(a.v_cache) + at;
+    bool any = false;
+    for (int i = c; i < end; ++i) any = any || !isfinite(Elem<T>::ld(v + i));
+    if (!any) continue;
+    const T* k = static_cast<const T*>(a.k_cache) + at;
+    float score = 0.f;
+    for (int d = 0; d < D; ++d) score = fmaf(Elem<T>::ld(q + d), Elem<T>::ld(k + d), score);
+    if (score == -INFINITY) continue;                          // (no weight)
+    for (int i = c; i < end; ++i) {
+      const float x = Elem<T>::ld(v + i);
+      if (!isfinite(x)) Elem<O>::st(to + i, Elem<O>::ld(to + i) + x);
+    }
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_q,
+            const __grid_constant__ FastParams p) {
+  using L = Smem<D>;
+  constexpr int kSlots = L::kSlots;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* s_q = smem;                                         // [2][D / 64][128 rows][128 B]
+  uint8_t* s_kv = smem + 2 * L::kQBytes;                       // [slots][D / 64][128 keys][128 B]
+  // Keys and values take the slots in turn: those of the block's tile u are in slots 2 u and 2 u + 1 modulo their number. Their barriers go by u, so that
+  // whoever looks at one kind only never meets a phase of the other.
+  uint64_t* key_full = reinterpret_cast<uint64_t*>(smem + L::kTiles);
+  uint64_t* value_full = key_full + kSlots;
+  uint64_t* empty = value_full + kSlots;                       // (by slot)
+  uint64_t* bar_clean = empty + kSlots;                        // values have been looked through
+  uint64_t* bar_q = bar_clean + kSlots;                        // queries of a group of warps are there
+  uint64_t* bar_free = bar_q + 2;                              // .. and their place is free again
+  uint64_t* bar_s = bar_free + 2;                              // scores are in tensor memory
+  uint64_t* bar_p = bar_s + 2;                                 // probabilities are, [group of warps][first keys, the others]
+  uint64_t* bar_o = bar_p + 4;                                 // .. and have been added to the output
+  uint64_t* bar_end = bar_o + 2;                               // steps of an item's end that both groups of warps have made
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_end + 3);
+  int* s_start = reinterpret_cast<int*>(tmem_slot + 4);
+  __shared__ int s_scan[kPlanThreads / 32];
+  __shared__ volatile int s_spoilt[kSpoilt];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const cacheir_b200_tree_args& a = p.a;
+
+  if (threadIdx.x == 288) {
+    prefetch_map(&tmap_q);
+    prefetch_map(&tmap_k);
+    prefetch_map(&tmap_v);
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(smem_u32(&key_full[s]), 1);
+      mbar_init(smem_u32(&value_full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+      mbar_init(smem_u32(&bar_clean[s]), 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(smem_u32(&bar_q[w]), 1);
+      mbar_init(smem_u32(&bar_free[w]), 8);
+      mbar_init(smem_u32(&bar_s[w]), 1);
+      mbar_init(smem_u32(&bar_p[2 * w]), kRows);
+      mbar_init(smem_u32(&bar_p[2 * w + 1]), kRows);
+      mbar_init(smem_u32(&bar_o[w]), 1);
+    }
+    for (int i = 0; i < 3; ++i) mbar_init(smem_u32(&bar_end[i]), 8);
+    mbar_fence_init();
+  }
+  if (threadIdx.x >= 256 && threadIdx.x < 256 + kSpoilt) s_spoilt[threadIdx.x - 256] = 0;
+  chain_enter();
+  if (warp == 8) tc_alloc(smem_u32(tmem_slot), 512);           // (beside the loads of the plan)
+  // ---- the plan: units of runs of sequences, a thread each ----
+  const int tile_rows = 2 * p.half_rows, run = (a.sequences + kPlanThreads - 1) / kPlanThreads;
+  int sum = 0, own = 0;
+  if (threadIdx.x < kPlanThreads) {
+    for (int b = threadIdx.x * run; b < min(static_cast<int>(threadIdx.x + 1) * run, a.sequences); ++b) own += sequence_units(a, tree_sequence(a, b), tile_rows);
+    sum = own;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= off) sum += up;
+    }
+    if (lane == 31) s_scan[warp] = sum;
+  }
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int i = 0; i < kPlanThreads / 32; ++i) {
+    if (i < warp) sum += s_scan[i];
+    total += s_scan[i];
+  }
+  if (threadIdx.x < kPlanThreads) s_start[threadIdx.x] = sum - own;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;                            // scores [2][128 columns] (probabilities over them), outputs [2][D]
+  const uint32_t tmem_o = tmem + 2 * kKeys;
+  const int group = a.heads / a.kv_heads, half_rows = p.half_rows;
+  const int ctas = max(1, min(total, static_cast<int>(gridDim.x)));
+  const bool takes_part = static_cast<int>(blockIdx.x) < min(ctas, total);
+  Walk walk(a, tile_rows, s_start, run, max(total, 1), ctas);
+  if (!takes_part) walk.end = walk.at;
+  bool ok = true;
+
+  if (warp == 11) {
+    // ------- values: those of drafted tokens are looked through, those behind the last key cleared -------
+    constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+    constexpr int kLanes = D / 8;                              // of a key's values
+    int slot = 1, item = 0, turn = 0;
+    uint32_t phase = 0;
+    while (ok && walk.next()) {
+      ++item;
+      for (int t = walk.tile; t < walk.tile + walk.tiles && ok; ++t) {
+        ok = warp_wait(smem_u32(&value_full[turn]), phase, (15 << 8) | 12);
+        if (!ok) break;
+        const int base = t * kKeys, from = max(min(walk.s.front, walk.keys) - base, 0);
+        if (from < kKeys) {
+          bool spoilt = false;
+          for (int key = from + lane / kLanes; key < kKeys; key += 32 / kLanes) {
+            const int c = lane % kLanes;
+            uint4* at = reinterpret_cast<uint4*>(s_kv + slot * L::kSlotBytes + (key / kChunk) * kChunk * D * 2 + (c >> 3) * kChunk * 128 + key % kChunk * 128 +
+                                                 ((c & 7) << 4));
+            if (base + key >= walk.keys) {
+              *at = make_uint4(0u, 0u, 0u, 0u);
+              continue;
+            }
+            uint4 v = *at;
+            const uint32_t bad[4] = {__vcmpeq2(v.x & kExponent, kExponent), __vcmpeq2(v.y & kExponent, kExponent), __vcmpeq2(v.z & kExponent, kExponent),
+                                     __vcmpeq2(v.w & kExponent, kExponent)};
+            if (bad[0] | bad[1] | bad[2] | bad[3]) {
+              spoilt = true;
+              *at = make_uint4(v.x & ~bad[0], v.y & ~bad[1], v.z & ~bad[2], v.w & ~bad[3]);
+            }
+          }
+          if (__any_sync(0xffffffffu, spoilt) && lane == 0) s_spoilt[item % kSpoilt] = item;
+          fence_async_smem();
+          __threadfence_block();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_clean[turn]));
+        slot += 2;
+        if (slot >= kSlots) slot -= kSlots;
+        if (++turn == kSlots) { turn = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp >= 9) {
+    // ------- copies: warp 9 keys, a lane per 16 of them and 64 columns; warp 10 values, a lane per 16 of them -------
+    const bool keys = warp == 9;
+    const int boxes = keys ? D / 64 : 1, chunk = lane / boxes, box = lane % boxes;
+    const bool copies = chunk < kKeys / kChunk;
+    const int outside = a.num_slots * a.kv_heads * a.page_size;         // rows behind the pool read as zeros
+    const uint32_t dst = smem_u32(s_kv) + (keys ? box * kKeys * 128 + chunk * kChunk * 128 : chunk * kChunk * D * 2);
+    const Division by_page(a.page_size);
+    uint64_t* full = keys ? key_full : value_full;
+    int slot = keys ? 0 : 1, turn = 0, q_place = 0;
+    uint32_t phase = 1, sent = 0, q_phase = 3;                 // (slots of a tile: its keys', its values'; q_phase: a bit for either place)
+    while (ok && walk.next()) {
+      const int32_t* pages = a.page_table + static_cast<size_t>(walk.b) * a.max_pages;
+      auto line_of = [&](int tile) {                           // first row of this lane's 16 in the pool
+        const int key = tile * kKeys + chunk * kChunk;
+        if (!copies || key >= walk.keys) return outside;
+        const int page = by_page.of(key), id = pages[page];
+        return id >= 0 && id < a.num_slots ? (id * a.kv_heads + walk.kvh) * a.page_size + key - page * a.page_size : outside;
+      };
+      int line = line_of(walk.tile);
+      if (!keys) {                                             // the item's queries: rows, heads, 64 columns at a time
+        const bool two = walk.rows > half_rows;
+        for (int w = 0; w < (two ? 2 : 1) && ok; ++w) {
+          const int place = two ? w : q_place;
+          ok = warp_wait(smem_u32(&bar_free[place]), q_phase >> place & 1, (15 << 8) | 7);
+          if (!ok) break;
+          q_phase ^= 1u << place;
+          if (lane == 0) {
+            mbar_expect_tx(smem_u32(&bar_q[place]), (D / 64) * half_rows * group * 128);
+            for (int z = 0; z < D / 64; ++z)
+              tma_load_4d(smem_u32(s_q + place * L::kQBytes + z * kRows * 128), &tmap_q, smem_u32(&bar_q[place]), 0, walk.kvh * group,
+                          walk.s.row + walk.row0 + w * half_rows, z);
+          }
+          __syncwarp();
+        }
+        if (!two) q_place ^= 1;
+      }
+      for (int t = walk.tile; t < walk.tile + walk.tiles && ok; ++t) {
+        const int next = t + 1 < walk.tile + walk.tiles ? line_of(t + 1) : 0;
+        ok = warp_wait(smem_u32(&empty[slot]), phase, (15 << 8) | 1);
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(smem_u32(&full[turn]), L::kSlotBytes);
+        __syncwarp();
+        if (copies) {
+          if (keys) tma_load_3d(dst + slot * L::kSlotBytes, &tmap_k, smem_u32(&full[turn]), 0, line, box);
+          else tma_load_3d(dst + slot * L::kSlotBytes, &tmap_v, smem_u32(&full[turn]), 0, line, 0);
+        }
+        ++sent;
+        slot += 2;
+        if (slot >= kSlots) { slot -= kSlots; phase ^= 1; }
+        turn = turn + 1 == kSlots ? 0 : turn + 1;
+        line = next;
+      }
+    }
+    // nothing may still be on its way when the block ends, also after a wait that gave up
+    for (uint32_t i = sent > kSlots ? sent - kSlots : 0; i < sent; ++i)
+      mbar_wait(smem_u32(&full[i % kSlots]), (i / kSlots) & 1, &g_tree_status, (15 << 8) | 2);
+    // (queries are waited for by the products; after a wait that gave up: both phases of both places)
+    if (!keys && !ok)
+      for (int w = 0; w < 4; ++w) mbar_wait(smem_u32(&bar_q[w >> 1]), w & 1, &g_tree_status, (15 << 8) | 2);
+  } else if (warp == 8) {
+    // ---------------- MMA issue ----------------
+    constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
+    const uint32_t id_s = (1u << 4) | (kType << 7) | (kType << 10) | (static_cast<uint32_t>(kKeys >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
+    const uint32_t id_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) |
+                          (static_cast<uint32_t>(kRows >> 4) << 24);
+    const uint64_t dq = smem_desc_sw128(smem_u32(s_q)), dk = smem_desc_sw128(smem_u32(s_kv)), dv = smem_desc_columns(smem_u32(s_kv));
+    // An item's steps: a tile each, or a tile for either group of warps; step j belongs to group j & 1. Scores are two steps ahead of outputs, and
+    // are issued right behind the output that frees their buffer.
+    const bool leader = elect_one();
+    int k_slot = 0, v_slot = 1, k_turn = 0, v_turn = 0, q_place = 0;    // slots; barriers; place of the queries of an item that both groups share
+    uint32_t k_phase = 0, v_phase = 0, q_phase = 0, p_phase = 0;    // (of the two buffers of queries and probabilities: a bit each)
+    while (ok && walk.next()) {
+      const bool two = walk.rows > half_rows;
+      const int steps = two ? 2 * walk.tiles : walk.tiles;
+      auto wait_scores = [&](int j) {                          // the operands of step j's scores
+        if (j < (two ? 2 : 1)) {                               // the item's queries are new
+          const int w = two ? j : q_place;
+          if (!warp_wait(smem_u32(&bar_q[w]), q_phase >> w & 1, (15 << 8) | 3)) return false;
+          q_phase ^= 1u << w;
+        }
+        return (two && (j & 1)) || warp_wait(smem_u32(&key_full[k_turn]), k_phase, (15 << 8) | 4);
+      };
+      auto score = [&](int j) {                                // (one lane)
+        const uint64_t q_at = dq + ((two ? j & 1 : q_place) * L::kQBytes >> 4), k_at = dk + (k_slot * L::kSlotBytes >> 4);
+        const uint32_t to = tmem + (j & 1) * kKeys;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          constexpr int kHalf = kRows * 128 >> 4;              // 64 columns further
+          mma_ss(to, q_at + (k >> 2) * kHalf + (k & 3) * 2, k_at + (k >> 2) * kHalf + (k & 3) * 2, id_s, k > 0 ? 1u : 0u);
+        }
+        tc_commit(smem_u32(&bar_s[j & 1]));
+        if (!two || (j & 1)) tc_commit(smem_u32(&empty[k_slot]));
+      };
+      auto scored = [&](int j) {                               // (the whole warp)
+        if (!two || (j & 1)) {
+          k_slot += 2;
+          if (k_slot >= kSlots) k_slot -= kSlots;
+          if (++k_turn == kSlots) { k_turn = 0; k_phase ^= 1; }
+        }
+      };
+      for (int j = 0; j < 2 && j < steps && ok; ++j) {
+        ok = wait_scores(j);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) score(j);
+        __syncwarp();
+        scored(j);
+      }
+      for (int j = 0; j < steps && ok; ++j) {
+        const int w = j & 1;
+        if (!(two && w)) ok = warp_wait(smem_u32(&bar_clean[v_turn]), v_phase, (15 << 8) | 5);
+        ok = ok && warp_wait(smem_u32(&bar_p[2 * w]), p_phase >> w & 1, (15 << 8) | 6);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t v_at = dv + (v_slot * L::kSlotBytes >> 4);
+        const uint32_t to = tmem_o + w * D, from = tmem + w * kKeys, add = j < 2 ? 0u : 1u;
+        const bool frees = !two || w, more = j + 2 < steps;
+        if (leader) {                                          // (the first keys while the others' probabilities are worked out)
+#pragma unroll
+          for (int k = 0; k < kFirst / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, k == 0 ? add : 1u);
+        }
+        __syncwarp();
+        if (more) ok = wait_scores(j + 2);
+        ok = ok && warp_wait(smem_u32(&bar_p[2 * w + 1]), p_phase >> w & 1, (15 << 8) | 6);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int k = kFirst / 16; k < kKeys / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, 1u);
+          tc_commit(smem_u32(&bar_o[w]));
+          if (frees) tc_commit(smem_u32(&empty[v_slot]));
+          if (more) score(j + 2);
+        }
+        __syncwarp();
+        p_phase ^= 1u << w;
+        if (frees) {
+          v_slot += 2;
+          if (v_slot >= kSlots) v_slot -= kSlots;
+          if (++v_turn == kSlots) { v_turn = 0; v_phase ^= 1; }
+        }
+        if (more) scored(j + 2);
+      }
+      if (!two) q_place ^= 1;
+    }
+  } else {
+    // ---------------- softmax: a thread per query row ----------------
+    const int w = warp >> 2, r = threadIdx.x & (kRows - 1);
+    const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int by_group = (65536 + group - 1) / group;          // n / group = n * by_group >> 16 for n < 256, group <= 64
+    const int token = r * by_group >> 16, head_of = r - token * group;
+    uint32_t s_phase = 0, o_phase = 0, end_phase = 0;
+    int q_place = 0, item = 0;                                 // where the queries of an item that both groups share are
+    TreeJoin join{};
+    while (ok && walk.next()) {
+      ++item;
+      const bool two = walk.rows > half_rows;
+      const int place = two ? w : q_place;
+      if (!two) q_place ^= 1;
+      const int in_item = (two ? w * half_rows : 0) + token;   // this thread's token of the item
+      const bool real = r < half_rows * group && in_item < walk.rows;
+      const int row = walk.row0 + (real ? in_item : 0), head = walk.kvh * group + head_of;
+      const int masked_from = min(walk.s.front, walk.keys);    // keys behind this need a look at the row's mask
+      float m_ref = -INFINITY, l_run = 0.f;
+      int steps = 0;
+      for (int t = two ? 0 : w; t < walk.tiles && ok; t += two ? 1 : 2, ++steps) {
+        const int base = (walk.tile + t) * kKeys;
+        const bool whole = base + kKeys <= masked_from;
+        uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        if (!whole) {                                          // 128 bits of the row, from the tile's first key on
+          const int from = base - walk.s.front, sh = from & 31;
+          uint32_t low = tree_word(a, walk.s, row, from >> 5);
+          if (from >> 5 < 0) low = 0xffffffffu;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int q = (from >> 5) + i + 1;
+            const uint32_t high = q < 0 ? 0xffffffffu : tree_word(a, walk.s, row, q);
+            const int left = walk.keys - base - 32 * i;        // keys there are from this word on
+            see[i] = __funnelshift_r(low, high, sh) & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
+            low = high;
+          }
+        }
+        ok = warp_wait(smem_u32(&bar_s[w]), s_phase, (15 << 8) | 8);
+        if (!ok) break;
+        s_phase ^= 1;
+        tc_fence_after();
+        const uint32_t scores = tmem + w * kKeys + lane_addr;
+        // The row's 128 scores are looked at twice. For the maximum the second half comes first: the first half then stays in registers,
+        // and its probabilities may be written over scores 0 .. 31 while the second half is still where it was.
+        uint32_t x[32], y[32];
+        auto masked = [&](uint32_t (&v)[32], uint32_t bits) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(bits >> i & 1)) v[i] = 0xff800000u;          // -inf
+        };
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto largest = [&](const uint32_t (&v)[32]) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            asm("max.f32 %0, %1, %2, %0;" : "+f"(mx[(i >> 1) & 3]) : "f"(__uint_as_float(v[i])), "f"(__uint_as_float(v[i + 1])));
+        };
+        tmem_ld_x32(scores + 64, x);
+        tmem_ld_x32(scores + 96, y);
+        tmem_wait_ld(x);
+        tmem_wait_ld(y);
+        if (!whole) { masked(x, see[2]); masked(y, see[3]); }
+        largest(x);
+        largest(y);
+        tmem_ld_x32(scores, x);
+        tmem_ld_x32(scores + 32, y);
+        tmem_wait_ld(x);
+        tmem_wait_ld(y);
+        if (!whole) { masked(x, see[0]); masked(y, see[1]); }
+        largest(x);
+        largest(y);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        const bool grown = real && top > m_ref + kStale;
+        if (__any_sync(0xffffffffu, grown)) {
+          const float fresh = grown ? top - kAhead : m_ref, alpha = grown ? ex2(m_ref - fresh) : 1.f;
+          m_ref = fresh;
+          l_run *= alpha;
+          if (steps > 0) {                                     // bring the output to the new reference (its last part came before these scores)
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tc_ld_x16(tmem_o + w * D + lane_addr + c, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_x16(tmem_o + w * D + lane_addr + c, o);
+            }
+          }
+        }
+        const float less = m_ref > -INFINITY ? -m_ref : 0.f;
+        f32x2 sum2[2] = {0ull, 0ull};
+        const f32x2 scale2 = pair(p.scale_log2, p.scale_log2), less2 = pair(less, less);
+        auto weigh = [&](const uint32_t (&v)[32], uint32_t* out) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float a0, a1;
+            unpair(fma2(pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), scale2, less2), a0, a1);
+            a0 = ex2(a0);
+            a1 = ex2(a1);
+            sum2[(i >> 1) & 1] = add2(sum2[(i >> 1) & 1], pair(a0, a1));
+            out[i >> 1] = pack_pair<T>(a0, a1);
+          }
+        };
+        {
+          uint32_t out[32];
+          weigh(x, out);
+          tmem_ld_x32(scores + 64, x);                         // (on its way meanwhile)
+          weigh(y, out + 16);
+          tmem_wait_ld(x);
+          tmem_ld_x32(scores + 96, y);
+          tmem_st_x32(scores, out);
+          if (!whole) masked(x, see[2]);
+          uint32_t rest[16];
+          weigh(x, rest);
+          tmem_wait_ld(y);
+          tmem_st_x16(scores + 32, rest);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(smem_u32(&bar_p[2 * w]));
+          if (!whole) masked(y, see[3]);
+          weigh(y, rest);
+          tmem_st_x16(scores + 48, rest);
+        }
+        float s0, s1, s2, s3;
+        unpair(sum2[0], s0, s1);
+        unpair(sum2[1], s2, s3);
+        l_run += (s0 + s1) + (s2 + s3);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&bar_p[2 * w + 1]));
+      }
+      if (!ok) break;
+      // ---- the item's end ----
+      if (steps > 0) {                                         // (the phase of this group's last output; those before it have not been waited for)
+        o_phase ^= (steps - 1) & 1;
+        ok = warp_wait(smem_u32(&bar_o[w]), o_phase, (15 << 8) | 11);
+        if (!ok) break;
+        o_phase ^= 1;
+      }
+      tc_fence_after();
+      auto together = [&](int i) {                             // both groups of warps have come here
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_end[i]));
+        const bool came = warp_wait(smem_u32(&bar_end[i]), end_phase, (15 << 8) | 13);
+        tc_fence_after();
+        return came;
+      };
+      uint8_t* s_place = s_q + place * L::kQBytes;             // (all scores of the item have been worked out)
+      float f_own = 1.f, f_other = 0.f;
+      if (!two) {
+        float2* s_ml = reinterpret_cast<float2*>(s_place);     // [2][128]
+        // (an item of one tile is the first group's alone, whose queries the second one must not write over)
+        if (steps > 0) s_ml[w * kRows + r] = make_float2(m_ref, l_run);
+        ok = together(0);
+        if (!ok) break;
+        const float2 other = w == 1 || walk.tiles > 1 ? s_ml[(w ^ 1) * kRows + r] : make_float2(-INFINITY, 0.f);
+        ok = together(1);
+        if (!ok) break;
+        const float m = fmaxf(m_ref, other.x);
+        f_own = m_ref > -INFINITY ? ex2(m_ref - m) : 0.f;
+        f_other = other.x > -INFINITY ? ex2(other.x - m) : 0.f;
+        // (a group whose keys all scored -inf has a sum of 0, or of NaN, which stays)
+        l_run = l_run * (m_ref > -INFINITY ? f_own : 1.f) + other.y * (other.x > -INFINITY ? f_other : 1.f);
+        m_ref = m;
+      }
+      const bool direct = walk.begins && walk.ends, spoilt = s_spoilt[item % kSpoilt] == item;
+      const int slot = 2 * blockIdx.x + (walk.begins ? 1 : 0), in_slot = (two ? w : 0) * kRows + r;
+      if (!direct && real && (two || w == 0)) *reinterpret_cast<float2*>(p.ml + (static_cast<size_t>(slot) * 2 * kRows + in_slot) * 2) = make_float2(m_ref, l_run);
+      const float scale = direct ? (l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f) : 1.f;
+      f_own *= scale;
+      f_other *= scale;
+      // a row's place in out, or in the scratch (-1: none)
+      const long long to_row = !real ? -1LL : direct ? static_cast<long long>(walk.s.row + row) * a.out_stride + static_cast<long long>(head) * D
+                                                     : (static_cast<long long>(slot) * 2 * kRows + in_slot) * D;
+      // By way of shared memory (the queries' place), so that a store writes whole lines: a lane has a row, a store 32 columns of four rows.
+      // (4 KB a warp: with heads of 64 the place has room for one group of warps, which then stores all columns)
+      constexpr bool kHalves = L::kQBytes >= 8 * 4096;
+      float* s_row = reinterpret_cast<float*>(s_place + (two || !kHalves ? warp & 3 : warp) * 4096);
+      const int c_begin = two ? 0 : kHalves ? w * (D / 2) : w * D, c_end = two || !kHalves ? D : c_begin + D / 2;
+#pragma unroll 1
+      for (int c = c_begin; c < c_end; c += 32) {
+        uint32_t x[32];
+        float o[32];
+        if (__any_sync(0xffffffffu, f_own != 0.f)) {
+          tmem_ld_x32(tmem_o + w * D + lane_addr + c, x);
+          tmem_wait_ld(x);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = f_own != 0.f ? __uint_as_float(x[i]) * f_own : 0.f;
+        if (!two && __any_sync(0xffffffffu, f_other != 0.f)) {
+          tmem_ld_x32(tmem_o + (w ^ 1) * D + lane_addr + c, x);
+          tmem_wait_ld(x);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = f_other != 0.f ? fmaf(__uint_as_float(x[i]), f_other, o[i]) : o[i];
+        }
+        if (l_run != l_run)                                    // (NaN among the scores of a group whose reference never moved)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = l_run;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<float4*>(s_row + staged(lane, 4 * i)) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int from = 4 * i + (lane >> 3);
+          const long long to = __shfl_sync(0xffffffffu, to_row, from);
+          const float4 v = *reinterpret_cast<const float4*>(s_row + staged(from, (lane & 7) * 4));
+          if (to >= 0) {
+            const size_t at = static_cast<size_t>(to) + c + (lane & 7) * 4;
+            if (direct) *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at) = make_uint2(pack_pair<T>(v.x, v.y), pack_pair<T>(v.z, v.w));
+            else *reinterpret_cast<float4*>(p.acc + at) = v;
+          }
+        }
+        __syncwarp();
+      }
+      if (spoilt && real) {
+        const int32_t* pages = a.page_table + static_cast<size_t>(walk.b) * a.max_pages;
+        if (direct) add_spoilt<T, D, T>(a, walk.s, pages, row, head, walk.tile, walk.tiles, walk.keys, c_begin, c_end, static_cast<T*>(a.out) + to_row);
+        else add_spoilt<T, D, float>(a, walk.s, pages, row, head, walk.tile, walk.tiles, walk.keys, c_begin, c_end, p.acc + to_row);
+      }
+      if (!two) {                                              // (the outputs may be written over)
+        ok = together(2);
+        if (!ok) break;
+        end_phase ^= 1;
+      }
+      if (walk.ends && !walk.begins) join = TreeJoin{walk.s.row + walk.row0, walk.rows, walk.kvh, walk.first};
+      tc_fence_before();
+      fence_async_smem();                                      // (the next queries come by copies)
+      __syncwarp();
+      if (two) { if (lane < 2) mbar_arrive(smem_u32(&bar_free[place])); }
+      else if (lane == 0) mbar_arrive(smem_u32(&bar_free[place]));
+    }
+    if (threadIdx.x == 0) p.joins[blockIdx.x] = join;
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tc_dealloc(tmem, 512);
+  }
+}
+
+// ---- the pieces of items that were cut ----
+// A block per (block of the first kernel, kJoinRows of its item's query rows), a warp per two rows, pieces in their order.
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinRows * 16)
+tree_pieces_kernel(const FastParams p) {
+  chain_enter();
+  const TreeJoin j = p.joins[blockIdx.x];
+  if (j.rows <= 0) return;
+  const cacheir_b200_tree_args& a = p.a;
+  const int group = a.heads / a.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kLanes = D / 4;                // of a row
+  const int n = static_cast<int>(blockIdx.x) - j.first + 1;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int place = blockIdx.y * kJoinRows + warp * 2 + e, r = place & (kRows - 1);
+    const int token = (place >> 7) * p.half_rows + r / group, head = r % group;
+    if (r >= p.half_rows * group || token >= j.rows) continue;
+    auto slot_of = [&](int i) { return 2 * (j.first + i) + (i == 0 ? 1 : 0); };
+    float m = -INFINITY, l = 0.f, f_last = 0.f;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const float2 v = i0 + lane < n ? *reinterpret_cast<const float2*>(p.ml + (static_cast<size_t>(slot_of(i0 + lane)) * 2 * kRows + place) * 2) : make_float2(-INFINITY, 0.f);
+      const float m_new = fmaxf(m, warp_max(v.x));
+      f_last = v.x > -INFINITY ? exp2f(v.x - m_new) : 0.f;
+      l = l * (m > -INFINITY ? exp2f(m - m_new) : 1.f) + warp_sum(v.y * (v.x > -INFINITY ? f_last : 1.f));
+      m = m_new;
+    }
+    const float scale = l > 0.f || l != l ? 1.f / l : 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int c = lane % kLanes * 4, part = lane / kLanes;                       // (lanes beside one another add up other pieces where a row has less than 32 of them)
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      float f = f_last;
+      if (n > 32) {                                                                // (weights of more than one round are worked out again)
+        const float x = i0 + lane < n ? p.ml[(static_cast<size_t>(slot_of(i0 + lane)) * 2 * kRows + place) * 2] : -INFINITY;
+        f = x > -INFINITY ? exp2f(x - m) : 0.f;
+      }
+#pragma unroll 4
+      for (int i = part; i < 32; i += 32 / kLanes) {
+        const float fi = __shfl_sync(0xffffffffu, f, i);
+        if (i0 + i < n && fi != 0.f) {
+          const float4 v = *reinterpret_cast<const float4*>(p.acc + (static_cast<size_t>(slot_of(i0 + i)) * 2 * kRows + place) * D + c);
+          o.x = fmaf(v.x, fi, o.x);
+          o.y = fmaf(v.y, fi, o.y);
+          o.z = fmaf(v.z, fi, o.z);
+          o.w = fmaf(v.w, fi, o.w);
+        }
+      }
+    }
+    if (kLanes < 32) {
+      o.x += __shfl_xor_sync(0xffffffffu, o.x, 16);
+      o.y += __shfl_xor_sync(0xffffffffu, o.y, 16);
+      o.z += __shfl_xor_sync(0xffffffffu, o.z, 16);
+      o.w += __shfl_xor_sync(0xffffffffu, o.w, 16);
+    }
+    if (l != l) o = make_float4(l, l, l, l);
+    if (part == 0)
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<size_t>(j.row + token) * a.out_stride + static_cast<size_t>(j.kvh * group + head) * D + c) =
+          make_uint2(pack_pair<T>(o.x * scale, o.y * scale), pack_pair<T>(o.z * scale, o.w * scale));
+  }
+}
+
+int half_rows_of(const cacheir_b200_tree_args& a) { return kRows / (a.heads / a.kv_heads); }
+// Units of all items, at most.
+long long most_units(const cacheir_b200_tree_args& a) {
+  const long long tiles = (static_cast<long long>(a.max_pages) * a.page_size + kKeys - 1) / kKeys;
+  return (kItemUnits + tiles) * a.kv_heads * (a.rows / (2 * half_rows_of(a)) + a.sequences);
+}
+
+template <typename T, int D>
+int launch_fast(const cacheir_b200_tree_args& a, cudaStream_t stream) {
+  CUtensorMap tk, tv, tq;
+  const uint64_t rows = static_cast<uint64_t>(a.num_slots) * a.kv_heads * a.page_size;
+  FastParams p;
+  p.a = a;
+  p.half_rows = half_rows_of(a);
+  p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  if (!encode_pool<T>(&tk, a.k_cache, rows, D, false) || !encode_pool<T>(&tv, a.v_cache, rows, D, true) ||
+      !encode_queries<T>(&tq, a.q, a.rows, a.heads, a.kv_heads, D, a.q_stride, p.half_rows))
+    return CACHEIR_B200_EUNSUPPORTED;
+  const long long most = most_units(a);
+  const int grid = static_cast<int>(most < kNumSMs ? most : kNumSMs);
+  p.joins = static_cast<TreeJoin*>(a.workspace);
+  p.ml = reinterpret_cast<float*>(p.joins + kNumSMs);
+  p.acc = p.ml + static_cast<size_t>(kNumSMs) * 2 * 2 * kRows * 2;
+  auto kern = tree_kernel<T, D>;
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = allow_shared_memory(done, reinterpret_cast<const void*>(kern), Smem<D>::kBytes);
+  if (e == cudaSuccess) e = launch_chained(kern, dim3(grid), dim3(kThreads), Smem<D>::kBytes, stream, tk, tv, tq, p);
+  if (e == cudaSuccess) e = launch_chained(tree_pieces_kernel<T, D>, dim3(grid, 2 * kRows / kJoinRows), dim3(kJoinRows * 16), 0, stream, p);
+  return e != cudaSuccess ? static_cast<int>(e) : launch_status();
+}
+
+}  // namespace
+
+size_t tree_fast_bytes(int dim) {
+  if (dim != 64 && dim != 128) return 0;
+  return kNumSMs * sizeof(TreeJoin) + static_cast<size_t>(kNumSMs) * 2 * 2 * kRows * (2 + dim) * 4;
+}
+
+bool tree_fast_supported(const cacheir_b200_tree_args& a) {
+  return (a.dtype == CACHEIR_B200_F16 || a.dtype == CACHEIR_B200_BF16) && (a.dim == 64 || a.dim == 128) && a.page_size % kChunk == 0 &&
+         a.heads / a.kv_heads <= kMaxHeadsPerKv && aligned_to(a.q, 16) && a.q_stride % 8 == 0 && aligned_to(a.k_cache, 16) && aligned_to(a.v_cache, 16) &&
+         aligned_to(a.out, 8) && a.out_stride % 4 == 0 && static_cast<long long>(a.num_slots) * a.kv_heads * a.page_size <= 0x7fffffffLL - kChunk &&
+         most_units(a) <= 0x7fffffffLL;
+}
+
+int launch_tree_fast(const cacheir_b200_tree_args& a, cudaStream_t stream) {
+  if (a.dtype == CACHEIR_B200_F16) return a.dim == 128 ? launch_fast<__half, 128>(a, stream) : launch_fast<__half, 64>(a, stream);
+  return a.dim == 128 ? launch_fast<__nv_bfloat16, 128>(a, stream) : launch_fast<__nv_bfloat16, 64>(a, stream);
+}
+
+int tree_device_status(bool reset) { return device_status_word(g_tree_status, reset); }
+
+}  // namespace cb200

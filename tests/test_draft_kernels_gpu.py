@@ -289,6 +289,17 @@ def test_many_sequences(sequences):
     Case(heads=4, kv_heads=2, dim=64, ctx=ctx, nodes=nodes, seed=sequences).check()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads, kv_heads", [(32, 8), (64, 4)])
+def test_blocks_with_many_items_of_many_tiles(dim, heads, kv_heads):
+    """Items of one group of query rows and of two, in turn, and no wait of a kernel has given up."""
+    from cacheir_b200 import _lib
+    rng = random.Random(dim + heads)
+    ctx, nodes = [rng.choice([0, 100, 800, 1500]) for _ in range(60)], [rng.choice([0, 1, 3, 17, 40]) for _ in range(60)]
+    Case(heads=heads, kv_heads=kv_heads, dim=dim, ctx=ctx, nodes=nodes, dtype=BF16, seed=dim).check()
+    assert _lib.load_group("drafts").cacheir_b200_drafts_device_status(0) == 0
+
+
 @pytest.mark.parametrize("lists", ["tree", None])
 def test_long_context_in_many_pieces(lists):
     got = Case(heads=4, kv_heads=1, ctx=(40000, 77), nodes=(6, 3), lists=lists, dtype=BF16, wide_q=2).check()
