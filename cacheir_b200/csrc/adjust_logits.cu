@@ -3,9 +3,12 @@
 //   c(t) = times that token t was said, known = c > 0 or t in the prompt
 //   x = known ? (x > 0 ? x / repetition : x * repetition) : x;  x -= frequency c;  x -= presence [c > 0];  x += bias(t);  -inf where not allowed
 //
-// Bound by memory: logits are read and written once. A block has a slice of the vocabulary and a run of rows. The tokens that fall into its slice
-// are counted in shared memory, once for all neighbouring rows of one sequence, and marked as bits; while the slice streams through registers only marked
-// tokens look at their counts. Counts are integers: the order of the additions does not matter.
+// Bound by memory: logits are read and written once, in a pass that knows nothing but the grammar's bits. A block has a slice of the vocabulary and a run of rows.
+// The tokens that fall into its slice are counted in shared memory, once for all neighbouring rows of one sequence, and listed; behind the pass the threads
+// share out (row, listed token) pairs, whose logits are asked for once more, mostly from L2. Looking at counts while the vectors are in registers was slower by far: eight
+// copies of the penalties' code a vector, of which instruction fetches alone took half the time (512 rows of 128256, 4096 tokens said: 325 us).
+// Drafted tokens are a short list beside the counts, of which every row takes those that it sees. Counts are integers: the order of the
+// additions does not matter.
 #include "cacheir_b200_drafts.h"
 #include "common.cuh"
 #include "serving_status.h"
@@ -14,7 +17,14 @@ namespace cb200 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kSlice = 4096;                           // tokens of a block, at most
+constexpr int kPairs = 4;                             // logits of listed tokens that a thread has under way
+#ifndef RUN
+#define RUN 16
+#endif
 constexpr uint32_t kInPrompt = 0x80000000u;
+constexpr uint32_t kDrafted = 0x40000000u;             // the list has the token
+constexpr uint32_t kTimes = 0x3fffffffu;
 
 struct LogitsParams {
   cacheir_b200_logits_args a;
@@ -22,128 +32,197 @@ struct LogitsParams {
   int run;                    // rows of a block
 };
 
-// Shared memory: marks [slice / 32 + 1], then counts [slice] (with a history or drafts), then entries of the bias [slice] (with one).
+__device__ __forceinline__ bool aligned_to_16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Shared memory: marks [slice / 32], then, where tokens can be marked, their list [slice], (with a history or drafts) counts [slice], (with a bias) entries of it
+// [slice], (with drafts) the drafted tokens.
 template <typename T, typename O, int VEC>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 adjust_logits_kernel(const LogitsParams p) {
+  constexpr int NV = kSlice / VEC / kThreads;          // vectors of a thread in a row
+  constexpr bool kWide = VEC > 1;
   chain_enter();
   extern __shared__ uint32_t smem[];
+  __shared__ int s_marked, s_drafted;
   const cacheir_b200_logits_args& a = p.a;
   const int lo = blockIdx.x * p.slice, size = min(p.slice, a.vocab - lo), words = p.slice / 32;
   const bool counting = a.history || a.draft_ids, biased = a.biases > 0;
-  uint32_t* marks = smem;                              // (one word more, which stays 0)
-  uint32_t* counts = smem + words + 1;
+  uint32_t* marks = smem;
+  uint32_t* counts = marks + words;
   int* entry = reinterpret_cast<int*>(counts + (counting ? p.slice : 0));
-  const int last = min(a.rows, static_cast<int>(blockIdx.y + 1) * p.run);
-  int current = -1;
-  for (int row = blockIdx.y * p.run; row < last; ++row) {
+  uint32_t* drafted = reinterpret_cast<uint32_t*>(entry + (biased ? p.slice : 0));   // token of the slice << 16 | row of the sequence
+  uint16_t* marked = reinterpret_cast<uint16_t*>(drafted + (a.draft_ids ? 32 * a.words : 0));
+  const int last = min(a.rows, static_cast<int>(blockIdx.y + 1) * p.run), allowed_words = (a.vocab + 31) / 32;
+  auto sequence_of = [&](int row) {
     const int seq = a.row_seq ? a.row_seq[row] : row;
-    if (seq < 0 || seq >= a.sequences) continue;
-    if (seq != current) {                              // count what its history says
+    return seq < a.sequences ? seq : -1;
+  };
+  auto input = [&](int row) { return static_cast<const T*>(a.logits) + static_cast<size_t>(row) * a.row_stride + lo; };
+  auto output = [&](int row) { return static_cast<O*>(a.out) + static_cast<size_t>(row) * a.out_stride + lo; };
+  auto grammar = [&](int row) { return reinterpret_cast<const uint32_t*>(a.allowed) + static_cast<size_t>(row) * allowed_words + lo / 32; };
+  // vectors begin where addresses allow it: `skew` tokens before the slice
+  auto skew_of = [&](const T* in) { return kWide ? static_cast<int>(reinterpret_cast<uintptr_t>(in) / sizeof(T) % VEC) : 0; };
+  const bool same = a.logits == a.out;
+
+  for (int row0 = blockIdx.y * p.run; row0 < last;) {
+    const int seq = sequence_of(row0);
+    int end = row0 + 1;
+    if (seq < 0) { row0 = end; continue; }
+    while (end < last && sequence_of(end) == seq) ++end;
+    // ---- the pass over the rows: values and bits of one are asked for while the one before is worked on (or tokens are counted) ----
+    const bool pass = !same || a.allowed;
+    uint4 ahead[kWide ? NV : 1];
+    uint2 bits[kWide ? NV : 1];
+    auto ask = [&](int row) {
+      const T* in = input(row);
+      const int skew = skew_of(in);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int t0 = (k * kThreads + static_cast<int>(threadIdx.x)) * VEC - skew;
+        if (t0 < 0 || t0 + VEC > size) continue;
+        ahead[k] = *reinterpret_cast<const uint4*>(in + t0);
+        if (a.allowed) {
+          const uint32_t* may = grammar(row) + (t0 >> 5);
+          bits[k].x = may[0];
+          if ((t0 & 31) + VEC > 32) bits[k].y = may[1];        // (the vector ends in the next word, which so there is)
+        }
+      }
+    };
+    if (kWide && pass) ask(row0);
+    // ---- what the sequence has said ----
+    if (counting || biased) {
       __syncthreads();
-      for (int i = threadIdx.x; i <= words; i += kThreads) marks[i] = 0;
+      for (int i = threadIdx.x; i < words; i += kThreads) marks[i] = 0;
       if (counting) for (int i = threadIdx.x; i < p.slice; i += kThreads) counts[i] = 0;
       if (biased) for (int i = threadIdx.x; i < p.slice; i += kThreads) entry[i] = 0;
+      if (threadIdx.x == 0) s_marked = s_drafted = 0;
       __syncthreads();
+      auto mark = [&](uint32_t t) {
+        const uint32_t bit = 1u << (t & 31);
+        if (!(atomicOr(&marks[t >> 5], bit) & bit)) marked[atomicAdd(&s_marked, 1)] = static_cast<uint16_t>(t);
+      };
       if (a.history) {
         const int32_t* said = a.history + static_cast<size_t>(seq) * a.history_width;
         const int n = min(a.history_lens[seq], a.history_width), prompt = a.prompt_lens ? a.prompt_lens[seq] : 0;
+#pragma unroll 4
         for (int i = threadIdx.x; i < n; i += kThreads) {
-          const uint32_t t = static_cast<uint32_t>(said[i] - lo);
-          if (said[i] >= 0 && t < static_cast<uint32_t>(size)) {
+          const int id = said[i];
+          const uint32_t t = static_cast<uint32_t>(id - lo);
+          if (id >= lo && t < static_cast<uint32_t>(size)) {
             if (i < prompt) atomicOr(&counts[t], kInPrompt);
             else atomicAdd(&counts[t], 1u);
-            atomicOr(&marks[t >> 5], 1u << (t & 31));
+            mark(t);
           }
         }
       }
       for (int i = threadIdx.x; i < a.biases; i += kThreads) {
         const int id = a.bias_ids[static_cast<size_t>(seq) * a.biases + i];
-        const uint32_t t = static_cast<uint32_t>(id - lo);
-        if (id >= 0 && t < static_cast<uint32_t>(size)) {
-          atomicMax(&entry[t], i + 1);
-          atomicOr(&marks[t >> 5], 1u << (t & 31));
+        if (id >= lo && id - lo < size) {
+          atomicMax(&entry[id - lo], i + 1);
+          mark(id - lo);
         }
       }
-      current = seq;
-      __syncthreads();
-    }
-    // the drafted tokens that this row sees (taken off again behind it)
-    auto drafted = [&](int sign) {
-      const int first = min(max(a.cu_rows[seq], 0), a.rows), end = min(max(a.cu_rows[seq + 1], 0), a.rows);
-      for (int j = threadIdx.x; j < min(end - first, 32 * a.words); j += kThreads)
-        if (a.visible[static_cast<size_t>(row) * a.words + (j >> 5)] >> (j & 31) & 1) {
+      if (a.draft_ids) {
+        const int first = min(max(a.cu_rows[seq], 0), a.rows), n = min(min(max(a.cu_rows[seq + 1], 0), a.rows) - first, 32 * a.words);
+        for (int j = threadIdx.x; j < n; j += kThreads) {
           const int64_t id = a.draft_ids[first + j];
-          if (id >= lo && id < lo + size) {
+          if (id >= lo && id - lo < size) {
             const uint32_t t = static_cast<uint32_t>(id - lo);
-            atomicAdd(&counts[t], static_cast<uint32_t>(sign));
-            atomicOr(&marks[t >> 5], 1u << (t & 31));
+            drafted[atomicAdd(&s_drafted, 1)] = t << 16 | static_cast<uint32_t>(j);
+            atomicOr(&counts[t], kDrafted);
+            mark(t);
           }
         }
-      __syncthreads();
-    };
-    if (a.draft_ids) drafted(1);
-    const float rep = a.repetition ? a.repetition[seq] : 1.f, freq = a.frequency ? a.frequency[seq] : 0.f, pres = a.presence ? a.presence[seq] : 0.f;
-    const float* values = a.bias_values + static_cast<size_t>(seq) * a.biases;
-    auto marked = [&](float x, int t) {                // token t of the slice
-      if (counting) {
-        const uint32_t c = counts[t], times = c & ~kInPrompt;
-        if (c) x = x > 0.f ? __fdiv_rn(x, rep) : x * rep;
-        if (times) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, static_cast<float>(times))), pres);
       }
-      if (biased && entry[t]) x = __fadd_rn(x, values[entry[t] - 1]);
-      return x;
-    };
-    const T* in = static_cast<const T*>(a.logits) + static_cast<size_t>(row) * a.row_stride + lo;
-    O* out = static_cast<O*>(a.out) + static_cast<size_t>(row) * a.out_stride + lo;
-    const uint32_t* allowed = a.allowed ? reinterpret_cast<const uint32_t*>(a.allowed) + static_cast<size_t>(row) * ((a.vocab + 31) / 32) + lo / 32 : nullptr;
-    const int allowed_words = (a.vocab + 31) / 32 - lo / 32;
-    // vectors begin where addresses allow it: `skew` tokens before the slice
-    const int skew = VEC > 1 ? static_cast<int>(reinterpret_cast<uintptr_t>(in) / sizeof(T) % VEC) : 0;
-    const bool same = static_cast<const void*>(in) == static_cast<const void*>(out) && sizeof(T) == sizeof(O);
-    for (int v = threadIdx.x; v * VEC < size + skew; v += kThreads) {
-      const int t0 = v * VEC - skew, w = max(t0, 0) >> 5, sh = t0 & 31;
-      uint32_t mark, may = 0xffffffffu;                // bits of the vector's tokens
-      if (t0 < 0) {
-        mark = marks[0] << -t0;
-        if (allowed) may = allowed[0] << -t0;
-      } else {
-        mark = __funnelshift_r(marks[w], marks[w + 1], sh);
-        if (allowed) may = __funnelshift_r(allowed[w], w + 1 < allowed_words && sh + VEC > 32 ? allowed[w + 1] : 0u, sh);
-      }
-      if (VEC < 32) { mark &= (1u << VEC) - 1; may &= (1u << VEC) - 1; }
-      const bool whole = t0 >= 0 && t0 + VEC <= size;
-      if (same && mark == 0 && (!allowed || may == (1u << VEC) - 1)) continue;
-      if (whole) {
-        float x[VEC];
-        VecIO<T, VEC>::ld(in + t0, x);
-        if (mark)
+    }
+    if (pass) {
+      for (int row = row0; row < end; ++row) {
+        const T* in = input(row);
+        O* out = output(row);
+        auto one = [&](int t) {
+          if (a.allowed && !(grammar(row)[t >> 5] >> (t & 31) & 1)) Elem<O>::st(out + t, -INFINITY);
+          else if (!same) Elem<O>::st(out + t, Elem<T>::ld(in + t));
+        };
+        if constexpr (kWide) {
+          uint4 raw[NV];
+          uint2 may[NV];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i)
-            if (mark >> i & 1) x[i] = marked(x[i], t0 + i);
-        if (allowed)
+          for (int k = 0; k < NV; ++k) { raw[k] = ahead[k]; may[k] = bits[k]; }
+          if (row + 1 < end) ask(row + 1);
+          const int skew = skew_of(in);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i)
-            if (!(may >> i & 1)) x[i] = -INFINITY;
-        if constexpr (sizeof(O) == sizeof(T)) {
-          VecIO<O, VEC>::st(out + t0, x);
+          for (int k = 0; k < NV; ++k) {
+            const int t0 = (k * kThreads + static_cast<int>(threadIdx.x)) * VEC - skew;
+            if (t0 < 0 || t0 + VEC > size) continue;
+            const uint32_t yes = a.allowed ? __funnelshift_r(may[k].x, may[k].y, t0 & 31) | ~((1u << VEC) - 1) : 0xffffffffu;
+            if (same && yes == 0xffffffffu) continue;
+            float x[VEC];
+            VecIO<T, VEC>::ld(reinterpret_cast<const T*>(&raw[k]), x);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+              if (!(yes >> i & 1)) x[i] = -INFINITY;
+            if constexpr (sizeof(O) == sizeof(T)) {
+              VecIO<O, VEC>::st(out + t0, x);
+            } else if (aligned_to_16(out + t0)) {
+#pragma unroll
+              for (int i = 0; i < VEC; i += 4) *reinterpret_cast<float4*>(out + t0 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) Elem<O>::st(out + t0 + i, x[i]);
+            }
+          }
+          // tokens of vectors that the slice has only a part of: fewer than VEC at either end
+          const int head = min((VEC - skew) % VEC, size), tail = head + (size - head) / VEC * VEC, i = threadIdx.x;
+          if (i < head) one(i);
+          else if (i >= 32 && tail + i - 32 < size) one(tail + i - 32);
         } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) Elem<O>::st(out + t0 + i, x[i]);
-        }
-      } else {
-        for (int i = max(-t0, 0); i < VEC && t0 + i < size; ++i) {
-          float x = Elem<T>::ld(in + t0 + i);
-          if (mark >> i & 1) x = marked(x, t0 + i);
-          if (allowed && !(may >> i & 1)) x = -INFINITY;
-          Elem<O>::st(out + t0 + i, x);
+#pragma unroll 4
+          for (int t = threadIdx.x; t < size; t += kThreads) one(t);
         }
       }
     }
-    if (a.draft_ids) {
+    // ---- tokens that were said, are drafted or have a bias ----
+    if (counting || biased) {
       __syncthreads();
-      drafted(-1);
+      const int many = s_drafted, rows = end - row0, pairs = s_marked * rows;
+      const float rep = a.repetition ? a.repetition[seq] : 1.f, freq = a.frequency ? a.frequency[seq] : 0.f, pres = a.presence ? a.presence[seq] : 0.f;
+      for (int i0 = threadIdx.x; i0 < pairs; i0 += kPairs * kThreads) {
+        T value[kPairs];
+        uint32_t may[kPairs];
+        int token[kPairs], at[kPairs];
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) {                     // (asked for together)
+          const int i = min(i0 + e * kThreads, pairs - 1), k = i / rows;
+          token[e] = marked[k];
+          at[e] = row0 + i - k * rows;
+          value[e] = input(at[e])[token[e]];
+          may[e] = a.allowed ? grammar(at[e])[token[e] >> 5] : 0xffffffffu;
+        }
+#pragma unroll 1
+        for (int e = 0; e < kPairs; ++e) {
+          int t = token[0], row = at[0];
+          T raw = value[0];
+          uint32_t word = may[0];
+#pragma unroll
+          for (int f = 1; f < kPairs; ++f)
+            if (e == f) { t = token[f]; row = at[f]; raw = value[f]; word = may[f]; }
+          if (i0 + e * kThreads >= pairs || !(word >> (t & 31) & 1)) continue;
+          float x = Elem<T>::ld(&raw);
+          const uint32_t c = counting ? counts[t] : 0u;
+          uint32_t times = c & kTimes;
+          if (c & kDrafted)
+            for (int d = 0; d < many; ++d) {
+              const uint32_t v = drafted[d], j = v & 0xffffu;
+              if (v >> 16 == static_cast<uint32_t>(t)) times += a.visible[static_cast<size_t>(row) * a.words + (j >> 5)] >> (j & 31) & 1;
+            }
+          if (times || (c & kInPrompt)) x = x > 0.f ? __fdiv_rn(x, rep) : x * rep;
+          if (times) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, static_cast<float>(times))), pres);
+          const int entry_of = biased ? entry[t] : 0;
+          if (entry_of) x = __fadd_rn(x, a.bias_values[static_cast<size_t>(seq) * a.biases + entry_of - 1]);
+          Elem<O>::st(output(row) + t, x);
+        }
+      }
     }
+    row0 = end;
   }
 }
 
@@ -151,14 +230,14 @@ template <typename T, typename O>
 int launch_adjust(const cacheir_b200_logits_args& a, cudaStream_t stream) {
   constexpr int VEC = 16 / sizeof(T);
   // Slices and runs: enough blocks for all SMs before rows share a count.
-  LogitsParams p{a, 8192, 1};
+  LogitsParams p{a, kSlice, 1};
   while (p.slice > 1024 && static_cast<long long>(a.rows) * ((a.vocab + p.slice - 1) / p.slice) < 4 * kNumSMs) p.slice /= 2;
   const int slices = (a.vocab + p.slice - 1) / p.slice;
-  while (p.run < 8 && static_cast<long long>(a.rows) * slices >= 16LL * p.run * kNumSMs) p.run *= 2;
+  while (p.run < RUN && static_cast<long long>(a.rows) * slices >= 12LL * p.run * kNumSMs) p.run *= 2;
   const int runs = (a.rows + p.run - 1) / p.run;
   if (runs > 65535) p.run = (a.rows + 65534) / 65535;
   const bool counting = a.history || a.draft_ids;
-  const size_t smem = (p.slice / 32 + 1 + (counting ? p.slice : 0) + (a.biases > 0 ? p.slice : 0)) * sizeof(uint32_t);
+  const size_t smem = (p.slice / 32 + (counting ? p.slice : 0) + (a.biases > 0 ? p.slice : 0) + (a.draft_ids ? 32 * a.words : 0)) * sizeof(uint32_t) + p.slice * sizeof(uint16_t);
   // vectors where a row's input and output begin at the same place of 16 bytes (with outputs of the same size)
   const bool wide = reinterpret_cast<uintptr_t>(a.logits) % sizeof(T) == 0 &&
                     (sizeof(T) != sizeof(O) || ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.out)) % 16 == 0 &&
@@ -166,7 +245,7 @@ int launch_adjust(const cacheir_b200_logits_args& a, cudaStream_t stream) {
   auto kern = wide ? adjust_logits_kernel<T, O, VEC> : adjust_logits_kernel<T, O, 1>;
   const dim3 grid(slices, (a.rows + p.run - 1) / p.run);
   static std::atomic<unsigned long long> done_wide{0}, done_any{0};
-  constexpr int most = (8192 / 32 + 1 + 2 * 8192) * 4;
+  constexpr int most = (kSlice / 32 + 2 * kSlice + 32 * CACHEIR_B200_MAX_DRAFT_WORDS) * 4 + kSlice * 2;
   cudaError_t e = allow_shared_memory(wide ? done_wide : done_any, reinterpret_cast<const void*>(kern), most);
   if (e == cudaSuccess) e = launch_chained(kern, grid, dim3(kThreads), smem, stream, p);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
@@ -188,7 +267,7 @@ extern "C" int cacheir_b200_adjust_logits(const cacheir_b200_logits_args* args, 
       (a.draft_ids && (!a.cu_rows || !a.visible || a.words <= 0)) || (a.biases > 0 && (!a.bias_ids || !a.bias_values)))
     return CACHEIR_B200_EINVAL;
   if (a.logits == a.out && a.dtype != a.out_dtype) return CACHEIR_B200_EINVAL;
-  if (a.vocab > 1 << 28 || (a.draft_ids && a.words > CACHEIR_B200_MAX_DRAFT_WORDS)) return CACHEIR_B200_ELIMIT;
+  if (a.vocab > 1 << 28 || a.history_width > 1 << 29 || (a.draft_ids && a.words > CACHEIR_B200_MAX_DRAFT_WORDS)) return CACHEIR_B200_ELIMIT;
   if (a.biases == 0) a.bias_ids = nullptr;
   if (a.dtype == CACHEIR_B200_F32) return launch_adjust<float, float>(a, as_stream(stream));
   if (a.dtype == CACHEIR_B200_F16)

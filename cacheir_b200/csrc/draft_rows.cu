@@ -125,54 +125,75 @@ accept_drafts_kernel(const cacheir_b200_accept_args a) {
   }
 }
 
-// ---- keep: a block a sequence and pool, a thread a column, which it moves in the order of the path ----
+// ---- keep: a block a sequence and some pools, a thread a column, which it moves in the order of the path ----
 constexpr int kKeepThreads = 128;
 constexpr int kKeepPools = 128;               // of a launch
-constexpr int kKeepDeep = 8;                  // rows that a thread has under way
+constexpr int kKeepShare = 4;                 // pools of a block, which a thread has under way together ..
+constexpr int kKeepDeep = 4;                  // .. with so many rows of each
+constexpr int kKeepMoves = 64;                // moves that a block looks up together
 
 struct KeepParams {
   cacheir_b200_keep_args a;
-  void* pools[kKeepPools];
+  int pools;
+  void* pool[kKeepPools];
 };
 
-// Row i's source is never a target before it, as row numbers rise along a path: all that is written before i is read lies in front of it.
+// A row's source is never a target before it, as row numbers rise along a path: all that is written before it is read lies in front of it.
+// What takes time is the way from counts over rows and slots to the values, four dependent loads; so it is gone once for several pools.
 template <typename V>
 __global__ void __launch_bounds__(kKeepThreads)
 keep_accepted_kernel(const __grid_constant__ KeepParams p) {
   chain_enter();
+  __shared__ int s_from[kKeepMoves], s_to[kKeepMoves];         // pool rows (a slot's page * heads * page size + its place), head 0; -1: none
   const cacheir_b200_keep_args& a = p.a;
   const int b = blockIdx.x;
-  const int count = min(a.counts[b], a.depth);
-  if (count <= 1) return;
   const int2 mine = rows_of(a.cu_rows, a.rows, b);
+  const int count = min(min(a.counts[b], a.depth), mine.y);
   const int32_t* path = a.path + static_cast<size_t>(b) * a.depth;
-  V* pool = static_cast<V*>(p.pools[blockIdx.y]);
   const int width = a.dim * (a.dtype == CACHEIR_B200_F32 ? 4 : 2) / static_cast<int>(sizeof(V));          // units of a line
   const long long outside = static_cast<long long>(a.num_slots) * a.page_size;
-  // first unit of a row of this column's head; -1: not in the pool
-  auto line_of = [&](int row, int head) {
+  auto line_of = [&](int row) {
     const int slot = row >= 0 && row < a.rows ? a.slots[row] : -1;
-    if (slot < 0 || slot >= outside) return -1LL;
-    return ((static_cast<long long>(slot / a.page_size) * a.kv_heads + head) * a.page_size + slot % a.page_size) * width;
+    return slot < 0 || slot >= outside ? -1 : slot;
   };
-  for (int c = blockIdx.z * kKeepThreads + threadIdx.x; c < a.kv_heads * width; c += gridDim.z * kKeepThreads) {
-    const int head = c / width, at = c - head * width;
-    for (int i0 = 1; i0 < count; i0 += kKeepDeep) {
-      V v[kKeepDeep];
-      long long to[kKeepDeep];
+  const int first_pool = blockIdx.y * kKeepShare, pools = min(kKeepShare, p.pools - first_pool);
+  for (int i0 = 1; i0 < count; i0 += kKeepMoves) {             // (rows of one round are read after those before it were written, in any thread)
+    const int moves = min(kKeepMoves, count - i0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < moves; i += kKeepThreads) {
+      const int row = path[i0 + i], to = mine.x + i0 + i;
+      s_from[i] = row == to ? -1 : line_of(row);
+      s_to[i] = line_of(to);
+    }
+    __syncthreads();
+    for (int c = blockIdx.z * kKeepThreads + threadIdx.x; c < a.kv_heads * width; c += gridDim.z * kKeepThreads) {
+      const int head = c / width, at = c - head * width;
+      auto place = [&](int slot) {
+        return ((static_cast<long long>(slot / a.page_size) * a.kv_heads + head) * a.page_size + slot % a.page_size) * width + at;
+      };
+      for (int j0 = 0; j0 < moves; j0 += kKeepDeep) {
+        V v[kKeepShare][kKeepDeep];
 #pragma unroll
-      for (int e = 0; e < kKeepDeep; ++e) {
-        const int i = i0 + e;
-        to[e] = -1;
-        if (i < count && i < mine.y && path[i] != mine.x + i) {
-          const long long from = line_of(path[i], head);
-          to[e] = from >= 0 ? line_of(mine.x + i, head) : -1;
-          if (to[e] >= 0) v[e] = pool[from + at];
+        for (int e = 0; e < kKeepDeep; ++e) {
+          const int j = min(j0 + e, moves - 1), from = s_from[j];
+          if (j0 + e < moves && from >= 0 && s_to[j] >= 0) {
+            const long long x = place(from);
+#pragma unroll
+            for (int k = 0; k < kKeepShare; ++k)
+              if (k < pools) v[k][e] = static_cast<const V*>(p.pool[first_pool + k])[x];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < kKeepDeep; ++e) {
+          const int j = min(j0 + e, moves - 1), to = s_to[j];
+          if (j0 + e < moves && to >= 0 && s_from[j] >= 0) {
+            const long long x = place(to);
+#pragma unroll
+            for (int k = 0; k < kKeepShare; ++k)
+              if (k < pools) static_cast<V*>(p.pool[first_pool + k])[x] = v[k][e];
+          }
         }
       }
-#pragma unroll
-      for (int e = 0; e < kKeepDeep; ++e)
-        if (to[e] >= 0) pool[to[e] + at] = v[e];
     }
   }
 }
@@ -184,10 +205,10 @@ int launch_keep(const cacheir_b200_keep_args& a, cudaStream_t stream) {
   for (int first = 0; first < a.pool_count; first += kKeepPools) {
     KeepParams p;
     p.a = a;
-    const int pools = a.pool_count - first < kKeepPools ? a.pool_count - first : kKeepPools;
-    for (int i = 0; i < pools; ++i) p.pools[i] = a.pools[first + i];
-    const cudaError_t e = launch_chained(keep_accepted_kernel<V>, dim3(a.sequences, pools, static_cast<unsigned>(chunks < 64 ? chunks : 64)), dim3(kKeepThreads), 0,
-                                         stream, p);
+    p.pools = a.pool_count - first < kKeepPools ? a.pool_count - first : kKeepPools;
+    for (int i = 0; i < p.pools; ++i) p.pool[i] = a.pools[first + i];
+    const dim3 grid(a.sequences, (p.pools + kKeepShare - 1) / kKeepShare, static_cast<unsigned>(chunks < 64 ? chunks : 64));
+    const cudaError_t e = launch_chained(keep_accepted_kernel<V>, grid, dim3(kKeepThreads), 0, stream, p);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   return launch_status();

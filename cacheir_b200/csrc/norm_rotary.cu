@@ -7,6 +7,7 @@
 // products are in 32 bits; a value is rounded once, where it is stored.
 #include "cacheir_b200_drafts.h"
 #include "common.cuh"
+#include "float_pairs.cuh"
 #include "rotary_turn.cuh"
 
 namespace cb200 {
@@ -14,6 +15,9 @@ namespace {
 
 constexpr int kMaxThreads = 256;
 constexpr int kMaxDim = 1024;
+constexpr int kTogether = 2;                // heads that a lane has under way
+
+using ptx::f32x2;
 
 // Row `row`'s place in the pool, in rows of a key/value head; -1: outside it.
 __device__ __forceinline__ long long pool_line(const cacheir_b200_rotary_args& p, int row) {
@@ -23,92 +27,142 @@ __device__ __forceinline__ long long pool_line(const cacheir_b200_rotary_args& p
   return static_cast<long long>(slot / p.page_size) * p.kv_heads * p.page_size + slot % p.page_size;
 }
 
-// A unit is VEC pairs (or 2 VEC values that do not turn): two vectors of VEC values. `lanes` units (a power of two, up to 32) are a head.
-template <typename T, int VEC>
+// A lane has VEC pairs (or 2 VEC values that do not turn) of a head, as two vectors of VEC values; LANES lanes are a head. pair_x(i), pair_y(i): which of
+// the 2 VEC values are the two of pair i.
+template <int VEC, bool HALF>
+__device__ __forceinline__ constexpr int pair_x(int i) { return HALF ? i : 2 * i; }
+template <int VEC, bool HALF>
+__device__ __forceinline__ constexpr int pair_y(int i) { return HALF ? VEC + i : 2 * i + 1; }
+
+template <typename T, int VEC, int LANES, bool HALF>
 __global__ void __launch_bounds__(kMaxThreads)
-norm_rotary_kernel(const cacheir_b200_norm_rotary_args args, const int lanes) {
+norm_rotary_kernel(const cacheir_b200_norm_rotary_args args) {
   chain_enter();
-  __shared__ float2 s_turn[kMaxDim / 2];
+  __shared__ __align__(16) float2 s_turn[LANES * VEC];
   const cacheir_b200_rotary_args& p = args.rotary;
-  const int row = blockIdx.x, threads = blockDim.x;
+  const int row = blockIdx.x, threads = blockDim.x, groups = threads / LANES;
   const long long line = pool_line(p, row);
   if (line < 0) return;
   const int half = p.rot / 2, position = p.positions[row];
   for (int i = threadIdx.x; i < half; i += threads) s_turn[i] = turn_cos_sin(p.turns[i], position, p.factor);
   __syncthreads();
-  const int turning = half / VEC, j = threadIdx.x & (lanes - 1);
-  const bool turns = j < turning, wide_turn = p.layout == CACHEIR_B200_ROTARY_HALF;
-  const int at = !turns ? p.rot + (j - turning) * 2 * VEC : wide_turn ? j * VEC : j * 2 * VEC;
-  const int second = turns && wide_turn ? at + half : at + VEC;
-  const int heads = p.heads + (p.slots ? 2 : 1) * p.kv_heads;
-  for (int u0 = 0; u0 < heads * lanes; u0 += threads) {
-    const int head = (u0 + static_cast<int>(threadIdx.x)) / lanes;
-    const bool active = head < heads, is_q = head < p.heads, is_v = head >= p.heads + p.kv_heads;
-    const int h = is_q ? head : (head - p.heads) % p.kv_heads;
-    float a[VEC] = {}, b[VEC] = {};
-    if (active) {
-      const T* src = is_q ? static_cast<const T*>(p.q) + row * p.q_stride
-                          : is_v ? static_cast<const T*>(p.v) + row * p.v_stride : static_cast<const T*>(p.k) + row * p.k_stride;
-      src += static_cast<size_t>(h) * p.dim;
-      VecIO<T, VEC>::ld(src + at, a);
-      VecIO<T, VEC>::ld(src + second, b);
+  const int turning = half / VEC, j = threadIdx.x & (LANES - 1);
+  const bool turns = j < turning;
+  const int at = !turns ? p.rot + (j - turning) * 2 * VEC : HALF ? j * VEC : j * 2 * VEC;
+  const int second = turns && HALF ? at + half : at + VEC;
+  const int behind_q = p.heads, behind_k = p.heads + p.kv_heads, heads = behind_k + (p.slots ? p.kv_heads : 0);
+  // the weights of this lane's values, of queries or keys, as pairs of pairs
+  f32x2 wx[VEC / 2], wy[VEC / 2];
+  const void* loaded = nullptr;
+  auto load_weights = [&](const void* weight) {
+    float w[2 * VEC];
+    if (!weight) {
+#pragma unroll
+      for (int i = 0; i < 2 * VEC; ++i) w[i] = 1.f;
+    } else if (sizeof(T) == 4 || args.weight_dtype != CACHEIR_B200_F32) {
+      float a[VEC], b[VEC];
+      VecIO<T, VEC>::ld(static_cast<const T*>(weight) + at, a);
+      VecIO<T, VEC>::ld(static_cast<const T*>(weight) + second, b);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { w[i] = a[i] + args.offset; w[VEC + i] = b[i] + args.offset; }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        w[i] = static_cast<const float*>(weight)[at + i] + args.offset;
+        w[VEC + i] = static_cast<const float*>(weight)[second + i] + args.offset;
+      }
     }
-    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
-    for (int off = lanes >> 1; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (!active) continue;
-    if (!is_v) {
-      const float r = rsqrtf(sum / static_cast<float>(p.dim) + args.eps);
-      const void* weight = is_q ? args.q_weight : args.k_weight;
-      if (weight) {
-        float wa[VEC], wb[VEC];
-        if (sizeof(T) == 4 || args.weight_dtype != CACHEIR_B200_F32) {
-          VecIO<T, VEC>::ld(static_cast<const T*>(weight) + at, wa);
-          VecIO<T, VEC>::ld(static_cast<const T*>(weight) + second, wb);
-        } else {
+    for (int i = 0; i < VEC; i += 2) {
+      wx[i / 2] = ptx::pair(w[pair_x<VEC, HALF>(i)], w[pair_x<VEC, HALF>(i + 1)]);
+      wy[i / 2] = ptx::pair(w[pair_y<VEC, HALF>(i)], w[pair_y<VEC, HALF>(i + 1)]);
+    }
+    loaded = weight;
+  };
+  load_weights(args.q_weight);
+  const float inverse = 1.f / static_cast<float>(p.dim);
+  // (values of several heads are asked for together: a store might be to what a later load reads, so that loads wait for the stores before them)
+  for (int head0 = threadIdx.x / LANES; head0 - static_cast<int>(threadIdx.x & 31) / LANES < heads; head0 += kTogether * groups) {         // (whole warps)
+    uint4 raw[kTogether][2];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            wa[i] = static_cast<const float*>(weight)[at + i];
-            wb[i] = static_cast<const float*>(weight)[second + i];
-          }
-        }
+    for (int e = 0; e < kTogether; ++e) {
+      const int head = head0 + e * groups;
+      if (head >= heads) continue;
+      const T* src = head < behind_q ? static_cast<const T*>(p.q) + row * p.q_stride + head * p.dim
+                                     : head < behind_k ? static_cast<const T*>(p.k) + row * p.k_stride + (head - behind_q) * p.dim
+                                                       : static_cast<const T*>(p.v) + row * p.v_stride + (head - behind_k) * p.dim;
+      raw[e][0] = *reinterpret_cast<const uint4*>(src + at);
+      raw[e][1] = *reinterpret_cast<const uint4*>(src + second);
+    }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          a[i] = a[i] * r * (wa[i] + args.offset);
-          b[i] = b[i] * r * (wb[i] + args.offset);
-        }
-      } else {
+    for (int e = 0; e < kTogether; ++e) {
+      const int head = head0 + e * groups;
+      float v[2 * VEC];
+      f32x2 x[VEC / 2], y[VEC / 2], squares = 0ull;
+      {
+        float a[VEC], b[VEC];
+        VecIO<T, VEC>::ld(reinterpret_cast<const T*>(&raw[e][0]), a);
+        VecIO<T, VEC>::ld(reinterpret_cast<const T*>(&raw[e][1]), b);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) { a[i] *= r; b[i] *= r; }
+        for (int i = 0; i < VEC; ++i) { v[i] = a[i]; v[VEC + i] = b[i]; }
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; i += 2) {
+        x[i / 2] = ptx::pair(v[pair_x<VEC, HALF>(i)], v[pair_x<VEC, HALF>(i + 1)]);
+        y[i / 2] = ptx::pair(v[pair_y<VEC, HALF>(i)], v[pair_y<VEC, HALF>(i + 1)]);
+        squares = ptx::fma2(x[i / 2], x[i / 2], ptx::fma2(y[i / 2], y[i / 2], squares));
+      }
+      float sum, more;
+      ptx::unpair(squares, sum, more);
+      sum += more;
+#pragma unroll
+      for (int off = LANES / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      if (head >= heads) continue;
+      if (head >= behind_k) {                              // values are copied
+        T* dst = static_cast<T*>(p.v_cache) + (static_cast<size_t>(line) + static_cast<size_t>(head - behind_k) * p.page_size) * p.dim;
+        *reinterpret_cast<uint4*>(dst + at) = raw[e][0];
+        *reinterpret_cast<uint4*>(dst + second) = raw[e][1];
+        continue;
+      }
+      const void* weight = head < behind_q ? args.q_weight : args.k_weight;
+      if (weight != loaded) load_weights(weight);
+      const float r = rsqrtf(fmaf(sum, inverse, args.eps));
+      const f32x2 r2 = ptx::pair(r, r);
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        x[i] = ptx::mul2(ptx::mul2(x[i], r2), wx[i]);
+        y[i] = ptx::mul2(ptx::mul2(y[i], r2), wy[i]);
       }
       if (turns) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float2 t = s_turn[j * VEC + i];
-          float x, y;
-          if (wide_turn) { x = a[i]; y = b[i]; }
-          else { x = i < VEC / 2 ? a[2 * i % VEC] : b[2 * i % VEC]; y = i < VEC / 2 ? a[(2 * i + 1) % VEC] : b[(2 * i + 1) % VEC]; }
-          const float rx = __fmaf_rn(x, t.x, -__fmul_rn(y, t.y)), ry = __fmaf_rn(x, t.y, __fmul_rn(y, t.x));
-          if (wide_turn) { a[i] = rx; b[i] = ry; }
-          else if (i < VEC / 2) { a[2 * i % VEC] = rx; a[(2 * i + 1) % VEC] = ry; }
-          else { b[2 * i % VEC] = rx; b[(2 * i + 1) % VEC] = ry; }
+        for (int i = 0; i < VEC / 2; ++i) {
+          const float4 t = *reinterpret_cast<const float4*>(&s_turn[j * VEC + 2 * i]);       // two cosines and sines
+          const f32x2 c = ptx::pair(t.x, t.z), s = ptx::pair(t.y, t.w), less = ptx::pair(-t.y, -t.w);
+          const f32x2 turned = ptx::fma2(x[i], c, ptx::mul2(y[i], less));
+          y[i] = ptx::fma2(x[i], s, ptx::mul2(y[i], c));
+          x[i] = turned;
         }
       }
-    }
-    auto put = [&](void* base, size_t from) {
-      T* dst = static_cast<T*>(base) + from;
-      VecIO<T, VEC>::st(dst + at, a);
-      VecIO<T, VEC>::st(dst + second, b);
-    };
-    const size_t pooled = (static_cast<size_t>(line) + static_cast<size_t>(h) * p.page_size) * p.dim;
-    if (is_q) {
-      if (p.q_out) put(p.q_out, static_cast<size_t>(row) * p.q_out_stride + static_cast<size_t>(h) * p.dim);
-    } else if (is_v) {
-      put(p.v_cache, pooled);
-    } else {
-      if (p.k_out) put(p.k_out, static_cast<size_t>(row) * p.k_out_stride + static_cast<size_t>(h) * p.dim);
-      if (p.slots) put(p.k_cache, pooled);
+      float a[VEC], b[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; i += 2) {
+        ptx::unpair(x[i / 2], v[pair_x<VEC, HALF>(i)], v[pair_x<VEC, HALF>(i + 1)]);
+        ptx::unpair(y[i / 2], v[pair_y<VEC, HALF>(i)], v[pair_y<VEC, HALF>(i + 1)]);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { a[i] = v[i]; b[i] = v[VEC + i]; }
+      auto put = [&](void* base, size_t from) {
+        T* dst = static_cast<T*>(base) + from;
+        VecIO<T, VEC>::st(dst + at, a);
+        VecIO<T, VEC>::st(dst + second, b);
+      };
+      if (head < behind_q) {
+        if (p.q_out) put(p.q_out, static_cast<size_t>(row) * p.q_out_stride + static_cast<size_t>(head) * p.dim);
+      } else {
+        const int h = head - behind_q;
+        if (p.k_out) put(p.k_out, static_cast<size_t>(row) * p.k_out_stride + static_cast<size_t>(h) * p.dim);
+        if (p.slots) put(p.k_cache, (static_cast<size_t>(line) + static_cast<size_t>(h) * p.page_size) * p.dim);
+      }
     }
   }
 }
@@ -175,19 +229,30 @@ norm_rotary_any_kernel(const cacheir_b200_norm_rotary_args args) {
   }
 }
 
+template <typename T, int VEC, int LANES>
+cudaError_t launch_lanes(const cacheir_b200_norm_rotary_args& args, int threads, cudaStream_t stream) {
+  return args.rotary.layout == CACHEIR_B200_ROTARY_HALF ? launch_chained(norm_rotary_kernel<T, VEC, LANES, true>, dim3(args.rotary.rows), dim3(threads), 0, stream, args)
+                                                        : launch_chained(norm_rotary_kernel<T, VEC, LANES, false>, dim3(args.rotary.rows), dim3(threads), 0, stream, args);
+}
+
 template <typename T>
 int launch_norm_rotary(const cacheir_b200_norm_rotary_args& args, cudaStream_t stream) {
   constexpr int VEC = 16 / sizeof(T);
   const cacheir_b200_rotary_args& a = args.rotary;
-  const int lanes = a.dim / (2 * VEC);
-  bool wide = a.dim % (2 * VEC) == 0 && a.rot % (2 * VEC) == 0 && lanes <= 32 && (lanes & (lanes - 1)) == 0;
+  bool wide = a.dim % (2 * VEC) == 0 && a.rot % (2 * VEC) == 0;
   for (const void* ptr : {a.q, a.k, a.v, static_cast<const void*>(a.q_out), static_cast<const void*>(a.k_out), static_cast<const void*>(a.k_cache),
                           static_cast<const void*>(a.v_cache), args.q_weight, args.k_weight})
     wide = wide && aligned_to(ptr, 16);
   for (long long stride : {a.q_stride, a.k_stride, a.v_stride, a.q_out_stride, a.k_out_stride}) wide = wide && stride % VEC == 0;
   const int threads = a.rows > 4096 ? 64 : a.rows > 4 * kNumSMs ? 128 : kMaxThreads;
-  const cudaError_t e = wide ? launch_chained(norm_rotary_kernel<T, VEC>, dim3(a.rows), dim3(threads), 0, stream, args, lanes)
-                             : launch_chained(norm_rotary_any_kernel<T>, dim3(a.rows), dim3(threads), 0, stream, args);
+  cudaError_t e;
+  switch (wide ? a.dim / (2 * VEC) : 0) {                  // lanes of a head
+    case 4: e = launch_lanes<T, VEC, 4>(args, threads, stream); break;
+    case 8: e = launch_lanes<T, VEC, 8>(args, threads, stream); break;
+    case 16: e = launch_lanes<T, VEC, 16>(args, threads, stream); break;
+    case 32: e = launch_lanes<T, VEC, 32>(args, threads, stream); break;
+    default: e = launch_chained(norm_rotary_any_kernel<T>, dim3(a.rows), dim3(threads), 0, stream, args);
+  }
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }
 
