@@ -19,12 +19,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kSlice = 4096;                           // tokens of a block, at most
 constexpr int kPairs = 4;                             // logits of listed tokens that a thread has under way
-#ifndef RUN
-#define RUN 16
-#endif
+constexpr int kRun = 8;                                // rows of a block, at most (16: 111 us for 95, as there are fewer blocks to even the work out)
+constexpr int kSaid = 8;                               // tokens of the history that a thread has under way
 constexpr uint32_t kInPrompt = 0x80000000u;
-constexpr uint32_t kDrafted = 0x40000000u;             // the list has the token
-constexpr uint32_t kTimes = 0x3fffffffu;
+constexpr uint32_t kDrafted = 0x40000000u;             // the list of drafted tokens has the token
+constexpr uint32_t kBiased = 0x20000000u;
+constexpr uint32_t kTimes = 0x1fffffffu;
 
 struct LogitsParams {
   cacheir_b200_logits_args a;
@@ -33,8 +33,8 @@ struct LogitsParams {
 };
 
 __device__ __forceinline__ bool aligned_to_16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-// Shared memory: marks [slice / 32], then, where tokens can be marked, their list [slice], (with a history or drafts) counts [slice], (with a bias) entries of it
-// [slice], (with drafts) the drafted tokens.
+// Shared memory: marks [slice / 32], then, where tokens can be marked, counts [slice], (with a bias) entries of it [slice], (with drafts) the drafted
+// tokens and what the rows see of them, and the list of marked tokens [slice].
 template <typename T, typename O, int VEC>
 __global__ void __launch_bounds__(kThreads, 4)
 adjust_logits_kernel(const LogitsParams p) {
@@ -42,20 +42,24 @@ adjust_logits_kernel(const LogitsParams p) {
   constexpr bool kWide = VEC > 1;
   chain_enter();
   extern __shared__ uint32_t smem[];
-  __shared__ int s_marked, s_drafted;
+  __shared__ int s_marked, s_drafted, s_seq[kRun];
   const cacheir_b200_logits_args& a = p.a;
   const int lo = blockIdx.x * p.slice, size = min(p.slice, a.vocab - lo), words = p.slice / 32;
-  const bool counting = a.history || a.draft_ids, biased = a.biases > 0;
+  const bool biased = a.biases > 0, counting = a.history || a.draft_ids || biased;
   uint32_t* marks = smem;
   uint32_t* counts = marks + words;
   int* entry = reinterpret_cast<int*>(counts + (counting ? p.slice : 0));
   uint32_t* drafted = reinterpret_cast<uint32_t*>(entry + (biased ? p.slice : 0));   // token of the slice << 16 | row of the sequence
-  uint16_t* marked = reinterpret_cast<uint16_t*>(drafted + (a.draft_ids ? 32 * a.words : 0));
-  const int last = min(a.rows, static_cast<int>(blockIdx.y + 1) * p.run), allowed_words = (a.vocab + 31) / 32;
-  auto sequence_of = [&](int row) {
-    const int seq = a.row_seq ? a.row_seq[row] : row;
-    return seq < a.sequences ? seq : -1;
-  };
+  uint32_t* sees = drafted + (a.draft_ids ? 32 * a.words : 0);                       // [rows of the block][words]
+  uint16_t* marked = reinterpret_cast<uint16_t*>(sees + (a.draft_ids ? p.run * a.words : 0));
+  const int begin = blockIdx.y * p.run, last = min(a.rows, begin + p.run), allowed_words = (a.vocab + 31) / 32;
+  if (static_cast<int>(threadIdx.x) < last - begin) {
+    const int seq = a.row_seq ? a.row_seq[begin + threadIdx.x] : begin + threadIdx.x;
+    s_seq[threadIdx.x] = seq < a.sequences ? seq : -1;
+  }
+  if (a.draft_ids)
+    for (int i = threadIdx.x; i < (last - begin) * a.words; i += kThreads) sees[i] = static_cast<uint32_t>(a.visible[static_cast<size_t>(begin) * a.words + i]);
+  __syncthreads();
   auto input = [&](int row) { return static_cast<const T*>(a.logits) + static_cast<size_t>(row) * a.row_stride + lo; };
   auto output = [&](int row) { return static_cast<O*>(a.out) + static_cast<size_t>(row) * a.out_stride + lo; };
   auto grammar = [&](int row) { return reinterpret_cast<const uint32_t*>(a.allowed) + static_cast<size_t>(row) * allowed_words + lo / 32; };
@@ -63,11 +67,11 @@ adjust_logits_kernel(const LogitsParams p) {
   auto skew_of = [&](const T* in) { return kWide ? static_cast<int>(reinterpret_cast<uintptr_t>(in) / sizeof(T) % VEC) : 0; };
   const bool same = a.logits == a.out;
 
-  for (int row0 = blockIdx.y * p.run; row0 < last;) {
-    const int seq = sequence_of(row0);
+  for (int row0 = begin; row0 < last;) {
+    const int seq = s_seq[row0 - begin];
     int end = row0 + 1;
     if (seq < 0) { row0 = end; continue; }
-    while (end < last && sequence_of(end) == seq) ++end;
+    while (end < last && s_seq[end - begin] == seq) ++end;
     // ---- the pass over the rows: values and bits of one are asked for while the one before is worked on (or tokens are counted) ----
     const bool pass = !same || a.allowed;
     uint4 ahead[kWide ? NV : 1];
@@ -88,11 +92,27 @@ adjust_logits_kernel(const LogitsParams p) {
       }
     };
     if (kWide && pass) ask(row0);
-    // ---- what the sequence has said ----
-    if (counting || biased) {
+    // ---- what the sequence has said (loads that do not depend on one another go out together) ----
+    float rep = 1.f, freq = 0.f, pres = 0.f;
+    if (counting) {
+      const int n = a.history ? min(a.history_lens[seq], a.history_width) : 0, prompt = a.history && a.prompt_lens ? a.prompt_lens[seq] : 0;
+      const int first = a.draft_ids ? min(max(a.cu_rows[seq], 0), a.rows) : 0;
+      const int drafts = a.draft_ids ? min(min(max(a.cu_rows[seq + 1], 0), a.rows) - first, 32 * a.words) : 0;
+      if (a.repetition) rep = a.repetition[seq];
+      if (a.frequency) freq = a.frequency[seq];
+      if (a.presence) pres = a.presence[seq];
+      const int32_t* said = a.history + static_cast<size_t>(seq) * a.history_width;
+      const size_t of_bias = static_cast<size_t>(seq) * a.biases;
+      int id[kSaid];
+#pragma unroll
+      for (int e = 0; e < kSaid; ++e) {
+        const int i = threadIdx.x + e * kThreads;
+        id[e] = a.history && i < a.history_width ? said[i] : -1;
+      }
+      const int bias_id = static_cast<int>(threadIdx.x) < a.biases ? a.bias_ids[of_bias + threadIdx.x] : -1;
       __syncthreads();
       for (int i = threadIdx.x; i < words; i += kThreads) marks[i] = 0;
-      if (counting) for (int i = threadIdx.x; i < p.slice; i += kThreads) counts[i] = 0;
+      for (int i = threadIdx.x; i < p.slice; i += kThreads) counts[i] = 0;
       if (biased) for (int i = threadIdx.x; i < p.slice; i += kThreads) entry[i] = 0;
       if (threadIdx.x == 0) s_marked = s_drafted = 0;
       __syncthreads();
@@ -100,37 +120,41 @@ adjust_logits_kernel(const LogitsParams p) {
         const uint32_t bit = 1u << (t & 31);
         if (!(atomicOr(&marks[t >> 5], bit) & bit)) marked[atomicAdd(&s_marked, 1)] = static_cast<uint16_t>(t);
       };
-      if (a.history) {
-        const int32_t* said = a.history + static_cast<size_t>(seq) * a.history_width;
-        const int n = min(a.history_lens[seq], a.history_width), prompt = a.prompt_lens ? a.prompt_lens[seq] : 0;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-          const int id = said[i];
-          const uint32_t t = static_cast<uint32_t>(id - lo);
-          if (id >= lo && t < static_cast<uint32_t>(size)) {
+      for (int i0 = threadIdx.x; i0 < n; i0 += kSaid * kThreads) {
+        int next[kSaid];
+#pragma unroll
+        for (int e = 0; e < kSaid; ++e) {
+          const int i = i0 + (kSaid + e) * kThreads;
+          next[e] = i < n ? said[i] : -1;
+        }
+#pragma unroll
+        for (int e = 0; e < kSaid; ++e) {
+          const int i = i0 + e * kThreads;
+          if (i < n && id[e] >= lo && id[e] - lo < size) {
+            const uint32_t t = static_cast<uint32_t>(id[e] - lo);
             if (i < prompt) atomicOr(&counts[t], kInPrompt);
             else atomicAdd(&counts[t], 1u);
             mark(t);
           }
         }
+#pragma unroll
+        for (int e = 0; e < kSaid; ++e) id[e] = next[e];
       }
-      for (int i = threadIdx.x; i < a.biases; i += kThreads) {
-        const int id = a.bias_ids[static_cast<size_t>(seq) * a.biases + i];
-        if (id >= lo && id - lo < size) {
-          atomicMax(&entry[id - lo], i + 1);
-          mark(id - lo);
+      for (int j = threadIdx.x; j < drafts; j += kThreads) {
+        const int64_t token = a.draft_ids[first + j];
+        if (token >= lo && token - lo < size) {
+          const uint32_t t = static_cast<uint32_t>(token - lo);
+          drafted[atomicAdd(&s_drafted, 1)] = t << 16 | static_cast<uint32_t>(j);
+          atomicOr(&counts[t], kDrafted);
+          mark(t);
         }
       }
-      if (a.draft_ids) {
-        const int first = min(max(a.cu_rows[seq], 0), a.rows), n = min(min(max(a.cu_rows[seq + 1], 0), a.rows) - first, 32 * a.words);
-        for (int j = threadIdx.x; j < n; j += kThreads) {
-          const int64_t id = a.draft_ids[first + j];
-          if (id >= lo && id - lo < size) {
-            const uint32_t t = static_cast<uint32_t>(id - lo);
-            drafted[atomicAdd(&s_drafted, 1)] = t << 16 | static_cast<uint32_t>(j);
-            atomicOr(&counts[t], kDrafted);
-            mark(t);
-          }
+      for (int i = threadIdx.x; i < a.biases; i += kThreads) {
+        const int token = i < kThreads ? bias_id : a.bias_ids[of_bias + i];
+        if (token >= lo && token - lo < size) {
+          atomicMax(&entry[token - lo], i + 1);
+          atomicOr(&counts[token - lo], kBiased);
+          mark(token - lo);
         }
       }
     }
@@ -181,13 +205,13 @@ adjust_logits_kernel(const LogitsParams p) {
       }
     }
     // ---- tokens that were said, are drafted or have a bias ----
-    if (counting || biased) {
+    if (counting) {
       __syncthreads();
       const int many = s_drafted, rows = end - row0, pairs = s_marked * rows;
-      const float rep = a.repetition ? a.repetition[seq] : 1.f, freq = a.frequency ? a.frequency[seq] : 0.f, pres = a.presence ? a.presence[seq] : 0.f;
       for (int i0 = threadIdx.x; i0 < pairs; i0 += kPairs * kThreads) {
         T value[kPairs];
         uint32_t may[kPairs];
+        float bias[kPairs];
         int token[kPairs], at[kPairs];
 #pragma unroll
         for (int e = 0; e < kPairs; ++e) {                     // (asked for together)
@@ -196,28 +220,23 @@ adjust_logits_kernel(const LogitsParams p) {
           at[e] = row0 + i - k * rows;
           value[e] = input(at[e])[token[e]];
           may[e] = a.allowed ? grammar(at[e])[token[e] >> 5] : 0xffffffffu;
+          bias[e] = counts[token[e]] & kBiased ? a.bias_values[static_cast<size_t>(seq) * a.biases + entry[token[e]] - 1] : 0.f;
         }
-#pragma unroll 1
-        for (int e = 0; e < kPairs; ++e) {
-          int t = token[0], row = at[0];
-          T raw = value[0];
-          uint32_t word = may[0];
 #pragma unroll
-          for (int f = 1; f < kPairs; ++f)
-            if (e == f) { t = token[f]; row = at[f]; raw = value[f]; word = may[f]; }
-          if (i0 + e * kThreads >= pairs || !(word >> (t & 31) & 1)) continue;
-          float x = Elem<T>::ld(&raw);
-          const uint32_t c = counting ? counts[t] : 0u;
+        for (int e = 0; e < kPairs; ++e) {
+          const int t = token[e], row = at[e];
+          if (i0 + e * kThreads >= pairs || !(may[e] >> (t & 31) & 1)) continue;
+          float x = Elem<T>::ld(&value[e]);
+          const uint32_t c = counts[t];
           uint32_t times = c & kTimes;
           if (c & kDrafted)
             for (int d = 0; d < many; ++d) {
               const uint32_t v = drafted[d], j = v & 0xffffu;
-              if (v >> 16 == static_cast<uint32_t>(t)) times += a.visible[static_cast<size_t>(row) * a.words + (j >> 5)] >> (j & 31) & 1;
+              if (v >> 16 == static_cast<uint32_t>(t)) times += sees[(row - begin) * a.words + (j >> 5)] >> (j & 31) & 1;
             }
           if (times || (c & kInPrompt)) x = x > 0.f ? __fdiv_rn(x, rep) : x * rep;
           if (times) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, static_cast<float>(times))), pres);
-          const int entry_of = biased ? entry[t] : 0;
-          if (entry_of) x = __fadd_rn(x, a.bias_values[static_cast<size_t>(seq) * a.biases + entry_of - 1]);
+          if (c & kBiased) x = __fadd_rn(x, bias[e]);
           Elem<O>::st(output(row) + t, x);
         }
       }
@@ -233,11 +252,12 @@ int launch_adjust(const cacheir_b200_logits_args& a, cudaStream_t stream) {
   LogitsParams p{a, kSlice, 1};
   while (p.slice > 1024 && static_cast<long long>(a.rows) * ((a.vocab + p.slice - 1) / p.slice) < 4 * kNumSMs) p.slice /= 2;
   const int slices = (a.vocab + p.slice - 1) / p.slice;
-  while (p.run < RUN && static_cast<long long>(a.rows) * slices >= 12LL * p.run * kNumSMs) p.run *= 2;
-  const int runs = (a.rows + p.run - 1) / p.run;
-  if (runs > 65535) p.run = (a.rows + 65534) / 65535;
-  const bool counting = a.history || a.draft_ids;
-  const size_t smem = (p.slice / 32 + (counting ? p.slice : 0) + (a.biases > 0 ? p.slice : 0) + (a.draft_ids ? 32 * a.words : 0)) * sizeof(uint32_t) + p.slice * sizeof(uint16_t);
+  while (p.run < kRun && static_cast<long long>(a.rows) * slices >= 6LL * p.run * kNumSMs) p.run *= 2;
+  if (a.rows > kRun * 65535LL) return CACHEIR_B200_ELIMIT;
+  if (a.rows > 65535) p.run = kRun;
+  const bool counting = a.history || a.draft_ids || a.biases > 0;
+  const size_t smem = (p.slice / 32 + (counting ? p.slice : 0) + (a.biases > 0 ? p.slice : 0) + (a.draft_ids ? (32 + p.run) * a.words : 0)) * sizeof(uint32_t) +
+                      p.slice * sizeof(uint16_t);
   // vectors where a row's input and output begin at the same place of 16 bytes (with outputs of the same size)
   const bool wide = reinterpret_cast<uintptr_t>(a.logits) % sizeof(T) == 0 &&
                     (sizeof(T) != sizeof(O) || ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.out)) % 16 == 0 &&
@@ -245,7 +265,7 @@ int launch_adjust(const cacheir_b200_logits_args& a, cudaStream_t stream) {
   auto kern = wide ? adjust_logits_kernel<T, O, VEC> : adjust_logits_kernel<T, O, 1>;
   const dim3 grid(slices, (a.rows + p.run - 1) / p.run);
   static std::atomic<unsigned long long> done_wide{0}, done_any{0};
-  constexpr int most = (kSlice / 32 + 2 * kSlice + 32 * CACHEIR_B200_MAX_DRAFT_WORDS) * 4 + kSlice * 2;
+  constexpr int most = (kSlice / 32 + 2 * kSlice + (32 + kRun) * CACHEIR_B200_MAX_DRAFT_WORDS) * 4 + kSlice * 2;
   cudaError_t e = allow_shared_memory(wide ? done_wide : done_any, reinterpret_cast<const void*>(kern), most);
   if (e == cudaSuccess) e = launch_chained(kern, grid, dim3(kThreads), smem, stream, p);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
@@ -267,7 +287,7 @@ extern "C" int cacheir_b200_adjust_logits(const cacheir_b200_logits_args* args, 
       (a.draft_ids && (!a.cu_rows || !a.visible || a.words <= 0)) || (a.biases > 0 && (!a.bias_ids || !a.bias_values)))
     return CACHEIR_B200_EINVAL;
   if (a.logits == a.out && a.dtype != a.out_dtype) return CACHEIR_B200_EINVAL;
-  if (a.vocab > 1 << 28 || a.history_width > 1 << 29 || (a.draft_ids && a.words > CACHEIR_B200_MAX_DRAFT_WORDS)) return CACHEIR_B200_ELIMIT;
+  if (a.vocab > 1 << 28 || a.history_width >= 1 << 29 || (a.draft_ids && a.words > CACHEIR_B200_MAX_DRAFT_WORDS)) return CACHEIR_B200_ELIMIT;
   if (a.biases == 0) a.bias_ids = nullptr;
   if (a.dtype == CACHEIR_B200_F32) return launch_adjust<float, float>(a, as_stream(stream));
   if (a.dtype == CACHEIR_B200_F16)

@@ -33,7 +33,6 @@ constexpr int kRows = 128;                     // query rows of a group of warps
 constexpr int kThreads = 384;
 constexpr int kMaxHeadsPerKv = 64;
 constexpr int kPlanThreads = 128;              // that lay the plan out, some sequences each
-constexpr int kJoinRows = 16;                  // query rows of a joining block
 constexpr float kAhead = 6.f;                  // a new reference is the maximum less this: probabilities start at 2^6 ..
 constexpr float kStale = 14.f;                 // .. and may grow to 2^14 (in fp16: 2^-24 of that is still a number)
 
@@ -156,17 +155,25 @@ struct Walk {
   }
 };
 
+// What the warps other than the keys' need to know of an item.
+struct Item {
+  TreeSequence s;
+  int b, row0, rows, kvh;
+  int tile, tiles, keys;       // (tiles 0: there are no more items)
+  int flags;                   // 1: begins here, 2: ends here
+};
+constexpr int kItems = 8;      // in shared memory: the keys' warp, which goes through them, is up to six ahead of the softmax
+
 template <int D>
 struct Smem {
   static constexpr int kSlotBytes = kKeys * D * 2;
   static constexpr int kSlots = D == 128 ? 5 : 10;
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kTiles = 2 * kQBytes + kSlots * kSlotBytes;
-  // then: barriers of keys, of values, empty, clean [slots], q[2], place of q[2], s[2], p[2][2], o[2], end[3]; tensor memory address; starts of runs
-  static constexpr int kBarriers = 4 * kSlots + 15;
-  static constexpr int kBytes = 1024 + kTiles + kBarriers * 8 + 16 + (kPlanThreads + 1) * 4;
+  // then: barriers of keys, of values, empty, clean [slots], q[2], place of q[2], s[2], p[2][2], o[2], end[3], items; tensor memory address; items; starts of runs
+  static constexpr int kBarriers = 4 * kSlots + 15 + kItems;
+  static constexpr int kBytes = 1024 + kTiles + kBarriers * 8 + 16 + kItems * static_cast<int>(sizeof(Item)) + kPlanThreads * 4;
 };
-constexpr int kSpoilt = 8;                     // items that a flag of spoilt values may be set ahead
 
 // Where a column of a lane's line of 32 lies in shared memory: lanes that read the same one reach different banks.
 __device__ __forceinline__ int staged(int lane, int column) { return lane * 32 + (((column >> 2) ^ (lane & 7)) << 2) + (column & 3); }
@@ -220,10 +227,12 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
   uint64_t* bar_p = bar_s + 2;                                 // probabilities are, [group of warps][first keys, the others]
   uint64_t* bar_o = bar_p + 4;                                 // .. and have been added to the output
   uint64_t* bar_end = bar_o + 2;                               // steps of an item's end that both groups of warps have made
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_end + 3);
-  int* s_start = reinterpret_cast<int*>(tmem_slot + 4);
+  uint64_t* bar_item = bar_end + 3;                            // the item is known
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_item + kItems);
+  Item* s_item = reinterpret_cast<Item*>(tmem_slot + 4);
+  int* s_start = reinterpret_cast<int*>(s_item + kItems);
   __shared__ int s_scan[kPlanThreads / 32];
-  __shared__ volatile int s_spoilt[kSpoilt];
+  __shared__ volatile int s_spoilt[kItems];                    // the last item of this place some of whose values are no numbers
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const cacheir_b200_tree_args& a = p.a;
 
@@ -246,9 +255,10 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
       mbar_init(smem_u32(&bar_o[w]), 1);
     }
     for (int i = 0; i < 3; ++i) mbar_init(smem_u32(&bar_end[i]), 8);
+    for (int i = 0; i < kItems; ++i) mbar_init(smem_u32(&bar_item[i]), 1);
     mbar_fence_init();
   }
-  if (threadIdx.x >= 256 && threadIdx.x < 256 + kSpoilt) s_spoilt[threadIdx.x - 256] = 0;
+  if (threadIdx.x >= 256 && threadIdx.x < 256 + kItems) s_spoilt[threadIdx.x - 256] = 0;
   chain_enter();
   if (warp == 8) tc_alloc(smem_u32(tmem_slot), 512);           // (beside the loads of the plan)
   // ---- the plan: units of runs of sequences, a thread each ----
@@ -279,30 +289,36 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
   const uint32_t tmem_o = tmem + 2 * kKeys;
   const int group = a.heads / a.kv_heads, half_rows = p.half_rows;
   const int ctas = max(1, min(total, static_cast<int>(gridDim.x)));
-  const bool takes_part = static_cast<int>(blockIdx.x) < min(ctas, total);
-  Walk walk(a, tile_rows, s_start, run, max(total, 1), ctas);
-  if (!takes_part) walk.end = walk.at;
   bool ok = true;
+  Item it;
+  int item = 0;                                                // of the block, counted from 1
+  auto next_item = [&] {
+    const int place = item % kItems;
+    ok = ok && warp_wait(smem_u32(&bar_item[place]), (item / kItems) & 1, (15 << 8) | 14);
+    if (!ok) return false;
+    it = s_item[place];
+    ++item;
+    return it.tiles > 0;
+  };
 
   if (warp == 11) {
     // ------- values: those of drafted tokens are looked through, those behind the last key cleared -------
     constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
     constexpr int kLanes = D / 8;                              // of a key's values
-    int slot = 1, item = 0, turn = 0;
+    int slot = 1, turn = 0;
     uint32_t phase = 0;
-    while (ok && walk.next()) {
-      ++item;
-      for (int t = walk.tile; t < walk.tile + walk.tiles && ok; ++t) {
+    while (next_item()) {
+      for (int t = it.tile; t < it.tile + it.tiles && ok; ++t) {
         ok = warp_wait(smem_u32(&value_full[turn]), phase, (15 << 8) | 12);
         if (!ok) break;
-        const int base = t * kKeys, from = max(min(walk.s.front, walk.keys) - base, 0);
+        const int base = t * kKeys, from = max(min(it.s.front, it.keys) - base, 0);
         if (from < kKeys) {
           bool spoilt = false;
           for (int key = from + lane / kLanes; key < kKeys; key += 32 / kLanes) {
             const int c = lane % kLanes;
             uint4* at = reinterpret_cast<uint4*>(s_kv + slot * L::kSlotBytes + (key / kChunk) * kChunk * D * 2 + (c >> 3) * kChunk * 128 + key % kChunk * 128 +
                                                  ((c & 7) << 4));
-            if (base + key >= walk.keys) {
+            if (base + key >= it.keys) {
               *at = make_uint4(0u, 0u, 0u, 0u);
               continue;
             }
@@ -314,7 +330,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
               *at = make_uint4(v.x & ~bad[0], v.y & ~bad[1], v.z & ~bad[2], v.w & ~bad[3]);
             }
           }
-          if (__any_sync(0xffffffffu, spoilt) && lane == 0) s_spoilt[item % kSpoilt] = item;
+          if (__any_sync(0xffffffffu, spoilt) && lane == 0) s_spoilt[item % kItems] = item;
           fence_async_smem();
           __threadfence_block();
         }
@@ -336,34 +352,15 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
     uint64_t* full = keys ? key_full : value_full;
     int slot = keys ? 0 : 1, turn = 0, q_place = 0;
     uint32_t phase = 1, sent = 0, q_phase = 3;                 // (slots of a tile: its keys', its values'; q_phase: a bit for either place)
-    while (ok && walk.next()) {
-      const int32_t* pages = a.page_table + static_cast<size_t>(walk.b) * a.max_pages;
-      auto line_of = [&](int tile) {                           // first row of this lane's 16 in the pool
-        const int key = tile * kKeys + chunk * kChunk;
-        if (!copies || key >= walk.keys) return outside;
-        const int page = by_page.of(key), id = pages[page];
-        return id >= 0 && id < a.num_slots ? (id * a.kv_heads + walk.kvh) * a.page_size + key - page * a.page_size : outside;
-      };
-      int line = line_of(walk.tile);
-      if (!keys) {                                             // the item's queries: rows, heads, 64 columns at a time
-        const bool two = walk.rows > half_rows;
-        for (int w = 0; w < (two ? 2 : 1) && ok; ++w) {
-          const int place = two ? w : q_place;
-          ok = warp_wait(smem_u32(&bar_free[place]), q_phase >> place & 1, (15 << 8) | 7);
-          if (!ok) break;
-          q_phase ^= 1u << place;
-          if (lane == 0) {
-            mbar_expect_tx(smem_u32(&bar_q[place]), (D / 64) * half_rows * group * 128);
-            for (int z = 0; z < D / 64; ++z)
-              tma_load_4d(smem_u32(s_q + place * L::kQBytes + z * kRows * 128), &tmap_q, smem_u32(&bar_q[place]), 0, walk.kvh * group,
-                          walk.s.row + walk.row0 + w * half_rows, z);
-          }
-          __syncwarp();
-        }
-        if (!two) q_place ^= 1;
-      }
-      for (int t = walk.tile; t < walk.tile + walk.tiles && ok; ++t) {
-        const int next = t + 1 < walk.tile + walk.tiles ? line_of(t + 1) : 0;
+    auto line_of = [&](int tile) {                             // first row of this lane's 16 in the pool
+      const int key = tile * kKeys + chunk * kChunk;
+      if (!copies || key >= it.keys) return outside;
+      const int page = by_page.of(key), id = a.page_table[static_cast<size_t>(it.b) * a.max_pages + page];
+      return id >= 0 && id < a.num_slots ? (id * a.kv_heads + it.kvh) * a.page_size + key - page * a.page_size : outside;
+    };
+    auto copy_tiles = [&](int line) {
+      for (int t = it.tile; t < it.tile + it.tiles && ok; ++t) {
+        const int next = t + 1 < it.tile + it.tiles ? line_of(t + 1) : 0;
         ok = warp_wait(smem_u32(&empty[slot]), phase, (15 << 8) | 1);
         if (!ok) break;
         if (lane == 0) mbar_expect_tx(smem_u32(&full[turn]), L::kSlotBytes);
@@ -377,6 +374,45 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
         if (slot >= kSlots) { slot -= kSlots; phase ^= 1; }
         turn = turn + 1 == kSlots ? 0 : turn + 1;
         line = next;
+      }
+    };
+    if (keys) {                                                // this warp goes through the block's share and says what the items are
+      Walk walk(a, tile_rows, s_start, run, max(total, 1), ctas);
+      if (static_cast<int>(blockIdx.x) >= min(ctas, total)) walk.end = walk.at;
+      TreeJoin join{};
+      bool more = true;
+      while (ok && more) {
+        more = walk.next();
+        it = Item{walk.s, walk.b, walk.row0, walk.rows, walk.kvh, walk.tile, more ? walk.tiles : 0, walk.keys, (walk.begins ? 1 : 0) | (walk.ends ? 2 : 0)};
+        if (lane == 0) {
+          s_item[item % kItems] = it;
+          mbar_arrive(smem_u32(&bar_item[item % kItems]));
+        }
+        ++item;
+        if (!more) break;
+        if (walk.ends && !walk.begins) join = TreeJoin{walk.s.row + walk.row0, walk.rows, walk.kvh, walk.first};
+        copy_tiles(line_of(it.tile));
+      }
+      if (lane == 0) p.joins[blockIdx.x] = join;
+    } else {
+      while (next_item()) {
+        const int line = line_of(it.tile);
+        const bool two = it.rows > half_rows;                  // the item's queries: rows, heads, 64 columns at a time
+        for (int w = 0; w < (two ? 2 : 1) && ok; ++w) {
+          const int place = two ? w : q_place;
+          ok = warp_wait(smem_u32(&bar_free[place]), q_phase >> place & 1, (15 << 8) | 7);
+          if (!ok) break;
+          q_phase ^= 1u << place;
+          if (lane == 0) {
+            mbar_expect_tx(smem_u32(&bar_q[place]), (D / 64) * half_rows * group * 128);
+            for (int z = 0; z < D / 64; ++z)
+              tma_load_4d(smem_u32(s_q + place * L::kQBytes + z * kRows * 128), &tmap_q, smem_u32(&bar_q[place]), 0, it.kvh * group,
+                          it.s.row + it.row0 + w * half_rows, z);
+          }
+          __syncwarp();
+        }
+        if (!two) q_place ^= 1;
+        copy_tiles(line);
       }
     }
     // nothing may still be on its way when the block ends, also after a wait that gave up
@@ -397,9 +433,9 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
     const bool leader = elect_one();
     int k_slot = 0, v_slot = 1, k_turn = 0, v_turn = 0, q_place = 0;    // slots; barriers; place of the queries of an item that both groups share
     uint32_t k_phase = 0, v_phase = 0, q_phase = 0, p_phase = 0;    // (of the two buffers of queries and probabilities: a bit each)
-    while (ok && walk.next()) {
-      const bool two = walk.rows > half_rows;
-      const int steps = two ? 2 * walk.tiles : walk.tiles;
+    while (next_item()) {
+      const bool two = it.rows > half_rows;
+      const int steps = two ? 2 * it.tiles : it.tiles;
       auto wait_scores = [&](int j) {                          // the operands of step j's scores
         if (j < (two ? 2 : 1)) {                               // the item's queries are new
           const int w = two ? j : q_place;
@@ -477,32 +513,30 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
     const int by_group = (65536 + group - 1) / group;          // n / group = n * by_group >> 16 for n < 256, group <= 64
     const int token = r * by_group >> 16, head_of = r - token * group;
     uint32_t s_phase = 0, o_phase = 0, end_phase = 0;
-    int q_place = 0, item = 0;                                 // where the queries of an item that both groups share are
-    TreeJoin join{};
-    while (ok && walk.next()) {
-      ++item;
-      const bool two = walk.rows > half_rows;
+    int q_place = 0;                                           // where the queries of an item that both groups share are
+    while (next_item()) {
+      const bool two = it.rows > half_rows;
       const int place = two ? w : q_place;
       if (!two) q_place ^= 1;
       const int in_item = (two ? w * half_rows : 0) + token;   // this thread's token of the item
-      const bool real = r < half_rows * group && in_item < walk.rows;
-      const int row = walk.row0 + (real ? in_item : 0), head = walk.kvh * group + head_of;
-      const int masked_from = min(walk.s.front, walk.keys);    // keys behind this need a look at the row's mask
+      const bool real = r < half_rows * group && in_item < it.rows;
+      const int row = it.row0 + (real ? in_item : 0), head = it.kvh * group + head_of;
+      const int masked_from = min(it.s.front, it.keys);    // keys behind this need a look at the row's mask
       float m_ref = -INFINITY, l_run = 0.f;
       int steps = 0;
-      for (int t = two ? 0 : w; t < walk.tiles && ok; t += two ? 1 : 2, ++steps) {
-        const int base = (walk.tile + t) * kKeys;
+      for (int t = two ? 0 : w; t < it.tiles && ok; t += two ? 1 : 2, ++steps) {
+        const int base = (it.tile + t) * kKeys;
         const bool whole = base + kKeys <= masked_from;
         uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
         if (!whole) {                                          // 128 bits of the row, from the tile's first key on
-          const int from = base - walk.s.front, sh = from & 31;
-          uint32_t low = tree_word(a, walk.s, row, from >> 5);
+          const int from = base - it.s.front, sh = from & 31;
+          uint32_t low = tree_word(a, it.s, row, from >> 5);
           if (from >> 5 < 0) low = 0xffffffffu;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int q = (from >> 5) + i + 1;
-            const uint32_t high = q < 0 ? 0xffffffffu : tree_word(a, walk.s, row, q);
-            const int left = walk.keys - base - 32 * i;        // keys there are from this word on
+            const uint32_t high = q < 0 ? 0xffffffffu : tree_word(a, it.s, row, q);
+            const int left = it.keys - base - 32 * i;        // keys there are from this word on
             see[i] = __funnelshift_r(low, high, sh) & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
             low = high;
           }
@@ -625,7 +659,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
         if (steps > 0) s_ml[w * kRows + r] = make_float2(m_ref, l_run);
         ok = together(0);
         if (!ok) break;
-        const float2 other = w == 1 || walk.tiles > 1 ? s_ml[(w ^ 1) * kRows + r] : make_float2(-INFINITY, 0.f);
+        const float2 other = w == 1 || it.tiles > 1 ? s_ml[(w ^ 1) * kRows + r] : make_float2(-INFINITY, 0.f);
         ok = together(1);
         if (!ok) break;
         const float m = fmaxf(m_ref, other.x);
@@ -635,20 +669,28 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
         l_run = l_run * (m_ref > -INFINITY ? f_own : 1.f) + other.y * (other.x > -INFINITY ? f_other : 1.f);
         m_ref = m;
       }
-      const bool direct = walk.begins && walk.ends, spoilt = s_spoilt[item % kSpoilt] == item;
-      const int slot = 2 * blockIdx.x + (walk.begins ? 1 : 0), in_slot = (two ? w : 0) * kRows + r;
+      const bool direct = it.flags == 3, spoilt = s_spoilt[item % kItems] == item;
+      const int slot = 2 * blockIdx.x + (it.flags & 1), in_slot = (two ? w : 0) * kRows + r;
       if (!direct && real && (two || w == 0)) *reinterpret_cast<float2*>(p.ml + (static_cast<size_t>(slot) * 2 * kRows + in_slot) * 2) = make_float2(m_ref, l_run);
       const float scale = direct ? (l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f) : 1.f;
       f_own *= scale;
       f_other *= scale;
-      // a row's place in out, or in the scratch (-1: none)
-      const long long to_row = !real ? -1LL : direct ? static_cast<long long>(walk.s.row + row) * a.out_stride + static_cast<long long>(head) * D
-                                                     : (static_cast<long long>(slot) * 2 * kRows + in_slot) * D;
       // By way of shared memory (the queries' place), so that a store writes whole lines: a lane has a row, a store 32 columns of four rows.
       // (4 KB a warp: with heads of 64 the place has room for one group of warps, which then stores all columns)
       constexpr bool kHalves = L::kQBytes >= 8 * 4096;
       float* s_row = reinterpret_cast<float*>(s_place + (two || !kHalves ? warp & 3 : warp) * 4096);
       const int c_begin = two ? 0 : kHalves ? w * (D / 2) : w * D, c_end = two || !kHalves ? D : c_begin + D / 2;
+      const size_t scratch_row = static_cast<size_t>(slot) * 2 * kRows + (two ? w : 0) * kRows;
+      // element at which a row of this warp (its four rows of every store: 4 i + lane / 8) begins in out, or in the scratch; -1: it is none
+      auto begin_of = [&](int in_warp) {
+        const int r2 = (warp & 3) * 32 + in_warp, token2 = r2 * by_group >> 16, in2 = (two ? w * half_rows : 0) + token2;
+        if (r2 >= half_rows * group || in2 >= it.rows) return -1LL;
+        return direct ? static_cast<long long>(it.s.row + it.row0 + in2) * a.out_stride + static_cast<long long>(it.kvh * group + r2 - token2 * group) * D
+                      : static_cast<long long>((scratch_row + r2) * D);
+      };
+      long long to[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) to[i] = begin_of(4 * i + (lane >> 3));
 #pragma unroll 1
       for (int c = c_begin; c < c_end; c += 32) {
         uint32_t x[32];
@@ -672,37 +714,39 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
         for (int i = 0; i < 8; ++i)
           *reinterpret_cast<float4*>(s_row + staged(lane, 4 * i)) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         __syncwarp();
+        float4 v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int from = 4 * i + (lane >> 3);
-          const long long to = __shfl_sync(0xffffffffu, to_row, from);
-          const float4 v = *reinterpret_cast<const float4*>(s_row + staged(from, (lane & 7) * 4));
-          if (to >= 0) {
-            const size_t at = static_cast<size_t>(to) + c + (lane & 7) * 4;
-            if (direct) *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at) = make_uint2(pack_pair<T>(v.x, v.y), pack_pair<T>(v.z, v.w));
-            else *reinterpret_cast<float4*>(p.acc + at) = v;
-          }
-        }
+        for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const float4*>(s_row + staged(4 * i + (lane >> 3), (lane & 7) * 4));
         __syncwarp();
+        const int column = c + (lane & 7) * 4;
+        if (direct) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (to[i] >= 0) *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + to[i] + column) = make_uint2(pack_pair<T>(v[i].x, v[i].y), pack_pair<T>(v[i].z, v[i].w));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (to[i] >= 0) *reinterpret_cast<float4*>(p.acc + to[i] + column) = v[i];
+        }
       }
+      __syncwarp();
       if (spoilt && real) {
-        const int32_t* pages = a.page_table + static_cast<size_t>(walk.b) * a.max_pages;
-        if (direct) add_spoilt<T, D, T>(a, walk.s, pages, row, head, walk.tile, walk.tiles, walk.keys, c_begin, c_end, static_cast<T*>(a.out) + to_row);
-        else add_spoilt<T, D, float>(a, walk.s, pages, row, head, walk.tile, walk.tiles, walk.keys, c_begin, c_end, p.acc + to_row);
+        const long long to_row = begin_of(lane);
+        const int32_t* pages = a.page_table + static_cast<size_t>(it.b) * a.max_pages;
+        if (direct) add_spoilt<T, D, T>(a, it.s, pages, row, head, it.tile, it.tiles, it.keys, c_begin, c_end, static_cast<T*>(a.out) + to_row);
+        else add_spoilt<T, D, float>(a, it.s, pages, row, head, it.tile, it.tiles, it.keys, c_begin, c_end, p.acc + to_row);
       }
       if (!two) {                                              // (the outputs may be written over)
         ok = together(2);
         if (!ok) break;
         end_phase ^= 1;
       }
-      if (walk.ends && !walk.begins) join = TreeJoin{walk.s.row + walk.row0, walk.rows, walk.kvh, walk.first};
       tc_fence_before();
       fence_async_smem();                                      // (the next queries come by copies)
       __syncwarp();
       if (two) { if (lane < 2) mbar_arrive(smem_u32(&bar_free[place])); }
       else if (lane == 0) mbar_arrive(smem_u32(&bar_free[place]));
     }
-    if (threadIdx.x == 0) p.joins[blockIdx.x] = join;
   }
   __syncwarp();
   tc_fence_before();
@@ -714,62 +758,77 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
 }
 
 // ---- the pieces of items that were cut ----
-// A block per (block of the first kernel, kJoinRows of its item's query rows), a warp per two rows, pieces in their order.
+// A block per (block of the first kernel, group of warps of its item), a warp per eight query rows, pieces in their order. (16 blocks of two rows a warp each,
+// most of which had nothing to do, took 13 us behind 32 trees where these take 5.)
+constexpr int kJoinThreads = 512;
+constexpr int kJoinPieces = 16;                // weights that lie in shared memory at a time
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinRows * 16)
+__global__ void __launch_bounds__(kJoinThreads)
 tree_pieces_kernel(const FastParams p) {
   chain_enter();
+  __shared__ float s_max[kRows], s_scale[kRows], s_weight[kJoinPieces][kRows];
   const TreeJoin j = p.joins[blockIdx.x];
-  if (j.rows <= 0) return;
+  if (j.rows <= static_cast<int>(blockIdx.y) * p.half_rows) return;
   const cacheir_b200_tree_args& a = p.a;
-  const int group = a.heads / a.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kLanes = D / 4;                // of a row
-  const int n = static_cast<int>(blockIdx.x) - j.first + 1;
+  const int group = a.heads / a.kv_heads, n = static_cast<int>(blockIdx.x) - j.first + 1;
+  const int rows = min(p.half_rows, j.rows - static_cast<int>(blockIdx.y) * p.half_rows) * group;       // query rows that there are
+  auto slot_of = [&](int i) { return 2 * (j.first + i) + (i == 0 ? 1 : 0); };
+  auto place_of = [&](int i, int r) { return static_cast<size_t>(slot_of(i)) * 2 * kRows + blockIdx.y * kRows + r; };
+  if (static_cast<int>(threadIdx.x) < rows) {
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) m = fmaxf(m, p.ml[2 * place_of(i, threadIdx.x)]);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float2 v = *reinterpret_cast<const float2*>(p.ml + 2 * place_of(i, threadIdx.x));
+      l += v.y * (v.x > -INFINITY ? exp2f(v.x - m) : 1.f);     // (a piece whose keys all scored -inf has a sum of 0, or of NaN, which stays)
+    }
+    s_max[threadIdx.x] = m;
+    s_scale[threadIdx.x] = l > 0.f || l != l ? 1.f / l : 0.f;
+  }
+  constexpr int kLanes = D / 4, kTogether = kRows * kLanes / kJoinThreads;       // lanes of a row; rows of a thread
+  const int c = threadIdx.x % kLanes * 4, first = threadIdx.x / kLanes;
+  float4 o[kTogether] = {};
+  for (int i0 = 0; i0 < n; i0 += kJoinPieces) {
+    const int pieces = min(kJoinPieces, n - i0);
+    __syncthreads();
+    for (int e = threadIdx.x; e < pieces * kRows; e += kJoinThreads) {
+      const int r = e % kRows, i = e / kRows;
+      if (r >= rows) continue;
+      const float x = p.ml[2 * place_of(i0 + i, r)];
+      s_weight[i][r] = x > -INFINITY ? exp2f(x - s_max[r]) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll 2
+    for (int i = 0; i < pieces; ++i) {
+      float4 v[kTogether];
+      float f[kTogether];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int place = blockIdx.y * kJoinRows + warp * 2 + e, r = place & (kRows - 1);
-    const int token = (place >> 7) * p.half_rows + r / group, head = r % group;
-    if (r >= p.half_rows * group || token >= j.rows) continue;
-    auto slot_of = [&](int i) { return 2 * (j.first + i) + (i == 0 ? 1 : 0); };
-    float m = -INFINITY, l = 0.f, f_last = 0.f;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const float2 v = i0 + lane < n ? *reinterpret_cast<const float2*>(p.ml + (static_cast<size_t>(slot_of(i0 + lane)) * 2 * kRows + place) * 2) : make_float2(-INFINITY, 0.f);
-      const float m_new = fmaxf(m, warp_max(v.x));
-      f_last = v.x > -INFINITY ? exp2f(v.x - m_new) : 0.f;
-      l = l * (m > -INFINITY ? exp2f(m - m_new) : 1.f) + warp_sum(v.y * (v.x > -INFINITY ? f_last : 1.f));
-      m = m_new;
-    }
-    const float scale = l > 0.f || l != l ? 1.f / l : 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int c = lane % kLanes * 4, part = lane / kLanes;                       // (lanes beside one another add up other pieces where a row has less than 32 of them)
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      float f = f_last;
-      if (n > 32) {                                                                // (weights of more than one round are worked out again)
-        const float x = i0 + lane < n ? p.ml[(static_cast<size_t>(slot_of(i0 + lane)) * 2 * kRows + place) * 2] : -INFINITY;
-        f = x > -INFINITY ? exp2f(x - m) : 0.f;
+      for (int e = 0; e < kTogether; ++e) {
+        const int r = first + e * (kRows / kTogether);
+        f[e] = r < rows ? s_weight[i][r] : 0.f;
+        if (f[e] != 0.f) v[e] = *reinterpret_cast<const float4*>(p.acc + place_of(i0 + i, r) * D + c);
       }
-#pragma unroll 4
-      for (int i = part; i < 32; i += 32 / kLanes) {
-        const float fi = __shfl_sync(0xffffffffu, f, i);
-        if (i0 + i < n && fi != 0.f) {
-          const float4 v = *reinterpret_cast<const float4*>(p.acc + (static_cast<size_t>(slot_of(i0 + i)) * 2 * kRows + place) * D + c);
-          o.x = fmaf(v.x, fi, o.x);
-          o.y = fmaf(v.y, fi, o.y);
-          o.z = fmaf(v.z, fi, o.z);
-          o.w = fmaf(v.w, fi, o.w);
+#pragma unroll
+      for (int e = 0; e < kTogether; ++e)
+        if (f[e] != 0.f) {
+          o[e].x = fmaf(v[e].x, f[e], o[e].x);
+          o[e].y = fmaf(v[e].y, f[e], o[e].y);
+          o[e].z = fmaf(v[e].z, f[e], o[e].z);
+          o[e].w = fmaf(v[e].w, f[e], o[e].w);
         }
-      }
     }
-    if (kLanes < 32) {
-      o.x += __shfl_xor_sync(0xffffffffu, o.x, 16);
-      o.y += __shfl_xor_sync(0xffffffffu, o.y, 16);
-      o.z += __shfl_xor_sync(0xffffffffu, o.z, 16);
-      o.w += __shfl_xor_sync(0xffffffffu, o.w, 16);
-    }
-    if (l != l) o = make_float4(l, l, l, l);
-    if (part == 0)
-      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<size_t>(j.row + token) * a.out_stride + static_cast<size_t>(j.kvh * group + head) * D + c) =
-          make_uint2(pack_pair<T>(o.x * scale, o.y * scale), pack_pair<T>(o.z * scale, o.w * scale));
+  }
+#pragma unroll
+  for (int e = 0; e < kTogether; ++e) {
+    const int r = first + e * (kRows / kTogether);
+    if (r >= rows) continue;
+    const float scale = s_scale[r];
+    if (scale != scale) o[e] = make_float4(scale, scale, scale, scale);
+    const int token = static_cast<int>(blockIdx.y) * p.half_rows + r / group;
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<size_t>(j.row + token) * a.out_stride + static_cast<size_t>(j.kvh * group + r % group) * D + c) =
+        make_uint2(pack_pair<T>(o[e].x * scale, o[e].y * scale), pack_pair<T>(o[e].z * scale, o[e].w * scale));
   }
 }
 
@@ -800,7 +859,7 @@ int launch_fast(const cacheir_b200_tree_args& a, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   cudaError_t e = allow_shared_memory(done, reinterpret_cast<const void*>(kern), Smem<D>::kBytes);
   if (e == cudaSuccess) e = launch_chained(kern, dim3(grid), dim3(kThreads), Smem<D>::kBytes, stream, tk, tv, tq, p);
-  if (e == cudaSuccess) e = launch_chained(tree_pieces_kernel<T, D>, dim3(grid, 2 * kRows / kJoinRows), dim3(kJoinRows * 16), 0, stream, p);
+  if (e == cudaSuccess) e = launch_chained(tree_pieces_kernel<T, D>, dim3(grid, 2), dim3(kJoinThreads), 0, stream, p);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }
 
