@@ -32,6 +32,7 @@ constexpr int kFirst = 96;                     // .. whose probabilities go to t
 constexpr int kRows = 128;                     // query rows of a group of warps
 constexpr int kThreads = 384;
 constexpr int kMaxHeadsPerKv = 64;
+constexpr int kWholeTiles = 4;                 // tokens that tables have room for, in tiles, up to which items are not cut
 constexpr int kPlanThreads = 128;              // that lay the plan out, some sequences each
 constexpr float kAhead = 6.f;                  // a new reference is the maximum less this: probabilities start at 2^6 ..
 constexpr float kStale = 14.f;                 // .. and may grow to 2^14 (in fp16: 2^-24 of that is still a number)
@@ -45,9 +46,11 @@ struct TreeJoin {
 struct FastParams {
   cacheir_b200_tree_args a;
   TreeJoin* joins;                             // [blocks]
-  float* ml;                                   // [blocks][2][256][2]: maxima (log2 domain) and denominators of the blocks' pieces
-  float* acc;                                  // [blocks][2][256][dim]: unnormalised outputs
+  float* ml;                                   // [blocks][2 pieces][2 groups][128][2]: maxima (log2 domain) and denominators
+  float* acc;                                  // [blocks][2 pieces][2 groups][dim / 4][128][4]: unnormalised outputs, rows side by side as the lanes are that have them
   int half_rows;                               // tokens of a group of warps
+  int whole;                                   // items are not cut
+  int out_wide;                                // rows of out begin at 32 bytes
   float scale_log2;
 };
 
@@ -55,6 +58,10 @@ struct FastParams {
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int code) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, &g_tree_status, code));
+}
+__device__ __forceinline__ void store_32_bytes(void* to, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 // n / d for a d that mostly is a power of two (pages).
 struct Division {
@@ -67,9 +74,12 @@ struct Division {
 };
 
 // ---- how the work is cut ----
-// An item of n key tiles is kItemUnits + n units: what it costs to begin with (queries, the first tile's latency, the output) is about
-// that of so many tiles. The units are dealt out as evenly as whole numbers can be.
-constexpr int kItemUnits = 2;
+// An item of n key tiles is kItemUnits + n kTileUnits units (kTwoUnits where two groups of warps have rows of their own, whose tiles take the longer the less
+// the memory is waited for): what it costs to begin with (queries, the first tile's latency, the output) is about that of two tiles. The units are dealt out
+// as evenly as whole numbers can be; a block has the tiles whose first unit is its own. Where items are not cut, each is a unit.
+constexpr int kItemUnits = 4;
+constexpr int kTileUnits = 2;
+constexpr int kTwoUnits = 3;
 
 struct Deal {
   int share, more;             // every block has `share` units, the first `more` one more
@@ -84,31 +94,44 @@ struct Deal {
 __device__ __forceinline__ int item_keys(const cacheir_b200_tree_args& a, const TreeSequence& s, int end) {
   return a.visible ? s.keys : max(min(s.keys, s.front + min(end, s.rows)), 0);
 }
-__device__ __forceinline__ int item_units(int keys) { return kItemUnits + max((keys + kKeys - 1) / kKeys, 1); }
+__device__ __forceinline__ int item_tiles(int keys) { return max((keys + kKeys - 1) / kKeys, 1); }
+struct Cost {
+  int tile_rows, whole;
+  // the units of a tile, and of an item, of so many rows
+  __device__ __forceinline__ int tile(int rows) const { return 2 * rows > tile_rows ? kTwoUnits : kTileUnits; }
+  __device__ __forceinline__ int item(int rows, int keys) const { return whole ? 1 : kItemUnits + item_tiles(keys) * tile(rows); }
+};
 // Of a sequence, for one key/value head after the other in every tile of rows.
-__device__ __forceinline__ int sequence_units(const cacheir_b200_tree_args& a, const TreeSequence& s, int tile_rows) {
-  const int tiles = (s.rows + tile_rows - 1) / tile_rows;
-  if (a.visible) return a.kv_heads * tiles * item_units(s.keys);
+__device__ __forceinline__ int sequence_units(const cacheir_b200_tree_args& a, const TreeSequence& s, const Cost& cost) {
+  const int tiles = (s.rows + cost.tile_rows - 1) / cost.tile_rows;
+  if (tiles == 0) return 0;
   int units = 0;
-  for (int j = 1; j <= tiles; ++j) units += item_units(item_keys(a, s, j * tile_rows));
-  return a.kv_heads * units;
+  if (a.visible) units = (tiles - 1) * cost.item(cost.tile_rows, s.keys);
+  else for (int j = 1; j < tiles; ++j) units += cost.item(cost.tile_rows, item_keys(a, s, j * cost.tile_rows));
+  return a.kv_heads * (units + cost.item(s.rows - (tiles - 1) * cost.tile_rows, s.keys));
 }
 
 // A block's share of the units, item by item.
 struct Walk {
   const cacheir_b200_tree_args& a;
+  Cost cost;
   Deal deal;
-  int at, end, tile_rows;
+  int at, end;
   int b, start;                // the sequence, and the first unit of its row tile
   TreeSequence s;
-  int row_tile, units;         // .. the row tile, and the units of an item in it
+  int row0, rows, keys, units; // .. the row tile: rows from row0 of the sequence on, what they see, and the units of an item in it
   // the item
-  int kvh, row0, rows, tile, tiles, keys, first;     // rows from row0 of the sequence on; key tiles tile .. tile + tiles - 1 of it are this block's;
-  bool begins, ends;                                 // block `first` has its first one
+  int kvh, tile, tiles, first; // key tiles tile .. tile + tiles - 1 of it are this block's; block `first` has its first one
+  bool begins, ends;
 
+  __device__ __forceinline__ void row_tile(int from) {
+    row0 = from;
+    rows = min(cost.tile_rows, s.rows - row0);
+    keys = item_keys(a, s, row0 + rows);
+    units = cost.item(rows, keys);
+  }
   // starts: the first units of runs of `run` sequences
-  __device__ __forceinline__ Walk(const cacheir_b200_tree_args& args, int rows_of_item, const int* starts, int run, int total, int ctas)
-      : a(args), deal(total, ctas), tile_rows(rows_of_item) {
+  __device__ __forceinline__ Walk(const cacheir_b200_tree_args& args, const Cost& c, const int* starts, int run, int total, int ctas) : a(args), cost(c), deal(total, ctas) {
     at = deal.begin(blockIdx.x);
     end = deal.begin(blockIdx.x + 1);
     int lo = 0, hi = kPlanThreads;                             // last run that starts at or before `at` (empty ones start where the next does)
@@ -116,39 +139,34 @@ struct Walk {
       const int mid = (lo + hi) >> 1;
       if (starts[mid] <= at) lo = mid; else hi = mid;
     }
-    b = lo * run;
+    b = min(lo * run, a.sequences - 1);
     start = starts[lo];
-    s = tree_sequence(a, min(b, a.sequences - 1));
-    row_tile = 0;
-    units = item_units(item_keys(a, s, tile_rows));
+    s = tree_sequence(a, b);
+    row_tile(0);
   }
   __device__ __forceinline__ bool next() {
     while (at < end) {
-      // the row tile that `at` is in
-      while (row_tile * tile_rows >= s.rows || start + a.kv_heads * units <= at) {
-        if (row_tile * tile_rows < s.rows) {
-          start += a.kv_heads * units;
-          ++row_tile;
-        }
-        if (row_tile * tile_rows >= s.rows) {
+      while (rows <= 0 || start + a.kv_heads * units <= at) {  // to the row tile that `at` is in
+        if (rows > 0) start += a.kv_heads * units;
+        if (rows > 0 && row0 + rows < s.rows) {
+          row_tile(row0 + rows);
+        } else {
           if (++b >= a.sequences) return false;
           s = tree_sequence(a, b);
-          row_tile = 0;
+          row_tile(0);
         }
-        units = item_units(item_keys(a, s, (row_tile + 1) * tile_rows));
       }
       kvh = (at - start) / units;
-      const int item0 = start + kvh * units, tile0 = item0 + kItemUnits, stop = min(end, item0 + units);
-      tile = max(at - tile0, 0);
-      tiles = stop - tile0 - tile;
-      begins = at <= tile0;
-      ends = stop == item0 + units;
+      const int item0 = start + kvh * units, stop = min(end, item0 + units), all = item_tiles(keys);
+      const int each = cost.tile(rows), tile0 = item0 + kItemUnits;
+      auto behind = [&](int unit) { return cost.whole ? (unit > item0 ? all : 0) : min((max(unit - tile0, 0) + each - 1) / each, all); };      // tiles that begin before a unit
+      tile = behind(at);
+      tiles = behind(stop) - tile;
+      begins = tile == 0;
+      ends = tile + tiles == all;
       at = stop;
-      if (tiles <= 0) continue;                                // (no more than an item's beginning: the next block has its tiles)
+      if (tiles <= 0) continue;                                // (no tile begins here)
       first = begins ? static_cast<int>(blockIdx.x) : deal.owner(tile0);
-      row0 = row_tile * tile_rows;
-      rows = min(tile_rows, s.rows - row0);
-      keys = item_keys(a, s, row0 + rows);
       return true;
     }
     return false;
@@ -170,18 +188,17 @@ struct Smem {
   static constexpr int kSlots = D == 128 ? 5 : 10;
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kTiles = 2 * kQBytes + kSlots * kSlotBytes;
-  // then: barriers of keys, of values, empty, clean [slots], q[2], place of q[2], s[2], p[2][2], o[2], end[3], items; tensor memory address; items; starts of runs
-  static constexpr int kBarriers = 4 * kSlots + 15 + kItems;
-  static constexpr int kBytes = 1024 + kTiles + kBarriers * 8 + 16 + kItems * static_cast<int>(sizeof(Item)) + kPlanThreads * 4;
+  // then: barriers of keys, of values, empty, clean [slots], q[2], place of q[2], s[2], p[2][2], o[2], end[2], items; tensor memory address; items; starts of runs, and later
+  // maxima and denominators of the second group of warps
+  static constexpr int kBarriers = 4 * kSlots + 14 + kItems;
+  static constexpr int kBytes = 1024 + kTiles + kBarriers * 8 + 16 + kItems * static_cast<int>(sizeof(Item)) + kRows * 8;
 };
 
-// Where a column of a lane's line of 32 lies in shared memory: lanes that read the same one reach different banks.
-__device__ __forceinline__ int staged(int lane, int column) { return lane * 32 + (((column >> 2) ^ (lane & 7)) << 2) + (column & 3); }
-// What row `row` of the item gets of values that are no numbers, of the tokens that it sees in the tiles from `tile` on, added to columns c .. end - 1
-// of its place `to`, which this warp has written.
+// What row `row` of the item gets of values that are no numbers, of the tokens that it sees in the tiles from `tile` on, added to its place
+// `to`, which this lane has written: a row of out, or with floats one of the scratch, whose columns lie in fours, 128 of them apart.
 template <typename T, int D, typename O>
-__device__ __noinline__ void add_spoilt(const cacheir_b200_tree_args& a, const TreeSequence s, const int32_t* pages, int row, int head, int tile, int tiles, int keys, int c,
-                                        int end, O* to) {
+__device__ __noinline__ void add_spoilt(const cacheir_b200_tree_args& a, const TreeSequence s, const int32_t* pages, int row, int head, int tile, int tiles, int keys,
+                                        O* to) {
   const int kvh = head / (a.heads / a.kv_heads);
   const T* q = static_cast<const T*>(a.q) + static_cast<size_t>(s.row + row) * a.q_stride + static_cast<size_t>(head) * D;
   for (int t = max(tile * kKeys, max(s.front, 0)); t < min((tile + tiles) * kKeys, keys); ++t) {
@@ -192,15 +209,16 @@ __device__ __noinline__ void add_spoilt(const cacheir_b200_tree_args& a, const T
     const size_t at = ((static_cast<size_t>(id) * a.kv_heads + kvh) * a.page_size + t % a.page_size) * D;
     const T* v = static_cast<const T*>(a.v_cache) + at;
     bool any = false;
-    for (int i = c; i < end; ++i) any = any || !isfinite(Elem<T>::ld(v + i));
+    for (int i = 0; i < D; ++i) any = any || !isfinite(Elem<T>::ld(v + i));
     if (!any) continue;
     const T* k = static_cast<const T*>(a.k_cache) + at;
     float score = 0.f;
     for (int d = 0; d < D; ++d) score = fmaf(Elem<T>::ld(q + d), Elem<T>::ld(k + d), score);
     if (score == -INFINITY) continue;                          // (no weight)
-    for (int i = c; i < end; ++i) {
+    for (int i = 0; i < D; ++i) {
       const float x = Elem<T>::ld(v + i);
-      if (!isfinite(x)) Elem<O>::st(to + i, Elem<O>::ld(to + i) + x);
+      O* at_to = to + (std::is_same<O, float>::value ? (i >> 2) * (kRows * 4) + (i & 3) : i);
+      if (!isfinite(x)) Elem<O>::st(at_to, Elem<O>::ld(at_to) + x);
     }
   }
 }
@@ -226,11 +244,13 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
   uint64_t* bar_s = bar_free + 2;                              // scores are in tensor memory
   uint64_t* bar_p = bar_s + 2;                                 // probabilities are, [group of warps][first keys, the others]
   uint64_t* bar_o = bar_p + 4;                                 // .. and have been added to the output
-  uint64_t* bar_end = bar_o + 2;                               // steps of an item's end that both groups of warps have made
-  uint64_t* bar_item = bar_end + 3;                            // the item is known
+  uint64_t* bar_end = bar_o + 2;                               // the second group's part of an item is done, and has been joined to the first one's
+  uint64_t* bar_item = bar_end + 2;                            // the item is known
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_item + kItems);
   Item* s_item = reinterpret_cast<Item*>(tmem_slot + 4);
   int* s_start = reinterpret_cast<int*>(s_item + kItems);
+  float2* s_ml = reinterpret_cast<float2*>(s_start);           // (when the first item ends the keys' warp has long found its share)
+  static_assert(kPlanThreads * 4 <= kRows * 8, "starts and maxima share their place");
   __shared__ int s_scan[kPlanThreads / 32];
   __shared__ volatile int s_spoilt[kItems];                    // the last item of this place some of whose values are no numbers
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -248,13 +268,13 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(smem_u32(&bar_q[w]), 1);
-      mbar_init(smem_u32(&bar_free[w]), 8);
+      mbar_init(smem_u32(&bar_free[w]), 1);
       mbar_init(smem_u32(&bar_s[w]), 1);
       mbar_init(smem_u32(&bar_p[2 * w]), kRows);
       mbar_init(smem_u32(&bar_p[2 * w + 1]), kRows);
       mbar_init(smem_u32(&bar_o[w]), 1);
     }
-    for (int i = 0; i < 3; ++i) mbar_init(smem_u32(&bar_end[i]), 8);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&bar_end[i]), 4);
     for (int i = 0; i < kItems; ++i) mbar_init(smem_u32(&bar_item[i]), 1);
     mbar_fence_init();
   }
@@ -262,10 +282,11 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
   chain_enter();
   if (warp == 8) tc_alloc(smem_u32(tmem_slot), 512);           // (beside the loads of the plan)
   // ---- the plan: units of runs of sequences, a thread each ----
-  const int tile_rows = 2 * p.half_rows, run = (a.sequences + kPlanThreads - 1) / kPlanThreads;
+  const Cost cost{2 * p.half_rows, p.whole};
+  const int run = (a.sequences + kPlanThreads - 1) / kPlanThreads;
   int sum = 0, own = 0;
   if (threadIdx.x < kPlanThreads) {
-    for (int b = threadIdx.x * run; b < min(static_cast<int>(threadIdx.x + 1) * run, a.sequences); ++b) own += sequence_units(a, tree_sequence(a, b), tile_rows);
+    for (int b = threadIdx.x * run; b < min(static_cast<int>(threadIdx.x + 1) * run, a.sequences); ++b) own += sequence_units(a, tree_sequence(a, b), cost);
     sum = own;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -288,7 +309,8 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
   const uint32_t tmem = *tmem_slot;                            // scores [2][128 columns] (probabilities over them), outputs [2][D]
   const uint32_t tmem_o = tmem + 2 * kKeys;
   const int group = a.heads / a.kv_heads, half_rows = p.half_rows;
-  const int ctas = max(1, min(total, static_cast<int>(gridDim.x)));
+  // (no block between those of an item's first and last tile is without one)
+  const int ctas = max(1, min(p.whole ? total : total / kTwoUnits, static_cast<int>(gridDim.x)));
   bool ok = true;
   Item it;
   int item = 0;                                                // of the block, counted from 1
@@ -330,7 +352,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
               *at = make_uint4(v.x & ~bad[0], v.y & ~bad[1], v.z & ~bad[2], v.w & ~bad[3]);
             }
           }
-          if (__any_sync(0xffffffffu, spoilt) && lane == 0) s_spoilt[item % kItems] = item;
+          if (__any_sync(0xffffffffu, spoilt) && lane == 0) s_spoilt[(item - 1) % kItems] = item;
           fence_async_smem();
           __threadfence_block();
         }
@@ -377,7 +399,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
       }
     };
     if (keys) {                                                // this warp goes through the block's share and says what the items are
-      Walk walk(a, tile_rows, s_start, run, max(total, 1), ctas);
+      Walk walk(a, cost, s_start, run, max(total, 1), ctas);
       if (static_cast<int>(blockIdx.x) >= min(ctas, total)) walk.end = walk.at;
       TreeJoin join{};
       bool more = true;
@@ -454,6 +476,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
         }
         tc_commit(smem_u32(&bar_s[j & 1]));
         if (!two || (j & 1)) tc_commit(smem_u32(&empty[k_slot]));
+        if (j >= (two ? steps - 2 : steps - 1)) tc_commit(smem_u32(&bar_free[two ? j & 1 : q_place]));      // (the last that look at these queries)
       };
       auto scored = [&](int j) {                               // (the whole warp)
         if (!two || (j & 1)) {
@@ -513,13 +536,12 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
     const int by_group = (65536 + group - 1) / group;          // n / group = n * by_group >> 16 for n < 256, group <= 64
     const int token = r * by_group >> 16, head_of = r - token * group;
     uint32_t s_phase = 0, o_phase = 0, end_phase = 0;
-    int q_place = 0;                                           // where the queries of an item that both groups share are
+    bool lent = false;                                         // (second group) its output has not been joined yet
     while (next_item()) {
       const bool two = it.rows > half_rows;
-      const int place = two ? w : q_place;
-      if (!two) q_place ^= 1;
       const int in_item = (two ? w * half_rows : 0) + token;   // this thread's token of the item
       const bool real = r < half_rows * group && in_item < it.rows;
+      const bool idle = !__any_sync(0xffffffffu, real);        // (a warp without rows: whatever it leaves as probabilities goes to outputs of nobody)
       const int row = it.row0 + (real ? in_item : 0), head = it.kvh * group + head_of;
       const int masked_from = min(it.s.front, it.keys);    // keys behind this need a look at the row's mask
       float m_ref = -INFINITY, l_run = 0.f;
@@ -544,6 +566,18 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
         ok = warp_wait(smem_u32(&bar_s[w]), s_phase, (15 << 8) | 8);
         if (!ok) break;
         s_phase ^= 1;
+        auto returned = [&] {                                  // the output may be written over
+          if (!lent) return;
+          lent = false;
+          ok = warp_wait(smem_u32(&bar_end[1]), end_phase, (15 << 8) | 13) && ok;
+          end_phase ^= 1;
+        };
+        if (idle) {
+          returned();
+          mbar_arrive(smem_u32(&bar_p[2 * w]));
+          mbar_arrive(smem_u32(&bar_p[2 * w + 1]));
+          continue;
+        }
         tc_fence_after();
         const uint32_t scores = tmem + w * kKeys + lane_addr;
         // The row's 128 scores are looked at twice. For the maximum the second half comes first: the first half then stays in registers,
@@ -620,6 +654,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
           tmem_wait_ld(y);
           tmem_st_x16(scores + 32, rest);
           tmem_wait_st();
+          returned();
           tc_fence_before();
           mbar_arrive(smem_u32(&bar_p[2 * w]));
           if (!whole) masked(y, see[3]);
@@ -643,25 +678,29 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
         o_phase ^= 1;
       }
       tc_fence_after();
-      auto together = [&](int i) {                             // both groups of warps have come here
+      // An item that both groups have had: the second one leaves its maxima and denominators and goes on, the first one adds its output to its own. (Each of them
+      // storing half of the columns, and waiting for the other one three times, took 2 us an item longer.)
+      float f_own = 1.f, f_other = 0.f;
+      if (!two && w == 1) {
+        if (lent) {                                            // (an item of one tile, of which this group had none: the last one may not have been joined)
+          lent = false;
+          ok = warp_wait(smem_u32(&bar_end[1]), end_phase, (15 << 8) | 13);
+          if (!ok) break;
+          end_phase ^= 1;
+        }
+        s_ml[r] = make_float2(m_ref, l_run);
+        lent = true;
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_end[i]));
-        const bool came = warp_wait(smem_u32(&bar_end[i]), end_phase, (15 << 8) | 13);
-        tc_fence_after();
-        return came;
-      };
-      uint8_t* s_place = s_q + place * L::kQBytes;             // (all scores of the item have been worked out)
-      float f_own = 1.f, f_other = 0.f;
+        if (lane == 0) mbar_arrive(smem_u32(&bar_end[0]));
+        continue;
+      }
       if (!two) {
-        float2* s_ml = reinterpret_cast<float2*>(s_place);     // [2][128]
-        // (an item of one tile is the first group's alone, whose queries the second one must not write over)
-        if (steps > 0) s_ml[w * kRows + r] = make_float2(m_ref, l_run);
-        ok = together(0);
+        ok = warp_wait(smem_u32(&bar_end[0]), end_phase, (15 << 8) | 13);
         if (!ok) break;
-        const float2 other = w == 1 || it.tiles > 1 ? s_ml[(w ^ 1) * kRows + r] : make_float2(-INFINITY, 0.f);
-        ok = together(1);
-        if (!ok) break;
+        end_phase ^= 1;
+        tc_fence_after();
+        const float2 other = s_ml[r];
         const float m = fmaxf(m_ref, other.x);
         f_own = m_ref > -INFINITY ? ex2(m_ref - m) : 0.f;
         f_other = other.x > -INFINITY ? ex2(other.x - m) : 0.f;
@@ -669,83 +708,60 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
         l_run = l_run * (m_ref > -INFINITY ? f_own : 1.f) + other.y * (other.x > -INFINITY ? f_other : 1.f);
         m_ref = m;
       }
-      const bool direct = it.flags == 3, spoilt = s_spoilt[item % kItems] == item;
-      const int slot = 2 * blockIdx.x + (it.flags & 1), in_slot = (two ? w : 0) * kRows + r;
-      if (!direct && real && (two || w == 0)) *reinterpret_cast<float2*>(p.ml + (static_cast<size_t>(slot) * 2 * kRows + in_slot) * 2) = make_float2(m_ref, l_run);
-      const float scale = direct ? (l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f) : 1.f;
-      f_own *= scale;
-      f_other *= scale;
-      // By way of shared memory (the queries' place), so that a store writes whole lines: a lane has a row, a store 32 columns of four rows.
-      // (4 KB a warp: with heads of 64 the place has room for one group of warps, which then stores all columns)
-      constexpr bool kHalves = L::kQBytes >= 8 * 4096;
-      float* s_row = reinterpret_cast<float*>(s_place + (two || !kHalves ? warp & 3 : warp) * 4096);
-      const int c_begin = two ? 0 : kHalves ? w * (D / 2) : w * D, c_end = two || !kHalves ? D : c_begin + D / 2;
-      const size_t scratch_row = static_cast<size_t>(slot) * 2 * kRows + (two ? w : 0) * kRows;
-      // element at which a row of this warp (its four rows of every store: 4 i + lane / 8) begins in out, or in the scratch; -1: it is none
-      auto begin_of = [&](int in_warp) {
-        const int r2 = (warp & 3) * 32 + in_warp, token2 = r2 * by_group >> 16, in2 = (two ? w * half_rows : 0) + token2;
-        if (r2 >= half_rows * group || in2 >= it.rows) return -1LL;
-        return direct ? static_cast<long long>(it.s.row + it.row0 + in2) * a.out_stride + static_cast<long long>(it.kvh * group + r2 - token2 * group) * D
-                      : static_cast<long long>((scratch_row + r2) * D);
-      };
-      long long to[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) to[i] = begin_of(4 * i + (lane >> 3));
+      const bool direct = it.flags == 3;
+      if (!idle) {
+        const float scale = direct ? (l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f) : 1.f;
+        f_own *= scale;
+        f_other *= scale;
+        const size_t place = (static_cast<size_t>(2 * blockIdx.x + (it.flags & 1)) * 2 + (two ? w : 0));          // of the piece in the scratch
+        T* const to = static_cast<T*>(a.out) + static_cast<size_t>(it.s.row + row) * a.out_stride + static_cast<size_t>(head) * D;
+        float* const acc = p.acc + place * (kRows * D) + r * 4;
+        if (!direct && real) *reinterpret_cast<float2*>(p.ml + (place * kRows + r) * 2) = make_float2(m_ref, l_run);
 #pragma unroll 1
-      for (int c = c_begin; c < c_end; c += 32) {
-        uint32_t x[32];
-        float o[32];
-        if (__any_sync(0xffffffffu, f_own != 0.f)) {
-          tmem_ld_x32(tmem_o + w * D + lane_addr + c, x);
-          tmem_wait_ld(x);
+        for (int c = 0; c < D; c += 32) {
+          uint32_t x[32];
+          float o[32];
+          if (__any_sync(0xffffffffu, f_own != 0.f)) {
+            tmem_ld_x32(tmem_o + w * D + lane_addr + c, x);
+            tmem_wait_ld(x);
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = f_own != 0.f ? __uint_as_float(x[i]) * f_own : 0.f;
+          if (!two && __any_sync(0xffffffffu, f_other != 0.f)) {
+            tmem_ld_x32(tmem_o + D + lane_addr + c, x);
+            tmem_wait_ld(x);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = f_other != 0.f ? fmaf(__uint_as_float(x[i]), f_other, o[i]) : o[i];
+          }
+          if (l_run != l_run)                                  // (NaN among the scores of a group whose reference never moved)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = l_run;
+          if (!real) continue;
+          if (direct) {
+            uint32_t v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = pack_pair<T>(o[2 * i], o[2 * i + 1]);
+            if (p.out_wide) {
+              store_32_bytes(to + c, v);
+              store_32_bytes(to + c + 16, v + 8);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) *reinterpret_cast<uint2*>(to + c + 2 * i) = make_uint2(v[i], v[i + 1]);
+            }
+          } else {                                             // (a lane's neighbours have the rows beside its own)
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(acc + (c + i) * kRows) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
         }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = f_own != 0.f ? __uint_as_float(x[i]) * f_own : 0.f;
-        if (!two && __any_sync(0xffffffffu, f_other != 0.f)) {
-          tmem_ld_x32(tmem_o + (w ^ 1) * D + lane_addr + c, x);
-          tmem_wait_ld(x);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = f_other != 0.f ? fmaf(__uint_as_float(x[i]), f_other, o[i]) : o[i];
+        if (s_spoilt[(item - 1) % kItems] == item && real) {
+          const int32_t* pages = a.page_table + static_cast<size_t>(it.b) * a.max_pages;
+          if (direct) add_spoilt<T, D, T>(a, it.s, pages, row, head, it.tile, it.tiles, it.keys, to);
+          else add_spoilt<T, D, float>(a, it.s, pages, row, head, it.tile, it.tiles, it.keys, acc);
         }
-        if (l_run != l_run)                                    // (NaN among the scores of a group whose reference never moved)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = l_run;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<float4*>(s_row + staged(lane, 4 * i)) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-        __syncwarp();
-        float4 v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const float4*>(s_row + staged(4 * i + (lane >> 3), (lane & 7) * 4));
-        __syncwarp();
-        const int column = c + (lane & 7) * 4;
-        if (direct) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (to[i] >= 0) *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + to[i] + column) = make_uint2(pack_pair<T>(v[i].x, v[i].y), pack_pair<T>(v[i].z, v[i].w));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (to[i] >= 0) *reinterpret_cast<float4*>(p.acc + to[i] + column) = v[i];
-        }
-      }
-      __syncwarp();
-      if (spoilt && real) {
-        const long long to_row = begin_of(lane);
-        const int32_t* pages = a.page_table + static_cast<size_t>(it.b) * a.max_pages;
-        if (direct) add_spoilt<T, D, T>(a, it.s, pages, row, head, it.tile, it.tiles, it.keys, c_begin, c_end, static_cast<T*>(a.out) + to_row);
-        else add_spoilt<T, D, float>(a, it.s, pages, row, head, it.tile, it.tiles, it.keys, c_begin, c_end, p.acc + to_row);
-      }
-      if (!two) {                                              // (the outputs may be written over)
-        ok = together(2);
-        if (!ok) break;
-        end_phase ^= 1;
       }
       tc_fence_before();
-      fence_async_smem();                                      // (the next queries come by copies)
       __syncwarp();
-      if (two) { if (lane < 2) mbar_arrive(smem_u32(&bar_free[place])); }
-      else if (lane == 0) mbar_arrive(smem_u32(&bar_free[place]));
+      if (!two && lane == 0) mbar_arrive(smem_u32(&bar_end[1]));
     }
   }
   __syncwarp();
@@ -758,77 +774,63 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
 }
 
 // ---- the pieces of items that were cut ----
-// A block per (block of the first kernel, group of warps of its item), a warp per eight query rows, pieces in their order. (16 blocks of two rows a warp each,
-// most of which had nothing to do, took 13 us behind 32 trees where these take 5.)
+// A block per (block of the first kernel, group of warps of its item), a lane a query row and every fourth four columns, pieces in their order. Output rows are
+// put together in shared memory, so that a store writes whole lines.
 constexpr int kJoinThreads = 512;
-constexpr int kJoinPieces = 16;                // weights that lie in shared memory at a time
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
 tree_pieces_kernel(const FastParams p) {
   chain_enter();
-  __shared__ float s_max[kRows], s_scale[kRows], s_weight[kJoinPieces][kRows];
+  constexpr int kFours = D / 4 * kRows / kJoinThreads;         // of a thread
+  constexpr int kLine = D * 2 + 16;                            // bytes of a row in shared memory (so that lanes beside one another reach different banks)
+  __shared__ __align__(16) uint8_t s_out[kRows * kLine];
   const TreeJoin j = p.joins[blockIdx.x];
-  if (j.rows <= static_cast<int>(blockIdx.y) * p.half_rows) return;
+  const int group_of = blockIdx.y;
+  if (j.rows <= group_of * p.half_rows) return;
   const cacheir_b200_tree_args& a = p.a;
   const int group = a.heads / a.kv_heads, n = static_cast<int>(blockIdx.x) - j.first + 1;
-  const int rows = min(p.half_rows, j.rows - static_cast<int>(blockIdx.y) * p.half_rows) * group;       // query rows that there are
-  auto slot_of = [&](int i) { return 2 * (j.first + i) + (i == 0 ? 1 : 0); };
-  auto place_of = [&](int i, int r) { return static_cast<size_t>(slot_of(i)) * 2 * kRows + blockIdx.y * kRows + r; };
-  if (static_cast<int>(threadIdx.x) < rows) {
+  const int rows = min(p.half_rows, j.rows - group_of * p.half_rows) * group;        // query rows that there are
+  const int r = threadIdx.x & (kRows - 1), part = threadIdx.x / kRows;
+  auto place_of = [&](int i) { return static_cast<size_t>(2 * (j.first + i) + (i == 0 ? 1 : 0)) * 2 + group_of; };
+  if (r < rows) {
     float m = -INFINITY, l = 0.f;
 #pragma unroll 8
-    for (int i = 0; i < n; ++i) m = fmaxf(m, p.ml[2 * place_of(i, threadIdx.x)]);
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const float2 v = *reinterpret_cast<const float2*>(p.ml + 2 * place_of(i, threadIdx.x));
-      l += v.y * (v.x > -INFINITY ? exp2f(v.x - m) : 1.f);     // (a piece whose keys all scored -inf has a sum of 0, or of NaN, which stays)
-    }
-    s_max[threadIdx.x] = m;
-    s_scale[threadIdx.x] = l > 0.f || l != l ? 1.f / l : 0.f;
-  }
-  constexpr int kLanes = D / 4, kTogether = kRows * kLanes / kJoinThreads;       // lanes of a row; rows of a thread
-  const int c = threadIdx.x % kLanes * 4, first = threadIdx.x / kLanes;
-  float4 o[kTogether] = {};
-  for (int i0 = 0; i0 < n; i0 += kJoinPieces) {
-    const int pieces = min(kJoinPieces, n - i0);
-    __syncthreads();
-    for (int e = threadIdx.x; e < pieces * kRows; e += kJoinThreads) {
-      const int r = e % kRows, i = e / kRows;
-      if (r >= rows) continue;
-      const float x = p.ml[2 * place_of(i0 + i, r)];
-      s_weight[i][r] = x > -INFINITY ? exp2f(x - s_max[r]) : 0.f;
-    }
-    __syncthreads();
+    for (int i = 0; i < n; ++i) m = fmaxf(m, p.ml[(place_of(i) * kRows + r) * 2]);
+    float4 o[kFours] = {};
 #pragma unroll 2
-    for (int i = 0; i < pieces; ++i) {
-      float4 v[kTogether];
-      float f[kTogether];
+    for (int i = 0; i < n; ++i) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.ml + (place_of(i) * kRows + r) * 2);
+      const float* acc = p.acc + place_of(i) * (kRows * D) + r * 4;
+      float4 v[kFours];
 #pragma unroll
-      for (int e = 0; e < kTogether; ++e) {
-        const int r = first + e * (kRows / kTogether);
-        f[e] = r < rows ? s_weight[i][r] : 0.f;
-        if (f[e] != 0.f) v[e] = *reinterpret_cast<const float4*>(p.acc + place_of(i0 + i, r) * D + c);
-      }
+      for (int k = 0; k < kFours; ++k) v[k] = *reinterpret_cast<const float4*>(acc + (part + k * (kJoinThreads / kRows)) * (kRows * 4));
+      const float f = ml.x > -INFINITY ? exp2f(ml.x - m) : 0.f;
+      l += ml.y * (ml.x > -INFINITY ? f : 1.f);                // (a piece whose keys all scored -inf has a sum of 0, or of NaN, which stays)
+      if (f != 0.f)
 #pragma unroll
-      for (int e = 0; e < kTogether; ++e)
-        if (f[e] != 0.f) {
-          o[e].x = fmaf(v[e].x, f[e], o[e].x);
-          o[e].y = fmaf(v[e].y, f[e], o[e].y);
-          o[e].z = fmaf(v[e].z, f[e], o[e].z);
-          o[e].w = fmaf(v[e].w, f[e], o[e].w);
+        for (int k = 0; k < kFours; ++k) {
+          o[k].x = fmaf(v[k].x, f, o[k].x);
+          o[k].y = fmaf(v[k].y, f, o[k].y);
+          o[k].z = fmaf(v[k].z, f, o[k].z);
+          o[k].w = fmaf(v[k].w, f, o[k].w);
         }
     }
-  }
+    const float scale = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
-  for (int e = 0; e < kTogether; ++e) {
-    const int r = first + e * (kRows / kTogether);
-    if (r >= rows) continue;
-    const float scale = s_scale[r];
-    if (scale != scale) o[e] = make_float4(scale, scale, scale, scale);
-    const int token = static_cast<int>(blockIdx.y) * p.half_rows + r / group;
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<size_t>(j.row + token) * a.out_stride + static_cast<size_t>(j.kvh * group + r % group) * D + c) =
-        make_uint2(pack_pair<T>(o[e].x * scale, o[e].y * scale), pack_pair<T>(o[e].z * scale, o[e].w * scale));
+    for (int k = 0; k < kFours; ++k) {
+      if (scale != scale) o[k] = make_float4(scale, scale, scale, scale);
+      *reinterpret_cast<uint2*>(s_out + r * kLine + (part + k * (kJoinThreads / kRows)) * 8) =
+          make_uint2(pack_pair<T>(o[k].x * scale, o[k].y * scale), pack_pair<T>(o[k].z * scale, o[k].w * scale));
+    }
+  }
+  __syncthreads();
+  constexpr int kLanes = D / 4;                                // of a row, 8 bytes each
+  const int first_token = j.row + group_of * p.half_rows;
+  for (int i = threadIdx.x; i < rows * kLanes; i += kJoinThreads) {
+    const int row = i / kLanes, c = i % kLanes * 4;
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<size_t>(first_token + row / group) * a.out_stride + static_cast<size_t>(j.kvh * group + row % group) * D + c) =
+        *reinterpret_cast<const uint2*>(s_out + row * kLine + c * 2);
   }
 }
 
@@ -836,7 +838,7 @@ int half_rows_of(const cacheir_b200_tree_args& a) { return kRows / (a.heads / a.
 // Units of all items, at most.
 long long most_units(const cacheir_b200_tree_args& a) {
   const long long tiles = (static_cast<long long>(a.max_pages) * a.page_size + kKeys - 1) / kKeys;
-  return (kItemUnits + tiles) * a.kv_heads * (a.rows / (2 * half_rows_of(a)) + a.sequences);
+  return (kItemUnits + kTwoUnits * tiles) * a.kv_heads * (a.rows / (2 * half_rows_of(a)) + a.sequences);
 }
 
 template <typename T, int D>
@@ -852,6 +854,9 @@ int launch_fast(const cacheir_b200_tree_args& a, cudaStream_t stream) {
     return CACHEIR_B200_EUNSUPPORTED;
   const long long most = most_units(a);
   const int grid = static_cast<int>(most < kNumSMs ? most : kNumSMs);
+  // Items of few tiles are not cut: joining their pieces takes longer than a block takes for all of them.
+  p.whole = static_cast<long long>(a.max_pages) * a.page_size <= kWholeTiles * kKeys;
+  p.out_wide = aligned_to(a.out, 32) && a.out_stride % 16 == 0;
   p.joins = static_cast<TreeJoin*>(a.workspace);
   p.ml = reinterpret_cast<float*>(p.joins + kNumSMs);
   p.acc = p.ml + static_cast<size_t>(kNumSMs) * 2 * 2 * kRows * 2;
@@ -859,7 +864,7 @@ int launch_fast(const cacheir_b200_tree_args& a, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   cudaError_t e = allow_shared_memory(done, reinterpret_cast<const void*>(kern), Smem<D>::kBytes);
   if (e == cudaSuccess) e = launch_chained(kern, dim3(grid), dim3(kThreads), Smem<D>::kBytes, stream, tk, tv, tq, p);
-  if (e == cudaSuccess) e = launch_chained(tree_pieces_kernel<T, D>, dim3(grid, 2), dim3(kJoinThreads), 0, stream, p);
+  if (e == cudaSuccess && !p.whole) e = launch_chained(tree_pieces_kernel<T, D>, dim3(grid, 2), dim3(kJoinThreads), 0, stream, p);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }
 
