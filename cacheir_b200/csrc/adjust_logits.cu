@@ -18,9 +18,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kSlice = 4096;                           // tokens of a block, at most
-constexpr int kPairs = 4;                             // logits of listed tokens that a thread has under way
+constexpr int kPairs = 2;                             // logits of listed tokens that a thread has under way
 constexpr int kRun = 8;                                // rows of a block, at most (16: 111 us for 95, as there are fewer blocks to even the work out)
-constexpr int kSaid = 8;                               // tokens of the history that a thread has under way
+constexpr int kSaid = 4;                               // tokens of the history that a thread has under way
 constexpr uint32_t kInPrompt = 0x80000000u;
 constexpr uint32_t kDrafted = 0x40000000u;             // the list of drafted tokens has the token
 constexpr uint32_t kBiased = 0x20000000u;
@@ -36,7 +36,7 @@ __device__ __forceinline__ bool aligned_to_16(const void* p) { return (reinterpr
 // Shared memory: marks [slice / 32], then, where tokens can be marked, counts [slice], (with a bias) entries of it [slice], (with drafts) the drafted
 // tokens and what the rows see of them, and the list of marked tokens [slice].
 template <typename T, typename O, int VEC>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 4)
 adjust_logits_kernel(const LogitsParams p) {
   constexpr int NV = kSlice / VEC / kThreads;          // vectors of a thread in a row
   constexpr bool kWide = VEC > 1;

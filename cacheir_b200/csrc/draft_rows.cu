@@ -128,9 +128,10 @@ accept_drafts_kernel(const cacheir_b200_accept_args a) {
 // ---- keep: a block a sequence and some pools, a thread a column, which it moves in the order of the path ----
 constexpr int kKeepThreads = 128;
 constexpr int kKeepPools = 128;               // of a launch
-constexpr int kKeepShare = 4;                 // pools of a block, which a thread has under way together ..
-constexpr int kKeepDeep = 4;                  // .. with so many rows of each
+constexpr int kKeepShare = 8;                 // pools of a block, which a thread has under way together ..
+constexpr int kKeepDeep = 2;                  // .. with so many rows of each
 constexpr int kKeepMoves = 64;                // moves that a block looks up together
+static_assert(kKeepMoves <= kKeepThreads, "a thread a move");
 
 struct KeepParams {
   cacheir_b200_keep_args a;
@@ -139,31 +140,34 @@ struct KeepParams {
 };
 
 // A row's source is never a target before it, as row numbers rise along a path: all that is written before it is read lies in front of it.
-// What takes time is the way from counts over rows and slots to the values, four dependent loads; so it is gone once for several pools.
+// What takes time is the way from the path over slots to the values, three dependent loads (rows are looked up before it is known how many count); so it is
+// gone once for several pools.
 template <typename V>
 __global__ void __launch_bounds__(kKeepThreads)
 keep_accepted_kernel(const __grid_constant__ KeepParams p) {
   chain_enter();
-  __shared__ int s_from[kKeepMoves], s_to[kKeepMoves];         // pool rows (a slot's page * heads * page size + its place), head 0; -1: none
+  __shared__ int s_from[kKeepMoves], s_to[kKeepMoves];         // slots; -1: none
   const cacheir_b200_keep_args& a = p.a;
   const int b = blockIdx.x;
-  const int2 mine = rows_of(a.cu_rows, a.rows, b);
-  const int count = min(min(a.counts[b], a.depth), mine.y);
   const int32_t* path = a.path + static_cast<size_t>(b) * a.depth;
   const int width = a.dim * (a.dtype == CACHEIR_B200_F32 ? 4 : 2) / static_cast<int>(sizeof(V));          // units of a line
   const long long outside = static_cast<long long>(a.num_slots) * a.page_size;
-  auto line_of = [&](int row) {
-    const int slot = row >= 0 && row < a.rows ? a.slots[row] : -1;
+  int row = static_cast<int>(threadIdx.x) < kKeepMoves && static_cast<int>(threadIdx.x) + 1 < a.depth ? path[threadIdx.x + 1] : -1;
+  const int2 mine = rows_of(a.cu_rows, a.rows, b);
+  const int count = min(min(a.counts[b], a.depth), mine.y);
+  auto line_of = [&](int r) {
+    const int slot = r >= 0 && r < a.rows ? a.slots[r] : -1;
     return slot < 0 || slot >= outside ? -1 : slot;
   };
   const int first_pool = blockIdx.y * kKeepShare, pools = min(kKeepShare, p.pools - first_pool);
   for (int i0 = 1; i0 < count; i0 += kKeepMoves) {             // (rows of one round are read after those before it were written, in any thread)
     const int moves = min(kKeepMoves, count - i0);
     __syncthreads();
-    for (int i = threadIdx.x; i < moves; i += kKeepThreads) {
-      const int row = path[i0 + i], to = mine.x + i0 + i;
-      s_from[i] = row == to ? -1 : line_of(row);
-      s_to[i] = line_of(to);
+    if (static_cast<int>(threadIdx.x) < moves) {
+      if (i0 > 1) row = path[i0 + threadIdx.x];
+      const int to = mine.x + i0 + threadIdx.x;
+      s_from[threadIdx.x] = row == to ? -1 : line_of(row);
+      s_to[threadIdx.x] = line_of(to);
     }
     __syncthreads();
     for (int c = blockIdx.z * kKeepThreads + threadIdx.x; c < a.kv_heads * width; c += gridDim.z * kKeepThreads) {
