@@ -193,20 +193,18 @@ def norm_rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None,
     pass and with one rounding. q_weight, k_weight [D] in the heads' type or float32 (None: no weight), offset 1 for weights that are kept less 1.
     v is appended as it is. All other arguments as there."""
     args, tensors = _rotary_call(q, k, v, rule, positions, slots, k_cache, v_cache, q_out, k_out)
-    dim, weight_code = q.shape[2], 0
-    for weight in (q_weight, k_weight):
-        if weight is not None and (weight.numel() != dim or not weight.is_contiguous()):
+    dim, weight = q.shape[2], k_weight if q_weight is None else q_weight
+    for w in (q_weight, k_weight):
+        if w is not None and (w.numel() != dim or not w.is_contiguous()):
             raise ValueError("weights must be contiguous [D]")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    if weights:
-        if any(w.dtype is not weights[0].dtype for w in weights) or weights[0].dtype not in (q.dtype, _F32):
-            raise TypeError("both weights must be of the heads' type, or float32")
-        weight_code = dtype_code(weights[0].dtype)
-    eps, offset = float(eps), float(offset)
-    if not (0.0 <= eps < math.inf and math.isfinite(offset)):
+    weight_dtype = _F32 if weight is None else weight.dtype
+    if (weight_dtype is not _F32 and weight_dtype is not q.dtype) or (k_weight is not None and k_weight.dtype is not weight_dtype):
+        raise TypeError("both weights must be of the heads' type, or float32")
+    if not (0.0 <= eps < math.inf and -math.inf < offset < math.inf):
         raise ValueError("eps must be finite and not negative, offset finite")
     if args:
-        _launch("norm_rotary_append", tensors + (q_weight, k_weight), args + NORM_BYTES.pack(_ptr(q_weight), _ptr(k_weight), weight_code, eps, offset), "drafts")
+        _launch("norm_rotary_append", (*tensors, q_weight, k_weight), args + NORM_BYTES.pack(_ptr(q_weight), _ptr(k_weight), dtype_code(weight_dtype), eps, offset),
+                "drafts")
 
 
 # ---- attention -----------------------------------------------------------------------------------------------------------
@@ -302,73 +300,67 @@ def adjust_logits(logits: torch.Tensor, *, row_seq: torch.Tensor | None = None, 
     shape = logits.shape
     if len(shape) != 2:
         raise ValueError("logits must be [R, V]")
-    rows, vocab = shape
+    (rows, vocab), (row_stride, stride), dtype = shape, logits.stride(), logits.dtype
+    if vocab < 1 or (stride != 1 and vocab > 1) or (rows > 1 and row_stride < vocab):
+        raise ValueError("logits must be [R, V] with dense rows that do not overlap")
     if out is None:
-        out = logits
-    strides = []
-    for name, t in (("logits", logits), ("out", out)):
-        if t.shape != shape or vocab < 1 or (t.stride(1) != 1 and vocab > 1) or (rows > 1 and t.stride(0) < vocab):
-            raise ValueError(f"{name} must be [R, V] with dense rows that do not overlap")
-        strides.append(t.stride(0) if rows > 1 else vocab)
-    if out.dtype is not logits.dtype and (out.dtype is not _F32 or out.data_ptr() == logits.data_ptr()):
-        raise TypeError("out must have the logits' type, or be another tensor of float32")
-    code, out_code = dtype_code(logits.dtype), dtype_code(out.dtype)
-    sequences, said, said_lens, prompt_lens, width = None, None, None, None, 0
-
-    def per_sequence(name: str, count: int) -> None:
-        nonlocal sequences
-        if sequences is None:
-            sequences = count
-        if count != sequences:
-            raise ValueError(f"{name}: all arguments must be of the same number of sequences")
+        out, out_stride = logits, row_stride
+    else:
+        if out.shape != shape:
+            raise ValueError("out must be [R, V] with dense rows that do not overlap")
+        out_stride, stride = out.stride()
+        if (stride != 1 and vocab > 1) or (rows > 1 and out_stride < vocab):
+            raise ValueError("out must be [R, V] with dense rows that do not overlap")
+        if out.dtype is not dtype and (out.dtype is not _F32 or out.data_ptr() == logits.data_ptr()):
+            raise TypeError("out must have the logits' type, or be another tensor of float32")
+    counts = []                                                       # what the arguments say about the number of sequences
+    said = said_lens = prompt_lens = draft_ids = visible = cu_rows = None
+    width = words = biases = 0
     if history is not None:
         said, said_lens, prompt_lens = history.tokens, history.lens, history.prompt_lens
         _check_ints("the history", said, said_lens, prompt_lens)
-        if len(said.shape) != 2 or said.shape[1] < 1 or said_lens.numel() != said.shape[0] or (prompt_lens is not None and prompt_lens.numel() != said.shape[0]):
+        if len(said.shape) != 2:
             raise ValueError("a history must have tokens [S, width], lens [S] and prompt_lens [S]")
-        width = said.shape[1]
-        per_sequence("history", said.shape[0])
-    draft_ids = visible = cu_rows = None
-    words = 0
+        count, width = said.shape
+        if width < 1 or said_lens.numel() != count or (prompt_lens is not None and prompt_lens.numel() != count):
+            raise ValueError("a history must have tokens [S, width], lens [S] and prompt_lens [S]")
+        counts.append(count)
     if drafts is not None:
         draft_ids, visible, cu_rows = drafts.ids, drafts.visible, drafts.cu_rows
         _check_ints("the drafts' masks and row starts", visible, cu_rows)
         _check_ids("drafted tokens", draft_ids, rows)
         words = _check_visible(visible, rows)
-        per_sequence("drafts", cu_rows.numel() - 1)
-    for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
+        counts.append(cu_rows.numel() - 1)
+    for t in (repetition, frequency, presence):
         if t is not None:
-            if t.dtype is not _F32 or not t.is_contiguous() or len(t.shape) != 1:
-                raise TypeError(f"{name} must be contiguous float32 [S]")
-            per_sequence(name, t.numel())
-    biases = 0
+            if t.dtype is not _F32 or t.dim() != 1 or not t.is_contiguous():
+                raise TypeError("repetition, frequency and presence must be contiguous float32 [S]")
+            counts.append(t.numel())
     if bias_ids is not None or bias_values is not None:
-        if bias_ids is None or bias_values is None or len(bias_ids.shape) != 2 or bias_ids.shape != bias_values.shape:
+        if bias_ids is None or bias_values is None or bias_ids.dim() != 2 or bias_ids.shape != bias_values.shape:
             raise ValueError("bias_ids and bias_values must both be [S, K]")
         _check_ints("bias_ids", bias_ids)
         if bias_values.dtype is not _F32 or not bias_values.is_contiguous():
             raise TypeError("bias_values must be contiguous float32")
-        biases = bias_ids.shape[1]
-        per_sequence("bias_ids", bias_ids.shape[0])
-    if allowed is not None:
-        _check_ints("allowed", allowed)
-        if len(allowed.shape) != 2 or allowed.shape[0] != rows or allowed.shape[1] != (vocab + 31) // 32:
-            raise ValueError("allowed must be [R, ceil(V / 32)]")
-    if row_seq is not None:
-        _check_ints("row_seq", row_seq)
-        if row_seq.numel() != rows:
-            raise ValueError("row_seq must be [R]")
-    if sequences is None:
-        sequences = rows if row_seq is None else 2 ** 31 - 1        # (nothing is a sequence's own: every row that has one)
+        count, biases = bias_ids.shape
+        counts.append(count)
+    _check_ints("allowed and row_seq", allowed, row_seq)
+    if allowed is not None and allowed.shape != (rows, (vocab + 31) // 32):
+        raise ValueError("allowed must be [R, ceil(V / 32)]")
+    if row_seq is not None and row_seq.numel() != rows:
+        raise ValueError("row_seq must be [R]")
+    # (where nothing is a sequence's own, every row that has one counts)
+    sequences = counts[0] if counts else rows if row_seq is None else 2 ** 31 - 1
+    if counts and (sequences < 1 or counts.count(sequences) != len(counts)):
+        raise ValueError("all arguments must be of the same number of sequences, one at least")
     if rows == 0:
         return out
     if row_seq is None and sequences != rows:
         raise ValueError("without row_seq there must be as many sequences as rows")
-    if sequences < 1:
-        raise ValueError("a call takes at least one sequence")
     args = LOGITS_BYTES.pack(logits.data_ptr(), out.data_ptr(), _ptr(row_seq), _ptr(said), _ptr(said_lens), _ptr(prompt_lens), _ptr(draft_ids), _ptr(cu_rows),
-                             _ptr(visible), _ptr(repetition), _ptr(frequency), _ptr(presence), _ptr(bias_ids), _ptr(bias_values), _ptr(allowed), strides[0],
-                             strides[1], rows, sequences, vocab, width, words, biases, code, out_code)
+                             _ptr(visible), _ptr(repetition), _ptr(frequency), _ptr(presence), _ptr(bias_ids), _ptr(bias_values), _ptr(allowed),
+                             row_stride if rows > 1 else vocab, out_stride if rows > 1 else vocab, rows, sequences, vocab, width, words, biases, dtype_code(dtype),
+                             dtype_code(out.dtype))
     _launch("adjust_logits", (logits, out, row_seq, said, said_lens, prompt_lens, draft_ids, cu_rows, visible, repetition, frequency, presence, bias_ids,
                               bias_values, allowed), args, "drafts")
     return out
