@@ -32,7 +32,7 @@ constexpr int kFirst = 96;                     // .. whose probabilities go to t
 constexpr int kRows = 128;                     // query rows of a group of warps
 constexpr int kThreads = 384;
 constexpr int kMaxHeadsPerKv = 64;
-constexpr int kWholeTiles = 4;                 // tokens that tables have room for, in tiles, up to which items are not cut
+constexpr int kWholeTiles = 8;                 // tokens that tables have room for, in tiles, up to which items are not cut
 constexpr int kPlanThreads = 128;              // that lay the plan out, some sequences each
 constexpr float kAhead = 6.f;                  // a new reference is the maximum less this: probabilities start at 2^6 ..
 constexpr float kStale = 14.f;                 // .. and may grow to 2^14 (in fp16: 2^-24 of that is still a number)
@@ -77,7 +77,7 @@ struct Division {
 // An item of n key tiles is kItemUnits + n kTileUnits units (kTwoUnits where two groups of warps have rows of their own, whose tiles take the longer the less
 // the memory is waited for): what it costs to begin with (queries, the first tile's latency, the output) is about that of two tiles. The units are dealt out
 // as evenly as whole numbers can be; a block has the tiles whose first unit is its own. Where items are not cut, each is a unit.
-constexpr int kItemUnits = 4;
+constexpr int kItemUnits = 6;
 constexpr int kTileUnits = 2;
 constexpr int kTwoUnits = 3;
 
@@ -180,17 +180,19 @@ struct Item {
   int tile, tiles, keys;       // (tiles 0: there are no more items)
   int flags;                   // 1: begins here, 2: ends here
 };
-constexpr int kItems = 8;      // in shared memory: the keys' warp, which goes through them, is up to six ahead of the softmax
 
 template <int D>
 struct Smem {
   static constexpr int kSlotBytes = kKeys * D * 2;
   static constexpr int kSlots = D == 128 ? 5 : 10;
   static constexpr int kQBytes = kRows * D * 2;
+  // Items in shared memory. The keys' warp, which goes through them, is no more tiles ahead of the outputs than there are slots (where their number is even, of the
+  // scores, which are two steps ahead of the outputs), and a group of warps may be an item behind these.
+  static constexpr int kItems = D == 128 ? 8 : 16;
   static constexpr int kTiles = 2 * kQBytes + kSlots * kSlotBytes;
-  // then: barriers of keys, of values, empty, clean [slots], q[2], place of q[2], s[2], p[2][2], o[2], end[2], items; tensor memory address; items; starts of runs, and later
-  // maxima and denominators of the second group of warps
-  static constexpr int kBarriers = 4 * kSlots + 14 + kItems;
+  // then: barriers of keys, of values, empty, clean [slots], q[2], place of q[2], s[2], p[2][2], o[2], given[2], taken[2], items; tensor memory address; items; starts of runs, and later
+  // maxima and denominators that one group of warps hands to the other
+  static constexpr int kBarriers = 4 * kSlots + 16 + kItems;
   static constexpr int kBytes = 1024 + kTiles + kBarriers * 8 + 16 + kItems * static_cast<int>(sizeof(Item)) + kRows * 8;
 };
 
@@ -223,12 +225,12 @@ __device__ __noinline__ void add_spoilt(const cacheir_b200_tree_args& a, const T
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool RUN_ON>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_q,
             const __grid_constant__ FastParams p) {
   using L = Smem<D>;
-  constexpr int kSlots = L::kSlots;
+  constexpr int kSlots = L::kSlots, kItems = L::kItems;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* s_q = smem;                                         // [2][D / 64][128 rows][128 B]
@@ -244,8 +246,9 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
   uint64_t* bar_s = bar_free + 2;                              // scores are in tensor memory
   uint64_t* bar_p = bar_s + 2;                                 // probabilities are, [group of warps][first keys, the others]
   uint64_t* bar_o = bar_p + 4;                                 // .. and have been added to the output
-  uint64_t* bar_end = bar_o + 2;                               // the second group's part of an item is done, and has been joined to the first one's
-  uint64_t* bar_item = bar_end + 2;                            // the item is known
+  uint64_t* bar_given = bar_o + 2;                             // a group's part of an item is done
+  uint64_t* bar_taken = bar_given + 2;                         // .. and has been added to the other one's
+  uint64_t* bar_item = bar_taken + 2;                            // the item is known
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_item + kItems);
   Item* s_item = reinterpret_cast<Item*>(tmem_slot + 4);
   int* s_start = reinterpret_cast<int*>(s_item + kItems);
@@ -273,8 +276,9 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
       mbar_init(smem_u32(&bar_p[2 * w]), kRows);
       mbar_init(smem_u32(&bar_p[2 * w + 1]), kRows);
       mbar_init(smem_u32(&bar_o[w]), 1);
+      mbar_init(smem_u32(&bar_given[w]), 4);
+      mbar_init(smem_u32(&bar_taken[w]), 4);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&bar_end[i]), 4);
     for (int i = 0; i < kItems; ++i) mbar_init(smem_u32(&bar_item[i]), 1);
     mbar_fence_init();
   }
@@ -450,64 +454,105 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
     const uint32_t id_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) |
                           (static_cast<uint32_t>(kRows >> 4) << 24);
     const uint64_t dq = smem_desc_sw128(smem_u32(s_q)), dk = smem_desc_sw128(smem_u32(s_kv)), dv = smem_desc_columns(smem_u32(s_kv));
-    // An item's steps: a tile each, or a tile for either group of warps; step j belongs to group j & 1. Scores are two steps ahead of outputs, and
-    // are issued right behind the output that frees their buffer.
+    // An item's steps: a tile each, or a tile for either half of the rows. They go to the two groups of warps in turn; scores are two steps ahead of outputs, and are
+    // issued right behind the output that frees their place. RUN_ON: both also across the end of an item, so that items of one tile keep both groups at work.
     const bool leader = elect_one();
-    int k_slot = 0, v_slot = 1, k_turn = 0, v_turn = 0, q_place = 0;    // slots; barriers; place of the queries of an item that both groups share
-    uint32_t k_phase = 0, v_phase = 0, q_phase = 0, p_phase = 0;    // (of the two buffers of queries and probabilities: a bit each)
-    while (next_item()) {
-      const bool two = it.rows > half_rows;
-      const int steps = two ? 2 * it.tiles : it.tiles;
-      auto wait_scores = [&](int j) {                          // the operands of step j's scores
-        if (j < (two ? 2 : 1)) {                               // the item's queries are new
-          const int w = two ? j : q_place;
-          if (!warp_wait(smem_u32(&bar_q[w]), q_phase >> w & 1, (15 << 8) | 3)) return false;
-          q_phase ^= 1u << w;
-        }
-        return (two && (j & 1)) || warp_wait(smem_u32(&key_full[k_turn]), k_phase, (15 << 8) | 4);
-      };
-      auto score = [&](int j) {                                // (one lane)
-        const uint64_t q_at = dq + ((two ? j & 1 : q_place) * L::kQBytes >> 4), k_at = dk + (k_slot * L::kSlotBytes >> 4);
-        const uint32_t to = tmem + (j & 1) * kKeys;
+    auto load_item = [&](int& n, Item& into) {
+      const int place = n % kItems;
+      ok = ok && warp_wait(smem_u32(&bar_item[place]), (n / kItems) & 1, (15 << 8) | 14);
+      if (!ok) return false;
+      into = s_item[place];
+      ++n;
+      return into.tiles > 0;
+    };
+    // the scores' side
+    int s_items = 0, s_step = 0, s_steps = 0, s_place = 0, s_group = 0, k_slot = 0, k_turn = 0;         // (s_place: of the next shared queries)
+    uint32_t k_phase = 0, q_phase = 0;                         // (q_phase: a bit for either place)
+    bool s_two = false, s_more = true;
+    uint64_t s_queries = dq;                                   // descriptor of the item's queries (of its first half)
+    // Waits for what the next step's scores need; false where there is no further step, or a wait gave up.
+    auto prepare = [&] {
+      if (!s_more) return false;
+      if (s_step == s_steps) {
+        Item next;
+        s_more = load_item(s_items, next);
+        if (!s_more) return false;
+        s_two = next.rows > half_rows;
+        s_steps = s_two ? 2 * next.tiles : next.tiles;
+        s_step = 0;
+        s_queries = dq + (s_two ? 0 : s_place * L::kQBytes >> 4);
+      }
+      if (s_step < (s_two ? 2 : 1)) {                          // the item's queries are new
+        const int place = s_two ? s_step : s_place;
+        ok = warp_wait(smem_u32(&bar_q[place]), q_phase >> place & 1, (15 << 8) | 3);
+        q_phase ^= 1u << place;
+      }
+      if (!(s_two && (s_step & 1))) ok = ok && warp_wait(smem_u32(&key_full[k_turn]), k_phase, (15 << 8) | 4);
+      return ok;
+    };
+    auto score = [&] {                                         // (one lane)
+      const bool second = s_two && (s_step & 1);
+      const uint64_t q_at = s_queries + (second ? L::kQBytes >> 4 : 0), k_at = dk + (k_slot * L::kSlotBytes >> 4);
+      const uint32_t to = tmem + s_group * kKeys;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          constexpr int kHalf = kRows * 128 >> 4;              // 64 columns further
-          mma_ss(to, q_at + (k >> 2) * kHalf + (k & 3) * 2, k_at + (k >> 2) * kHalf + (k & 3) * 2, id_s, k > 0 ? 1u : 0u);
-        }
-        tc_commit(smem_u32(&bar_s[j & 1]));
-        if (!two || (j & 1)) tc_commit(smem_u32(&empty[k_slot]));
-        if (j >= (two ? steps - 2 : steps - 1)) tc_commit(smem_u32(&bar_free[two ? j & 1 : q_place]));      // (the last that look at these queries)
-      };
-      auto scored = [&](int j) {                               // (the whole warp)
-        if (!two || (j & 1)) {
-          k_slot += 2;
-          if (k_slot >= kSlots) k_slot -= kSlots;
-          if (++k_turn == kSlots) { k_turn = 0; k_phase ^= 1; }
-        }
-      };
-      for (int j = 0; j < 2 && j < steps && ok; ++j) {
-        ok = wait_scores(j);
-        if (!ok) break;
+      for (int k = 0; k < D / 16; ++k) {
+        constexpr int kHalf = kRows * 128 >> 4;                // 64 columns further
+        mma_ss(to, q_at + (k >> 2) * kHalf + (k & 3) * 2, k_at + (k >> 2) * kHalf + (k & 3) * 2, id_s, k > 0 ? 1u : 0u);
+      }
+      tc_commit(smem_u32(&bar_s[s_group]));
+      if (!s_two || second) tc_commit(smem_u32(&empty[k_slot]));
+      if (s_step >= s_steps - (s_two ? 2 : 1)) tc_commit(smem_u32(&bar_free[s_two ? s_step & 1 : s_place]));        // (the last that look at these queries)
+    };
+    auto scored = [&] {                                        // (the whole warp)
+      if (!s_two || (s_step & 1)) {
+        k_slot += 2;
+        if (k_slot >= kSlots) k_slot -= kSlots;
+        if (++k_turn == kSlots) { k_turn = 0; k_phase ^= 1; }
+      }
+      ++s_step;
+      s_group ^= 1;
+      if (s_step == s_steps && !s_two) s_place ^= 1;
+    };
+    auto first_scores = [&] {
+      for (int j = 0; j < 2; ++j) {
+        if (!prepare()) break;
         tc_fence_after();
-        if (leader) score(j);
+        if (leader) score();
         __syncwarp();
-        scored(j);
+        scored();
+        if (!RUN_ON && s_step == s_steps) break;
+      }
+    };
+    if (RUN_ON) first_scores();
+    // the outputs' side
+    int a_items = 0, group_of = 0, v_slot = 1, v_turn = 0;
+    uint32_t v_phase = 0, p_phase = 0;                         // (p_phase: a bit for either group)
+    Item add_item;
+    while (ok && load_item(a_items, add_item)) {
+      const bool two = add_item.rows > half_rows;
+      const int steps = two ? 2 * add_item.tiles : add_item.tiles;
+      if (!RUN_ON) {
+        s_group = group_of = 0;
+        first_scores();
       }
       for (int j = 0; j < steps && ok; ++j) {
-        const int w = j & 1;
-        if (!(two && w)) ok = warp_wait(smem_u32(&bar_clean[v_turn]), v_phase, (15 << 8) | 5);
+        const int w = group_of;
+        const bool frees = !two || (j & 1);
+        if (!(two && (j & 1))) ok = warp_wait(smem_u32(&bar_clean[v_turn]), v_phase, (15 << 8) | 5);
         ok = ok && warp_wait(smem_u32(&bar_p[2 * w]), p_phase >> w & 1, (15 << 8) | 6);
         if (!ok) break;
         tc_fence_after();
         const uint64_t v_at = dv + (v_slot * L::kSlotBytes >> 4);
         const uint32_t to = tmem_o + w * D, from = tmem + w * kKeys, add = j < 2 ? 0u : 1u;
-        const bool frees = !two || w, more = j + 2 < steps;
         if (leader) {                                          // (the first keys while the others' probabilities are worked out)
 #pragma unroll
           for (int k = 0; k < kFirst / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, k == 0 ? add : 1u);
         }
         __syncwarp();
-        if (more) ok = wait_scores(j + 2);
+        // (mostly the item goes on, and its next keys are all there is to wait for: this warp's chain of instructions is what the tensor cores wait for)
+        bool more;
+        if (s_step >= 2 && s_step < s_steps) more = ok = (s_two && (s_step & 1)) || warp_wait(smem_u32(&key_full[k_turn]), k_phase, (15 << 8) | 4);
+        else more = RUN_ON && prepare();
         ok = ok && warp_wait(smem_u32(&bar_p[2 * w + 1]), p_phase >> w & 1, (15 << 8) | 6);
         if (!ok) break;
         tc_fence_after();
@@ -516,18 +561,18 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
           for (int k = kFirst / 16; k < kKeys / 16; ++k) mma_ts(to, from + k * 8, v_at + k * (kChunk * D * 2 >> 4), id_o, 1u);
           tc_commit(smem_u32(&bar_o[w]));
           if (frees) tc_commit(smem_u32(&empty[v_slot]));
-          if (more) score(j + 2);
+          if (more) score();
         }
         __syncwarp();
         p_phase ^= 1u << w;
+        group_of ^= 1;
         if (frees) {
           v_slot += 2;
           if (v_slot >= kSlots) v_slot -= kSlots;
           if (++v_turn == kSlots) { v_turn = 0; v_phase ^= 1; }
         }
-        if (more) scored(j + 2);
+        if (more) scored();
       }
-      if (!two) q_place ^= 1;
     }
   } else {
     // ---------------- softmax: a thread per query row ----------------
@@ -535,30 +580,44 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int by_group = (65536 + group - 1) / group;          // n / group = n * by_group >> 16 for n < 256, group <= 64
     const int token = r * by_group >> 16, head_of = r - token * group;
-    uint32_t s_phase = 0, o_phase = 0, end_phase = 0;
-    bool lent = false;                                         // (second group) its output has not been joined yet
-    while (next_item()) {
-      const bool two = it.rows > half_rows;
-      const int in_item = (two ? w * half_rows : 0) + token;   // this thread's token of the item
-      const bool real = r < half_rows * group && in_item < it.rows;
+    uint32_t s_phase = 0, o_phase = 0, given_phase = 0, taken_phase = 0;
+    bool lent = false;                                         // this group's output has not been added to the other one's yet
+    int before = 0;                                            // steps of the items before, modulo 2: they go to the groups in turn
+    // (an item's numbers stay in shared memory: in registers they were spilled)
+    for (;; ) {
+      const int ring = item % kItems;
+      ok = ok && warp_wait(smem_u32(&bar_item[ring]), (item / kItems) & 1, (15 << 8) | 14);
+      if (!ok) break;
+      ++item;
+      const Item& now = s_item[ring];
+      if (now.tiles <= 0) break;
+      const bool two = now.rows > half_rows;
+      // which half of the rows is this group's, or its first tile (the group that has the item's first tile also stores what comes of it)
+      const int place_of = w ^ before;
+      if (!two) {
+        if (RUN_ON) before ^= now.tiles & 1;
+        if (place_of >= now.tiles) continue;                    // (an item of one tile, which is the other group's)
+      }
+      const int in_item = (two ? place_of * half_rows : 0) + token;      // this thread's token of the item
+      const bool real = r < half_rows * group && in_item < now.rows;
       const bool idle = !__any_sync(0xffffffffu, real);        // (a warp without rows: whatever it leaves as probabilities goes to outputs of nobody)
-      const int row = it.row0 + (real ? in_item : 0), head = it.kvh * group + head_of;
-      const int masked_from = min(it.s.front, it.keys);    // keys behind this need a look at the row's mask
+      const int row = now.row0 + (real ? in_item : 0), head = now.kvh * group + head_of;
+      const int masked_from = min(now.s.front, now.keys);    // keys behind this need a look at the row's mask
       float m_ref = -INFINITY, l_run = 0.f;
       int steps = 0;
-      for (int t = two ? 0 : w; t < it.tiles && ok; t += two ? 1 : 2, ++steps) {
-        const int base = (it.tile + t) * kKeys;
+      for (int t = two ? 0 : place_of; t < now.tiles && ok; t += two ? 1 : 2, ++steps) {
+        const int base = (now.tile + t) * kKeys;
         const bool whole = base + kKeys <= masked_from;
         uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
         if (!whole) {                                          // 128 bits of the row, from the tile's first key on
-          const int from = base - it.s.front, sh = from & 31;
-          uint32_t low = tree_word(a, it.s, row, from >> 5);
+          const int from = base - now.s.front, sh = from & 31;
+          uint32_t low = tree_word(a, now.s, row, from >> 5);
           if (from >> 5 < 0) low = 0xffffffffu;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int q = (from >> 5) + i + 1;
-            const uint32_t high = q < 0 ? 0xffffffffu : tree_word(a, it.s, row, q);
-            const int left = it.keys - base - 32 * i;        // keys there are from this word on
+            const uint32_t high = q < 0 ? 0xffffffffu : tree_word(a, now.s, row, q);
+            const int left = now.keys - base - 32 * i;        // keys there are from this word on
             see[i] = __funnelshift_r(low, high, sh) & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
             low = high;
           }
@@ -569,8 +628,8 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
         auto returned = [&] {                                  // the output may be written over
           if (!lent) return;
           lent = false;
-          ok = warp_wait(smem_u32(&bar_end[1]), end_phase, (15 << 8) | 13) && ok;
-          end_phase ^= 1;
+          ok = warp_wait(smem_u32(&bar_taken[w]), taken_phase, (15 << 8) | 13) && ok;
+          taken_phase ^= 1;
         };
         if (idle) {
           returned();
@@ -671,34 +730,27 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
       }
       if (!ok) break;
       // ---- the item's end ----
-      if (steps > 0) {                                         // (the phase of this group's last output; those before it have not been waited for)
-        o_phase ^= (steps - 1) & 1;
-        ok = warp_wait(smem_u32(&bar_o[w]), o_phase, (15 << 8) | 11);
-        if (!ok) break;
-        o_phase ^= 1;
-      }
+      o_phase ^= (steps - 1) & 1;                              // (the phase of this group's last output; those before it have not been waited for)
+      ok = warp_wait(smem_u32(&bar_o[w]), o_phase, (15 << 8) | 11);
+      if (!ok) break;
+      o_phase ^= 1;
       tc_fence_after();
-      // An item that both groups have had: the second one leaves its maxima and denominators and goes on, the first one adds its output to its own. (Each of them
-      // storing half of the columns, and waiting for the other one three times, took 2 us an item longer.)
+      // An item that both groups have had: one leaves its maxima and denominators and goes on, the one that had the first tile adds its output to its own. (Each of
+      // them storing half of the columns, and waiting for the other one three times, took 2 us an item longer.)
       float f_own = 1.f, f_other = 0.f;
-      if (!two && w == 1) {
-        if (lent) {                                            // (an item of one tile, of which this group had none: the last one may not have been joined)
-          lent = false;
-          ok = warp_wait(smem_u32(&bar_end[1]), end_phase, (15 << 8) | 13);
-          if (!ok) break;
-          end_phase ^= 1;
-        }
+      if (!two && place_of == 1) {
         s_ml[r] = make_float2(m_ref, l_run);
         lent = true;
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_end[0]));
+        if (lane == 0) mbar_arrive(smem_u32(&bar_given[w]));
         continue;
       }
-      if (!two) {
-        ok = warp_wait(smem_u32(&bar_end[0]), end_phase, (15 << 8) | 13);
+      const bool joins = !two && now.tiles > 1;
+      if (joins) {
+        ok = warp_wait(smem_u32(&bar_given[w ^ 1]), given_phase, (15 << 8) | 13);
         if (!ok) break;
-        end_phase ^= 1;
+        given_phase ^= 1;
         tc_fence_after();
         const float2 other = s_ml[r];
         const float m = fmaxf(m_ref, other.x);
@@ -708,13 +760,13 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
         l_run = l_run * (m_ref > -INFINITY ? f_own : 1.f) + other.y * (other.x > -INFINITY ? f_other : 1.f);
         m_ref = m;
       }
-      const bool direct = it.flags == 3;
+      const bool direct = now.flags == 3;
       if (!idle) {
         const float scale = direct ? (l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f) : 1.f;
         f_own *= scale;
         f_other *= scale;
-        const size_t place = (static_cast<size_t>(2 * blockIdx.x + (it.flags & 1)) * 2 + (two ? w : 0));          // of the piece in the scratch
-        T* const to = static_cast<T*>(a.out) + static_cast<size_t>(it.s.row + row) * a.out_stride + static_cast<size_t>(head) * D;
+        const size_t place = (static_cast<size_t>(2 * blockIdx.x + (now.flags & 1)) * 2 + (two ? place_of : 0));          // of the piece in the scratch
+        T* const to = static_cast<T*>(a.out) + static_cast<size_t>(now.s.row + row) * a.out_stride + static_cast<size_t>(head) * D;
         float* const acc = p.acc + place * (kRows * D) + r * 4;
         if (!direct && real) *reinterpret_cast<float2*>(p.ml + (place * kRows + r) * 2) = make_float2(m_ref, l_run);
 #pragma unroll 1
@@ -727,8 +779,8 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = f_own != 0.f ? __uint_as_float(x[i]) * f_own : 0.f;
-          if (!two && __any_sync(0xffffffffu, f_other != 0.f)) {
-            tmem_ld_x32(tmem_o + D + lane_addr + c, x);
+          if (joins && __any_sync(0xffffffffu, f_other != 0.f)) {
+            tmem_ld_x32(tmem_o + (w ^ 1) * D + lane_addr + c, x);
             tmem_wait_ld(x);
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = f_other != 0.f ? fmaf(__uint_as_float(x[i]), f_other, o[i]) : o[i];
@@ -753,15 +805,15 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
             for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(acc + (c + i) * kRows) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
         }
-        if (s_spoilt[(item - 1) % kItems] == item && real) {
-          const int32_t* pages = a.page_table + static_cast<size_t>(it.b) * a.max_pages;
-          if (direct) add_spoilt<T, D, T>(a, it.s, pages, row, head, it.tile, it.tiles, it.keys, to);
-          else add_spoilt<T, D, float>(a, it.s, pages, row, head, it.tile, it.tiles, it.keys, acc);
+        if (s_spoilt[ring] == item && real) {
+          const int32_t* pages = a.page_table + static_cast<size_t>(now.b) * a.max_pages;
+          if (direct) add_spoilt<T, D, T>(a, now.s, pages, row, head, now.tile, now.tiles, now.keys, to);
+          else add_spoilt<T, D, float>(a, now.s, pages, row, head, now.tile, now.tiles, now.keys, acc);
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (!two && lane == 0) mbar_arrive(smem_u32(&bar_end[1]));
+      if (joins && lane == 0) mbar_arrive(smem_u32(&bar_taken[w ^ 1]));
     }
   }
   __syncwarp();
@@ -860,9 +912,12 @@ int launch_fast(const cacheir_b200_tree_args& a, cudaStream_t stream) {
   p.joins = static_cast<TreeJoin*>(a.workspace);
   p.ml = reinterpret_cast<float*>(p.joins + kNumSMs);
   p.acc = p.ml + static_cast<size_t>(kNumSMs) * 2 * 2 * kRows * 2;
-  auto kern = tree_kernel<T, D>;
-  static std::atomic<unsigned long long> done{0};
-  cudaError_t e = allow_shared_memory(done, reinterpret_cast<const void*>(kern), Smem<D>::kBytes);
+  // Blocks with several short items each go on from one to the next (150 sequences of up to 66 tokens, 32 query and 8 key/value heads of 64: 43.8 us without, 35.5 with;
+  // 16 trees on long sequences: 183.6 without, 192.9 with, as the warp that issues the products has more to look after).
+  const bool run_on = p.whole && (a.rows / (2 * p.half_rows) + static_cast<long long>(a.sequences)) * a.kv_heads > 2 * kNumSMs;
+  auto kern = run_on ? tree_kernel<T, D, true> : tree_kernel<T, D, false>;
+  static std::atomic<unsigned long long> done[2]{{0}, {0}};
+  cudaError_t e = allow_shared_memory(done[run_on], reinterpret_cast<const void*>(kern), Smem<D>::kBytes);
   if (e == cudaSuccess) e = launch_chained(kern, dim3(grid), dim3(kThreads), Smem<D>::kBytes, stream, tk, tv, tq, p);
   if (e == cudaSuccess && !p.whole) e = launch_chained(tree_pieces_kernel<T, D>, dim3(grid, 2), dim3(kJoinThreads), 0, stream, p);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();

@@ -300,6 +300,17 @@ def test_blocks_with_many_items_of_many_tiles(dim, heads, kv_heads):
     assert _lib.load_group("drafts").cacheir_b200_drafts_device_status(0) == 0
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("most", [60, 300, 900])
+def test_blocks_with_many_short_items(dim, most):
+    """Items of one tile, of two and of three, of one half of the rows and of both, one after the other in every block."""
+    from cacheir_b200 import _lib
+    rng = random.Random(dim + most)
+    ctx, nodes = [rng.choice([0, 3, 90, 150, most]) for _ in range(200)], [rng.choice([0, 1, 2, 20]) for _ in range(200)]
+    Case(heads=32, kv_heads=4, dim=dim, ctx=ctx, nodes=nodes, lists=None, dtype=F16, seed=dim).check()
+    assert _lib.load_group("drafts").cacheir_b200_drafts_device_status(0) == 0
+
+
 @pytest.mark.parametrize("lists", ["tree", None])
 def test_long_context_in_many_pieces(lists):
     got = Case(heads=4, kv_heads=1, ctx=(40000, 77), nodes=(6, 3), lists=lists, dtype=BF16, wide_q=2).check()
