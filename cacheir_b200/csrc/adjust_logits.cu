@@ -9,6 +9,10 @@
 // copies of the penalties' code a vector, of which instruction fetches alone took half the time (512 rows of 128256, 4096 tokens said: 325 us).
 // Drafted tokens are a short list beside the counts, of which every row takes those that it sees. Counts are integers: the order of the
 // additions does not matter.
+//
+// 512 rows of 128256 in bf16 (32 sequences of up to 4096 tokens, 16 drafted rows each, a grammar): 81 us, of which 41 us are the bytes at the copy's rate; with the grammar
+// alone 50 us. The rest is latency: a block counts before its pass (5 us, 3000 tokens in four rounds of loads and three barriers) and changes listed
+// tokens behind it (3 us, 13 where the frequent tokens are), and only the other blocks of its SM are at work meanwhile. 64 rows of 50001 in fp32 9.1 us, one row 3.8 us.
 #include "cacheir_b200_drafts.h"
 #include "common.cuh"
 #include "serving_status.h"
@@ -19,7 +23,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kSlice = 4096;                           // tokens of a block, at most
 constexpr int kPairs = 2;                             // logits of listed tokens that a thread has under way
-constexpr int kRun = 8;                                // rows of a block, at most (16: 111 us for 95, as there are fewer blocks to even the work out)
+constexpr int kRun = 8;                                // rows of a block, at most (16 took 111 us where 8 took 95, as there are fewer blocks to even the work out)
 constexpr int kSaid = 4;                               // tokens of the history that a thread has under way
 constexpr uint32_t kInPrompt = 0x80000000u;
 constexpr uint32_t kDrafted = 0x40000000u;             // the list of drafted tokens has the token

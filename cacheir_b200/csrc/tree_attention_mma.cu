@@ -10,7 +10,7 @@
 // softmax, a thread per query row, each with scores, probabilities and an output of its own in tensor memory. Above 128 query rows each group
 // has its own 128 of them and both use the same keys. With fewer, which is what decoding with drafts has mostly, both have the same
 // rows and take turns with the key tiles: what bounds such an item is the memory's rate, and one group alone would not keep up with it. The two halves are added up
-// from tensor memory at the item's end.
+// from tensor memory at the item's end, by the group that had its first tile, while the other one is at work on the next item.
 //
 // Masks are looked at only in tiles that hold drafted tokens: 128 bits a row, shifted to the tile. Whatever stands in a key that a row does not
 // see, its weight is 0; but 0 times a value that is no number is none. So one more warp looks through the drafted tokens' values before the second product has them, puts
@@ -18,6 +18,14 @@
 //
 // A row's maximum is a reference that moves only when it is exceeded by 2^14, so that outputs are hardly ever rescaled; probabilities are rounded to
 // the element type as the second MMA's operand, their sums are not.
+//
+// Measured (both kernels, replayed from a graph; 32 query and 8 key/value heads of 128 in fp16 where nothing else is said): 32 trees of 12 to 16 tokens behind 256 to
+// 4096 75 us, of which 47 us are the bytes; 4 chains of up to 5 tokens behind 90000 to 131072 315 to 330 us (bytes 263); 16 trees of 40 to 64 tokens behind 1000 to
+// 8192, 64 heads, bf16, 180 to 190 us (products 80, at the rate of short bursts); two trees of 8 tokens behind 300 10.6 us. In the main loop an item of one group's
+// rows takes 1.5 us a tile, which is the memory's rate; one of two groups' rows 1.8 us, 3300 cycles, of which the tensor cores work 2048: probabilities lie over the scores that they come from,
+// so that a group's scores, softmax (1024 cycles of exponentials alone) and second product follow one another, and only the other group's fill the gaps. First scores come
+// 4 to 7 us after the launch, an item's end takes 1.5 to 3 us, the pieces 5. Scores of 64 keys at a time, in two places a group, would close the gaps,
+// but the tensor cores take as long for 64 keys as for 128 (the queries are read again): 84, 372 and 216 us for the first three.
 #include "attention_ptx.cuh"
 #include "hybrid_common.cuh"
 #include "tree_attention.cuh"
@@ -32,7 +40,9 @@ constexpr int kFirst = 96;                     // .. whose probabilities go to t
 constexpr int kRows = 128;                     // query rows of a group of warps
 constexpr int kThreads = 384;
 constexpr int kMaxHeadsPerKv = 64;
-constexpr int kWholeTiles = 8;                 // tokens that tables have room for, in tiles, up to which items are not cut
+// Tokens that tables have room for, in tiles, up to which items are not cut: joining their pieces takes longer than a block takes for all of them (67 sequences of up to 502
+// tokens 52 us, cut 57; 3 of up to 897 with one key/value head 13.2, cut 15.7).
+constexpr int kWholeTiles = 8;
 constexpr int kPlanThreads = 128;              // that lay the plan out, some sequences each
 constexpr float kAhead = 6.f;                  // a new reference is the maximum less this: probabilities start at 2^6 ..
 constexpr float kStale = 14.f;                 // .. and may grow to 2^14 (in fp16: 2^-24 of that is still a number)
@@ -75,8 +85,9 @@ struct Division {
 
 // ---- how the work is cut ----
 // An item of n key tiles is kItemUnits + n kTileUnits units (kTwoUnits where two groups of warps have rows of their own, whose tiles take the longer the less
-// the memory is waited for): what it costs to begin with (queries, the first tile's latency, the output) is about that of two tiles. The units are dealt out
-// as evenly as whole numbers can be; a block has the tiles whose first unit is its own. Where items are not cut, each is a unit.
+// the memory is waited for): what it costs to begin with (queries, the first tile's latency, the output) is about that of three tiles. The units are dealt out
+// as evenly as whole numbers can be; a block has the tiles whose first unit is its own. Where items are not cut, each is a unit. (32 trees and 16 wide ones: 6, 2, 3 units
+// 75.9 and 186 us; 4, 2, 3 75.0 and 193; 2, 2, 3 75.0 and 200; 4, 2, 4 75.0 and 221; 3, 2, 2 74.6 and 190.)
 constexpr int kItemUnits = 6;
 constexpr int kTileUnits = 2;
 constexpr int kTwoUnits = 3;
@@ -906,7 +917,6 @@ int launch_fast(const cacheir_b200_tree_args& a, cudaStream_t stream) {
     return CACHEIR_B200_EUNSUPPORTED;
   const long long most = most_units(a);
   const int grid = static_cast<int>(most < kNumSMs ? most : kNumSMs);
-  // Items of few tiles are not cut: joining their pieces takes longer than a block takes for all of them.
   p.whole = static_cast<long long>(a.max_pages) * a.page_size <= kWholeTiles * kKeys;
   p.out_wide = aligned_to(a.out, 32) && a.out_stride % 16 == 0;
   p.joins = static_cast<TreeJoin*>(a.workspace);
