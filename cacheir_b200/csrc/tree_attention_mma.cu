@@ -348,23 +348,29 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
       for (int t = it.tile; t < it.tile + it.tiles && ok; ++t) {
         ok = warp_wait(smem_u32(&value_full[turn]), phase, (15 << 8) | 12);
         if (!ok) break;
-        const int base = t * kKeys, from = max(min(it.s.front, it.keys) - base, 0);
-        if (from < kKeys) {
+        // (behind the 16 keys in which the last one lies there are zeros already)
+        const int base = t * kKeys, from = max(min(it.s.front, it.keys) - base, 0), until = min((it.keys - base + kChunk - 1) / kChunk * kChunk, kKeys);
+        if (from < until) {
           bool spoilt = false;
-          for (int key = from + lane / kLanes; key < kKeys; key += 32 / kLanes) {
+          constexpr int kAtOnce = 2;                           // 16-byte words of a lane under way
+          for (int first = from + lane / kLanes; first < until; first += kAtOnce * (32 / kLanes)) {
             const int c = lane % kLanes;
-            uint4* at = reinterpret_cast<uint4*>(s_kv + slot * L::kSlotBytes + (key / kChunk) * kChunk * D * 2 + (c >> 3) * kChunk * 128 + key % kChunk * 128 +
-                                                 ((c & 7) << 4));
-            if (base + key >= it.keys) {
-              *at = make_uint4(0u, 0u, 0u, 0u);
-              continue;
-            }
-            uint4 v = *at;
-            const uint32_t bad[4] = {__vcmpeq2(v.x & kExponent, kExponent), __vcmpeq2(v.y & kExponent, kExponent), __vcmpeq2(v.z & kExponent, kExponent),
-                                     __vcmpeq2(v.w & kExponent, kExponent)};
-            if (bad[0] | bad[1] | bad[2] | bad[3]) {
-              spoilt = true;
-              *at = make_uint4(v.x & ~bad[0], v.y & ~bad[1], v.z & ~bad[2], v.w & ~bad[3]);
+            auto word = [&](int key) {
+              return reinterpret_cast<uint4*>(s_kv + slot * L::kSlotBytes + (key / kChunk) * kChunk * D * 2 + (c >> 3) * kChunk * 128 + key % kChunk * 128 + ((c & 7) << 4));
+            };
+            uint4 v[kAtOnce];
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) v[e] = *word(min(first + e * (32 / kLanes), until - 1));
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) {
+              const int key = first + e * (32 / kLanes);
+              const uint32_t bad[4] = {__vcmpeq2(v[e].x & kExponent, kExponent), __vcmpeq2(v[e].y & kExponent, kExponent), __vcmpeq2(v[e].z & kExponent, kExponent),
+                                       __vcmpeq2(v[e].w & kExponent, kExponent)};
+              const bool behind = base + key >= it.keys;       // (nobody sees it)
+              if (key < until && (behind || (bad[0] | bad[1] | bad[2] | bad[3]))) {
+                spoilt = spoilt || !behind;
+                *word(key) = behind ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(v[e].x & ~bad[0], v[e].y & ~bad[1], v[e].z & ~bad[2], v[e].w & ~bad[3]);
+              }
             }
           }
           if (__any_sync(0xffffffffu, spoilt) && lane == 0) s_spoilt[(item - 1) % kItems] = item;
@@ -837,15 +843,15 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
 }
 
 // ---- the pieces of items that were cut ----
-// A block per (block of the first kernel, group of warps of its item), a lane a query row and every fourth four columns, pieces in their order. Output rows are
-// put together in shared memory, so that a store writes whole lines.
+// A block per (block of the first kernel, group of warps of its item), a lane a query row, pieces in their order. Up to 32 rows a warp has them all and a sixteenth of the
+// columns, and with fewer rows its lanes share the pieces out as well (one row of 32 heads behind 100000 tokens, 19 pieces of four query rows each: 33 us with a row's lane for itself).
+// Output rows are put together in shared memory, so that a store writes whole lines.
 constexpr int kJoinThreads = 512;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
 tree_pieces_kernel(const FastParams p) {
   chain_enter();
-  constexpr int kFours = D / 4 * kRows / kJoinThreads;         // of a thread
   constexpr int kLine = D * 2 + 16;                            // bytes of a row in shared memory (so that lanes beside one another reach different banks)
   __shared__ __align__(16) uint8_t s_out[kRows * kLine];
   const TreeJoin j = p.joins[blockIdx.x];
@@ -854,38 +860,70 @@ tree_pieces_kernel(const FastParams p) {
   const cacheir_b200_tree_args& a = p.a;
   const int group = a.heads / a.kv_heads, n = static_cast<int>(blockIdx.x) - j.first + 1;
   const int rows = min(p.half_rows, j.rows - group_of * p.half_rows) * group;        // query rows that there are
-  const int r = threadIdx.x & (kRows - 1), part = threadIdx.x / kRows;
   auto place_of = [&](int i) { return static_cast<size_t>(2 * (j.first + i) + (i == 0 ? 1 : 0)) * 2 + group_of; };
-  if (r < rows) {
+  // Row r, every `parts`th four columns from `part` on, every `shares`th piece from `share` on (by the lanes of a warp).
+  auto join = [&](auto fours, auto deep, int r, int part, int parts, int share, int shares) {
+    constexpr int kFours = decltype(fours)::value, kDeep = decltype(deep)::value;    // fours of a thread; pieces under way
+    const bool real = r < rows;
     float m = -INFINITY, l = 0.f;
 #pragma unroll 8
-    for (int i = 0; i < n; ++i) m = fmaxf(m, p.ml[(place_of(i) * kRows + r) * 2]);
+    for (int i = share; i < n; i += shares) m = fmaxf(m, real ? p.ml[(place_of(i) * kRows + r) * 2] : -INFINITY);
+    for (int off = 16; off >= 32 / shares && off > 0 && shares > 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
     float4 o[kFours] = {};
-#pragma unroll 2
-    for (int i = 0; i < n; ++i) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.ml + (place_of(i) * kRows + r) * 2);
-      const float* acc = p.acc + place_of(i) * (kRows * D) + r * 4;
-      float4 v[kFours];
+    for (int i0 = share; i0 < n; i0 += kDeep * shares) {
+      float2 ml[kDeep];
+      float4 v[kDeep][kFours];
 #pragma unroll
-      for (int k = 0; k < kFours; ++k) v[k] = *reinterpret_cast<const float4*>(acc + (part + k * (kJoinThreads / kRows)) * (kRows * 4));
-      const float f = ml.x > -INFINITY ? exp2f(ml.x - m) : 0.f;
-      l += ml.y * (ml.x > -INFINITY ? f : 1.f);                // (a piece whose keys all scored -inf has a sum of 0, or of NaN, which stays)
-      if (f != 0.f)
+      for (int e = 0; e < kDeep; ++e) {
+        const int i = i0 + e * shares;
+        ml[e] = make_float2(-INFINITY, 0.f);
+        if (real && i < n) {
+          ml[e] = *reinterpret_cast<const float2*>(p.ml + (place_of(i) * kRows + r) * 2);
+          const float* acc = p.acc + place_of(i) * (kRows * D) + r * 4;
 #pragma unroll
-        for (int k = 0; k < kFours; ++k) {
-          o[k].x = fmaf(v[k].x, f, o[k].x);
-          o[k].y = fmaf(v[k].y, f, o[k].y);
-          o[k].z = fmaf(v[k].z, f, o[k].z);
-          o[k].w = fmaf(v[k].w, f, o[k].w);
+          for (int k = 0; k < kFours; ++k) v[e][k] = *reinterpret_cast<const float4*>(acc + (part + k * parts) * (kRows * 4));
         }
+      }
+#pragma unroll
+      for (int e = 0; e < kDeep; ++e) {
+        const float f = ml[e].x > -INFINITY ? exp2f(ml[e].x - m) : 0.f;
+        l += ml[e].y * (ml[e].x > -INFINITY ? f : 1.f);        // (a piece whose keys all scored -inf has a sum of 0, or of NaN, which stays)
+        if (f != 0.f)
+#pragma unroll
+          for (int k = 0; k < kFours; ++k) {
+            o[k].x = fmaf(v[e][k].x, f, o[k].x);
+            o[k].y = fmaf(v[e][k].y, f, o[k].y);
+            o[k].z = fmaf(v[e][k].z, f, o[k].z);
+            o[k].w = fmaf(v[e][k].w, f, o[k].w);
+          }
+      }
     }
+    for (int off = 16; off >= 32 / shares && off > 0 && shares > 1; off >>= 1) {
+      l += __shfl_xor_sync(0xffffffffu, l, off);
+#pragma unroll
+      for (int k = 0; k < kFours; ++k) {
+        o[k].x += __shfl_xor_sync(0xffffffffu, o[k].x, off);
+        o[k].y += __shfl_xor_sync(0xffffffffu, o[k].y, off);
+        o[k].z += __shfl_xor_sync(0xffffffffu, o[k].z, off);
+        o[k].w += __shfl_xor_sync(0xffffffffu, o[k].w, off);
+      }
+    }
+    if (!real || share != 0) return;
     const float scale = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
     for (int k = 0; k < kFours; ++k) {
       if (scale != scale) o[k] = make_float4(scale, scale, scale, scale);
-      *reinterpret_cast<uint2*>(s_out + r * kLine + (part + k * (kJoinThreads / kRows)) * 8) =
+      *reinterpret_cast<uint2*>(s_out + r * kLine + (part + k * parts) * 8) =
           make_uint2(pack_pair<T>(o[k].x * scale, o[k].y * scale), pack_pair<T>(o[k].z * scale, o[k].w * scale));
     }
+  };
+  constexpr int kWarps = kJoinThreads / 32, kParts = kJoinThreads / kRows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (rows <= 32) {
+    const int wide = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32;           // lanes that have rows of their own
+    join(std::integral_constant<int, D / 4 / kWarps>{}, std::integral_constant<int, 4>{}, lane & (wide - 1), warp, kWarps, lane / wide, 32 / wide);
+  } else {
+    join(std::integral_constant<int, D / 4 / kParts>{}, std::integral_constant<int, 2>{}, threadIdx.x & (kRows - 1), threadIdx.x / kRows, kParts, 0, 1);
   }
   __syncthreads();
   constexpr int kLanes = D / 4;                                // of a row, 8 bytes each
@@ -929,7 +967,7 @@ int launch_fast(const cacheir_b200_tree_args& a, cudaStream_t stream) {
   static std::atomic<unsigned long long> done[2]{{0}, {0}};
   cudaError_t e = allow_shared_memory(done[run_on], reinterpret_cast<const void*>(kern), Smem<D>::kBytes);
   if (e == cudaSuccess) e = launch_chained(kern, dim3(grid), dim3(kThreads), Smem<D>::kBytes, stream, tk, tv, tq, p);
-  if (e == cudaSuccess && !p.whole) e = launch_chained(tree_pieces_kernel<T, D>, dim3(grid, 2), dim3(kJoinThreads), 0, stream, p);
+  if (e == cudaSuccess && !p.whole) e = launch_chained(tree_pieces_kernel<T, D>, dim3(grid, a.rows > p.half_rows ? 2 : 1), dim3(kJoinThreads), 0, stream, p);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }
 
