@@ -317,6 +317,25 @@ def test_long_context_in_many_pieces(lists):
     assert bool(torch.isfinite(got).all())
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads, nodes", [(1, 1), (3, 1), (1, 5), (4, 2), (3, 4), (16, 1), (5, 5), (32, 1), (11, 3), (32, 3)])
+def test_few_rows_in_many_pieces(heads, nodes, dim):
+    """Pieces are joined by lanes that share them out; one of them holds nothing but keys without weight, another a value that is no number, for the last row alone."""
+    case = Case(heads=heads, kv_heads=1, dim=dim, ctx=(30000, 9000), nodes=(nodes, nodes), lists=None, dtype=BF16, seed=heads)
+    case.q[:] = case.q.abs()
+    for t in range(5000, 6000):
+        page, offset = case.place(0, t)
+        case.keys[page, :, offset] = -math.inf
+    page, offset = case.place(1, 9000 + nodes - 1)
+    case.values[page, :, offset] = math.nan
+    want, bound = case.want()
+    got = case.call()
+    last = slice(2 * nodes - 1, 2 * nodes)
+    assert bool(torch.isnan(got[last]).all())
+    _close(got[: 2 * nodes - 1], want[: 2 * nodes - 1], bound[: 2 * nodes - 1])
+    assert torch.equal(got[: 2 * nodes - 1], case.call()[: 2 * nodes - 1])
+
+
 def test_a_long_chain_of_rows():
     """A prompt's rows over its own cache: no mask, more rows than words have bits."""
     Case(heads=4, kv_heads=2, dim=64, ctx=(100,), nodes=(1100,), lists=None).check()
