@@ -1,7 +1,7 @@
 // Drafted tokens as rows: their positions and the rows that they see, the accepted path, and its keys and values moved together.
 //
 // All three are bound by latency: a few thousand numbers, and of the moved keys and values little more than what a launch takes. 128 sequences of 33 to 64 rows, 32 layers of
-// 8 heads of 128 in fp16: 4.2, 2.7 and 15.9 us one by one, 27 us together (the 63 MB that move 9.7 us); 4 sequences of 6 to 8 rows, 4 layers: 5.9 us together.
+// 8 heads of 128 in fp16: 2.2, 2.7 and 15.0 us one by one, 22.6 us together (the 63 MB that move 9.7 us); 4 sequences of 6 to 8 rows, 4 layers: 5.6 us together.
 #include "cacheir_b200_drafts.h"
 #include "common.cuh"
 
@@ -14,14 +14,14 @@ __device__ __forceinline__ int2 rows_of(const int32_t* cu_rows, int rows, int b)
   return make_int2(lo, max(min(max(cu_rows[b + 1], 0), rows) - lo, 0));
 }
 
-// ---- map: a block a sequence, a thread a row, which walks up ----
+// ---- map: a block a sequence, a thread a row, which walks up among the rows of its round and goes on from what the rounds before have written ----
 constexpr int kMapThreads = 64;
-constexpr int kMapStaged = 1024;              // rows of a sequence whose parents lie in shared memory
+static_assert(kMapThreads == 64, "a round's rows are the bits of a 64-bit word");
 
 __global__ void __launch_bounds__(kMapThreads)
 map_drafts_kernel(const cacheir_b200_draft_map_args a) {
   chain_enter();
-  __shared__ int s_parent[kMapStaged];
+  __shared__ int s_parent[kMapThreads];
   const int b = blockIdx.x;
   if (b == a.sequences) {                     // rows behind the last sequence
     const int2 last = rows_of(a.cu_rows, a.rows, a.sequences - 1);
@@ -35,27 +35,30 @@ map_drafts_kernel(const cacheir_b200_draft_map_args a) {
   const int n = mine.y, first = a.seq_lens[b] - n;
   if (n > 32 * a.words && threadIdx.x == 0) atomicMax(a.status, n);
   const int32_t* parents = a.parents + mine.x;
-  for (int i = threadIdx.x; i < min(n, kMapStaged); i += kMapThreads) s_parent[i] = parents[i];
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kMapThreads) {
-    int32_t* line = a.visible + static_cast<size_t>(mine.x + i) * a.words;
-    // numbers fall on the way up, so that a word is written once, when the walk has left it
-    int w = a.words - 1, depth = -1;
-    uint32_t bits = 0;
-    for (int at = i; at >= 0;) {
+  const int tid = threadIdx.x;
+  int next = tid < n ? parents[tid] : -1;
+  for (int base = 0; base < n; base += kMapThreads) {
+    const int i = base + tid;
+    __syncthreads();                          // (what the round before wrote is there, and its parents are not looked at any more)
+    s_parent[tid] = next;
+    next = i + kMapThreads < n ? parents[i + kMapThreads] : -1;
+    __syncthreads();
+    if (i >= n) continue;
+    int at = i, depth = -1;
+    uint64_t bits = 0;
+    while (at >= base) {
       ++depth;
-      for (; w > at >> 5; --w) {
-        line[w] = static_cast<int32_t>(bits);
-        bits = 0;
-      }
-      if (at >> 5 == w) bits |= 1u << (at & 31);        // (rows behind the words' bits have none)
-      const int up = at < kMapStaged ? s_parent[at] : parents[at];
-      at = up < at ? up : -1;
+      bits |= 1ull << (at - base);
+      const int up = s_parent[at - base];
+      at = up < at ? max(up, -1) : -1;
     }
-    for (; w >= 0; --w) {
-      line[w] = static_cast<int32_t>(bits);
-      bits = 0;
-    }
+    // (numbers fall on the way up: what is left of it lies in earlier rounds)
+    if (at >= 0) depth += a.positions[mine.x + at] - first + 1;
+    const int32_t* above = a.visible + static_cast<size_t>(mine.x + max(at, 0)) * a.words;
+    int32_t* line = a.visible + static_cast<size_t>(mine.x + i) * a.words;
+    const int here = base >> 5;               // word of the round's first row
+    for (int w = 0; w < a.words; ++w)         // (rows behind the words' bits have none)
+      line[w] = w < here ? (at >= 0 ? above[w] : 0) : w == here ? static_cast<int32_t>(bits) : w == here + 1 ? static_cast<int32_t>(bits >> 32) : 0;
     a.positions[mine.x + i] = first + depth;
   }
 }
@@ -104,7 +107,7 @@ accept_drafts_kernel(const cacheir_b200_accept_args a) {
         at = i * 32 + __ffs(hit) - 1;
       }
     }
-    for (int r0 = kHeld * 32; !found && r0 < n; r0 += 32) {
+    for (int r0 = max(kHeld * 32, at & ~31); !found && r0 < n; r0 += 32) {          // (a row follows an earlier one: a path takes one look at every row)
       const int r = r0 + lane;
       const uint32_t hit = __ballot_sync(0xffffffffu, r > at && r < n && parents[min(r, n - 1)] == at && ids[min(r, n - 1)] == next);
       if (hit) {
@@ -129,8 +132,8 @@ accept_drafts_kernel(const cacheir_b200_accept_args a) {
 // ---- keep: a block a sequence and some pools, a thread a column, which it moves in the order of the path ----
 constexpr int kKeepThreads = 128;
 constexpr int kKeepPools = 128;               // of a launch
-constexpr int kKeepShare = 8;                 // pools of a block, which a thread has under way together ..
-constexpr int kKeepDeep = 2;                  // .. with so many rows of each
+constexpr int kKeepShare = 4;                 // pools of a block, which a thread has under way together (16 took 18.3 us, 8 15.9) ..
+constexpr int kKeepDeep = 3;                  // .. with so many rows of each
 constexpr int kKeepMoves = 64;                // moves that a block looks up together
 static_assert(kKeepMoves <= kKeepThreads, "a thread a move");
 

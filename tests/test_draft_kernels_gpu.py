@@ -736,6 +736,40 @@ def test_a_tree_of_more_rows_than_bits_says_so():
     assert tree.positions.tolist() == list(range(40)) + list(range(50)) and tree.visible[39].tolist() == [-1]
 
 
+@pytest.mark.parametrize("shape", ["chain", "near", "far"])
+def test_a_path_of_many_rows(shape):
+    """Rows far behind the words' bits: positions and paths all the same, in a time that grows as the rows do."""
+    from cacheir_b200 import draft_ops, serving_ops
+    rng, n, words = random.Random(3), 30000, 3
+    parents = [i - 1 if shape == "chain" else rng.randrange(max(0, i - 90) if shape == "near" else 0, i) if i else -1 for i in range(n)]
+    parents[70] = 70                                               # (no earlier row)
+    depths, seen = [], []
+    for i, up in enumerate(parents):
+        mine = 1 << i if i < 32 * words else 0
+        depths.append(depths[up] + 1 if 0 <= up < i else 0)
+        seen.append(mine | (seen[up] if 0 <= up < i else 0))
+    tokens, tree = serving_ops.token_map(n, 1, DEV), draft_ops.draft_tree(n, words, DEV)
+    tokens.cu_rows.copy_(_i32([0, n]))
+    seq_lens = _i32([n + 5])
+    draft_ops.map_drafts(_i32(parents), seq_lens, tokens, tree)
+    assert tree.positions.tolist() == [5 + d for d in depths] and int(tree.status) == n
+    want = torch.tensor([[(bits >> 32 * w) & 0xffffffff for w in range(words)] for bits in seen])
+    assert torch.equal(tree.visible.long().cpu() & 0xffffffff, want)
+
+    parents[70] = 69
+    follows = {}
+    for i, up in enumerate(parents):
+        follows.setdefault(up, []).append(i)
+    ids, chosen, path = list(range(n)), [-5] * n, [0]              # the path that always takes the last row
+    while path[-1] in follows:
+        path.append(follows[path[-1]][-1])
+        chosen[path[-2]] = path[-1]
+    accepted = draft_ops.accepted_drafts(1, n, DEV)
+    draft_ops.accept_drafts(torch.tensor(chosen, device=DEV), torch.tensor(ids, device=DEV), _i32(parents), seq_lens, tokens, accepted)
+    assert int(accepted.counts) == len(path) and accepted.rows[0, : len(path)].tolist() == path
+    assert bool((accepted.rows[0, len(path):] == -1).all()) and int(accepted.next_ids) == -5 and int(accepted.keep_lens) == 5 + len(path)
+
+
 @pytest.mark.parametrize("dtype, dim", [(F16, 128), (BF16, 64), (F32, 128), (F16, 33), (F32, 5), (BF16, 7)])
 @pytest.mark.parametrize("layers", [1, 70])
 def test_accepted_keys_and_values_lie_together(dtype, dim, layers):
