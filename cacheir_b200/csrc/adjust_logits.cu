@@ -37,14 +37,6 @@ struct LogitsParams {
 };
 
 __device__ __forceinline__ bool aligned_to_16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-// The tokens of a word of logits, each as it is where its bit is set, else -inf.
-template <typename T>
-__device__ __forceinline__ uint32_t allowed_word(uint32_t raw, uint32_t bits) {
-  if (sizeof(T) == 4) return bits & 1 ? raw : 0xff800000u;
-  const uint32_t keep = (bits & 1 ? 0x0000ffffu : 0u) | (bits & 2 ? 0xffff0000u : 0u);
-  return (raw & keep) | ((std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u) & ~keep);
-}
-
 // Shared memory: marks [slice / 32], then, where tokens can be marked, counts [slice], (with a bias) entries of it [slice], (with drafts) the drafted
 // tokens and what the rows see of them, and the list of marked tokens [slice].
 template <typename T, typename O, int VEC>
@@ -53,7 +45,7 @@ adjust_logits_kernel(const LogitsParams p) {
   constexpr int NV = kSlice / VEC / kThreads;          // vectors of a thread in a row
   constexpr bool kWide = VEC > 1;
   chain_enter();
-  extern __shared__ __align__(16) uint32_t smem[];
+  extern __shared__ uint32_t smem[];
   __shared__ int s_marked, s_drafted, s_seq[kRun];
   const cacheir_b200_logits_args& a = p.a;
   const int lo = blockIdx.x * p.slice, size = min(p.slice, a.vocab - lo), words = p.slice / 32;
@@ -123,8 +115,9 @@ adjust_logits_kernel(const LogitsParams p) {
       }
       const int bias_id = static_cast<int>(threadIdx.x) < a.biases ? a.bias_ids[of_bias + threadIdx.x] : -1;
       __syncthreads();
-      // (marks, counts and entries lie one behind the other, and are a multiple of 16 bytes each)
-      for (int i = threadIdx.x; i < (words + (biased ? 2 : 1) * p.slice) / 4; i += kThreads) reinterpret_cast<uint4*>(marks)[i] = make_uint4(0u, 0u, 0u, 0u);
+      for (int i = threadIdx.x; i < words; i += kThreads) marks[i] = 0;
+      for (int i = threadIdx.x; i < p.slice; i += kThreads) counts[i] = 0;
+      if (biased) for (int i = threadIdx.x; i < p.slice; i += kThreads) entry[i] = 0;
       if (threadIdx.x == 0) s_marked = s_drafted = 0;
       __syncthreads();
       auto mark = [&](uint32_t t) {
@@ -190,24 +183,16 @@ adjust_logits_kernel(const LogitsParams p) {
             if (t0 < 0 || t0 + VEC > size) continue;
             const uint32_t yes = a.allowed ? __funnelshift_r(may[k].x, may[k].y, t0 & 31) | ~((1u << VEC) - 1) : 0xffffffffu;
             if (same && yes == 0xffffffffu) continue;
-            if constexpr (sizeof(O) == sizeof(T)) {            // (bits are copied, or those of -inf are put in their place)
-              if (a.allowed) {
-                raw[k].x = allowed_word<T>(raw[k].x, yes);
-                raw[k].y = allowed_word<T>(raw[k].y, yes >> (4 / sizeof(T)));
-                raw[k].z = allowed_word<T>(raw[k].z, yes >> (8 / sizeof(T)));
-                raw[k].w = allowed_word<T>(raw[k].w, yes >> (12 / sizeof(T)));
-              }
-              *reinterpret_cast<uint4*>(out + t0) = raw[k];
-              continue;
-            }
             float x[VEC];
             VecIO<T, VEC>::ld(reinterpret_cast<const T*>(&raw[k]), x);
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
               if (!(yes >> i & 1)) x[i] = -INFINITY;
-            if (aligned_to_16(out + t0)) {
+            if constexpr (sizeof(O) == sizeof(T)) {
+              VecIO<O, VEC>::st(out + t0, x);
+            } else if (aligned_to_16(out + t0)) {
 #pragma unroll
-              for (int i = 0; i < VEC; i += 4) *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + t0 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+              for (int i = 0; i < VEC; i += 4) *reinterpret_cast<float4*>(out + t0 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
             } else {
 #pragma unroll
               for (int i = 0; i < VEC; ++i) Elem<O>::st(out + t0 + i, x[i]);
