@@ -331,7 +331,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
   int item = 0;                                                // of the block, counted from 1
   auto next_item = [&] {
     const int place = item % kItems;
-    ok = ok && warp_wait(smem_u32(&bar_item[place]), (item / kItems) & 1, (15 << 8) | 14);
+    ok = ok && warp_wait(smem_u32(&bar_item[place]), (item / kItems) & 1, (17 << 8) | 14);
     if (!ok) return false;
     it = s_item[place];
     ++item;
@@ -346,7 +346,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
     uint32_t phase = 0;
     while (next_item()) {
       for (int t = it.tile; t < it.tile + it.tiles && ok; ++t) {
-        ok = warp_wait(smem_u32(&value_full[turn]), phase, (15 << 8) | 12);
+        ok = warp_wait(smem_u32(&value_full[turn]), phase, (17 << 8) | 12);
         if (!ok) break;
         // (behind the 16 keys in which the last one lies there are zeros already)
         const int base = t * kKeys, from = max(min(it.s.front, it.keys) - base, 0), until = min((it.keys - base + kChunk - 1) / kChunk * kChunk, kKeys);
@@ -404,7 +404,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
     auto copy_tiles = [&](int line) {
       for (int t = it.tile; t < it.tile + it.tiles && ok; ++t) {
         const int next = t + 1 < it.tile + it.tiles ? line_of(t + 1) : 0;
-        ok = warp_wait(smem_u32(&empty[slot]), phase, (15 << 8) | 1);
+        ok = warp_wait(smem_u32(&empty[slot]), phase, (17 << 8) | 1);
         if (!ok) break;
         if (lane == 0) mbar_expect_tx(smem_u32(&full[turn]), L::kSlotBytes);
         __syncwarp();
@@ -443,7 +443,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
         const bool two = it.rows > half_rows;                  // the item's queries: rows, heads, 64 columns at a time
         for (int w = 0; w < (two ? 2 : 1) && ok; ++w) {
           const int place = two ? w : q_place;
-          ok = warp_wait(smem_u32(&bar_free[place]), q_phase >> place & 1, (15 << 8) | 7);
+          ok = warp_wait(smem_u32(&bar_free[place]), q_phase >> place & 1, (17 << 8) | 7);
           if (!ok) break;
           q_phase ^= 1u << place;
           if (lane == 0) {
@@ -460,10 +460,10 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
     }
     // nothing may still be on its way when the block ends, also after a wait that gave up
     for (uint32_t i = sent > kSlots ? sent - kSlots : 0; i < sent; ++i)
-      mbar_wait(smem_u32(&full[i % kSlots]), (i / kSlots) & 1, &g_tree_status, (15 << 8) | 2);
+      mbar_wait(smem_u32(&full[i % kSlots]), (i / kSlots) & 1, &g_tree_status, (17 << 8) | 2);
     // (queries are waited for by the products; after a wait that gave up: both phases of both places)
     if (!keys && !ok)
-      for (int w = 0; w < 4; ++w) mbar_wait(smem_u32(&bar_q[w >> 1]), w & 1, &g_tree_status, (15 << 8) | 2);
+      for (int w = 0; w < 4; ++w) mbar_wait(smem_u32(&bar_q[w >> 1]), w & 1, &g_tree_status, (17 << 8) | 2);
   } else if (warp == 8) {
     // ---------------- MMA issue ----------------
     constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
@@ -476,7 +476,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
     const bool leader = elect_one();
     auto load_item = [&](int& n, Item& into) {
       const int place = n % kItems;
-      ok = ok && warp_wait(smem_u32(&bar_item[place]), (n / kItems) & 1, (15 << 8) | 14);
+      ok = ok && warp_wait(smem_u32(&bar_item[place]), (n / kItems) & 1, (17 << 8) | 14);
       if (!ok) return false;
       into = s_item[place];
       ++n;
@@ -501,10 +501,10 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
       }
       if (s_step < (s_two ? 2 : 1)) {                          // the item's queries are new
         const int place = s_two ? s_step : s_place;
-        ok = warp_wait(smem_u32(&bar_q[place]), q_phase >> place & 1, (15 << 8) | 3);
+        ok = warp_wait(smem_u32(&bar_q[place]), q_phase >> place & 1, (17 << 8) | 3);
         q_phase ^= 1u << place;
       }
-      if (!(s_two && (s_step & 1))) ok = ok && warp_wait(smem_u32(&key_full[k_turn]), k_phase, (15 << 8) | 4);
+      if (!(s_two && (s_step & 1))) ok = ok && warp_wait(smem_u32(&key_full[k_turn]), k_phase, (17 << 8) | 4);
       return ok;
     };
     auto score = [&] {                                         // (one lane)
@@ -555,8 +555,8 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
       for (int j = 0; j < steps && ok; ++j) {
         const int w = group_of;
         const bool frees = !two || (j & 1);
-        if (!(two && (j & 1))) ok = warp_wait(smem_u32(&bar_clean[v_turn]), v_phase, (15 << 8) | 5);
-        ok = ok && warp_wait(smem_u32(&bar_p[2 * w]), p_phase >> w & 1, (15 << 8) | 6);
+        if (!(two && (j & 1))) ok = warp_wait(smem_u32(&bar_clean[v_turn]), v_phase, (17 << 8) | 5);
+        ok = ok && warp_wait(smem_u32(&bar_p[2 * w]), p_phase >> w & 1, (17 << 8) | 6);
         if (!ok) break;
         tc_fence_after();
         const uint64_t v_at = dv + (v_slot * L::kSlotBytes >> 4);
@@ -568,9 +568,9 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
         __syncwarp();
         // (mostly the item goes on, and its next keys are all there is to wait for: this warp's chain of instructions is what the tensor cores wait for)
         bool more;
-        if (s_step >= 2 && s_step < s_steps) more = ok = (s_two && (s_step & 1)) || warp_wait(smem_u32(&key_full[k_turn]), k_phase, (15 << 8) | 4);
+        if (s_step >= 2 && s_step < s_steps) more = ok = (s_two && (s_step & 1)) || warp_wait(smem_u32(&key_full[k_turn]), k_phase, (17 << 8) | 4);
         else more = RUN_ON && prepare();
-        ok = ok && warp_wait(smem_u32(&bar_p[2 * w + 1]), p_phase >> w & 1, (15 << 8) | 6);
+        ok = ok && warp_wait(smem_u32(&bar_p[2 * w + 1]), p_phase >> w & 1, (17 << 8) | 6);
         if (!ok) break;
         tc_fence_after();
         if (leader) {
@@ -603,7 +603,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
     // (an item's numbers stay in shared memory: in registers they were spilled)
     for (;; ) {
       const int ring = item % kItems;
-      ok = ok && warp_wait(smem_u32(&bar_item[ring]), (item / kItems) & 1, (15 << 8) | 14);
+      ok = ok && warp_wait(smem_u32(&bar_item[ring]), (item / kItems) & 1, (17 << 8) | 14);
       if (!ok) break;
       ++item;
       const Item& now = s_item[ring];
@@ -639,13 +639,13 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
             low = high;
           }
         }
-        ok = warp_wait(smem_u32(&bar_s[w]), s_phase, (15 << 8) | 8);
+        ok = warp_wait(smem_u32(&bar_s[w]), s_phase, (17 << 8) | 8);
         if (!ok) break;
         s_phase ^= 1;
         auto returned = [&] {                                  // the output may be written over
           if (!lent) return;
           lent = false;
-          ok = warp_wait(smem_u32(&bar_taken[w]), taken_phase, (15 << 8) | 13) && ok;
+          ok = warp_wait(smem_u32(&bar_taken[w]), taken_phase, (17 << 8) | 13) && ok;
           taken_phase ^= 1;
         };
         if (idle) {
@@ -748,7 +748,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
       if (!ok) break;
       // ---- the item's end ----
       o_phase ^= (steps - 1) & 1;                              // (the phase of this group's last output; those before it have not been waited for)
-      ok = warp_wait(smem_u32(&bar_o[w]), o_phase, (15 << 8) | 11);
+      ok = warp_wait(smem_u32(&bar_o[w]), o_phase, (17 << 8) | 11);
       if (!ok) break;
       o_phase ^= 1;
       tc_fence_after();
@@ -765,7 +765,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
       }
       const bool joins = !two && now.tiles > 1;
       if (joins) {
-        ok = warp_wait(smem_u32(&bar_given[w ^ 1]), given_phase, (15 << 8) | 13);
+        ok = warp_wait(smem_u32(&bar_given[w ^ 1]), given_phase, (17 << 8) | 13);
         if (!ok) break;
         given_phase ^= 1;
         tc_fence_after();
