@@ -156,6 +156,12 @@ def test_trees_of_all_heads_and_types(dtype, heads, kv_heads, dim):
     Case(heads=heads, kv_heads=kv_heads, dim=dim, dtype=dtype, ctx=(0, 37, 300), nodes=(7, 1, 33), lists="tree", seed=dim).check()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("dim", [1, 63, 65, 127, 129, 192, 200, 256, 257, 320, 511])
+def test_heads_of_any_size(dtype, dim):
+    Case(heads=6, kv_heads=2, dim=dim, dtype=dtype, ctx=(70, 0, 513), nodes=(9, 3, 40), seed=dim).check()
+
+
 @pytest.mark.parametrize("page", [16, 32, 128, 8, 5, 48])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_page_sizes(page, dtype):
