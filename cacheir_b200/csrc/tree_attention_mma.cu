@@ -198,12 +198,14 @@ struct Smem {
   static constexpr int kSlots = D == 128 ? 5 : 10;
   static constexpr int kQBytes = kRows * D * 2;
   // Items in shared memory. The keys' warp, which goes through them, is no more tiles ahead of the outputs than there are slots (where their number is even, of the
-  // scores, which are two steps ahead of the outputs), and a group of warps may be an item behind these.
+  // scores, which are two steps ahead of the outputs), but a group of warps may be any number of items behind these: those of one tile that follow may all be the other group's. So
+  // both groups say when they are done with a place; whoever else reads it has done so by then, as no group ends an item before its outputs are there.
   static constexpr int kItems = D == 128 ? 8 : 16;
   static constexpr int kTiles = 2 * kQBytes + kSlots * kSlotBytes;
-  // then: barriers of keys, of values, empty, clean [slots], q[2], place of q[2], s[2], p[2][2], o[2], given[2], taken[2], items; tensor memory address; items; starts of runs, and later
+  // then: barriers of keys, of values, empty, clean [slots], q[2], place of q[2], s[2], p[2][2], o[2], given[2], taken[2], items, places of items;
+  // tensor memory address; items; starts of runs, and later
   // maxima and denominators that one group of warps hands to the other
-  static constexpr int kBarriers = 4 * kSlots + 16 + kItems;
+  static constexpr int kBarriers = 4 * kSlots + 16 + 2 * kItems;
   static constexpr int kBytes = 1024 + kTiles + kBarriers * 8 + 16 + kItems * static_cast<int>(sizeof(Item)) + kRows * 8;
 };
 
@@ -260,7 +262,8 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
   uint64_t* bar_given = bar_o + 2;                             // a group's part of an item is done
   uint64_t* bar_taken = bar_given + 2;                         // .. and has been added to the other one's
   uint64_t* bar_item = bar_taken + 2;                            // the item is known
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_item + kItems);
+  uint64_t* bar_done = bar_item + kItems;                      // .. and both groups of warps are done with it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_done + kItems);
   Item* s_item = reinterpret_cast<Item*>(tmem_slot + 4);
   int* s_start = reinterpret_cast<int*>(s_item + kItems);
   float2* s_ml = reinterpret_cast<float2*>(s_start);           // (when the first item ends the keys' warp has long found its share)
@@ -290,7 +293,10 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
       mbar_init(smem_u32(&bar_given[w]), 4);
       mbar_init(smem_u32(&bar_taken[w]), 4);
     }
-    for (int i = 0; i < kItems; ++i) mbar_init(smem_u32(&bar_item[i]), 1);
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(smem_u32(&bar_item[i]), 1);
+      mbar_init(smem_u32(&bar_done[i]), 2 * kRows / 32);
+    }
     mbar_fence_init();
   }
   if (threadIdx.x >= 256 && threadIdx.x < 256 + kItems) s_spoilt[threadIdx.x - 256] = 0;
@@ -426,6 +432,8 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
       bool more = true;
       while (ok && more) {
         more = walk.next();
+        ok = warp_wait(smem_u32(&bar_done[item % kItems]), ((item / kItems) & 1) ^ 1, (17 << 8) | 15);
+        if (!ok) break;
         it = Item{walk.s, walk.b, walk.row0, walk.rows, walk.kvh, walk.tile, more ? walk.tiles : 0, walk.keys, (walk.begins ? 1 : 0) | (walk.ends ? 2 : 0)};
         if (lane == 0) {
           s_item[item % kItems] = it;
@@ -608,12 +616,19 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
       ++item;
       const Item& now = s_item[ring];
       if (now.tiles <= 0) break;
+      auto done = [&] {                                        // (`now` is not looked at any more)
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_done[ring]));
+      };
       const bool two = now.rows > half_rows;
       // which half of the rows is this group's, or its first tile (the group that has the item's first tile also stores what comes of it)
       const int place_of = w ^ before;
       if (!two) {
         if (RUN_ON) before ^= now.tiles & 1;
-        if (place_of >= now.tiles) continue;                    // (an item of one tile, which is the other group's)
+        if (place_of >= now.tiles) {                            // (an item of one tile, which is the other group's)
+          done();
+          continue;
+        }
       }
       const int in_item = (two ? place_of * half_rows : 0) + token;      // this thread's token of the item
       const bool real = r < half_rows * group && in_item < now.rows;
@@ -761,6 +776,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_given[w]));
+        done();
         continue;
       }
       const bool joins = !two && now.tiles > 1;
@@ -831,6 +847,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ 
       tc_fence_before();
       __syncwarp();
       if (joins && lane == 0) mbar_arrive(smem_u32(&bar_taken[w ^ 1]));
+      done();
     }
   }
   __syncwarp();

@@ -317,6 +317,27 @@ def test_blocks_with_many_short_items(dim, most):
     assert _lib.load_group("drafts").cacheir_b200_drafts_device_status(0) == 0
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_group_of_warps_far_behind_the_other(dim):
+    """Chains whose later rows, which are one group's, go through many tokens for one that is no number, among hundreds of sequences of one tile, which are all the
+    other group's: more than there are places for items in shared memory."""
+    from cacheir_b200 import _lib
+    ctx, nodes = [], []
+    for part in range(3):
+        ctx += [900] + [3 + part] * 150
+        nodes += [200 + part] + [1] * 150
+    case = Case(heads=32, kv_heads=8, dim=dim, ctx=ctx, nodes=nodes, lists=None, dtype=BF16, seed=dim)
+    for b in range(0, len(nodes), 151):
+        page, offset = case.place(b, ctx[b] + nodes[b] - 1)
+        case.values[page, :, offset, ::5] = math.inf
+    want, bound = case.want()
+    got = case.call()
+    plain = torch.isfinite(want)
+    assert bool((torch.isfinite(got.double()) == plain).all()) and not bool(plain.all())
+    _close(torch.where(plain, got.double(), 0.0), torch.where(plain, want, 0.0), bound)
+    assert _lib.load_group("drafts").cacheir_b200_drafts_device_status(0) == 0
+
+
 @pytest.mark.parametrize("lists", ["tree", None])
 def test_long_context_in_many_pieces(lists):
     got = Case(heads=4, kv_heads=1, ctx=(40000, 77), nodes=(6, 3), lists=lists, dtype=BF16, wide_q=2).check()
