@@ -253,6 +253,50 @@ def test_what_a_row_does_not_see_may_hold_anything(dtype, ctx, nodes, heads, lis
     assert bool(torch.isnan(want).any()) and bool(plain.any())
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads, dim, ctx, nodes", [(8, 128, 5, 300), (8, 64, 2000, 120), (64, 128, 900, 40), (3, 64, 0, 33), (16, 128, 3000, 70)])
+@pytest.mark.parametrize("lists", ["tree", None])
+def test_many_values_that_are_no_numbers(dtype, heads, dim, ctx, nodes, lists):
+    """Infinities of either sign and NaN in many rows' values, some of whose keys have scores of -inf and so no weight."""
+    kv_heads = 1 if heads == 3 else 2
+    case = Case(heads=heads, kv_heads=kv_heads, dim=dim, ctx=(ctx, 30), nodes=(nodes, 9), dtype=dtype, lists=lists, seed=heads)
+    case.q[:] = case.q.abs()
+    rng = random.Random(nodes)
+    for j in rng.sample(range(nodes), nodes // 3):
+        page, offset = case.place(0, ctx + j)
+        for kind in (math.inf, -math.inf, math.nan):
+            if rng.random() < 0.5:
+                case.values[page, rng.randrange(kv_heads), offset, rng.randrange(dim)] = kind
+        if rng.random() < 0.3:
+            case.keys[page, :, offset] = -math.inf
+    want, bound = case.want()
+    got = case.call()
+    assert bool(torch.isnan(want).any()) and bool((want == math.inf).any()) and bool((want == -math.inf).any())
+    _close(got, want, bound)
+
+
+def test_one_infinite_value_takes_little_time():
+    """Rows look for it together (one by one the call took a hundred times as long, and waits of very long chains would have run out)."""
+    case = Case(dim=128, ctx=(100,), nodes=(6000,), lists=None, dtype=BF16)
+
+    def shortest():
+        times = []
+        for _ in range(6):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            case.call()
+            end.record()
+            end.synchronize()
+            times.append(begin.elapsed_time(end))
+        return min(times)
+
+    plain = shortest()
+    page, offset = case.place(0, 6099)
+    case.values[page, :, offset, 5] = math.inf
+    assert shortest() < 20 * plain
+    assert bool((case.out[5999, :, 5] == math.inf).all()) and int(torch.isfinite(case.out).logical_not().sum()) == 8
+
+
 def test_scores_of_minus_infinity_and_nan():
     case = Case(ctx=(300, 300), nodes=(4, 4), dtype=BF16)
     case.q[:] = case.q.abs()
