@@ -275,6 +275,21 @@ int launch_adjust(const cacheir_b200_logits_args& a, cudaStream_t stream) {
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }
 
+// Whether a row of out lies over a row of logits (rows may lie between one another).
+bool rows_overlap(const cacheir_b200_logits_args& a) {
+  const uintptr_t in = reinterpret_cast<uintptr_t>(a.logits), out = reinterpret_cast<uintptr_t>(a.out);
+  const uint64_t in_row = static_cast<uint64_t>(a.vocab) * dtype_size(a.dtype), out_row = static_cast<uint64_t>(a.vocab) * dtype_size(a.out_dtype);
+  auto in_at = [&](int r) { return in + static_cast<uint64_t>(r) * static_cast<uint64_t>(a.row_stride) * dtype_size(a.dtype); };
+  auto out_at = [&](int r) { return out + static_cast<uint64_t>(r) * static_cast<uint64_t>(a.out_stride) * dtype_size(a.out_dtype); };
+  if (in_at(a.rows - 1) + in_row <= out || out_at(a.rows - 1) + out_row <= in) return false;
+  for (int i = 0, j = 0; i < a.rows && j < a.rows;) {          // in the order of their addresses
+    const uint64_t x = in_at(i), y = out_at(j);
+    if (x < y + out_row && y < x + in_row) return true;
+    if (x < y) ++i; else ++j;
+  }
+  return false;
+}
+
 }  // namespace
 }  // namespace cb200
 
@@ -290,7 +305,8 @@ extern "C" int cacheir_b200_adjust_logits(const cacheir_b200_logits_args* args, 
   if ((a.rows > 1 && (a.row_stride < a.vocab || a.out_stride < a.vocab)) || a.biases < 0 || (a.history && (!a.history_lens || a.history_width <= 0)) ||
       (a.draft_ids && (!a.cu_rows || !a.visible || a.words <= 0)) || (a.biases > 0 && (!a.bias_ids || !a.bias_values)))
     return CACHEIR_B200_EINVAL;
-  if (a.logits == a.out && a.dtype != a.out_dtype) return CACHEIR_B200_EINVAL;
+  const bool same = a.logits == a.out;
+  if (same ? a.dtype != a.out_dtype || (a.rows > 1 && a.row_stride != a.out_stride) : rows_overlap(a)) return CACHEIR_B200_EINVAL;
   if (a.vocab > 1 << 28 || a.history_width >= 1 << 29 || (a.draft_ids && a.words > CACHEIR_B200_MAX_DRAFT_WORDS)) return CACHEIR_B200_ELIMIT;
   if (a.biases == 0) a.bias_ids = nullptr;
   if (a.dtype == CACHEIR_B200_F32) return launch_adjust<float, float>(a, as_stream(stream));

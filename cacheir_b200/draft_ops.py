@@ -296,7 +296,7 @@ def adjust_logits(logits: torch.Tensor, *, row_seq: torch.Tensor | None = None, 
     row_seq: int32 [R] (None: row r is of sequence r); rows of a sequence outside 0 .. S - 1 are left as they are in `out`. repetition (above 0),
     frequency, presence: float32 [S]. bias_ids int32, bias_values float32 [S, K]: of several entries with one token the last counts, ids outside
     the vocabulary (-1) are none. allowed: int32 [R, ceil(V / 32)], bit t % 32 of word t // 32. out: default in place (then only what changes is
-    written); of the logits' type or float32. Worked out in 32 bits, rounded once. Logits and out have dense rows (the row stride may be wider)."""
+    written), else rows that do not lie over those of the logits; of their type or float32. Worked out in 32 bits, rounded once. Logits and out have dense rows (the row stride may be wider)."""
     shape = logits.shape
     if len(shape) != 2:
         raise ValueError("logits must be [R, V]")
@@ -313,6 +313,8 @@ def adjust_logits(logits: torch.Tensor, *, row_seq: torch.Tensor | None = None, 
             raise ValueError("out must be [R, V] with dense rows that do not overlap")
         if out.dtype is not dtype and (out.dtype is not _F32 or out.data_ptr() == logits.data_ptr()):
             raise TypeError("out must have the logits' type, or be another tensor of float32")
+        if rows > 1 and out_stride != row_stride and out.data_ptr() == logits.data_ptr():
+            raise ValueError("logits that are changed in place keep their row stride")
     counts = []                                                       # what the arguments say about the number of sequences
     said = said_lens = prompt_lens = draft_ids = visible = cu_rows = None
     width = words = biases = 0

@@ -82,7 +82,8 @@ int cacheir_b200_tree_attention(const cacheir_b200_tree_args* args, void* stream
  *   repetition (> 0), frequency, presence float [sequences]; each NULL: without
  *   bias_ids int32 [sequences][biases], bias_values float: of several entries with one token the last counts
  *   allowed int32 [rows][ceil(vocab / 32)]: bit t % 32 of word t / 32, 1 where the token may come
- * Tokens outside the vocabulary are left out. out may be logits; it has the same type or is float32. Up to 524280 rows, vocabularies of up to 2^28,
+ * Tokens outside the vocabulary are left out. out has the same type or is float32. It may be logits, with the same type and row stride; other rows of it that lie over
+ * rows of logits are refused (CACHEIR_B200_EINVAL). Up to 524280 rows, vocabularies of up to 2^28,
  * histories of fewer than 2^29 tokens, words <= 32 (CACHEIR_B200_ELIMIT). */
 typedef struct {
   const void* logits;

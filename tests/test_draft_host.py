@@ -104,6 +104,28 @@ def test_c_entry_points_refuse_before_they_launch(lib):
         assert getattr(lib, "cacheir_b200_" + name)(None, None) == -1
 
 
+def test_logits_that_lie_over_one_another_are_refused(lib):
+    """Values that do not change are not written where out is the logits: another row stride, or rows that lie partly over one another, would leave the wrong ones. What
+    lies between the rows, or apart, goes on to the next check (here: words)."""
+    from cacheir_b200 import draft_ops
+    from cacheir_b200._lib import LogitsArgs
+
+    at = 1 << 20
+    call = lambda out, row_stride=20, out_stride=20, rows=3, dtype=1, out_dtype=1: lib.cacheir_b200_adjust_logits(ctypes.byref(LogitsArgs(
+        logits=at, out=out, draft_ids=at, cu_rows=at, visible=at, rows=rows, sequences=3, vocab=9, words=33, row_stride=row_stride, out_stride=out_stride, dtype=dtype,
+        out_dtype=out_dtype)), None)
+    over = [call(at, out_stride=24), call(at, row_stride=9), call(at + 16), call(at - 16), call(at + 40), call(at + 56), call(at - 40 * 2 - 2), call(at + 18, out_dtype=0),
+            call(at - 34, rows=1, out_dtype=0), call(at + 18, out_stride=24), call(at + 200, row_stride=100, out_stride=9)]
+    assert over == [-1] * len(over)
+    # (out_stride 22: bytes 18 to 36, 62 to 80 and 106 to 124, of logits 0 to 18, 40 to 58 and 80 to 98)
+    apart = [call(at), call(at, rows=1, out_stride=24), call(at + 18, rows=1, row_stride=0), call(at + 18, out_stride=22), call(at + 18), call(at + 22), call(at - 22), call(at + 2 * 40 + 18), call(at - 2 * 40 - 18), call(at - 36, rows=1, out_dtype=0),
+             call(at + 20, row_stride=40, out_stride=20, out_dtype=0), call(at + 1000, out_stride=9)]
+    assert apart == [-5] * len(apart)
+    room = torch.zeros(200)
+    with pytest.raises(ValueError, match="row stride"):
+        draft_ops.adjust_logits(room[:60].view(3, 20)[:, :9], out=room[:90].view(3, 30)[:, :9], allowed=_i32(3, 1))
+
+
 def _i32(*shape):
     return torch.zeros(shape, dtype=torch.int32)
 
