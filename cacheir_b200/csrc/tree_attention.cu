@@ -2,7 +2,7 @@
 // and the C entry point.
 //
 // A tile is 32 (row, head) pairs of one sequence that share a key/value head; its keys are cut into pieces, which leave their maximum, sum and
-// unnormalised output, and the pieces of a row are joined in order. Within a piece 64 keys at a time, 64 columns of them at a time in shared memory as 32-bit floats;
+// unnormalised output, and the pieces of a row are joined in order; with one piece the output is written as it ends. Within a piece 64 keys at a time, 64 columns of them at a time in shared memory as 32-bit floats;
 // a thread has 2 x 4 scores, and for every 64 columns 2 x 4 outputs in registers, reads four numbers at a time of either operand, and has the next 64 columns on their way
 // meanwhile. 32 trees of 12 to 16 tokens behind 256 to 4096, 32 query and 8 key/value heads, take 1980 us in fp32 with heads of 128, 2420 in bf16 with heads of
 // 96 and 4630 with heads of 256 (with tiles of eight rows and a number at a time 6652 and 5226 of the first two; the ordinary decode attention of as many single rows 2685, 3060 and 3350).
@@ -28,7 +28,7 @@ constexpr size_t general_smem(int dim) {
 struct TreeParts {
   float* ml;       // [pieces][rows][heads][2]
   float* acc;      // [pieces][rows][heads][dim]
-  int pieces;
+  int pieces;      // 1: there is no scratch
 };
 
 // Heads of up to kChunks * kColumns.
@@ -38,7 +38,7 @@ tree_general_kernel(const cacheir_b200_tree_args a, const TreeParts parts) {
   chain_enter();
   extern __shared__ __align__(16) float smem[];
   __shared__ long long s_line[2][kTileKeys];           // where a key of this tile, or of the next, begins in the pools; -1: it is not there
-  __shared__ float s_scale[kTileRows];
+  __shared__ float s_scale[kTileRows], s_sum[kTileRows];
   const int D = a.dim, group = a.heads / a.kv_heads, chunks = chunks_of(D), q_line = chunks * kColumns + 4;
   const int piece = blockIdx.x % parts.pieces, kvh = blockIdx.x / parts.pieces % a.kv_heads, place = blockIdx.x / parts.pieces / a.kv_heads;
   float* s_q = smem;                                   // [kTileRows][q_line]
@@ -185,6 +185,29 @@ tree_general_kernel(const cacheir_b200_tree_args a, const TreeParts parts) {
       }
     }
   }
+  if (parts.pieces == 1) {                                       // nobody else has keys of these rows
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (lane == 0) s_sum[4 * warp + e] = l_run[e];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (2 * ty + i >= rows) continue;
+      const int pair = first + 2 * ty + i;
+      const float l = s_sum[2 * ty + i];
+      T* to = static_cast<T*>(a.out) + static_cast<size_t>(s.row + pair / group) * a.out_stride + static_cast<size_t>(kvh * group + pair % group) * D;
+#pragma unroll
+      for (int chunk = 0; chunk < kChunks; ++chunk) {
+        if (chunk >= chunks) break;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int d = chunk * kColumns + 4 * tx + c;
+          if (d < D) Elem<T>::st(to + d, l > 0.f || l != l ? acc[chunk][i][c] / l : 0.f);
+        }
+      }
+    }
+    return;
+  }
   auto at_pair = [&](int r) {                                    // of the scratch
     const int pair = first + r;
     return (static_cast<size_t>(piece) * a.rows + s.row + pair / group) * a.heads + kvh * group + pair % group;
@@ -264,7 +287,7 @@ int launch_general(const cacheir_b200_tree_args& a, cudaStream_t stream) {
   const int chunks = chunks_of(a.dim);
   cudaError_t e = chunks == 1 ? launch_tiles<T, 1>(a, parts, blocks, stream) : chunks == 2 ? launch_tiles<T, 2>(a, parts, blocks, stream)
                   : chunks <= 4 ? launch_tiles<T, 4>(a, parts, blocks, stream) : launch_tiles<T, kGeneralDim / kColumns>(a, parts, blocks, stream);
-  if (e == cudaSuccess) e = launch_chained(tree_join_kernel<T>, dim3(static_cast<unsigned>(ends)), dim3(128), 0, stream, a, parts);
+  if (e == cudaSuccess && parts.pieces > 1) e = launch_chained(tree_join_kernel<T>, dim3(static_cast<unsigned>(ends)), dim3(128), 0, stream, a, parts);
   return e != cudaSuccess ? static_cast<int>(e) : launch_status();
 }
 
@@ -275,7 +298,8 @@ using namespace cb200;
 
 extern "C" size_t cacheir_b200_tree_attention_workspace_bytes(int rows, int heads, int dim) {
   if (rows <= 0 || heads <= 0 || dim <= 0) return 0;
-  const size_t general = static_cast<size_t>(tree_pieces(rows, heads, dim)) * rows * heads * (dim + 2) * 4, fast = tree_fast_bytes(dim);
+  const int pieces = tree_pieces(rows, heads, dim);
+  const size_t general = pieces > 1 ? static_cast<size_t>(pieces) * rows * heads * (dim + 2) * 4 : 0, fast = tree_fast_bytes(dim);
   return general > fast ? general : fast;
 }
 
@@ -290,7 +314,8 @@ extern "C" int cacheir_b200_tree_attention(const cacheir_b200_tree_args* args, v
   if (a.sequences > 65535 || a.rows > 1 << 24 || a.kv_heads > 65535 || static_cast<long long>(a.max_pages) * a.page_size > 1LL << 30 ||
       (a.visible && a.words > CACHEIR_B200_MAX_DRAFT_WORDS))
     return CACHEIR_B200_ELIMIT;
-  if (!a.workspace || a.workspace_bytes < cacheir_b200_tree_attention_workspace_bytes(a.rows, a.heads, a.dim)) return CACHEIR_B200_EWORKSPACE;
+  const size_t need = cacheir_b200_tree_attention_workspace_bytes(a.rows, a.heads, a.dim);
+  if ((need > 0 && !a.workspace) || a.workspace_bytes < need) return CACHEIR_B200_EWORKSPACE;
   if (!aligned_to(a.workspace, 16)) return CACHEIR_B200_EALIGN;
   if (!(a.softmax_scale > 0.f)) a.softmax_scale = 1.0f / sqrtf(static_cast<float>(a.dim));
   if (a.rows == 1) a.q_stride = a.out_stride = static_cast<long long>(a.heads) * a.dim;

@@ -31,7 +31,8 @@ __device__ __forceinline__ uint32_t tree_word(const cacheir_b200_tree_args& a, c
   return s.rows - 32 * q < 32 ? bits & ((1u << (s.rows - 32 * q)) - 1u) : bits;
 }
 
-// Partial results of the general kernel: for every (piece, row, head) a maximum (log2 domain) and a denominator, and the unnormalised output.
+// Partial results of the general kernel, where keys are cut into pieces: for every (piece, row, head) a maximum (log2 domain) and a denominator, and the unnormalised
+// output. As many pieces as 64 MB of outputs hold; rows that fill more than half of that are not cut and need no scratch, which so does not grow with the batch.
 constexpr int kMaxTreePieces = 64;
 inline int tree_pieces(int rows, int heads, int dim) {
   const size_t one = static_cast<size_t>(rows) * heads * dim * 4, n = (static_cast<size_t>(64) << 20) / (one > 0 ? one : 1);

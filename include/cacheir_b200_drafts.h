@@ -47,8 +47,8 @@ int cacheir_b200_norm_rotary_append(const cacheir_b200_norm_rotary_args* args, v
  * [sequences][max_pages], page ids outside the pool read as zeros; tokens behind max_pages * page_size are not there.
  * Up to 65535 sequences, 2^24 rows, as many key/value heads as 65535, tables of up to 2^30 tokens, words <= 32 (CACHEIR_B200_ELIMIT), heads
  * of up to 512 (CACHEIR_B200_EUNSUPPORTED).
- *   workspace: cacheir_b200_tree_attention_workspace_bytes(...) bytes, 16-byte aligned, used by this call's kernels only: calls that may
- *   overlap need one each.
+ *   workspace: cacheir_b200_tree_attention_workspace_bytes(...) bytes (enough for whatever kernel serves the call, 68 MB at most with heads of 128; 0: NULL will do),
+ *   16-byte aligned, used by this call's kernels only: calls that may overlap need one each.
  * Partial results are joined in a fixed order: the same bits for the same arguments. */
 #define CACHEIR_B200_MAX_DRAFT_WORDS 32
 typedef struct {

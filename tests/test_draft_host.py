@@ -104,6 +104,16 @@ def test_c_entry_points_refuse_before_they_launch(lib):
         assert getattr(lib, "cacheir_b200_" + name)(None, None) == -1
 
 
+def test_scratch_of_attention_does_not_grow_with_the_batch(lib):
+    size = lib.cacheir_b200_tree_attention_workspace_bytes
+    for dim in (1, 33, 64, 96, 128, 256, 512):
+        for heads in (1, 8, 64):
+            sizes = [size(rows, heads, dim) for rows in (1, 2, 63, 64, 500, 4096, 16384, 1 << 20, 1 << 24)]
+            # outputs of 64 MB in pieces and two numbers beside each, or the tensor cores' two pieces a block
+            assert max(sizes) <= (64 << 20) * (dim + 2) // dim
+            assert sizes[-1] == (size(1 << 23, heads, dim) if dim in (64, 128) else 0)
+
+
 def test_logits_that_lie_over_one_another_are_refused(lib):
     """Values that do not change are not written where out is the logits: another row stride, or rows that lie partly over one another, would leave the wrong ones. What
     lies between the rows, or apart, goes on to the next check (here: words)."""

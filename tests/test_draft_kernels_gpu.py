@@ -412,6 +412,18 @@ def test_a_long_chain_of_rows():
     Case(heads=4, kv_heads=2, dim=64, ctx=(100,), nodes=(1100,), lists=None).check()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_that_are_not_cut_and_need_no_scratch(dtype):
+    from cacheir_b200 import draft_ops
+    case = Case(heads=8, kv_heads=2, dim=512, ctx=(20, 7, 0, 4), nodes=(1500, 600, 0, 40), padded=2, lists=None, dtype=dtype, seed=3)
+    assert draft_ops.tree_attention_workspace_bytes(case.q.shape[0], 8, 512) == 0
+    case.values[case.place(1, 606)[0], :, case.place(1, 606)[1], 9] = math.inf       # (of the last row alone)
+    want, bound = case.want()
+    got = case.call()
+    _close(got, want, bound)
+    assert bool((got[2140:] == 7.0).all()) and int((got == math.inf).sum()) == 8
+
+
 def test_strides_alignment_and_workspaces():
     from cacheir_b200 import draft_ops
     case = Case(ctx=(200, 31), nodes=(7, 12), wide_q=4, dtype=BF16)
