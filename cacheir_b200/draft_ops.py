@@ -267,7 +267,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 # ---- logits ----------------------------------------------------------------------------------------------------------------
 @dataclass
 class TokenHistory:
-    """What every sequence has said: int32 tokens [S, width], of which lens[b] count; the first prompt_lens[b] of them are the prompt (None: none)."""
+    """What every sequence has said: int32 tokens [S, width], of which lens[b] count; the first prompt_lens[b] of them are the prompt (None: none). Beside
+    `DraftedTokens` a token is in one of the two only: see there."""
 
     tokens: torch.Tensor
     lens: torch.Tensor
@@ -276,7 +277,11 @@ class TokenHistory:
 
 @dataclass
 class DraftedTokens:
-    """The rows' own tokens (int64 [R]) and which of them each sees (`visible` and `cu_rows` as in `tree_attention`)."""
+    """The rows' own tokens (int64 [R]) and which of them each sees (`visible` and `cu_rows` as in `tree_attention`).
+
+    Row 0 of a sequence, its last certain token, is among what its rows see, and would count twice if the history held it too. So either history.lens ends in
+    front of it, and ids has it: it counts as generated; or the history holds it and ids[row 0] is -1. The latter is what the first step behind a prompt
+    needs, whose row 0 is a token of the prompt, and will do for every step. `accept_drafts` does not look at ids of rows 0."""
 
     ids: torch.Tensor
     visible: torch.Tensor
@@ -289,7 +294,7 @@ def adjust_logits(logits: torch.Tensor, *, row_seq: torch.Tensor | None = None, 
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """Logits [R, V] as the next token is to be picked from, before `ops.argmax_rows` or `token_logprobs`. For token t of a row of sequence b
 
-        c = times that t was generated (history behind the prompt) or is drafted in front of the row, itself included
+        c = times that t was generated (history behind the prompt) or is drafted in front of the row, itself included (row 0: see `DraftedTokens`)
         where c > 0 or t is in the prompt: x / repetition[b] where x > 0, else x * repetition[b]
         x - frequency[b] * c - (presence[b] where c > 0) + bias of t, and -inf where t is not allowed
 

@@ -78,7 +78,10 @@ int cacheir_b200_tree_attention(const cacheir_b200_tree_args* args, void* stream
  * worked out in 32 bits and rounded once. Stands beside cacheir_b200_argmax_rows and cacheir_b200_token_logprobs, which follow it.
  *   row_seq int32 [rows] (NULL: row r is of sequence r): rows whose sequence is outside 0 .. sequences - 1 are left as they were in out
  *   history int32 [sequences][history_width], history_lens, prompt_lens int32 [sequences] (prompt_lens NULL: no prompt); NULL: no history
- *   draft_ids int64 [rows] with cu_rows (see above) and visible int32 [rows][words] (as in cacheir_b200_tree_attention); NULL: none
+ *   draft_ids int64 [rows] with cu_rows (see above) and visible int32 [rows][words] (as in cacheir_b200_tree_attention); NULL: none.
+ *     Row 0, a sequence's last certain token, is among what its rows see. So either the history ends in front of it, and it counts as generated through its
+ *     draft_ids; or the history holds it, as generated or, in the first step behind a prompt, as the prompt's last token, and its draft_ids is -1. With both it
+ *     counts twice. (cacheir_b200_accept_drafts does not look at draft_ids of row 0.)
  *   repetition (> 0), frequency, presence float [sequences]; each NULL: without
  *   bias_ids int32 [sequences][biases], bias_values float: of several entries with one token the last counts
  *   allowed int32 [rows][ceil(vocab / 32)]: bit t % 32 of word t / 32, 1 where the token may come

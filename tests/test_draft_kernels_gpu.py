@@ -761,6 +761,37 @@ def test_logits_on_another_stream_and_captured():
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("row_0", ["in the history", "among the drafts", "of the prompt"])
+def test_drafted_tokens_are_penalized_like_said_ones(row_0):
+    """A row's logits are those of a sequence whose history ends with the tokens that the row follows, row 0's among them."""
+    from cacheir_b200 import draft_ops
+    rng, gen = random.Random(6), torch.Generator(device=DEV).manual_seed(6)
+    nodes, vocab, width = (6, 1, 40, 9), 301, 80
+    trees = [_seen(tree) for tree in _trees(rng, nodes, "tree")]
+    prompts = [[rng.randrange(vocab) for _ in range(rng.randrange(1, 12))] for _ in nodes]
+    answers = [[] if row_0 == "of the prompt" else [rng.randrange(40) for _ in range(rng.randrange(1, 20))] for _ in nodes]
+    ids, lines, firsts = [], [], []
+    for seen, prompt, answer in zip(trees, prompts, answers):
+        certain = prompt + answer                                     # (row 0 is the last of them)
+        own = [certain[-1]] + [rng.randrange(40) for _ in seen[1:]]
+        lines += [certain + [own[j] for j in row[1:]] for row in seen]
+        firsts += [len(prompt)] * len(seen)
+        ids += [own[0] if row_0 == "among the drafts" else -1] + own[1:]
+    logits = torch.randn(len(ids), vocab, device=DEV, generator=gen) * 4
+    rand = lambda: torch.rand(len(nodes), device=DEV, generator=gen)
+    penalties = dict(repetition=0.8 + rand(), frequency=rand() - 0.2, presence=rand() - 0.2)
+    row_seq = _i32([b for b, n in enumerate(nodes) for _ in range(n)])
+    padded = lambda line: line + [7] * (width - len(line))
+    want = draft_ops.adjust_logits(logits.clone(), history=draft_ops.TokenHistory(_i32([padded(line) for line in lines]), _i32([len(line) for line in lines]), _i32(firsts)),
+                                   **{name: value[row_seq.long()].contiguous() for name, value in penalties.items()})
+    said = [prompt + answer[: -1 if row_0 == "among the drafts" else None] for prompt, answer in zip(prompts, answers)]
+    history = draft_ops.TokenHistory(_i32([padded(line) for line in said]), _i32([len(line) for line in said]), _i32([len(prompt) for prompt in prompts]))
+    visible = _i32([line for seen in trees for line in _words(seen, 2)])
+    got = draft_ops.adjust_logits(logits.clone(), row_seq=row_seq, history=history, **penalties,
+                                  drafts=draft_ops.DraftedTokens(torch.tensor(ids, device=DEV), visible, _i32(_starts(nodes))))
+    assert torch.equal(got, want) and not torch.equal(got, logits)
+
+
 # ---- drafts ----------------------------------------------------------------------------------------------------------------
 def _walk(parents, ids, chosen, depth):
     path, pick = [], -1
@@ -974,3 +1005,60 @@ def test_a_step_with_drafts_says_what_single_tokens_say():
     assert kept > 2 * steps * sequences, "drafts were accepted"
     torch.cuda.synchronize()
     graph = None
+
+
+def test_a_step_with_penalties_says_what_single_tokens_say(monkeypatch):
+    """The same with a history of all certain tokens, row 0's among them, and penalties: the history grows by what was accepted."""
+    from cacheir_b200 import draft_ops, serving_ops
+    heads, kv_heads, dim, vocab, sequences, most, width = 8, 2, 64, 97, 3, 7, 90
+    sizes = (heads, kv_heads, dim, vocab)
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    shared = dict(embed=torch.randn(vocab, (heads + 2 * kv_heads) * dim, device=DEV, generator=gen).to(BF16), head=torch.randn(heads * dim, vocab, device=DEV, generator=gen).to(BF16),
+                  rule=serving_ops.rotary_rule(dim, 1e4, layout="half"), q_weight=torch.ones(dim, dtype=BF16, device=DEV) * 2, k_weight=torch.ones(dim, dtype=BF16, device=DEV) * 2,
+                  repetition=torch.tensor([1.3, 1.0, 1.1], device=DEV))
+    history = draft_ops.TokenHistory(torch.zeros(sequences, width, dtype=torch.int32, device=DEV), _i32([1] * sequences), _i32([1] * sequences))
+    plain = draft_ops.adjust_logits
+
+    def adjust(logits, *, drafts, **more):
+        ids = drafts.ids.clone()
+        ids[:: len(ids) // sequences] = -1                            # (rows 0, which the history has)
+        return plain(logits, history=history, frequency=torch.tensor([0.5, 2.0, 0.0], device=DEV), presence=torch.tensor([0.0, 1.0, 3.0], device=DEV),
+                     drafts=draft_ops.DraftedTokens(ids, drafts.visible, drafts.cu_rows), **more)
+
+    monkeypatch.setattr(draft_ops, "adjust_logits", adjust)
+
+    def run(rows, count, drafted):
+        """What is said in steps of so many rows a sequence."""
+        pools = [torch.zeros(40, kv_heads, 16, dim, dtype=BF16, device=DEV) for _ in range(2)]
+        s = dict(shared, table=torch.zeros(sequences, 10, dtype=torch.int32, device=DEV), lens=_i32([0] * sequences), new=_i32([rows] * sequences),
+                 free=torch.randperm(40, device=DEV, generator=gen).to(torch.int32), count=_i32([40]), tokens=serving_ops.token_map(rows * sequences, sequences, DEV),
+                 parents=_i32(([-1, 0, 0, 1, 1, 3, 3])[:rows] * sequences), tree=draft_ops.draft_tree(rows * sequences, 1, DEV),
+                 ids=torch.zeros(rows * sequences, dtype=torch.int64, device=DEV), keys=pools[0], values=pools[1], handle=draft_ops.page_pools(pools),
+                 q=torch.zeros(rows * sequences, heads, dim, dtype=BF16, device=DEV), out=torch.zeros(rows * sequences, heads, dim, dtype=BF16, device=DEV),
+                 workspace=torch.empty(draft_ops.tree_attention_workspace_bytes(rows * sequences, heads, dim), dtype=torch.uint8, device=DEV),
+                 allowed=torch.full((rows * sequences, 4), -1, dtype=torch.int32, device=DEV), accepted=draft_ops.accepted_drafts(sequences, most, DEV))
+        lines, steps = [[1], [2], [3]], 0
+        while min(len(line) for line in lines) < count:
+            for b, line in enumerate(lines):
+                history.tokens[b, : len(line)] = _i32(line)
+            history.lens.copy_(_i32([len(line) for line in lines]))
+            ids = [token for b, line in enumerate(lines) for token in [line[-1]] + drafted(b, line)]
+            s["ids"].copy_(torch.tensor(ids, device=DEV))
+            _step(s, sizes)
+            counts, path, following = s["accepted"].counts.tolist(), s["accepted"].rows.tolist(), s["accepted"].next_ids.tolist()
+            for b, line in enumerate(lines):
+                line += [ids[r] for r in path[b][1: counts[b]]] + [following[b]]
+            steps += 1
+        return lines, steps
+
+    said, _ = run(1, 60, lambda b, line: [])
+    rng = random.Random(4)
+
+    def guess(b, line):
+        ahead = said[b][len(line):] + [0] * most
+        return [ahead[0] if rng.random() < 0.8 else 50, 51, ahead[1], 52, 53, ahead[2]]
+
+    lines, steps = run(most, 50, guess)
+    assert [line[:50] for line in lines] == [truth[:50] for truth in said]
+    assert steps < 40, "drafts were accepted"
+    assert all(len(set(line)) > 10 for line in lines), "penalties keep the lines from going round"
