@@ -718,6 +718,51 @@ def test_adjusted_logits(dtype, rows, sequences, vocab, kind):
     assert torch.equal(logits, out), "in place: the same values"
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows, sequences", [(130, 7), (200, 9), (512, 21), (520, 100)])
+@pytest.mark.parametrize("kind", ["all", "drafts", "grammar"])
+def test_adjusted_logits_of_blocks_with_several_rows(dtype, rows, sequences, kind):
+    """Blocks of 2, 4 and 8 rows, whose sequence changes inside them or which have a row of no sequence: rows that share a count, and a count that begins again."""
+    from cacheir_b200 import draft_ops
+    vocab = 33001
+    logits, row_seq, more = _logits_case(rows, sequences, vocab, dtype, rows, width=200 if kind == "all" else 0, biases=30 if kind == "all" else 0, grammar=kind != "drafts",
+                                         drafts=kind != "grammar", wide=rows % 3)
+    want, size = _logits_want(logits, row_seq, more)
+    nobody = [3, 64, rows // 2 + 1, rows - 2]
+    if kind == "grammar":
+        more["row_seq"] = _i32(row_seq)
+    more["row_seq"][nobody] = -1
+    live = [r for r in range(rows) if r not in nobody]
+    want, size = want[live], torch.nan_to_num(size[live], posinf=0.0)
+    # (the bound of the test above)
+    bound = 8 * 2.0 ** -24 * size + _half_step(dtype) * (size if dtype is F32 else torch.nan_to_num(want, neginf=0.0).abs() + 8 * 2.0 ** -24 * size) + 2.0 ** -25
+    call = {k: v for k, v in more.items() if not k.startswith("_")}
+    before = logits.clone()
+    out = torch.full((rows, vocab), 3.0, dtype=dtype, device=DEV)
+    draft_ops.adjust_logits(logits, out=out, **call)
+    assert torch.equal(logits, before) and bool((out[nobody] == 3.0).all())
+    _close(out[live], want, bound, kind)
+    draft_ops.adjust_logits(logits, **call)
+    assert torch.equal(logits[live], out[live]) and torch.equal(logits[nobody], before[nobody])
+
+
+def test_adjusted_logits_of_more_rows_than_a_grid_has():
+    from cacheir_b200 import draft_ops
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    rows, vocab, sequences = 70001, 45, 5
+    logits = torch.randn(rows, vocab, device=DEV, generator=gen)
+    row_seq = torch.randint(0, sequences, (rows,), device=DEV, generator=gen).to(torch.int32)
+    tokens = torch.randint(0, vocab, (sequences, 9), device=DEV, generator=gen).to(torch.int32)
+    presence = torch.arange(1, sequences + 1, device=DEV).float() / 4
+    allowed = torch.randint(-2 ** 31, 2 ** 31, (rows, 2), device=DEV, generator=gen).to(torch.int32)
+    said = torch.zeros(sequences, vocab, dtype=torch.bool, device=DEV).scatter_(1, tokens.long(), True)
+    want = torch.where(said, -presence[:, None], 0.0)[row_seq.long()] + logits
+    at = torch.arange(vocab, device=DEV)
+    want = torch.where((allowed[:, at // 32] >> (at % 32) & 1) != 0, want, -math.inf)
+    draft_ops.adjust_logits(logits, row_seq=row_seq, history=draft_ops.TokenHistory(tokens, _i32([9] * sequences)), presence=presence, allowed=allowed)
+    assert torch.equal(logits, want)
+
+
 def test_logits_rows_of_no_sequence_are_left_alone():
     from cacheir_b200 import draft_ops
     logits, row_seq, more = _logits_case(9, 3, 777, BF16, 4, width=50, grammar=True)
