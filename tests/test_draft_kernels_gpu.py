@@ -599,6 +599,46 @@ def test_normed_heads_of_few_and_many_rows(rows, heads, kv_heads):
         assert float((length - 8.0).abs().max()) <= 8.0 * 2.0 ** -8, "turns keep a normed head's length"
 
 
+@pytest.mark.parametrize("rows, heads, kv_heads, dim, rot", [(33, 32, 8, 128, 128), (700, 32, 8, 128, 128), (5000, 32, 8, 128, 128), (33, 64, 8, 128, 32), (700, 64, 8, 128, 32), (5000, 64, 8, 128, 128),
+                                                             (700, 40, 5, 64, 64), (700, 20, 4, 256, 64), (33, 25, 5, 80, 20), (700, 11, 1, 33, 32), (5000, 9, 3, 96, 96)])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_normed_heads_of_many_a_lane(rows, heads, kv_heads, dim, rot, layout, dtype):
+    """More heads than a block has lanes for at a time: several heads a lane, queries, keys and values among them, with weights that differ."""
+    from cacheir_b200 import draft_ops, serving_ops
+    page, gen = 16, torch.Generator(device=DEV).manual_seed(rows + heads)
+    fused = (torch.randn(rows, (heads + 2 * kv_heads) * dim, device=DEV, generator=gen) * 3).to(dtype)
+    q, k, v = (fused[:, lo * dim: hi * dim].view(rows, -1, dim) for lo, hi in ((0, heads), (heads, heads + kv_heads), (heads + kv_heads, heads + 2 * kv_heads)))
+    weights = [(1 + 0.3 * torch.randn(dim, device=DEV, generator=gen)).to(dtype if rows != 700 else F32), (2 + 0.3 * torch.randn(dim, device=DEV, generator=gen)).to(dtype if rows != 700 else F32)]
+    if rows == 33:
+        weights[0 if heads == 32 else 1] = None
+    offset, eps = (1.0 if rows == 700 else 0.0), 1e-5
+    rule = serving_ops.rotary_rule(rot, 10000.0, layout=layout)
+    freq = (10000.0 ** (-2.0 * torch.arange(rot // 2, dtype=torch.float64) / rot)).to(DEV)
+    positions = torch.randint(0, 100000, (rows,), device=DEV, generator=gen).to(torch.int32)
+    pages = rows // page + 2
+    slots = torch.randperm(pages * page, device=DEV, generator=gen)[:rows].to(torch.int32)
+    slots[rows // 2] = -1
+    pools = [torch.full((pages, kv_heads, page, dim), 5.0, dtype=dtype, device=DEV) for _ in range(2)]
+    q_out, k_out = torch.full((rows, heads, dim), 9.0, dtype=dtype, device=DEV), torch.full((rows, kv_heads, dim), 9.0, dtype=dtype, device=DEV)
+    draft_ops.norm_rotary_append(q, k, v, rule, positions, weights[0], weights[1], eps=eps, offset=offset, slots=slots, k_cache=pools[0], v_cache=pools[1],
+                                 q_out=q_out, k_out=k_out)
+    steps = (dim / 32 + 16) * 2.0 ** -24                           # (as above)
+    live = torch.ones(rows, dtype=torch.bool, device=DEV)
+    live[rows // 2] = False
+    for out, x, w in ((q_out, q, weights[0]), (k_out, k, weights[1])):
+        want, size = _norm_want(x, w, offset, eps, freq, positions, rot, layout)
+        bound = _half_step(dtype) * (want.abs() + steps * size) + steps * size
+        _close(out[live], want[live], bound[live], str(dtype))
+        assert bool((out[~live] == 9.0).all())
+    flat = slots[live].long()
+    assert torch.equal(pools[0][flat // page, :, flat % page], k_out[live]) and torch.equal(pools[1][flat // page, :, flat % page], v[live])
+    rest = torch.ones(pages * page, dtype=torch.bool, device=DEV)
+    rest[flat] = False
+    rest = rest.nonzero()[:, 0]
+    assert all(bool((pool[rest // page, :, rest % page] == 5.0).all()) for pool in pools)
+
+
 def test_norms_without_weights_are_the_rotary_append_of_normed_heads():
     from cacheir_b200 import draft_ops, serving_ops
     gen = torch.Generator(device=DEV).manual_seed(3)
