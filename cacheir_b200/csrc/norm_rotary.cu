@@ -246,15 +246,16 @@ int launch_norm_rotary(const cacheir_b200_norm_rotary_args& args, cudaStream_t s
                           static_cast<const void*>(a.v_cache), args.q_weight, args.k_weight})
     wide = wide && aligned_to(ptr, 16);
   for (long long stride : {a.q_stride, a.k_stride, a.v_stride, a.q_out_stride, a.k_out_stride}) wide = wide && stride % VEC == 0;
-  // Few rows want as much of a row under way as there is. Else small blocks, of the size that leaves the fewest lanes without a head in the last round, and
-  // of equal ones the larger (2001 rows of 32 + 8 + 8 heads of 128 in bf16: 15.8 us with 96 threads, 17.2 with 64, 18.4 with 128), but not where there are
-  // very many rows (16384 rows of 64 + 8 + 8 heads in fp16: 129.6 us with 64 threads, 138.5 with 96, 148 with 128).
-  const int lanes = wide ? a.dim / (2 * VEC) : 0, units = (a.heads + (a.slots ? 2 : 1) * a.kv_heads) * (wide ? lanes : 32);
+  // Few rows want as much of a row under way as there is; many want small blocks. Of 64 and 96 threads the larger where its blocks are through in as many rounds of the SMs as
+  // the smaller's, 12 or 8 on an SM by their registers (fp32 16 or 10): 1000 rows of 32 + 8 + 8 heads of 128 in bf16 7.6 us with 96 threads, 9.5 with 64; 1500 rows 14.0 and
+  // 11.7; 2001 16.0 and 17.2; 2600 20.4 and 19.5; 16384 94 and 87; in fp32 2001 rows 22.1 and 19.6, 2600 25.1 and 29.2. Heads that the general kernel serves are a warp's work each, with
+  // more to wait for: 2001 rows of 32 + 8 + 8 of 96 in bf16 50.9 us with 256 threads, 60.5 with 128, 83 with 64; 5000 rows 110.5, 111 and 126; 16384 341, 329 and 337.
+  const int lanes = wide ? a.dim / (2 * VEC) : 0;
+  const bool general = lanes != 4 && lanes != 8 && lanes != 16 && lanes != 32;
+  auto rounds = [&](int blocks) { return (a.rows + blocks * kNumSMs - 1) / (blocks * kNumSMs); };
   int threads = kMaxThreads;
-  if (a.rows > 4 * kNumSMs) {
-    auto taken = [&](int n) { return (units + kTogether * n - 1) / (kTogether * n) * n; };
-    threads = taken(96) < taken(64) || (taken(96) == taken(64) && a.rows <= 4096) ? 96 : 64;
-  }
+  if (general) threads = a.rows > 4096 ? 128 : kMaxThreads;
+  else if (a.rows > 4 * kNumSMs) threads = rounds(sizeof(T) == 4 ? 10 : 8) == rounds(sizeof(T) == 4 ? 16 : 12) ? 96 : 64;
   cudaError_t e;
   switch (lanes) {
     case 4: e = launch_lanes<T, VEC, 4>(args, threads, stream); break;
