@@ -1,7 +1,8 @@
 // Drafted tokens as rows: their positions and the rows that they see, the accepted path, and its keys and values moved together.
 //
-// All three are bound by latency: a few thousand numbers, and of the moved keys and values little more than what a launch takes. 128 sequences of 33 to 64 rows, 32 layers of
-// 8 heads of 128 in fp16: 2.2, 2.7 and 15.0 us one by one, 22.6 us together (the 63 MB that move 9.7 us); 4 sequences of 6 to 8 rows, 4 layers: 5.6 us together.
+// All three are bound by latency: positions and paths are a few thousand numbers, and the first value that is moved is known after three loads that depend on one another. 128
+// sequences of 33 to 64 rows, 32 layers of 8 heads of 128 in fp16: 2.2, 2.7 and 15.0 us one by one (the 63 MB that are moved take 9.7), 22.6 us together; 4 sequences of 6 to 8
+// rows, 4 layers: 5.4 us together.
 #include "cacheir_b200_drafts.h"
 #include "common.cuh"
 

@@ -4,8 +4,8 @@
 // A tile is 32 (row, head) pairs of one sequence that share a key/value head; its keys are cut into pieces, which leave their maximum, sum and
 // unnormalised output, and the pieces of a row are joined in order; with one piece the output is written as it ends. Within a piece 64 keys at a time, 64 columns of them at a time in shared memory as 32-bit floats;
 // a thread has 2 x 4 scores, and for every 64 columns 2 x 4 outputs in registers, reads four numbers at a time of either operand, and has the next 64 columns on their way
-// meanwhile. 32 trees of 12 to 16 tokens behind 256 to 4096, 32 query and 8 key/value heads, take 1980 us in fp32 with heads of 128, 2420 in bf16 with heads of
-// 96 and 4630 with heads of 256 (with tiles of eight rows and a number at a time 6652 and 5226 of the first two; the ordinary decode attention of as many single rows 2685, 3060 and 3350).
+// meanwhile. 32 trees of 12 to 16 tokens behind 256 to 4096, 32 query and 8 key/value heads, take 1970 us in fp32 with heads of 128, 2440 in bf16 with heads of
+// 96 and 4640 with heads of 256 (with tiles of eight rows and a number at a time 6652 and 5226 of the first two; the ordinary decode attention of as many single rows 2685, 3060 and 3350).
 // Most of that is waiting: two barriers around every 64 columns. So as many blocks as the registers allow share an SM, though a few numbers are spilled: three took 1980 and
 // 4630 us where two took 2541 and 7700, and four 2205 in fp32; heads of more than 256 two blocks (14.4 ms with heads of 512, 22.8 with one).
 #include "tree_attention.cuh"

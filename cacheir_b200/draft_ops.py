@@ -223,7 +223,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     seq_lens: int32 [S], the rows among them; cu_rows: int32 [S + 1], sequence b has the rows cu_rows[b] .. cu_rows[b + 1] - 1. visible: int32
     [R, words], bit j % 32 of word j // 32 for row j of the sequence (`map_drafts` makes them; any other mask will do); None: a chain, rows see those
     before them and themselves. Rows that see nothing give zeros; rows behind the last sequence are left as they were in `out`. What a row does not
-    see may hold anything, NaN too. D up to 512, S up to 65535, R up to 2^24. `workspace`: `tree_attention_workspace_bytes(R, H, D)` bytes of any type; calls that
+    see may hold anything, NaN too. On the tensor cores (16 bits, D 64 or 128, pages of a multiple of 16) probabilities are rounded to q's type before they meet
+    the values, elsewhere not; the rest is in 32 bits. D up to 512, S up to 65535, R up to 2^24. `workspace`: `tree_attention_workspace_bytes(R, H, D)` bytes of any type; calls that
     may overlap need one each (default: a fresh one)."""
     rows, heads, dim, q_stride = _check_heads("q", q)
     shape = k_cache.shape

@@ -49,6 +49,8 @@ int cacheir_b200_norm_rotary_append(const cacheir_b200_norm_rotary_args* args, v
  * of up to 512 (CACHEIR_B200_EUNSUPPORTED).
  *   workspace: cacheir_b200_tree_attention_workspace_bytes(...) bytes (enough for whatever kernel serves the call, 68 MB at most with heads of 128; 0: NULL will do),
  *   16-byte aligned, used by this call's kernels only: calls that may overlap need one each.
+ * Scores, sums and outputs are in 32 bits. 16-bit types with heads of 64 or 128 and pages of a multiple of 16 tokens go to the tensor cores, which take the softmax's
+ * probabilities rounded to the element type; in all other calls these have 32 bits too.
  * Partial results are joined in a fixed order: the same bits for the same arguments. */
 #define CACHEIR_B200_MAX_DRAFT_WORDS 32
 typedef struct {
