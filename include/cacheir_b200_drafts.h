@@ -42,7 +42,8 @@ int cacheir_b200_norm_rotary_append(const cacheir_b200_norm_rotary_args* args, v
  *   those j whose bit j % 32 of visible[row][j / 32] is set (visible int32 [rows][words]; rows j >= 32 words are seen by none), or
  *   visible NULL: the rows j <= i (a chain).
  * A row that sees nothing gives zeros; rows behind the last sequence are left as they were in out. What a row does not see may hold
- * anything, also numbers that are none. A key with a score of -inf has no weight; NaN among a row's scores gives NaN.
+ * anything, also numbers that are none. A key with a score of -inf has no weight (in front of the rows, weight 0: its value has to be a number); NaN among a row's
+ * scores gives NaN.
  * q, out [rows][heads][dim], rows q_stride / out_stride elements apart; pools [num_slots][kv_heads][page_size][dim]; page_table
  * [sequences][max_pages], page ids outside the pool read as zeros; tokens behind max_pages * page_size are not there.
  * Up to 65535 sequences, 2^24 rows, as many key/value heads as 65535, tables of up to 2^30 tokens, words <= 32 (CACHEIR_B200_ELIMIT), heads
